@@ -350,8 +350,7 @@ def run(st):
             S.attend_tree(st["cache"], st["segs"], st["queries"], st["parents"], st["out"], st["lse"])
             return st["out"], st["lse"]
         if op == "observe":
-            S.observe_cache(st["cache"], st["segs"], st["queries"], st["lse"], st["weights"], weights_in=st["weights_in"], decay=0.5,
-                            weight_head_stride=st["total"])
+            S.observe_cache(st["cache"], st["segs"], st["queries"], st["lse"], st["weights"], st["total"], weights_in=st["weights_in"], decay=0.5)
             return st["weights"]
         to = st["to"]
         S.evict_cache(st["cache"], st["segs"], st["weights"], st["total"], st["budget"], sink_window=st["sink"], recent_window=st["recent"],
