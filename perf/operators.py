@@ -189,7 +189,7 @@ def prepare(case, seed):
             # what earlier steps left there, of the size of what this one adds
             st["weights_in"] = torch.rand(case["kv_heads"], st["total"], generator=_gen(seed + 1), device=DEV) * (case["group"] * case["tokens"] / case["rows"])
             st["weights"] = torch.empty_like(st["weights_in"])
-            st["lse"] = _softmax_parts(st, _scores(st))[1]  # (what the attention of the same step wrote)
+            st["lse"] = _softmax_parts(st, _scores(st))[1].contiguous()  # (what the attention of the same step wrote)
     if own:  # the handles that a program keeps: where its cache lies, where its queries come to lie, the table of its sequences
         import slhav2_b200 as S
 
