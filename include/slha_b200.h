@@ -393,6 +393,132 @@ int32_t slha_b200_attend_topk(const uint32_t* top_index, const float* top_score,
                               float* weights_out);
 
 /*
+ * Exact attention over a cache of key and value rows, and what keeps such a cache
+ * small.  No counterpart in the reference.  The rows stand beside the tiles: where
+ * slha_b200_score_topk + slha_b200_attend_topk attend to the tiles that score best,
+ * these calls attend to every row a query may see, and the removal of rows takes
+ * their tiles along.
+ *
+ * A segment here is one sequence: its rows lie at tile_begin .. tile_begin +
+ * n_tiles of the cache (for every KV head), its query tokens at query_begin ..
+ * query_begin + n_queries, and row i has position index_base + i where the cache
+ * brings no positions.  Query head g belongs to KV head g / (n_heads / n_kv_heads).
+ * Rows, queries and outputs of one call have one type (float32 or bfloat16);
+ * scores, softmax and sums are held in float32, with bfloat16 rows the weights are
+ * rounded to bfloat16 before they meet the values.
+ * head_dim is at most 256; every pointer, row, token and head stride of rows,
+ * queries and outputs is a multiple of 16 bytes, head_dim of 16 bytes too
+ * (SLHA_ERR_DIMENSION otherwise).  Rows, positions, documents, queries, outputs,
+ * lse and weights are device memory of the calling thread's device; the other
+ * arrays, and the segments, host or device.
+ * A call can be captured into a CUDA graph where its segments (at most 64) are host
+ * memory and its other arrays device memory; working memory then belongs to the
+ * graph.
+ */
+typedef struct {
+    const void* keys;            /* element (row, KV head, i) at row * key_row_stride + head * key_head_stride + i */
+    const void* values;          /* likewise */
+    int32_t dtype;               /* SLHA_B200_F32 or SLHA_B200_BF16, of rows, queries and outputs */
+    uint32_t head_dim;
+    uint32_t n_kv_heads;
+    uint64_t key_row_stride;     /* strides in elements */
+    uint64_t key_head_stride;
+    uint64_t value_row_stride;
+    uint64_t value_head_stride;
+    const uint32_t* positions;   /* of row r, KV head h: [h * entry_head_stride + r]; NULL: index_base + i */
+    const uint32_t* documents;   /* likewise; NULL: one document */
+    uint64_t entry_head_stride;  /* 0: the KV heads share positions and documents */
+    const uint32_t* rows;        /* per segment the rows it has now, at most n_tiles; NULL: n_tiles */
+} SlhaB200KvCache;
+
+/*
+ * Query tokens and what they see.  The score of a query (token t, head g) and a row is
+ *   s = scale * <q, k>, then softcap * tanh(s / softcap) where softcap > 0,
+ *   then s - slopes[g] * |position of t - position of the row| where slopes is given.
+ * A token sees a row where their documents are equal and either the row's position is
+ * below the segment's prefix, or the row's position is not after the token's (unless
+ * causal is 0) and, where window > 0, the two are less than window apart.  A token that
+ * sees no row has output zero and lse -inf.  Rows that a token does not see may hold
+ * anything, infinities and NaN too.
+ */
+typedef struct {
+    const void* q;               /* element (token, head, i) at token * token_stride + head * head_stride + i */
+    uint32_t n_tokens;
+    uint32_t n_heads;            /* a multiple of the cache's n_kv_heads */
+    uint64_t token_stride;
+    uint64_t head_stride;
+    float scale;
+    float softcap;               /* 0: none */
+    uint32_t window;             /* 0: none */
+    int32_t causal;
+    const float* slopes;         /* n_heads; NULL: none */
+    const uint32_t* prefix;      /* per segment; NULL: none */
+    const uint32_t* positions;   /* n_tokens; NULL (only where the cache brings no positions either): a segment's
+                                    tokens are its last rows */
+    const uint32_t* documents;   /* n_tokens; given where the cache's are */
+} SlhaB200CacheQueries;
+
+/* Attention: out (element (token, head, i) at token * out_token_stride + head *
+ * out_head_stride + i) and, where lse_out is not NULL, the logarithm of the summed
+ * exponentials [n_tokens][n_heads].  Tokens of no segment are left as they are.  One
+ * token a segment is a decode step, many are a prompt or a chunk of one; work is split
+ * over the rows where there are few tokens, and joined in a fixed order. */
+int32_t slha_b200_attend_cache(const SlhaB200KvCache* cache, const SlhaB200Segment* segments, size_t n_segments,
+                               const SlhaB200CacheQueries* queries, void* out, uint64_t out_token_stride,
+                               uint64_t out_head_stride, float* lse_out);
+
+/* The same for a tree of drafted tokens (at most 256 a segment): a segment's tokens are
+ * its last n_queries rows, parents[t] (n_tokens, counted within the segment and smaller
+ * than t's own number; anything else means a root) says which drafted token t follows.
+ * Among the drafted rows a token sees itself and its ancestors; of the rows before them
+ * what the rules above allow.  Without positions a drafted token and its row have the
+ * position of the first drafted row plus the token's depth. */
+int32_t slha_b200_attend_tree(const SlhaB200KvCache* cache, const SlhaB200Segment* segments, size_t n_segments,
+                              const SlhaB200CacheQueries* queries, const uint32_t* parents, void* out,
+                              uint64_t out_token_stride, uint64_t out_head_stride, float* lse_out);
+
+/* The weight each row received: weights_out[h * weight_head_stride + r] = decay *
+ * weights_in[the same] + the sum of exp(s - lse) over the segment's tokens and the query
+ * heads of KV head h that see row r; lse as slha_b200_attend_cache wrote it for the same
+ * queries.  weights_in may be weights_out, or NULL (nothing received so far); entries of
+ * rows of no segment are left as they are.  The cache's values are not read (may be NULL). */
+int32_t slha_b200_observe_cache(const SlhaB200KvCache* cache, const SlhaB200Segment* segments, size_t n_segments,
+                                const SlhaB200CacheQueries* queries, const float* lse, const float* weights_in,
+                                float decay, float* weights_out, uint64_t weight_head_stride);
+
+/* Removal of the rows that received the least weight, from every KV head of a segment on
+ * its own: of n rows min(n, budget) stay.  Rows whose position is below sink_window, or
+ * less than recent_window from the segment's newest, stay first (the pool's
+ * sink_window / recent_window), then those of the largest weight; equal ones, and NaN
+ * below all, go by the lower row.  A row that stays and lies below the budget keeps its
+ * place; the places of the others there are taken, in order, by the rows that stay from
+ * beyond it, so that in place only those move.  (Attention does not depend on the order
+ * of rows that carry their positions.) */
+typedef struct {
+    const float* weights;                /* [h * weight_head_stride + r] */
+    uint64_t weight_head_stride;
+    uint32_t budget;                     /* at least 1 */
+    uint32_t sink_window;
+    uint32_t recent_window;
+    const SlhaB200KvCache* to;           /* where the rows go, not overlapping the cache; NULL: in place */
+    const SlhaB200Segment* to_segments;  /* with `to`: tile_begin and n_tiles (at least min(n, budget)) of each segment there */
+    float* weights_to;                   /* NULL: weights are not moved; in place: the array of `weights` or NULL */
+    uint64_t weights_to_head_stride;
+    const SciRustSlhaTile* tiles;        /* tile of row r, KV head h: [h * tile_head_stride + r]; NULL: none */
+    uint64_t tile_head_stride;
+    SciRustSlhaTile* tiles_to;           /* with `to` and tiles */
+    uint64_t tiles_to_head_stride;
+    uint32_t* source_out;                /* [n_segments][n_kv_heads][budget]: the row that came to each place; NULL: not wanted */
+    uint32_t* rows_out;                  /* n_segments: min(n, budget); may be the array that the cache's `rows` names; NULL: not wanted */
+} SlhaB200CacheEviction;
+
+/* Positions and documents are moved with their rows where both caches have them; they are
+ * then the KV heads' own there (entry_head_stride > 0, unless there is one KV head).  All
+ * arrays of SlhaB200CacheEviction but to_segments are device memory. */
+int32_t slha_b200_evict_cache(const SlhaB200KvCache* cache, const SlhaB200Segment* segments, size_t n_segments,
+                              const SlhaB200CacheEviction* eviction);
+
+/*
  * Token-range sharding over the GPUs of one node, one handle per rank (one
  * process or host thread per GPU).  The reference has no multi-device path;
  * these calls implement the sharding the tile scores' independence allows

@@ -111,6 +111,65 @@ pub struct SlhaB200PoolConfig {
     pub recent_window: u32,
 }
 
+/// A cache of key and value rows.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct SlhaB200KvCache {
+    pub keys: *const c_void,
+    pub values: *const c_void,
+    pub dtype: i32,
+    pub head_dim: u32,
+    pub n_kv_heads: u32,
+    pub key_row_stride: u64,
+    pub key_head_stride: u64,
+    pub value_row_stride: u64,
+    pub value_head_stride: u64,
+    pub positions: *const u32,
+    pub documents: *const u32,
+    pub entry_head_stride: u64,
+    pub rows: *const u32,
+}
+
+/// Query tokens of a cache and what they see.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct SlhaB200CacheQueries {
+    pub q: *const c_void,
+    pub n_tokens: u32,
+    pub n_heads: u32,
+    pub token_stride: u64,
+    pub head_stride: u64,
+    pub scale: f32,
+    pub softcap: f32,
+    pub window: u32,
+    pub causal: i32,
+    pub slopes: *const f32,
+    pub prefix: *const u32,
+    pub positions: *const u32,
+    pub documents: *const u32,
+}
+
+/// Removal of the rows that received the least weight.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct SlhaB200CacheEviction {
+    pub weights: *const f32,
+    pub weight_head_stride: u64,
+    pub budget: u32,
+    pub sink_window: u32,
+    pub recent_window: u32,
+    pub to: *const SlhaB200KvCache,
+    pub to_segments: *const SlhaB200Segment,
+    pub weights_to: *mut f32,
+    pub weights_to_head_stride: u64,
+    pub tiles: *const SciRustSlhaTile,
+    pub tile_head_stride: u64,
+    pub tiles_to: *mut SciRustSlhaTile,
+    pub tiles_to_head_stride: u64,
+    pub source_out: *mut u32,
+    pub rows_out: *mut u32,
+}
+
 extern "C" {
     // ---- part 1: slha-c/include/slha.h:123-278 -------------------------------------------------
     pub fn slha_abi_version() -> u32;
@@ -158,6 +217,17 @@ extern "C" {
     pub fn slha_b200_score_topk_noalloc(tiles: *const SciRustSlhaTile, segments: *const SlhaB200Segment, n_segments: usize, q_coarse: *const f32, q_sign: *const u64, n_queries: usize, k: u32, out_index: *mut u32, out_score: *mut f32, out_count: *mut u32) -> i32;
     pub fn slha_b200_score_segments(tiles: *const SciRustSlhaTile, segments: *const SlhaB200Segment, n_segments: usize, q_coarse: *const f32, q_sign: *const u64, n_queries: usize, scores_out: *mut f32, scores_len: usize, row_offsets: *const u64, row_len: u32, fill: f32) -> i32;
     pub fn slha_b200_attend_topk(top_index: *const u32, top_score: *const f32, top_count: *const u32, n_queries: usize, k: u32, scale: f32, values: *const c_void, value_dtype: i32, d_v: usize, value_row_stride: usize, value_row_base: *const u64, out: *mut f32, weights_out: *mut f32) -> i32;
+    pub fn slha_b200_attend_cache(cache: *const SlhaB200KvCache, segments: *const SlhaB200Segment, n_segments: usize,
+        queries: *const SlhaB200CacheQueries, out: *mut c_void, out_token_stride: u64, out_head_stride: u64,
+        lse_out: *mut f32) -> i32;
+    pub fn slha_b200_attend_tree(cache: *const SlhaB200KvCache, segments: *const SlhaB200Segment, n_segments: usize,
+        queries: *const SlhaB200CacheQueries, parents: *const u32, out: *mut c_void, out_token_stride: u64,
+        out_head_stride: u64, lse_out: *mut f32) -> i32;
+    pub fn slha_b200_observe_cache(cache: *const SlhaB200KvCache, segments: *const SlhaB200Segment, n_segments: usize,
+        queries: *const SlhaB200CacheQueries, lse: *const f32, weights_in: *const f32, decay: f32,
+        weights_out: *mut f32, weight_head_stride: u64) -> i32;
+    pub fn slha_b200_evict_cache(cache: *const SlhaB200KvCache, segments: *const SlhaB200Segment, n_segments: usize,
+        eviction: *const SlhaB200CacheEviction) -> i32;
     pub fn slha_b200_shard_unique_id(id_out: *mut c_void) -> i32;
     pub fn slha_b200_shard_init(nccl_unique_id: *const c_void, rank: i32, world: i32, out: *mut *mut SlhaB200Shard) -> i32;
     pub fn slha_b200_shard_destroy(shard: *mut SlhaB200Shard) -> i32;

@@ -95,6 +95,10 @@ SIGNATURES = {
     "slha_b200_topk_merge_strided": (_i32, [_vp, _vp, _u32, _u64, _u32, _u32, _u32, _vp, _vp]),
     "slha_b200_topk_merge_sorted_strided": (_i32, [_vp, _vp, _u32, _u64, _u32, _u32, _u32, _vp, _vp]),
     "slha_b200_attend_topk": (_i32, [_vp, _vp, _vp, _sz, _u32, C.c_float, _vp, _i32, _sz, _sz, _vp, _vp, _vp]),
+    "slha_b200_attend_cache": (_i32, [_vp, _vp, _sz, _vp, _vp, _u64, _u64, _vp]),
+    "slha_b200_attend_tree": (_i32, [_vp, _vp, _sz, _vp, _vp, _vp, _u64, _u64, _vp]),
+    "slha_b200_observe_cache": (_i32, [_vp, _vp, _sz, _vp, _vp, _vp, C.c_float, _vp, _u64]),
+    "slha_b200_evict_cache": (_i32, [_vp, _vp, _sz, _vp]),
     "slha_b200_shard_unique_id": (_i32, [_vp]),
     "slha_b200_shard_init": (_i32, [_vp, _i32, _i32, C.POINTER(_vp)]),
     "slha_b200_shard_destroy": (_i32, [_vp]),
@@ -491,6 +495,112 @@ def attend_topk(top_index, top_score, k, scale, values, d_v, value_dtype=F32, to
                                                 d_v if value_row_stride is None else value_row_stride, ptr(base), ptr(out),
                                                 ptr(weights_out)))
     return out
+
+
+class _KvCache(C.Structure):
+    _fields_ = [
+        ("keys", _vp), ("values", _vp), ("dtype", _i32), ("head_dim", _u32), ("n_kv_heads", _u32),
+        ("key_row_stride", _u64), ("key_head_stride", _u64), ("value_row_stride", _u64), ("value_head_stride", _u64),
+        ("positions", _vp), ("documents", _vp), ("entry_head_stride", _u64), ("rows", _vp),
+    ]
+
+
+class _CacheQueries(C.Structure):
+    _fields_ = [
+        ("q", _vp), ("n_tokens", _u32), ("n_heads", _u32), ("token_stride", _u64), ("head_stride", _u64), ("scale", C.c_float), ("softcap", C.c_float),
+        ("window", _u32), ("causal", _i32), ("slopes", _vp), ("prefix", _vp), ("positions", _vp), ("documents", _vp),
+    ]
+
+
+class _CacheEviction(C.Structure):
+    _fields_ = [
+        ("weights", _vp), ("weight_head_stride", _u64), ("budget", _u32), ("sink_window", _u32), ("recent_window", _u32), ("to", _vp), ("to_segments", _vp),
+        ("weights_to", _vp), ("weights_to_head_stride", _u64), ("tiles", _vp), ("tile_head_stride", _u64), ("tiles_to", _vp), ("tiles_to_head_stride", _u64),
+        ("source_out", _vp), ("rows_out", _vp),
+    ]
+
+
+class KvCache:
+    """Where a cache of key and value rows lies (SlhaB200KvCache): device memory, by default [row][kv_head][head_dim].  `positions` and `documents` are
+    the rows' own (uint32; KV head h at h * entry_head_stride), `rows` the rows each segment has now.  Keeps the arrays that it names alive."""
+
+    def __init__(self, keys, values, n_kv_heads, head_dim, dtype=BF16, key_row_stride=None, key_head_stride=None, value_row_stride=None,
+                 value_head_stride=None, positions=None, documents=None, entry_head_stride=0, rows=None):
+        def stride(given, default):
+            return default if given is None else given
+
+        rows = None if rows is None else _np(rows, np.uint32)
+        self.kept = (keys, values, positions, documents, rows)
+        self.head_dim, self.n_kv_heads, self.dtype = head_dim, n_kv_heads, dtype
+        self.c = _KvCache(ptr(keys), ptr(values), dtype, head_dim, n_kv_heads, stride(key_row_stride, n_kv_heads * head_dim), stride(key_head_stride, head_dim),
+                          stride(value_row_stride, n_kv_heads * head_dim), stride(value_head_stride, head_dim), ptr(positions), ptr(documents),
+                          entry_head_stride, ptr(rows))
+        self.address = C.addressof(self.c)
+
+
+class CacheQueries:
+    """Query tokens of a cache and what they see (SlhaB200CacheQueries): q in device memory, by default [token][head][head_dim]; scale by default
+    head_dim ** -0.5.  Keeps the arrays that it names alive."""
+
+    def __init__(self, q, n_tokens, n_heads, head_dim, scale=None, softcap=0.0, window=0, causal=True, slopes=None, prefix=None, positions=None, documents=None,
+                 token_stride=None, head_stride=None):
+        slopes = None if slopes is None else _np(slopes, np.float32)
+        prefix, positions, documents = (None if x is None else _np(x, np.uint32) for x in (prefix, positions, documents))
+        self.kept = (q, slopes, prefix, positions, documents)
+        self.n_heads, self.head_dim = n_heads, head_dim
+        self.c = _CacheQueries(ptr(q), n_tokens, n_heads, n_heads * head_dim if token_stride is None else token_stride,
+                               head_dim if head_stride is None else head_stride, head_dim ** -0.5 if scale is None else scale, softcap, window,
+                               1 if causal else 0, ptr(slopes), ptr(prefix), ptr(positions), ptr(documents))
+        self.address = C.addressof(self.c)
+
+
+def _segments(segments):
+    if isinstance(segments, np.ndarray) and segments.dtype == SEGMENT_DTYPE and segments.flags["C_CONTIGUOUS"]:
+        return segments
+    return np.ascontiguousarray(segments, SEGMENT_DTYPE)
+
+
+def attend_cache(cache, segments, queries, out, lse_out=None, out_token_stride=None, out_head_stride=None):
+    """Exact attention of `queries` (CacheQueries) over `cache` (KvCache): out [token][head][head_dim] of the cache's type and, where given, lse_out
+    [token][head] float32, both device memory; see slha_b200_attend_cache."""
+    seg = _segments(segments)
+    d = cache.head_dim
+    _check(load_library().slha_b200_attend_cache(cache.address, seg.ctypes.data, len(seg), queries.address, ptr(out),
+                                                 queries.n_heads * d if out_token_stride is None else out_token_stride,
+                                                 d if out_head_stride is None else out_head_stride, ptr(lse_out)))
+    return out
+
+
+def attend_tree(cache, segments, queries, parents, out, lse_out=None, out_token_stride=None, out_head_stride=None):
+    """attend_cache for trees of drafted tokens: a segment's tokens are its last rows, parents[t] (uint32, counted within the segment, below t's own number;
+    anything else: a root) the token that t follows; see slha_b200_attend_tree."""
+    seg = _segments(segments)
+    par = _np(parents, np.uint32)
+    d = cache.head_dim
+    _check(load_library().slha_b200_attend_tree(cache.address, seg.ctypes.data, len(seg), queries.address, ptr(par), ptr(out),
+                                                queries.n_heads * d if out_token_stride is None else out_token_stride,
+                                                d if out_head_stride is None else out_head_stride, ptr(lse_out)))
+    return out
+
+
+def observe_cache(cache, segments, queries, lse, weights_out, weight_head_stride, weights_in=None, decay=1.0):
+    """The weight each row received: weights_out [kv_head][row] = decay * weights_in + the softmax weights of the tokens that see it (lse as attend_cache wrote
+    it); see slha_b200_observe_cache."""
+    seg = _segments(segments)
+    _check(load_library().slha_b200_observe_cache(cache.address, seg.ctypes.data, len(seg), queries.address, ptr(lse), ptr(weights_in), decay,
+                                                  ptr(weights_out), weight_head_stride))
+    return weights_out
+
+
+def evict_cache(cache, segments, weights, weight_head_stride, budget, sink_window=0, recent_window=0, to=None, to_segments=None, weights_to=None,
+                weights_to_head_stride=0, tiles=None, tile_head_stride=0, tiles_to=None, tiles_to_head_stride=0, source_out=None, rows_out=None):
+    """Removal of the rows of least weight, `budget` stay a KV head; in place, or into the cache `to`; see slha_b200_evict_cache."""
+    seg = _segments(segments)
+    to_seg = None if to_segments is None else _segments(to_segments)
+    e = _CacheEviction(ptr(weights), weight_head_stride, budget, sink_window, recent_window, None if to is None else to.address,
+                       None if to_seg is None else to_seg.ctypes.data, ptr(weights_to), weights_to_head_stride, ptr(tiles), tile_head_stride, ptr(tiles_to),
+                       tiles_to_head_stride, ptr(source_out), ptr(rows_out))
+    _check(load_library().slha_b200_evict_cache(cache.address, seg.ctypes.data, len(seg), C.addressof(e)))
 
 
 def shard_unique_id():

@@ -1,0 +1,127 @@
+// Exact attention over a cache of key and value rows: what its kernels share (cache_attend.cu, cache_observe.cu, cache_evict.cu) and the
+// launchers that the C ABI calls (capi_cache.cuh).
+#pragma once
+
+#include <atomic>
+#include <vector>
+
+#include "runtime.cuh"
+
+namespace slha {
+
+constexpr uint32_t CACHE_TABLE = 64;         // segments whose table travels in a kernel's parameters
+constexpr uint32_t TREE_MOST = 256;          // drafted tokens of a segment
+constexpr uint32_t CACHE_DIM_MOST = 256;
+
+// A segment and its share of a launch's work.
+struct CacheSeg {
+    uint64_t row_begin;
+    uint32_t n_rows, query_begin, n_queries, base;
+    uint32_t item_begin;   // first work item
+    uint32_t block_begin;  // first block of query rows, of the segments whose rows are split
+    uint32_t chunk_tiles;  // key tiles of an item
+    uint32_t n_chunks;     // items of a block of query rows
+    uint32_t seg;          // its number in the caller's table
+    uint32_t pad;
+    uint64_t to_begin;     // its first row's place where rows go to
+};
+struct CacheTable {
+    CacheSeg s[CACHE_TABLE];
+};
+struct CacheArgs {
+    const void *keys, *values, *q;
+    void* out;
+    float* lse;
+    uint64_t krs, khs, vrs, vhs, qts, qhs, ots, ohs;  // strides in elements
+    const uint32_t *row_pos, *row_doc;
+    uint64_t entry_hs;
+    const uint32_t *rows, *q_pos, *q_doc, *prefix, *parents;
+    const float* slopes;
+    const CacheSeg* table;  // null: in the parameters
+    float *part_o, *part_ml;
+    const float *lse_in, *w_in;  // observe
+    float* w_out;
+    uint64_t w_hs;
+    float decay;
+    uint32_t n_segs, n_kv, group, d, n_heads, n_tokens;
+    float scale, cap;
+    uint32_t window_last;  // the largest distance that is seen
+    int32_t causal;
+    int32_t tree;
+};
+struct EvictArgs {
+    const void *keys, *values;
+    void *to_keys, *to_values;
+    uint64_t krs, khs, vrs, vhs, tkrs, tkhs, tvrs, tvhs;  // strides in bytes
+    const uint32_t *pos, *doc;
+    uint32_t *to_pos, *to_doc;
+    uint64_t entry_hs, to_entry_hs;
+    const float* w;
+    float* to_w;
+    uint64_t w_hs, to_w_hs;
+    const unsigned char* tiles;
+    unsigned char* to_tiles;
+    uint64_t tile_hs, to_tile_hs;
+    const uint32_t* rows;
+    uint32_t *rows_out, *source, *places, *holes, *stay;
+    const CacheSeg* table;
+    uint32_t n_segs, n_kv, row_bytes, budget, room, sink, recent, in_place;
+};
+
+#ifdef __CUDACC__
+// the segment that work item `item` belongs to: the last one that begins at or before it
+template <typename F>
+__device__ __forceinline__ uint32_t cache_find(uint32_t n, uint32_t item, F begin) {
+    uint32_t lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) >> 1;
+        if (begin(mid) <= item) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+// Whether a token sees a row.
+struct CacheSight {
+    uint32_t window_last, prefix;
+    int causal;
+    __device__ __forceinline__ bool sees(uint32_t qp, uint32_t kp) const {
+        const bool past = kp <= qp;
+        const uint32_t away = past ? qp - kp : kp - qp;
+        return ((past || !causal) && away <= window_last) || kp < prefix;
+    }
+};
+#endif
+
+// Working memory of one call: the thread's, or under capture memory that the graph allocates and frees with every run, so that graphs share none.
+struct CacheMemory {
+    Ctx* c;
+    void* graph = nullptr;
+    Status get(size_t bytes, void** out) {
+        if (!ctx_capturing(c)) return ctx_device_scratch(c, bytes, out);
+        SLHA_CUDA(cudaMallocAsync(&graph, bytes, c->stream));
+        *out = graph;
+        return Status();
+    }
+    Status done() {
+        if (graph) SLHA_CUDA(cudaFreeAsync(graph, c->stream));
+        return Status();
+    }
+};
+// The table of a launch: in the kernel's parameters, or uploaded where it is longer.
+Status cache_table(Ctx* c, const std::vector<CacheSeg>& segs, CacheTable* inl, const CacheSeg** dev);
+// Raises a kernel's limit of dynamic shared memory, once per kernel and device.
+template <auto KERNEL>
+Status cache_smem(Ctx* c, size_t bytes) {
+    static std::atomic<uint32_t> raised{0};
+    const uint32_t bit = 1u << c->device;
+    if (raised.load(std::memory_order_relaxed) & bit) return Status();
+    SLHA_CUDA(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    raised.fetch_or(bit, std::memory_order_relaxed);
+    return Status();
+}
+
+Status launch_attend_cache(Ctx* c, CacheArgs a, int dtype, const std::vector<SlhaB200Segment>& segs);
+Status launch_observe_cache(Ctx* c, CacheArgs a, int dtype, const std::vector<SlhaB200Segment>& segs);
+Status launch_evict_cache(Ctx* c, EvictArgs a, const std::vector<SlhaB200Segment>& segs, const std::vector<SlhaB200Segment>& to_segs);
+
+}  // namespace slha

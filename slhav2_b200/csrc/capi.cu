@@ -10,6 +10,7 @@
 #include <cstring>
 #include <functional>
 
+#include "cache.cuh"
 #include "pool.cuh"
 #include "runtime.cuh"
 
@@ -378,3 +379,4 @@ void slha_weights_free(SlhaModel* model) { (void)slha_weights_release(model); }
 }  // extern "C"
 
 #include "capi_b200.cuh"
+#include "capi_cache.cuh"
