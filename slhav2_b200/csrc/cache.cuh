@@ -80,6 +80,18 @@ __device__ __forceinline__ uint32_t cache_find(uint32_t n, uint32_t item, F begi
     }
     return lo;
 }
+// tanh.  Up to 1 a polynomial in x^2, the minimax one of tanh(x) / x (found by exchange of extrema in 40 digits): 5e-8 relative in exact arithmetic, 1.2e-7 of 1 in
+// float32; beyond, CUDA's.
+__device__ __forceinline__ float tanh_small(float x) {
+    const float u = x * x;
+    float p = fmaf(u, 1.041022640341338e-3f, -6.203379131937655e-3f);
+    p = fmaf(u, p, 2.028998046010164e-2f);
+    p = fmaf(u, p, -5.345702958893045e-2f);
+    p = fmaf(u, p, 1.3325204076281205e-1f);
+    p = fmaf(u, p, -3.3332839153106564e-1f);
+    return x * fmaf(u, p, 9.999999502407769e-1f);
+}
+__device__ __forceinline__ float cache_tanh(float x) { return fabsf(x) <= 1.0f ? tanh_small(x) : tanhf(x); }
 // Whether a token sees a row.
 struct CacheSight {
     uint32_t window_last, prefix;
@@ -90,7 +102,29 @@ struct CacheSight {
         return ((past || !causal) && away <= window_last) || kp < prefix;
     }
 };
+// Positions and documents of a tile's rows, or of a block's query rows.
+struct CacheRanges {
+    uint32_t pmin, pmax, dmin, dmax;
+};
+// 0: none of a tile's rows is seen by any of a block's query rows, 2: all are by all, 1: otherwise.  drafts: the tile holds drafted rows; inside: it ends before the last row does.
+__device__ __forceinline__ int cache_tile_class(const CacheRanges& k, const CacheRanges& q, const CacheSight& sight, bool drafts, bool inside) {
+    if (k.dmin > q.dmax || k.dmax < q.dmin) return 0;
+    const uint32_t near_ = k.pmax < q.pmin ? q.pmin - k.pmax : k.pmin > q.pmax ? k.pmin - q.pmax : 0u;
+    const uint32_t far_ = max(q.pmax > k.pmin ? q.pmax - k.pmin : 0u, k.pmax > q.pmin ? k.pmax - q.pmin : 0u);
+    if (!drafts && k.pmin >= sight.prefix && ((sight.causal && k.pmin > q.pmax) || near_ > sight.window_last)) return 0;
+    const bool all = k.pmax < sight.prefix || ((!sight.causal || k.pmax <= q.pmin) && far_ <= sight.window_last);
+    return all && !drafts && inside && k.dmin == k.dmax && q.dmin == q.dmax && k.dmin == q.dmin ? 2 : 1;
+}
 #endif
+
+// Work items: every segment's tiles in runs of at most `most`.
+struct CacheWork {
+    std::vector<CacheSeg> segs;
+    uint64_t items = 0, blocks = 0;  // blocks: of query rows whose segments are split
+    uint32_t chunks = 1;             // the most runs of one segment
+};
+void cache_cut(CacheWork* w, uint32_t group, uint32_t mb, uint32_t kt, uint32_t most);
+uint32_t cache_longest_run(const CacheWork& w, uint32_t group, uint32_t mb, uint32_t kt, uint32_t n_kv, uint32_t slots);
 
 // Working memory of one call: the thread's, or under capture memory that the graph allocates and frees with every run, so that graphs share none.
 struct CacheMemory {
@@ -120,6 +154,9 @@ Status cache_smem(Ctx* c, size_t bytes) {
     return Status();
 }
 
+Status cache_part_memory(CacheArgs* a, const CacheWork& w, uint32_t mb, CacheMemory* mem);  // where the parts of split segments go
+Status launch_cache_join(Ctx* c, CacheArgs a, int dtype, const CacheWork& w, uint32_t mb);
+Status launch_attend_wide(Ctx* c, CacheArgs a, CacheWork w);
 Status launch_attend_cache(Ctx* c, CacheArgs a, int dtype, const std::vector<SlhaB200Segment>& segs);
 Status launch_observe_cache(Ctx* c, CacheArgs a, int dtype, const std::vector<SlhaB200Segment>& segs);
 Status launch_evict_cache(Ctx* c, EvictArgs a, const std::vector<SlhaB200Segment>& segs, const std::vector<SlhaB200Segment>& to_segs);

@@ -41,10 +41,6 @@ struct Shape {
     static_assert(SMEM_TREE <= 227 * 1024, "shared memory of an SM");
 };
 
-struct Ranges {
-    uint32_t pmin, pmax, dmin, dmax;
-};
-
 template <typename T, int D, int WM>
 __global__ void __launch_bounds__(ATT_THREADS, Shape<T, D, WM>::CTAS) cache_attend_kernel(const __grid_constant__ CacheArgs a, const __grid_constant__ CacheTable tab) {
     using S = Shape<T, D, WM>;
@@ -116,7 +112,7 @@ __global__ void __launch_bounds__(ATT_THREADS, Shape<T, D, WM>::CTAS) cache_atte
     }
     __syncthreads();
     if (warp == 0) {
-        Ranges q{0xFFFFFFFFu, 0u, 0xFFFFFFFFu, 0u};
+        CacheRanges q{0xFFFFFFFFu, 0u, 0xFFFFFFFFu, 0u};
         for (int r = lane; r < S::MB; r += 32) {
             q.pmin = min(q.pmin, s_qp[r]);
             q.pmax = max(q.pmax, s_qp[r]);
@@ -131,7 +127,7 @@ __global__ void __launch_bounds__(ATT_THREADS, Shape<T, D, WM>::CTAS) cache_atte
     }
     copy_wait<0>();
     __syncthreads();
-    const Ranges qr{s_range[0], s_range[1], s_range[2], s_range[3]};
+    const CacheRanges qr{s_range[0], s_range[1], s_range[2], s_range[3]};
     AFrag<T> qa[sizeof(T) == 2 && D <= 128 ? D / 16 : 1];
     constexpr bool Q_HELD = sizeof(T) == 2 && D <= 128;
     constexpr int KSTEPS = D / (sizeof(T) == 2 ? 16 : 8);
@@ -140,16 +136,7 @@ __global__ void __launch_bounds__(ATT_THREADS, Shape<T, D, WM>::CTAS) cache_atte
 #pragma unroll
         for (int kk = 0; kk < KSTEPS; ++kk) qa[kk].template load<D>(sq, wm * 16, kk, lane);
 
-    // 0 no row of the tile is seen by any of the block's query rows, 1 some are, 2 all are by all
-    const auto tile_class = [&](const Ranges& k, uint32_t first, uint32_t last) -> int {
-        if (k.dmin > qr.dmax || k.dmax < qr.dmin) return 0;
-        const uint32_t near_ = k.pmax < qr.pmin ? qr.pmin - k.pmax : k.pmin > qr.pmax ? k.pmin - qr.pmax : 0u;
-        const uint32_t far_ = max(qr.pmax > k.pmin ? qr.pmax - k.pmin : 0u, k.pmax > qr.pmin ? k.pmax - qr.pmin : 0u);
-        const bool drafts = a.tree && last >= ctx;
-        if (!drafts && k.pmin >= sight.prefix && ((sight.causal && k.pmin > qr.pmax) || near_ > sight.window_last)) return 0;
-        const bool all = k.pmax < sight.prefix || ((!sight.causal || k.pmax <= qr.pmin) && far_ <= sight.window_last);
-        return all && !drafts && last < n && k.dmin == k.dmax && qr.dmin == qr.dmax && k.dmin == qr.dmin ? 2 : 1;
-    };
+    const auto tile_class = [&](const CacheRanges& k, uint32_t last) { return cache_tile_class(k, qr, sight, a.tree && last >= ctx, last < n); };
 
     float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 #pragma unroll
@@ -166,7 +153,7 @@ __global__ void __launch_bounds__(ATT_THREADS, Shape<T, D, WM>::CTAS) cache_atte
         if (arrays) {
             for (uint32_t j = warp; j < in_round; j += ATT_THREADS / 32) {
                 const uint32_t first = (r0 + j) * S::KT, last = first + S::KT - 1;
-                Ranges k{0xFFFFFFFFu, 0u, has_doc ? 0xFFFFFFFFu : 0u, 0u};
+                CacheRanges k{0xFFFFFFFFu, 0u, has_doc ? 0xFFFFFFFFu : 0u, 0u};
 #pragma unroll
                 for (int e = 0; e < S::KT / 32; ++e) {
                     const uint32_t i = min(first + lane + e * 32, n - 1);
@@ -185,12 +172,12 @@ __global__ void __launch_bounds__(ATT_THREADS, Shape<T, D, WM>::CTAS) cache_atte
                     k.dmin = __reduce_min_sync(0xFFFFFFFFu, k.dmin);
                     k.dmax = __reduce_max_sync(0xFFFFFFFFu, k.dmax);
                 }
-                if (lane == 0) s_cls[j] = (unsigned char)tile_class(k, first, last);
+                if (lane == 0) s_cls[j] = (unsigned char)tile_class(k, last);
             }
         } else {
             for (uint32_t j = tid; j < in_round; j += ATT_THREADS) {
                 const uint32_t first = (r0 + j) * S::KT, last = first + S::KT - 1;
-                s_cls[j] = (unsigned char)tile_class(Ranges{sg.base + first, sg.base + min(last, n - 1), 0u, 0u}, first, last);
+                s_cls[j] = (unsigned char)tile_class(CacheRanges{sg.base + first, sg.base + min(last, n - 1), 0u, 0u}, last);
             }
         }
         __syncthreads();
@@ -251,7 +238,7 @@ __global__ void __launch_bounds__(ATT_THREADS, Shape<T, D, WM>::CTAS) cache_atte
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     s[i][e] *= to_log2;
-                    if (has_cap) s[i][e] = cap2 * tanhf(s[i][e]);
+                    if (has_cap) s[i][e] = cap2 * cache_tanh(s[i][e]);
                 }
             if (!all || has_slope) {
                 const uint32_t* kp_s = reinterpret_cast<const uint32_t*>(sm + (li % S::STAGES) * S::STAGE + 2 * S::TILE);
@@ -465,14 +452,9 @@ __global__ void __launch_bounds__(JOIN_THREADS) cache_join_kernel(const __grid_c
     if (a.lse && lane == 0) a.lse[tok * a.n_heads + qh] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * LN2;
 }
 
-// Work items: every segment's tiles in runs of at most `most`.
-struct Work {
-    std::vector<CacheSeg> segs;
-    uint64_t items = 0, blocks = 0;  // blocks: of query rows whose segments are split
-    uint32_t chunks = 1;             // the most runs of one segment
-};
-uint64_t blocks_of(const CacheSeg& s, uint32_t group, uint32_t mb) { return ((uint64_t)s.n_queries * group + mb - 1) / mb; }
-void cut(Work* w, uint32_t group, uint32_t mb, uint32_t kt, uint32_t most) {
+}  // namespace
+static uint64_t blocks_of(const CacheSeg& s, uint32_t group, uint32_t mb) { return ((uint64_t)s.n_queries * group + mb - 1) / mb; }
+void cache_cut(CacheWork* w, uint32_t group, uint32_t mb, uint32_t kt, uint32_t most) {
     w->items = w->blocks = 0;
     w->chunks = 1;
     for (CacheSeg& c : w->segs) {
@@ -490,7 +472,7 @@ void cut(Work* w, uint32_t group, uint32_t mb, uint32_t kt, uint32_t most) {
 }
 // The longest run of tiles of an item.  In units of a tile's time: what fits on the GPU at once takes as long as its longest item, more than that the mean load
 // and half an item at the end; an item costs about four tiles to begin, joining about three and a little for every part.
-uint32_t longest_run(const Work& w, uint32_t group, uint32_t mb, uint32_t kt, uint32_t n_kv, uint32_t slots) {
+uint32_t cache_longest_run(const CacheWork& w, uint32_t group, uint32_t mb, uint32_t kt, uint32_t n_kv, uint32_t slots) {
     uint32_t most = 1;
     double total = 0.0;
     for (const CacheSeg& c : w.segs) {
@@ -514,46 +496,57 @@ uint32_t longest_run(const Work& w, uint32_t group, uint32_t mb, uint32_t kt, ui
     return best;
 }
 
+// Joins the parts of the segments that were split: only they take part, their blocks of query rows are numbered through.
+Status launch_cache_join(Ctx* c, CacheArgs a, int dtype, const CacheWork& w, uint32_t mb) {
+    std::vector<CacheSeg> split;
+    uint32_t rows = 0;
+    for (const CacheSeg& s : w.segs)
+        if (s.n_chunks > 1) {
+            split.push_back(s);
+            rows = std::max(rows, std::min(mb, s.n_queries * a.group));
+        }
+    CacheTable tab;
+    SLHA_TRY(cache_table(c, split, &tab, &a.table));
+    a.n_segs = (uint32_t)split.size();
+    const uint32_t per = (rows + JOIN_THREADS / 32 - 1) / (JOIN_THREADS / 32);
+    if (w.blocks * a.n_kv * per > 0x7FFFFFFFull) return Status(SLHA_ERR_CAPACITY, "attention over a cache: too many blocks of query rows");
+    const dim3 grid((uint32_t)(w.blocks * a.n_kv * per));
+    SLHA_CUDA(dtype == SLHA_B200_BF16 ? launch_behind(cache_join_kernel<__nv_bfloat16>, grid, dim3(JOIN_THREADS), 0, c->stream, a, tab, mb, per)
+                                      : launch_behind(cache_join_kernel<float>, grid, dim3(JOIN_THREADS), 0, c->stream, a, tab, mb, per));
+    count_launch();
+    return Status();
+}
+Status cache_part_memory(CacheArgs* a, const CacheWork& w, uint32_t mb, CacheMemory* mem) {
+    if (!w.blocks) return Status();
+    const size_t rows = (size_t)w.items * a->n_kv * mb;
+    void* p;
+    SLHA_TRY(mem->get(pad256(rows * a->d * 4) + rows * 8, &p));
+    a->part_o = (float*)p;
+    a->part_ml = (float*)((char*)p + pad256(rows * a->d * 4));
+    return Status();
+}
+
+namespace {
 template <typename T, int D, int WM>
-Status launch_class(Ctx* c, CacheArgs a, Work w) {
+Status launch_class(Ctx* c, CacheArgs a, CacheWork w) {
     using S = Shape<T, D, WM>;
     const uint32_t slots = (uint32_t)sm_count(c->device) * S::CTAS;
-    cut(&w, a.group, S::MB, S::KT, longest_run(w, a.group, S::MB, S::KT, a.n_kv, slots));
+    cache_cut(&w, a.group, S::MB, S::KT, cache_longest_run(w, a.group, S::MB, S::KT, a.n_kv, slots));
     if (w.items * a.n_kv > 0x7FFFFFFFull) return Status(SLHA_ERR_CAPACITY, "attention over a cache: too many blocks of query rows");
     CacheTable tab;
     SLHA_TRY(cache_table(c, w.segs, &tab, &a.table));
     a.n_segs = (uint32_t)w.segs.size();
     CacheMemory mem{c};
-    if (w.blocks) {
-        const size_t rows = (size_t)w.items * a.n_kv * S::MB;
-        void* p;
-        SLHA_TRY(mem.get(pad256(rows * a.d * 4) + rows * 8, &p));
-        a.part_o = (float*)p;
-        a.part_ml = (float*)((char*)p + pad256(rows * a.d * 4));
-    }
+    SLHA_TRY(cache_part_memory(&a, w, S::MB, &mem));
     const size_t smem = a.tree ? S::SMEM_TREE : S::SMEM;
     SLHA_TRY((cache_smem<cache_attend_kernel<T, D, WM>>(c, S::SMEM_TREE)));
     SLHA_CUDA(launch_behind(cache_attend_kernel<T, D, WM>, dim3((uint32_t)(w.items * a.n_kv)), dim3(ATT_THREADS), smem, c->stream, a, tab));
     count_launch();
-    if (w.blocks) {
-        // only the split segments take part: their blocks of query rows are numbered through
-        Work j;
-        for (const CacheSeg& s : w.segs)
-            if (s.n_chunks > 1) j.segs.push_back(s);
-        CacheTable jtab;
-        SLHA_TRY(cache_table(c, j.segs, &jtab, &a.table));
-        a.n_segs = (uint32_t)j.segs.size();
-        uint32_t rows = 0;
-        for (const CacheSeg& s : j.segs) rows = std::max(rows, std::min<uint32_t>(S::MB, s.n_queries * a.group));
-        const uint32_t per = (rows + JOIN_THREADS / 32 - 1) / (JOIN_THREADS / 32);
-        if (w.blocks * a.n_kv * per > 0x7FFFFFFFull) return Status(SLHA_ERR_CAPACITY, "attention over a cache: too many blocks of query rows");
-        SLHA_CUDA(launch_behind(cache_join_kernel<T>, dim3((uint32_t)(w.blocks * a.n_kv * per)), dim3(JOIN_THREADS), 0, c->stream, a, jtab, (uint32_t)S::MB, per));
-        count_launch();
-    }
+    if (w.blocks) SLHA_TRY(launch_cache_join(c, a, sizeof(T) == 2 ? SLHA_B200_BF16 : SLHA_B200_F32, w, S::MB));
     return mem.done();
 }
 template <typename T, int D>
-Status launch_dim(Ctx* c, const CacheArgs& a, int wm, Work w) {
+Status launch_dim(Ctx* c, const CacheArgs& a, int wm, CacheWork w) {
     return wm == 1 ? launch_class<T, D, 1>(c, a, std::move(w)) : wm == 2 ? launch_class<T, D, 2>(c, a, std::move(w)) : launch_class<T, D, 4>(c, a, std::move(w));
 }
 
@@ -574,7 +567,7 @@ Status cache_table(Ctx* c, const std::vector<CacheSeg>& segs, CacheTable* inl, c
 Status launch_attend_cache(Ctx* c, CacheArgs a, int dtype, const std::vector<SlhaB200Segment>& segs) {
     // Segments of at most 16, of at most 32 and of more query rows a KV head: a launch each, so that a batch of decoded tokens beside a prompt keeps
     // the kernel that suits it.
-    Work of[3];
+    CacheWork of[3];
     for (size_t i = 0; i < segs.size(); ++i) {
         const SlhaB200Segment& s = segs[i];
         if (s.n_queries == 0) continue;
@@ -591,6 +584,10 @@ Status launch_attend_cache(Ctx* c, CacheArgs a, int dtype, const std::vector<Slh
     for (int k = 0; k < 3; ++k) {
         if (of[k].segs.empty()) continue;
         const int wm = 1 << k;
+        if (k == 2 && dtype == SLHA_B200_BF16 && a.d <= 128 && a.scale >= 0.0f) {
+            SLHA_TRY(launch_attend_wide(c, a, std::move(of[k])));
+            continue;
+        }
         if (dtype == SLHA_B200_BF16)
             SLHA_TRY(a.d <= 64 ? (launch_dim<__nv_bfloat16, 64>(c, a, wm, std::move(of[k])))
                      : a.d <= 128 ? (launch_dim<__nv_bfloat16, 128>(c, a, wm, std::move(of[k])))

@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(OBS_THREADS) cache_observe_kernel(const __grid
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             float x = s[i][h * 2 + c] * a.scale;
-                            if (has_cap) x = a.cap * tanhf(x / a.cap);
+                            if (has_cap) x = a.cap * cache_tanh(x / a.cap);
                             if (has_slope) x = fmaf(-sl[h], (float)(kp <= qp[h] ? qp[h] - kp : kp - qp[h]), x);
                             if (!all && !(first + col < n && sight.sees(qp[h], kp) && kd == qd[h])) x = -INFINITY;
                             sum[i][c] += exp2_fast((x - lse[h]) * LOG2E);

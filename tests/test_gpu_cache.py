@@ -681,3 +681,25 @@ def test_host_arrays_where_device_memory_is_asked_for_are_refused():
         S.observe_cache(cache, segs, queries, np.zeros(2, F), w, 100)
     assert e.value.code == S.ERR_DEVICE and "lse" in e.value.message
     assert C.sizeof(type(cache.c)) == 96
+
+
+# ---- many query rows: two tiles of 128 a block
+@pytest.mark.parametrize("d", [64, 128, 80])
+@pytest.mark.parametrize("tokens,lens,kv,group", [(33, (33, 100), 1, 1), (128, (128, 129, 500), 1, 1), (129, (129, 700), 2, 1), (64, (1000, 64), 2, 4), (100, (100, 3001), 1, 8), (300, (300,), 2, 3)])
+def test_blocks_of_many_query_rows(d, tokens, lens, kv, group):
+    rng = np.random.default_rng(tokens * d)
+    call, raw = make(rng, lens, tokens, kv, group, d, True)
+    a = check(call, raw, True)
+    b = results(call, True, *on_device(call, raw, True))
+    assert np.array_equal(a[0], b[0]) and np.array_equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("q_scale", [1e-6, 1.0, 12.0, 100.0])
+@pytest.mark.parametrize("cap", [0.0, 1.0, 30.0])
+def test_many_query_rows_whose_largest_scores_come_late(q_scale, cap):
+    # keys grow along the segment, so that the running maximum rises tile after tile
+    rng = np.random.default_rng(int(q_scale * 10) + int(cap))
+    call, raw = make(rng, (1500,), 70, 1, 4, 64, True, q_scale=q_scale, softcap=cap)
+    grow = np.linspace(0.05, 2.0, 1500)[:, None, None]
+    call.keys, raw = K.as_type(call.keys * grow, True)[0], (K.as_type(call.keys * grow, True)[1], raw[1], raw[2])
+    check(call, raw, True)
