@@ -82,14 +82,16 @@ __device__ __forceinline__ uint32_t cache_find(uint32_t n, uint32_t item, F begi
 }
 // tanh.  Up to 1 a polynomial in x^2, the minimax one of tanh(x) / x (found by exchange of extrema in 40 digits): 5e-8 relative in exact arithmetic, 1.2e-7 of 1 in
 // float32; beyond, CUDA's.
+constexpr float TANH_0 = 9.999999502407769e-1f, TANH_1 = -3.3332839153106564e-1f, TANH_2 = 1.3325204076281205e-1f, TANH_3 = -5.345702958893045e-2f,
+                TANH_4 = 2.028998046010164e-2f, TANH_5 = -6.203379131937655e-3f, TANH_6 = 1.041022640341338e-3f;
 __device__ __forceinline__ float tanh_small(float x) {
     const float u = x * x;
-    float p = fmaf(u, 1.041022640341338e-3f, -6.203379131937655e-3f);
-    p = fmaf(u, p, 2.028998046010164e-2f);
-    p = fmaf(u, p, -5.345702958893045e-2f);
-    p = fmaf(u, p, 1.3325204076281205e-1f);
-    p = fmaf(u, p, -3.3332839153106564e-1f);
-    return x * fmaf(u, p, 9.999999502407769e-1f);
+    float p = fmaf(u, TANH_6, TANH_5);
+    p = fmaf(u, p, TANH_4);
+    p = fmaf(u, p, TANH_3);
+    p = fmaf(u, p, TANH_2);
+    p = fmaf(u, p, TANH_1);
+    return x * fmaf(u, p, TANH_0);
 }
 __device__ __forceinline__ float cache_tanh(float x) { return fabsf(x) <= 1.0f ? tanh_small(x) : tanhf(x); }
 // Whether a token sees a row.
@@ -156,7 +158,7 @@ Status cache_smem(Ctx* c, size_t bytes) {
 
 Status cache_part_memory(CacheArgs* a, const CacheWork& w, uint32_t mb, CacheMemory* mem);  // where the parts of split segments go
 Status launch_cache_join(Ctx* c, CacheArgs a, int dtype, const CacheWork& w, uint32_t mb);
-Status launch_attend_wide(Ctx* c, CacheArgs a, CacheWork w);
+Status launch_attend_wide(Ctx* c, CacheArgs a, CacheWork w, bool* taken);
 Status launch_attend_cache(Ctx* c, CacheArgs a, int dtype, const std::vector<SlhaB200Segment>& segs);
 Status launch_observe_cache(Ctx* c, CacheArgs a, int dtype, const std::vector<SlhaB200Segment>& segs);
 Status launch_evict_cache(Ctx* c, EvictArgs a, const std::vector<SlhaB200Segment>& segs, const std::vector<SlhaB200Segment>& to_segs);

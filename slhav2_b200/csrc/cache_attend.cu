@@ -584,9 +584,10 @@ Status launch_attend_cache(Ctx* c, CacheArgs a, int dtype, const std::vector<Slh
     for (int k = 0; k < 3; ++k) {
         if (of[k].segs.empty()) continue;
         const int wm = 1 << k;
-        if (k == 2 && dtype == SLHA_B200_BF16 && a.d <= 128 && a.scale >= 0.0f) {
-            SLHA_TRY(launch_attend_wide(c, a, std::move(of[k])));
-            continue;
+        if (k == 2 && dtype == SLHA_B200_BF16 && a.d <= 128 && a.scale > 0.0f) {
+            bool taken;
+            SLHA_TRY(launch_attend_wide(c, a, of[k], &taken));
+            if (taken) continue;
         }
         if (dtype == SLHA_B200_BF16)
             SLHA_TRY(a.d <= 64 ? (launch_dim<__nv_bfloat16, 64>(c, a, wm, std::move(of[k])))

@@ -3,10 +3,12 @@
 // A CTA takes 256 query rows of one KV head, as two tiles of 128, and a run of the segment's rows in tiles of 128 keys.  Both products run on tcgen05:
 // S = Q K^T (128 x 128, both operands in shared memory) into TMEM, O += P V with P in TMEM, where it takes the place of the S it was made from, and V as it lies
 // (its rows along the contraction).  Four warps a tile of query rows turn S into P, a row a thread; while one tile's scores are turned the other tile's products run.  One
-// thread issues the products, three warps fetch (cp.async, so that rows may lie at any stride of 16 bytes), two key and two value tiles ahead.
+// thread issues the products, one warp fetches, two key and two value tiles ahead: whole tiles by TMA (one map of all rows and KV heads), the tile behind which a segment
+// ends by cp.async, which reads nothing beyond the end and leaves zeros there.
 //
 // O is not scaled with every growth of a row's maximum: weights are taken against the maximum of an earlier tile until a score exceeds it by 2^8 (P then holds up to 256, as
 // exact as below 1), which hardly ever happens after the first tiles.
+#include <cuda.h>
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -18,7 +20,9 @@ namespace slha {
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-constexpr int THREADS = 384, WARPS = THREADS / 32, KT = 128, MB = 256, FETCHERS = 96, MMA_WARP = 8;
+constexpr int THREADS = 384, WARPS = THREADS / 32, KT = 128, MB = 256, MMA_WARP = 8, FETCH_WARP = 9;
+// Registers a thread: 168 for all at the launch; the two warpgroups that hold a row of scores take 200, the third (two of its warps idle) gives them up: 2 x 200 + 104 = 3 x 168.
+constexpr int REGS_ALL = 168, REGS_ROWS = 200, REGS_REST = 104;
 constexpr uint32_t RUN_MOST = 1024;           // key tiles of an item
 constexpr uint32_t HALF = 128 * 128;          // bytes of 128 rows x 64 elements
 constexpr uint32_t SPINS = 1u << 22;          // polls of a wait before it gives up (a fraction of a second)
@@ -28,8 +32,8 @@ template <int D>
 struct Wide {
     static constexpr int HALVES = D / 64;
     static constexpr uint32_t TILE = HALVES * HALF;
-    static constexpr uint32_t K_AT = 2 * TILE, V_AT = 4 * TILE, META_AT = 6 * TILE;   // META: 4 x (positions, documents) of a key tile
-    static constexpr uint32_t LIST_AT = META_AT + 4 * 2 * KT * 4, CLS_AT = LIST_AT + RUN_MOST * 2, ROWS_AT = CLS_AT + RUN_MOST;  // ROWS: position, document, slope, token
+    static constexpr uint32_t K_AT = 2 * TILE, V_AT = 4 * TILE, META_AT = 6 * TILE;   // META: 4 x (positions, documents, distances) of a key tile
+    static constexpr uint32_t LIST_AT = META_AT + 4 * 3 * KT * 4, CLS_AT = LIST_AT + RUN_MOST * 2, ROWS_AT = CLS_AT + RUN_MOST;  // ROWS: position, document, slope, token
     static constexpr uint32_t RANGE_AT = ROWS_AT + 4 * MB * 4, BAR_AT = RANGE_AT + 64, TREE_AT = BAR_AT + 256;
     static constexpr uint32_t SMEM = TREE_AT + 1024, SMEM_TREE = SMEM + TREE_MOST * 8 + MB * (TREE_MOST / 8);
     static_assert(SMEM_TREE <= 227 * 1024, "shared memory of an SM");
@@ -47,6 +51,14 @@ __device__ __forceinline__ bool bar_wait(uint32_t addr, uint32_t parity) {
         if (i > 64) __nanosleep(32);
     }
     return false;
+}
+__device__ __forceinline__ void bar_expect(uint32_t addr, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(addr), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, uint32_t x, uint32_t y, uint32_t z, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(dst), "l"(map), "r"(x), "r"(y),
+                 "r"(z), "r"(bar)
+                 : "memory");
 }
 __device__ __forceinline__ void tc_commit_to(uint32_t addr) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(addr) : "memory");
@@ -71,6 +83,34 @@ __device__ __forceinline__ void mma_shared(uint32_t d, uint64_t a, uint64_t b, u
 __device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add) {
     asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
 }
+template <int N>
+__device__ __forceinline__ void regs_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_less() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(N)); }
+// two float32 at a time
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t r, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;\n" : "=f"(x), "=f"(y) : "l"(r)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// the low x bits of a word
+__device__ __forceinline__ uint32_t low_bits(int x) { return x <= 0 ? 0u : x >= 32 ? 0xFFFFFFFFu : (1u << x) - 1u; }
 #define R8(x, i) "=r"(x[i]), "=r"(x[i + 1]), "=r"(x[i + 2]), "=r"(x[i + 3]), "=r"(x[i + 4]), "=r"(x[i + 5]), "=r"(x[i + 6]), "=r"(x[i + 7])
 #define W8(x, i) "r"(x[i]), "r"(x[i + 1]), "r"(x[i + 2]), "r"(x[i + 3]), "r"(x[i + 4]), "r"(x[i + 5]), "r"(x[i + 6]), "r"(x[i + 7])
 // Columns of this thread's TMEM lane; to be waited for (tmem_wait) and held before they are used.
@@ -90,6 +130,11 @@ __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
 __device__ __forceinline__ bool odd_pair(uint32_t w) { return (w & 0x7F800000u) == 0x7F800000u || (w & 0x00007F80u) == 0x00007F80u; }
 
+// The rows as tensors of three dimensions: an element of a row, then row and KV head, the one of the smaller stride first.
+struct WideMaps {
+    CUtensorMap k, v;
+    uint32_t k_head_first, v_head_first;
+};
 // What a CTA works on.
 struct Item {
     CacheSeg sg;
@@ -168,7 +213,7 @@ __device__ __noinline__ void by_rows(const CacheArgs& a, const Item& w, const ui
 }
 
 template <int D>
-__global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __grid_constant__ CacheArgs a, const __grid_constant__ CacheTable tab) {
+__global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __grid_constant__ CacheArgs a, const __grid_constant__ WideMaps maps, const __grid_constant__ CacheTable tab) {
     using S = Wide<D>;
     dep_wait();
     extern __shared__ unsigned char raw[];
@@ -192,6 +237,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
         w.end_tile = min(tiles, w.first_tile + w.sg.chunk_tiles);
     }
     w.sight = CacheSight{a.window_last, a.prefix ? a.prefix[w.sg.seg] : 0u, a.causal};
+    const CacheSight sight = w.sight;
     w.entry = w.head * a.entry_hs + w.sg.row_begin;
     const bool has_pos = a.row_pos, has_doc = a.row_doc, has_slope = a.slopes, has_cap = a.cap > 0.0f;
     const uint32_t used = min((uint32_t)MB, w.q_rows - w.row0);
@@ -216,15 +262,15 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
 
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
-            bar_init(bar(K_FULL + i), FETCHERS);
-            bar_init(bar(V_FULL + i), FETCHERS);
+            bar_init(bar(K_FULL + i), 1);
+            bar_init(bar(V_FULL + i), 1);
             bar_init(bar(K_FREE + i), 1);
             bar_init(bar(V_FREE + i), 1);
             bar_init(bar(S_FULL + i), 1);
             bar_init(bar(P_FULL + i), 128);
         }
         bar_init(bar(O_FULL), 1);
-        for (int i = 0; i < 4; ++i) bar_init(bar(META_FULL + i), FETCHERS);
+        for (int i = 0; i < 4; ++i) bar_init(bar(META_FULL + i), 1);
         *s_odd = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
@@ -336,16 +382,20 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
     __syncthreads();
     tc_after();
     const uint32_t tmem = *s_tmem;
+    const bool arrays = has_pos || has_doc, drafts_listed = a.tree && (arrays || a.q_pos || sight.window_last != 0xFFFFFFFFu);  // drafted rows whose positions count
+    const uint32_t near_pos = s_qp[0];  // distances are taken from here, so that those of rows nearby are exact in float32
     bool fail = false;
 
     if (warp < 8) {
         // ---- scores to weights: a query row a thread
+        regs_more<REGS_ROWS>();
         const uint32_t t = warp >> 2, r = tid;
         if (t == 0 || two) {
             const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21), ts = lanes + t * 128, to = lanes + 256 + t * 128;
             const float to_log2 = has_cap ? a.scale / a.cap : a.scale * LOG2E, cap2 = a.cap * LOG2E;
-            const uint32_t qp = s_qp[r], qd = s_qd[r];
-            const float slope = s_slope[r];
+            const uint32_t qp = s_qp[r], qd = s_qd[r], n = w.n, ctx = w.ctx, base = w.sg.base, first_tile = w.first_tile;
+            const float slope = s_slope[r], q_at = (float)((long long)qp - (long long)near_pos);
+            const uint32_t* anc = s_anc + s_tok[r] * (TREE_MOST / 32);
             float m = -INFINITY, l = 0.0f;
             for (uint32_t li = 0; li < cnt; ++li) {
                 if (!__all_sync(0xFFFFFFFFu, bar_wait(bar(S_FULL + t), li & 1))) {
@@ -353,7 +403,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
                     break;
                 }
                 tc_after();
-                const uint32_t what = s_list[li];
+                const uint32_t what = s_list[li], first = (first_tile + (what >> 2)) * KT;
                 const bool all = what >> t & 1;
                 uint32_t u[128];
                 float* s = reinterpret_cast<float*>(u);
@@ -363,50 +413,108 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
 #pragma unroll
                 for (int c = 0; c < 128; ++c) asm volatile("" : "+r"(u[c]));
                 float mul = to_log2, top = -INFINITY;
-                if (!all || has_slope || has_cap) {
+                if (has_cap) {
                     mul = 1.0f;
-                    if (has_cap) {
-                        float big = 0.0f;
+                    float big = 0.0f;
 #pragma unroll
-                        for (int c = 0; c < 128; ++c) big = fmaxf(big, fabsf(s[c]));
-                        if (__any_sync(0xFFFFFFFFu, !(big * to_log2 <= 1.0f))) {
+                    for (int c = 0; c < 128; ++c) big = fmaxf(big, fabsf(s[c]));
+                    if (__any_sync(0xFFFFFFFFu, !(big * to_log2 <= 1.0f))) {
 #pragma unroll
-                            for (int c = 0; c < 128; ++c) {  // tanh x = 1 - 2 / (exp(2 x) + 1)
-                                const float e = exp2_fast(s[c] * to_log2 * (2.0f * LOG2E));
-                                s[c] = fmaf(-2.0f * cap2, __frcp_rn(e + 1.0f), cap2);
-                            }
-                        } else {
-#pragma unroll
-                            for (int c = 0; c < 128; ++c) s[c] = cap2 * tanh_small(s[c] * to_log2);
+                        for (int c = 0; c < 128; ++c) {  // tanh x = 1 - 2 / (exp(2 x) + 1)
+                            const float e = exp2_fast(s[c] * to_log2 * (2.0f * LOG2E));
+                            s[c] = fmaf(-2.0f * cap2, __fdividef(1.0f, e + 1.0f), cap2);
                         }
-                    } else {
+                    } else {  // tanh_small, two at a time
+                        const uint64_t in = pair(to_log2, to_log2), out = pair(cap2, cap2);
 #pragma unroll
-                        for (int c = 0; c < 128; ++c) s[c] *= to_log2;
-                    }
-                    if (!all || has_slope) {
-                        if (!__all_sync(0xFFFFFFFFu, bar_wait(bar(META_FULL + (li & 3)), li >> 2 & 1))) {
-                            fail = true;
-                            break;
-                        }
-                        const uint4* kp4 = reinterpret_cast<const uint4*>(s_meta + (li & 3) * 2 * KT);
-                        const uint32_t first = (w.first_tile + (what >> 2)) * KT;
-#pragma unroll
-                        for (int c = 0; c < 128; c += 4) {
-                            const uint4 p4 = kp4[c / 4], d4 = has_doc ? kp4[KT / 4 + c / 4] : make_uint4(0u, 0u, 0u, 0u);
-                            const uint32_t kp[4] = {p4.x, p4.y, p4.z, p4.w}, kd[4] = {d4.x, d4.y, d4.z, d4.w};
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const uint32_t away = kp[e] <= qp ? qp - kp[e] : kp[e] - qp;
-                                if (has_slope) s[c + e] = fmaf(-slope, (float)away, s[c + e]);
-                                if (!all) {
-                                    const uint32_t row = first + c + e;
-                                    bool seen = row < w.n && w.sight.sees(qp, kp[e]) && kd[e] == qd;
-                                    if (a.tree && row >= w.ctx && row < w.n) seen = seen && (s_anc[s_tok[r] * (TREE_MOST / 32) + ((row - w.ctx) >> 5)] >> ((row - w.ctx) & 31) & 1u);
-                                    if (!seen) s[c + e] = -INFINITY;
-                                }
-                            }
+                        for (int c = 0; c < 128; c += 2) {
+                            const uint64_t x = mul2(pair(s[c], s[c + 1]), in), v = mul2(x, x);
+                            uint64_t p = fma2(v, pair(TANH_6, TANH_6), pair(TANH_5, TANH_5));
+                            p = fma2(v, p, pair(TANH_4, TANH_4));
+                            p = fma2(v, p, pair(TANH_3, TANH_3));
+                            p = fma2(v, p, pair(TANH_2, TANH_2));
+                            p = fma2(v, p, pair(TANH_1, TANH_1));
+                            p = fma2(v, p, pair(TANH_0, TANH_0));
+                            unpair(mul2(mul2(x, out), p), s[c], s[c + 1]);
                         }
                     }
+                }
+                const bool listed = has_slope || (!all && (arrays || (drafts_listed && first + KT > ctx)));  // the fetching warp has left the rows' positions
+                if (listed && !__all_sync(0xFFFFFFFFu, bar_wait(bar(META_FULL + (li & 3)), li >> 2 & 1))) {
+                    fail = true;
+                    break;
+                }
+                const uint4* kp4 = reinterpret_cast<const uint4*>(s_meta + (li & 3) * 3 * KT);
+                if (has_slope) {
+#pragma unroll
+                    for (int c = 0; c < 128; c += 4) {
+                        const float4 k = *reinterpret_cast<const float4*>(kp4 + KT / 2 + c / 4);
+                        s[c] = fmaf(s[c], mul, -slope * fabsf(q_at - k.x));
+                        s[c + 1] = fmaf(s[c + 1], mul, -slope * fabsf(q_at - k.y));
+                        s[c + 2] = fmaf(s[c + 2], mul, -slope * fabsf(q_at - k.z));
+                        s[c + 3] = fmaf(s[c + 3], mul, -slope * fabsf(q_at - k.w));
+                    }
+                    mul = 1.0f;
+                }
+                if (!all) {
+                    uint32_t seen[4];  // bits of the rows that this query row sees
+                    if (listed && (arrays || (drafts_listed && first + KT > ctx))) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            seen[j] = 0;
+#pragma unroll 1
+                            for (int g = 0; g < 8; ++g) {
+                                const uint4 p4 = kp4[j * 8 + g], d4 = has_doc ? kp4[KT / 4 + j * 8 + g] : make_uint4(qd, qd, qd, qd);
+                                uint32_t bits = (sight.sees(qp, p4.x) && d4.x == qd ? 1u : 0u) | (sight.sees(qp, p4.y) && d4.y == qd ? 2u : 0u) |
+                                                (sight.sees(qp, p4.z) && d4.z == qd ? 4u : 0u) | (sight.sees(qp, p4.w) && d4.w == qd ? 8u : 0u);
+                                seen[j] |= bits << g * 4;
+                            }
+                        }
+                    } else {  // positions one after another: what is seen are one or two runs
+                        const long long at = (long long)base + first;
+                        const long long low = (long long)qp - sight.window_last - at, high = (sight.causal ? (long long)qp : (long long)qp + sight.window_last) - at + 1;
+                        const int lo = (int)max(0ll, min(low, 128ll)), hi = (int)max(0ll, min(high, 128ll)), pre = (int)max(0ll, min((long long)sight.prefix - at, 128ll));
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) seen[j] = (low_bits(hi - 32 * j) & ~low_bits(lo - 32 * j)) | low_bits(pre - 32 * j);
+                        if (a.tree && first + KT > ctx) {  // (no window: what comes before the drafted rows is seen)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) seen[j] = low_bits((int)ctx - (int)first - 32 * j);
+                        }
+                    }
+                    if (a.tree && first + KT > ctx) {  // of the drafted rows only itself and its ancestors
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int from = (int)first + 32 * j - (int)ctx;  // the word's first row, counted among the drafted
+                            const uint32_t before = low_bits(-from);
+                            uint32_t line = 0;
+                            if (from > -32 && from < (int)TREE_MOST) {
+                                const int word = from >> 5, off = from & 31;  // (word -1: the rows before)
+                                const uint32_t lo = word >= 0 ? anc[word] : 0u, hi = word + 1 < (int)(TREE_MOST / 32) ? anc[word + 1] : 0u;
+                                line = __funnelshift_r(lo, hi, off);
+                            }
+                            seen[j] = drafts_listed ? seen[j] & (before | line) : (seen[j] & before) | (line & ~before);
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        seen[j] &= low_bits((int)min(n - first, 128u) - 32 * j);
+#pragma unroll
+                        for (int c = 0; c < 32; ++c)
+                            if (!(seen[j] >> c & 1u)) s[32 * j + c] = -INFINITY;
+                    }
+                    // values of a tile that not all see
+                    if (!__all_sync(0xFFFFFFFFu, bar_wait(bar(V_FULL + (li & 1)), li >> 1 & 1))) {
+                        fail = true;
+                        break;
+                    }
+                    bool odd = false;
+#pragma unroll 4
+                    for (uint32_t i = tid & 127; i < S::TILE / 16; i += 128) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(sm + S::V_AT + (li & 1) * S::TILE + i * 16);
+                        odd |= odd_pair(x.x) || odd_pair(x.y) || odd_pair(x.z) || odd_pair(x.w);
+                    }
+                    if (odd) *s_odd = 1u;
+                    __syncwarp();
                 }
 #pragma unroll
                 for (int c = 0; c < 128; ++c) top = fmaxf(top, s[c]);
@@ -427,20 +535,28 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
                     }
                 }
                 const float use = m == -INFINITY ? 0.0f : m;
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                const uint64_t mul_2 = pair(mul, mul), use_2 = pair(-use, -use);
+                uint64_t sum_a = pair(0.0f, 0.0f), sum_b = sum_a;
 #pragma unroll
                 for (int c = 0; c < 128; c += 32) {
                     uint32_t p[16];
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
-                        const float x = exp2_fast(fmaf(s[c + e], mul, -use)), y = exp2_fast(fmaf(s[c + e + 1], mul, -use));
-                        sum[e & 2] += x;
-                        sum[(e & 2) + 1] += y;
+                        float x, y;
+                        unpair(fma2(pair(s[c + e], s[c + e + 1]), mul_2, use_2), x, y);
+                        x = exp2_fast(x);
+                        y = exp2_fast(y);
+                        if (e & 2) sum_a = add2(sum_a, pair(x, y));
+                        else sum_b = add2(sum_b, pair(x, y));
                         p[e / 2] = pack_bf16(x, y);
                     }
                     tmem_st16(ts + c / 2, p);
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                {
+                    float x, y;
+                    unpair(add2(sum_a, sum_b), x, y);
+                    l += x + y;
+                }
                 tmem_wait_st();
                 tc_before();
                 bar_arrive(bar(P_FULL + t));
@@ -475,7 +591,10 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
             }
             if (there) out.statistics(a, w, r, m, l);
         }
-    } else if (warp == MMA_WARP) {
+        regs_less<REGS_ALL>();
+    } else {
+        regs_less<REGS_REST>();
+        if (warp == MMA_WARP) {
         // ---- the products
         uint32_t lead;
         asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xFFFFFFFF;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(lead));
@@ -532,79 +651,98 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
             tc_commit_to(bar(O_FULL));
         }
         __syncwarp();
-    } else {
-        // ---- rows into shared memory.  A tile's copies are announced when the next ones have been issued.
-        const uint32_t x0 = tid - 288;
+        } else if (warp == FETCH_WARP) {
+        // ---- rows into shared memory
         const unsigned char* kb = static_cast<const unsigned char*>(a.keys) + (w.sg.row_begin * a.krs + w.head * a.khs) * 2;
         const unsigned char* vb = static_cast<const unsigned char*>(a.values) + (w.sg.row_begin * a.vrs + w.head * a.vhs) * 2;
         constexpr int PIECES = S::HALVES * 8;
-        const auto fetch = [&](uint32_t dst, const unsigned char* from, uint64_t stride, uint32_t first) {
-            for (uint32_t i = x0; i < KT * PIECES; i += FETCHERS) {
-                const uint32_t r = i / PIECES, c = i % PIECES, row = first + r;
-                const bool there = row < w.n && c * 8 < a.d;
-                copy16(dst + (c >> 3) * HALF + r * 128 + (((c & 7) ^ (r & 7)) << 4), there ? from + row * stride * 2 + c * 16 : from, there);
+        const auto fetch = [&](uint32_t dst, const CUtensorMap* map, bool head_first, const unsigned char* from, uint64_t stride, uint32_t first, uint32_t full) {
+            if (first + KT <= w.n) {
+                if (lane == 0) {
+                    const uint32_t row = (uint32_t)w.sg.row_begin + first;
+                    bar_expect(full, S::TILE);
+#pragma unroll
+                    for (int h = 0; h < S::HALVES; ++h) tma_load(dst + h * HALF, map, h * 64, head_first ? w.head : row, head_first ? row : w.head, full);
+                }
+            } else {
+                for (uint32_t i = lane; i < KT * PIECES; i += 32) {
+                    const uint32_t r = i / PIECES, c = i % PIECES, row = first + r;
+                    const bool there = row < w.n && c * 8 < a.d;
+                    copy16(dst + (c >> 3) * HALF + r * 128 + (((c & 7) ^ (r & 7)) << 4), there ? from + row * stride * 2 + c * 16 : from, there);
+                }
+                copy_commit();
+                copy_wait<0>();
+                asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                __syncwarp();
+                if (lane == 0) bar_arrive(full);
             }
-            copy_commit();
-        };
-        const auto say = [&](int which) {
-            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-            bar_arrive(bar(which));
-        };
-        // values of a tile that not all see: a thread looks at the pieces that it has fetched
-        const auto look = [&](uint32_t li) {
-            if ((s_list[li] & 3u) == (two ? 3u : 1u) || (!two && (s_list[li] & 1u))) return;
-            bool odd = false;
-            for (uint32_t i = x0; i < KT * PIECES; i += FETCHERS) {
-                const uint32_t r = i / PIECES, c = i % PIECES;
-                const uint4 v = *reinterpret_cast<const uint4*>(sm + S::V_AT + (li & 1) * S::TILE + (c >> 3) * HALF + r * 128 + (((c & 7) ^ (r & 7)) << 4));
-                odd |= odd_pair(v.x) || odd_pair(v.y) || odd_pair(v.z) || odd_pair(v.w);
-            }
-            if (odd) *s_odd = 1u;
         };
         for (uint32_t li = 0; li < cnt; ++li) {
-            const uint32_t slot = li & 1, first = (w.first_tile + (s_list[li] >> 2)) * KT;
-            if (li >= 2 && !bar_wait(bar(K_FREE + slot), (li >> 1) - 1 & 1)) {
+            const uint32_t slot = li & 1, what = s_list[li], first = (w.first_tile + (what >> 2)) * KT;
+            if (li >= 2 && !__all_sync(0xFFFFFFFFu, bar_wait(bar(K_FREE + slot), (li >> 1) - 1 & 1))) {
                 fail = true;
                 break;
             }
+            fetch(sb + S::K_AT + slot * S::TILE, &maps.k, maps.k_head_first, kb, a.krs, first, bar(K_FULL + slot));
             // (the tile four before this one has been turned into weights: its positions are no longer read)
-            for (uint32_t i = x0; i < KT; i += FETCHERS) {
-                const uint32_t row = min(first + i, w.n - 1);
-                uint32_t* at = s_meta + (li & 3) * 2 * KT + i;
-                at[0] = has_pos ? a.row_pos[w.entry + row] : a.tree && row >= w.ctx ? w.sg.base + w.ctx + s_depth[row - w.ctx] : w.sg.base + row;
-                if (has_doc) at[KT] = a.row_doc[w.entry + row];
+            const bool whole = (what & (two ? 3u : 1u)) == (two ? 3u : 1u);
+            if (has_slope || (!whole && (arrays || (drafts_listed && first + KT > w.ctx)))) {
+                for (uint32_t i = lane; i < KT; i += 32) {
+                    const uint32_t row = min(first + i, w.n - 1);
+                    uint32_t* at = s_meta + (li & 3) * 3 * KT + i;
+                    const uint32_t p = has_pos ? a.row_pos[w.entry + row] : a.tree && row >= w.ctx ? w.sg.base + w.ctx + s_depth[row - w.ctx] : w.sg.base + row;
+                    at[0] = p;
+                    if (has_doc) at[KT] = a.row_doc[w.entry + row];
+                    at[2 * KT] = __float_as_uint((float)((long long)p - (long long)near_pos));
+                }
             }
-            bar_arrive(bar(META_FULL + (li & 3)));
-            fetch(sb + S::K_AT + slot * S::TILE, kb, a.krs, first);
-            if (li > 0) {
-                copy_wait<1>();
-                look(li - 1);
-                say(V_FULL + (slot ^ 1));
-            }
-            if (li >= 2 && !bar_wait(bar(V_FREE + slot), (li >> 1) - 1 & 1)) {
+            __syncwarp();
+            if (lane == 0) bar_arrive(bar(META_FULL + (li & 3)));
+            if (li >= 2 && !__all_sync(0xFFFFFFFFu, bar_wait(bar(V_FREE + slot), (li >> 1) - 1 & 1))) {
                 fail = true;
                 break;
             }
-            fetch(sb + S::V_AT + slot * S::TILE, vb, a.vrs, first);
-            copy_wait<1>();
-            say(K_FULL + slot);
+            fetch(sb + S::V_AT + slot * S::TILE, &maps.v, maps.v_head_first, vb, a.vrs, first, bar(V_FULL + slot));
         }
-        copy_wait<0>();
-        if (cnt && !fail) {
-            look(cnt - 1);
-            say(V_FULL + (cnt - 1 & 1));
         }
     }
     if (fail) *s_odd = 1u;
     tc_before();
-    __syncthreads();
+    __syncthreads();  // (the rows' warps have given their registers back: none of the others takes them while one still has to get them)
     tc_after();
+    if (warp >= 8) regs_more<REGS_ALL>();
     if (warp == MMA_WARP) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512u) : "memory");
-    if (*s_odd) by_rows(a, w, s_qp, s_qd, s_slope, s_tok, s_depth, s_anc);
+    if (*s_odd) {
+        const Item again = w;
+        by_rows(a, again, s_qp, s_qd, s_slope, s_tok, s_depth, s_anc);
+    }
+}
+
+// A map of rows x KV heads x elements in boxes of 128 rows of one KV head x 64 elements; false where the driver does not take the layout.
+bool wide_map(CUtensorMap* map, const void* base, uint64_t row_stride, uint64_t head_stride, uint64_t rows, uint32_t heads, uint32_t d, uint32_t* head_first) {
+    using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const Encode encode = []() -> Encode {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) {
+            cudaGetLastError();
+            return nullptr;
+        }
+        return reinterpret_cast<Encode>(p);
+    }();
+    if (!encode || rows > 0x7FFFFFFFull) return false;
+    if (heads == 1) head_stride = row_stride * rows;  // (never stepped by)
+    *head_first = head_stride < row_stride;
+    const cuuint64_t dims[3] = {d, *head_first ? heads : rows, *head_first ? rows : heads};
+    const cuuint64_t strides[2] = {(*head_first ? head_stride : row_stride) * 2, (*head_first ? row_stride : head_stride) * 2};
+    const cuuint32_t box[3] = {64, *head_first ? 1u : (cuuint32_t)KT, *head_first ? (cuuint32_t)KT : 1u}, each[3] = {1, 1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <int D>
-Status launch_wide(Ctx* c, CacheArgs a, CacheWork w) {
+Status launch_wide(Ctx* c, CacheArgs a, CacheWork w, const WideMaps& maps) {
     using S = Wide<D>;
     cache_cut(&w, a.group, MB, KT, std::min(RUN_MOST, cache_longest_run(w, a.group, MB, KT, a.n_kv, (uint32_t)sm_count(c->device))));
     if (w.items * a.n_kv > 0x7FFFFFFFull) return Status(SLHA_ERR_CAPACITY, "attention over a cache: too many blocks of query rows");
@@ -614,7 +752,12 @@ Status launch_wide(Ctx* c, CacheArgs a, CacheWork w) {
     CacheMemory mem{c};
     SLHA_TRY(cache_part_memory(&a, w, MB, &mem));
     SLHA_TRY((cache_smem<cache_attend_wide_kernel<D>>(c, S::SMEM_TREE)));
-    SLHA_CUDA(launch_behind(cache_attend_wide_kernel<D>, dim3((uint32_t)(w.items * a.n_kv)), dim3(THREADS), a.tree ? S::SMEM_TREE : S::SMEM, c->stream, a, tab));
+    static const int regs = []() {
+        cudaFuncAttributes at;
+        return cudaFuncGetAttributes(&at, cache_attend_wide_kernel<D>) == cudaSuccess ? at.numRegs : 0;
+    }();
+    if (regs != REGS_ALL) return Status(SLHA_ERR_DEVICE, "attention over a cache: the kernel was built with other registers than its warps share out");
+    SLHA_CUDA(launch_behind(cache_attend_wide_kernel<D>, dim3((uint32_t)(w.items * a.n_kv)), dim3(THREADS), a.tree ? S::SMEM_TREE : S::SMEM, c->stream, a, maps, tab));
     count_launch();
     if (w.blocks) SLHA_TRY(launch_cache_join(c, a, SLHA_B200_BF16, w, MB));
     return mem.done();
@@ -622,6 +765,14 @@ Status launch_wide(Ctx* c, CacheArgs a, CacheWork w) {
 
 }  // namespace
 
-Status launch_attend_wide(Ctx* c, CacheArgs a, CacheWork w) { return a.d <= 64 ? launch_wide<64>(c, a, std::move(w)) : launch_wide<128>(c, a, std::move(w)); }
+Status launch_attend_wide(Ctx* c, CacheArgs a, CacheWork w, bool* taken) {
+    uint64_t rows = 0;
+    for (const CacheSeg& s : w.segs) rows = std::max(rows, s.row_begin + s.n_rows);
+    WideMaps maps;
+    *taken = wide_map(&maps.k, a.keys, a.krs, a.khs, std::max<uint64_t>(rows, 1), a.n_kv, a.d, &maps.k_head_first) &&
+             wide_map(&maps.v, a.values, a.vrs, a.vhs, std::max<uint64_t>(rows, 1), a.n_kv, a.d, &maps.v_head_first);
+    if (!*taken) return Status();
+    return a.d <= 64 ? launch_wide<64>(c, a, std::move(w), maps) : launch_wide<128>(c, a, std::move(w), maps);
+}
 
 }  // namespace slha
