@@ -33,13 +33,13 @@ struct Wide {
     static constexpr int HALVES = D / 64;
     static constexpr uint32_t TILE = HALVES * HALF;
     static constexpr uint32_t K_AT = 2 * TILE, V_AT = 4 * TILE, META_AT = 6 * TILE;   // META: 4 x (positions, documents, distances) of a key tile
-    static constexpr uint32_t LIST_AT = META_AT + 4 * 3 * KT * 4, CLS_AT = LIST_AT + RUN_MOST * 2, ROWS_AT = CLS_AT + RUN_MOST;  // ROWS: position, document, slope, token
-    static constexpr uint32_t RANGE_AT = ROWS_AT + 4 * MB * 4, BAR_AT = RANGE_AT + 64, TREE_AT = BAR_AT + 256;
+    static constexpr uint32_t LIST_AT = META_AT + 4 * 3 * KT * 4, CLS_AT = LIST_AT + RUN_MOST * 2, ROWS_AT = CLS_AT + RUN_MOST;  // ROWS: offset in q (64 bits), position, document, slope, token
+    static constexpr uint32_t RANGE_AT = ROWS_AT + 6 * MB * 4, BAR_AT = RANGE_AT + 64, TREE_AT = BAR_AT + 256;
     static constexpr uint32_t SMEM = TREE_AT + 1024, SMEM_TREE = SMEM + TREE_MOST * 8 + MB * (TREE_MOST / 8);
     static_assert(SMEM_TREE <= 227 * 1024, "shared memory of an SM");
 };
 // barriers, 8 bytes each
-enum { K_FULL = 0, V_FULL = 2, K_FREE = 4, V_FREE = 6, S_FULL = 8, P_FULL = 10, O_FULL = 12, TMEM_WORD = 13, ODD_WORD = 14, META_FULL = 16 };
+enum { K_FULL = 0, V_FULL = 2, K_FREE = 4, V_FREE = 6, S_FULL = 8, P_FULL = 10, O_FULL = 12, TMEM_WORD = 13, ODD_WORD = 14, META_FULL = 16, P_HALF = 20 };
 
 __device__ __forceinline__ void bar_init(uint32_t addr, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(addr), "r"(count) : "memory"); }
 __device__ __forceinline__ void bar_arrive(uint32_t addr) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(addr) : "memory"); }
@@ -246,7 +246,8 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
     uint32_t* s_meta = reinterpret_cast<uint32_t*>(sm + S::META_AT);
     uint16_t* s_list = reinterpret_cast<uint16_t*>(sm + S::LIST_AT);
     unsigned char* s_cls = sm + S::CLS_AT;
-    uint32_t* s_qp = reinterpret_cast<uint32_t*>(sm + S::ROWS_AT);
+    uint64_t* s_q = reinterpret_cast<uint64_t*>(sm + S::ROWS_AT);
+    uint32_t* s_qp = reinterpret_cast<uint32_t*>(s_q + MB);
     uint32_t* s_qd = s_qp + MB;
     float* s_slope = reinterpret_cast<float*>(s_qd + MB);
     uint32_t* s_tok = reinterpret_cast<uint32_t*>(s_slope + MB);
@@ -267,6 +268,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
             bar_init(bar(K_FREE + i), 1);
             bar_init(bar(V_FREE + i), 1);
             bar_init(bar(S_FULL + i), 1);
+            bar_init(bar(P_HALF + i), 128);
             bar_init(bar(P_FULL + i), 128);
         }
         bar_init(bar(O_FULL), 1);
@@ -298,24 +300,21 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
         }
         __syncthreads();
     }
-    {
-        const unsigned char* q = static_cast<const unsigned char*>(a.q);
-        for (int i = tid; i < (two ? MB : 128) * S::HALVES * 8; i += THREADS) {
-            const uint32_t r = i / (S::HALVES * 8), c = i % (S::HALVES * 8), row = w.row0 + r;
-            const bool there = row < w.q_rows && c * 8 < a.d;
-            const uint64_t at = there ? (uint64_t)(w.sg.query_begin + row / a.group) * a.qts + (uint64_t)(w.head * a.group + row % a.group) * a.qhs + c * 8 : 0;
-            copy16(sb + (r >> 7) * S::TILE + (c >> 3) * HALF + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4), q + at * 2, there);
-        }
-        copy_commit();
-    }
-    for (uint32_t r = tid; r < MB; r += THREADS) {
-        const uint32_t row = min(w.row0 + r, w.q_rows - 1), tok = row / a.group;
+    for (uint32_t r = tid; r < MB; r += THREADS) {  // (rows behind the last repeat it, and are zeros among the queries)
+        const uint32_t row = min(w.row0 + r, w.q_rows - 1), tok = row / a.group, h = w.head * a.group + row - tok * a.group;
+        s_q[r] = ((uint64_t)(w.sg.query_begin + tok) * a.qts + (uint64_t)h * a.qhs) * 2;
         s_qp[r] = a.q_pos ? a.q_pos[w.sg.query_begin + tok] : w.sg.base + w.ctx + (a.tree ? s_depth[tok] : tok);
         s_qd[r] = has_doc ? a.q_doc[w.sg.query_begin + tok] : 0u;
-        s_slope[r] = has_slope ? a.slopes[w.head * a.group + row % a.group] * LOG2E : 0.0f;
+        s_slope[r] = has_slope ? a.slopes[h] * LOG2E : 0.0f;
         s_tok[r] = tok - tok0;
     }
     __syncthreads();
+    for (int i = tid; i < (two ? MB : 128) * S::HALVES * 8; i += THREADS) {
+        const uint32_t r = i / (S::HALVES * 8), c = i % (S::HALVES * 8);
+        const bool there = r < used && c * 8 < a.d;
+        copy16(sb + (r >> 7) * S::TILE + (c >> 3) * HALF + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4), static_cast<const unsigned char*>(a.q) + (there ? s_q[r] + c * 16 : 0), there);
+    }
+    copy_commit();
     if (warp < 2) {  // positions and documents of either tile of query rows
         CacheRanges q{0xFFFFFFFFu, 0u, 0xFFFFFFFFu, 0u};
         for (int r = warp * 128 + lane; r < warp * 128 + 128; r += 32) {
@@ -340,26 +339,32 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
             return (x || y ? 1 : 0) | (x == 2 ? 2 : 0) | (y == 2 ? 4 : 0);
         };
         if (has_pos || has_doc) {
-            for (uint32_t j = warp; j < in_run; j += WARPS) {
-                const uint32_t first = (w.first_tile + j) * KT;
-                CacheRanges k{0xFFFFFFFFu, 0u, has_doc ? 0xFFFFFFFFu : 0u, 0u};
+            constexpr int AT_ONCE = 3;  // tiles whose loads a warp has under way
+            for (uint32_t j0 = warp; j0 < in_run; j0 += WARPS * AT_ONCE) {
+                CacheRanges k[AT_ONCE];
 #pragma unroll
-                for (int e = 0; e < KT / 32; ++e) {
-                    const uint32_t i = min(first + lane + e * 32, w.n - 1);
-                    const uint32_t p = has_pos ? a.row_pos[w.entry + i] : w.sg.base + i;
-                    k.pmin = min(k.pmin, p);
-                    k.pmax = max(k.pmax, p);
-                    if (has_doc) {
-                        const uint32_t d = a.row_doc[w.entry + i];
-                        k.dmin = min(k.dmin, d);
-                        k.dmax = max(k.dmax, d);
+                for (int x = 0; x < AT_ONCE; ++x) {
+                    const uint32_t first = (w.first_tile + min(j0 + x * WARPS, in_run - 1)) * KT;
+                    k[x] = CacheRanges{0xFFFFFFFFu, 0u, has_doc ? 0xFFFFFFFFu : 0u, 0u};
+#pragma unroll
+                    for (int e = 0; e < KT / 32; ++e) {
+                        const uint32_t i = min(first + lane + e * 32, w.n - 1);
+                        const uint32_t p = has_pos ? a.row_pos[w.entry + i] : w.sg.base + i, d = has_doc ? a.row_doc[w.entry + i] : 0u;
+                        k[x].pmin = min(k[x].pmin, p);
+                        k[x].pmax = max(k[x].pmax, p);
+                        k[x].dmin = min(k[x].dmin, d);
+                        k[x].dmax = max(k[x].dmax, d);
                     }
                 }
-                k.pmin = __reduce_min_sync(0xFFFFFFFFu, k.pmin);
-                k.pmax = __reduce_max_sync(0xFFFFFFFFu, k.pmax);
-                k.dmin = __reduce_min_sync(0xFFFFFFFFu, k.dmin);
-                k.dmax = __reduce_max_sync(0xFFFFFFFFu, k.dmax);
-                if (lane == 0) s_cls[j] = (unsigned char)classes(k, first + KT - 1);
+#pragma unroll
+                for (int x = 0; x < AT_ONCE; ++x) {
+                    const uint32_t j = j0 + x * WARPS;
+                    k[x].pmin = __reduce_min_sync(0xFFFFFFFFu, k[x].pmin);
+                    k[x].pmax = __reduce_max_sync(0xFFFFFFFFu, k[x].pmax);
+                    k[x].dmin = __reduce_min_sync(0xFFFFFFFFu, k[x].dmin);
+                    k[x].dmax = __reduce_max_sync(0xFFFFFFFFu, k[x].dmax);
+                    if (lane == 0 && j < in_run) s_cls[j] = (unsigned char)classes(k[x], (w.first_tile + j) * KT + KT - 1);
+                }
             }
         } else {
             for (uint32_t j = tid; j < in_run; j += THREADS) {
@@ -412,7 +417,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
                 tmem_wait_ld();
 #pragma unroll
                 for (int c = 0; c < 128; ++c) asm volatile("" : "+r"(u[c]));
-                float mul = to_log2, top = -INFINITY;
+                float mul = to_log2, top;
                 if (has_cap) {
                     mul = 1.0f;
                     float big = 0.0f;
@@ -516,9 +521,14 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
                     if (odd) *s_odd = 1u;
                     __syncwarp();
                 }
+                {
+                    float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int c = 0; c < 128; ++c) top = fmaxf(top, s[c]);
-                top *= mul;
+                    for (int c = 0; c < 128; c += 8)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[e] = fmaxf(x[e], fmaxf(s[c + 2 * e], s[c + 2 * e + 1]));
+                    top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * mul;
+                }
                 if (__any_sync(0xFFFFFFFFu, top > m + LAZY)) {
                     const float now = fmaxf(m, top), f = m == -INFINITY ? 0.0f : exp2_fast(m - now);
                     m = now;
@@ -543,7 +553,8 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
                         float x, y;
-                        unpair(fma2(pair(s[c + e], s[c + e + 1]), mul_2, use_2), x, y);
+                        const uint64_t z = fma2(pair(s[c + e], s[c + e + 1]), mul_2, use_2);
+                        unpair(z, x, y);
                         x = exp2_fast(x);
                         y = exp2_fast(y);
                         if (e & 2) sum_a = add2(sum_a, pair(x, y));
@@ -551,6 +562,11 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
                         p[e / 2] = pack_bf16(x, y);
                     }
                     tmem_st16(ts + c / 2, p);
+                    if (c == 32) {  // the products with the first half of the values may begin
+                        tmem_wait_st();
+                        tc_before();
+                        bar_arrive(bar(P_HALF + t));
+                    }
                 }
                 {
                     float x, y;
@@ -565,31 +581,57 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
                 fail = !__all_sync(0xFFFFFFFFu, bar_wait(bar(O_FULL), 0));
                 tc_after();
             }
-            // (TMEM is read by the whole warp, behind the rows' end too)
+            // Rows leave through shared memory, where the queries were: a warp writes whole rows.
             const bool there = r < used;
-            const RowOut out = row_out(a, w, there ? r : 0);
-            const float inv = out.out ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
+            const uint32_t tok = tok0 + s_tok[r], q_head = w.head * a.group + (there ? w.row0 + r - tok * a.group : 0u);
+            const bool whole = w.sg.n_chunks == 1;
+            const uint64_t part = ((uint64_t)w.item * a.n_kv + w.head) * MB + r;
+            const uint64_t mine = whole ? (uint64_t)a.out + ((uint64_t)(w.sg.query_begin + tok) * a.ots + (uint64_t)q_head * a.ohs) * 2 : (uint64_t)(a.part_o + part * a.d);
+            const float inv = !cnt || l == 0.0f ? 0.0f : whole ? 1.0f / l : 1.0f;
+            constexpr int LINE = D * 2, LINE_PIECES = LINE / 16;  // bytes of a row at a time: all of its bfloat16 elements, or half of its float32 ones
+            unsigned char* stage = sm + t * S::TILE + (warp & 3) * 32 * LINE;
+            __syncwarp();
+            for (int pass = 0; pass < (whole ? 1 : 2); ++pass) {
 #pragma unroll
-            for (int c = 0; c < D; c += 16) {
-                __syncwarp();
-                uint32_t o[16];
-                tmem_ld16(to + c, o);
-                float x[16];
+                for (int c = 0; c < D / 16; ++c) {
+                    if (!whole && c >= D / 32) break;
+                    uint32_t o[16];
+                    tmem_ld16(to + pass * (D / 2) + c * 16, o);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) x[e] = cnt && l != 0.0f ? __uint_as_float(o[e]) * inv : 0.0f;
+                    for (int e = 0; e < 16; ++e) o[e] = inv != 0.0f ? __float_as_uint(__uint_as_float(o[e]) * inv) : 0u;
+                    if (whole) {
 #pragma unroll
-                for (int h = 0; h < 16; h += 8) {
-                    if (!there || c + h >= (int)a.d) continue;
-                    if (out.out) {
-                        *reinterpret_cast<uint4*>(out.out + (c + h) * 2) =
-                            make_uint4(pack_bf16(x[h], x[h + 1]), pack_bf16(x[h + 2], x[h + 3]), pack_bf16(x[h + 4], x[h + 5]), pack_bf16(x[h + 6], x[h + 7]));
+                        for (int h = 0; h < 2; ++h) {
+                            uint32_t x[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) x[e] = pack_bf16(__uint_as_float(o[8 * h + 2 * e]), __uint_as_float(o[8 * h + 2 * e + 1]));
+                            *reinterpret_cast<uint4*>(stage + lane * LINE + (((c * 2 + h) ^ (lane & 7)) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
+                        }
                     } else {
-                        *reinterpret_cast<float4*>(out.part + c + h) = make_float4(x[h], x[h + 1], x[h + 2], x[h + 3]);
-                        *reinterpret_cast<float4*>(out.part + c + h + 4) = make_float4(x[h + 4], x[h + 5], x[h + 6], x[h + 7]);
+#pragma unroll
+                        for (int h = 0; h < 4; ++h)
+                            *reinterpret_cast<uint4*>(stage + lane * LINE + (((c * 4 + h) ^ (lane & 7)) << 4)) = make_uint4(o[4 * h], o[4 * h + 1], o[4 * h + 2], o[4 * h + 3]);
                     }
                 }
+                __syncwarp();
+#pragma unroll 4
+                for (int i = lane; i < 32 * LINE_PIECES; i += 32) {
+                    const int row = i / LINE_PIECES, c = i % LINE_PIECES;
+                    const uint64_t dst = __shfl_sync(0xFFFFFFFFu, mine, row);
+                    const uint4 x = *reinterpret_cast<const uint4*>(stage + row * LINE + ((c ^ (row & 7)) << 4));
+                    const uint32_t col = whole ? c * 8 : pass * (D / 2) + c * 4;
+                    if ((warp * 32 + row) < (int)used && col < a.d) *reinterpret_cast<uint4*>(dst + col * (whole ? 2 : 4)) = x;
+                }
+                __syncwarp();
             }
-            if (there) out.statistics(a, w, r, m, l);
+            if (there) {
+                if (whole) {
+                    if (a.lse) a.lse[(uint64_t)(w.sg.query_begin + tok) * a.n_heads + q_head] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
+                } else {
+                    a.part_ml[part * 2] = l == 0.0f ? -INFINITY : m;
+                    a.part_ml[part * 2 + 1] = l;
+                }
+            }
         }
         regs_less<REGS_ALL>();
     } else {
@@ -608,10 +650,16 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
                 }
                 tc_commit_to(bar(S_FULL + t));
             };
-            const auto values = [&](uint32_t li, uint32_t t) {
+            const auto values = [&](uint32_t li, uint32_t t) {  // in two halves, as the weights come
                 const uint32_t v = sb + S::V_AT + (li & 1) * S::TILE;
 #pragma unroll
-                for (int kk = 0; kk < KT / 16; ++kk) mma_tmem(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, desc_across(v + kk * 2048), wide_idesc(D, true), li > 0 || kk > 0);
+                for (int h = 0; h < 2; ++h) {
+                    if (!bar_wait(bar((h ? P_FULL : P_HALF) + t), li & 1)) return false;
+                    tc_after();
+#pragma unroll
+                    for (int kk = h * 4; kk < h * 4 + 4; ++kk) mma_tmem(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, desc_across(v + kk * 2048), wide_idesc(D, true), li > 0 || kk > 0);
+                }
+                return true;
             };
             fail = !bar_wait(bar(K_FULL), 0);
             if (!fail) {
@@ -621,12 +669,10 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
             }
             for (uint32_t li = 0; li < cnt && !fail; ++li) {
                 const bool more = li + 1 < cnt;
-                if (!bar_wait(bar(V_FULL + (li & 1)), li >> 1 & 1) || !bar_wait(bar(P_FULL), li & 1)) {
+                if (!bar_wait(bar(V_FULL + (li & 1)), li >> 1 & 1) || !values(li, 0)) {
                     fail = true;
                     break;
                 }
-                tc_after();
-                values(li, 0);
                 if (more) {
                     if (!bar_wait(bar(K_FULL + (li + 1 & 1)), (li + 1) >> 1 & 1)) {
                         fail = true;
@@ -634,13 +680,9 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
                     }
                     scores(li + 1, 0);
                 }
-                if (two) {
-                    if (!bar_wait(bar(P_FULL + 1), li & 1)) {
-                        fail = true;
-                        break;
-                    }
-                    tc_after();
-                    values(li, 1);
+                if (two && !values(li, 1)) {
+                    fail = true;
+                    break;
                 }
                 tc_commit_to(bar(V_FREE + (li & 1)));
                 if (more) {
