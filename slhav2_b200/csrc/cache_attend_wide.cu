@@ -33,13 +33,13 @@ struct Wide {
     static constexpr int HALVES = D / 64;
     static constexpr uint32_t TILE = HALVES * HALF;
     static constexpr uint32_t K_AT = 2 * TILE, V_AT = 4 * TILE, META_AT = 6 * TILE;   // META: 4 x (positions, documents, distances) of a key tile
-    static constexpr uint32_t LIST_AT = META_AT + 4 * 3 * KT * 4, CLS_AT = LIST_AT + RUN_MOST * 2, ROWS_AT = CLS_AT + RUN_MOST;  // ROWS: offset in q (64 bits), position, document, slope, token
+    static constexpr uint32_t LIST_AT = META_AT + 4 * 3 * KT * 4, CLS_AT = LIST_AT + RUN_MOST * 4, ROWS_AT = CLS_AT + RUN_MOST;  // ROWS: offset in q (64 bits), position, document, slope, token
     static constexpr uint32_t RANGE_AT = ROWS_AT + 6 * MB * 4, BAR_AT = RANGE_AT + 64, TREE_AT = BAR_AT + 256;
     static constexpr uint32_t SMEM = TREE_AT + 1024, SMEM_TREE = SMEM + TREE_MOST * 8 + MB * (TREE_MOST / 8);
     static_assert(SMEM_TREE <= 227 * 1024, "shared memory of an SM");
 };
 // barriers, 8 bytes each
-enum { K_FULL = 0, V_FULL = 2, K_FREE = 4, V_FREE = 6, S_FULL = 8, P_FULL = 10, O_FULL = 12, TMEM_WORD = 13, ODD_WORD = 14, META_FULL = 16, P_HALF = 20 };
+enum { K_FULL = 0, V_FULL = 2, K_FREE = 4, V_FREE = 6, S_FULL = 8, P_FULL = 10, O_FULL = 12, TMEM_WORD = 13, ODD_WORD = 14, META_FULL = 16, P_HALF = 20, Q_FULL = 22 };
 
 __device__ __forceinline__ void bar_init(uint32_t addr, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(addr), "r"(count) : "memory"); }
 __device__ __forceinline__ void bar_arrive(uint32_t addr) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(addr) : "memory"); }
@@ -59,6 +59,9 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, u
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(dst), "l"(map), "r"(x), "r"(y),
                  "r"(z), "r"(bar)
                  : "memory");
+}
+__device__ __forceinline__ void tma_store(const CUtensorMap* map, uint32_t src, uint32_t x, uint32_t y, uint32_t z) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];\n" ::"l"(map), "r"(x), "r"(y), "r"(z), "r"(src) : "memory");
 }
 __device__ __forceinline__ void tc_commit_to(uint32_t addr) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(addr) : "memory");
@@ -128,17 +131,19 @@ __device__ __forceinline__ void tmem_st16(uint32_t t, const uint32_t* x) {
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
-__device__ __forceinline__ bool odd_pair(uint32_t w) { return (w & 0x7F800000u) == 0x7F800000u || (w & 0x00007F80u) == 0x00007F80u; }
+// bits 31 and 15: whether the two bfloat16 are not finite (their exponents' bits are all set)
+__device__ __forceinline__ uint32_t odd_pair(uint32_t w) { return (w & 0x7F807F80u) + 0x00800080u; }
 
-// The rows as tensors of three dimensions: an element of a row, then row and KV head, the one of the smaller stride first.
+// The rows as tensors of three dimensions: an element of a row, then row and KV head, the one of the smaller stride first.  Queries and outputs: element, head, token.
 struct WideMaps {
     CUtensorMap k, v;
-    uint32_t k_head_first, v_head_first;
+    CUtensorMap q, out;  // boxes of 32 query rows, where the head's group divides 32
+    uint32_t k_head_first, v_head_first, q_boxes, out_boxes;
 };
 // What a CTA works on.
 struct Item {
     CacheSeg sg;
-    uint32_t head, item, row0, q_rows, n, ctx, first_tile, end_tile;
+    uint32_t head, item, row0, q_rows, n, ctx;
     CacheSight sight;
     uint64_t entry;
 };
@@ -169,7 +174,7 @@ __device__ __forceinline__ RowOut row_out(const CacheArgs& a, const Item& w, uin
 // The item again on the CUDA cores, a warp a query row and a row of the cache at a time, where only what is seen is read: for values that are not finite in a tile that not all see
 // (a weight of zero would not keep them out of the sums), and where a wait ran out.
 __device__ __noinline__ void by_rows(const CacheArgs& a, const Item& w, const uint32_t* s_qp, const uint32_t* s_qd, const float* s_slope, const uint32_t* s_tok, const uint32_t* s_depth,
-                                     const uint32_t* s_anc) {
+                                     const uint32_t* s_anc, const uint32_t* s_list, uint32_t cnt) {
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q);
     const __nv_bfloat16* k = static_cast<const __nv_bfloat16*>(a.keys) + w.sg.row_begin * a.krs + w.head * a.khs;
@@ -182,7 +187,9 @@ __device__ __noinline__ void by_rows(const CacheArgs& a, const Item& w, const ui
         float x[4] = {0, 0, 0, 0}, o[4] = {0, 0, 0, 0}, m = -INFINITY, l = 0.0f;
         if (mine)
             for (int e = 0; e < 4; ++e) x[e] = __bfloat162float(qr[c + e]);
-        for (uint32_t i = w.first_tile * KT; i < min(w.end_tile * KT, w.n); ++i) {
+        for (uint32_t j = 0; j < cnt * KT; ++j) {
+            const uint32_t i = (s_list[j / KT] >> 2) * KT + j % KT;
+            if (i >= w.n) continue;
             const bool drafted = a.tree && i >= w.ctx;
             const uint32_t kp = a.row_pos ? a.row_pos[w.entry + i] : drafted ? w.sg.base + w.ctx + s_depth[i - w.ctx] : w.sg.base + i;
             if (!w.sight.sees(s_qp[r], kp) || (a.row_doc && a.row_doc[w.entry + i] != s_qd[r])) continue;
@@ -230,12 +237,8 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
     w.n = a.rows ? min(a.rows[w.sg.seg], w.sg.n_rows) : w.sg.n_rows;
     w.ctx = w.n - min(w.n, w.sg.n_queries);
     w.q_rows = w.sg.n_queries * a.group;
-    w.row0 = (w.item - w.sg.item_begin) / w.sg.n_chunks * MB;
-    {
-        const uint32_t chunk = (w.item - w.sg.item_begin) % w.sg.n_chunks, tiles = (w.n + KT - 1) / KT;
-        w.first_tile = min(tiles, chunk * w.sg.chunk_tiles);
-        w.end_tile = min(tiles, w.first_tile + w.sg.chunk_tiles);
-    }
+    const uint32_t block = (w.item - w.sg.item_begin) / w.sg.n_chunks, chunk = (w.item - w.sg.item_begin) - block * w.sg.n_chunks, tiles = (w.n + KT - 1) / KT;
+    w.row0 = block * MB;
     w.sight = CacheSight{a.window_last, a.prefix ? a.prefix[w.sg.seg] : 0u, a.causal};
     const CacheSight sight = w.sight;
     w.entry = w.head * a.entry_hs + w.sg.row_begin;
@@ -244,7 +247,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
     const bool two = used > 128;
 
     uint32_t* s_meta = reinterpret_cast<uint32_t*>(sm + S::META_AT);
-    uint16_t* s_list = reinterpret_cast<uint16_t*>(sm + S::LIST_AT);
+    uint32_t* s_list = reinterpret_cast<uint32_t*>(sm + S::LIST_AT);
     unsigned char* s_cls = sm + S::CLS_AT;
     uint64_t* s_q = reinterpret_cast<uint64_t*>(sm + S::ROWS_AT);
     uint32_t* s_qp = reinterpret_cast<uint32_t*>(s_q + MB);
@@ -261,20 +264,65 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
     const auto bar = [&](int which) { return bars + which * 8; };
     const uint32_t tok0 = w.row0 / a.group;
 
-    if (tid == 0) {
-        for (int i = 0; i < 2; ++i) {
-            bar_init(bar(K_FULL + i), 1);
-            bar_init(bar(V_FULL + i), 1);
-            bar_init(bar(K_FREE + i), 1);
-            bar_init(bar(V_FREE + i), 1);
-            bar_init(bar(S_FULL + i), 1);
-            bar_init(bar(P_HALF + i), 128);
-            bar_init(bar(P_FULL + i), 128);
+    const bool arrays = has_pos || has_doc, drafts_listed = a.tree && (arrays || a.q_pos || sight.window_last != 0xFFFFFFFFu);  // drafted rows whose positions count
+    const bool plain = !arrays && !a.tree && !a.q_pos;  // all positions follow from the segment: the fetching warp finds the tiles alone
+    uint32_t cnt = 0;
+    if (warp == FETCH_WARP) {
+        if (lane == 0) {
+            for (int i = 0; i < 2; ++i) {
+                bar_init(bar(K_FULL + i), 1);
+                bar_init(bar(V_FULL + i), 1);
+                bar_init(bar(K_FREE + i), 1);
+                bar_init(bar(V_FREE + i), 1);
+                bar_init(bar(S_FULL + i), 1);
+                bar_init(bar(P_HALF + i), 128);
+                bar_init(bar(P_FULL + i), 128);
+            }
+            bar_init(bar(O_FULL), 1);
+            bar_init(bar(Q_FULL), 1);
+            for (int i = 0; i < 4; ++i) bar_init(bar(META_FULL + i), 1);
+            *s_odd = 0;
+            asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+            if (maps.q_boxes) {  // 32 query rows a box
+                const uint32_t boxes = two ? 8 : 4, step = 32 / a.group, t0 = w.sg.query_begin + tok0;
+                bar_expect(bar(Q_FULL), boxes * S::TILE / 4);
+                for (uint32_t i = 0; i < boxes; ++i)
+#pragma unroll
+                    for (int h = 0; h < S::HALVES; ++h)
+                        tma_load(sb + (i >> 2) * S::TILE + h * HALF + (i & 3) * 4096, &maps.q, h * 64, w.head * a.group, t0 + i * step, bar(Q_FULL));
+            }
         }
-        bar_init(bar(O_FULL), 1);
-        for (int i = 0; i < 4; ++i) bar_init(bar(META_FULL + i), 1);
-        *s_odd = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+        __syncwarp();
+    }
+    if (plain) {
+        // Which tiles are visited, and which of them either tile of query rows sees as a whole.  Of a split segment the item takes its share of them.  Every warp goes through
+        // them, so that each knows how many there are; the fetching one writes the list.
+        const uint32_t p0 = w.sg.base + w.ctx, last_tok = w.sg.n_queries - 1;
+        const auto pos = [&](uint32_t row) { return p0 + min(row / a.group, last_tok); };
+        const CacheRanges qa{pos(w.row0), pos(w.row0 + 127), 0u, 0u}, qb{pos(w.row0 + 128), pos(w.row0 + 255), 0u, 0u};
+        const auto class_of = [&](uint32_t j) -> uint32_t {
+            const uint32_t first = j * KT, last = first + KT - 1;
+            if (j >= tiles) return 0u;
+            const CacheRanges k{w.sg.base + first, w.sg.base + min(last, w.n - 1), 0u, 0u};
+            const int x = cache_tile_class(k, qa, sight, false, last < w.n), y = cache_tile_class(k, qb, sight, false, last < w.n);
+            return (x || y ? 1u : 0u) | (x == 2 ? 2u : 0u) | (y == 2 ? 4u : 0u);
+        };
+        uint32_t skip = 0, most = RUN_MOST;
+        if (w.sg.n_chunks > 1) {
+            uint32_t visited = 0;
+            for (uint32_t j0 = 0; j0 < tiles; j0 += 32) visited += __popc(__ballot_sync(0xFFFFFFFFu, class_of(j0 + lane) != 0));
+            skip = (uint32_t)((uint64_t)visited * chunk / w.sg.n_chunks);
+            most = (uint32_t)((uint64_t)visited * (chunk + 1) / w.sg.n_chunks) - skip;
+        }
+        uint32_t met = 0;
+        for (uint32_t j0 = 0; j0 < tiles && met < skip + most; j0 += 32) {
+            const uint32_t cls = class_of(j0 + lane), mask = __ballot_sync(0xFFFFFFFFu, cls != 0), at = met + __popc(mask & ((1u << lane) - 1u));
+            if (warp == FETCH_WARP && cls && at >= skip && at < skip + most) s_list[at - skip] = (j0 + lane) << 2 | cls >> 1;
+            met += __popc(mask);
+        }
+        cnt = met > skip ? min(met - skip, most) : 0u;
+        __syncwarp();
     }
     if (warp == MMA_WARP) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(bar(TMEM_WORD)), "r"(512u) : "memory");
@@ -308,87 +356,119 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
         s_slope[r] = has_slope ? a.slopes[h] * LOG2E : 0.0f;
         s_tok[r] = tok - tok0;
     }
-    __syncthreads();
-    for (int i = tid; i < (two ? MB : 128) * S::HALVES * 8; i += THREADS) {
-        const uint32_t r = i / (S::HALVES * 8), c = i % (S::HALVES * 8);
-        const bool there = r < used && c * 8 < a.d;
-        copy16(sb + (r >> 7) * S::TILE + (c >> 3) * HALF + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4), static_cast<const unsigned char*>(a.q) + (there ? s_q[r] + c * 16 : 0), there);
-    }
-    copy_commit();
-    if (warp < 2) {  // positions and documents of either tile of query rows
-        CacheRanges q{0xFFFFFFFFu, 0u, 0xFFFFFFFFu, 0u};
-        for (int r = warp * 128 + lane; r < warp * 128 + 128; r += 32) {
-            q.pmin = min(q.pmin, s_qp[r]);
-            q.pmax = max(q.pmax, s_qp[r]);
-            q.dmin = min(q.dmin, s_qd[r]);
-            q.dmax = max(q.dmax, s_qd[r]);
+    if (!maps.q_boxes) {
+        __syncthreads();
+        for (int i = tid; i < (two ? MB : 128) * S::HALVES * 8; i += THREADS) {
+            const uint32_t r = i / (S::HALVES * 8), c = i % (S::HALVES * 8);
+            const bool there = r < used && c * 8 < a.d;
+            copy16(sb + (r >> 7) * S::TILE + (c >> 3) * HALF + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4), static_cast<const unsigned char*>(a.q) + (there ? s_q[r] + c * 16 : 0), there);
         }
-        q.pmin = __reduce_min_sync(0xFFFFFFFFu, q.pmin);
-        q.pmax = __reduce_max_sync(0xFFFFFFFFu, q.pmax);
-        q.dmin = __reduce_min_sync(0xFFFFFFFFu, q.dmin);
-        q.dmax = __reduce_max_sync(0xFFFFFFFFu, q.dmax);
-        if (lane == 0) s_range[warp * 4] = q.pmin, s_range[warp * 4 + 1] = q.pmax, s_range[warp * 4 + 2] = q.dmin, s_range[warp * 4 + 3] = q.dmax;
+        copy_commit();
+        copy_wait<0>();
+        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");  // (the queries, read by the products)
     }
-    __syncthreads();
-    const uint32_t in_run = w.end_tile - w.first_tile;
-    {   // which tiles are visited, and which of them either tile of query rows sees as a whole
-        const CacheRanges qa{s_range[0], s_range[1], s_range[2], s_range[3]}, qb{s_range[4], s_range[5], s_range[6], s_range[7]};
-        const auto classes = [&](const CacheRanges& k, uint32_t last) {
-            const bool drafts = a.tree && last >= w.ctx, inside = last < w.n;
-            const int x = cache_tile_class(k, qa, w.sight, drafts, inside), y = cache_tile_class(k, qb, w.sight, drafts, inside);
-            return (x || y ? 1 : 0) | (x == 2 ? 2 : 0) | (y == 2 ? 4 : 0);
-        };
-        if (has_pos || has_doc) {
-            constexpr int AT_ONCE = 3;  // tiles whose loads a warp has under way
-            for (uint32_t j0 = warp; j0 < in_run; j0 += WARPS * AT_ONCE) {
-                CacheRanges k[AT_ONCE];
+    if (!plain) {
+        // the same, from the arrays: all warps look, a tile each at a time
+        const uint32_t first_tile = min(tiles, chunk * w.sg.chunk_tiles), in_run = min(tiles - first_tile, w.sg.chunk_tiles);
+        __syncthreads();
+        if (warp < 2) {  // positions and documents of either tile of query rows
+            CacheRanges q{0xFFFFFFFFu, 0u, 0xFFFFFFFFu, 0u};
+            for (int r = warp * 128 + lane; r < warp * 128 + 128; r += 32) {
+                q.pmin = min(q.pmin, s_qp[r]);
+                q.pmax = max(q.pmax, s_qp[r]);
+                q.dmin = min(q.dmin, s_qd[r]);
+                q.dmax = max(q.dmax, s_qd[r]);
+            }
+            q.pmin = __reduce_min_sync(0xFFFFFFFFu, q.pmin);
+            q.pmax = __reduce_max_sync(0xFFFFFFFFu, q.pmax);
+            q.dmin = __reduce_min_sync(0xFFFFFFFFu, q.dmin);
+            q.dmax = __reduce_max_sync(0xFFFFFFFFu, q.dmax);
+            if (lane == 0) s_range[warp * 4] = q.pmin, s_range[warp * 4 + 1] = q.pmax, s_range[warp * 4 + 2] = q.dmin, s_range[warp * 4 + 3] = q.dmax;
+        }
+        __syncthreads();
+        {   // which tiles are visited, and which of them either tile of query rows sees as a whole
+            const CacheRanges qa{s_range[0], s_range[1], s_range[2], s_range[3]}, qb{s_range[4], s_range[5], s_range[6], s_range[7]};
+            const auto classes = [&](const CacheRanges& k, uint32_t last) {
+                const bool drafts = a.tree && last >= w.ctx, inside = last < w.n;
+                const int x = cache_tile_class(k, qa, w.sight, drafts, inside), y = cache_tile_class(k, qb, w.sight, drafts, inside);
+                return (x || y ? 1 : 0) | (x == 2 ? 2 : 0) | (y == 2 ? 4 : 0);
+            };
+            if (has_pos || has_doc) {
+                constexpr int AT_ONCE = 3;  // tiles whose loads a warp has under way
+                for (uint32_t j0 = warp; j0 < in_run; j0 += WARPS * AT_ONCE) {
+                    CacheRanges k[AT_ONCE];
 #pragma unroll
-                for (int x = 0; x < AT_ONCE; ++x) {
-                    const uint32_t first = (w.first_tile + min(j0 + x * WARPS, in_run - 1)) * KT;
-                    k[x] = CacheRanges{0xFFFFFFFFu, 0u, has_doc ? 0xFFFFFFFFu : 0u, 0u};
+                    for (int x = 0; x < AT_ONCE; ++x) {
+                        const uint32_t first = (first_tile + min(j0 + x * WARPS, in_run - 1)) * KT;
+                        k[x] = CacheRanges{0xFFFFFFFFu, 0u, has_doc ? 0xFFFFFFFFu : 0u, 0u};
 #pragma unroll
-                    for (int e = 0; e < KT / 32; ++e) {
-                        const uint32_t i = min(first + lane + e * 32, w.n - 1);
-                        const uint32_t p = has_pos ? a.row_pos[w.entry + i] : w.sg.base + i, d = has_doc ? a.row_doc[w.entry + i] : 0u;
-                        k[x].pmin = min(k[x].pmin, p);
-                        k[x].pmax = max(k[x].pmax, p);
-                        k[x].dmin = min(k[x].dmin, d);
-                        k[x].dmax = max(k[x].dmax, d);
+                        for (int e = 0; e < KT / 32; ++e) {
+                            const uint32_t i = min(first + lane + e * 32, w.n - 1);
+                            const uint32_t p = has_pos ? a.row_pos[w.entry + i] : w.sg.base + i, d = has_doc ? a.row_doc[w.entry + i] : 0u;
+                            k[x].pmin = min(k[x].pmin, p);
+                            k[x].pmax = max(k[x].pmax, p);
+                            k[x].dmin = min(k[x].dmin, d);
+                            k[x].dmax = max(k[x].dmax, d);
+                        }
+                    }
+#pragma unroll
+                    for (int x = 0; x < AT_ONCE; ++x) {
+                        const uint32_t j = j0 + x * WARPS;
+                        k[x].pmin = __reduce_min_sync(0xFFFFFFFFu, k[x].pmin);
+                        k[x].pmax = __reduce_max_sync(0xFFFFFFFFu, k[x].pmax);
+                        k[x].dmin = __reduce_min_sync(0xFFFFFFFFu, k[x].dmin);
+                        k[x].dmax = __reduce_max_sync(0xFFFFFFFFu, k[x].dmax);
+                        if (lane == 0 && j < in_run) s_cls[j] = (unsigned char)classes(k[x], (first_tile + j) * KT + KT - 1);
                     }
                 }
-#pragma unroll
-                for (int x = 0; x < AT_ONCE; ++x) {
-                    const uint32_t j = j0 + x * WARPS;
-                    k[x].pmin = __reduce_min_sync(0xFFFFFFFFu, k[x].pmin);
-                    k[x].pmax = __reduce_max_sync(0xFFFFFFFFu, k[x].pmax);
-                    k[x].dmin = __reduce_min_sync(0xFFFFFFFFu, k[x].dmin);
-                    k[x].dmax = __reduce_max_sync(0xFFFFFFFFu, k[x].dmax);
-                    if (lane == 0 && j < in_run) s_cls[j] = (unsigned char)classes(k[x], (w.first_tile + j) * KT + KT - 1);
+            } else {
+                for (uint32_t j = tid; j < in_run; j += THREADS) {
+                    const uint32_t first = (first_tile + j) * KT, last = first + KT - 1;
+                    s_cls[j] = (unsigned char)classes(CacheRanges{w.sg.base + first, w.sg.base + min(last, w.n - 1), 0u, 0u}, last);
                 }
             }
-        } else {
-            for (uint32_t j = tid; j < in_run; j += THREADS) {
-                const uint32_t first = (w.first_tile + j) * KT, last = first + KT - 1;
-                s_cls[j] = (unsigned char)classes(CacheRanges{w.sg.base + first, w.sg.base + min(last, w.n - 1), 0u, 0u}, last);
-            }
+        }
+        __syncthreads();
+        for (uint32_t j0 = 0; j0 < in_run; j0 += 32) {  // (every warp counts, the first one writes)
+            const int cls = j0 + lane < in_run ? s_cls[j0 + lane] : 0;
+            const uint32_t mask = __ballot_sync(0xFFFFFFFFu, cls != 0);
+            if (warp == 0 && cls) s_list[cnt + __popc(mask & ((1u << lane) - 1u))] = (first_tile + j0 + lane) << 2 | cls >> 1;
+            cnt += __popc(mask);
         }
     }
-    copy_wait<0>();
-    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");  // (the queries, read by the products)
-    __syncthreads();
-    uint32_t cnt = 0;
-    for (uint32_t j0 = 0; j0 < in_run; j0 += 32) {  // (every warp counts, the first one writes)
-        const int cls = j0 + lane < in_run ? s_cls[j0 + lane] : 0;
-        const uint32_t mask = __ballot_sync(0xFFFFFFFFu, cls != 0);
-        if (warp == 0 && cls) s_list[cnt + __popc(mask & ((1u << lane) - 1u))] = (uint16_t)((j0 + lane) << 2 | cls >> 1);
-        cnt += __popc(mask);
+    const unsigned char* kb = static_cast<const unsigned char*>(a.keys) + (w.sg.row_begin * a.krs + w.head * a.khs) * 2;
+    const unsigned char* vb = static_cast<const unsigned char*>(a.values) + (w.sg.row_begin * a.vrs + w.head * a.vhs) * 2;
+    constexpr int PIECES = S::HALVES * 8;
+    const auto fetch = [&](uint32_t dst, const CUtensorMap* map, bool head_first, const unsigned char* from, uint64_t stride, uint32_t first, uint32_t full) {
+        if (first + KT <= w.n) {
+            if (lane == 0) {
+                const uint32_t row = (uint32_t)w.sg.row_begin + first;
+                bar_expect(full, S::TILE);
+#pragma unroll
+                for (int h = 0; h < S::HALVES; ++h) tma_load(dst + h * HALF, map, h * 64, head_first ? w.head : row, head_first ? row : w.head, full);
+            }
+        } else {
+            for (uint32_t i = lane; i < KT * PIECES; i += 32) {
+                const uint32_t r = i / PIECES, c = i % PIECES, row = first + r;
+                const bool there = row < w.n && c * 8 < a.d;
+                copy16(dst + (c >> 3) * HALF + r * 128 + (((c & 7) ^ (r & 7)) << 4), there ? from + row * stride * 2 + c * 16 : from, there);
+            }
+            copy_commit();
+            copy_wait<0>();
+            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+            __syncwarp();
+            if (lane == 0) bar_arrive(full);
+        }
+    };
+    if (warp == FETCH_WARP && plain && cnt) {  // the first keys, while the others get ready
+        __syncwarp();
+        fetch(sb + S::K_AT, &maps.k, maps.k_head_first, kb, a.krs, (s_list[0] >> 2) * KT, bar(K_FULL));
     }
     tc_before();
     __syncthreads();
     tc_after();
-    const uint32_t tmem = *s_tmem;
-    const bool arrays = has_pos || has_doc, drafts_listed = a.tree && (arrays || a.q_pos || sight.window_last != 0xFFFFFFFFu);  // drafted rows whose positions count
-    const uint32_t near_pos = s_qp[0];  // distances are taken from here, so that those of rows nearby are exact in float32
+    const uint32_t tmem = *s_tmem;  // (read by all warps alike: with a value of its own for one of them, the compiler issued each product in a loop over the lanes)
+    const uint32_t near_pos = plain ? w.sg.base + w.ctx + tok0 : s_qp[0];  // distances are taken from here, so that those of rows nearby are exact in float32
     bool fail = false;
 
     if (warp < 8) {
@@ -398,7 +478,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
         if (t == 0 || two) {
             const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21), ts = lanes + t * 128, to = lanes + 256 + t * 128;
             const float to_log2 = has_cap ? a.scale / a.cap : a.scale * LOG2E, cap2 = a.cap * LOG2E;
-            const uint32_t qp = s_qp[r], qd = s_qd[r], n = w.n, ctx = w.ctx, base = w.sg.base, first_tile = w.first_tile;
+            const uint32_t qp = s_qp[r], qd = s_qd[r], n = w.n, ctx = w.ctx, base = w.sg.base;
             const float slope = s_slope[r], q_at = (float)((long long)qp - (long long)near_pos);
             const uint32_t* anc = s_anc + s_tok[r] * (TREE_MOST / 32);
             float m = -INFINITY, l = 0.0f;
@@ -408,7 +488,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
                     break;
                 }
                 tc_after();
-                const uint32_t what = s_list[li], first = (first_tile + (what >> 2)) * KT;
+                const uint32_t what = s_list[li], first = (what >> 2) * KT;
                 const bool all = what >> t & 1;
                 uint32_t u[128];
                 float* s = reinterpret_cast<float*>(u);
@@ -512,12 +592,15 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
                         fail = true;
                         break;
                     }
-                    bool odd = false;
+                    // (where both tiles of query rows see a part of it, each looks at a half)
+                    const bool share = two && !(what & 3u);
+                    uint32_t odd = 0;
 #pragma unroll 4
-                    for (uint32_t i = tid & 127; i < S::TILE / 16; i += 128) {
+                    for (uint32_t i = share ? tid : tid & 127; i < S::TILE / 16; i += share ? 256 : 128) {
                         const uint4 x = *reinterpret_cast<const uint4*>(sm + S::V_AT + (li & 1) * S::TILE + i * 16);
-                        odd |= odd_pair(x.x) || odd_pair(x.y) || odd_pair(x.z) || odd_pair(x.w);
+                        odd |= odd_pair(x.x) | odd_pair(x.y) | odd_pair(x.z) | odd_pair(x.w);
                     }
+                    odd &= 0x80008000u;
                     if (odd) *s_odd = 1u;
                     __syncwarp();
                 }
@@ -553,8 +636,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
                         float x, y;
-                        const uint64_t z = fma2(pair(s[c + e], s[c + e + 1]), mul_2, use_2);
-                        unpair(z, x, y);
+                        unpair(fma2(pair(s[c + e], s[c + e + 1]), mul_2, use_2), x, y);
                         x = exp2_fast(x);
                         y = exp2_fast(y);
                         if (e & 2) sum_a = add2(sum_a, pair(x, y));
@@ -589,9 +671,36 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
             const uint64_t mine = whole ? (uint64_t)a.out + ((uint64_t)(w.sg.query_begin + tok) * a.ots + (uint64_t)q_head * a.ohs) * 2 : (uint64_t)(a.part_o + part * a.d);
             const float inv = !cnt || l == 0.0f ? 0.0f : whole ? 1.0f / l : 1.0f;
             constexpr int LINE = D * 2, LINE_PIECES = LINE / 16;  // bytes of a row at a time: all of its bfloat16 elements, or half of its float32 ones
-            unsigned char* stage = sm + t * S::TILE + (warp & 3) * 32 * LINE;
+            unsigned char* const stage = sm + t * S::TILE + (warp & 3) * 4096;  // 32 lines of 128 bytes in either half, as the boxes have them
+            const auto piece = [&](int row, int c) { return reinterpret_cast<uint4*>(stage + (c >> 3) * HALF + row * 128 + (((c & 7) ^ (row & 7)) << 4)); };
+            const bool boxed = whole && maps.out_boxes && (uint32_t)(warp + 1) * 32 <= used;  // all 32 rows of the warp at once
+            if (boxed) {
+                __syncwarp();
+#pragma unroll
+                for (int c = 0; c < D / 16; ++c) {
+                    uint32_t o[16];
+                    tmem_ld16(to + c * 16, o);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[e] = inv != 0.0f ? __float_as_uint(__uint_as_float(o[e]) * inv) : 0u;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t x[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[e] = pack_bf16(__uint_as_float(o[8 * h + 2 * e]), __uint_as_float(o[8 * h + 2 * e + 1]));
+                        *piece(lane, c * 2 + h) = make_uint4(x[0], x[1], x[2], x[3]);
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                __syncwarp();
+                if (lane == 0) {
+#pragma unroll
+                    for (int h = 0; h < S::HALVES; ++h)
+                        tma_store(&maps.out, sb + t * S::TILE + h * HALF + (warp & 3) * 4096, h * 64, w.head * a.group, w.sg.query_begin + tok0 + warp * (32 / a.group));
+                    asm volatile("cp.async.bulk.commit_group;\ncp.async.bulk.wait_group 0;\n" ::: "memory");
+                }
+            }
             __syncwarp();
-            for (int pass = 0; pass < (whole ? 1 : 2); ++pass) {
+            for (int pass = 0; pass < (boxed ? 0 : whole ? 1 : 2); ++pass) {
 #pragma unroll
                 for (int c = 0; c < D / 16; ++c) {
                     if (!whole && c >= D / 32) break;
@@ -605,12 +714,12 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
                             uint32_t x[4];
 #pragma unroll
                             for (int e = 0; e < 4; ++e) x[e] = pack_bf16(__uint_as_float(o[8 * h + 2 * e]), __uint_as_float(o[8 * h + 2 * e + 1]));
-                            *reinterpret_cast<uint4*>(stage + lane * LINE + (((c * 2 + h) ^ (lane & 7)) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
+                            *piece(lane, c * 2 + h) = make_uint4(x[0], x[1], x[2], x[3]);
                         }
                     } else {
 #pragma unroll
                         for (int h = 0; h < 4; ++h)
-                            *reinterpret_cast<uint4*>(stage + lane * LINE + (((c * 4 + h) ^ (lane & 7)) << 4)) = make_uint4(o[4 * h], o[4 * h + 1], o[4 * h + 2], o[4 * h + 3]);
+                            *piece(lane, c * 4 + h) = make_uint4(o[4 * h], o[4 * h + 1], o[4 * h + 2], o[4 * h + 3]);
                     }
                 }
                 __syncwarp();
@@ -618,7 +727,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
                 for (int i = lane; i < 32 * LINE_PIECES; i += 32) {
                     const int row = i / LINE_PIECES, c = i % LINE_PIECES;
                     const uint64_t dst = __shfl_sync(0xFFFFFFFFu, mine, row);
-                    const uint4 x = *reinterpret_cast<const uint4*>(stage + row * LINE + ((c ^ (row & 7)) << 4));
+                    const uint4 x = *piece(row, c);
                     const uint32_t col = whole ? c * 8 : pass * (D / 2) + c * 4;
                     if ((warp * 32 + row) < (int)used && col < a.d) *reinterpret_cast<uint4*>(dst + col * (whole ? 2 : 4)) = x;
                 }
@@ -661,7 +770,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
                 }
                 return true;
             };
-            fail = !bar_wait(bar(K_FULL), 0);
+            fail = (maps.q_boxes && !bar_wait(bar(Q_FULL), 0)) || !bar_wait(bar(K_FULL), 0);
             if (!fail) {
                 scores(0, 0);
                 if (two) scores(0, 1);
@@ -695,37 +804,13 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
         __syncwarp();
         } else if (warp == FETCH_WARP) {
         // ---- rows into shared memory
-        const unsigned char* kb = static_cast<const unsigned char*>(a.keys) + (w.sg.row_begin * a.krs + w.head * a.khs) * 2;
-        const unsigned char* vb = static_cast<const unsigned char*>(a.values) + (w.sg.row_begin * a.vrs + w.head * a.vhs) * 2;
-        constexpr int PIECES = S::HALVES * 8;
-        const auto fetch = [&](uint32_t dst, const CUtensorMap* map, bool head_first, const unsigned char* from, uint64_t stride, uint32_t first, uint32_t full) {
-            if (first + KT <= w.n) {
-                if (lane == 0) {
-                    const uint32_t row = (uint32_t)w.sg.row_begin + first;
-                    bar_expect(full, S::TILE);
-#pragma unroll
-                    for (int h = 0; h < S::HALVES; ++h) tma_load(dst + h * HALF, map, h * 64, head_first ? w.head : row, head_first ? row : w.head, full);
-                }
-            } else {
-                for (uint32_t i = lane; i < KT * PIECES; i += 32) {
-                    const uint32_t r = i / PIECES, c = i % PIECES, row = first + r;
-                    const bool there = row < w.n && c * 8 < a.d;
-                    copy16(dst + (c >> 3) * HALF + r * 128 + (((c & 7) ^ (r & 7)) << 4), there ? from + row * stride * 2 + c * 16 : from, there);
-                }
-                copy_commit();
-                copy_wait<0>();
-                asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-                __syncwarp();
-                if (lane == 0) bar_arrive(full);
-            }
-        };
         for (uint32_t li = 0; li < cnt; ++li) {
-            const uint32_t slot = li & 1, what = s_list[li], first = (w.first_tile + (what >> 2)) * KT;
+            const uint32_t slot = li & 1, what = s_list[li], first = (what >> 2) * KT;
             if (li >= 2 && !__all_sync(0xFFFFFFFFu, bar_wait(bar(K_FREE + slot), (li >> 1) - 1 & 1))) {
                 fail = true;
                 break;
             }
-            fetch(sb + S::K_AT + slot * S::TILE, &maps.k, maps.k_head_first, kb, a.krs, first, bar(K_FULL + slot));
+            if (!plain || li > 0) fetch(sb + S::K_AT + slot * S::TILE, &maps.k, maps.k_head_first, kb, a.krs, first, bar(K_FULL + slot));
             // (the tile four before this one has been turned into weights: its positions are no longer read)
             const bool whole = (what & (two ? 3u : 1u)) == (two ? 3u : 1u);
             if (has_slope || (!whole && (arrays || (drafts_listed && first + KT > w.ctx)))) {
@@ -756,29 +841,45 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
     if (warp == MMA_WARP) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512u) : "memory");
     if (*s_odd) {
         const Item again = w;
-        by_rows(a, again, s_qp, s_qd, s_slope, s_tok, s_depth, s_anc);
+        by_rows(a, again, s_qp, s_qd, s_slope, s_tok, s_depth, s_anc, s_list, cnt);
     }
 }
 
-// A map of rows x KV heads x elements in boxes of 128 rows of one KV head x 64 elements; false where the driver does not take the layout.
-bool wide_map(CUtensorMap* map, const void* base, uint64_t row_stride, uint64_t head_stride, uint64_t rows, uint32_t heads, uint32_t d, uint32_t* head_first) {
-    using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+using WideEncode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
                                 CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-    static const Encode encode = []() -> Encode {
+WideEncode wide_encode() {
+    static const WideEncode encode = []() -> WideEncode {
         void* p = nullptr;
         cudaDriverEntryPointQueryResult found;
         if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) {
             cudaGetLastError();
             return nullptr;
         }
-        return reinterpret_cast<Encode>(p);
+        return reinterpret_cast<WideEncode>(p);
     }();
+    return encode;
+}
+// A map of rows x KV heads x elements in boxes of 128 rows of one KV head x 64 elements; false where the driver does not take the layout.
+bool wide_map(CUtensorMap* map, const void* base, uint64_t row_stride, uint64_t head_stride, uint64_t rows, uint32_t heads, uint32_t d, uint32_t* head_first) {
+    const WideEncode encode = wide_encode();
     if (!encode || rows > 0x7FFFFFFFull) return false;
     if (heads == 1) head_stride = row_stride * rows;  // (never stepped by)
     *head_first = head_stride < row_stride;
     const cuuint64_t dims[3] = {d, *head_first ? heads : rows, *head_first ? rows : heads};
     const cuuint64_t strides[2] = {(*head_first ? head_stride : row_stride) * 2, (*head_first ? row_stride : head_stride) * 2};
     const cuuint32_t box[3] = {64, *head_first ? 1u : (cuuint32_t)KT, *head_first ? (cuuint32_t)KT : 1u}, each[3] = {1, 1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Queries or outputs in boxes of 32 rows of a KV head (32 / group tokens of its group); false where the layout or the group does not allow it.
+bool wide_row_map(CUtensorMap* map, const void* base, uint64_t token_stride, uint64_t head_stride, const CacheArgs& a) {
+    if (32 % a.group || (a.n_heads > 1 && head_stride >= token_stride)) return false;
+    const WideEncode encode = wide_encode();
+    if (!encode) return false;
+    if (a.n_heads == 1) head_stride = token_stride;  // (never stepped by)
+    const cuuint64_t dims[3] = {a.d, a.n_heads, a.n_tokens}, strides[2] = {head_stride * 2, token_stride * 2};
+    const cuuint32_t box[3] = {64, a.group, 32 / a.group}, each[3] = {1, 1, 1};
     return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -814,6 +915,8 @@ Status launch_attend_wide(Ctx* c, CacheArgs a, CacheWork w, bool* taken) {
     *taken = wide_map(&maps.k, a.keys, a.krs, a.khs, std::max<uint64_t>(rows, 1), a.n_kv, a.d, &maps.k_head_first) &&
              wide_map(&maps.v, a.values, a.vrs, a.vhs, std::max<uint64_t>(rows, 1), a.n_kv, a.d, &maps.v_head_first);
     if (!*taken) return Status();
+    maps.q_boxes = wide_row_map(&maps.q, a.q, a.qts, a.qhs, a);
+    maps.out_boxes = wide_row_map(&maps.out, a.out, a.ots, a.ohs, a);
     return a.d <= 64 ? launch_wide<64>(c, a, std::move(w), maps) : launch_wide<128>(c, a, std::move(w), maps);
 }
 
