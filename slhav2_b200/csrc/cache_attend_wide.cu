@@ -12,6 +12,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "cache.cuh"
 #include "cache_mma.cuh"
@@ -111,6 +112,15 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     uint64_t r;
     asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
     return r;
+}
+// tanh_small's polynomial at v = x^2
+__device__ __forceinline__ uint64_t tanh_poly(uint64_t v) {
+    uint64_t p = fma2(v, pair(TANH_6, TANH_6), pair(TANH_5, TANH_5));
+    p = fma2(v, p, pair(TANH_4, TANH_4));
+    p = fma2(v, p, pair(TANH_3, TANH_3));
+    p = fma2(v, p, pair(TANH_2, TANH_2));
+    p = fma2(v, p, pair(TANH_1, TANH_1));
+    return fma2(v, p, pair(TANH_0, TANH_0));
 }
 // the low x bits of a word
 __device__ __forceinline__ uint32_t low_bits(int x) { return x <= 0 ? 0u : x >= 32 ? 0xFFFFFFFFu : (1u << x) - 1u; }
@@ -219,7 +229,9 @@ __device__ __noinline__ void by_rows(const CacheArgs& a, const Item& w, const ui
     }
 }
 
-template <int D>
+// CAP: scores are capped.  RICH: rows with positions or documents of their own, tokens with positions of their own, trees, or a distance bias.  (Instances of their own: what a
+// kernel does not need costs it registers and instruction cache in the loop over the tiles; with all in one, 8192 tokens of 32 heads took 937 us, alone 876.)
+template <int D, bool CAP, bool RICH>
 __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __grid_constant__ CacheArgs a, const __grid_constant__ WideMaps maps, const __grid_constant__ CacheTable tab) {
     using S = Wide<D>;
     dep_wait();
@@ -238,11 +250,16 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
     w.ctx = w.n - min(w.n, w.sg.n_queries);
     w.q_rows = w.sg.n_queries * a.group;
     const uint32_t block = (w.item - w.sg.item_begin) / w.sg.n_chunks, chunk = (w.item - w.sg.item_begin) - block * w.sg.n_chunks, tiles = (w.n + KT - 1) / KT;
-    w.row0 = block * MB;
+    {   // (the last blocks first: under a causal mask they see most)
+        const uint32_t turned = (w.q_rows + MB - 1) / MB - 1 - block;
+        w.row0 = turned * MB;
+        w.item = w.sg.item_begin + turned * w.sg.n_chunks + chunk;  // (where the parts of its rows go)
+    }
     w.sight = CacheSight{a.window_last, a.prefix ? a.prefix[w.sg.seg] : 0u, a.causal};
     const CacheSight sight = w.sight;
     w.entry = w.head * a.entry_hs + w.sg.row_begin;
-    const bool has_pos = a.row_pos, has_doc = a.row_doc, has_slope = a.slopes, has_cap = a.cap > 0.0f;
+    const bool has_pos = RICH && a.row_pos, has_doc = RICH && a.row_doc, has_slope = RICH && a.slopes, is_tree = RICH && a.tree;
+    constexpr bool has_cap = CAP;
     const uint32_t used = min((uint32_t)MB, w.q_rows - w.row0);
     const bool two = used > 128;
 
@@ -264,8 +281,8 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
     const auto bar = [&](int which) { return bars + which * 8; };
     const uint32_t tok0 = w.row0 / a.group;
 
-    const bool arrays = has_pos || has_doc, drafts_listed = a.tree && (arrays || a.q_pos || sight.window_last != 0xFFFFFFFFu);  // drafted rows whose positions count
-    const bool plain = !arrays && !a.tree && !a.q_pos;  // all positions follow from the segment: the fetching warp finds the tiles alone
+    const bool arrays = has_pos || has_doc, drafts_listed = is_tree && (arrays || a.q_pos || sight.window_last != 0xFFFFFFFFu);  // drafted rows whose positions count
+    const bool plain = !RICH || (!arrays && !is_tree && !a.q_pos);  // all positions follow from the segment: the fetching warp finds the tiles alone
     uint32_t cnt = 0;
     if (warp == FETCH_WARP) {
         if (lane == 0) {
@@ -328,7 +345,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(bar(TMEM_WORD)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
     }
-    if (a.tree) {
+    if (is_tree) {
         for (uint32_t j = tid; j < w.sg.n_queries; j += THREADS) {
             const uint32_t p = a.parents[w.sg.query_begin + j];
             s_par[j] = p < j ? p : 0xFFFFFFFFu;
@@ -351,7 +368,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
     for (uint32_t r = tid; r < MB; r += THREADS) {  // (rows behind the last repeat it, and are zeros among the queries)
         const uint32_t row = min(w.row0 + r, w.q_rows - 1), tok = row / a.group, h = w.head * a.group + row - tok * a.group;
         s_q[r] = ((uint64_t)(w.sg.query_begin + tok) * a.qts + (uint64_t)h * a.qhs) * 2;
-        s_qp[r] = a.q_pos ? a.q_pos[w.sg.query_begin + tok] : w.sg.base + w.ctx + (a.tree ? s_depth[tok] : tok);
+        s_qp[r] = a.q_pos ? a.q_pos[w.sg.query_begin + tok] : w.sg.base + w.ctx + (is_tree ? s_depth[tok] : tok);
         s_qd[r] = has_doc ? a.q_doc[w.sg.query_begin + tok] : 0u;
         s_slope[r] = has_slope ? a.slopes[h] * LOG2E : 0.0f;
         s_tok[r] = tok - tok0;
@@ -389,7 +406,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
         {   // which tiles are visited, and which of them either tile of query rows sees as a whole
             const CacheRanges qa{s_range[0], s_range[1], s_range[2], s_range[3]}, qb{s_range[4], s_range[5], s_range[6], s_range[7]};
             const auto classes = [&](const CacheRanges& k, uint32_t last) {
-                const bool drafts = a.tree && last >= w.ctx, inside = last < w.n;
+                const bool drafts = is_tree && last >= w.ctx, inside = last < w.n;
                 const int x = cache_tile_class(k, qa, w.sight, drafts, inside), y = cache_tile_class(k, qb, w.sight, drafts, inside);
                 return (x || y ? 1 : 0) | (x == 2 ? 2 : 0) | (y == 2 ? 4 : 0);
             };
@@ -498,29 +515,34 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
 #pragma unroll
                 for (int c = 0; c < 128; ++c) asm volatile("" : "+r"(u[c]));
                 float mul = to_log2, top;
+                bool fused = false;  // the cap is applied on the way to the weights
                 if (has_cap) {
-                    mul = 1.0f;
-                    float big = 0.0f;
+                    float high[2] = {-INFINITY, -INFINITY}, low[2] = {INFINITY, INFINITY};
 #pragma unroll
-                    for (int c = 0; c < 128; ++c) big = fmaxf(big, fabsf(s[c]));
-                    if (__any_sync(0xFFFFFFFFu, !(big * to_log2 <= 1.0f))) {
+                    for (int c = 0; c < 128; c += 4)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            high[e] = fmaxf(high[e], fmaxf(s[c + 2 * e], s[c + 2 * e + 1]));
+                            low[e] = fminf(low[e], fminf(s[c + 2 * e], s[c + 2 * e + 1]));
+                        }
+                    const float x = fmaxf(high[0], high[1]) * to_log2;
+                    const bool small = __all_sync(0xFFFFFFFFu, x <= 1.0f && fminf(low[0], low[1]) * to_log2 >= -1.0f);
+                    fused = small && all && !has_slope;
+                    mul = 1.0f;
+                    if (fused) {  // (tanh grows: the largest score is that of the largest product)
+                        top = cap2 * tanh_small(x);
+                    } else if (small) {
+                        const uint64_t in = pair(to_log2, to_log2), out = pair(cap2, cap2);
+#pragma unroll
+                        for (int c = 0; c < 128; c += 2) {
+                            const uint64_t y = mul2(pair(s[c], s[c + 1]), in);
+                            unpair(mul2(mul2(y, out), tanh_poly(mul2(y, y))), s[c], s[c + 1]);
+                        }
+                    } else {
 #pragma unroll
                         for (int c = 0; c < 128; ++c) {  // tanh x = 1 - 2 / (exp(2 x) + 1)
                             const float e = exp2_fast(s[c] * to_log2 * (2.0f * LOG2E));
                             s[c] = fmaf(-2.0f * cap2, __fdividef(1.0f, e + 1.0f), cap2);
-                        }
-                    } else {  // tanh_small, two at a time
-                        const uint64_t in = pair(to_log2, to_log2), out = pair(cap2, cap2);
-#pragma unroll
-                        for (int c = 0; c < 128; c += 2) {
-                            const uint64_t x = mul2(pair(s[c], s[c + 1]), in), v = mul2(x, x);
-                            uint64_t p = fma2(v, pair(TANH_6, TANH_6), pair(TANH_5, TANH_5));
-                            p = fma2(v, p, pair(TANH_4, TANH_4));
-                            p = fma2(v, p, pair(TANH_3, TANH_3));
-                            p = fma2(v, p, pair(TANH_2, TANH_2));
-                            p = fma2(v, p, pair(TANH_1, TANH_1));
-                            p = fma2(v, p, pair(TANH_0, TANH_0));
-                            unpair(mul2(mul2(x, out), p), s[c], s[c + 1]);
                         }
                     }
                 }
@@ -543,16 +565,14 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
                 }
                 if (!all) {
                     uint32_t seen[4];  // bits of the rows that this query row sees
-                    if (listed && (arrays || (drafts_listed && first + KT > ctx))) {
+                    if (has_pos || (drafts_listed && first + KT > ctx)) {
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             seen[j] = 0;
-#pragma unroll 1
+#pragma unroll 2
                             for (int g = 0; g < 8; ++g) {
-                                const uint4 p4 = kp4[j * 8 + g], d4 = has_doc ? kp4[KT / 4 + j * 8 + g] : make_uint4(qd, qd, qd, qd);
-                                uint32_t bits = (sight.sees(qp, p4.x) && d4.x == qd ? 1u : 0u) | (sight.sees(qp, p4.y) && d4.y == qd ? 2u : 0u) |
-                                                (sight.sees(qp, p4.z) && d4.z == qd ? 4u : 0u) | (sight.sees(qp, p4.w) && d4.w == qd ? 8u : 0u);
-                                seen[j] |= bits << g * 4;
+                                const uint4 p = kp4[j * 8 + g];
+                                seen[j] |= ((sight.sees(qp, p.x) ? 1u : 0u) | (sight.sees(qp, p.y) ? 2u : 0u) | (sight.sees(qp, p.z) ? 4u : 0u) | (sight.sees(qp, p.w) ? 8u : 0u)) << g * 4;
                             }
                         }
                     } else {  // positions one after another: what is seen are one or two runs
@@ -561,12 +581,24 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
                         const int lo = (int)max(0ll, min(low, 128ll)), hi = (int)max(0ll, min(high, 128ll)), pre = (int)max(0ll, min((long long)sight.prefix - at, 128ll));
 #pragma unroll
                         for (int j = 0; j < 4; ++j) seen[j] = (low_bits(hi - 32 * j) & ~low_bits(lo - 32 * j)) | low_bits(pre - 32 * j);
-                        if (a.tree && first + KT > ctx) {  // (no window: what comes before the drafted rows is seen)
+                        if (is_tree && first + KT > ctx) {  // (no window: what comes before the drafted rows is seen)
 #pragma unroll
                             for (int j = 0; j < 4; ++j) seen[j] = low_bits((int)ctx - (int)first - 32 * j);
                         }
                     }
-                    if (a.tree && first + KT > ctx) {  // of the drafted rows only itself and its ancestors
+                    if (has_doc) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            uint32_t bits = 0;
+#pragma unroll 4
+                            for (int g = 0; g < 8; ++g) {
+                                const uint4 d = kp4[KT / 4 + j * 8 + g];
+                                bits |= ((d.x == qd ? 1u : 0u) | (d.y == qd ? 2u : 0u) | (d.z == qd ? 4u : 0u) | (d.w == qd ? 8u : 0u)) << g * 4;
+                            }
+                            seen[j] &= bits;
+                        }
+                    }
+                    if (is_tree && first + KT > ctx) {  // of the drafted rows only itself and its ancestors
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             const int from = (int)first + 32 * j - (int)ctx;  // the word's first row, counted among the drafted
@@ -604,7 +636,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
                     if (odd) *s_odd = 1u;
                     __syncwarp();
                 }
-                {
+                if (!fused) {
                     float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                     for (int c = 0; c < 128; c += 8)
@@ -630,26 +662,38 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
                 const float use = m == -INFINITY ? 0.0f : m;
                 const uint64_t mul_2 = pair(mul, mul), use_2 = pair(-use, -use);
                 uint64_t sum_a = pair(0.0f, 0.0f), sum_b = sum_a;
+                const auto weights = [&](auto capped) {
+                    const uint64_t in = pair(to_log2, to_log2), out = pair(cap2, cap2);
 #pragma unroll
-                for (int c = 0; c < 128; c += 32) {
-                    uint32_t p[16];
+                    for (int c = 0; c < 128; c += 32) {
+                        uint32_t p[16];
 #pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        float x, y;
-                        unpair(fma2(pair(s[c + e], s[c + e + 1]), mul_2, use_2), x, y);
-                        x = exp2_fast(x);
-                        y = exp2_fast(y);
-                        if (e & 2) sum_a = add2(sum_a, pair(x, y));
-                        else sum_b = add2(sum_b, pair(x, y));
-                        p[e / 2] = pack_bf16(x, y);
+                        for (int e = 0; e < 32; e += 2) {
+                            float x, y;
+                            uint64_t z = pair(s[c + e], s[c + e + 1]);
+                            if constexpr (decltype(capped)::value) {
+                                z = mul2(z, in);
+                                z = fma2(mul2(z, tanh_poly(mul2(z, z))), out, use_2);
+                            } else {
+                                z = fma2(z, mul_2, use_2);
+                            }
+                            unpair(z, x, y);
+                            x = exp2_fast(x);
+                            y = exp2_fast(y);
+                            if (e & 2) sum_a = add2(sum_a, pair(x, y));
+                            else sum_b = add2(sum_b, pair(x, y));
+                            p[e / 2] = pack_bf16(x, y);
+                        }
+                        tmem_st16(ts + c / 2, p);
+                        if (c == 32) {  // the products with the first half of the values may begin
+                            tmem_wait_st();
+                            tc_before();
+                            bar_arrive(bar(P_HALF + t));
+                        }
                     }
-                    tmem_st16(ts + c / 2, p);
-                    if (c == 32) {  // the products with the first half of the values may begin
-                        tmem_wait_st();
-                        tc_before();
-                        bar_arrive(bar(P_HALF + t));
-                    }
-                }
+                };
+                if (fused) weights(std::true_type());
+                else weights(std::false_type());
                 {
                     float x, y;
                     unpair(add2(sum_a, sum_b), x, y);
@@ -817,7 +861,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
                 for (uint32_t i = lane; i < KT; i += 32) {
                     const uint32_t row = min(first + i, w.n - 1);
                     uint32_t* at = s_meta + (li & 3) * 3 * KT + i;
-                    const uint32_t p = has_pos ? a.row_pos[w.entry + row] : a.tree && row >= w.ctx ? w.sg.base + w.ctx + s_depth[row - w.ctx] : w.sg.base + row;
+                    const uint32_t p = has_pos ? a.row_pos[w.entry + row] : is_tree && row >= w.ctx ? w.sg.base + w.ctx + s_depth[row - w.ctx] : w.sg.base + row;
                     at[0] = p;
                     if (has_doc) at[KT] = a.row_doc[w.entry + row];
                     at[2 * KT] = __float_as_uint((float)((long long)p - (long long)near_pos));
@@ -884,7 +928,7 @@ bool wide_row_map(CUtensorMap* map, const void* base, uint64_t token_stride, uin
                   CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int D>
+template <int D, bool CAP, bool RICH>
 Status launch_wide(Ctx* c, CacheArgs a, CacheWork w, const WideMaps& maps) {
     using S = Wide<D>;
     cache_cut(&w, a.group, MB, KT, std::min(RUN_MOST, cache_longest_run(w, a.group, MB, KT, a.n_kv, (uint32_t)sm_count(c->device))));
@@ -894,13 +938,14 @@ Status launch_wide(Ctx* c, CacheArgs a, CacheWork w, const WideMaps& maps) {
     a.n_segs = (uint32_t)w.segs.size();
     CacheMemory mem{c};
     SLHA_TRY(cache_part_memory(&a, w, MB, &mem));
-    SLHA_TRY((cache_smem<cache_attend_wide_kernel<D>>(c, S::SMEM_TREE)));
+    constexpr auto kernel = cache_attend_wide_kernel<D, CAP, RICH>;
+    SLHA_TRY((cache_smem<kernel>(c, S::SMEM_TREE)));
     static const int regs = []() {
         cudaFuncAttributes at;
-        return cudaFuncGetAttributes(&at, cache_attend_wide_kernel<D>) == cudaSuccess ? at.numRegs : 0;
+        return cudaFuncGetAttributes(&at, cache_attend_wide_kernel<D, CAP, RICH>) == cudaSuccess ? at.numRegs : 0;
     }();
     if (regs != REGS_ALL) return Status(SLHA_ERR_DEVICE, "attention over a cache: the kernel was built with other registers than its warps share out");
-    SLHA_CUDA(launch_behind(cache_attend_wide_kernel<D>, dim3((uint32_t)(w.items * a.n_kv)), dim3(THREADS), a.tree ? S::SMEM_TREE : S::SMEM, c->stream, a, maps, tab));
+    SLHA_CUDA(launch_behind(kernel, dim3((uint32_t)(w.items * a.n_kv)), dim3(THREADS), a.tree ? S::SMEM_TREE : S::SMEM, c->stream, a, maps, tab));
     count_launch();
     if (w.blocks) SLHA_TRY(launch_cache_join(c, a, SLHA_B200_BF16, w, MB));
     return mem.done();
@@ -917,7 +962,12 @@ Status launch_attend_wide(Ctx* c, CacheArgs a, CacheWork w, bool* taken) {
     if (!*taken) return Status();
     maps.q_boxes = wide_row_map(&maps.q, a.q, a.qts, a.qhs, a);
     maps.out_boxes = wide_row_map(&maps.out, a.out, a.ots, a.ohs, a);
-    return a.d <= 64 ? launch_wide<64>(c, a, std::move(w), maps) : launch_wide<128>(c, a, std::move(w), maps);
+    const bool rich = a.row_pos || a.row_doc || a.q_pos || a.slopes || a.tree;
+    if (a.d <= 64)
+        return a.cap > 0.0f ? (rich ? launch_wide<64, true, true>(c, a, std::move(w), maps) : launch_wide<64, true, false>(c, a, std::move(w), maps))
+                            : (rich ? launch_wide<64, false, true>(c, a, std::move(w), maps) : launch_wide<64, false, false>(c, a, std::move(w), maps));
+    return a.cap > 0.0f ? (rich ? launch_wide<128, true, true>(c, a, std::move(w), maps) : launch_wide<128, true, false>(c, a, std::move(w), maps))
+                        : (rich ? launch_wide<128, false, true>(c, a, std::move(w), maps) : launch_wide<128, false, false>(c, a, std::move(w), maps));
 }
 
 }  // namespace slha
