@@ -928,10 +928,61 @@ bool wide_row_map(CUtensorMap* map, const void* base, uint64_t token_stride, uin
                   CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Shares the segments' tiles out: each block of query rows visits some, in n_chunks items.  In units of a tile's time (1.8 us) an item costs about eight to begin and to end; what
+// fits on the GPU at once takes as long as its longest item, more than that the mean load and half an item.  Where there are two blocks for every SM nothing is split.
+void wide_share(const CacheArgs& a, CacheWork* w, uint32_t slots) {
+    const bool known = !a.row_pos && !a.row_doc && !a.q_pos && !a.tree && !a.prefix && !a.rows;  // what a block visits follows from the table
+    std::vector<uint32_t> most(w->segs.size());
+    double total = 0.0, blocks = 0.0;
+    uint32_t longest = 1;
+    for (size_t i = 0; i < w->segs.size(); ++i) {
+        const CacheSeg& s = w->segs[i];
+        const uint32_t n = s.n_rows, tiles = std::max(1u, (uint32_t)(((uint64_t)n + KT - 1) / KT)), ctx = n - std::min(n, s.n_queries);
+        const uint64_t count = ((uint64_t)s.n_queries * a.group + MB - 1) / MB;
+        most[i] = known ? 1 : tiles;
+        if (known && n)
+            for (uint64_t b = 0; b < count; ++b) {
+                const uint64_t p0 = ctx + b * MB / a.group, p1 = ctx + std::min<uint64_t>((b * MB + MB - 1) / a.group, s.n_queries - 1);
+                const uint64_t lo = p0 > a.window_last ? p0 - a.window_last : 0, hi = std::min<uint64_t>(n - 1, a.causal ? p1 : p1 + a.window_last);
+                const uint32_t visited = hi >= lo ? (uint32_t)(hi / KT - lo / KT + 1) : 1;
+                most[i] = std::max(most[i], visited);
+                total += (double)visited * a.n_kv;
+            }
+        else total += (double)count * tiles * a.n_kv;
+        blocks += (double)count * a.n_kv;
+        longest = std::max(longest, most[i]);
+    }
+    uint32_t best = std::min(longest, RUN_MOST);
+    if (blocks < 2.0 * slots) {
+        double best_time = 1e300;
+        for (uint32_t run = best;; run = std::min(run - 1, run * 7 / 8)) {
+            double items = 0.0;
+            for (size_t i = 0; i < w->segs.size(); ++i) items += (double)(((uint64_t)w->segs[i].n_queries * a.group + MB - 1) / MB) * ((most[i] + run - 1) / run) * a.n_kv;
+            const double time = items <= slots ? run + 8.0 : total / slots + 8.0 * items / slots + 0.5 * run;
+            if (time + (run < longest ? 3.0 : 0.0) < best_time) best_time = time + (run < longest ? 3.0 : 0.0), best = run;
+            if (run <= 2) break;
+        }
+    }
+    w->items = w->blocks = 0;
+    w->chunks = 1;
+    for (size_t i = 0; i < w->segs.size(); ++i) {
+        CacheSeg& s = w->segs[i];
+        const uint32_t tiles = std::max(1u, (uint32_t)(((uint64_t)s.n_rows + KT - 1) / KT));
+        const uint64_t count = ((uint64_t)s.n_queries * a.group + MB - 1) / MB;
+        s.n_chunks = (most[i] + best - 1) / best;
+        s.chunk_tiles = (tiles + s.n_chunks - 1) / s.n_chunks;
+        s.item_begin = (uint32_t)w->items;
+        s.block_begin = (uint32_t)w->blocks;
+        w->items += count * s.n_chunks;
+        if (s.n_chunks > 1) w->blocks += count;
+        w->chunks = std::max(w->chunks, s.n_chunks);
+    }
+}
+
 template <int D, bool CAP, bool RICH>
 Status launch_wide(Ctx* c, CacheArgs a, CacheWork w, const WideMaps& maps) {
     using S = Wide<D>;
-    cache_cut(&w, a.group, MB, KT, std::min(RUN_MOST, cache_longest_run(w, a.group, MB, KT, a.n_kv, (uint32_t)sm_count(c->device))));
+    wide_share(a, &w, (uint32_t)sm_count(c->device));
     if (w.items * a.n_kv > 0x7FFFFFFFull) return Status(SLHA_ERR_CAPACITY, "attention over a cache: too many blocks of query rows");
     CacheTable tab;
     SLHA_TRY(cache_table(c, w.segs, &tab, &a.table));
