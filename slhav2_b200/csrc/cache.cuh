@@ -160,6 +160,7 @@ Status cache_part_memory(CacheArgs* a, const CacheWork& w, uint32_t mb, CacheMem
 Status launch_cache_join(Ctx* c, CacheArgs a, int dtype, const CacheWork& w, uint32_t mb);
 Status launch_attend_wide(Ctx* c, CacheArgs a, CacheWork w, bool* taken);
 Status launch_attend_cache(Ctx* c, CacheArgs a, int dtype, const std::vector<SlhaB200Segment>& segs);
+Status launch_observe_wide(Ctx* c, CacheArgs a, std::vector<CacheSeg> segs, uint64_t most_rows, bool* taken);
 Status launch_observe_cache(Ctx* c, CacheArgs a, int dtype, const std::vector<SlhaB200Segment>& segs);
 Status launch_evict_cache(Ctx* c, EvictArgs a, const std::vector<SlhaB200Segment>& segs, const std::vector<SlhaB200Segment>& to_segs);
 

@@ -241,6 +241,11 @@ Status launch_observe_cache(Ctx* c, CacheArgs a, int dtype, const std::vector<Sl
         most = std::max(most, (uint64_t)s.n_queries * a.group);
     }
     if (table.empty()) return Status();
+    if (dtype == SLHA_B200_BF16) {
+        bool taken;
+        SLHA_TRY(launch_observe_wide(c, a, table, most, &taken));
+        if (taken) return Status();
+    }
     return dtype == SLHA_B200_BF16 ? launch_observe_d<__nv_bfloat16>(c, a, table, most <= 16) : launch_observe_d<float>(c, a, table, most <= 16);
 }
 
