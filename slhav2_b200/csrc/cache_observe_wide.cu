@@ -1,7 +1,7 @@
 // The weight that each cached row received, for bfloat16 rows of up to 128 dimensions and up to 512 query rows a KV head (the arithmetic is that of cache_observe.cu).
 //
 // Scores as S^T = K Q^T on tcgen05: a tile of 128 keys is the M side, so that a thread has a key's scores in its own TMEM lane and its weight is a sum over the thread's own
-// columns: no sum crosses threads (with many query rows, two threads share a key).  A CTA takes the queries of one KV head, which stay in shared memory, and a run of key tiles,
+// columns: no sum crosses threads (with many query rows, four threads share a key).  A CTA takes the queries of one KV head, which stay in shared memory, and a run of key tiles,
 // each of which is read once (TMA, the tile behind which a segment ends by cp.async).  While one block of scores is summed, the next is multiplied.
 #include <cuda_bf16.h>
 
@@ -15,15 +15,15 @@ namespace {
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int KT = 128;
 
-// MANY: up to 512 query rows, two threads a key, one CTA an SM; else up to 32, one thread a key, two CTAs an SM
+// MANY: up to 512 query rows, four threads a key, one CTA an SM; else up to 32, one thread a key, two CTAs an SM
 template <int D, bool MANY>
 struct Obs {
     static constexpr int HALVES = D / 64, ROWS = MANY ? 512 : 32, BLOCK = MANY ? 256 : 32;  // query rows in all, and of a product
-    static constexpr int SUMMERS = MANY ? 256 : 128, THREADS = SUMMERS + 64, MMA_WARP = SUMMERS / 32, FETCH_WARP = MMA_WARP + 1;
+    static constexpr int SUMMERS = MANY ? 512 : 128, THREADS = SUMMERS + 64, MMA_WARP = SUMMERS / 32, FETCH_WARP = MMA_WARP + 1;
     static constexpr int STAGES = MANY ? 2 : (D == 64 ? 5 : 3);
     static constexpr uint32_t TILE = HALVES * HALF, Q_HALF = ROWS * 128, TMEM = MANY ? 512 : 64;
     static constexpr uint32_t K_AT = HALVES * Q_HALF, ROW_AT = K_AT + STAGES * TILE;  // per query row: lse in units of log 2 (two parts), position, document, slope, distance
-    static constexpr uint32_t SUM_AT = ROW_AT + 6 * ROWS * 4, BAR_AT = SUM_AT + (MANY ? KT * 4 : 0), SMEM = BAR_AT + 128 + 1024;
+    static constexpr uint32_t SUM_AT = ROW_AT + 6 * ROWS * 4, BAR_AT = SUM_AT + (MANY ? 3 * KT * 4 : 0), SMEM = BAR_AT + 128 + 1024;
     static constexpr int CTAS = MANY ? 1 : 2;
     static_assert(CTAS * (SMEM + 1024) <= 228 * 1024, "shared memory of an SM");
 };
@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(Obs<D, MANY>::THREADS, Obs<D, MANY>::CTAS)
     };
 
     if (warp < S::SUMMERS / 32) {
-        const uint32_t half = MANY ? warp >> 2 : 0, k_row = (warp & 3) * 32 + lane;
+        const uint32_t quarter = MANY ? warp >> 2 : 0, k_row = (warp & 3) * 32 + lane;
         const float to_log2 = has_cap ? a.scale / a.cap : a.scale * LOG2E, cap2 = a.cap * LOG2E;
         const bool bent = has_cap || has_slope;
         bool alone = false;  // a wait ran out: this warp goes on with dot products of its own
@@ -142,22 +142,22 @@ __global__ void __launch_bounds__(Obs<D, MANY>::THREADS, Obs<D, MANY>::CTAS)
             const uint32_t row = j * KT + k_row, there = min(row, n - 1);
             const uint64_t at = head * a.w_hs + sg.row_begin + row;
             const uint32_t kp = has_pos ? a.row_pos[entry + there] : sg.base + there, kd = has_doc ? a.row_doc[entry + there] : 0u;
-            const float before = a.w_in && half == 0 && row < n ? a.w_in[at] : 0.0f, k_at = (float)((long long)kp - (long long)near_pos);
+            const float before = a.w_in && quarter == 0 && row < n ? a.w_in[at] : 0.0f, k_at = (float)((long long)kp - (long long)near_pos);
             float sum = 0.0f;
             if (visited(j)) {
                 // whether all query rows see the warp's keys
                 const uint32_t far_ = max(qr.pmax > kp ? qr.pmax - kp : 0u, kp > qr.pmin ? kp - qr.pmin : 0u);
                 const bool all = __all_sync(0xFFFFFFFFu, (!has_doc || (qr.dmin == qr.dmax && kd == qr.dmin)) && (kp < sight.prefix || ((!sight.causal || kp <= qr.pmin) && far_ <= sight.window_last)));
                 for (uint32_t b = 0; b < blocks; ++b, ++use) {
-                    const uint32_t cols = columns(b), buf = use & 1, mine = MANY ? cols / 2 : cols, c_from = half * mine, r_from = b * S::BLOCK + c_from;
+                    const uint32_t cols = columns(b), buf = use & 1, r_from = b * S::BLOCK;
                     if (!alone) alone = !__all_sync(0xFFFFFFFFu, bar_wait(bar(S_FULL + buf), use >> 1 & 1));
                     tc_after();
-                    for (uint32_t c0 = 0; c0 < mine && r_from + c0 < q_rows; c0 += 16) {
+                    for (uint32_t c0 = quarter * 16; c0 < cols && r_from + c0 < q_rows; c0 += MANY ? 64 : 16) {
                         uint32_t u[16];
                         float* s = reinterpret_cast<float*>(u);
                         __syncwarp();
                         if (!alone) {
-                            tmem_ld16(tmem + ((uint32_t)(warp & 3) << 21) + buf * S::BLOCK + c_from + c0, u);
+                            tmem_ld16(tmem + ((uint32_t)(warp & 3) << 21) + buf * S::BLOCK + c0, u);
                         } else {
 #pragma unroll 1
                             for (int c = 0; c < 16; ++c) {
@@ -202,13 +202,13 @@ __global__ void __launch_bounds__(Obs<D, MANY>::THREADS, Obs<D, MANY>::CTAS)
                     bar_arrive(bar(S_FREE + buf));
                 }
             }
-            if constexpr (MANY) {  // the two halves of a key meet
-                if (half) s_sum[k_row] = sum;
-                asm volatile("bar.sync 1, 256;\n" ::: "memory");
-                if (!half) sum += s_sum[k_row];
-                asm volatile("bar.sync 1, 256;\n" ::: "memory");
+            if constexpr (MANY) {  // a key's four sums meet
+                if (quarter) s_sum[(quarter - 1) * KT + k_row] = sum;
+                asm volatile("bar.sync 1, 512;\n" ::: "memory");
+                if (!quarter) sum = (sum + s_sum[k_row]) + (s_sum[KT + k_row] + s_sum[2 * KT + k_row]);
+                asm volatile("bar.sync 1, 512;\n" ::: "memory");
             }
-            if (half == 0 && row < n) a.w_out[at] = a.w_in && a.decay != 0.0f ? fmaf(a.decay, before, sum) : sum;
+            if (quarter == 0 && row < n) a.w_out[at] = a.w_in && a.decay != 0.0f ? fmaf(a.decay, before, sum) : sum;
         }
     } else if (warp == S::MMA_WARP) {
         uint32_t lead;
