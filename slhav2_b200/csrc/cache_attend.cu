@@ -394,47 +394,73 @@ __global__ void __launch_bounds__(ATT_THREADS, Shape<T, D, WM>::CTAS) cache_atte
     }
 }
 
-// Joins the parts of query rows whose segment's rows were split: a warp a query row.
+// Joins the parts of query rows whose segment's rows were split.  WARPS warps a query row: each takes every WARPS-th part, their sums meet in shared memory in the warps' order.
 constexpr int JOIN_THREADS = 128;
-template <typename T>
+template <typename T, int WARPS>
 __global__ void __launch_bounds__(JOIN_THREADS) cache_join_kernel(const __grid_constant__ CacheArgs a, const __grid_constant__ CacheTable tab, uint32_t mb, uint32_t blocks_of) {
     dep_wait();
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    constexpr int ROWS = JOIN_THREADS / 32 / WARPS, FLIGHT = WARPS > 1 ? 8 : 3;
+    __shared__ float4 s_acc[WARPS > 1 ? WARPS : 1][64];
+    __shared__ float s_sum[WARPS];
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, mine = warp % WARPS;
     const uint32_t part = blockIdx.x % blocks_of, at = blockIdx.x / blocks_of, head = at % a.n_kv, qb = at / a.n_kv;
     const CacheSeg* table = a.table ? a.table : tab.s;
     const uint32_t seg = cache_find(a.n_segs, qb, [&](uint32_t i) { return table[i].block_begin; });
     const CacheSeg sg = table[seg];
-    const uint32_t block = qb - sg.block_begin, r = part * (JOIN_THREADS / 32) + warp, row = block * mb + r;
-    if (r >= mb || row >= sg.n_queries * a.group) return;
+    const uint32_t block = qb - sg.block_begin, r = part * ROWS + warp / WARPS, row = block * mb + r;
+    if (r >= mb || row >= sg.n_queries * a.group) return;  // (with more than one warp a row: all of them)
     const uint64_t first = ((uint64_t)(sg.item_begin + block * sg.n_chunks) * a.n_kv + head) * mb + r, step = (uint64_t)a.n_kv * mb;
     float top = -INFINITY;
     for (uint32_t c = lane; c < sg.n_chunks; c += 32) top = fmaxf(top, a.part_ml[(first + c * step) * 2]);
     for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
     float4 acc[2] = {make_float4(0.0f, 0.0f, 0.0f, 0.0f), make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
     float sum = 0.0f;
-    for (uint32_t c0 = 0; c0 < sg.n_chunks; c0 += 32) {
-        float f = 0.0f, lf = 0.0f;
-        if (c0 + lane < sg.n_chunks) {
-            const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + (first + (c0 + lane) * step) * 2);
-            f = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - top);
-            lf = ml.y * f;
-        }
-        for (int x = 16; x; x >>= 1) lf += __shfl_xor_sync(0xFFFFFFFFu, lf, x);
-        sum += lf;
-        const uint32_t here = min(32u, sg.n_chunks - c0);
-#pragma unroll 4
-        for (uint32_t c = 0; c < here; ++c) {
-            const float fc = __shfl_sync(0xFFFFFFFFu, f, c);
-            const float* src = a.part_o + (first + (c0 + c) * step) * a.d;
+    const uint32_t v_count = a.d > 128 ? 2 : 1;
+    for (uint32_t c0 = mine; c0 < sg.n_chunks; c0 += WARPS * FLIGHT) {
+        float2 ml[FLIGHT];
+        float4 x[FLIGHT];
 #pragma unroll
-            for (int v = 0; v < 2; ++v)
-                if (lane * 4 + v * 128 < a.d) {
-                    const float4 x = *reinterpret_cast<const float4*>(src + lane * 4 + v * 128);
-                    acc[v].x = fmaf(fc, x.x, acc[v].x);
-                    acc[v].y = fmaf(fc, x.y, acc[v].y);
-                    acc[v].z = fmaf(fc, x.z, acc[v].z);
-                    acc[v].w = fmaf(fc, x.w, acc[v].w);
-                }
+        for (int i = 0; i < FLIGHT; ++i) {
+            const uint32_t c = c0 + i * WARPS;
+            const bool there = c < sg.n_chunks;
+            ml[i] = there ? *reinterpret_cast<const float2*>(a.part_ml + (first + c * step) * 2) : make_float2(-INFINITY, 0.0f);
+            x[i] = there && lane * 4 < a.d ? *reinterpret_cast<const float4*>(a.part_o + (first + c * step) * a.d + lane * 4) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+#pragma unroll
+        for (int i = 0; i < FLIGHT; ++i) {
+            const float f = ml[i].x == -INFINITY ? 0.0f : exp2_fast(ml[i].x - top);
+            sum = fmaf(f, ml[i].y, sum);
+            acc[0].x = fmaf(f, x[i].x, acc[0].x);
+            acc[0].y = fmaf(f, x[i].y, acc[0].y);
+            acc[0].z = fmaf(f, x[i].z, acc[0].z);
+            acc[0].w = fmaf(f, x[i].w, acc[0].w);
+        }
+        if (v_count == 2)
+#pragma unroll
+            for (int i = 0; i < FLIGHT; ++i) {
+                const uint32_t c = c0 + i * WARPS;
+                if (c >= sg.n_chunks || lane * 4 + 128 >= a.d) continue;
+                const float4 y = *reinterpret_cast<const float4*>(a.part_o + (first + c * step) * a.d + lane * 4 + 128);
+                const float f = ml[i].x == -INFINITY ? 0.0f : exp2_fast(ml[i].x - top);
+                acc[1].x = fmaf(f, y.x, acc[1].x);
+                acc[1].y = fmaf(f, y.y, acc[1].y);
+                acc[1].z = fmaf(f, y.z, acc[1].z);
+                acc[1].w = fmaf(f, y.w, acc[1].w);
+            }
+    }
+    if constexpr (WARPS > 1) {
+        s_acc[mine][lane] = acc[0];
+        s_acc[mine][32 + lane] = acc[1];
+        if (lane == 0) s_sum[mine] = sum;
+        __syncthreads();
+        if (mine) return;
+        for (int w = 1; w < WARPS; ++w) {
+            sum += s_sum[w];
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+                const float4 y = s_acc[w][v * 32 + lane];
+                acc[v].x += y.x, acc[v].y += y.y, acc[v].z += y.z, acc[v].w += y.w;
+            }
         }
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -508,11 +534,13 @@ Status launch_cache_join(Ctx* c, CacheArgs a, int dtype, const CacheWork& w, uin
     CacheTable tab;
     SLHA_TRY(cache_table(c, split, &tab, &a.table));
     a.n_segs = (uint32_t)split.size();
-    const uint32_t per = (rows + JOIN_THREADS / 32 - 1) / (JOIN_THREADS / 32);
+    // four warps a row where it has many parts (35 parts of a row: 19 us with one warp, 5 with four)
+    const uint32_t warps = w.chunks > 8 ? 4 : 1, at_once = JOIN_THREADS / 32 / warps, per = (rows + at_once - 1) / at_once;
     if (w.blocks * a.n_kv * per > 0x7FFFFFFFull) return Status(SLHA_ERR_CAPACITY, "attention over a cache: too many blocks of query rows");
     const dim3 grid((uint32_t)(w.blocks * a.n_kv * per));
-    SLHA_CUDA(dtype == SLHA_B200_BF16 ? launch_behind(cache_join_kernel<__nv_bfloat16>, grid, dim3(JOIN_THREADS), 0, c->stream, a, tab, mb, per)
-                                      : launch_behind(cache_join_kernel<float>, grid, dim3(JOIN_THREADS), 0, c->stream, a, tab, mb, per));
+    const bool bf = dtype == SLHA_B200_BF16;
+    SLHA_CUDA(launch_behind(warps == 4 ? (bf ? cache_join_kernel<__nv_bfloat16, 4> : cache_join_kernel<float, 4>) : (bf ? cache_join_kernel<__nv_bfloat16, 1> : cache_join_kernel<float, 1>),
+                            grid, dim3(JOIN_THREADS), 0, c->stream, a, tab, mb, per));
     count_launch();
     return Status();
 }

@@ -1,16 +1,19 @@
 // Removal of the cached rows that received the least weight (slha_b200_evict_cache).
 //
 // Two kernels.  The first, a CTA for each KV head of a segment, finds which min(n, budget) of the n rows stay: the budget-th largest of the rows' keys by
-// radix selection (8 bits a pass, from the top), equal keys by the lower row, and writes for each place below the budget the row that comes to it.  The
+// radix selection (11 bits, 11, 10), equal keys by the lower row, and writes for each place below the budget the row that comes to it.  The
 // second moves rows.  A kept row below the budget stays where it is, so in place only rows from beyond the budget move, into places that no row is read from.
+#include <cooperative_groups.h>
+
 #include <algorithm>
+#include <type_traits>
 
 #include "cache.cuh"
 
 namespace slha {
 namespace {
 
-constexpr int SEL_THREADS = 1024, SEL_WARPS = SEL_THREADS / 32, SEL_EACH = 4;
+constexpr int SEL_THREADS = 1024, SEL_WARPS = SEL_THREADS / 32, SEL_BINS = 2048;
 constexpr uint32_t SEL_HELD = 49152;  // keys that fit in shared memory
 
 // weights in the order of unsigned numbers: pinned rows above all, NaN below all, -0 like 0
@@ -21,169 +24,228 @@ __device__ __forceinline__ uint32_t weight_key(float w, bool pinned) {
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-// sums of `x` over the threads before this one, and over all
-__device__ __forceinline__ uint32_t scan_threads(uint32_t x, uint32_t* sh, uint32_t* total) {
+// the sum of `x` over the threads before this one
+__device__ __forceinline__ uint32_t scan_threads(uint32_t x, uint32_t* sh) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     uint32_t s = x;
     for (int o = 1; o < 32; o <<= 1) {
         const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, s, o);
         if (lane >= o) s += y;
     }
-    __syncthreads();
     if (lane == 31) sh[warp] = s;
     __syncthreads();
-    if (warp == 0) {
-        uint32_t v = sh[lane];
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, v, o);
-            if (lane >= o) v += y;
-        }
-        sh[lane] = v;
-    }
-    __syncthreads();
-    *total = sh[SEL_WARPS - 1];
-    return s - x + (warp ? sh[warp - 1] : 0u);
+    return s - x + __reduce_add_sync(0xFFFFFFFFu, lane < warp ? sh[lane] : 0u);
 }
 
-__global__ void __launch_bounds__(SEL_THREADS) cache_select_kernel(const __grid_constant__ EvictArgs a, const __grid_constant__ CacheTable tab) {
+// A cluster of C CTAs has a KV head of a segment: a run of its rows each, in it a run a warp, in 128s a run of four a lane.
+template <int C>
+__global__ void __cluster_dims__(C, 1, 1) __launch_bounds__(SEL_THREADS) cache_select_kernel(const __grid_constant__ EvictArgs a, const __grid_constant__ CacheTable tab) {
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
     dep_wait();
-    extern __shared__ uint32_t s_key[];
-    __shared__ uint32_t s_hist[8][256], s_scan[SEL_WARPS], s_found[2], s_last;
-    const int tid = threadIdx.x, lane = tid & 31;
-    const uint32_t at = blockIdx.x / a.n_kv, head = blockIdx.x % a.n_kv;
+    extern __shared__ __align__(16) uint32_t s_key[];
+    __shared__ uint32_t s_hist[SEL_BINS], s_scan[SEL_WARPS], s_found[2], s_last, s_warp[SEL_WARPS], s_all[3];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t which = blockIdx.x / C, rank_of = C > 1 ? cluster.block_rank() : 0u, at = which / a.n_kv, head = which % a.n_kv;
     const CacheSeg sg = (a.table ? a.table : tab.s)[at];
     const uint32_t n = a.rows ? min(a.rows[sg.seg], sg.n_rows) : sg.n_rows;
     const uint32_t budget = a.budget, stay = min(n, budget);
-    uint32_t* source = a.places + (uint64_t)blockIdx.x * a.room;
-    uint32_t* hole = a.holes + (uint64_t)blockIdx.x * a.room;
+    uint32_t* source = a.places + (uint64_t)which * a.room;
+    uint32_t* hole = a.holes + (uint64_t)which * a.room;
     uint32_t* wanted = a.source ? a.source + ((uint64_t)sg.seg * a.n_kv + head) * budget : nullptr;
-    if (tid == 0) a.stay[blockIdx.x] = stay;
-    const uint64_t entry = head * a.entry_hs + sg.row_begin;
-    const float* w = a.w + head * a.w_hs + sg.row_begin;
+    if (tid == 0 && rank_of == 0) a.stay[which] = stay;
     if (n <= budget) {
-        for (uint32_t i = tid; i < n; i += SEL_THREADS) {
+        for (uint32_t i = rank_of * SEL_THREADS + tid; i < n; i += C * SEL_THREADS) {
             source[i] = i;
             if (wanted) wanted[i] = i;
         }
         return;
     }
-    const auto position = [&](uint32_t i) { return a.pos ? a.pos[entry + i] : sg.base + i; };
+    const uint64_t entry = head * a.entry_hs + sg.row_begin;
+    const float* w = a.w + head * a.w_hs + sg.row_begin;
+    // this CTA's rows and this warp's (of the CTA's, counted from its first)
+    const uint32_t run = (n + C * SEL_WARPS * 128 - 1) / (C * SEL_WARPS * 128) * 128, base = min(n, rank_of * SEL_WARPS * run), own = min(n, base + SEL_WARPS * run) - base;
+    const uint32_t from = min(own, warp * run), to = min(own, from + run);
+    const auto position = [&](uint32_t i) { return a.pos ? a.pos[entry + base + i] : sg.base + base + i; };
+    constexpr int FLIGHT = 8;  // loads that a thread has under way
+    const bool held = own <= SEL_HELD, kept_pos = a.recent && a.pos && held;
     if (tid == 0) s_last = 0;
     __syncthreads();
     if (a.recent) {
-        uint32_t last = 0;
+        uint32_t last = a.pos ? 0u : sg.base + n - 1;
         if (a.pos)
-            for (uint32_t i = tid; i < n; i += SEL_THREADS) last = max(last, a.pos[entry + i]);
-        else last = sg.base + n - 1;
+            for (uint32_t i0 = tid; i0 < own; i0 += SEL_THREADS * FLIGHT) {
+                uint32_t p[FLIGHT];
+#pragma unroll
+                for (int f = 0; f < FLIGHT; ++f) p[f] = i0 + f * SEL_THREADS < own ? a.pos[entry + base + i0 + f * SEL_THREADS] : 0u;
+#pragma unroll
+                for (int f = 0; f < FLIGHT; ++f) {
+                    last = max(last, p[f]);
+                    if (kept_pos && i0 + f * SEL_THREADS < own) s_key[i0 + f * SEL_THREADS] = p[f];  // (until the keys take their place)
+                }
+            }
         last = __reduce_max_sync(0xFFFFFFFFu, last);
         if (lane == 0) atomicMax(&s_last, last);
-        __syncthreads();
     }
-    const uint32_t newest = s_last;
-    const auto make_key = [&](uint32_t i) {
-        const uint32_t p = position(i);
-        return weight_key(w[i], p < a.sink || (a.recent && newest - p < a.recent));
-    };
-    const bool held = n <= SEL_HELD;
+    if (C > 1) cluster.sync();
+    else __syncthreads();
+    uint32_t newest = s_last;
+    for (int r = 1; r < C; ++r) newest = max(newest, *cluster.map_shared_rank(&s_last, (rank_of + r) % C));
+    const auto key_at = [&](uint32_t p, float x) { return weight_key(x, p < a.sink || (a.recent && newest - p < a.recent)); };
     if (held) {
-        for (uint32_t i = tid; i < n; i += SEL_THREADS) s_key[i] = make_key(i);
-        __syncthreads();
+        for (uint32_t i0 = tid; i0 < own; i0 += SEL_THREADS * FLIGHT) {
+            float x[FLIGHT];
+            uint32_t p[FLIGHT];
+#pragma unroll
+            for (int f = 0; f < FLIGHT; ++f) {
+                const uint32_t i = i0 + f * SEL_THREADS;
+                x[f] = i < own ? w[base + i] : 0.0f;
+                p[f] = i < own ? (kept_pos ? s_key[i] : position(i)) : 0u;
+            }
+#pragma unroll
+            for (int f = 0; f < FLIGHT; ++f)
+                if (i0 + f * SEL_THREADS < own) s_key[i0 + f * SEL_THREADS] = key_at(p[f], x[f]);
+        }
     }
-    const auto key_of = [&](uint32_t i) { return held ? s_key[i] : make_key(i); };
+    // four rows' keys from row i on (of the CTA's); rows behind the warp's last: 0, which is below all that stay but perhaps their equal
+    const auto four = [&](uint32_t i, uint32_t (&k)[4]) {
+        if (held) {
+            const uint4 x = *reinterpret_cast<const uint4*>(s_key + i);
+            k[0] = x.x, k[1] = x.y, k[2] = x.z, k[3] = x.w;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (i + e >= to) k[e] = 0u;
+            else if (!held) k[e] = key_at(position(i + e), w[base + i + e]);
+    };
 
     // the stay-th largest key, and how many of the keys equal to it stay
     uint32_t prefix = 0, left = stay;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        for (int i = tid; i < 8 * 256; i += SEL_THREADS) (&s_hist[0][0])[i] = 0;
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+        const uint32_t bins = pass == 2 ? 1024u : 2048u, settled = pass == 0 ? 0u : pass == 1 ? 0xFFE00000u : 0xFFFFFC00u;
+        for (int i = tid; i < SEL_BINS; i += SEL_THREADS) s_hist[i] = 0;
         __syncthreads();
-        for (uint32_t i0 = 0; i0 < n; i0 += SEL_THREADS) {
-            const uint32_t i = i0 + tid;
-            const uint32_t k = i < n ? key_of(i) : 0u;
-            const bool in = i < n && (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8)));
-            // one addition for the lanes of a warp that share a bucket with the first of them; the others add alone
-            const uint32_t bin = (k >> shift) & 255u, who = __ballot_sync(0xFFFFFFFFu, in);
-            if (who) {
-                const int lead = __ffs(who) - 1;
-                const uint32_t lead_bin = __shfl_sync(0xFFFFFFFFu, bin, lead);
-                const uint32_t same = __ballot_sync(0xFFFFFFFFu, in && bin == lead_bin);
-                if (lane == lead) atomicAdd(&s_hist[(tid >> 5) & 7][bin], (uint32_t)__popc(same));
-                else if (in && bin != lead_bin) atomicAdd(&s_hist[(tid >> 5) & 7][bin], 1u);
+        for (uint32_t i0 = from; i0 < to; i0 += 128) {  // (a warp without rows begins at no multiple of 128)
+            const uint32_t i = i0 + lane * 4;
+            uint32_t k[4];
+            four(i, k);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const bool in = i + e < to && !((k[e] ^ prefix) & settled);
+                const uint32_t bin = (k[e] >> shift) & (bins - 1);
+                // (a warp whose keys are all alike, as where nothing has been seen yet, adds once)
+                int alike;
+                __match_all_sync(0xFFFFFFFFu, in ? bin : 0xFFFFFFFFu, &alike);
+                if (alike ? in && lane == 0 : in) atomicAdd(&s_hist[bin], alike ? 32u : 1u);
             }
         }
-        __syncthreads();
-        if (tid < 32) {  // buckets from the top: lane 0 the highest eight
-            uint32_t c[8], sum = 0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                uint32_t x = 0;
-                for (int h = 0; h < 8; ++h) x += s_hist[h][255 - lane * 8 - j];
-                c[j] = x;
-                sum += x;
-            }
-            uint32_t before = sum;
-            for (int o = 1; o < 32; o <<= 1) {
-                const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, before, o);
-                if (lane >= o) before += y;
-            }
-            before -= sum;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                if (before < left && before + c[j] >= left) s_found[0] = 255 - lane * 8 - j, s_found[1] = left - before;
-                before += c[j];
-            }
+        if (C > 1) cluster.sync();
+        else __syncthreads();
+        // buckets from the top, two a thread
+        uint32_t c[2] = {s_hist[SEL_BINS - 1 - tid * 2], s_hist[SEL_BINS - 2 - tid * 2]};
+        for (int r = 1; r < C; ++r) {
+            const uint32_t* other = cluster.map_shared_rank(s_hist, (rank_of + r) % C);
+            c[0] += other[SEL_BINS - 1 - tid * 2];
+            c[1] += other[SEL_BINS - 2 - tid * 2];
         }
-        __syncthreads();
+        uint32_t before = scan_threads(c[0] + c[1], s_scan);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            if (before < left && before + c[j] >= left) s_found[0] = SEL_BINS - 1 - tid * 2 - j, s_found[1] = left - before;
+            before += c[j];
+        }
+        if (C > 1) cluster.sync();  // (also: the others have read this CTA's buckets)
+        else __syncthreads();
         prefix |= s_found[0] << shift;
         left = s_found[1];
-        __syncthreads();
     }
-    // rows in order: which stay, the free places below the budget, the rows from beyond that take them
-    uint32_t equal = 0, holes = 0, late = 0;
-    for (uint32_t i0 = 0; i0 < n; i0 += SEL_THREADS * SEL_EACH) {
-        uint32_t k[SEL_EACH], eq = 0, total;
-#pragma unroll
-        for (int j = 0; j < SEL_EACH; ++j) {
-            const uint32_t i = i0 + tid * SEL_EACH + j;
-            k[j] = i < n ? key_of(i) : 0u;
-            eq += i < n && k[j] == prefix;
+    // In the rows' order: how many equal the last key that stays; then which stay, the free places below the budget and the rows from beyond that take them.
+    const auto before_me = [&](uint32_t x, int slot) {  // the sum over the warps, of this CTA and those before it, before this one (x: a lane's)
+        x = __reduce_add_sync(0xFFFFFFFFu, x);
+        __syncthreads();
+        if (lane == 0) s_warp[warp] = x;
+        __syncthreads();
+        if (tid < 32) {
+            const uint32_t all = __reduce_add_sync(0xFFFFFFFFu, s_warp[lane]);
+            if (lane == 0) s_all[slot] = all;
         }
-        uint32_t rank = equal + scan_threads(eq, s_scan, &total);
-        equal += total;
-        bool keep[SEL_EACH];
-        uint32_t h = 0, f = 0;
-#pragma unroll
-        for (int j = 0; j < SEL_EACH; ++j) {
-            const uint32_t i = i0 + tid * SEL_EACH + j;
-            keep[j] = i < n && (k[j] > prefix || (k[j] == prefix && rank < left));
-            rank += i < n && k[j] == prefix;
-            h += i < budget && !keep[j];
-            f += i >= budget && keep[j];
+        uint32_t sum = __reduce_add_sync(0xFFFFFFFFu, lane < warp ? s_warp[lane] : 0u);
+        if (C > 1) {
+            cluster.sync();
+            for (uint32_t r = 0; r < rank_of; ++r) sum += *cluster.map_shared_rank(&s_all[slot], r);
         }
-        // (free places in the low half, rows from beyond in the high one: at most 4096 of each here)
-        const uint32_t both = scan_threads(h | f << 16, s_scan, &total);
-        uint32_t free_at = holes + (both & 0xFFFFu), late_at = late + (both >> 16);
-        holes += total & 0xFFFFu;
-        late += total >> 16;
+        return sum;
+    };
+    uint32_t equal_mine = 0;
+    for (uint32_t i = from + lane * 4; i < to; i += 128) {
+        uint32_t k[4];
+        four(i, k);
 #pragma unroll
-        for (int j = 0; j < SEL_EACH; ++j) {
-            const uint32_t i = i0 + tid * SEL_EACH + j;
-            if (i >= budget) continue;
-            if (!keep[j]) {
-                hole[free_at++] = i;
-            } else {
-                source[i] = i;
-                if (wanted) wanted[i] = i;
+        for (int e = 0; e < 4; ++e) equal_mine += i + e < to && k[e] == prefix;
+    }
+    const uint32_t equal = before_me(equal_mine, 0);
+    uint32_t rank = equal;
+    const auto sum_before = [&](uint32_t x) {  // over the lanes before this one, x at most 4
+        const uint32_t below = (1u << lane) - 1u;
+        return __popc(__ballot_sync(0xFFFFFFFFu, x & 1u) & below) + 2 * __popc(__ballot_sync(0xFFFFFFFFu, x & 2u) & below) + 4 * __popc(__ballot_sync(0xFFFFFFFFu, x & 4u) & below);
+    };
+    const auto keeps = [&](uint32_t i) {  // a bit for each of four rows
+        uint32_t k[4], keep = 0, eq = 0;
+        four(i, k);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            keep |= (i + e < to && k[e] > prefix ? 1u : 0u) << e;
+            eq |= (i + e < to && k[e] == prefix ? 1u : 0u) << e;
+        }
+        if (__any_sync(0xFFFFFFFFu, eq)) {
+            uint32_t r = rank + sum_before(__popc(eq));
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (eq >> e & 1u) keep |= (r++ < left ? 1u : 0u) << e;
+            rank += __reduce_add_sync(0xFFFFFFFFu, __popc(eq));
+        }
+        return keep;
+    };
+    const auto lies = [&](uint32_t i, uint32_t end) { return base + i >= end ? 0u : end - base - i < 4 ? (1u << (end - base - i)) - 1u : 15u; };  // which of four rows lie below `end`
+    uint32_t free_mine = 0, late_mine = 0;
+    for (uint32_t i0 = from; i0 < to; i0 += 128) {
+        const uint32_t i = i0 + lane * 4, keep = keeps(i), front = lies(i, budget);
+        free_mine += __popc(~keep & lies(i, base + to) & front);
+        late_mine += __popc(keep & ~front);
+    }
+    uint32_t free_at = before_me(free_mine, 1), late_at = before_me(late_mine, 2);
+    rank = equal;
+    for (uint32_t i0 = from; i0 < to && base + i0 < budget; i0 += 128) {
+        const uint32_t i = i0 + lane * 4, keep = keeps(i), front = lies(i, budget), open = ~keep & lies(i, base + to) & front;
+        uint32_t place = free_at + sum_before(__popc(open));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t row = base + i + e;
+            if (open >> e & 1u) hole[place++] = row;
+            if (keep & front & (1u << e)) {
+                source[row] = row;
+                if (wanted) wanted[row] = row;
             }
         }
-        __syncthreads();  // (all places below the budget are known before the first row from beyond it asks for one)
+        free_at += __reduce_add_sync(0xFFFFFFFFu, __popc(open));
+    }
+    if (C > 1) cluster.sync();  // (all free places are known)
+    else __syncthreads();
+    if (__all_sync(0xFFFFFFFFu, late_mine == 0)) return;
+    rank = equal;
+    for (uint32_t i0 = from; i0 < to; i0 += 128) {
+        const uint32_t i = i0 + lane * 4, comes = keeps(i) & ~lies(i, budget);
+        if (!__any_sync(0xFFFFFFFFu, comes)) continue;
+        uint32_t next = late_at + sum_before(__popc(comes));
 #pragma unroll
-        for (int j = 0; j < SEL_EACH; ++j) {
-            const uint32_t i = i0 + tid * SEL_EACH + j;
-            if (i < budget || !keep[j]) continue;
-            const uint32_t place = hole[late_at++];
-            source[place] = i;
-            if (wanted) wanted[place] = i;
-        }
+        for (int e = 0; e < 4; ++e)
+            if (comes >> e & 1u) {
+                const uint32_t place = hole[next++];
+                source[place] = base + i + e;
+                if (wanted) wanted[place] = base + i + e;
+            }
+        late_at += __reduce_add_sync(0xFFFFFFFFu, __popc(comes));
     }
 }
 
@@ -272,7 +334,7 @@ Status launch_evict_cache(Ctx* c, EvictArgs a, const std::vector<SlhaB200Segment
     const uint32_t room = a.room = std::min(a.budget, most);
     const uint64_t heads = (uint64_t)table.size() * a.n_kv, blocks = ((uint64_t)room + MOVE_PLACES - 1) / MOVE_PLACES;
     if (heads == 0) return Status();
-    if (heads * std::max<uint64_t>(blocks, 1) > 0x7FFFFFFFull) return Status(SLHA_ERR_CAPACITY, "slha_b200_evict_cache: too many rows");
+    if (heads * std::max<uint64_t>(blocks, 8) > 0x7FFFFFFFull) return Status(SLHA_ERR_CAPACITY, "slha_b200_evict_cache: too many rows");
     CacheTable tab;
     SLHA_TRY(cache_table(c, table, &tab, &a.table));
     a.n_segs = (uint32_t)table.size();
@@ -282,9 +344,18 @@ Status launch_evict_cache(Ctx* c, EvictArgs a, const std::vector<SlhaB200Segment
     a.places = static_cast<uint32_t*>(p);
     a.holes = a.places + heads * room;
     a.stay = a.holes + heads * room;
-    const size_t smem = (size_t)std::min(most, SEL_HELD) * 4;
-    SLHA_TRY((cache_smem<cache_select_kernel>(c, SEL_HELD * 4)));
-    SLHA_CUDA(launch_behind(cache_select_kernel, dim3((uint32_t)heads), dim3(SEL_THREADS), smem, c->stream, a, tab));
+    // CTAs of a cluster: as many as find an SM each, where every warp still has 128 rows (64 heads of 32768 rows: one CTA 71 us, two 30)
+    uint32_t c_size = 1;
+    while (c_size < 8 && heads * c_size * 2 <= (uint64_t)sm_count(c->device) && most > c_size * SEL_THREADS * 4) c_size *= 2;
+    const size_t share = ((size_t)most + c_size * SEL_WARPS * 128 - 1) / (c_size * SEL_WARPS * 128) * SEL_WARPS * 128, smem = std::min<size_t>(share, SEL_HELD) * 4;
+    const auto select = [&](auto kernel_of) -> Status {
+        constexpr auto kernel = cache_select_kernel<decltype(kernel_of)::value>;
+        SLHA_TRY((cache_smem<kernel>(c, SEL_HELD * 4)));
+        SLHA_CUDA(launch_behind(kernel, dim3((uint32_t)(heads * c_size)), dim3(SEL_THREADS), smem, c->stream, a, tab));
+        return Status();
+    };
+    SLHA_TRY(c_size == 8 ? select(std::integral_constant<int, 8>()) : c_size == 4 ? select(std::integral_constant<int, 4>()) : c_size == 2 ? select(std::integral_constant<int, 2>())
+                                                                                                                              : select(std::integral_constant<int, 1>()));
     count_launch();
     const uint32_t pieces = 2 * a.row_bytes / 16;
     const dim3 grid((uint32_t)(heads * std::max<uint64_t>(blocks, 1)));
