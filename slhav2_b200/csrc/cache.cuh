@@ -48,6 +48,7 @@ struct CacheArgs {
     uint32_t window_last;  // the largest distance that is seen
     int32_t causal;
     int32_t tree;
+    uint32_t cluster;  // CTAs that share a block of query rows and join their sums themselves (every segment has so many runs), or 0
 };
 struct EvictArgs {
     const void *keys, *values;
@@ -125,8 +126,6 @@ struct CacheWork {
     uint64_t items = 0, blocks = 0;  // blocks: of query rows whose segments are split
     uint32_t chunks = 1;             // the most runs of one segment
 };
-void cache_cut(CacheWork* w, uint32_t group, uint32_t mb, uint32_t kt, uint32_t most);
-uint32_t cache_longest_run(const CacheWork& w, uint32_t group, uint32_t mb, uint32_t kt, uint32_t n_kv, uint32_t slots);
 
 // Working memory of one call: the thread's, or under capture memory that the graph allocates and frees with every run, so that graphs share none.
 struct CacheMemory {
@@ -143,6 +142,23 @@ struct CacheMemory {
         return Status();
     }
 };
+// launch_behind with clusters of `size` CTAs
+template <typename... P, typename... A>
+inline cudaError_t launch_cluster(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, uint32_t size, A&&... args) {
+    cudaLaunchAttribute attr[2]{};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim = {size, 1, 1};
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = size > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...);
+}
 // The table of a launch: in the kernel's parameters, or uploaded where it is longer.
 Status cache_table(Ctx* c, const std::vector<CacheSeg>& segs, CacheTable* inl, const CacheSeg** dev);
 // Raises a kernel's limit of dynamic shared memory, once per kernel and device.

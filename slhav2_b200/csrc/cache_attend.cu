@@ -8,6 +8,7 @@
 // A CTA takes a block of 16, 32 or 64 query rows of one KV head (row = token x the head's group of query heads, so that the keys are read once for the group) and
 // a run of the segment's rows in tiles of 64 (float32: 32).  Four warps: with 16 query rows each takes a quarter of a tile's keys, with 64 each takes
 // its own 16 rows.  Tiles arrive by cp.async, two or three ahead.
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -36,7 +37,7 @@ struct Shape {
                               ML_AT = RANGE_AT + 32, TREE_AT = ML_AT + 64 * 2 * 4;
     static constexpr uint32_t SMEM = TREE_AT, SMEM_TREE = TREE_AT + TREE_MOST * 8 + MB * (TREE_MOST / 8);
     static constexpr int PITCH = D + 8;  // floats of a query row on the way out
-    static_assert(64 * PITCH * 4 <= STAGES * STAGE, "the sums leave through the stages");
+    static_assert(64 * PITCH * 4 <= STAGES * STAGE && (WM == 4 || (64 * PITCH + MB * (D + 2)) * 4 <= STAGES * STAGE), "the sums leave through the stages");
     static constexpr int CTAS = D == 256 ? 1 : 2;
     static_assert(SMEM_TREE <= 227 * 1024, "shared memory of an SM");
 };
@@ -49,7 +50,9 @@ __global__ void __launch_bounds__(ATT_THREADS, Shape<T, D, WM>::CTAS) cache_atte
     extern __shared__ __align__(1024) unsigned char sm[];
     const uint32_t sb = smem_addr(sm);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wm = warp % WM, wn = warp / WM, g = lane >> 2, t4 = lane & 3;
-    const uint32_t head = blockIdx.x % a.n_kv, item = blockIdx.x / a.n_kv;
+    namespace cg = cooperative_groups;
+    const uint32_t cl = WM <= 2 && a.cluster ? a.cluster : 1, of_cluster = blockIdx.x % cl;
+    const uint32_t head = blockIdx.x / cl % a.n_kv, item = blockIdx.x / cl / a.n_kv * cl + of_cluster;
     const CacheSeg* table = a.table ? a.table : tab.s;
     const uint32_t seg = cache_find(a.n_segs, item, [&](uint32_t i) { return table[i].item_begin; });
     const CacheSeg sg = table[seg];
@@ -361,8 +364,12 @@ __global__ void __launch_bounds__(ATT_THREADS, Shape<T, D, WM>::CTAS) cache_atte
                 m[h] == -INFINITY ? make_float2(0.0f, 0.0f) : make_float2(o[i][h * 2] * f, o[i][h * 2 + 1] * f);
     }
     __syncthreads();
-    const bool whole = sg.n_chunks == 1;
+    const bool whole = sg.n_chunks == 1, shared = cl > 1;
     const uint32_t used = min((uint32_t)S::MB, q_rows - row0);
+    // of a cluster: the CTA's own sums, maxima and sums of weights for the others to read
+    float* const s_own = s_o + 64 * S::PITCH;
+    float* const s_own_m = s_own + S::MB * D;
+    float* const s_own_l = s_own_m + S::MB;
     for (uint32_t i = tid; i < used * (D / 4); i += ATT_THREADS) {
         const uint32_t r = i / (D / 4), c = i % (D / 4) * 4, row = row0 + r;
         if (c >= a.d) continue;
@@ -378,7 +385,10 @@ __global__ void __launch_bounds__(ATT_THREADS, Shape<T, D, WM>::CTAS) cache_atte
             const float4 y = *reinterpret_cast<const float4*>(s_o + (w * S::MB + r) * S::PITCH + c);
             x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
         }
-        if (whole) {
+        if (shared) {
+            *reinterpret_cast<float4*>(s_own + r * D + c) = x;
+            if (c == 0) s_own_m[r] = top, s_own_l[r] = sum;
+        } else if (whole) {
             const uint64_t tok = sg.query_begin + row / a.group;
             const uint32_t qh = head * a.group + row % a.group;
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -392,6 +402,33 @@ __global__ void __launch_bounds__(ATT_THREADS, Shape<T, D, WM>::CTAS) cache_atte
             if (c == 0) a.part_ml[at * 2] = top, a.part_ml[at * 2 + 1] = sum;
         }
     }
+    if (!shared) return;
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    for (uint32_t i = of_cluster * ATT_THREADS + tid; i < used * (D / 4); i += cl * ATT_THREADS) {
+        const uint32_t r = i / (D / 4), c = i % (D / 4) * 4, row = row0 + r;
+        if (c >= a.d) continue;
+        float top = -INFINITY, sum = 0.0f;
+        for (uint32_t p = 0; p < cl; ++p) top = fmaxf(top, cluster.map_shared_rank(s_own_m, p)[r]);
+        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (uint32_t p = 0; p < cl; ++p) {
+            const float mp = cluster.map_shared_rank(s_own_m, p)[r], f = mp == -INFINITY ? 0.0f : exp2_fast(mp - top);
+            const float4 y = *reinterpret_cast<const float4*>(cluster.map_shared_rank(s_own, p) + r * D + c);
+            sum = fmaf(f, cluster.map_shared_rank(s_own_l, p)[r], sum);
+            x.x = fmaf(f, y.x, x.x);
+            x.y = fmaf(f, y.y, x.y);
+            x.z = fmaf(f, y.z, x.z);
+            x.w = fmaf(f, y.w, x.w);
+        }
+        const uint64_t tok = sg.query_begin + row / a.group;
+        const uint32_t qh = head * a.group + row % a.group;
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        unsigned char* dst = static_cast<unsigned char*>(a.out) + (tok * a.ots + qh * a.ohs + c) * sizeof(T);
+        if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
+        else *reinterpret_cast<float4*>(dst) = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+        if (a.lse && c == 0) a.lse[tok * a.n_heads + qh] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * LN2;
+    }
+    cluster.sync();  // (the others have read this CTA's sums)
 }
 
 // Joins the parts of query rows whose segment's rows were split.  WARPS warps a query row: each takes every WARPS-th part, their sums meet in shared memory in the warps' order.
@@ -480,25 +517,26 @@ __global__ void __launch_bounds__(JOIN_THREADS) cache_join_kernel(const __grid_c
 
 }  // namespace
 static uint64_t blocks_of(const CacheSeg& s, uint32_t group, uint32_t mb) { return ((uint64_t)s.n_queries * group + mb - 1) / mb; }
-void cache_cut(CacheWork* w, uint32_t group, uint32_t mb, uint32_t kt, uint32_t most) {
+static void cut(CacheWork* w, uint32_t group, uint32_t mb, uint32_t kt, uint32_t most, uint32_t cluster) {
     w->items = w->blocks = 0;
     w->chunks = 1;
     for (CacheSeg& c : w->segs) {
         const uint32_t tiles = std::max(1u, (uint32_t)(((uint64_t)c.n_rows + kt - 1) / kt));
         const uint64_t blocks = blocks_of(c, group, mb);
-        c.n_chunks = (tiles + most - 1) / most;
+        c.n_chunks = cluster ? cluster : (tiles + most - 1) / most;
         c.chunk_tiles = (tiles + c.n_chunks - 1) / c.n_chunks;
-        c.n_chunks = (tiles + c.chunk_tiles - 1) / c.chunk_tiles;
+        if (!cluster) c.n_chunks = (tiles + c.chunk_tiles - 1) / c.chunk_tiles;
         c.item_begin = (uint32_t)w->items;
         c.block_begin = (uint32_t)w->blocks;
         w->items += blocks * c.n_chunks;
-        if (c.n_chunks > 1) w->blocks += blocks;
+        if (c.n_chunks > 1 && !cluster) w->blocks += blocks;
         w->chunks = std::max(w->chunks, c.n_chunks);
     }
 }
 // The longest run of tiles of an item.  In units of a tile's time: what fits on the GPU at once takes as long as its longest item, more than that the mean load
 // and half an item at the end; an item costs about four tiles to begin, joining about three and a little for every part.
-uint32_t cache_longest_run(const CacheWork& w, uint32_t group, uint32_t mb, uint32_t kt, uint32_t n_kv, uint32_t slots) {
+// *cluster: how many CTAs share a block of query rows and join their sums through each other's shared memory, where that takes less time than a second kernel (0: none do).
+static uint32_t longest_run(const CacheWork& w, uint32_t group, uint32_t mb, uint32_t kt, uint32_t n_kv, uint32_t slots, bool clusters, uint32_t* cluster) {
     uint32_t most = 1;
     double total = 0.0;
     for (const CacheSeg& c : w.segs) {
@@ -519,6 +557,15 @@ uint32_t cache_longest_run(const CacheWork& w, uint32_t group, uint32_t mb, uint
         if (time < best_time) best_time = time, best = run;
         if (run <= 2) break;
     }
+    *cluster = 0;
+    if (clusters)
+        for (uint32_t cl = 2; cl <= 8; cl *= 2) {
+            double items = 0.0;
+            for (const CacheSeg& c : w.segs) items += (double)blocks_of(c, group, mb) * cl * n_kv;
+            const uint32_t run = (most + cl - 1) / cl;
+            const double time = (items <= slots ? run : total / slots + 0.5 * run) + 4.0 * std::ceil(items / slots) + 0.5;
+            if (time < best_time) best_time = time, *cluster = cl;
+        }
     return best;
 }
 
@@ -559,7 +606,8 @@ template <typename T, int D, int WM>
 Status launch_class(Ctx* c, CacheArgs a, CacheWork w) {
     using S = Shape<T, D, WM>;
     const uint32_t slots = (uint32_t)sm_count(c->device) * S::CTAS;
-    cache_cut(&w, a.group, S::MB, S::KT, cache_longest_run(w, a.group, S::MB, S::KT, a.n_kv, slots));
+    const uint32_t run = longest_run(w, a.group, S::MB, S::KT, a.n_kv, slots, WM <= 2, &a.cluster);
+    cut(&w, a.group, S::MB, S::KT, run, a.cluster);
     if (w.items * a.n_kv > 0x7FFFFFFFull) return Status(SLHA_ERR_CAPACITY, "attention over a cache: too many blocks of query rows");
     CacheTable tab;
     SLHA_TRY(cache_table(c, w.segs, &tab, &a.table));
@@ -568,7 +616,7 @@ Status launch_class(Ctx* c, CacheArgs a, CacheWork w) {
     SLHA_TRY(cache_part_memory(&a, w, S::MB, &mem));
     const size_t smem = a.tree ? S::SMEM_TREE : S::SMEM;
     SLHA_TRY((cache_smem<cache_attend_kernel<T, D, WM>>(c, S::SMEM_TREE)));
-    SLHA_CUDA(launch_behind(cache_attend_kernel<T, D, WM>, dim3((uint32_t)(w.items * a.n_kv)), dim3(ATT_THREADS), smem, c->stream, a, tab));
+    SLHA_CUDA(launch_cluster(cache_attend_kernel<T, D, WM>, dim3((uint32_t)(w.items * a.n_kv)), dim3(ATT_THREADS), smem, c->stream, std::max(a.cluster, 1u), a, tab));
     count_launch();
     if (w.blocks) SLHA_TRY(launch_cache_join(c, a, sizeof(T) == 2 ? SLHA_B200_BF16 : SLHA_B200_F32, w, S::MB));
     return mem.done();

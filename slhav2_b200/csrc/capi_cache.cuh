@@ -5,21 +5,21 @@
 namespace {
 
 // Memory that kernels of the calling thread's device read or write in place.
-Status cache_device_memory(Ctx* c, const void* p, const char* name) {
+Status cache_device_memory(Ctx* c, const void* p, const char* fn, const char* what) {
     cudaPointerAttributes at;
     const bool known = cudaPointerGetAttributes(&at, p) == cudaSuccess;
     if (!known) cudaGetLastError();
     if (!known || (at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged))
-        return Status(SLHA_ERR_DEVICE, std::string(name) + " must be device memory");
+        return Status(SLHA_ERR_DEVICE, std::string(fn) + ": " + what + " must be device memory");
     if (at.type == cudaMemoryTypeDevice && at.device != c->device)
-        return Status(SLHA_ERR_DEVICE, std::string(name) + " lies on another device than the calling thread's");
+        return Status(SLHA_ERR_DEVICE, std::string(fn) + ": " + what + " lies on another device than the calling thread's");
     return Status();
 }
 // Short arrays, host or device; host ones cannot be captured.
 template <typename T>
-Status cache_stage(Ctx* c, const T* p, size_t n, const T** dev, const char* name) {
+Status cache_stage(Ctx* c, const T* p, size_t n, const T** dev, const char* fn, const char* what) {
     if (p && n) {
-        if (is_device_ptr(p)) SLHA_TRY(cache_device_memory(c, p, name));
+        if (is_device_ptr(p)) SLHA_TRY(cache_device_memory(c, p, fn, what));
         else SLHA_TRY(ctx_no_capture(c));
     }
     return stage_in_t(c, p, n, dev);
@@ -30,10 +30,10 @@ void cache_host_segments(const SlhaB200Segment* segments, size_t n, std::vector<
     *on_device = n && is_device_ptr(segments);
     if (n && !*on_device) std::memcpy(out->data(), segments, n * sizeof(SlhaB200Segment));
 }
-Status cache_device_segments(Ctx* c, const SlhaB200Segment* segments, std::vector<SlhaB200Segment>* out, bool on_device) {
+Status cache_device_segments(Ctx* c, const SlhaB200Segment* segments, std::vector<SlhaB200Segment>* out, bool on_device, const char* fn) {
     if (on_device) {
         SLHA_TRY(ctx_no_capture(c));
-        SLHA_TRY(cache_device_memory(c, segments, "segments"));
+        SLHA_TRY(cache_device_memory(c, segments, fn, "segments"));
         SLHA_CUDA(cudaMemcpyAsync(out->data(), segments, out->size() * sizeof(SlhaB200Segment), cudaMemcpyDeviceToHost, c->stream));
         SLHA_CUDA(cudaStreamSynchronize(c->stream));
     }
@@ -43,24 +43,24 @@ Status cache_device_segments(Ctx* c, const SlhaB200Segment* segments, std::vecto
 bool cache_aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 Status cache_check(const SlhaB200KvCache* k, const char* fn, bool with_values) {
-    const std::string name = std::string(fn) + ": ";
-    if (!k->keys || (with_values && !k->values)) return Status(SLHA_ERR_NULL, name + "keys or values are NULL");
-    if (k->dtype != SLHA_B200_F32 && k->dtype != SLHA_B200_BF16) return Status(SLHA_ERR_DIMENSION, name + "dtype must be SLHA_B200_F32 or SLHA_B200_BF16");
+    const auto name = [&](const char* what) { return std::string(fn) + ": " + what; };
+    if (!k->keys || (with_values && !k->values)) return Status(SLHA_ERR_NULL, name("keys or values are NULL"));
+    if (k->dtype != SLHA_B200_F32 && k->dtype != SLHA_B200_BF16) return Status(SLHA_ERR_DIMENSION, name("dtype must be SLHA_B200_F32 or SLHA_B200_BF16"));
     const size_t each = 16 / key_elem_bytes(k->dtype);
     if (k->head_dim == 0 || k->head_dim > CACHE_DIM_MOST || k->head_dim % each)
-        return Status(SLHA_ERR_DIMENSION, name + "head_dim must be a multiple of 16 bytes in 1..256 elements");
-    if (k->n_kv_heads == 0 || k->n_kv_heads > 65535) return Status(SLHA_ERR_DIMENSION, name + "n_kv_heads must be in 1..65535");
+        return Status(SLHA_ERR_DIMENSION, name("head_dim must be a multiple of 16 bytes in 1..256 elements"));
+    if (k->n_kv_heads == 0 || k->n_kv_heads > 65535) return Status(SLHA_ERR_DIMENSION, name("n_kv_heads must be in 1..65535"));
     if (k->key_row_stride % each || k->key_head_stride % each || (with_values && (k->value_row_stride % each || k->value_head_stride % each)))
-        return Status(SLHA_ERR_DIMENSION, name + "row and head strides must be multiples of 16 bytes");
-    if (!cache_aligned(k->keys) || (with_values && !cache_aligned(k->values))) return Status(SLHA_ERR_DIMENSION, name + "keys and values must begin on a multiple of 16 bytes");
+        return Status(SLHA_ERR_DIMENSION, name("row and head strides must be multiples of 16 bytes"));
+    if (!cache_aligned(k->keys) || (with_values && !cache_aligned(k->values))) return Status(SLHA_ERR_DIMENSION, name("keys and values must begin on a multiple of 16 bytes"));
     return Status();
 }
 Status cache_memory(Ctx* c, const SlhaB200KvCache* k, const char* fn, bool with_values) {
-    const std::string name = std::string(fn) + ": ";
-    SLHA_TRY(cache_device_memory(c, k->keys, (name + "keys").c_str()));
-    if (with_values) SLHA_TRY(cache_device_memory(c, k->values, (name + "values").c_str()));
-    if (k->positions) SLHA_TRY(cache_device_memory(c, k->positions, (name + "positions of rows").c_str()));
-    if (k->documents) SLHA_TRY(cache_device_memory(c, k->documents, (name + "documents of rows").c_str()));
+    const auto name = [&](const char* what) { return std::string(fn) + ": " + what; };
+    SLHA_TRY(cache_device_memory(c, k->keys, fn, "keys"));
+    if (with_values) SLHA_TRY(cache_device_memory(c, k->values, fn, "values"));
+    if (k->positions) SLHA_TRY(cache_device_memory(c, k->positions, fn, "positions of rows"));
+    if (k->documents) SLHA_TRY(cache_device_memory(c, k->documents, fn, "documents of rows"));
     return Status();
 }
 // Rows of a table whose last position, index_base + n_tiles - 1, no longer fits.
@@ -72,32 +72,32 @@ Status cache_positions_fit(const std::vector<SlhaB200Segment>& segs, const char*
 }
 
 Status cache_check_queries(const SlhaB200KvCache* k, const SlhaB200CacheQueries* q, const char* fn) {
-    const std::string name = std::string(fn) + ": ";
+    const auto name = [&](const char* what) { return std::string(fn) + ": " + what; };
     const size_t each = 16 / key_elem_bytes(k->dtype);
-    if (!q->q) return Status(SLHA_ERR_NULL, name + "q is NULL");
-    if (q->n_heads == 0 || q->n_heads % k->n_kv_heads) return Status(SLHA_ERR_DIMENSION, name + "n_heads must be a positive multiple of n_kv_heads");
+    if (!q->q) return Status(SLHA_ERR_NULL, name("q is NULL"));
+    if (q->n_heads == 0 || q->n_heads % k->n_kv_heads) return Status(SLHA_ERR_DIMENSION, name("n_heads must be a positive multiple of n_kv_heads"));
     if (q->token_stride % each || q->head_stride % each || !cache_aligned(q->q))
-        return Status(SLHA_ERR_DIMENSION, name + "q must begin on a multiple of 16 bytes and its strides be multiples of 16 bytes");
+        return Status(SLHA_ERR_DIMENSION, name("q must begin on a multiple of 16 bytes and its strides be multiples of 16 bytes"));
     if (!std::isfinite(q->scale) || !std::isfinite(q->softcap) || q->softcap < 0.0f)
-        return Status(SLHA_ERR_NONFINITE, name + "scale must be finite, softcap finite and not negative");
-    if (k->positions && !q->positions) return Status(SLHA_ERR_NULL, name + "the cache's rows have positions, the queries have none");
-    if ((k->documents != nullptr) != (q->documents != nullptr)) return Status(SLHA_ERR_NULL, name + "documents must be given for rows and queries, or for neither");
+        return Status(SLHA_ERR_NONFINITE, name("scale must be finite, softcap finite and not negative"));
+    if (k->positions && !q->positions) return Status(SLHA_ERR_NULL, name("the cache's rows have positions, the queries have none"));
+    if ((k->documents != nullptr) != (q->documents != nullptr)) return Status(SLHA_ERR_NULL, name("documents must be given for rows and queries, or for neither"));
     return Status();
 }
 Status cache_check_segments(const SlhaB200KvCache* k, const std::vector<SlhaB200Segment>& segs, const SlhaB200CacheQueries* q, bool tree, const char* fn) {
-    const std::string name = std::string(fn) + ": ";
+    const auto name = [&](const char* what) { return std::string(fn) + ": " + what; };
     for (const SlhaB200Segment& s : segs) {
-        if ((uint64_t)s.query_begin + s.n_queries > q->n_tokens) return Status(SLHA_ERR_DIMENSION, name + "a segment's query tokens reach beyond n_tokens");
-        if ((uint64_t)s.n_queries * (q->n_heads / k->n_kv_heads) > 0x7FFFFFFFull) return Status(SLHA_ERR_CAPACITY, name + "too many query rows in a segment");
+        if ((uint64_t)s.query_begin + s.n_queries > q->n_tokens) return Status(SLHA_ERR_DIMENSION, name("a segment's query tokens reach beyond n_tokens"));
+        if ((uint64_t)s.n_queries * (q->n_heads / k->n_kv_heads) > 0x7FFFFFFFull) return Status(SLHA_ERR_CAPACITY, name("too many query rows in a segment"));
         if (tree && (s.n_queries > TREE_MOST || s.n_queries > s.n_tiles))
-            return Status(SLHA_ERR_DIMENSION, name + "a segment's drafted tokens are at most 256, and its last rows are theirs");
+            return Status(SLHA_ERR_DIMENSION, name("a segment's drafted tokens are at most 256, and its last rows are theirs"));
     }
     return cache_positions_fit(segs, fn);
 }
 // What attention and observation share: cache and queries into the kernels' arguments.
 Status cache_arguments(Ctx* c, const SlhaB200KvCache* k, size_t n_segs, const SlhaB200CacheQueries* q, const char* fn, CacheArgs* a) {
-    const std::string name = std::string(fn) + ": ";
-    SLHA_TRY(cache_device_memory(c, q->q, (name + "q").c_str()));
+    const auto name = [&](const char* what) { return std::string(fn) + ": " + what; };
+    SLHA_TRY(cache_device_memory(c, q->q, fn, "q"));
     *a = CacheArgs{};
     a->keys = k->keys;
     a->values = k->values;
@@ -111,11 +111,11 @@ Status cache_arguments(Ctx* c, const SlhaB200KvCache* k, size_t n_segs, const Sl
     a->row_pos = k->positions;
     a->row_doc = k->documents;
     a->entry_hs = k->entry_head_stride;
-    SLHA_TRY(cache_stage(c, k->rows, n_segs, &a->rows, "rows"));
-    SLHA_TRY(cache_stage(c, q->positions, q->n_tokens, &a->q_pos, "positions of queries"));
-    SLHA_TRY(cache_stage(c, q->documents, q->n_tokens, &a->q_doc, "documents of queries"));
-    SLHA_TRY(cache_stage(c, q->prefix, n_segs, &a->prefix, "prefix"));
-    SLHA_TRY(cache_stage(c, q->slopes, q->n_heads, &a->slopes, "slopes"));
+    SLHA_TRY(cache_stage(c, k->rows, n_segs, &a->rows, fn, "rows"));
+    SLHA_TRY(cache_stage(c, q->positions, q->n_tokens, &a->q_pos, fn, "positions of queries"));
+    SLHA_TRY(cache_stage(c, q->documents, q->n_tokens, &a->q_doc, fn, "documents of queries"));
+    SLHA_TRY(cache_stage(c, q->prefix, n_segs, &a->prefix, fn, "prefix"));
+    SLHA_TRY(cache_stage(c, q->slopes, q->n_heads, &a->slopes, fn, "slopes"));
     a->n_kv = k->n_kv_heads;
     a->n_heads = q->n_heads;
     a->group = q->n_heads / k->n_kv_heads;
@@ -131,7 +131,7 @@ Status cache_arguments(Ctx* c, const SlhaB200KvCache* k, size_t n_segs, const Sl
 int32_t attend_cache_any(const char* fn, const SlhaB200KvCache* cache, const SlhaB200Segment* segments, size_t n_segments, const SlhaB200CacheQueries* queries,
                          const uint32_t* parents, bool tree, void* out, uint64_t out_token_stride, uint64_t out_head_stride, float* lse_out) {
     return ffi([&]() -> Status {
-        const std::string name = std::string(fn) + ": ";
+        const auto name = [&](const char* what) { return std::string(fn) + ": " + what; };
         if (!cache || !queries || (n_segments && !segments)) return Status(SLHA_ERR_NULL, std::string(fn) + " received a NULL pointer");
         if (n_segments == 0 || queries->n_tokens == 0) return Status();
         if (!out || (tree && !parents)) return Status(SLHA_ERR_NULL, std::string(fn) + " received a NULL pointer");
@@ -139,7 +139,7 @@ int32_t attend_cache_any(const char* fn, const SlhaB200KvCache* cache, const Slh
         SLHA_TRY(cache_check_queries(cache, queries, fn));
         const size_t each = 16 / key_elem_bytes(cache->dtype);
         if (out_token_stride % each || out_head_stride % each || !cache_aligned(out))
-            return Status(SLHA_ERR_DIMENSION, name + "out must begin on a multiple of 16 bytes and its strides be multiples of 16 bytes");
+            return Status(SLHA_ERR_DIMENSION, name("out must begin on a multiple of 16 bytes and its strides be multiples of 16 bytes"));
         std::vector<SlhaB200Segment> segs;
         bool device_segs;
         cache_host_segments(segments, n_segments, &segs, &device_segs);
@@ -147,15 +147,15 @@ int32_t attend_cache_any(const char* fn, const SlhaB200KvCache* cache, const Slh
         CallScope cs;
         if (!cs.ok()) return cs.st;
         Ctx* c = cs.c;
-        SLHA_TRY(cache_device_segments(c, segments, &segs, device_segs));
+        SLHA_TRY(cache_device_segments(c, segments, &segs, device_segs, fn));
         if (device_segs) SLHA_TRY(cache_check_segments(cache, segs, queries, tree, fn));
         SLHA_TRY(cache_memory(c, cache, fn, true));
-        SLHA_TRY(cache_device_memory(c, out, (name + "out").c_str()));
-        if (lse_out) SLHA_TRY(cache_device_memory(c, lse_out, (name + "lse_out").c_str()));
+        SLHA_TRY(cache_device_memory(c, out, fn, "out"));
+        if (lse_out) SLHA_TRY(cache_device_memory(c, lse_out, fn, "lse_out"));
         CacheArgs a;
         SLHA_TRY(cache_arguments(c, cache, n_segments, queries, fn, &a));
         if (tree) {
-            SLHA_TRY(cache_stage(c, parents, queries->n_tokens, &a.parents, "parents"));
+            SLHA_TRY(cache_stage(c, parents, queries->n_tokens, &a.parents, fn, "parents"));
             a.tree = 1;
         }
         a.out = out;
@@ -185,10 +185,10 @@ int32_t slha_b200_observe_cache(const SlhaB200KvCache* cache, const SlhaB200Segm
                                 const float* lse, const float* weights_in, float decay, float* weights_out, uint64_t weight_head_stride) {
     return ffi([&]() -> Status {
         const char* fn = "slha_b200_observe_cache";
-        const std::string name = std::string(fn) + ": ";
+        const auto name = [&](const char* what) { return std::string(fn) + ": " + what; };
         if (!cache || !queries || !lse || !weights_out || (n_segments && !segments)) return Status(SLHA_ERR_NULL, std::string(fn) + " received a NULL pointer");
         if (n_segments == 0) return Status();
-        if (!std::isfinite(decay)) return Status(SLHA_ERR_NONFINITE, name + "decay is not finite");
+        if (!std::isfinite(decay)) return Status(SLHA_ERR_NONFINITE, name("decay is not finite"));
         SLHA_TRY(cache_check(cache, fn, false));
         SLHA_TRY(cache_check_queries(cache, queries, fn));
         std::vector<SlhaB200Segment> segs;
@@ -198,12 +198,12 @@ int32_t slha_b200_observe_cache(const SlhaB200KvCache* cache, const SlhaB200Segm
         CallScope cs;
         if (!cs.ok()) return cs.st;
         Ctx* c = cs.c;
-        SLHA_TRY(cache_device_segments(c, segments, &segs, device_segs));
+        SLHA_TRY(cache_device_segments(c, segments, &segs, device_segs, fn));
         if (device_segs) SLHA_TRY(cache_check_segments(cache, segs, queries, false, fn));
         SLHA_TRY(cache_memory(c, cache, fn, false));
-        SLHA_TRY(cache_device_memory(c, lse, (name + "lse").c_str()));
-        SLHA_TRY(cache_device_memory(c, weights_out, (name + "weights_out").c_str()));
-        if (weights_in) SLHA_TRY(cache_device_memory(c, weights_in, (name + "weights_in").c_str()));
+        SLHA_TRY(cache_device_memory(c, lse, fn, "lse"));
+        SLHA_TRY(cache_device_memory(c, weights_out, fn, "weights_out"));
+        if (weights_in) SLHA_TRY(cache_device_memory(c, weights_in, fn, "weights_in"));
         CacheArgs a;
         SLHA_TRY(cache_arguments(c, cache, n_segments, queries, fn, &a));
         a.lse_in = lse;
@@ -220,26 +220,26 @@ int32_t slha_b200_observe_cache(const SlhaB200KvCache* cache, const SlhaB200Segm
 int32_t slha_b200_evict_cache(const SlhaB200KvCache* cache, const SlhaB200Segment* segments, size_t n_segments, const SlhaB200CacheEviction* ev) {
     return ffi([&]() -> Status {
         const char* fn = "slha_b200_evict_cache";
-        const std::string name = std::string(fn) + ": ";
+        const auto name = [&](const char* what) { return std::string(fn) + ": " + what; };
         if (!cache || !ev || (n_segments && !segments) || (ev && (!ev->weights || (ev->to && !ev->to_segments))))
             return Status(SLHA_ERR_NULL, std::string(fn) + " received a NULL pointer");
         if (n_segments == 0) return Status();
-        if (ev->budget == 0) return Status(SLHA_ERR_DIMENSION, name + "budget must be at least 1");
+        if (ev->budget == 0) return Status(SLHA_ERR_DIMENSION, name("budget must be at least 1"));
         const SlhaB200KvCache* to = ev->to ? ev->to : cache;
         const bool in_place = !ev->to;
         if (to->dtype != cache->dtype || to->head_dim != cache->head_dim || to->n_kv_heads != cache->n_kv_heads)
-            return Status(SLHA_ERR_DIMENSION, name + "both caches must have the same dtype, head_dim and n_kv_heads");
+            return Status(SLHA_ERR_DIMENSION, name("both caches must have the same dtype, head_dim and n_kv_heads"));
         if ((to->positions && !cache->positions) || (to->documents && !cache->documents))
-            return Status(SLHA_ERR_NULL, name + "positions or documents are to be moved, but the rows have none");
+            return Status(SLHA_ERR_NULL, name("positions or documents are to be moved, but the rows have none"));
         if ((to->positions || to->documents) && to->n_kv_heads > 1 && to->entry_head_stride == 0)
-            return Status(SLHA_ERR_DIMENSION, name + "each KV head keeps other rows: positions and documents must be its own where they go (entry_head_stride > 0)");
-        if (ev->tiles && !in_place && !ev->tiles_to) return Status(SLHA_ERR_NULL, name + "tiles are given without tiles_to");
+            return Status(SLHA_ERR_DIMENSION, name("each KV head keeps other rows: positions and documents must be its own where they go (entry_head_stride > 0)"));
+        if (ev->tiles && !in_place && !ev->tiles_to) return Status(SLHA_ERR_NULL, name("tiles are given without tiles_to"));
         if (in_place && ev->weights_to && (ev->weights_to != ev->weights || ev->weights_to_head_stride != ev->weight_head_stride))
-            return Status(SLHA_ERR_DIMENSION, name + "in place, weights_to is the array of weights or NULL");
+            return Status(SLHA_ERR_DIMENSION, name("in place, weights_to is the array of weights or NULL"));
         if (in_place && ev->tiles_to && (ev->tiles_to != ev->tiles || ev->tiles_to_head_stride != ev->tile_head_stride))
-            return Status(SLHA_ERR_DIMENSION, name + "in place, tiles_to is the array of tiles or NULL");
+            return Status(SLHA_ERR_DIMENSION, name("in place, tiles_to is the array of tiles or NULL"));
         SciRustSlhaTile* tiles_to = in_place ? const_cast<SciRustSlhaTile*>(ev->tiles) : ev->tiles_to;
-        if (ev->tiles && (!cache_aligned(ev->tiles) || !cache_aligned(tiles_to))) return Status(SLHA_ERR_DIMENSION, name + "tiles must begin on a multiple of 16 bytes");
+        if (ev->tiles && (!cache_aligned(ev->tiles) || !cache_aligned(tiles_to))) return Status(SLHA_ERR_DIMENSION, name("tiles must begin on a multiple of 16 bytes"));
         SLHA_TRY(cache_check(cache, fn, true));
         if (!in_place) SLHA_TRY(cache_check(to, fn, true));
         std::vector<SlhaB200Segment> segs, to_segs;
@@ -250,26 +250,26 @@ int32_t slha_b200_evict_cache(const SlhaB200KvCache* cache, const SlhaB200Segmen
             SLHA_TRY(cache_positions_fit(segs, fn));
             for (size_t i = 0; i < to_segs.size(); ++i)
                 if (to_segs[i].n_tiles < std::min(segs[i].n_tiles, ev->budget))
-                    return Status(SLHA_ERR_CAPACITY, name + "segment " + std::to_string(i) + " of the other cache has no room for the rows that stay");
+                    return Status(SLHA_ERR_CAPACITY, name("segment ") + std::to_string(i) + " of the other cache has no room for the rows that stay");
             return Status();
         };
         if (!device_segs && !device_to) SLHA_TRY(check_segments());
         CallScope cs;
         if (!cs.ok()) return cs.st;
         Ctx* c = cs.c;
-        SLHA_TRY(cache_device_segments(c, segments, &segs, device_segs));
-        if (!in_place) SLHA_TRY(cache_device_segments(c, ev->to_segments, &to_segs, device_to));
+        SLHA_TRY(cache_device_segments(c, segments, &segs, device_segs, fn));
+        if (!in_place) SLHA_TRY(cache_device_segments(c, ev->to_segments, &to_segs, device_to, fn));
         if (device_segs || device_to) SLHA_TRY(check_segments());
         SLHA_TRY(cache_memory(c, cache, fn, true));
         if (!in_place) SLHA_TRY(cache_memory(c, to, fn, true));
-        SLHA_TRY(cache_device_memory(c, ev->weights, (name + "weights").c_str()));
-        if (ev->weights_to) SLHA_TRY(cache_device_memory(c, ev->weights_to, (name + "weights_to").c_str()));
+        SLHA_TRY(cache_device_memory(c, ev->weights, fn, "weights"));
+        if (ev->weights_to) SLHA_TRY(cache_device_memory(c, ev->weights_to, fn, "weights_to"));
         if (ev->tiles) {
-            SLHA_TRY(cache_device_memory(c, ev->tiles, (name + "tiles").c_str()));
-            SLHA_TRY(cache_device_memory(c, tiles_to, (name + "tiles_to").c_str()));
+            SLHA_TRY(cache_device_memory(c, ev->tiles, fn, "tiles"));
+            SLHA_TRY(cache_device_memory(c, tiles_to, fn, "tiles_to"));
         }
-        if (ev->source_out) SLHA_TRY(cache_device_memory(c, ev->source_out, (name + "source_out").c_str()));
-        if (ev->rows_out) SLHA_TRY(cache_device_memory(c, ev->rows_out, (name + "rows_out").c_str()));
+        if (ev->source_out) SLHA_TRY(cache_device_memory(c, ev->source_out, fn, "source_out"));
+        if (ev->rows_out) SLHA_TRY(cache_device_memory(c, ev->rows_out, fn, "rows_out"));
         EvictArgs a{};
         const uint64_t e = key_elem_bytes(cache->dtype);
         a.keys = cache->keys;
@@ -298,7 +298,7 @@ int32_t slha_b200_evict_cache(const SlhaB200KvCache* cache, const SlhaB200Segmen
         a.to_tiles = reinterpret_cast<unsigned char*>(tiles_to);
         a.tile_hs = ev->tile_head_stride;
         a.to_tile_hs = in_place ? ev->tile_head_stride : ev->tiles_to_head_stride;
-        SLHA_TRY(cache_stage(c, cache->rows, n_segments, &a.rows, "rows"));
+        SLHA_TRY(cache_stage(c, cache->rows, n_segments, &a.rows, fn, "rows"));
         a.rows_out = ev->rows_out;
         a.source = ev->source_out;
         a.n_kv = cache->n_kv_heads;
