@@ -48,14 +48,11 @@ __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], 
     asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t tf32_of(float x) {
-    uint32_t u;
-    asm("cvt.rna.tf32.f32 %0, %1;\n" : "=r"(u) : "f"(x));
-    return u;
-}
+// x as the nearest number of 11 bits (ties away from zero) and the exact rest, of which the products take the first 11 bits.  (In integers: cvt.rna.tf32 takes three
+// instructions, two of them with the rest's made this kernel's largest part.)  An infinity's rest is NaN.
 __device__ __forceinline__ void tf32_split(float x, uint32_t& hi, uint32_t& lo) {
-    hi = tf32_of(x);
-    lo = tf32_of(x - __uint_as_float(hi));
+    hi = (__float_as_uint(x) + 0x1000u) & 0xFFFFE000u;
+    lo = __float_as_uint(x - __uint_as_float(hi));
 }
 __device__ __forceinline__ void mma_f32(float (&d)[4], const uint32_t (&ah)[4], const uint32_t (&al)[4], float b0, float b1) {
     uint32_t bh0, bl0, bh1, bl1;

@@ -138,11 +138,21 @@ __global__ void __launch_bounds__(Obs<D, MANY>::THREADS, Obs<D, MANY>::CTAS)
         const bool bent = has_cap || has_slope;
         bool alone = false;  // a wait ran out: this warp goes on with dot products of its own
         uint32_t use = 0;
-        for (uint32_t j = first_tile; j < end_tile; ++j) {
+        // what a key brings along, fetched while the tile before its own is summed
+        uint32_t next_kp = 0, next_kd = 0;
+        float next_w = 0.0f;
+        const auto ahead = [&](uint32_t j) {
             const uint32_t row = j * KT + k_row, there = min(row, n - 1);
+            next_kp = has_pos ? a.row_pos[entry + there] : sg.base + there;
+            if (has_doc) next_kd = a.row_doc[entry + there];
+            if (a.w_in && quarter == 0 && row < n) next_w = a.w_in[head * a.w_hs + sg.row_begin + row];
+        };
+        ahead(first_tile);
+        for (uint32_t j = first_tile; j < end_tile; ++j) {
+            const uint32_t row = j * KT + k_row, there = min(row, n - 1), kp = next_kp, kd = next_kd;
             const uint64_t at = head * a.w_hs + sg.row_begin + row;
-            const uint32_t kp = has_pos ? a.row_pos[entry + there] : sg.base + there, kd = has_doc ? a.row_doc[entry + there] : 0u;
-            const float before = a.w_in && quarter == 0 && row < n ? a.w_in[at] : 0.0f, k_at = (float)((long long)kp - (long long)near_pos);
+            const float before = next_w, k_at = (float)((long long)kp - (long long)near_pos);
+            if (j + 1 < end_tile) ahead(j + 1);
             float sum = 0.0f;
             if (visited(j)) {
                 // whether all query rows see the warp's keys
