@@ -32,7 +32,7 @@ struct Wide {
     static constexpr uint32_t TILE = HALVES * HALF;
     static constexpr uint32_t K_AT = 2 * TILE, V_AT = 4 * TILE, META_AT = 6 * TILE;   // META: 4 x (positions, documents, distances) of a key tile
     static constexpr uint32_t LIST_AT = META_AT + 4 * 3 * KT * 4, CLS_AT = LIST_AT + RUN_MOST * 4, ROWS_AT = CLS_AT + RUN_MOST;  // ROWS: offset in q (64 bits), position, document, slope, token
-    static constexpr uint32_t RANGE_AT = ROWS_AT + 6 * MB * 4, BAR_AT = RANGE_AT + 64, TREE_AT = BAR_AT + 256;
+    static constexpr uint32_t RANGE_AT = ROWS_AT + 6 * MB * 4, ITEM_AT = RANGE_AT + 64, BAR_AT = ITEM_AT + 256, TREE_AT = BAR_AT + 256;
     static constexpr uint32_t SMEM = TREE_AT + 1024, SMEM_TREE = SMEM + TREE_MOST * 8 + MB * (TREE_MOST / 8);
     static_assert(SMEM_TREE <= 227 * 1024, "shared memory of an SM");
 };
@@ -58,6 +58,8 @@ struct Item {
     uint32_t head, item, row0, q_rows, n, ctx;
     CacheSight sight;
     uint64_t entry;
+    uint32_t near_pos;                // where distances are taken from, so that those of rows nearby are exact in float32
+    bool two, arrays, drafts_listed;  // both tiles of query rows; positions or documents of the rows' own; drafted rows whose positions count
 };
 
 // A query row's result: to the outputs, or as the part of a split segment.
@@ -131,6 +133,119 @@ __device__ __noinline__ void by_rows(const CacheArgs& a, const Item& w, const ui
     }
 }
 
+// A tile's scores that are more than products: capped, biased, masked.  Read from TMEM and written back in units of log 2, 32 columns at a time.  (A function, in loops that are not
+// unrolled, so that the loop over the tiles stays short: where the same stood in it, every tile's weights took 15 % longer.)  Where not all rows are seen, the values are looked over
+// too.  False where a wait ran out.
+template <int D>
+__device__ __noinline__ bool bend_tile(const CacheArgs& a, unsigned char* sm, uint32_t ts, uint32_t r, uint32_t t, uint32_t li) {
+    using S = Wide<D>;
+    const Item& w = *reinterpret_cast<const Item*>(sm + S::ITEM_AT);
+    const uint32_t* const s_qp = reinterpret_cast<const uint32_t*>(sm + S::ROWS_AT) + 2 * MB;
+    const uint32_t bars = smem_addr(sm) + S::BAR_AT;
+    const auto bar = [&](int which) { return bars + which * 8; };
+    const uint32_t what = reinterpret_cast<const uint32_t*>(sm + S::LIST_AT)[li], first = (what >> 2) * KT, n = w.n, ctx = w.ctx;
+    const bool all = what >> t & 1, has_slope = a.slopes, drafts = a.tree && first + KT > ctx;
+    const bool by_pos = a.row_pos || (w.drafts_listed && drafts), listed = !all && (w.arrays || (w.drafts_listed && drafts));  // the fetching warp has left the rows' positions
+    if ((has_slope || listed) && !__all_sync(0xFFFFFFFFu, bar_wait(bar(META_FULL + (li & 3)), li >> 2 & 1))) return false;
+    const uint4* kp4 = reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(sm + S::META_AT) + (li & 3) * 3 * KT);
+    const uint32_t qp = s_qp[r], qd = s_qp[MB + r];
+    const float slope = __uint_as_float(s_qp[2 * MB + r]), q_at = (float)((long long)qp - (long long)w.near_pos);
+    const uint32_t* anc = reinterpret_cast<const uint32_t*>(sm + S::TREE_AT) + 2 * TREE_MOST + (a.tree ? s_qp[3 * MB + r] * (TREE_MOST / 32) : 0u);
+    const CacheSight sight = w.sight;
+    const bool has_cap = a.cap > 0.0f;
+    const float to_log2 = has_cap ? a.scale / a.cap : a.scale * LOG2E, cap2 = a.cap * LOG2E;
+    // positions one after another: what is seen are one or two runs
+    const long long at = (long long)w.sg.base + first;
+    const long long low = (long long)qp - sight.window_last - at, high = (sight.causal ? (long long)qp : (long long)qp + sight.window_last) - at + 1;
+    const int lo = (int)max(0ll, min(low, 128ll)), hi = (int)max(0ll, min(high, 128ll)), pre = (int)max(0ll, min((long long)sight.prefix - at, 128ll)), inside = (int)min(n - first, 128u);
+#pragma unroll 1
+    for (int j = 0; j < 4; ++j) {
+        uint32_t u[32];
+        float* s = reinterpret_cast<float*>(u);
+        tmem_ld32(ts + 32 * j, u);
+        tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < 32; ++c) asm volatile("" : "+r"(u[c]));
+        if (has_cap) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c) {
+                const float x = s[c] * to_log2;
+                // tanh x = 1 - 2 / (exp(2 x) + 1) where the polynomial ends
+                s[c] = fabsf(x) <= 1.0f ? cap2 * tanh_small(x) : fmaf(-2.0f * cap2, __fdividef(1.0f, exp2_fast(x * (2.0f * LOG2E)) + 1.0f), cap2);
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < 32; ++c) s[c] *= to_log2;
+        }
+        if (has_slope) {
+#pragma unroll
+            for (int c = 0; c < 32; c += 4) {
+                const float4 k = *reinterpret_cast<const float4*>(kp4 + KT / 2 + j * 8 + c / 4);
+                s[c] = fmaf(-slope, fabsf(q_at - k.x), s[c]);
+                s[c + 1] = fmaf(-slope, fabsf(q_at - k.y), s[c + 1]);
+                s[c + 2] = fmaf(-slope, fabsf(q_at - k.z), s[c + 2]);
+                s[c + 3] = fmaf(-slope, fabsf(q_at - k.w), s[c + 3]);
+            }
+        }
+        if (!all) {
+            uint32_t seen = 0;  // bits of the rows that this query row sees
+            if (by_pos) {
+#pragma unroll 2
+                for (int g = 0; g < 8; ++g) {
+                    const uint4 p = kp4[j * 8 + g];
+                    seen |= ((sight.sees(qp, p.x) ? 1u : 0u) | (sight.sees(qp, p.y) ? 2u : 0u) | (sight.sees(qp, p.z) ? 4u : 0u) | (sight.sees(qp, p.w) ? 8u : 0u)) << g * 4;
+                }
+            } else if (drafts) {  // (no window: what comes before the drafted rows is seen)
+                seen = low_bits((int)ctx - (int)first - 32 * j);
+            } else {
+                seen = (low_bits(hi - 32 * j) & ~low_bits(lo - 32 * j)) | low_bits(pre - 32 * j);
+            }
+            if (a.row_doc) {
+                uint32_t bits = 0;
+#pragma unroll 4
+                for (int g = 0; g < 8; ++g) {
+                    const uint4 d = kp4[KT / 4 + j * 8 + g];
+                    bits |= ((d.x == qd ? 1u : 0u) | (d.y == qd ? 2u : 0u) | (d.z == qd ? 4u : 0u) | (d.w == qd ? 8u : 0u)) << g * 4;
+                }
+                seen &= bits;
+            }
+            if (drafts) {  // of the drafted rows only itself and its ancestors
+                const int from = (int)first + 32 * j - (int)ctx;  // the word's first row, counted among the drafted
+                const uint32_t before = low_bits(-from);
+                uint32_t line = 0;
+                if (from > -32 && from < (int)TREE_MOST) {
+                    const int word = from >> 5, off = from & 31;  // (word -1: the rows before)
+                    const uint32_t l = word >= 0 ? anc[word] : 0u, h = word + 1 < (int)(TREE_MOST / 32) ? anc[word + 1] : 0u;
+                    line = __funnelshift_r(l, h, off);
+                }
+                seen = w.drafts_listed ? seen & (before | line) : (seen & before) | (line & ~before);
+            }
+            seen &= low_bits(inside - 32 * j);
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+                if (!(seen >> c & 1u)) s[c] = -INFINITY;
+        }
+        __syncwarp();
+        tmem_st16(ts + 32 * j, u);
+        tmem_st16(ts + 32 * j + 16, u + 16);
+    }
+    tmem_wait_st();
+    if (!all) {
+        // values of a tile that not all see (where both tiles of query rows see a part of it, each looks at a half)
+        if (!__all_sync(0xFFFFFFFFu, bar_wait(bar(V_FULL + (li & 1)), li >> 1 & 1))) return false;
+        const bool share = w.two && !(what & 3u);
+        uint32_t odd = 0;
+#pragma unroll 4
+        for (uint32_t i = share ? r : r & 127; i < S::TILE / 16; i += share ? 256 : 128) {
+            const uint4 x = *reinterpret_cast<const uint4*>(sm + S::V_AT + (li & 1) * S::TILE + i * 16);
+            odd |= odd_pair(x.x) | odd_pair(x.y) | odd_pair(x.z) | odd_pair(x.w);
+        }
+        if (odd & 0x80008000u) *reinterpret_cast<volatile uint32_t*>(sm + S::BAR_AT + ODD_WORD * 8) = 1u;
+    }
+    __syncwarp();
+    return true;
+}
+
 // CAP: scores are capped.  RICH: rows with positions or documents of their own, tokens with positions of their own, trees, or a distance bias.  (Instances of their own: what a
 // kernel does not need costs it registers and instruction cache in the loop over the tiles; with all in one, 8192 tokens of 32 heads took 937 us, alone 876.)
 template <int D, bool CAP, bool RICH>
@@ -185,6 +300,12 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
 
     const bool arrays = has_pos || has_doc, drafts_listed = is_tree && (arrays || a.q_pos || sight.window_last != 0xFFFFFFFFu);  // drafted rows whose positions count
     const bool plain = !RICH || (!arrays && !is_tree && !a.q_pos);  // all positions follow from the segment: the fetching warp finds the tiles alone
+    const uint32_t near_pos = a.q_pos ? a.q_pos[w.sg.query_begin + tok0] : w.sg.base + w.ctx + (is_tree ? 0u : tok0);
+    w.near_pos = near_pos;
+    w.two = two;
+    w.arrays = arrays;
+    w.drafts_listed = drafts_listed;
+    if (tid == 0) *reinterpret_cast<Item*>(sm + S::ITEM_AT) = w;
     uint32_t cnt = 0;
     if (warp == FETCH_WARP) {
         if (lane == 0) {
@@ -387,7 +508,6 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
     __syncthreads();
     tc_after();
     const uint32_t tmem = *s_tmem;  // (read by all warps alike: with a value of its own for one of them, the compiler issued each product in a loop over the lanes)
-    const uint32_t near_pos = plain ? w.sg.base + w.ctx + tok0 : s_qp[0];  // distances are taken from here, so that those of rows nearby are exact in float32
     bool fail = false;
 
     if (warp < 8) {
@@ -397,9 +517,6 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
         if (t == 0 || two) {
             const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21), ts = lanes + t * 128, to = lanes + 256 + t * 128;
             const float to_log2 = has_cap ? a.scale / a.cap : a.scale * LOG2E, cap2 = a.cap * LOG2E;
-            const uint32_t qp = s_qp[r], qd = s_qd[r], n = w.n, ctx = w.ctx, base = w.sg.base;
-            const float slope = s_slope[r], q_at = (float)((long long)qp - (long long)near_pos);
-            const uint32_t* anc = s_anc + s_tok[r] * (TREE_MOST / 32);
             float m = -INFINITY, l = 0.0f;
             for (uint32_t li = 0; li < cnt; ++li) {
                 if (!__all_sync(0xFFFFFFFFu, bar_wait(bar(S_FULL + t), li & 1))) {
@@ -407,18 +524,25 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
                     break;
                 }
                 tc_after();
-                const uint32_t what = s_list[li], first = (what >> 2) * KT;
-                const bool all = what >> t & 1;
+                const bool all = s_list[li] >> t & 1;
+                const bool bent = !all || has_slope;
+                if (bent && !bend_tile<D>(a, sm, ts, r, t, li)) {
+                    fail = true;
+                    break;
+                }
                 uint32_t u[128];
                 float* s = reinterpret_cast<float*>(u);
+                const auto load = [&]() {
 #pragma unroll
-                for (int c = 0; c < 128; c += 32) tmem_ld32(ts + c, u + c);
-                tmem_wait_ld();
+                    for (int c = 0; c < 128; c += 32) tmem_ld32(ts + c, u + c);
+                    tmem_wait_ld();
 #pragma unroll
-                for (int c = 0; c < 128; ++c) asm volatile("" : "+r"(u[c]));
-                float mul = to_log2, top;
+                    for (int c = 0; c < 128; ++c) asm volatile("" : "+r"(u[c]));
+                };
+                load();
+                float mul = bent ? 1.0f : to_log2, top;
                 bool fused = false;  // the cap is applied on the way to the weights
-                if (has_cap) {
+                if (CAP && !bent) {
                     float high[2] = {-INFINITY, -INFINITY}, low[2] = {INFINITY, INFINITY};
 #pragma unroll
                     for (int c = 0; c < 128; c += 4)
@@ -428,115 +552,17 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
                             low[e] = fminf(low[e], fminf(s[c + 2 * e], s[c + 2 * e + 1]));
                         }
                     const float x = fmaxf(high[0], high[1]) * to_log2;
-                    const bool small = __all_sync(0xFFFFFFFFu, x <= 1.0f && fminf(low[0], low[1]) * to_log2 >= -1.0f);
-                    fused = small && all && !has_slope;
                     mul = 1.0f;
+                    fused = __all_sync(0xFFFFFFFFu, x <= 1.0f && fminf(low[0], low[1]) * to_log2 >= -1.0f);
                     if (fused) {  // (tanh grows: the largest score is that of the largest product)
                         top = cap2 * tanh_small(x);
-                    } else if (small) {
-                        const uint64_t in = pair(to_log2, to_log2), out = pair(cap2, cap2);
-#pragma unroll
-                        for (int c = 0; c < 128; c += 2) {
-                            const uint64_t y = mul2(pair(s[c], s[c + 1]), in);
-                            unpair(mul2(mul2(y, out), tanh_poly(mul2(y, y))), s[c], s[c + 1]);
-                        }
                     } else {
-#pragma unroll
-                        for (int c = 0; c < 128; ++c) {  // tanh x = 1 - 2 / (exp(2 x) + 1)
-                            const float e = exp2_fast(s[c] * to_log2 * (2.0f * LOG2E));
-                            s[c] = fmaf(-2.0f * cap2, __fdividef(1.0f, e + 1.0f), cap2);
+                        if (!bend_tile<D>(a, sm, ts, r, t, li)) {
+                            fail = true;
+                            break;
                         }
+                        load();
                     }
-                }
-                const bool listed = has_slope || (!all && (arrays || (drafts_listed && first + KT > ctx)));  // the fetching warp has left the rows' positions
-                if (listed && !__all_sync(0xFFFFFFFFu, bar_wait(bar(META_FULL + (li & 3)), li >> 2 & 1))) {
-                    fail = true;
-                    break;
-                }
-                const uint4* kp4 = reinterpret_cast<const uint4*>(s_meta + (li & 3) * 3 * KT);
-                if (has_slope) {
-#pragma unroll
-                    for (int c = 0; c < 128; c += 4) {
-                        const float4 k = *reinterpret_cast<const float4*>(kp4 + KT / 2 + c / 4);
-                        s[c] = fmaf(s[c], mul, -slope * fabsf(q_at - k.x));
-                        s[c + 1] = fmaf(s[c + 1], mul, -slope * fabsf(q_at - k.y));
-                        s[c + 2] = fmaf(s[c + 2], mul, -slope * fabsf(q_at - k.z));
-                        s[c + 3] = fmaf(s[c + 3], mul, -slope * fabsf(q_at - k.w));
-                    }
-                    mul = 1.0f;
-                }
-                if (!all) {
-                    uint32_t seen[4];  // bits of the rows that this query row sees
-                    if (has_pos || (drafts_listed && first + KT > ctx)) {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            seen[j] = 0;
-#pragma unroll 2
-                            for (int g = 0; g < 8; ++g) {
-                                const uint4 p = kp4[j * 8 + g];
-                                seen[j] |= ((sight.sees(qp, p.x) ? 1u : 0u) | (sight.sees(qp, p.y) ? 2u : 0u) | (sight.sees(qp, p.z) ? 4u : 0u) | (sight.sees(qp, p.w) ? 8u : 0u)) << g * 4;
-                            }
-                        }
-                    } else {  // positions one after another: what is seen are one or two runs
-                        const long long at = (long long)base + first;
-                        const long long low = (long long)qp - sight.window_last - at, high = (sight.causal ? (long long)qp : (long long)qp + sight.window_last) - at + 1;
-                        const int lo = (int)max(0ll, min(low, 128ll)), hi = (int)max(0ll, min(high, 128ll)), pre = (int)max(0ll, min((long long)sight.prefix - at, 128ll));
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) seen[j] = (low_bits(hi - 32 * j) & ~low_bits(lo - 32 * j)) | low_bits(pre - 32 * j);
-                        if (is_tree && first + KT > ctx) {  // (no window: what comes before the drafted rows is seen)
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) seen[j] = low_bits((int)ctx - (int)first - 32 * j);
-                        }
-                    }
-                    if (has_doc) {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            uint32_t bits = 0;
-#pragma unroll 4
-                            for (int g = 0; g < 8; ++g) {
-                                const uint4 d = kp4[KT / 4 + j * 8 + g];
-                                bits |= ((d.x == qd ? 1u : 0u) | (d.y == qd ? 2u : 0u) | (d.z == qd ? 4u : 0u) | (d.w == qd ? 8u : 0u)) << g * 4;
-                            }
-                            seen[j] &= bits;
-                        }
-                    }
-                    if (is_tree && first + KT > ctx) {  // of the drafted rows only itself and its ancestors
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int from = (int)first + 32 * j - (int)ctx;  // the word's first row, counted among the drafted
-                            const uint32_t before = low_bits(-from);
-                            uint32_t line = 0;
-                            if (from > -32 && from < (int)TREE_MOST) {
-                                const int word = from >> 5, off = from & 31;  // (word -1: the rows before)
-                                const uint32_t lo = word >= 0 ? anc[word] : 0u, hi = word + 1 < (int)(TREE_MOST / 32) ? anc[word + 1] : 0u;
-                                line = __funnelshift_r(lo, hi, off);
-                            }
-                            seen[j] = drafts_listed ? seen[j] & (before | line) : (seen[j] & before) | (line & ~before);
-                        }
-                    }
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        seen[j] &= low_bits((int)min(n - first, 128u) - 32 * j);
-#pragma unroll
-                        for (int c = 0; c < 32; ++c)
-                            if (!(seen[j] >> c & 1u)) s[32 * j + c] = -INFINITY;
-                    }
-                    // values of a tile that not all see
-                    if (!__all_sync(0xFFFFFFFFu, bar_wait(bar(V_FULL + (li & 1)), li >> 1 & 1))) {
-                        fail = true;
-                        break;
-                    }
-                    // (where both tiles of query rows see a part of it, each looks at a half)
-                    const bool share = two && !(what & 3u);
-                    uint32_t odd = 0;
-#pragma unroll 4
-                    for (uint32_t i = share ? tid : tid & 127; i < S::TILE / 16; i += share ? 256 : 128) {
-                        const uint4 x = *reinterpret_cast<const uint4*>(sm + S::V_AT + (li & 1) * S::TILE + i * 16);
-                        odd |= odd_pair(x.x) | odd_pair(x.y) | odd_pair(x.z) | odd_pair(x.w);
-                    }
-                    odd &= 0x80008000u;
-                    if (odd) *s_odd = 1u;
-                    __syncwarp();
                 }
                 if (!fused) {
                     float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -594,8 +620,12 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
                         }
                     }
                 };
-                if (fused) weights(std::true_type());
-                else weights(std::false_type());
+                if constexpr (CAP) {
+                    if (fused) weights(std::true_type());
+                    else weights(std::false_type());
+                } else {
+                    weights(std::false_type());
+                }
                 {
                     float x, y;
                     unpair(add2(sum_a, sum_b), x, y);
@@ -786,8 +816,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
     if (warp >= 8) regs_more<REGS_ALL>();
     if (warp == MMA_WARP) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512u) : "memory");
     if (*s_odd) {
-        const Item again = w;
-        by_rows(a, again, s_qp, s_qd, s_slope, s_tok, s_depth, s_anc, s_list, cnt);
+        by_rows(a, *reinterpret_cast<const Item*>(sm + S::ITEM_AT), s_qp, s_qd, s_slope, s_tok, s_depth, s_anc, s_list, cnt);
     }
 }
 
