@@ -20,7 +20,7 @@ namespace slha {
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-constexpr int THREADS = 384, WARPS = THREADS / 32, KT = 128, MB = 256, MMA_WARP = 8, FETCH_WARP = 9;
+constexpr int THREADS = 384, WARPS = THREADS / 32, KT = 128, MB = 256, MMA_WARP = 8, FETCH_WARP = 9;  // (the last two look over values)
 // Registers a thread: 168 for all at the launch; the two warpgroups that hold a row of scores take 200, the third (two of its warps idle) gives them up: 2 x 200 + 104 = 3 x 168.
 constexpr int REGS_ALL = 168, REGS_ROWS = 200, REGS_REST = 104;
 constexpr uint32_t RUN_MOST = 1024;           // key tiles of an item
@@ -59,7 +59,7 @@ struct Item {
     CacheSight sight;
     uint64_t entry;
     uint32_t near_pos;                // where distances are taken from, so that those of rows nearby are exact in float32
-    bool two, arrays, drafts_listed;  // both tiles of query rows; positions or documents of the rows' own; drafted rows whose positions count
+    bool arrays, drafts_listed;  // positions or documents of the rows' own; drafted rows whose positions count
 };
 
 // A query row's result: to the outputs, or as the part of a split segment.
@@ -133,9 +133,9 @@ __device__ __noinline__ void by_rows(const CacheArgs& a, const Item& w, const ui
     }
 }
 
-// A tile's scores that are more than products: capped, biased, masked.  Read from TMEM and written back in units of log 2, 32 columns at a time.  (A function, in loops that are not
-// unrolled, so that the loop over the tiles stays short: where the same stood in it, every tile's weights took 15 % longer.)  Where not all rows are seen, the values are looked over
-// too.  False where a wait ran out.
+// A tile's scores that are more than products: capped, biased, masked.  Read from TMEM and written back, 32 columns at a time, in units of log 2 where a cap or a distance bends them; where
+// all that a warp's rows see of 32 columns is all, they stay as they are.  (A function, in loops that are hardly
+// unrolled, so that the loop over the tiles stays short: where the same stood in it, every tile's weights took 15 % longer.)  False where a wait ran out.
 template <int D>
 __device__ __noinline__ bool bend_tile(const CacheArgs& a, unsigned char* sm, uint32_t ts, uint32_t r, uint32_t t, uint32_t li) {
     using S = Wide<D>;
@@ -152,7 +152,7 @@ __device__ __noinline__ bool bend_tile(const CacheArgs& a, unsigned char* sm, ui
     const float slope = __uint_as_float(s_qp[2 * MB + r]), q_at = (float)((long long)qp - (long long)w.near_pos);
     const uint32_t* anc = reinterpret_cast<const uint32_t*>(sm + S::TREE_AT) + 2 * TREE_MOST + (a.tree ? s_qp[3 * MB + r] * (TREE_MOST / 32) : 0u);
     const CacheSight sight = w.sight;
-    const bool has_cap = a.cap > 0.0f;
+    const bool has_cap = a.cap > 0.0f, bends = has_cap || has_slope;
     const float to_log2 = has_cap ? a.scale / a.cap : a.scale * LOG2E, cap2 = a.cap * LOG2E;
     // positions one after another: what is seen are one or two runs
     const long long at = (long long)w.sg.base + first;
@@ -160,35 +160,9 @@ __device__ __noinline__ bool bend_tile(const CacheArgs& a, unsigned char* sm, ui
     const int lo = (int)max(0ll, min(low, 128ll)), hi = (int)max(0ll, min(high, 128ll)), pre = (int)max(0ll, min((long long)sight.prefix - at, 128ll)), inside = (int)min(n - first, 128u);
 #pragma unroll 1
     for (int j = 0; j < 4; ++j) {
-        uint32_t u[32];
-        float* s = reinterpret_cast<float*>(u);
-        tmem_ld32(ts + 32 * j, u);
-        tmem_wait_ld();
-#pragma unroll
-        for (int c = 0; c < 32; ++c) asm volatile("" : "+r"(u[c]));
-        if (has_cap) {
-#pragma unroll
-            for (int c = 0; c < 32; ++c) {
-                const float x = s[c] * to_log2;
-                // tanh x = 1 - 2 / (exp(2 x) + 1) where the polynomial ends
-                s[c] = fabsf(x) <= 1.0f ? cap2 * tanh_small(x) : fmaf(-2.0f * cap2, __fdividef(1.0f, exp2_fast(x * (2.0f * LOG2E)) + 1.0f), cap2);
-            }
-        } else {
-#pragma unroll
-            for (int c = 0; c < 32; ++c) s[c] *= to_log2;
-        }
-        if (has_slope) {
-#pragma unroll
-            for (int c = 0; c < 32; c += 4) {
-                const float4 k = *reinterpret_cast<const float4*>(kp4 + KT / 2 + j * 8 + c / 4);
-                s[c] = fmaf(-slope, fabsf(q_at - k.x), s[c]);
-                s[c + 1] = fmaf(-slope, fabsf(q_at - k.y), s[c + 1]);
-                s[c + 2] = fmaf(-slope, fabsf(q_at - k.z), s[c + 2]);
-                s[c + 3] = fmaf(-slope, fabsf(q_at - k.w), s[c + 3]);
-            }
-        }
+        uint32_t seen = 0xFFFFFFFFu;  // bits of the rows that this query row sees
         if (!all) {
-            uint32_t seen = 0;  // bits of the rows that this query row sees
+            seen = 0;
             if (by_pos) {
 #pragma unroll 2
                 for (int g = 0; g < 8; ++g) {
@@ -221,27 +195,55 @@ __device__ __noinline__ bool bend_tile(const CacheArgs& a, unsigned char* sm, ui
                 seen = w.drafts_listed ? seen & (before | line) : (seen & before) | (line & ~before);
             }
             seen &= low_bits(inside - 32 * j);
+        }
+        if (!bends && __all_sync(0xFFFFFFFFu, seen == 0xFFFFFFFFu)) continue;
+        uint32_t u[32];
+        float* s = reinterpret_cast<float*>(u);
+        tmem_ld32(ts + 32 * j, u);
+        tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < 32; ++c) asm volatile("" : "+r"(u[c]));
+        if (has_cap) {
+            float big = 0.0f;
+#pragma unroll
+            for (int c = 0; c < 32; ++c) big = fmaxf(big, fabsf(s[c]));
+            if (__all_sync(0xFFFFFFFFu, big * to_log2 <= 1.0f)) {
+                const uint64_t in = pair(to_log2, to_log2), out = pair(cap2, cap2);
+#pragma unroll
+                for (int c = 0; c < 32; c += 2) {
+                    const uint64_t y = mul2(pair(s[c], s[c + 1]), in);
+                    unpair(mul2(mul2(y, tanh_poly(mul2(y, y))), out), s[c], s[c + 1]);
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < 32; ++c) {  // tanh x = 1 - 2 / (exp(2 x) + 1)
+                    const float e = exp2_fast(s[c] * to_log2 * (2.0f * LOG2E));
+                    s[c] = fmaf(-2.0f * cap2, __fdividef(1.0f, e + 1.0f), cap2);
+                }
+            }
+        } else if (has_slope) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c) s[c] *= to_log2;
+        }
+        if (has_slope) {
+#pragma unroll
+            for (int c = 0; c < 32; c += 4) {
+                const float4 k = *reinterpret_cast<const float4*>(kp4 + KT / 2 + j * 8 + c / 4);
+                s[c] = fmaf(-slope, fabsf(q_at - k.x), s[c]);
+                s[c + 1] = fmaf(-slope, fabsf(q_at - k.y), s[c + 1]);
+                s[c + 2] = fmaf(-slope, fabsf(q_at - k.z), s[c + 2]);
+                s[c + 3] = fmaf(-slope, fabsf(q_at - k.w), s[c + 3]);
+            }
+        }
+        if (!all)
 #pragma unroll
             for (int c = 0; c < 32; ++c)
                 if (!(seen >> c & 1u)) s[c] = -INFINITY;
-        }
         __syncwarp();
         tmem_st16(ts + 32 * j, u);
         tmem_st16(ts + 32 * j + 16, u + 16);
     }
     tmem_wait_st();
-    if (!all) {
-        // values of a tile that not all see (where both tiles of query rows see a part of it, each looks at a half)
-        if (!__all_sync(0xFFFFFFFFu, bar_wait(bar(V_FULL + (li & 1)), li >> 1 & 1))) return false;
-        const bool share = w.two && !(what & 3u);
-        uint32_t odd = 0;
-#pragma unroll 4
-        for (uint32_t i = share ? r : r & 127; i < S::TILE / 16; i += share ? 256 : 128) {
-            const uint4 x = *reinterpret_cast<const uint4*>(sm + S::V_AT + (li & 1) * S::TILE + i * 16);
-            odd |= odd_pair(x.x) | odd_pair(x.y) | odd_pair(x.z) | odd_pair(x.w);
-        }
-        if (odd & 0x80008000u) *reinterpret_cast<volatile uint32_t*>(sm + S::BAR_AT + ODD_WORD * 8) = 1u;
-    }
     __syncwarp();
     return true;
 }
@@ -299,10 +301,9 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
     const uint32_t tok0 = w.row0 / a.group;
 
     const bool arrays = has_pos || has_doc, drafts_listed = is_tree && (arrays || a.q_pos || sight.window_last != 0xFFFFFFFFu);  // drafted rows whose positions count
-    const bool plain = !RICH || (!arrays && !is_tree && !a.q_pos);  // all positions follow from the segment: the fetching warp finds the tiles alone
+    const bool plain = !RICH || (!arrays && !a.q_pos);  // all positions follow from the segment
     const uint32_t near_pos = a.q_pos ? a.q_pos[w.sg.query_begin + tok0] : w.sg.base + w.ctx + (is_tree ? 0u : tok0);
     w.near_pos = near_pos;
-    w.two = two;
     w.arrays = arrays;
     w.drafts_listed = drafts_listed;
     if (tid == 0) *reinterpret_cast<Item*>(sm + S::ITEM_AT) = w;
@@ -313,7 +314,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
                 bar_init(bar(K_FULL + i), 1);
                 bar_init(bar(V_FULL + i), 1);
                 bar_init(bar(K_FREE + i), 1);
-                bar_init(bar(V_FREE + i), 1);
+                bar_init(bar(V_FREE + i), 3);
                 bar_init(bar(S_FULL + i), 1);
                 bar_init(bar(P_HALF + i), 128);
                 bar_init(bar(P_FULL + i), 128);
@@ -339,13 +340,15 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
         // Which tiles are visited, and which of them either tile of query rows sees as a whole.  Of a split segment the item takes its share of them.  Every warp goes through
         // them, so that each knows how many there are; the fetching one writes the list.
         const uint32_t p0 = w.sg.base + w.ctx, last_tok = w.sg.n_queries - 1;
-        const auto pos = [&](uint32_t row) { return p0 + min(row / a.group, last_tok); };
+        // (of a tree's tokens: between the first one's and that of the last in a chain)
+        const auto pos = [&](uint32_t row) { return is_tree ? p0 + (row == w.row0 || row == w.row0 + 128 ? 0u : last_tok) : p0 + min(row / a.group, last_tok); };
         const CacheRanges qa{pos(w.row0), pos(w.row0 + 127), 0u, 0u}, qb{pos(w.row0 + 128), pos(w.row0 + 255), 0u, 0u};
         const auto class_of = [&](uint32_t j) -> uint32_t {
             const uint32_t first = j * KT, last = first + KT - 1;
             if (j >= tiles) return 0u;
             const CacheRanges k{w.sg.base + first, w.sg.base + min(last, w.n - 1), 0u, 0u};
-            const int x = cache_tile_class(k, qa, sight, false, last < w.n), y = cache_tile_class(k, qb, sight, false, last < w.n);
+            const bool drafts = is_tree && last >= w.ctx;
+            const int x = cache_tile_class(k, qa, sight, drafts, last < w.n), y = cache_tile_class(k, qb, sight, drafts, last < w.n);
             return (x || y ? 1u : 0u) | (x == 2 ? 2u : 0u) | (y == 2 ? 4u : 0u);
         };
         uint32_t skip = 0, most = RUN_MOST;
@@ -363,6 +366,34 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
         }
         cnt = met > skip ? min(met - skip, most) : 0u;
         __syncwarp();
+    }
+    const unsigned char* kb = static_cast<const unsigned char*>(a.keys) + (w.sg.row_begin * a.krs + w.head * a.khs) * 2;
+    const unsigned char* vb = static_cast<const unsigned char*>(a.values) + (w.sg.row_begin * a.vrs + w.head * a.vhs) * 2;
+    constexpr int PIECES = S::HALVES * 8;
+    const auto fetch = [&](uint32_t dst, const CUtensorMap* map, bool head_first, const unsigned char* from, uint64_t stride, uint32_t first, uint32_t full) {
+        if (first + KT <= w.n) {
+            if (lane == 0) {
+                const uint32_t row = (uint32_t)w.sg.row_begin + first;
+                bar_expect(full, S::TILE);
+#pragma unroll
+                for (int h = 0; h < S::HALVES; ++h) tma_load(dst + h * HALF, map, h * 64, head_first ? w.head : row, head_first ? row : w.head, full);
+            }
+        } else {
+            for (uint32_t i = lane; i < KT * PIECES; i += 32) {
+                const uint32_t r = i / PIECES, c = i % PIECES, row = first + r;
+                const bool there = row < w.n && c * 8 < a.d;
+                copy16(dst + (c >> 3) * HALF + r * 128 + (((c & 7) ^ (r & 7)) << 4), there ? from + row * stride * 2 + c * 16 : from, there);
+            }
+            copy_commit();
+            copy_wait<0>();
+            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+            __syncwarp();
+            if (lane == 0) bar_arrive(full);
+        }
+    };
+    if (warp == FETCH_WARP && plain && cnt) {  // the first keys, while the others get ready
+        __syncwarp();
+        fetch(sb + S::K_AT, &maps.k, maps.k_head_first, kb, a.krs, (s_list[0] >> 2) * KT, bar(K_FULL));
     }
     if (warp == MMA_WARP) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(bar(TMEM_WORD)), "r"(512u) : "memory");
@@ -441,6 +472,11 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
                     for (int x = 0; x < AT_ONCE; ++x) {
                         const uint32_t first = (first_tile + min(j0 + x * WARPS, in_run - 1)) * KT;
                         k[x] = CacheRanges{0xFFFFFFFFu, 0u, has_doc ? 0xFFFFFFFFu : 0u, 0u};
+                    if (!has_pos) {  // (no token sees a row of them, whatever its document)
+                        const CacheRanges by_place{w.sg.base + first, w.sg.base + min(first + KT - 1, w.n - 1), min(qa.dmin, qb.dmin), max(qa.dmax, qb.dmax)};
+                        const CacheRanges both{min(qa.pmin, qb.pmin), max(qa.pmax, qb.pmax), by_place.dmin, by_place.dmax};
+                        if (!cache_tile_class(by_place, both, sight, is_tree && first + KT > w.ctx, true)) continue;
+                    }
 #pragma unroll
                         for (int e = 0; e < KT / 32; ++e) {
                             const uint32_t i = min(first + lane + e * 32, w.n - 1);
@@ -458,7 +494,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
                         k[x].pmax = __reduce_max_sync(0xFFFFFFFFu, k[x].pmax);
                         k[x].dmin = __reduce_min_sync(0xFFFFFFFFu, k[x].dmin);
                         k[x].dmax = __reduce_max_sync(0xFFFFFFFFu, k[x].dmax);
-                        if (lane == 0 && j < in_run) s_cls[j] = (unsigned char)classes(k[x], (first_tile + j) * KT + KT - 1);
+                        if (lane == 0 && j < in_run) s_cls[j] = k[x].pmin > k[x].pmax ? 0 : (unsigned char)classes(k[x], (first_tile + j) * KT + KT - 1);
                     }
                 }
             } else {
@@ -475,34 +511,6 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
             if (warp == 0 && cls) s_list[cnt + __popc(mask & ((1u << lane) - 1u))] = (first_tile + j0 + lane) << 2 | cls >> 1;
             cnt += __popc(mask);
         }
-    }
-    const unsigned char* kb = static_cast<const unsigned char*>(a.keys) + (w.sg.row_begin * a.krs + w.head * a.khs) * 2;
-    const unsigned char* vb = static_cast<const unsigned char*>(a.values) + (w.sg.row_begin * a.vrs + w.head * a.vhs) * 2;
-    constexpr int PIECES = S::HALVES * 8;
-    const auto fetch = [&](uint32_t dst, const CUtensorMap* map, bool head_first, const unsigned char* from, uint64_t stride, uint32_t first, uint32_t full) {
-        if (first + KT <= w.n) {
-            if (lane == 0) {
-                const uint32_t row = (uint32_t)w.sg.row_begin + first;
-                bar_expect(full, S::TILE);
-#pragma unroll
-                for (int h = 0; h < S::HALVES; ++h) tma_load(dst + h * HALF, map, h * 64, head_first ? w.head : row, head_first ? row : w.head, full);
-            }
-        } else {
-            for (uint32_t i = lane; i < KT * PIECES; i += 32) {
-                const uint32_t r = i / PIECES, c = i % PIECES, row = first + r;
-                const bool there = row < w.n && c * 8 < a.d;
-                copy16(dst + (c >> 3) * HALF + r * 128 + (((c & 7) ^ (r & 7)) << 4), there ? from + row * stride * 2 + c * 16 : from, there);
-            }
-            copy_commit();
-            copy_wait<0>();
-            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-            __syncwarp();
-            if (lane == 0) bar_arrive(full);
-        }
-    };
-    if (warp == FETCH_WARP && plain && cnt) {  // the first keys, while the others get ready
-        __syncwarp();
-        fetch(sb + S::K_AT, &maps.k, maps.k_head_first, kb, a.krs, (s_list[0] >> 2) * KT, bar(K_FULL));
     }
     tc_before();
     __syncthreads();
@@ -540,8 +548,8 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
                     for (int c = 0; c < 128; ++c) asm volatile("" : "+r"(u[c]));
                 };
                 load();
-                float mul = bent ? 1.0f : to_log2, top;
-                bool fused = false;  // the cap is applied on the way to the weights
+                float mul = bent && (CAP || has_slope) ? 1.0f : to_log2, top;
+                bool fused = false, brief = false;  // the cap is applied on the way to the weights, by a polynomial of degree 6 or of degree 4
                 if (CAP && !bent) {
                     float high[2] = {-INFINITY, -INFINITY}, low[2] = {INFINITY, INFINITY};
 #pragma unroll
@@ -553,7 +561,9 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
                         }
                     const float x = fmaxf(high[0], high[1]) * to_log2;
                     mul = 1.0f;
-                    fused = __all_sync(0xFFFFFFFFu, x <= 1.0f && fminf(low[0], low[1]) * to_log2 >= -1.0f);
+                    const float furthest = fmaxf(x, -fminf(low[0], low[1]) * to_log2);
+                    fused = __all_sync(0xFFFFFFFFu, furthest <= 1.0f);
+                    brief = __all_sync(0xFFFFFFFFu, furthest <= TANH_BRIEF);
                     if (fused) {  // (tanh grows: the largest score is that of the largest product)
                         top = cap2 * tanh_small(x);
                     } else {
@@ -601,7 +611,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
                             uint64_t z = pair(s[c + e], s[c + e + 1]);
                             if constexpr (decltype(capped)::value) {
                                 z = mul2(z, in);
-                                z = fma2(mul2(z, tanh_poly(mul2(z, z))), out, use_2);
+                                z = fma2(mul2(z, decltype(capped)::value == 1 ? tanh_poly(mul2(z, z)) : tanh_poly_brief(mul2(z, z))), out, use_2);
                             } else {
                                 z = fma2(z, mul_2, use_2);
                             }
@@ -621,10 +631,11 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
                     }
                 };
                 if constexpr (CAP) {
-                    if (fused) weights(std::true_type());
-                    else weights(std::false_type());
+                    if (brief) weights(std::integral_constant<int, 2>());
+                    else if (fused) weights(std::integral_constant<int, 1>());
+                    else weights(std::integral_constant<int, 0>());
                 } else {
-                    weights(std::false_type());
+                    weights(std::integral_constant<int, 0>());
                 }
                 {
                     float x, y;
@@ -672,7 +683,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
 #pragma unroll
                     for (int h = 0; h < S::HALVES; ++h)
                         tma_store(&maps.out, sb + t * S::TILE + h * HALF + (warp & 3) * 4096, h * 64, w.head * a.group, w.sg.query_begin + tok0 + warp * (32 / a.group));
-                    asm volatile("cp.async.bulk.commit_group;\ncp.async.bulk.wait_group 0;\n" ::: "memory");
+                    asm volatile("cp.async.bulk.commit_group;\ncp.async.bulk.wait_group.read 0;\n" ::: "memory");
                 }
             }
             __syncwarp();
@@ -807,6 +818,25 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
             }
             fetch(sb + S::V_AT + slot * S::TILE, &maps.v, maps.v_head_first, vb, a.vrs, first, bar(V_FULL + slot));
         }
+        } else {
+        // ---- values of tiles that not all see: where one is not finite, a weight of zero does not keep it out of the sums, and the item is done again by rows
+        for (uint32_t li = 0; li < cnt; ++li) {
+            if (!__all_sync(0xFFFFFFFFu, bar_wait(bar(V_FULL + (li & 1)), li >> 1 & 1))) {
+                fail = true;
+                break;
+            }
+            if ((s_list[li] & (two ? 3u : 1u)) != (two ? 3u : 1u)) {
+                uint32_t odd = 0;
+#pragma unroll 8
+                for (uint32_t i = tid - 320; i < S::TILE / 16; i += 64) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(sm + S::V_AT + (li & 1) * S::TILE + i * 16);
+                    odd |= odd_pair(x.x) | odd_pair(x.y) | odd_pair(x.z) | odd_pair(x.w);
+                }
+                if (odd & 0x80008000u) *s_odd = 1u;
+            }
+            __syncwarp();
+            if (lane == 0) bar_arrive(bar(V_FREE + (li & 1)));
+        }
         }
     }
     if (fail) *s_odd = 1u;
@@ -816,6 +846,8 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
     if (warp >= 8) regs_more<REGS_ALL>();
     if (warp == MMA_WARP) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512u) : "memory");
     if (*s_odd) {
+        asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");  // (rows that left as boxes lie there before they are written again)
+        __syncthreads();
         by_rows(a, *reinterpret_cast<const Item*>(sm + S::ITEM_AT), s_qp, s_qd, s_slope, s_tok, s_depth, s_anc, s_list, cnt);
     }
 }
