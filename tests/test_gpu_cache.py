@@ -703,3 +703,137 @@ def test_many_query_rows_whose_largest_scores_come_late(q_scale, cap):
     grow = np.linspace(0.05, 2.0, 1500)[:, None, None]
     call.keys, raw = K.as_type(call.keys * grow, True)[0], (K.as_type(call.keys * grow, True)[1], raw[1], raw[2])
     check(call, raw, True)
+
+
+@pytest.mark.parametrize("more", [dict(), dict(softcap=9.0), dict(softcap=0.7), dict(alibi=True), dict(window=200), dict(window=40, prefix=True, softcap=5.0), dict(prefix=True, alibi=True), dict(causal=False),
+                                  dict(causal=False, window=111, alibi=True), dict(docs=True), dict(docs=True, alibi=True, softcap=8.0), dict(moved=True), dict(moved=True, docs=True, window=700),
+                                  dict(q_only=True), dict(negative=True), dict(zero=True)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_wide_blocks_under_every_rule(more, d):
+    rng = np.random.default_rng(len(str(more)) + d)
+    lens, kv, group, tokens = (130, 700, 1290), 2, 4, 70
+    total = sum(lens)
+    kind = {k: v for k, v in more.items() if k in ("softcap", "window", "causal")}
+    if more.get("alibi"):
+        kind["slopes"] = (2.0 ** -np.arange(1, kv * group + 1)).astype(F)
+    if more.get("prefix"):
+        kind["prefix"] = np.array([130, 300, 17], np.uint32)
+    if more.get("docs"):
+        doc = np.concatenate([np.sort(rng.integers(1, 5, n)) for n in lens]).astype(np.uint32)
+        kind["row_doc"] = np.stack([doc] * kv)
+        kind["q_doc"] = np.concatenate([doc[e - tokens:e] for e in np.cumsum(lens)])
+    if more.get("moved"):
+        kind["row_pos"] = np.stack([np.concatenate([rng.permutation(2 * n)[:n] for n in lens]) for _ in range(kv)]).astype(np.uint32)
+        kind["q_pos"] = np.concatenate([2 * n - tokens + np.arange(tokens) for n in lens]).astype(np.uint32)
+    if more.get("q_only"):
+        kind["q_pos"] = np.concatenate([np.sort(rng.integers(0, n, tokens)) for n in lens]).astype(np.uint32)
+    call, raw = make(rng, lens, tokens, kv, group, d, True, **kind)
+    if more.get("negative"):
+        call.scale = -call.scale
+    if more.get("zero"):
+        call.scale = 0.0
+    check(call, raw, True)
+    if not more.get("negative") and total:
+        cache, segs, queries = on_device(call, raw, True)
+        _, lse = results(call, True, cache, segs, queries)
+        w = S.to_device(np.zeros((kv, total), F))
+        S.observe_cache(cache, segs, queries, S.to_device(lse), w, total)
+        want, tol = call.received(lse, np.zeros((kv, total), F), 1.0)
+        held(w.download(F, kv * total).reshape(kv, total), want, tol)
+
+
+@pytest.mark.parametrize("tokens,group,lens", [(100, 4, (900, 130)), (33, 1, (500,)), (512, 1, (600,))])
+def test_wide_blocks_where_hidden_rows_hold_anything(tokens, group, lens):
+    rng = np.random.default_rng(tokens)
+    kv, d, total = 2, 128, sum(lens)
+    ends = np.cumsum(lens)
+    doc = rng.integers(0, 3, total).astype(np.uint32)
+    for e in ends:
+        doc[e - tokens:e] = rng.integers(0, 2, tokens)
+    call, raw = make(rng, lens, tokens, kv, group, d, True, row_doc=np.stack([doc] * kv), q_doc=np.concatenate([doc[e - tokens:e] for e in ends]))
+    want = call.attend(True)
+    before = np.zeros((kv, total), F)
+    for r in raw[:2]:
+        r[doc == 2] = K.as_type(rng.choice(np.array([np.nan, np.inf, -np.inf], F), r[doc == 2].shape), True)[1]
+    cache, segs, queries = on_device(call, raw, True)
+    got = results(call, True, cache, segs, queries)
+    held(got[1], want[1], want[3])
+    held(got[0], want[0], want[2])
+    w = S.to_device(before)
+    S.observe_cache(cache, segs, queries, S.to_device(got[1]), w, total)
+    weights, tol = call.received(got[1], before, 1.0)
+    held(w.download(F, kv * total).reshape(kv, total), weights, tol)
+    # rows behind a segment's end, and the rest of the last tile, belong to nobody
+    call, raw = make(rng, (tokens + 70, 400), tokens, kv, group, d, True)
+    call.segs[1:] = []
+    want = call.attend(True)
+    for r in raw[:2]:
+        r[tokens + 70:] = K.as_type(np.full(r[tokens + 70:].shape, np.nan), True)[1]
+    got = results(call, True, *on_device(call, raw, True))
+    held(got[0][:tokens], want[0][:tokens], want[2][:tokens])
+
+
+def test_wide_blocks_of_other_layouts_and_row_counts_on_the_device():
+    # keys [kv_head][row][d] with gaps, values [row][kv_head][d], queries [head][token]: no boxes of queries and outputs; then strides that no map of rows takes
+    rng = np.random.default_rng(81)
+    kv, group, d, lens, tokens = 2, 4, 128, (900, 333), 40
+    call, raw = make(rng, lens, tokens, kv, group, d, True)
+    call.rows = np.array([777, 4000], np.uint32)
+    total, heads = sum(lens), kv * group
+    want = call.attend(True)
+    for head_gap, row_gap in ((0, 8), (24, 40)):
+        k = np.zeros((kv, total * (d + row_gap) + head_gap), np.uint16)
+        k[:, :total * (d + row_gap)].reshape(kv, total, d + row_gap)[:, :, :d] = raw[0].transpose(1, 0, 2)
+        q = np.ascontiguousarray(raw[2].transpose(1, 0, 2))
+        rows = S.to_device(call.rows)
+        cache = S.KvCache(S.to_device(k), S.to_device(raw[1]), kv, d, key_row_stride=d + row_gap, key_head_stride=total * (d + row_gap) + head_gap, rows=rows)
+        queries = S.CacheQueries(S.to_device(q), 2 * tokens, heads, d, token_stride=d, head_stride=2 * tokens * d)
+        out, lse = S.to_device(np.zeros((heads, 2 * tokens, d), np.uint16)), S.DeviceBuffer(8 * tokens * heads)
+        S.attend_cache(cache, S.make_segments(call.segs), queries, out, lse, out_token_stride=d, out_head_stride=2 * tokens * d)
+        o = K.from_bf16(out.download(np.uint16, heads * 2 * tokens * d)).reshape(heads, 2 * tokens, d).transpose(1, 0, 2)
+        held(o, want[0], want[2])
+        held(lse.download(F, 2 * tokens * heads).reshape(2 * tokens, heads), want[1], want[3])
+        w = S.to_device(np.zeros((kv, total), F))
+        S.observe_cache(cache, S.make_segments(call.segs), queries, lse, w, total)
+        weights, tol = call.received(lse.download(F, 2 * tokens * heads).reshape(2 * tokens, heads), np.zeros((kv, total), F), 1.0)
+        held(w.download(F, kv * total).reshape(kv, total), weights, tol)
+
+
+def test_wide_blocks_of_many_segments_and_of_long_ones_in_parts():
+    rng = np.random.default_rng(82)
+    lens = rng.integers(40, 160, 70)
+    check(*make(rng, lens, 40, 1, 1, 64, True), True)
+    call, raw = make(rng, (20000, 300), (64, 33), 1, 1, 64, True, window=9000)
+    check(call, raw, True)
+    call, raw = make(rng, (6000,), 64, 1, 2, 128, True, parents=tree(rng, "random", 64), softcap=12.0)
+    check(call, raw, True)
+
+
+@pytest.mark.parametrize("n", [140000, 1300])
+def test_many_tokens_over_a_long_cache_agree_with_few(n):
+    # the same token among 40 and alone: two kernels, splits of more tiles than a run holds
+    rng = np.random.default_rng(n)
+    kv, group, d = 1, 1, 64
+    call, raw = make(rng, (n,), 40, kv, group, d, True)
+    cache, segs, queries = on_device(call, raw, True)
+    many = results(call, True, cache, segs, queries)
+    one = S.CacheQueries(S.to_device(raw[2][39:]), 1, 1, d)
+    out, lse = S.DeviceBuffer(2 * d), S.DeviceBuffer(4)
+    S.attend_cache(cache, S.make_segments([(0, n, 0, 1, 0)]), one, out, lse)
+    got = K.from_bf16(out.download(np.uint16, d))
+    assert abs(float(lse.download(F, 1)[0]) - float(many[1][39, 0])) <= 2e-5
+    mag = np.abs(call.values).max()
+    assert np.all(np.abs(got - many[0][39, 0]) <= 2.0 ** -7 * mag)
+
+
+@pytest.mark.parametrize("n_kv,n,budget", [(1, 700, 90), (3, 5000, 4000), (40, 9000, 100), (200, 300, 150), (1, 131072, 70000)])
+def test_removal_by_clusters_of_every_size(n_kv, n, budget):
+    rng = np.random.default_rng(n)
+    w = rng.integers(0, 50, (n_kv, n)).astype(F)
+    k = rng.integers(0, 65536, (n, n_kv, 8)).astype(np.uint16)
+    cache = S.KvCache(S.to_device(k), S.to_device(k), n_kv, 8)
+    src = S.DeviceBuffer(4 * n_kv * budget)
+    S.evict_cache(cache, S.make_segments([(0, n, 0, 0, 0)]), S.to_device(w), n, budget, sink_window=3, recent_window=11, source_out=src)
+    got = src.download(np.uint32, n_kv * budget).reshape(n_kv, budget)
+    for h in range(0, n_kv, max(1, n_kv // 4)):
+        assert np.array_equal(got[h], K.evict(w[h], np.arange(n), budget, 3, 11))
