@@ -37,7 +37,7 @@ struct Shape {
                               ML_AT = RANGE_AT + 32, TREE_AT = ML_AT + 64 * 2 * 4;
     static constexpr uint32_t SMEM = TREE_AT, SMEM_TREE = TREE_AT + TREE_MOST * 8 + MB * (TREE_MOST / 8);
     static constexpr int PITCH = D + 8;  // floats of a query row on the way out
-    static_assert(64 * PITCH * 4 <= STAGES * STAGE && (WM == 4 || (64 * PITCH + MB * (D + 2)) * 4 <= STAGES * STAGE), "the sums leave through the stages");
+    static_assert(64 * PITCH * 4 <= STAGES * STAGE && (64 * PITCH + MB * (D + 2)) * 4 <= STAGES * STAGE + Q_BYTES, "the sums leave through the stages and the queries behind them");
     static constexpr int CTAS = D == 256 ? 1 : 2;
     static_assert(SMEM_TREE <= 227 * 1024, "shared memory of an SM");
 };
@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(ATT_THREADS, Shape<T, D, WM>::CTAS) cache_atte
     const uint32_t sb = smem_addr(sm);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wm = warp % WM, wn = warp / WM, g = lane >> 2, t4 = lane & 3;
     namespace cg = cooperative_groups;
-    const uint32_t cl = WM <= 2 && a.cluster ? a.cluster : 1, of_cluster = blockIdx.x % cl;
+    const uint32_t cl = a.cluster ? a.cluster : 1, of_cluster = blockIdx.x % cl;
     const uint32_t head = blockIdx.x / cl % a.n_kv, item = blockIdx.x / cl / a.n_kv * cl + of_cluster;
     const CacheSeg* table = a.table ? a.table : tab.s;
     const uint32_t seg = cache_find(a.n_segs, item, [&](uint32_t i) { return table[i].item_begin; });
@@ -536,7 +536,7 @@ static void cut(CacheWork* w, uint32_t group, uint32_t mb, uint32_t kt, uint32_t
 // The longest run of tiles of an item.  In units of a tile's time: what fits on the GPU at once takes as long as its longest item, more than that the mean load
 // and half an item at the end; an item costs about four tiles to begin, joining about three and a little for every part.
 // *cluster: how many CTAs share a block of query rows and join their sums through each other's shared memory, where that takes less time than a second kernel (0: none do).
-static uint32_t longest_run(const CacheWork& w, uint32_t group, uint32_t mb, uint32_t kt, uint32_t n_kv, uint32_t slots, bool clusters, uint32_t* cluster) {
+static uint32_t longest_run(const CacheWork& w, uint32_t group, uint32_t mb, uint32_t kt, uint32_t n_kv, uint32_t slots, uint32_t* cluster) {
     uint32_t most = 1;
     double total = 0.0;
     for (const CacheSeg& c : w.segs) {
@@ -558,14 +558,13 @@ static uint32_t longest_run(const CacheWork& w, uint32_t group, uint32_t mb, uin
         if (run <= 2) break;
     }
     *cluster = 0;
-    if (clusters)
-        for (uint32_t cl = 2; cl <= 8; cl *= 2) {
-            double items = 0.0;
-            for (const CacheSeg& c : w.segs) items += (double)blocks_of(c, group, mb) * cl * n_kv;
-            const uint32_t run = (most + cl - 1) / cl;
-            const double time = (items <= slots ? run : total / slots + 0.5 * run) + 4.0 * std::ceil(items / slots) + 0.5;
-            if (time < best_time) best_time = time, *cluster = cl;
-        }
+    for (uint32_t cl = 2; cl <= 8; cl *= 2) {
+        double items = 0.0;
+        for (const CacheSeg& c : w.segs) items += (double)blocks_of(c, group, mb) * cl * n_kv;
+        const uint32_t run = (most + cl - 1) / cl;
+        const double time = (items <= slots ? run : total / slots + 0.5 * run) + 4.0 * std::ceil(items / slots) + 0.5;
+        if (time < best_time) best_time = time, *cluster = cl;
+    }
     return best;
 }
 
@@ -606,7 +605,7 @@ template <typename T, int D, int WM>
 Status launch_class(Ctx* c, CacheArgs a, CacheWork w) {
     using S = Shape<T, D, WM>;
     const uint32_t slots = (uint32_t)sm_count(c->device) * S::CTAS;
-    const uint32_t run = longest_run(w, a.group, S::MB, S::KT, a.n_kv, slots, WM <= 2, &a.cluster);
+    const uint32_t run = longest_run(w, a.group, S::MB, S::KT, a.n_kv, slots, &a.cluster);
     cut(&w, a.group, S::MB, S::KT, run, a.cluster);
     if (w.items * a.n_kv > 0x7FFFFFFFull) return Status(SLHA_ERR_CAPACITY, "attention over a cache: too many blocks of query rows");
     CacheTable tab;

@@ -44,7 +44,7 @@ __global__ void __cluster_dims__(C, 1, 1) __launch_bounds__(SEL_THREADS) cache_s
     cg::cluster_group cluster = cg::this_cluster();
     dep_wait();
     extern __shared__ __align__(16) uint32_t s_key[];
-    __shared__ uint32_t s_hist[SEL_BINS], s_scan[SEL_WARPS], s_found[2], s_last, s_warp[SEL_WARPS], s_all[3];
+    __shared__ uint32_t s_hist[SEL_BINS], s_scan[SEL_WARPS], s_found[3], s_last, s_warp[SEL_WARPS], s_all[3];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t which = blockIdx.x / C, rank_of = C > 1 ? cluster.block_rank() : 0u, at = which / a.n_kv, head = which % a.n_kv;
     const CacheSeg sg = (a.table ? a.table : tab.s)[at];
@@ -152,13 +152,18 @@ __global__ void __cluster_dims__(C, 1, 1) __launch_bounds__(SEL_THREADS) cache_s
         uint32_t before = scan_threads(c[0] + c[1], s_scan);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            if (before < left && before + c[j] >= left) s_found[0] = SEL_BINS - 1 - tid * 2 - j, s_found[1] = left - before;
+            if (before < left && before + c[j] >= left) s_found[0] = SEL_BINS - 1 - tid * 2 - j, s_found[1] = left - before, s_found[2] = c[j];
             before += c[j];
         }
         if (C > 1) cluster.sync();  // (also: the others have read this CTA's buckets)
         else __syncthreads();
         prefix |= s_found[0] << shift;
         left = s_found[1];
+        if (left == s_found[2] && prefix) {  // all of the bucket stay: so do those above the number before it, and no others
+            --prefix;
+            left = 0;
+            break;
+        }
     }
     // In the rows' order: how many equal the last key that stays; then which stay, the free places below the budget and the rows from beyond that take them.
     const auto before_me = [&](uint32_t x, int slot) {  // the sum over the warps, of this CTA and those before it, before this one (x: a lane's)
@@ -272,6 +277,23 @@ __global__ void __launch_bounds__(MOVE_THREADS) cache_move_kernel(const __grid_c
     const unsigned char* v = static_cast<const unsigned char*>(a.values) + sg.row_begin * a.vrs + head * a.vhs;
     unsigned char* tk = static_cast<unsigned char*>(a.to_keys) + sg.to_begin * a.tkrs + head * a.tkhs;
     unsigned char* tv = static_cast<unsigned char*>(a.to_values) + sg.to_begin * a.tvrs + head * a.tvhs;
+    // (all loads of tiles and of single words are under way before the first row is stored)
+    uint4 tile[2];
+    uint32_t word[3];
+    const unsigned char* from_tile = a.tiles + (head * a.tile_hs + sg.row_begin) * TILE_BYTES + tid % 8 * 16;
+    if (a.tiles)
+#pragma unroll
+        for (int f = 0; f < 2; ++f) {
+            const uint32_t src = s_src[tid / 8 + f * 32];
+            if (src != 0xFFFFFFFFu) tile[f] = *reinterpret_cast<const uint4*>(from_tile + (uint64_t)src * TILE_BYTES);
+        }
+    const bool words = tid < MOVE_PLACES && s_src[tid < MOVE_PLACES ? tid : 0] != 0xFFFFFFFFu;
+    if (words) {
+        const uint64_t src = head * a.entry_hs + sg.row_begin + s_src[tid];
+        if (a.to_pos) word[0] = a.pos[src];
+        if (a.to_doc) word[1] = a.doc[src];
+        if (a.to_w) word[2] = __float_as_uint(a.w[head * a.w_hs + sg.row_begin + s_src[tid]]);
+    }
     constexpr int AT_ONCE = MOVE_THREADS / LANES, FLIGHT = MOVE_PLACES / AT_ONCE < 8 ? MOVE_PLACES / AT_ONCE : 8;
     const uint32_t lane = tid % LANES, group = tid / LANES, half = a.row_bytes / 16;
     for (uint32_t piece = lane; piece < 2 * half; piece += LANES) {
@@ -293,25 +315,16 @@ __global__ void __launch_bounds__(MOVE_THREADS) cache_move_kernel(const __grid_c
         }
     }
     if (a.tiles) {
-        const unsigned char* from = a.tiles + (head * a.tile_hs + sg.row_begin) * TILE_BYTES;
-        unsigned char* to = a.to_tiles + (head * a.to_tile_hs + sg.to_begin) * TILE_BYTES;
-        uint4 x[2];
+        unsigned char* to = a.to_tiles + (head * a.to_tile_hs + sg.to_begin) * TILE_BYTES + tid % 8 * 16;
 #pragma unroll
-        for (int f = 0; f < 2; ++f) {
-            const uint32_t i = tid / 8 + f * 32;
-            if (s_src[i] != 0xFFFFFFFFu) x[f] = *reinterpret_cast<const uint4*>(from + (uint64_t)s_src[i] * TILE_BYTES + tid % 8 * 16);
-        }
-#pragma unroll
-        for (int f = 0; f < 2; ++f) {
-            const uint32_t i = tid / 8 + f * 32;
-            if (s_src[i] != 0xFFFFFFFFu) *reinterpret_cast<uint4*>(to + (uint64_t)(p0 + i) * TILE_BYTES + tid % 8 * 16) = x[f];
-        }
+        for (int f = 0; f < 2; ++f)
+            if (s_src[tid / 8 + f * 32] != 0xFFFFFFFFu) *reinterpret_cast<uint4*>(to + (uint64_t)(p0 + tid / 8 + f * 32) * TILE_BYTES) = tile[f];
     }
-    if (tid < MOVE_PLACES && s_src[tid] != 0xFFFFFFFFu) {
-        const uint64_t src = head * a.entry_hs + sg.row_begin + s_src[tid], to = head * a.to_entry_hs + sg.to_begin + p0 + tid;
-        if (a.to_pos) a.to_pos[to] = a.pos[src];
-        if (a.to_doc) a.to_doc[to] = a.doc[src];
-        if (a.to_w) a.to_w[head * a.to_w_hs + sg.to_begin + p0 + tid] = a.w[head * a.w_hs + sg.row_begin + s_src[tid]];
+    if (words) {
+        const uint64_t to = head * a.to_entry_hs + sg.to_begin + p0 + tid;
+        if (a.to_pos) a.to_pos[to] = word[0];
+        if (a.to_doc) a.to_doc[to] = word[1];
+        if (a.to_w) a.to_w[head * a.to_w_hs + sg.to_begin + p0 + tid] = __uint_as_float(word[2]);
     }
 }
 

@@ -145,7 +145,7 @@ bool wide_map(CUtensorMap* map, const void* base, uint64_t row_stride, uint64_t 
 
 // Queries or outputs in boxes of 32 rows of a KV head (32 / group tokens of its group); false where the layout or the group does not allow it.
 bool wide_row_map(CUtensorMap* map, const void* base, uint64_t token_stride, uint64_t head_stride, const CacheArgs& a) {
-    if (32 % a.group || (a.n_heads > 1 && head_stride >= token_stride)) return false;
+    if (32 % a.group || (a.n_heads > 1 && head_stride >= token_stride) || a.n_tokens > 0x7FFFFFFFu) return false;
     const WideEncode encode = wide_encode();
     if (!encode) return false;
     if (a.n_heads == 1) head_stride = token_stride;  // (never stepped by)

@@ -80,6 +80,7 @@ Status cache_check_queries(const SlhaB200KvCache* k, const SlhaB200CacheQueries*
         return Status(SLHA_ERR_DIMENSION, name("q must begin on a multiple of 16 bytes and its strides be multiples of 16 bytes"));
     if (!std::isfinite(q->scale) || !std::isfinite(q->softcap) || q->softcap < 0.0f)
         return Status(SLHA_ERR_NONFINITE, name("scale must be finite, softcap finite and not negative"));
+    if (q->softcap > 0.0f && !std::isfinite(q->scale / q->softcap)) return Status(SLHA_ERR_NONFINITE, name("scale / softcap must be finite"));
     if (k->positions && !q->positions) return Status(SLHA_ERR_NULL, name("the cache's rows have positions, the queries have none"));
     if ((k->documents != nullptr) != (q->documents != nullptr)) return Status(SLHA_ERR_NULL, name("documents must be given for rows and queries, or for neither"));
     return Status();

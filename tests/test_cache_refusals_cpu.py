@@ -39,7 +39,7 @@ def test_what_no_call_with_queries_takes(call):
     refused(S.ERR_NULL, "q is NULL", call, cache(), SEG, queries(q=None))
     for bad in (dict(n_heads=0), dict(n_heads=3), dict(token_stride=3), dict(head_stride=1), dict(q=A + 8)):
         refused(S.ERR_DIMENSION, "", call, cache(), SEG, queries(**bad))
-    for bad in (dict(scale=float("nan")), dict(softcap=-1.0), dict(softcap=float("inf"))):
+    for bad in (dict(scale=float("nan")), dict(softcap=-1.0), dict(softcap=float("inf")), dict(softcap=1e-42, scale=1.0)):
         refused(S.ERR_NONFINITE, "finite", call, cache(), SEG, queries(**bad))
     refused(S.ERR_NULL, "positions", call, cache(positions=A), SEG, queries())
     refused(S.ERR_NULL, "documents", call, cache(documents=A), SEG, queries())
