@@ -622,7 +622,9 @@ Status launch_class(Ctx* c, CacheArgs a, CacheWork w) {
 }
 template <typename T, int D>
 Status launch_dim(Ctx* c, const CacheArgs& a, int wm, CacheWork w) {
-    return wm == 1 ? launch_class<T, D, 1>(c, a, std::move(w)) : wm == 2 ? launch_class<T, D, 2>(c, a, std::move(w)) : launch_class<T, D, 4>(c, a, std::move(w));
+    if constexpr (sizeof(T) == 2)
+        if (wm == 2) return launch_class<T, D, 2>(c, a, std::move(w));
+    return wm == 1 ? launch_class<T, D, 1>(c, a, std::move(w)) : launch_class<T, D, 4>(c, a, std::move(w));
 }
 
 }  // namespace
@@ -641,7 +643,10 @@ Status cache_table(Ctx* c, const std::vector<CacheSeg>& segs, CacheTable* inl, c
 
 Status launch_attend_cache(Ctx* c, CacheArgs a, int dtype, const std::vector<SlhaB200Segment>& segs) {
     // Segments of at most 16, of at most 32 and of more query rows a KV head: a launch each, so that a batch of decoded tokens beside a prompt keeps
-    // the kernel that suits it.
+    // the kernel that suits it.  8 KV heads of 128 dimensions, us in blocks of 16, 32, 64 query rows and with the kernel for many (whose tensor cores take 128 rows at a time):
+    //   bfloat16, 16 x 8192 rows: 4 query rows 82, 100, 138, 116; 16: 84, 104, 144, 120; 20: 140, 106, 145, 120; 32: 141, 107, 147, 119; 36: -, 194, 148, 120; 256: -, 724, 615, 140
+    //             1 x 4096 rows: 4 query rows 10.0, 10.8, 12.4, 14.1; 20: 12.8, 13.5, 16.7, 16.2; 36: -, 15.6, 17.6, 16.5; 256: -, 35, 32, 24
+    //   float32, 4 x 2048 rows: 16 query rows 30, 78, 58; 32: 49, 81, 59; 64: 90, 93, 63 (blocks of 32 hold two CTAs' registers and are never the quickest: 16 up to 32 rows)
     CacheWork of[3];
     for (size_t i = 0; i < segs.size(); ++i) {
         const SlhaB200Segment& s = segs[i];
@@ -654,7 +659,7 @@ Status launch_attend_cache(Ctx* c, CacheArgs a, int dtype, const std::vector<Slh
         g.base = s.index_base;
         g.seg = (uint32_t)i;
         const uint64_t rows = (uint64_t)s.n_queries * a.group;
-        of[rows <= 16 ? 0 : rows <= 32 ? 1 : 2].segs.push_back(g);
+        of[rows <= 16 || (rows <= 32 && dtype == SLHA_B200_F32) ? 0 : rows <= 32 ? 1 : 2].segs.push_back(g);
     }
     for (int k = 0; k < 3; ++k) {
         if (of[k].segs.empty()) continue;

@@ -357,9 +357,11 @@ Status launch_evict_cache(Ctx* c, EvictArgs a, const std::vector<SlhaB200Segment
     a.places = static_cast<uint32_t*>(p);
     a.holes = a.places + heads * room;
     a.stay = a.holes + heads * room;
-    // CTAs of a cluster: as many as find an SM each, where every warp still has 128 rows (64 heads of 32768 rows: one CTA 71 us, two 30)
-    uint32_t c_size = 1;
-    while (c_size < 8 && heads * c_size * 2 <= (uint64_t)sm_count(c->device) && most > c_size * SEL_THREADS * 4) c_size *= 2;
+    // CTAs of a cluster: as many as find an SM each, of eight only where they find it beyond doubt (a cluster lies within a group of SMs: 16 heads in eights took two turns, 52 us
+    // for 26 in fours).  8 heads, selection and 64 rows' places, in ones, twos, fours, eights: 8192 rows 18, 19, 19, 19 us; 16384 27, 24, 22, 22; 32768 44, 33, 26, 30;
+    // 65536 106, 51, 34, 34; 131072 204, 112, 50, 42.
+    uint32_t c_size = most >= 65536 ? 8 : most >= 16384 ? 4 : 1;
+    while (c_size > 1 && heads * c_size > (uint64_t)sm_count(c->device) * (c_size == 8 ? 2 : 3) / 3) c_size /= 2;
     const size_t share = ((size_t)most + c_size * SEL_WARPS * 128 - 1) / (c_size * SEL_WARPS * 128) * SEL_WARPS * 128, smem = std::min<size_t>(share, SEL_HELD) * 4;
     const auto select = [&](auto kernel_of) -> Status {
         constexpr auto kernel = cache_select_kernel<decltype(kernel_of)::value>;

@@ -1,7 +1,7 @@
 // The weight that each cached row received, for bfloat16 rows of up to 128 dimensions and up to 512 query rows a KV head (the arithmetic is that of cache_observe.cu).
 //
 // Scores as S^T = K Q^T on tcgen05: a tile of 128 keys is the M side, so that a thread has a key's scores in its own TMEM lane and its weight is a sum over the thread's own
-// columns: no sum crosses threads (with many query rows, four threads share a key).  A CTA takes the queries of one KV head, which stay in shared memory, and a run of key tiles,
+// columns: no sum crosses threads (with many query rows four threads share a key).  A CTA takes the queries of one KV head, which stay in shared memory, and a run of key tiles,
 // each of which is read once (TMA, the tile behind which a segment ends by cp.async).  While one block of scores is summed, the next is multiplied.
 #include <cuda_bf16.h>
 
@@ -15,29 +15,38 @@ namespace {
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int KT = 128;
 
-// MANY: up to 512 query rows, four threads a key, one CTA an SM; else up to 32, one thread a key, two CTAs an SM
-template <int D, bool MANY>
+// FEW: up to 32 query rows, a thread a key, two CTAs an SM, blocks of scores in two places by turns.  MID: up to 256, four groups of 128 threads, each with a tile and a place of its
+// own, so that no sum crosses threads and nobody waits for another group.  MANY: up to 512, four threads a key, two places by turns.
+//
+// MID wants four tiles at a time and a run of them behind those, so FEW takes up to 32 query rows in runs of up to 8 tiles, and MANY what has more rows in runs of up to 4.
+// Measured, 8 KV heads of 128 dimensions, us:
+//   64 sequences of 1024 rows (runs of 8), 4 query rows: FEW 33, MID 39, MANY 49; one of 8192 (4): 5.6, 6.0, 7.4; 8 of 8192 (28): 32, 25, 36; with 32 query rows 38, 27, 40
+//   one sequence of 4096 rows (2), 64 query rows: MID 9.0, MANY 7.1; of 16384 (7): 13.9, 14.9; of 32768 (14): 16, 22; with 256 query rows 40, 43
+// and cache_observe.cu's kernel takes 40, 56 (4, 32 query rows on 8 of 8192), 39, 119 (64, 256 on 32768): it takes rows beyond 512 query rows, 128 dimensions, and float32.
+enum { FEW = 0, MID = 1, MANY = 2 };
+template <int D, int MODE>
 struct Obs {
-    static constexpr int HALVES = D / 64, ROWS = MANY ? 512 : 32, BLOCK = MANY ? 256 : 32;  // query rows in all, and of a product
-    static constexpr int SUMMERS = MANY ? 512 : 128, THREADS = SUMMERS + 64, MMA_WARP = SUMMERS / 32, FETCH_WARP = MMA_WARP + 1;
-    static constexpr int STAGES = MANY ? 2 : (D == 64 ? 5 : 3);
-    static constexpr uint32_t TILE = HALVES * HALF, Q_HALF = ROWS * 128, TMEM = MANY ? 512 : 64;
+    static constexpr int HALVES = D / 64, ROWS = MODE == MANY ? 512 : MODE == MID ? 256 : 32, BLOCK = MODE == MANY ? 256 : MODE == MID ? 128 : 32;  // query rows in all, and of a product
+    static constexpr int GROUPS = MODE == MID ? 4 : 1, PLACES = MODE == MID ? 4 : 2;
+    static constexpr int SUMMERS = MODE == FEW ? 128 : 512, THREADS = SUMMERS + 64, MMA_WARP = SUMMERS / 32, FETCH_WARP = MMA_WARP + 1;
+    static constexpr int STAGES = MODE == MANY ? 2 : MODE == MID ? 4 : (D == 64 ? 5 : 3);
+    static constexpr uint32_t TILE = HALVES * HALF, Q_HALF = ROWS * 128, PLACE = MODE == FEW ? 64 : BLOCK, TMEM = PLACES * PLACE;  // columns of a place, and of all
     static constexpr uint32_t K_AT = HALVES * Q_HALF, ROW_AT = K_AT + STAGES * TILE;  // per query row: lse in units of log 2 (two parts), position, document, slope, distance
-    static constexpr uint32_t SUM_AT = ROW_AT + 6 * ROWS * 4, BAR_AT = SUM_AT + (MANY ? 3 * KT * 4 : 0), SMEM = BAR_AT + 128 + 1024;
-    static constexpr int CTAS = MANY ? 1 : 2;
+    static constexpr uint32_t SUM_AT = ROW_AT + 6 * ROWS * 4, BAR_AT = SUM_AT + (MODE == MANY ? 3 * KT * 4 : 0), SMEM = BAR_AT + 256 + 1024;
+    static constexpr int CTAS = MODE == FEW ? 2 : 1;
     static_assert(CTAS * (SMEM + 1024) <= 228 * 1024, "shared memory of an SM");
 };
-enum { K_FULL = 0, K_FREE = 5, S_FULL = 10, S_FREE = 12, Q_FULL = 14, TMEM_WORD = 15 };
+enum { K_FULL = 0, K_FREE = 5, S_FULL = 10, S_FREE = 14, Q_FULL = 18, TMEM_WORD = 19 };
 
 struct ObsMaps {
     CUtensorMap k, q;
     uint32_t k_head_first, q_boxes;
 };
 
-template <int D, bool MANY>
-__global__ void __launch_bounds__(Obs<D, MANY>::THREADS, Obs<D, MANY>::CTAS)
+template <int D, int MODE>
+__global__ void __launch_bounds__(Obs<D, MODE>::THREADS, Obs<D, MODE>::CTAS)
     cache_observe_wide_kernel(const __grid_constant__ CacheArgs a, const __grid_constant__ ObsMaps maps, const __grid_constant__ CacheTable tab) {
-    using S = Obs<D, MANY>;
+    using S = Obs<D, MODE>;
     dep_wait();
     extern __shared__ unsigned char raw[];
     const uint32_t sb = (smem_addr(raw) + 1023u) & ~1023u;
@@ -63,12 +72,16 @@ __global__ void __launch_bounds__(Obs<D, MANY>::THREADS, Obs<D, MANY>::CTAS)
     const uint32_t bars = sb + S::BAR_AT;
     const auto bar = [&](int which) { return bars + which * 8; };
     // rows of a block of query rows, as columns: a multiple of 16
+    // The tensor cores cut their sums off after each step of 16 elements, towards zero: eight steps of a score of 90 (8 once scaled) lose 1.3e-6 of its weight.  Where the columns
+    // suffice a score is two sums, of 64 elements each, which halves that (8 x 8192 rows after a decode step: 1.1e-6 -> 4.1e-7).
+    constexpr uint32_t SECOND = S::PLACE / 2;
+    const bool halved = D > 64 && MODE != MANY && q_rows <= SECOND;
     const auto columns = [&](uint32_t b) { return min((uint32_t)S::BLOCK, (q_rows - b * S::BLOCK + 31) / 32 * 32); };
 
     if (warp == S::FETCH_WARP) {
         if (lane == 0) {
             for (int i = 0; i < S::STAGES; ++i) bar_init(bar(K_FULL + i), 1), bar_init(bar(K_FREE + i), 1);
-            for (int i = 0; i < 2; ++i) bar_init(bar(S_FULL + i), 1), bar_init(bar(S_FREE + i), S::SUMMERS);
+            for (int i = 0; i < S::PLACES; ++i) bar_init(bar(S_FULL + i), 1), bar_init(bar(S_FREE + i), S::SUMMERS / S::GROUPS);
             bar_init(bar(Q_FULL), 1);
             asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
@@ -133,7 +146,7 @@ __global__ void __launch_bounds__(Obs<D, MANY>::THREADS, Obs<D, MANY>::CTAS)
     };
 
     if (warp < S::SUMMERS / 32) {
-        const uint32_t quarter = MANY ? warp >> 2 : 0, k_row = (warp & 3) * 32 + lane;
+        const uint32_t quarter = MODE == MANY ? warp >> 2 : 0, group = MODE == MID ? warp >> 2 : 0, k_row = (warp & 3) * 32 + lane;
         const float to_log2 = has_cap ? a.scale / a.cap : a.scale * LOG2E, cap2 = a.cap * LOG2E;
         const bool bent = has_cap || has_slope;
         bool alone = false;  // a wait ran out: this warp goes on with dot products of its own
@@ -147,27 +160,34 @@ __global__ void __launch_bounds__(Obs<D, MANY>::THREADS, Obs<D, MANY>::CTAS)
             if (has_doc) next_kd = a.row_doc[entry + there];
             if (a.w_in && quarter == 0 && row < n) next_w = a.w_in[head * a.w_hs + sg.row_begin + row];
         };
-        ahead(first_tile);
-        for (uint32_t j = first_tile; j < end_tile; ++j) {
+        if (first_tile + group < end_tile) ahead(first_tile + group);
+        for (uint32_t j = first_tile + group; j < end_tile; j += S::GROUPS) {
             const uint32_t row = j * KT + k_row, there = min(row, n - 1), kp = next_kp, kd = next_kd;
             const uint64_t at = head * a.w_hs + sg.row_begin + row;
             const float before = next_w, k_at = (float)((long long)kp - (long long)near_pos);
-            if (j + 1 < end_tile) ahead(j + 1);
+            if (j + S::GROUPS < end_tile) ahead(j + S::GROUPS);
             float sum = 0.0f;
             if (visited(j)) {
                 // whether all query rows see the warp's keys
                 const uint32_t far_ = max(qr.pmax > kp ? qr.pmax - kp : 0u, kp > qr.pmin ? kp - qr.pmin : 0u);
                 const bool all = __all_sync(0xFFFFFFFFu, (!has_doc || (qr.dmin == qr.dmax && kd == qr.dmin)) && (kp < sight.prefix || ((!sight.causal || kp <= qr.pmin) && far_ <= sight.window_last)));
                 for (uint32_t b = 0; b < blocks; ++b, ++use) {
-                    const uint32_t cols = columns(b), buf = use & 1, r_from = b * S::BLOCK;
-                    if (!alone) alone = !__all_sync(0xFFFFFFFFu, bar_wait(bar(S_FULL + buf), use >> 1 & 1));
+                    const uint32_t cols = columns(b), buf = MODE == MID ? group : use & 1, r_from = b * S::BLOCK;
+                    if (!alone) alone = !__all_sync(0xFFFFFFFFu, bar_wait(bar(S_FULL + buf), MODE == MID ? use & 1 : use >> 1 & 1));
                     tc_after();
-                    for (uint32_t c0 = quarter * 16; c0 < cols && r_from + c0 < q_rows; c0 += MANY ? 64 : 16) {
+                    for (uint32_t c0 = quarter * 16; c0 < cols && r_from + c0 < q_rows; c0 += MODE == MANY ? 64 : 16) {
                         uint32_t u[16];
                         float* s = reinterpret_cast<float*>(u);
                         __syncwarp();
                         if (!alone) {
-                            tmem_ld16(tmem + ((uint32_t)(warp & 3) << 21) + buf * S::BLOCK + c0, u);
+                            const uint32_t from = tmem + ((uint32_t)(warp & 3) << 21) + buf * S::PLACE + c0;
+                            tmem_ld16(from, u);
+                            if (halved) {
+                                uint32_t more[16];
+                                tmem_ld16(from + SECOND, more);
+#pragma unroll
+                                for (int c = 0; c < 16; ++c) s[c] += __uint_as_float(more[c]);
+                            }
                         } else {
 #pragma unroll 1
                             for (int c = 0; c < 16; ++c) {
@@ -199,9 +219,8 @@ __global__ void __launch_bounds__(Obs<D, MANY>::THREADS, Obs<D, MANY>::CTAS)
                                 const float slope[4] = {sl.x, sl.y, sl.z, sl.w}, q_at[4] = {qa.x, qa.y, qa.z, qa.w};
 #pragma unroll
                                 for (int e = 0; e < 4; ++e) {
-                                    float x = has_cap ? cap2 * cache_tanh(s[c + e] * to_log2) : s[c + e] * to_log2;
-                                    x = fmaf(-slope[e], fabsf(q_at[e] - k_at), x);
-                                    x = exp2_fast((x - h4[e]) - l4[e]);
+                                    float x = (has_cap ? fmaf(cap2, cache_tanh(s[c + e] * to_log2), -h4[e]) : fmaf(s[c + e], to_log2, -h4[e])) - l4[e];
+                                    x = exp2_fast(fmaf(-slope[e], fabsf(q_at[e] - k_at), x));
                                     part[e & 1] += r0 + c + e < q_rows && (all || (sight.sees(qp[e], kp) && kd == qd[e])) ? x : 0.0f;
                                 }
                             }
@@ -212,7 +231,7 @@ __global__ void __launch_bounds__(Obs<D, MANY>::THREADS, Obs<D, MANY>::CTAS)
                     bar_arrive(bar(S_FREE + buf));
                 }
             }
-            if constexpr (MANY) {  // a key's four sums meet
+            if constexpr (MODE == MANY) {  // a key's four sums meet
                 if (quarter) s_sum[(quarter - 1) * KT + k_row] = sum;
                 asm volatile("bar.sync 1, 512;\n" ::: "memory");
                 if (!quarter) sum = (sum + s_sum[k_row]) + (s_sum[KT + k_row] + s_sum[2 * KT + k_row]);
@@ -226,25 +245,52 @@ __global__ void __launch_bounds__(Obs<D, MANY>::THREADS, Obs<D, MANY>::CTAS)
         if (lead && (q_rows == 0 || !maps.q_boxes || bar_wait(bar(Q_FULL), 0))) {
             uint32_t use = 0, step = 0;
             bool ok = true;
-            for (uint32_t j = first_tile; j < end_tile && ok; ++j) {
-                if (!visited(j)) continue;
-                const uint32_t st = step % S::STAGES;
-                ok = bar_wait(bar(K_FULL + st), step / S::STAGES & 1);
-                for (uint32_t b = 0; b < blocks && ok; ++b, ++use) {
-                    const uint32_t buf = use & 1;
-                    if (use >= 2 && !bar_wait(bar(S_FREE + buf), (use >> 1) - 1 & 1)) {
-                        ok = false;
-                        break;
-                    }
-                    tc_after();
-                    const uint32_t k = sb + S::K_AT + st * S::TILE, q = sb + b * S::BLOCK * 128, idesc = wide_idesc(columns(b), false);
+            const auto product = [&](uint32_t st, uint32_t b, uint32_t place) {
+                const uint32_t k = sb + S::K_AT + st * S::TILE, q = sb + b * S::BLOCK * 128, idesc = wide_idesc(columns(b), false);
 #pragma unroll
-                    for (int kk = 0; kk < D / 16; ++kk)
-                        mma_shared(tmem + buf * S::BLOCK, desc_along(k + (kk >> 2) * HALF + (kk & 3) * 32), desc_along(q + (kk >> 2) * S::Q_HALF + (kk & 3) * 32), idesc, kk > 0);
-                    tc_commit_to(bar(S_FULL + buf));
+                for (int kk = 0; kk < D / 16; ++kk)
+                    mma_shared(tmem + place * S::PLACE + (halved && kk >= 4 ? SECOND : 0), desc_along(k + (kk >> 2) * HALF + (kk & 3) * 32), desc_along(q + (kk >> 2) * S::Q_HALF + (kk & 3) * 32), idesc,
+                               kk > 0 && !(halved && kk == 4));
+                tc_commit_to(bar(S_FULL + place));
+            };
+            if constexpr (MODE == MID) {
+                uint32_t uses[4] = {0, 0, 0, 0};
+                for (uint32_t j = first_tile; j < end_tile && ok; j += 4) {  // four tiles, a group's each; their first blocks, then their second ones
+                    uint32_t stage[4];
+                    for (uint32_t b = 0; b < blocks && ok; ++b)
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) {
+                            if (!ok || j + g >= end_tile || !visited(j + g)) continue;
+                            if (b == 0) {
+                                stage[g] = step % S::STAGES;
+                                ok = bar_wait(bar(K_FULL + stage[g]), step / S::STAGES & 1);
+                                ++step;
+                            }
+                            if (ok && uses[g]) ok = bar_wait(bar(S_FREE + g), (uses[g] - 1) & 1);
+                            if (!ok) continue;
+                            ++uses[g];
+                            tc_after();
+                            product(stage[g], b, g);
+                            if (b + 1 == blocks) tc_commit_to(bar(K_FREE + stage[g]));
+                        }
                 }
-                if (ok) tc_commit_to(bar(K_FREE + st));
-                ++step;
+            } else {
+                for (uint32_t j = first_tile; j < end_tile && ok; ++j) {
+                    if (!visited(j)) continue;
+                    const uint32_t st = step % S::STAGES;
+                    ok = bar_wait(bar(K_FULL + st), step / S::STAGES & 1);
+                    for (uint32_t b = 0; b < blocks && ok; ++b, ++use) {
+                        const uint32_t buf = use & 1;
+                        if (use >= 2 && !bar_wait(bar(S_FREE + buf), (use >> 1) - 1 & 1)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_after();
+                        product(st, b, buf);
+                    }
+                    if (ok) tc_commit_to(bar(K_FREE + st));
+                    ++step;
+                }
             }
         }
         __syncwarp();
@@ -284,25 +330,30 @@ __global__ void __launch_bounds__(Obs<D, MANY>::THREADS, Obs<D, MANY>::CTAS)
     if (warp == S::MMA_WARP) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(S::TMEM) : "memory");
 }
 
-template <int D, bool MANY>
-Status launch_observe_wide_t(Ctx* c, CacheArgs a, std::vector<CacheSeg>& segs, const ObsMaps& maps) {
-    using S = Obs<D, MANY>;
-    // Runs of tiles: as long as all CTAs that fit on the GPU at once have one (MANY), or a few each, which hide one another's beginning and end.
-    const uint64_t slots = (uint64_t)sm_count(c->device) * S::CTAS;
+// The run of tiles of which as many as there are places make up all rows, at most the longest segment's.
+uint32_t even_run(const std::vector<CacheSeg>& segs, uint32_t n_kv, uint64_t places, uint32_t* longest) {
     uint64_t total = 0;
-    uint32_t longest = 1;
+    *longest = 1;
     for (const CacheSeg& s : segs) {
         const uint32_t tiles = (uint32_t)(((uint64_t)s.n_rows + KT - 1) / KT);
-        total += (uint64_t)tiles * a.n_kv;
-        longest = std::max(longest, tiles);
+        total += (uint64_t)tiles * n_kv;
+        *longest = std::max(*longest, tiles);
     }
-    uint32_t run = (uint32_t)std::min<uint64_t>(longest, (total + slots - 1) / slots);
+    return (uint32_t)std::min<uint64_t>(*longest, (total + places - 1) / places);
+}
+
+template <int D, int MODE>
+Status launch_observe_wide_t(Ctx* c, CacheArgs a, std::vector<CacheSeg>& segs, const ObsMaps& maps) {
+    using S = Obs<D, MODE>;
+    // Runs of tiles: as long as all CTAs that fit on the GPU at once have one (MID, MANY), or a few each, which hide one another's beginning and end.
+    const uint64_t slots = (uint64_t)sm_count(c->device) * S::CTAS;
+    uint32_t longest, run = even_run(segs, a.n_kv, slots, &longest);
     const auto count = [&](uint32_t r) {
         uint64_t items = 0;
         for (const CacheSeg& s : segs) items += (((uint64_t)s.n_rows + KT - 1) / KT + r - 1) / r;
         return items * a.n_kv;
     };
-    if (MANY || segs.size() == 1)
+    if (MODE != FEW || segs.size() == 1)
         while (run < longest && count(run) > slots) ++run;
     else run = std::max(run / 3, std::min(run, 4u));
     uint64_t items = 0;
@@ -316,7 +367,7 @@ Status launch_observe_wide_t(Ctx* c, CacheArgs a, std::vector<CacheSeg>& segs, c
     CacheTable tab;
     SLHA_TRY(cache_table(c, segs, &tab, &a.table));
     a.n_segs = (uint32_t)segs.size();
-    constexpr auto kernel = cache_observe_wide_kernel<D, MANY>;
+    constexpr auto kernel = cache_observe_wide_kernel<D, MODE>;
     SLHA_TRY((cache_smem<kernel>(c, S::SMEM)));
     SLHA_CUDA(launch_behind(kernel, dim3((uint32_t)(items * a.n_kv)), dim3(S::THREADS), S::SMEM, c->stream, a, maps, tab));
     count_launch();
@@ -334,8 +385,12 @@ Status launch_observe_wide(Ctx* c, CacheArgs a, std::vector<CacheSeg> segs, uint
     if (!wide_map(&maps.k, a.keys, a.krs, a.khs, rows, a.n_kv, a.d, &maps.k_head_first)) return Status();
     maps.q_boxes = wide_row_map(&maps.q, a.q, a.qts, a.qhs, a);
     *taken = true;
-    if (a.d <= 64) return most_rows > 32 ? launch_observe_wide_t<64, true>(c, a, segs, maps) : launch_observe_wide_t<64, false>(c, a, segs, maps);
-    return most_rows > 32 ? launch_observe_wide_t<128, true>(c, a, segs, maps) : launch_observe_wide_t<128, false>(c, a, segs, maps);
+    uint32_t longest;
+    const uint32_t run = even_run(segs, a.n_kv, sm_count(c->device), &longest);
+    const int mode = most_rows <= 32 ? (run <= 8 ? FEW : MID) : most_rows <= 256 && run > 4 ? MID : MANY;
+    if (a.d <= 64)
+        return mode == FEW ? launch_observe_wide_t<64, FEW>(c, a, segs, maps) : mode == MID ? launch_observe_wide_t<64, MID>(c, a, segs, maps) : launch_observe_wide_t<64, MANY>(c, a, segs, maps);
+    return mode == FEW ? launch_observe_wide_t<128, FEW>(c, a, segs, maps) : mode == MID ? launch_observe_wide_t<128, MID>(c, a, segs, maps) : launch_observe_wide_t<128, MANY>(c, a, segs, maps);
 }
 
 }  // namespace slha

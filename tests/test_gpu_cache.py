@@ -837,3 +837,30 @@ def test_removal_by_clusters_of_every_size(n_kv, n, budget):
     got = src.download(np.uint32, n_kv * budget).reshape(n_kv, budget)
     for h in range(0, n_kv, max(1, n_kv // 4)):
         assert np.array_equal(got[h], K.evict(w[h], np.arange(n), budget, 3, 11))
+
+
+@pytest.mark.parametrize("n_kv,n,budget", [(1, 16384, 90), (3, 20001, 20000), (60, 17000, 500), (13, 70000, 600), (2, 65536, 65535)])
+def test_removal_from_long_caches(n_kv, n, budget):
+    test_removal_by_clusters_of_every_size(n_kv, n, budget)
+
+
+@pytest.mark.parametrize("tokens,group,lens", [(1, 4, (20000, 77)), (8, 4, (19990, 130)), (5, 1, (12000, 9000)), (9, 4, (10000,)), (64, 4, (9999,)), (43, 3, (5000, 129, 6000)), (65, 4, (3000,))])
+@pytest.mark.parametrize("more", [dict(), dict(softcap=5.0, alibi=True), dict(docs=True), dict(window=3000)])
+def test_weights_of_rows_in_long_runs_of_tiles(tokens, group, lens, more):
+    rng = np.random.default_rng(tokens * 7 + group)
+    kv, d, total = 8, 64, sum(lens)
+    kind = {k: v for k, v in more.items() if k in ("softcap", "window")}
+    if more.get("alibi"):
+        kind["slopes"] = (2.0 ** -np.arange(1, kv * group + 1) / 64).astype(F)
+    if more.get("docs"):
+        doc = np.sort(rng.integers(1, 4, total)).astype(np.uint32)
+        kind["row_doc"] = np.stack([doc] * kv)
+        kind["q_doc"] = rng.integers(1, 5, tokens * len(lens)).astype(np.uint32)
+    call, raw = make(rng, lens, tokens, kv, group, d, True, **kind)
+    cache, segs, queries = on_device(call, raw, True)
+    _, lse = results(call, True, cache, segs, queries)
+    before = rng.random((kv, total)).astype(F)
+    w = S.to_device(before)
+    S.observe_cache(cache, segs, queries, S.to_device(lse), w, total, weights_in=w, decay=0.5)
+    want, tol = call.received(lse, before, 0.5)
+    held(w.download(F, kv * total).reshape(kv, total), want, tol)
