@@ -5,6 +5,9 @@
 // in one pass over the rows: a running maximum m and sum l a query row, out's sums scaled by exp(m_old - m_new) when the maximum grows.  Scores are held in
 // units of log 2 (exp is one instruction there).
 //
+// One token's work is bound by the bytes of its rows: 131072 rows of 8 KV heads of 128 dimensions (537 MB), scores capped, 92 to 100 us = 5.4 to 5.8 TB/s; 48 sequences of 6000
+// on the average with positions and a distance bias 220 to 229 us (1.2 GB, 5.3 to 5.5 TB/s); 512 rows 6.5 us: a launch and the chain of one tile's loads, products, softmax and the join.  float32 rows are bound by the products (three of tf32 for one): 5 x 37 tokens of 12 heads of 96 dimensions over 1500 rows each 50 us.
+//
 // A CTA takes a block of 16, 32 or 64 query rows of one KV head (row = token x the head's group of query heads, so that the keys are read once for the group) and
 // a run of the segment's rows in tiles of 64 (float32: 32).  Four warps: with 16 query rows each takes a quarter of a tile's keys, with 64 each takes
 // its own 16 rows.  Tiles arrive by cp.async, two or three ahead.
@@ -536,6 +539,7 @@ static void cut(CacheWork* w, uint32_t group, uint32_t mb, uint32_t kt, uint32_t
 // The longest run of tiles of an item.  In units of a tile's time: what fits on the GPU at once takes as long as its longest item, more than that the mean load
 // and half an item at the end; an item costs about four tiles to begin, joining about three and a little for every part.
 // *cluster: how many CTAs share a block of query rows and join their sums through each other's shared memory, where that takes less time than a second kernel (0: none do).
+// One token over 512 rows: 6.5 us by a cluster, 8.0 by a second kernel; 8 x 4096 rows 26.2 and 28.7; 1 x 2048, where more than eight parts are worth it, 9.1 and 8.5.
 static uint32_t longest_run(const CacheWork& w, uint32_t group, uint32_t mb, uint32_t kt, uint32_t n_kv, uint32_t slots, uint32_t* cluster) {
     uint32_t most = 1;
     double total = 0.0;
@@ -580,7 +584,7 @@ Status launch_cache_join(Ctx* c, CacheArgs a, int dtype, const CacheWork& w, uin
     CacheTable tab;
     SLHA_TRY(cache_table(c, split, &tab, &a.table));
     a.n_segs = (uint32_t)split.size();
-    // four warps a row where it has many parts (35 parts of a row: 19 us with one warp, 5 with four)
+    // four warps a row where it has many parts (131072 rows in 35 parts: 90 us in all with one warp, 84 with four; 64 x 4096 rows in 2 parts 177 with one, 180 with four)
     const uint32_t warps = w.chunks > 8 ? 4 : 1, at_once = JOIN_THREADS / 32 / warps, per = (rows + at_once - 1) / at_once;
     if (w.blocks * a.n_kv * per > 0x7FFFFFFFull) return Status(SLHA_ERR_CAPACITY, "attention over a cache: too many blocks of query rows");
     const dim3 grid((uint32_t)(w.blocks * a.n_kv * per));
@@ -646,7 +650,7 @@ Status launch_attend_cache(Ctx* c, CacheArgs a, int dtype, const std::vector<Slh
     // the kernel that suits it.  8 KV heads of 128 dimensions, us in blocks of 16, 32, 64 query rows and with the kernel for many (whose tensor cores take 128 rows at a time):
     //   bfloat16, 16 x 8192 rows: 4 query rows 82, 100, 138, 116; 16: 84, 104, 144, 120; 20: 140, 106, 145, 120; 32: 141, 107, 147, 119; 36: -, 194, 148, 120; 256: -, 724, 615, 140
     //             1 x 4096 rows: 4 query rows 10.0, 10.8, 12.4, 14.1; 20: 12.8, 13.5, 16.7, 16.2; 36: -, 15.6, 17.6, 16.5; 256: -, 35, 32, 24
-    //   float32, 4 x 2048 rows: 16 query rows 30, 78, 58; 32: 49, 81, 59; 64: 90, 93, 63 (blocks of 32 hold two CTAs' registers and are never the quickest: 16 up to 32 rows)
+    //   float32, 4 x 2048 rows: 16 query rows 30, 78, 58; 32: 49, 81, 59; 64: 90, 93, 63 (blocks of 32 are never the quickest)
     CacheWork of[3];
     for (size_t i = 0; i < segs.size(); ++i) {
         const SlhaB200Segment& s = segs[i];

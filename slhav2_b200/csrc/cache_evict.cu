@@ -3,6 +3,10 @@
 // Two kernels.  The first, a CTA for each KV head of a segment, finds which min(n, budget) of the n rows stay: the budget-th largest of the rows' keys by
 // radix selection (11 bits, 11, 10), equal keys by the lower row, and writes for each place below the budget the row that comes to it.  The
 // second moves rows.  A kept row below the budget stays where it is, so in place only rows from beyond the budget move, into places that no row is read from.
+//
+// Bound by latency where caches are short (1100 rows, 1024 stay: 13.5 us, two launches and three passes over a few words) and by bytes where rows move: 8 prompts of up to 32768 rows
+// into caches of 4096, tiles with them, 96 us, of which the selection is 41 (its words are read once, into shared memory; the passes over them are bound by shared atomics and barriers)
+// and the moving 55 (6.2 TB/s).
 #include <cooperative_groups.h>
 
 #include <algorithm>

@@ -3,6 +3,8 @@
 //
 // With lse at hand a row's weight is a sum of its own column, so a CTA takes 128 keys (float32: 64) of one KV head, which stay in shared memory (and as operands in
 // registers), and goes through the segment's query rows: every key is read once, no sum is shared between CTAs and their order is fixed.
+// With few query rows bound by the rows' bytes (8 KV heads of 128 dimensions, 8 x 8192 rows, 4 query rows: 40 us, 3.5 TB/s), with many by the products and exponentials (256 query
+// rows over 32768 rows: 119 us).  bfloat16 rows of up to 128 dimensions have a kernel that takes 25 and 40 us for these (cache_observe_wide.cu).
 #include <cuda_bf16.h>
 
 #include <algorithm>

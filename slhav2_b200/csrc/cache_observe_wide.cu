@@ -3,6 +3,8 @@
 // Scores as S^T = K Q^T on tcgen05: a tile of 128 keys is the M side, so that a thread has a key's scores in its own TMEM lane and its weight is a sum over the thread's own
 // columns: no sum crosses threads (with many query rows four threads share a key).  A CTA takes the queries of one KV head, which stay in shared memory, and a run of key tiles,
 // each of which is read once (TMA, the tile behind which a segment ends by cp.async).  While one block of scores is summed, the next is multiplied.
+// With few query rows bound by the rows' bytes (16 sequences of 5750 rows on the average after a decode step: 39 us, 5.0 TB/s), with many by one exponential a score and what surrounds it (256 query
+// rows of 8 KV heads over 32768 rows: 39 us, 1.7e12 scores a second; the special-function units alone would take 15 us).
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -18,11 +20,12 @@ constexpr int KT = 128;
 // FEW: up to 32 query rows, a thread a key, two CTAs an SM, blocks of scores in two places by turns.  MID: up to 256, four groups of 128 threads, each with a tile and a place of its
 // own, so that no sum crosses threads and nobody waits for another group.  MANY: up to 512, four threads a key, two places by turns.
 //
-// MID wants four tiles at a time and a run of them behind those, so FEW takes up to 32 query rows in runs of up to 8 tiles, and MANY what has more rows in runs of up to 4.
-// Measured, 8 KV heads of 128 dimensions, us:
-//   64 sequences of 1024 rows (runs of 8), 4 query rows: FEW 33, MID 39, MANY 49; one of 8192 (4): 5.6, 6.0, 7.4; 8 of 8192 (28): 32, 25, 36; with 32 query rows 38, 27, 40
-//   one sequence of 4096 rows (2), 64 query rows: MID 9.0, MANY 7.1; of 16384 (7): 13.9, 14.9; of 32768 (14): 16, 22; with 256 query rows 40, 43
-// and cache_observe.cu's kernel takes 40, 56 (4, 32 query rows on 8 of 8192), 39, 119 (64, 256 on 32768): it takes rows beyond 512 query rows, 128 dimensions, and float32.
+// MID wants four tiles at a time and a run of them behind those, and has one CTA an SM: FEW takes up to 32 query rows where an SM's share is 8 tiles or less, and up to 16 where runs for
+// all SMs would be uneven; MANY takes more than 32 where that share is 4 or less.  Measured, 8 KV heads of 128 dimensions, us:
+//   4 query rows, sequences: 64 x 1024 rows (runs of 8) FEW 31, MID 39, MANY 49; 1 x 8192 (4) 5.6, 6.0, 7.4; 8 x 8192 (28) 27, 25, 36; 16 of 2700 to 8192 35, 38
+//   32 query rows: 64 x 1024 41, 47, 57; 32 x 4096 62, 54, 79; 8 x 8192 38, 27, 40
+//   64 query rows: 1 x 4096 (2) MID 9.0, MANY 7.1; 1 x 16384 (7) 13.9, 14.9; 1 x 32768 (14) 16, 22; 256 query rows on 1 x 32768 40, 43
+// and cache_observe.cu's kernel takes 40, 56 (4, 32 query rows on 8 x 8192), 39, 119 (64, 256 on 32768): it takes rows beyond 512 query rows, 128 dimensions, and float32.
 enum { FEW = 0, MID = 1, MANY = 2 };
 template <int D, int MODE>
 struct Obs {
@@ -330,32 +333,35 @@ __global__ void __launch_bounds__(Obs<D, MODE>::THREADS, Obs<D, MODE>::CTAS)
     if (warp == S::MMA_WARP) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(S::TMEM) : "memory");
 }
 
-// The run of tiles of which as many as there are places make up all rows, at most the longest segment's.
-uint32_t even_run(const std::vector<CacheSeg>& segs, uint32_t n_kv, uint64_t places, uint32_t* longest) {
-    uint64_t total = 0;
-    *longest = 1;
-    for (const CacheSeg& s : segs) {
-        const uint32_t tiles = (uint32_t)(((uint64_t)s.n_rows + KT - 1) / KT);
-        total += (uint64_t)tiles * n_kv;
-        *longest = std::max(*longest, tiles);
+// How long runs of tiles may be: evenly shared by so many places, and so long that there is one for each place at most (`once`, unless the segments are too many or too short).
+struct Runs {
+    uint32_t even, fit = 1;
+    bool once = true;
+    Runs(const std::vector<CacheSeg>& segs, uint32_t n_kv, uint64_t places) {
+        uint64_t total = 0;
+        uint32_t longest = 1;
+        const auto tiles = [](const CacheSeg& s) { return (uint32_t)(((uint64_t)s.n_rows + KT - 1) / KT); };
+        for (const CacheSeg& s : segs) {
+            total += (uint64_t)tiles(s) * n_kv;
+            longest = std::max(longest, tiles(s));
+        }
+        even = (uint32_t)std::min<uint64_t>(longest, (total + places - 1) / places);
+        for (fit = even;; ++fit) {
+            uint64_t items = 0;
+            for (const CacheSeg& s : segs) items += (tiles(s) + fit - 1) / fit;
+            once = items * n_kv <= places;
+            if (once || fit == longest) break;
+        }
     }
-    return (uint32_t)std::min<uint64_t>(*longest, (total + places - 1) / places);
-}
+};
 
 template <int D, int MODE>
 Status launch_observe_wide_t(Ctx* c, CacheArgs a, std::vector<CacheSeg>& segs, const ObsMaps& maps) {
     using S = Obs<D, MODE>;
-    // Runs of tiles: as long as all CTAs that fit on the GPU at once have one (MID, MANY), or a few each, which hide one another's beginning and end.
-    const uint64_t slots = (uint64_t)sm_count(c->device) * S::CTAS;
-    uint32_t longest, run = even_run(segs, a.n_kv, slots, &longest);
-    const auto count = [&](uint32_t r) {
-        uint64_t items = 0;
-        for (const CacheSeg& s : segs) items += (((uint64_t)s.n_rows + KT - 1) / KT + r - 1) / r;
-        return items * a.n_kv;
-    };
-    if (MODE != FEW || segs.size() == 1)
-        while (run < longest && count(run) > slots) ++run;
-    else run = std::max(run / 3, std::min(run, 4u));
+    // One run for each CTA that fits on the GPU at once, or of FEW, whose second CTA of an SM hides the first one's beginning and end, where such runs would be uneven (16 sequences of
+    // 2700 to 8192 rows: 43 us, 39 in runs of two thirds) one and a half.
+    const Runs r(segs, a.n_kv, (uint64_t)sm_count(c->device) * S::CTAS);
+    const uint32_t run = MODE != FEW || r.fit <= std::max(4u, r.even + r.even / 10) ? r.fit : std::max(4u, r.even * 2 / 3);
     uint64_t items = 0;
     for (CacheSeg& s : segs) {
         const uint32_t tiles = (uint32_t)(((uint64_t)s.n_rows + KT - 1) / KT), parts = (tiles + run - 1) / run;
@@ -385,9 +391,9 @@ Status launch_observe_wide(Ctx* c, CacheArgs a, std::vector<CacheSeg> segs, uint
     if (!wide_map(&maps.k, a.keys, a.krs, a.khs, rows, a.n_kv, a.d, &maps.k_head_first)) return Status();
     maps.q_boxes = wide_row_map(&maps.q, a.q, a.qts, a.qhs, a);
     *taken = true;
-    uint32_t longest;
-    const uint32_t run = even_run(segs, a.n_kv, sm_count(c->device), &longest);
-    const int mode = most_rows <= 32 ? (run <= 8 ? FEW : MID) : most_rows <= 256 && run > 4 ? MID : MANY;
+    const Runs r(segs, a.n_kv, sm_count(c->device));
+    const bool even = r.once && r.fit <= r.even + r.even / 5;
+    const int mode = most_rows <= 32 && (r.even <= 8 || (most_rows <= 16 && !even)) ? FEW : most_rows <= 256 && (most_rows <= 32 || r.even > 4) ? MID : MANY;
     if (a.d <= 64)
         return mode == FEW ? launch_observe_wide_t<64, FEW>(c, a, segs, maps) : mode == MID ? launch_observe_wide_t<64, MID>(c, a, segs, maps) : launch_observe_wide_t<64, MANY>(c, a, segs, maps);
     return mode == FEW ? launch_observe_wide_t<128, FEW>(c, a, segs, maps) : mode == MID ? launch_observe_wide_t<128, MID>(c, a, segs, maps) : launch_observe_wide_t<128, MANY>(c, a, segs, maps);
