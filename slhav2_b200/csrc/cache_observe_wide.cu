@@ -335,8 +335,8 @@ __global__ void __launch_bounds__(Obs<D, MODE>::THREADS, Obs<D, MODE>::CTAS)
 
 // How long runs of tiles may be: evenly shared by so many places, and so long that there is one for each place at most (`once`, unless the segments are too many or too short).
 struct Runs {
-    uint32_t even, fit = 1;
-    bool once = true;
+    uint32_t even, fit;
+    bool once;
     Runs(const std::vector<CacheSeg>& segs, uint32_t n_kv, uint64_t places) {
         uint64_t total = 0;
         uint32_t longest = 1;
@@ -346,11 +346,17 @@ struct Runs {
             longest = std::max(longest, tiles(s));
         }
         even = (uint32_t)std::min<uint64_t>(longest, (total + places - 1) / places);
-        for (fit = even;; ++fit) {
+        const auto fits = [&](uint32_t run) {
             uint64_t items = 0;
-            for (const CacheSeg& s : segs) items += (tiles(s) + fit - 1) / fit;
-            once = items * n_kv <= places;
-            if (once || fit == longest) break;
+            for (const CacheSeg& s : segs) items += ((uint64_t)tiles(s) + run - 1) / run;
+            return items * n_kv <= places;
+        };
+        fit = longest;
+        once = fits(longest);
+        for (uint32_t low = even; once && low < fit;) {  // (longer runs are never more)
+            const uint32_t mid = low + (fit - low) / 2;
+            if (fits(mid)) fit = mid;
+            else low = mid + 1;
         }
     }
 };
