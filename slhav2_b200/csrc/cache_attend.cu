@@ -232,11 +232,7 @@ __global__ void __launch_bounds__(ATT_THREADS, Shape<T, D, WM>::CTAS) cache_atte
 #pragma unroll
                 for (int kk = 0; kk < KSTEPS; ++kk) scores_step<T, D, S::NT>(s, qa[kk], st, key0, kk, lane);
             } else {
-#pragma unroll 4
-                for (int kk = 0; kk < KSTEPS; ++kk) {
-                    qa[0].template load<D>(sq, wm * 16, kk, lane);
-                    scores_step<T, D, S::NT>(s, qa[0], st, key0, kk, lane);
-                }
+                scores_of<T, D, S::NT>(s, [&](int kk) -> const AFrag<T>& { qa[0].template load<D>(sq, wm * 16, kk, lane); return qa[0]; }, st, key0, lane);
             }
             // scores in units of log 2
 #pragma unroll

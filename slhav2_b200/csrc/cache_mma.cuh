@@ -119,6 +119,26 @@ __device__ __forceinline__ void scores_step(float (&s)[N][4], const AFrag<T>& a,
         }
     }
 }
+// All k steps of s[n][.] = Q K^T; load(kk) brings the A operand of one.  The tensor cores cut each product's sum off towards zero: float32 sums are taken four steps at a time and added
+// here, to the nearest (7 x 18 drafted tokens over 390 rows, 128 dimensions: outputs 2.2e-6 off without, 6.5e-7 with; 5 % of the time).
+template <typename T, int D, int N, typename Load>
+__device__ __forceinline__ void scores_of(float (&s)[N][4], Load load, uint32_t kbase, int key0, int lane) {
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll 4
+        for (int kk = 0; kk < D / 16; ++kk) scores_step<T, D, N>(s, load(kk), kbase, key0, kk, lane);
+    } else {
+#pragma unroll 1
+        for (int k4 = 0; k4 < D / 8; k4 += 4) {
+            float part[N][4] = {};
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) scores_step<T, D, N>(part, load(k4 + kk), kbase, key0, k4 + kk, lane);
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[n][e] += part[n][e];
+        }
+    }
+}
 // o[.] += P V for the 8 N keys from key0 on; p as scores_step leaves its sums (a thread's columns 2t and 2t + 1: for float32 they stand for the k indices t and
 // t + 4, the rows of V accordingly)
 template <typename T, int D, int N>
@@ -137,19 +157,25 @@ __device__ __forceinline__ void values_step(float (&o)[D / 8][4], const float (&
         }
     } else {
         const int g = lane >> 2, t = lane & 3;
+        uint32_t h[N][4], l[N][4];
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            uint32_t h[4], l[4];
-            tf32_split(p[n][0], h[0], l[0]);
-            tf32_split(p[n][2], h[1], l[1]);
-            tf32_split(p[n][1], h[2], l[2]);
-            tf32_split(p[n][3], h[3], l[3]);
+            tf32_split(p[n][0], h[n][0], l[n][0]);
+            tf32_split(p[n][2], h[n][1], l[n][1]);
+            tf32_split(p[n][1], h[n][2], l[n][2]);
+            tf32_split(p[n][3], h[n][3], l[n][3]);
+        }
 #pragma unroll
-            for (int d = 0; d < D / 8; ++d) {
+        for (int d = 0; d < D / 8; ++d) {
+            float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // (as for the scores)
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
                 const float b0 = __uint_as_float(lds(Tile<T, D>::elem(vbase, key0 + n * 8 + 2 * t, d * 8 + g)));
                 const float b1 = __uint_as_float(lds(Tile<T, D>::elem(vbase, key0 + n * 8 + 2 * t + 1, d * 8 + g)));
-                mma_f32(o[d], h, l, b0, b1);
+                mma_f32(part, h[n], l[n], b0, b1);
             }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[d][e] += part[e];
         }
     }
 }

@@ -149,15 +149,19 @@ __global__ void __launch_bounds__(OBS_THREADS) cache_observe_kernel(const __grid
 #pragma unroll
                 for (int i = 0; i < S::NT; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.0f;
                 AFrag<T> q;
-#pragma unroll
-                for (int kk = 0; kk < KSTEPS; ++kk) {
+                const auto load = [&](int kk) -> const AFrag<T>& {
                     q.template load<D>(sq, r0, kk, lane);
-                    if constexpr (S::HELD) {
+                    return q;
+                };
+                if constexpr (S::HELD) {
+#pragma unroll
+                    for (int kk = 0; kk < KSTEPS; ++kk) {
+                        load(kk);
 #pragma unroll
                         for (int i = 0; i < S::NT; ++i) mma_bf16(s[i], q.a, kf[kk][2 * i], kf[kk][2 * i + 1]);
-                    } else {
-                        scores_step<T, D, S::NT>(s, q, sb, key0, kk, lane);
                     }
+                } else {
+                    scores_of<T, D, S::NT>(s, load, sb, key0, lane);
                 }
                 const int ra = r0 + g;
                 const float lse[2] = {__uint_as_float(rows[3 * QB + ra]), __uint_as_float(rows[3 * QB + ra + 8])};
