@@ -6,7 +6,7 @@
 // units of log 2 (exp is one instruction there).
 //
 // One token's work is bound by the bytes of its rows: 131072 rows of 8 KV heads of 128 dimensions (537 MB), scores capped, 92 to 100 us = 5.4 to 5.8 TB/s; 48 sequences of 6000
-// on the average with positions and a distance bias 220 to 229 us (1.2 GB, 5.3 to 5.5 TB/s); 512 rows 6.5 us: a launch and the chain of one tile's loads, products, softmax and the join.  float32 rows are bound by the products (three of tf32 for one): 5 x 37 tokens of 12 heads of 96 dimensions over 1500 rows each 50 us.
+// on the average with positions and a distance bias 220 to 229 us (1.2 GB, 5.3 to 5.5 TB/s); 512 rows 6.5 us: a launch and the chain of one tile's loads, products, softmax and the join.  float32 rows are bound by the products (three of tf32 for one): 5 x 37 tokens of 12 heads of 96 dimensions over 1500 rows each 54 us.
 //
 // A CTA takes a block of 16, 32 or 64 query rows of one KV head (row = token x the head's group of query heads, so that the keys are read once for the group) and
 // a run of the segment's rows in tiles of 64 (float32: 32).  Four warps: with 16 query rows each takes a quarter of a tile's keys, with 64 each takes

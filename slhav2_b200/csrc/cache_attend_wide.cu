@@ -142,7 +142,7 @@ __device__ __noinline__ void by_rows(const CacheArgs& a, const Item& w, const ui
 // A tile's scores that are more than products: capped, biased, masked.  Read from TMEM and written back, 32 columns at a time, in units of log 2 where a cap or a distance bends them; where
 // all that a warp's rows see of 32 columns is all, they stay as they are.  (A function, in loops that are hardly
 // unrolled, so that the loop over the tiles stays short: where the same stood in it, every tile's weights took 15 % longer.)  False where a wait ran out.
-template <int D>
+template <int D, bool SLOPED>
 __device__ __noinline__ bool bend_tile(const CacheArgs& a, unsigned char* sm, uint32_t ts, uint32_t r, uint32_t t, uint32_t li) {
     using S = Wide<D>;
     const Item& w = *reinterpret_cast<const Item*>(sm + S::ITEM_AT);
@@ -150,7 +150,8 @@ __device__ __noinline__ bool bend_tile(const CacheArgs& a, unsigned char* sm, ui
     const uint32_t bars = smem_addr(sm) + S::BAR_AT;
     const auto bar = [&](int which) { return bars + which * 8; };
     const uint32_t what = reinterpret_cast<const uint32_t*>(sm + S::LIST_AT)[li], first = (what >> 2) * KT, n = w.n, ctx = w.ctx;
-    const bool all = what >> t & 1, has_slope = a.slopes, drafts = a.tree && first + KT > ctx;
+    constexpr bool has_slope = SLOPED;
+    const bool all = what >> t & 1, drafts = a.tree && first + KT > ctx;
     const bool by_pos = a.row_pos || (w.drafts_listed && drafts), listed = !all && (w.arrays || (w.drafts_listed && drafts));  // the fetching warp has left the rows' positions
     if ((has_slope || listed) && !__all_sync(0xFFFFFFFFu, bar_wait(bar(META_FULL + (li & 3)), li >> 2 & 1))) return false;
     const uint4* kp4 = reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(sm + S::META_AT) + (li & 3) * 3 * KT);
@@ -254,9 +255,10 @@ __device__ __noinline__ bool bend_tile(const CacheArgs& a, unsigned char* sm, ui
     return true;
 }
 
-// CAP: scores are capped.  RICH: rows with positions or documents of their own, tokens with positions of their own, trees, or a distance bias.  (Instances of their own: what a
-// kernel does not need costs it registers and instruction cache in the loop over the tiles; with all in one, 8192 tokens of 32 heads took 937 us, alone 876.)
-template <int D, bool CAP, bool RICH>
+// CAP: scores are capped.  RICH: rows with positions or documents of their own, tokens with positions of their own, or trees; SLOPED: these or not, and a distance bias.  (Instances of
+// their own: what a kernel does not need costs it registers and instruction cache in the loop over the tiles; with all in one, 8192 tokens of 32 heads took 937 us, alone 876.)
+enum { PLAIN = 0, RICH = 1, SLOPED = 2 };
+template <int D, bool CAP, int KIND>
 __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __grid_constant__ CacheArgs a, const __grid_constant__ WideMaps maps, const __grid_constant__ CacheTable tab) {
     using S = Wide<D>;
     dep_wait();
@@ -283,7 +285,8 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
     w.sight = CacheSight{a.window_last, a.prefix ? a.prefix[w.sg.seg] : 0u, a.causal};
     const CacheSight sight = w.sight;
     w.entry = w.head * a.entry_hs + w.sg.row_begin;
-    const bool has_pos = RICH && a.row_pos, has_doc = RICH && a.row_doc, has_slope = RICH && a.slopes, is_tree = RICH && a.tree;
+    constexpr bool has_slope = KIND == SLOPED;
+    const bool has_pos = KIND != PLAIN && a.row_pos, has_doc = KIND != PLAIN && a.row_doc, is_tree = KIND != PLAIN && a.tree;
     constexpr bool has_cap = CAP;
     const uint32_t used = min((uint32_t)MB, w.q_rows - w.row0);
     const bool two = used > 128;
@@ -307,7 +310,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
     const uint32_t tok0 = w.row0 / a.group;
 
     const bool arrays = has_pos || has_doc, drafts_listed = is_tree && (arrays || a.q_pos || sight.window_last != 0xFFFFFFFFu);  // drafted rows whose positions count
-    const bool plain = !RICH || (!arrays && !a.q_pos);  // all positions follow from the segment
+    const bool plain = KIND == PLAIN || (!arrays && !a.q_pos);  // all positions follow from the segment
     const uint32_t near_pos = a.q_pos ? a.q_pos[w.sg.query_begin + tok0] : w.sg.base + w.ctx + (is_tree ? 0u : tok0);
     w.near_pos = near_pos;
     w.arrays = arrays;
@@ -539,8 +542,21 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
                 }
                 tc_after();
                 const bool all = s_list[li] >> t & 1;
-                const bool bent = !all || has_slope;
-                if (bent && !bend_tile<D>(a, sm, ts, r, t, li)) {
+                // Where a tile is seen as a whole and the warp's rows all have it on one side, the bias is near + step column, added on the way to the weights; its largest score is then only
+                // bounded, by the largest product and the largest bias, which may be 2^64 too high and still leaves weights from 2^-62 of the row's largest on.
+                // (8192 causal tokens, 32 heads: 961 us with all tiles bent, 534 so.)
+                bool straight = false;
+                float step = 0.0f, near = 0.0f;
+                if constexpr (has_slope && !CAP) {
+                    const long long at = (long long)w.sg.base + (s_list[li] >> 2) * KT;
+                    const bool after = (long long)s_qp[r] >= at + KT - 1;
+                    const float slope = s_slope[r];
+                    step = after ? slope : -slope;
+                    near = -slope * fabsf((float)((long long)s_qp[r] - at));
+                    straight = __all_sync(0xFFFFFFFFu, all && !has_pos && !is_tree && (after || (long long)s_qp[r] <= at) && fabsf(slope) * (KT - 1) <= 64.0f);
+                }
+                const bool bent = !straight && (!all || has_slope);
+                if (bent && !bend_tile<D, has_slope>(a, sm, ts, r, t, li)) {
                     fail = true;
                     break;
                 }
@@ -573,7 +589,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
                     if (fused) {  // (tanh grows: the largest score is that of the largest product)
                         top = cap2 * tanh_small(x);
                     } else {
-                        if (!bend_tile<D>(a, sm, ts, r, t, li)) {
+                        if (!bend_tile<D, has_slope>(a, sm, ts, r, t, li)) {
                             fail = true;
                             break;
                         }
@@ -587,6 +603,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
 #pragma unroll
                         for (int e = 0; e < 4; ++e) x[e] = fmaxf(x[e], fmaxf(s[c + 2 * e], s[c + 2 * e + 1]));
                     top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * mul;
+                    if (straight) top += fmaxf(near, fmaf(step, KT - 1, near));
                 }
                 if (__any_sync(0xFFFFFFFFu, top > m + LAZY)) {
                     const float now = fmaxf(m, top), f = m == -INFINITY ? 0.0f : exp2_fast(m - now);
@@ -606,6 +623,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
                 const float use = m == -INFINITY ? 0.0f : m;
                 const uint64_t mul_2 = pair(mul, mul), use_2 = pair(-use, -use);
                 uint64_t sum_a = pair(0.0f, 0.0f), sum_b = sum_a;
+                constexpr int BIASED = 3;
                 const auto weights = [&](auto capped) {
                     const uint64_t in = pair(to_log2, to_log2), out = pair(cap2, cap2);
 #pragma unroll
@@ -615,9 +633,11 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
                         for (int e = 0; e < 32; e += 2) {
                             float x, y;
                             uint64_t z = pair(s[c + e], s[c + e + 1]);
-                            if constexpr (decltype(capped)::value) {
+                            if constexpr (decltype(capped)::value == 1 || decltype(capped)::value == 2) {
                                 z = mul2(z, in);
                                 z = fma2(mul2(z, decltype(capped)::value == 1 ? tanh_poly(mul2(z, z)) : tanh_poly_brief(mul2(z, z))), out, use_2);
+                            } else if constexpr (decltype(capped)::value == BIASED) {
+                                z = fma2(z, mul_2, pair(fmaf(step, (float)(c + e), near - use), fmaf(step, (float)(c + e + 1), near - use)));
                             } else {
                                 z = fma2(z, mul_2, use_2);
                             }
@@ -640,6 +660,8 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
                     if (brief) weights(std::integral_constant<int, 2>());
                     else if (fused) weights(std::integral_constant<int, 1>());
                     else weights(std::integral_constant<int, 0>());
+                } else if (has_slope && straight) {
+                    weights(std::integral_constant<int, BIASED>());
                 } else {
                     weights(std::integral_constant<int, 0>());
                 }
@@ -909,7 +931,7 @@ void wide_share(const CacheArgs& a, CacheWork* w, uint32_t slots) {
     }
 }
 
-template <int D, bool CAP, bool RICH>
+template <int D, bool CAP, int KIND>
 Status launch_wide(Ctx* c, CacheArgs a, CacheWork w, const WideMaps& maps) {
     using S = Wide<D>;
     wide_share(a, &w, (uint32_t)sm_count(c->device));
@@ -919,17 +941,25 @@ Status launch_wide(Ctx* c, CacheArgs a, CacheWork w, const WideMaps& maps) {
     a.n_segs = (uint32_t)w.segs.size();
     CacheMemory mem{c};
     SLHA_TRY(cache_part_memory(&a, w, MB, &mem));
-    constexpr auto kernel = cache_attend_wide_kernel<D, CAP, RICH>;
+    constexpr auto kernel = cache_attend_wide_kernel<D, CAP, KIND>;
     SLHA_TRY((cache_smem<kernel>(c, S::SMEM_TREE)));
     static const int regs = []() {
         cudaFuncAttributes at;
-        return cudaFuncGetAttributes(&at, cache_attend_wide_kernel<D, CAP, RICH>) == cudaSuccess ? at.numRegs : 0;
+        return cudaFuncGetAttributes(&at, cache_attend_wide_kernel<D, CAP, KIND>) == cudaSuccess ? at.numRegs : 0;
     }();
     if (regs != REGS_ALL) return Status(SLHA_ERR_DEVICE, "attention over a cache: the kernel was built with other registers than its warps share out");
     SLHA_CUDA(launch_behind(kernel, dim3((uint32_t)(w.items * a.n_kv)), dim3(THREADS), a.tree ? S::SMEM_TREE : S::SMEM, c->stream, a, maps, tab));
     count_launch();
     if (w.blocks) SLHA_TRY(launch_cache_join(c, a, SLHA_B200_BF16, w, MB));
     return mem.done();
+}
+
+template <int D>
+Status launch_wide_d(Ctx* c, const CacheArgs& a, CacheWork w, const WideMaps& maps, int kind) {
+    const bool cap = a.cap > 0.0f;
+    if (kind == PLAIN) return cap ? launch_wide<D, true, PLAIN>(c, a, std::move(w), maps) : launch_wide<D, false, PLAIN>(c, a, std::move(w), maps);
+    if (kind == RICH) return cap ? launch_wide<D, true, RICH>(c, a, std::move(w), maps) : launch_wide<D, false, RICH>(c, a, std::move(w), maps);
+    return cap ? launch_wide<D, true, SLOPED>(c, a, std::move(w), maps) : launch_wide<D, false, SLOPED>(c, a, std::move(w), maps);
 }
 
 }  // namespace
@@ -943,12 +973,8 @@ Status launch_attend_wide(Ctx* c, CacheArgs a, CacheWork w, bool* taken) {
     if (!*taken) return Status();
     maps.q_boxes = wide_row_map(&maps.q, a.q, a.qts, a.qhs, a);
     maps.out_boxes = wide_row_map(&maps.out, a.out, a.ots, a.ohs, a);
-    const bool rich = a.row_pos || a.row_doc || a.q_pos || a.slopes || a.tree;
-    if (a.d <= 64)
-        return a.cap > 0.0f ? (rich ? launch_wide<64, true, true>(c, a, std::move(w), maps) : launch_wide<64, true, false>(c, a, std::move(w), maps))
-                            : (rich ? launch_wide<64, false, true>(c, a, std::move(w), maps) : launch_wide<64, false, false>(c, a, std::move(w), maps));
-    return a.cap > 0.0f ? (rich ? launch_wide<128, true, true>(c, a, std::move(w), maps) : launch_wide<128, true, false>(c, a, std::move(w), maps))
-                        : (rich ? launch_wide<128, false, true>(c, a, std::move(w), maps) : launch_wide<128, false, false>(c, a, std::move(w), maps));
+    const int kind = a.slopes ? SLOPED : a.row_pos || a.row_doc || a.q_pos || a.tree ? RICH : PLAIN;
+    return a.d <= 64 ? launch_wide_d<64>(c, a, std::move(w), maps, kind) : launch_wide_d<128>(c, a, std::move(w), maps, kind);
 }
 
 }  // namespace slha

@@ -864,3 +864,21 @@ def test_weights_of_rows_in_long_runs_of_tiles(tokens, group, lens, more):
     S.observe_cache(cache, segs, queries, S.to_device(lse), w, total, weights_in=w, decay=0.5)
     want, tol = call.received(lse, before, 0.5)
     held(w.download(F, kv * total).reshape(kv, total), want, tol)
+
+
+@pytest.mark.parametrize("more", [dict(), dict(causal=False), dict(window=333), dict(docs=True), dict(prefix=np.array([200, 0, 650], np.uint32)), dict(softcap=9.0), dict(ahead=True)])
+@pytest.mark.parametrize("size", [0.003, 0.3, -0.05, 3.0])
+def test_wide_blocks_whose_bias_grows_by_the_row(more, size):
+    # slopes that differ by head, some zero: tiles before, behind and around the tokens; sizes on both sides of where the largest score is only bounded
+    rng = np.random.default_rng(91)
+    lens, tokens, kv, group, d = (1500, 131, 700), 70, 2, 4, 64
+    kind = {k: v for k, v in more.items() if k in ("causal", "window", "prefix", "softcap")}
+    kind["slopes"] = (size * np.array([1, 0.5, 0, 0.25, 1, 1, 0.9, 0.7])).astype(F)
+    if more.get("docs"):
+        doc = np.concatenate([np.sort(rng.integers(1, 3, n)) for n in lens]).astype(np.uint32)
+        kind["row_doc"] = np.stack([doc] * kv)
+        kind["q_doc"] = np.concatenate([doc[e - tokens:e] for e in np.cumsum(lens)])
+    if more.get("ahead"):  # tokens far before and far behind all rows
+        kind["q_pos"] = np.concatenate([np.arange(tokens), 5000000 + np.arange(tokens), 300 + 3 * np.arange(tokens)]).astype(np.uint32)
+        kind["causal"] = False
+    check(*make(rng, lens, tokens, kv, group, d, True, **kind), True)
