@@ -5,7 +5,7 @@
 // second moves rows.  A kept row below the budget stays where it is, so in place only rows from beyond the budget move, into places that no row is read from.
 //
 // Bound by latency where caches are short (1100 rows, 1024 stay: 13.5 us, two launches and three passes over a few words) and by bytes where rows move: 8 prompts of up to 32768 rows
-// into caches of 4096, tiles with them, 96 us, of which the selection is 41 (its words are read once, into shared memory; the passes over them are bound by shared atomics and barriers)
+// into caches of 4096, tiles with them, 94 us, of which the selection is 39 (its words are read once, into shared memory; the passes over them are bound by shared atomics and barriers)
 // and the moving 55 (6.2 TB/s).
 #include <cooperative_groups.h>
 
@@ -74,6 +74,7 @@ __global__ void __cluster_dims__(C, 1, 1) __launch_bounds__(SEL_THREADS) cache_s
     constexpr int FLIGHT = 8;  // loads that a thread has under way
     const bool held = own <= SEL_HELD, kept_pos = a.recent && a.pos && held;
     if (tid == 0) s_last = 0;
+    for (int i = tid; i < SEL_BINS; i += SEL_THREADS) s_hist[i] = 0;
     __syncthreads();
     if (a.recent) {
         uint32_t last = a.pos ? 0u : sg.base + n - 1;
@@ -96,8 +97,15 @@ __global__ void __cluster_dims__(C, 1, 1) __launch_bounds__(SEL_THREADS) cache_s
     uint32_t newest = s_last;
     for (int r = 1; r < C; ++r) newest = max(newest, *cluster.map_shared_rank(&s_last, (rank_of + r) % C));
     const auto key_at = [&](uint32_t p, float x) { return weight_key(x, p < a.sink || (a.recent && newest - p < a.recent)); };
-    if (held) {
-        for (uint32_t i0 = tid; i0 < own; i0 += SEL_THREADS * FLIGHT) {
+    // (a warp whose keys are all alike, as where nothing has been seen yet, adds once)
+    const auto add = [&](uint32_t bin, bool in) {
+        int alike;
+        __match_all_sync(0xFFFFFFFFu, in ? bin : 0xFFFFFFFFu, &alike);
+        if (alike ? in && lane == 0 : in) atomicAdd(&s_hist[bin], alike ? 32u : 1u);
+    };
+    if (held) {  // the keys take their places, and are counted by their first 11 bits
+        for (uint32_t i00 = 0; i00 < own; i00 += SEL_THREADS * FLIGHT) {
+            const uint32_t i0 = i00 + tid;
             float x[FLIGHT];
             uint32_t p[FLIGHT];
 #pragma unroll
@@ -107,8 +115,12 @@ __global__ void __cluster_dims__(C, 1, 1) __launch_bounds__(SEL_THREADS) cache_s
                 p[f] = i < own ? (kept_pos ? s_key[i] : position(i)) : 0u;
             }
 #pragma unroll
-            for (int f = 0; f < FLIGHT; ++f)
-                if (i0 + f * SEL_THREADS < own) s_key[i0 + f * SEL_THREADS] = key_at(p[f], x[f]);
+            for (int f = 0; f < FLIGHT; ++f) {
+                const bool in = i0 + f * SEL_THREADS < own;
+                const uint32_t k = key_at(p[f], x[f]);
+                if (in) s_key[i0 + f * SEL_THREADS] = k;
+                add(k >> 21, in);
+            }
         }
     }
     // four rows' keys from row i on (of the CTA's); rows behind the warp's last: 0, which is below all that stay but perhaps their equal
@@ -128,20 +140,18 @@ __global__ void __cluster_dims__(C, 1, 1) __launch_bounds__(SEL_THREADS) cache_s
     for (int pass = 0; pass < 3; ++pass) {
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
         const uint32_t bins = pass == 2 ? 1024u : 2048u, settled = pass == 0 ? 0u : pass == 1 ? 0xFFE00000u : 0xFFFFFC00u;
-        for (int i = tid; i < SEL_BINS; i += SEL_THREADS) s_hist[i] = 0;
-        __syncthreads();
-        for (uint32_t i0 = from; i0 < to; i0 += 128) {  // (a warp without rows begins at no multiple of 128)
+        if (pass > 0) {
+            for (int i = tid; i < SEL_BINS; i += SEL_THREADS) s_hist[i] = 0;
+            __syncthreads();
+        }
+        for (uint32_t i0 = from; i0 < to && !(held && pass == 0); i0 += 128) {  // (a warp without rows begins at no multiple of 128)
             const uint32_t i = i0 + lane * 4;
             uint32_t k[4];
             four(i, k);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const bool in = i + e < to && !((k[e] ^ prefix) & settled);
-                const uint32_t bin = (k[e] >> shift) & (bins - 1);
-                // (a warp whose keys are all alike, as where nothing has been seen yet, adds once)
-                int alike;
-                __match_all_sync(0xFFFFFFFFu, in ? bin : 0xFFFFFFFFu, &alike);
-                if (alike ? in && lane == 0 : in) atomicAdd(&s_hist[bin], alike ? 32u : 1u);
+                add((k[e] >> shift) & (bins - 1), in);
             }
         }
         if (C > 1) cluster.sync();
