@@ -93,9 +93,13 @@ __device__ __forceinline__ RowOut row_out(const CacheArgs& a, const Item& w, uin
 
 // The item again on the CUDA cores, a warp a query row and a row of the cache at a time, where only what is seen is read: for values that are not finite in a tile that not all see
 // (a weight of zero would not keep them out of the sums), and where a wait ran out.
-__device__ __noinline__ void by_rows(const CacheArgs& a, const Item& w, const uint32_t* s_qp, const uint32_t* s_qd, const float* s_slope, const uint32_t* s_tok, const uint32_t* s_depth,
-                                     const uint32_t* s_anc, const uint32_t* s_list, uint32_t cnt) {
+__device__ __noinline__ void by_rows(uint32_t bars, bool q_boxes, const CacheArgs& a, const Item& w, const uint32_t* s_qp, const uint32_t* s_qd, const float* s_slope, const uint32_t* s_tok,
+                                     const uint32_t* s_depth, const uint32_t* s_anc, const uint32_t* s_list, uint32_t cnt) {
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    // (where somebody gave up, copies may still be under way; a fill that was never begun lets the wait run out)
+    bar_settle(bars + K_FULL * 8, cnt, 2);
+    bar_settle(bars + V_FULL * 8, cnt, 2);
+    bar_settle(bars + Q_FULL * 8, q_boxes ? 1 : 0, 1);
     const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q);
     const __nv_bfloat16* k = static_cast<const __nv_bfloat16*>(a.keys) + w.sg.row_begin * a.krs + w.head * a.khs;
     const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(a.values) + w.sg.row_begin * a.vrs + w.head * a.vhs;
@@ -521,6 +525,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
             cnt += __popc(mask);
         }
     }
+    if (warp == FETCH_WARP && !cnt && maps.q_boxes) bar_wait(bar(Q_FULL), 0);  // (no product waits for the queries then, and rows of zeros leave through their place)
     tc_before();
     __syncthreads();
     tc_after();
@@ -876,7 +881,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
     if (*s_odd) {
         asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");  // (rows that left as boxes lie there before they are written again)
         __syncthreads();
-        by_rows(a, *reinterpret_cast<const Item*>(sm + S::ITEM_AT), s_qp, s_qd, s_slope, s_tok, s_depth, s_anc, s_list, cnt);
+        by_rows(bars, maps.q_boxes != 0, a, *reinterpret_cast<const Item*>(sm + S::ITEM_AT), s_qp, s_qd, s_slope, s_tok, s_depth, s_anc, s_list, cnt);
     }
 }
 

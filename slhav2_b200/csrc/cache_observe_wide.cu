@@ -41,6 +41,12 @@ struct Obs {
 };
 enum { K_FULL = 0, K_FREE = 5, S_FULL = 10, S_FREE = 14, Q_FULL = 18, TMEM_WORD = 19 };
 
+// At the end of a block: no copy is under way, whoever gave up before.
+__device__ __noinline__ void settle(uint32_t keys, uint32_t fills, uint32_t stages, uint32_t queries, uint32_t boxes) {
+    bar_settle(keys, fills, stages);
+    bar_settle(queries, boxes, 1);
+}
+
 struct ObsMaps {
     CUtensorMap k, q;
     uint32_t k_head_first, q_boxes;
@@ -326,6 +332,8 @@ __global__ void __launch_bounds__(Obs<D, MODE>::THREADS, Obs<D, MODE>::CTAS)
             }
             ++step;
         }
+        settle(bar(K_FULL), step, S::STAGES, bar(Q_FULL), maps.q_boxes && q_rows ? 1 : 0);
+        __syncwarp();
     }
     tc_before();
     __syncthreads();

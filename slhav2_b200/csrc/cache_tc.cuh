@@ -23,6 +23,10 @@ __device__ __forceinline__ bool bar_wait(uint32_t addr, uint32_t parity) {
     }
     return false;
 }
+// Waits for the last fills of a ring of `stages` barriers of which `fills` were begun, so that no copy is under way when a block ends, whoever gave up before.
+__device__ __forceinline__ void bar_settle(uint32_t bars, uint32_t fills, uint32_t stages) {
+    for (uint32_t i = fills > stages ? fills - stages : 0; i < fills; ++i) bar_wait(bars + i % stages * 8, i / stages & 1);
+}
 __device__ __forceinline__ void bar_expect(uint32_t addr, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(addr), "r"(bytes) : "memory");
 }

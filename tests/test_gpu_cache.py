@@ -882,3 +882,19 @@ def test_wide_blocks_whose_bias_grows_by_the_row(more, size):
         kind["q_pos"] = np.concatenate([np.arange(tokens), 5000000 + np.arange(tokens), 300 + 3 * np.arange(tokens)]).astype(np.uint32)
         kind["causal"] = False
     check(*make(rng, lens, tokens, kv, group, d, True, **kind), True)
+
+
+@pytest.mark.parametrize("d,group,tokens", [(128, 4, 40), (64, 1, 300), (128, 8, 33)])
+def test_wide_blocks_without_a_row_among_others(d, group, tokens):
+    # sequences whose rows are gone, and tokens of a document that no row has: zeros, while blocks beside them work
+    rng = np.random.default_rng(d + tokens)
+    lens, kv = (600, 400, 700, 333, 512, 64) * 4, 3
+    call, raw = make(rng, lens, tokens, kv, group, d, True)
+    call.rows = np.array([600, 0, 350, 0, 512, 0] * 4, np.uint32)
+    out, lse = check(call, raw, True)
+    for i in range(1, len(lens), 2):
+        assert np.all(out[i * tokens:(i + 1) * tokens] == 0) and np.all(lse[i * tokens:(i + 1) * tokens] == -np.inf)
+    total = sum(lens)
+    call, raw = make(rng, lens, tokens, kv, group, d, True, row_doc=np.ones((kv, total), np.uint32), q_doc=np.repeat(np.arange(len(lens)) % 2, tokens).astype(np.uint32))
+    out, lse = check(call, raw, True)
+    assert np.all(out.reshape(len(lens), tokens, -1)[::2] == 0) and np.all(lse.reshape(len(lens), tokens, -1)[::2] == -np.inf)
