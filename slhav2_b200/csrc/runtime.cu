@@ -4,6 +4,7 @@
 
 #include <sys/stat.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cmath>
 #include <cstdio>
@@ -46,6 +47,7 @@ namespace {
 struct Block {
     char* p = nullptr;
     size_t cap = 0, off = 0;
+    bool named = false;  // by a graph, which a captured call took memory for: never given back before the thread ends
 };
 // The small tables that calls upload (ctx_upload): a copy may read its slot until the slot's event, so a slot is written again
 // only after that.  One wait per stream, for its newest event in half the ring, covers the half; a wait for an event that is long
@@ -156,13 +158,25 @@ Status get_ctx(Ctx** out) {
 }
 bool sync_by_default(const Ctx* c) { return c->own_stream; }
 
+namespace {
+// (an error means that another stream's capture forbids to ask)
+bool capturing(cudaStream_t s) {
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(s, &cap) == cudaSuccess) return cap != cudaStreamCaptureStatusNone;
+    cudaGetLastError();
+    return true;
+}
+}  // namespace
+
 Status ctx_device_scratch(Ctx* c, size_t bytes, void** out) {
     bytes = pad256(std::max<size_t>(bytes, 256));
     auto& blocks = tls.blocks[c->device];
+    const bool named = capturing(c->stream);
     for (Block& b : blocks) {
         if (b.cap - b.off >= bytes) {
             *out = b.p + b.off;
             b.off += bytes;
+            b.named |= named;
             return Status();
         }
     }
@@ -170,6 +184,7 @@ Status ctx_device_scratch(Ctx* c, size_t bytes, void** out) {
     nb.cap = std::max<size_t>(bytes, blocks.empty() ? (size_t)8 << 20 : blocks.back().cap * 2);
     SLHA_CUDA(cudaMalloc((void**)&nb.p, nb.cap));
     nb.off = bytes;
+    nb.named = named;
     *out = nb.p;
     blocks.push_back(nb);
     return Status();
@@ -183,13 +198,6 @@ Status ctx_host_scratch(Ctx* c, size_t bytes, void** out) {
 }
 
 namespace {
-// (an error means that another stream's capture forbids to ask)
-bool capturing(cudaStream_t s) {
-    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-    if (cudaStreamIsCapturing(s, &cap) == cudaSuccess) return cap != cudaStreamCaptureStatusNone;
-    cudaGetLastError();
-    return true;
-}
 unsigned long long stream_id(cudaStream_t s) {
     unsigned long long id = 0;
     if (cudaStreamGetId(s, &id) != cudaSuccess) cudaGetLastError();
@@ -286,16 +294,18 @@ CallScope::CallScope() {
     tls.plans_used[c->device] = false;
     wait_for(tls.arena[c->device], c->stream);
     // the previous call has returned, so its staging memory may be reused; when
-    // the arena had to chain blocks, replace them by one block of the total size
-    if (blocks.size() > 1) {
-        size_t total = 0;
-        cudaStreamSynchronize(c->stream);
-        for (Block& b : blocks) { total += b.cap; cudaFree(b.p); }
-        blocks.clear();
-        Block nb;
-        nb.cap = total;
-        if (cudaMalloc((void**)&nb.p, nb.cap) == cudaSuccess) blocks.push_back(nb);
-        else cudaGetLastError();
+    // the arena had to chain blocks, replace those that no graph names by one of their total size
+    // (not under capture, which neither waits nor frees: the chain lasts until a call that is not captured)
+    const auto loose = [](const Block& b) { return !b.named; };
+    if (std::count_if(blocks.begin(), blocks.end(), loose) > 1 && !capturing(c->stream)) {
+        if (cudaStreamSynchronize(c->stream) == cudaSuccess) {
+            Block nb;
+            for (Block& b : blocks)
+                if (loose(b)) nb.cap += b.cap, cudaFree(b.p);
+            blocks.erase(std::remove_if(blocks.begin(), blocks.end(), loose), blocks.end());
+            if (cudaMalloc((void**)&nb.p, nb.cap) == cudaSuccess) blocks.push_back(nb);
+        }
+        cudaGetLastError();
     }
     for (Block& b : blocks) b.off = 0;
     for (auto& hb : tls.hblocks[c->device]) cudaFreeHost(hb.first);

@@ -1,0 +1,109 @@
+"""The calls on a cache of rows where a caller goes to the edge of what they allow: captured behind calls of any size, arrays that are written again at once, positions
+far apart, memory beside a call's own, values that are not finite, long caches.  Plain forms and bounds as in tests/cache_cases.py."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from tests import cache_cases as K
+from tests import helpers as H
+from tests import test_gpu_cache as T
+from tests.test_gpu_streams import Streams
+
+pytestmark = pytest.mark.gpu
+S = pytest.importorskip("slhav2_b200")
+F = np.float32
+
+
+def in_a_thread(work):
+    """The library's working memory belongs to the thread: a new one begins without any."""
+    import threading
+
+    bad = []
+
+    def run():
+        try:
+            work()
+        except BaseException as e:  # noqa: BLE001
+            bad.append(e)
+
+    t = threading.Thread(target=run)
+    t.start()
+    t.join()
+    if bad:
+        raise bad[0]
+
+
+def chunk_with_large_parts(rng):
+    """64 tokens over 20000 rows in parts of more than the 8 MB that a thread's working memory begins with."""
+    call, raw = T.make(rng, (20000,), 64, 2, 4, 128, True, causal=True)
+    cache, segs, queries = T.on_device(call, raw, True)
+    out = S.DeviceBuffer(call.q.size * 2)
+    return lambda: S.attend_cache(cache, segs, queries, out)
+
+
+# ---- graphs
+def test_a_call_is_captured_behind_calls_that_chained_working_memory():
+    # a small call, one whose parts do not fit beside it, then a capture: nothing is waited for or given back under it
+    rng = np.random.default_rng(1)
+    call, raw = T.make(rng, (20000,), 1, 2, 4, 128, True)
+    handles = T.on_device(call, raw, True)
+    out, lse = S.DeviceBuffer(call.q.size * 2), S.DeviceBuffer(call.q.size * 4)
+    large = chunk_with_large_parts(rng)
+    want = call.attend(True)
+    S.synchronize()
+
+    def work():
+        with Streams(1) as st:
+            rt, graph, exe = st.rt, C.c_void_p(), C.c_void_p()
+            S.set_stream(st.all[0].value)
+            S.attend_cache(*handles, out, lse)
+            large()
+            out.upload(np.zeros(call.q.size, np.uint16))
+            assert rt.cudaStreamBeginCapture(st.all[0], 0) == 0
+            S.attend_cache(*handles, out, lse)
+            assert rt.cudaStreamEndCapture(st.all[0], C.byref(graph)) == 0
+            assert rt.cudaGraphInstantiate(C.byref(exe), graph, C.c_ulonglong(0)) == 0
+            for _ in range(2):
+                large()
+                assert rt.cudaGraphLaunch(exe, st.all[0]) == 0
+            S.synchronize()
+            T.held(K.from_bf16(out.download(np.uint16, call.q.size)).reshape(call.q.shape), want[0], want[2])
+            rt.cudaGraphExecDestroy(exe)
+            rt.cudaGraphDestroy(graph)
+
+    in_a_thread(work)
+
+
+def test_working_memory_that_a_graph_names_stays():
+    # the pool's question is captured with memory of the thread; calls that chain more of it, and put the chain together, come before the graph runs
+    rng = np.random.default_rng(2)
+    large = chunk_with_large_parts(rng)
+    gm = S.Model.from_projection(H.make_model_pair(128, seed=61)[1], 128, 61)
+    pools = [S.TilePool(3000, 2**40) for _ in range(2)]
+    for p in pools:
+        p.append_keys(gm, H.gaussian_keys(65, 3000, 128), S.CODEC_MIXED)
+    qc, qs = H.random_queries(1, 12)
+    dq, ds = S.to_device(qc), S.to_device(qs)
+    S.synchronize()
+
+    def work():
+        with Streams(1) as st:
+            rt, graph, exe = st.rt, C.c_void_p(), C.c_void_p()
+            S.set_stream(st.all[0].value)
+            pools[1].observe_query(dq, ds, 3.0)
+            assert rt.cudaStreamBeginCapture(st.all[0], 2) == 0
+            pools[0].observe_query(dq, ds, 3.0)
+            assert rt.cudaStreamEndCapture(st.all[0], C.byref(graph)) == 0
+            assert rt.cudaGraphInstantiate(C.byref(exe), graph, C.c_ulonglong(0)) == 0
+            for _ in range(2):
+                large()
+                assert rt.cudaGraphLaunch(exe, st.all[0]) == 0
+                pools[1].observe_query(dq, ds, 3.0)
+            assert rt.cudaGraphLaunch(exe, st.all[0]) == 0
+            S.synchronize()
+            rt.cudaGraphExecDestroy(exe)
+            rt.cudaGraphDestroy(graph)
+
+    in_a_thread(work)
+    assert pools[0].read()[2].tobytes() == pools[1].read()[2].tobytes()
