@@ -410,7 +410,8 @@ int32_t slha_b200_attend_topk(const uint32_t* top_index, const float* top_score,
  * queries and outputs is a multiple of 16 bytes, head_dim of 16 bytes too
  * (SLHA_ERR_DIMENSION otherwise).  Rows, positions, documents, queries, outputs,
  * lse and weights are device memory of the calling thread's device; the other
- * arrays, and the segments, host or device.
+ * arrays, and the segments, host or device.  Host ones are copied before a call
+ * returns, and may then be written again.
  * A call can be captured into a CUDA graph where its segments (at most 64) are host
  * memory and its other arrays device memory; working memory then belongs to the
  * graph.

@@ -15,14 +15,16 @@ Status cache_device_memory(Ctx* c, const void* p, const char* fn, const char* wh
         return Status(SLHA_ERR_DEVICE, std::string(fn) + ": " + what + " lies on another device than the calling thread's");
     return Status();
 }
-// Short arrays, host or device; host ones cannot be captured.
+// Short arrays, host or device; host ones cannot be captured.  They are copied before the call returns, from page-locked memory too, which a copy on the stream would read later.
 template <typename T>
 Status cache_stage(Ctx* c, const T* p, size_t n, const T** dev, const char* fn, const char* what) {
-    if (p && n) {
-        if (is_device_ptr(p)) SLHA_TRY(cache_device_memory(c, p, fn, what));
-        else SLHA_TRY(ctx_no_capture(c));
-    }
-    return stage_in_t(c, p, n, dev);
+    *dev = p;
+    if (!p || !n) return Status();
+    if (is_device_ptr(p)) return cache_device_memory(c, p, fn, what);
+    void* d;
+    SLHA_TRY(ctx_upload(c, p, n * sizeof(T), &d));
+    *dev = static_cast<const T*>(d);
+    return Status();
 }
 // A table in device memory is read behind the caller's work on this stream; one in host memory is there before the device is asked for anything.
 void cache_host_segments(const SlhaB200Segment* segments, size_t n, std::vector<SlhaB200Segment>* out, bool* on_device) {

@@ -107,3 +107,40 @@ def test_working_memory_that_a_graph_names_stays():
 
     in_a_thread(work)
     assert pools[0].read()[2].tobytes() == pools[1].read()[2].tobytes()
+
+
+
+# ---- arrays in host memory
+def test_short_arrays_may_be_written_again_once_a_call_has_returned():
+    # page-locked ones too, while the call's stream is still busy with what came before
+    torch = pytest.importorskip("torch")
+    rng = np.random.default_rng(3)
+    t, lens = 40, (300, 200)
+    parents = np.concatenate([T.tree(rng, "random", t) for _ in lens])
+    call, raw = T.make(rng, lens, t, 2, 2, 64, True, parents=parents)
+    call.rows = np.array([250, 200], np.uint32)
+    call.slopes, call.prefix = np.array([0.5, 0.25, 0.125, 0.0], F), np.array([10, 0], np.uint32)
+    call.q_pos = rng.integers(150, 260, 2 * t).astype(np.uint32)
+    want = call.attend(True)
+    pin = lambda x: torch.from_numpy(x.view(np.int32) if x.dtype == np.uint32 else x).pin_memory()  # noqa: E731
+    p, rows, slopes, prefix, q_pos = (pin(x) for x in (parents, call.rows, call.slopes, call.prefix, call.q_pos))
+    cache = S.KvCache(S.to_device(raw[0]), S.to_device(raw[1]), 2, 64, rows=rows)
+    queries = S.CacheQueries(S.to_device(raw[2]), 2 * t, 4, 64, scale=call.scale, slopes=slopes, prefix=prefix, positions=q_pos)
+    out, lse = S.DeviceBuffer(call.q.size * 2), S.DeviceBuffer(2 * t * 4 * 4)
+    st = torch.cuda.Stream()
+    busy = torch.zeros(8192, 8192, device="cuda")
+    torch.cuda.synchronize()
+    try:
+        S.set_stream(st.cuda_stream)
+        S.attend_tree(cache, S.make_segments(call.segs), queries, p, out, lse)  # (what a first call does only once)
+        with torch.cuda.stream(st):
+            for _ in range(20):
+                busy @ busy
+        S.attend_tree(cache, S.make_segments(call.segs), queries, p, out, lse)
+        for x in (p, rows, slopes, prefix, q_pos):
+            x.zero_()
+        torch.cuda.synchronize()
+    finally:
+        S.set_stream(None)
+    T.held(K.from_bf16(out.download(np.uint16, call.q.size)).reshape(call.q.shape), want[0], want[2])
+    T.held(lse.download(F, 2 * t * 4).reshape(2 * t, 4), want[1], want[3])
