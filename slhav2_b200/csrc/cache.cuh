@@ -105,6 +105,10 @@ struct CacheSight {
         return ((past || !causal) && away <= window_last) || kp < prefix;
     }
 };
+// The distance of two positions.  Where many are taken from one token, as the difference of two float32, either position counted from one nearby: that costs no conversion. With the
+// token within 2^23 of where it is counted from, its own is exact, and the row's rounding is at most twice that of the distance; tokens further away take their distances in integers.
+constexpr uint32_t DISTANCE_NEAR = 1u << 23;
+__device__ __forceinline__ float cache_distance(uint32_t a, uint32_t b) { return (float)(a <= b ? b - a : a - b); }
 // Positions and documents of a tile's rows, or of a block's query rows.
 struct CacheRanges {
     uint32_t pmin, pmax, dmin, dmax;

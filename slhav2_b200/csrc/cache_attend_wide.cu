@@ -64,7 +64,7 @@ struct Item {
     uint32_t head, item, row0, q_rows, n, ctx;
     CacheSight sight;
     uint64_t entry;
-    uint32_t near_pos;                // where distances are taken from, so that those of rows nearby are exact in float32
+    uint32_t near_pos;                // where distances are taken from (see cache_distance)
     bool arrays, drafts_listed;  // positions or documents of the rows' own; drafted rows whose positions count
 };
 
@@ -123,8 +123,7 @@ __device__ __noinline__ void by_rows(uint32_t bars, bool q_boxes, const CacheArg
                 for (int e = 0; e < 4; ++e) s = fmaf(x[e], __bfloat162float(k[(uint64_t)i * a.krs + c + e]), s);
             for (int b = 16; b; b >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, b);
             s = a.cap > 0.0f ? a.cap * LOG2E * cache_tanh(s * a.scale / a.cap) : s * a.scale * LOG2E;
-            const uint32_t away = kp <= s_qp[r] ? s_qp[r] - kp : kp - s_qp[r];
-            s = fmaf(-s_slope[r], (float)away, s);
+            s = fmaf(-s_slope[r], cache_distance(s_qp[r], kp), s);
             const float top = fmaxf(m, s), use = top == -INFINITY ? 0.0f : top, f = exp2_fast(m - use), p = exp2_fast(s - use);
             m = top;
             l = fmaf(l, f, p);
@@ -162,6 +161,7 @@ __device__ __noinline__ bool bend_tile(const CacheArgs& a, unsigned char* sm, ui
     const uint32_t qp = s_qp[r], qd = s_qp[MB + r];
     const float slope = __uint_as_float(s_qp[2 * MB + r]), q_at = (float)((long long)qp - (long long)w.near_pos);
     const uint32_t* anc = reinterpret_cast<const uint32_t*>(sm + S::TREE_AT) + 2 * TREE_MOST + (a.tree ? s_qp[3 * MB + r] * (TREE_MOST / 32) : 0u);
+    const bool apart = has_slope && __any_sync(0xFFFFFFFFu, cache_distance(qp, w.near_pos) > (float)DISTANCE_NEAR);
     const CacheSight sight = w.sight;
     const bool has_cap = a.cap > 0.0f, bends = has_cap || has_slope;
     const float to_log2 = has_cap ? a.scale / a.cap : a.scale * LOG2E, cap2 = a.cap * LOG2E;
@@ -236,7 +236,16 @@ __device__ __noinline__ bool bend_tile(const CacheArgs& a, unsigned char* sm, ui
 #pragma unroll
             for (int c = 0; c < 32; ++c) s[c] *= to_log2;
         }
-        if (has_slope) {
+        if (apart) {
+#pragma unroll
+            for (int c = 0; c < 32; c += 4) {
+                const uint4 k = kp4[j * 8 + c / 4];
+                s[c] = fmaf(-slope, cache_distance(qp, k.x), s[c]);
+                s[c + 1] = fmaf(-slope, cache_distance(qp, k.y), s[c + 1]);
+                s[c + 2] = fmaf(-slope, cache_distance(qp, k.z), s[c + 2]);
+                s[c + 3] = fmaf(-slope, cache_distance(qp, k.w), s[c + 3]);
+            }
+        } else if (has_slope) {
 #pragma unroll
             for (int c = 0; c < 32; c += 4) {
                 const float4 k = *reinterpret_cast<const float4*>(kp4 + KT / 2 + j * 8 + c / 4);

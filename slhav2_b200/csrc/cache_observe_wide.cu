@@ -147,6 +147,7 @@ __global__ void __launch_bounds__(Obs<D, MODE>::THREADS, Obs<D, MODE>::CTAS)
     qr.pmax = __reduce_max_sync(0xFFFFFFFFu, qr.pmax);
     qr.dmin = __reduce_min_sync(0xFFFFFFFFu, qr.dmin);
     qr.dmax = __reduce_max_sync(0xFFFFFFFFu, qr.dmax);
+    const bool apart = has_slope && qr.pmax - qr.pmin > DISTANCE_NEAR;  // (see cache_distance)
     // Tiles of which, by their place alone, no token sees a row are not read.
     const auto visited = [&](uint32_t j) {
         if (q_rows == 0) return false;
@@ -229,7 +230,7 @@ __global__ void __launch_bounds__(Obs<D, MODE>::THREADS, Obs<D, MODE>::CTAS)
 #pragma unroll
                                 for (int e = 0; e < 4; ++e) {
                                     float x = (has_cap ? fmaf(cap2, cache_tanh(s[c + e] * to_log2), -h4[e]) : fmaf(s[c + e], to_log2, -h4[e])) - l4[e];
-                                    x = exp2_fast(fmaf(-slope[e], fabsf(q_at[e] - k_at), x));
+                                    x = exp2_fast(fmaf(-slope[e], apart ? cache_distance(qp[e], kp) : fabsf(q_at[e] - k_at), x));
                                     part[e & 1] += r0 + c + e < q_rows && (all || (sight.sees(qp[e], kp) && kd == qd[e])) ? x : 0.0f;
                                 }
                             }

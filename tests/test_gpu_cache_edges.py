@@ -144,3 +144,29 @@ def test_short_arrays_may_be_written_again_once_a_call_has_returned():
         S.set_stream(None)
     T.held(K.from_bf16(out.download(np.uint16, call.q.size)).reshape(call.q.shape), want[0], want[2])
     T.held(lse.download(F, 2 * t * 4).reshape(2 * t, 4), want[1], want[3])
+
+
+
+# ---- positions far apart
+@pytest.mark.parametrize("tokens,group,d", [(1, 4, 64), (40, 4, 64), (40, 4, 128), (70, 1, 64), (3, 4, 64)])
+@pytest.mark.parametrize("moved", [True, False])
+@pytest.mark.parametrize("softcap", [0.0, 8.0])
+def test_distances_between_positions_that_are_far_from_the_first_token_s(tokens, group, d, moved, softcap):
+    # tokens near 1000 and near 2^31 in one block: a distance is the difference of two positions, however far both are from the block's first token
+    rng = np.random.default_rng(tokens + d)
+    n, kv, far = 500, 2, 2 ** 31
+    if moved:
+        row_pos = np.stack([rng.permutation(np.concatenate([np.arange(800, 1050), far - 100 + np.arange(250)])) for _ in range(kv)]).astype(np.uint32)
+        base = 0
+    else:
+        row_pos, base = None, far - 100
+    near = 1000 + np.arange((tokens + 1) // 2)
+    q_pos = np.concatenate([near, far + 60 + 2 * np.arange(tokens - len(near))]).astype(np.uint32)
+    slopes = (0.6 * 2.0 ** -np.arange(kv * group)).astype(F)
+    call, raw = T.make(rng, (n,), tokens, kv, group, d, True, bases=[base], row_pos=row_pos, q_pos=q_pos, slopes=slopes, window=300, causal=False, softcap=softcap)
+    _, lse = T.check(call, raw, True)
+    cache, segs, queries = T.on_device(call, raw, True)
+    w = S.to_device(np.zeros((kv, n), F))
+    S.observe_cache(cache, segs, queries, S.to_device(lse), w, n)
+    want, tol = call.received(lse, np.zeros((kv, n), F), 1.0)
+    T.held(w.download(F, kv * n).reshape(kv, n), want, tol)
