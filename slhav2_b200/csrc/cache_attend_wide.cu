@@ -218,7 +218,7 @@ __device__ __noinline__ bool bend_tile(const CacheArgs& a, unsigned char* sm, ui
             float big = 0.0f;
 #pragma unroll
             for (int c = 0; c < 32; ++c) big = fmaxf(big, fabsf(s[c]));
-            if (__all_sync(0xFFFFFFFFu, big * to_log2 <= 1.0f)) {
+            if (__all_sync(0xFFFFFFFFu, big * to_log2 <= 1.0f || w.row0 + r >= w.q_rows)) {
                 const uint64_t in = pair(to_log2, to_log2), out = pair(cap2, cap2);
 #pragma unroll
                 for (int c = 0; c < 32; c += 2) {
@@ -441,7 +441,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
         }
         __syncthreads();
     }
-    for (uint32_t r = tid; r < MB; r += THREADS) {  // (rows behind the last repeat it, and are zeros among the queries)
+    for (uint32_t r = tid; r < MB; r += THREADS) {  // (rows behind the last repeat it; their queries are zeros or, where boxes bring them, those of other tokens)
         const uint32_t row = min(w.row0 + r, w.q_rows - 1), tok = row / a.group, h = w.head * a.group + row - tok * a.group;
         s_q[r] = ((uint64_t)(w.sg.query_begin + tok) * a.qts + (uint64_t)h * a.qhs) * 2;
         s_qp[r] = a.q_pos ? a.q_pos[w.sg.query_begin + tok] : w.sg.base + w.ctx + (is_tree ? s_depth[tok] : tok);
@@ -549,6 +549,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
             const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21), ts = lanes + t * 128, to = lanes + 256 + t * 128;
             const float to_log2 = has_cap ? a.scale / a.cap : a.scale * LOG2E, cap2 = a.cap * LOG2E;
             float m = -INFINITY, l = 0.0f;
+            const bool there = r < used;  // (rows behind the last have no part in what a warp decides for all its rows: equal inputs give equal bits)
             for (uint32_t li = 0; li < cnt; ++li) {
                 if (!__all_sync(0xFFFFFFFFu, bar_wait(bar(S_FULL + t), li & 1))) {
                     fail = true;
@@ -598,8 +599,8 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
                     const float x = fmaxf(high[0], high[1]) * to_log2;
                     mul = 1.0f;
                     const float furthest = fmaxf(x, -fminf(low[0], low[1]) * to_log2);
-                    fused = __all_sync(0xFFFFFFFFu, furthest <= 1.0f);
-                    brief = __all_sync(0xFFFFFFFFu, furthest <= TANH_BRIEF);
+                    fused = __all_sync(0xFFFFFFFFu, furthest <= 1.0f || !there);
+                    brief = __all_sync(0xFFFFFFFFu, furthest <= TANH_BRIEF || !there);
                     if (fused) {  // (tanh grows: the largest score is that of the largest product)
                         top = cap2 * tanh_small(x);
                     } else {
@@ -619,7 +620,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
                     top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * mul;
                     if (straight) top += fmaxf(near, fmaf(step, KT - 1, near));
                 }
-                if (__any_sync(0xFFFFFFFFu, top > m + LAZY)) {
+                if (__any_sync(0xFFFFFFFFu, top > m + LAZY && there)) {
                     const float now = fmaxf(m, top), f = m == -INFINITY ? 0.0f : exp2_fast(m - now);
                     m = now;
                     l *= f;
@@ -693,7 +694,6 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
                 tc_after();
             }
             // Rows leave through shared memory, where the queries were: a warp writes whole rows.
-            const bool there = r < used;
             const uint32_t tok = tok0 + s_tok[r], q_head = w.head * a.group + (there ? w.row0 + r - tok * a.group : 0u);
             const bool whole = w.sg.n_chunks == 1;
             const uint64_t part = ((uint64_t)w.item * a.n_kv + w.head) * MB + r;

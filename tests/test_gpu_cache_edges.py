@@ -170,3 +170,28 @@ def test_distances_between_positions_that_are_far_from_the_first_token_s(tokens,
     S.observe_cache(cache, segs, queries, S.to_device(lse), w, n)
     want, tol = call.received(lse, np.zeros((kv, n), F), 1.0)
     T.held(w.download(F, kv * n).reshape(kv, n), want, tol)
+
+
+
+# ---- memory beside a call's own
+@pytest.mark.parametrize("tokens,group,d", [(33, 1, 64), (100, 1, 128), (37, 8, 128), (9, 4, 64), (131, 4, 64)])
+@pytest.mark.parametrize("more", [dict(), dict(softcap=6.0), dict(alibi=True), dict(softcap=6.0, alibi=True, window=90)])
+def test_equal_inputs_give_equal_bits_whatever_lies_behind_the_queries(tokens, group, d, more):
+    rng = np.random.default_rng(tokens)
+    kind = {k: v for k, v in more.items() if k != "alibi"}
+    if more.get("alibi"):
+        kind["slopes"] = (2.0 ** -np.arange(1, 2 * group + 1)).astype(F)
+    call, raw = T.make(rng, (700, 10), (tokens, 40), 2, group, d, True, **kind)
+    call.segs = call.segs[:1]
+    grow = np.linspace(0.1, 2.0, 710)[:, None, None]
+    call.keys, raw = K.as_type(call.keys * grow, True)[0], (K.as_type(call.keys * grow, True)[1], raw[1], raw[2].copy())
+    before = None
+    for other in (0.0, 1.0, 300.0, -3e4, np.nan, np.inf):
+        raw[2][tokens:] = K.as_type(np.full(raw[2][tokens:].shape, other), True)[1]
+        handles = T.on_device(call, raw, True)
+        o, z = T.results(call, True, *handles)
+        w = S.to_device(np.zeros((2, 710), F))
+        S.observe_cache(handles[0], handles[1], handles[2], S.to_device(z), w, 710)
+        now = o[:tokens].tobytes(), z[:tokens].tobytes(), w.download(F, 1420).tobytes()
+        assert before in (None, now), other
+        before = now
