@@ -38,12 +38,12 @@ struct Wide {
     static constexpr uint32_t TILE = HALVES * HALF;
     static constexpr uint32_t K_AT = 2 * TILE, V_AT = 4 * TILE, META_AT = 6 * TILE;   // META: 4 x (positions, documents, distances) of a key tile
     static constexpr uint32_t LIST_AT = META_AT + 4 * 3 * KT * 4, CLS_AT = LIST_AT + RUN_MOST * 4, ROWS_AT = CLS_AT + RUN_MOST;  // ROWS: offset in q (64 bits), position, document, slope, token
-    static constexpr uint32_t RANGE_AT = ROWS_AT + 6 * MB * 4, ITEM_AT = RANGE_AT + 64, BAR_AT = ITEM_AT + 256, TREE_AT = BAR_AT + 256;
+    static constexpr uint32_t RANGE_AT = ROWS_AT + 6 * MB * 4, ODD_AT = RANGE_AT + 64, ITEM_AT = ODD_AT + RUN_MOST * 2, BAR_AT = ITEM_AT + 256, TREE_AT = BAR_AT + 256;
     static constexpr uint32_t SMEM = TREE_AT + 1024, SMEM_TREE = SMEM + TREE_MOST * 8 + MB * (TREE_MOST / 8);
     static_assert(SMEM_TREE <= 227 * 1024, "shared memory of an SM");
 };
 // barriers, 8 bytes each
-enum { K_FULL = 0, V_FULL = 2, K_FREE = 4, V_FREE = 6, S_FULL = 8, P_FULL = 10, O_FULL = 12, TMEM_WORD = 13, ODD_WORD = 14, META_FULL = 16, P_HALF = 20, Q_FULL = 22 };
+enum { K_FULL = 0, V_FULL = 2, K_FREE = 4, V_FREE = 6, S_FULL = 8, P_FULL = 10, O_FULL = 12, TMEM_WORD = 13, FAIL_WORD = 14, META_FULL = 16, P_HALF = 20, Q_FULL = 22, V_CLEAN = 23 };
 
 template <int N>
 __device__ __forceinline__ void regs_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(N)); }
@@ -91,8 +91,90 @@ __device__ __forceinline__ RowOut row_out(const CacheArgs& a, const Item& w, uin
     return o;
 }
 
-// The item again on the CUDA cores, a warp a query row and a row of the cache at a time, where only what is seen is read: for values that are not finite in a tile that not all see
-// (a weight of zero would not keep them out of the sums), and where a wait ran out.
+// Whether query row r sees row i of the segment, whose position is kp and whose document is kd.
+__device__ __forceinline__ bool row_sees(const CacheArgs& a, const Item& w, const uint32_t* s_qp, const uint32_t* s_qd, const uint32_t* s_tok, const uint32_t* s_anc, uint32_t r, uint32_t i,
+                                         uint32_t kp, uint32_t kd) {
+    if (!w.sight.sees(s_qp[r], kp) || kd != s_qd[r]) return false;
+    return !a.tree || i < w.ctx || (s_anc[s_tok[r] * (TREE_MOST / 32) + ((i - w.ctx) >> 5)] >> ((i - w.ctx) & 31) & 1u);
+}
+__device__ __forceinline__ uint32_t row_position(const CacheArgs& a, const Item& w, const uint32_t* s_depth, uint32_t i) {
+    return a.row_pos ? a.row_pos[w.entry + i] : a.tree && i >= w.ctx ? w.sg.base + w.ctx + s_depth[i - w.ctx] : w.sg.base + i;
+}
+
+// Values that are not finite in tiles that not all see: the products took zeros in their place (a weight of zero would not keep them out of the sums).  Here they reach the sums of the
+// query rows that see them: a bit for each query row, element and sign, then the results.  Only the rows that hold such values, and the seven beside each, are read again (256 query rows of 2 KV heads on
+// 32768 rows with a row that nobody sees every 64: 44 us, 50 where those rows are NaN; 131072 rows 102 and 128, every other row 102 and 361).
+template <int D>
+__device__ __noinline__ void odd_values(const CacheArgs& a, unsigned char* sm, uint32_t cnt) {
+    using S = Wide<D>;
+    const Item& w = *reinterpret_cast<const Item*>(sm + S::ITEM_AT);
+    const uint32_t* const s_qp = reinterpret_cast<const uint32_t*>(sm + S::ROWS_AT) + 2 * MB;
+    const uint32_t *const s_qd = s_qp + MB, *const s_tok = s_qp + 3 * MB, *const s_depth = reinterpret_cast<const uint32_t*>(sm + S::TREE_AT) + TREE_MOST, *const s_anc = s_depth + TREE_MOST;
+    const uint32_t *const s_list = reinterpret_cast<const uint32_t*>(sm + S::LIST_AT), *const s_odd = reinterpret_cast<const uint32_t*>(sm + S::ODD_AT);
+    uint32_t* const s_sign = reinterpret_cast<uint32_t*>(sm + S::K_AT);  // [query row][+, -][128 elements]; the tiles are no longer needed
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, used = min((uint32_t)MB, w.q_rows - w.row0), c = lane * 4;
+    for (uint32_t i = threadIdx.x; i < MB * 8; i += THREADS) s_sign[i] = 0;
+    __syncthreads();
+    const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(a.values) + w.sg.row_begin * a.vrs + w.head * a.vhs;
+    uint32_t turn = 0;
+    for (uint32_t l0 = 0; l0 < cnt; l0 += 32) {
+        const uint32_t mine = l0 + lane < cnt ? s_odd[(l0 + lane) >> 1] >> (lane & 1) * 16 & 0xFFFFu : 0u;
+        for (uint32_t tiles = __ballot_sync(0xFFFFFFFFu, mine != 0); tiles; tiles &= tiles - 1) {
+            const uint32_t at = __ffs(tiles) - 1, first = (s_list[l0 + at] >> 2) * KT, rows = min((uint32_t)KT, w.n - first);
+            for (uint32_t parts = __shfl_sync(0xFFFFFFFFu, mine, at); parts; parts &= parts - 1) {
+                if (turn++ % WARPS != warp) continue;
+                const uint32_t j0 = (__ffs(parts) - 1) * 8;
+                uint2 x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = j0 + e < rows && c < a.d ? *reinterpret_cast<const uint2*>(v + (uint64_t)(first + j0 + e) * a.vrs + c) : make_uint2(0u, 0u);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const uint32_t odd = odd_pair(x[e].x) | odd_pair(x[e].y);
+                    if (!__any_sync(0xFFFFFFFFu, odd & 0x80008000u)) continue;
+                    uint32_t plus = 0, minus = 0;  // of the lane's four elements; NaN: both
+                    const uint32_t bits[4] = {x[e].x & 0xFFFFu, x[e].x >> 16, x[e].y & 0xFFFFu, x[e].y >> 16};
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) {
+                        const uint32_t size = bits[y] & 0x7FFFu;
+                        if (size < 0x7F80u) continue;
+                        if (size > 0x7F80u || !(bits[y] & 0x8000u)) plus |= 1u << y;
+                        if (size > 0x7F80u || (bits[y] & 0x8000u)) minus |= 1u << y;
+                    }
+                    const uint32_t eight = 0xFFu << (lane & 24);
+                    plus = __reduce_or_sync(eight, plus << (lane & 7) * 4);
+                    minus = __reduce_or_sync(eight, minus << (lane & 7) * 4);
+                    uint32_t word[8];
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) word[y] = __shfl_sync(0xFFFFFFFFu, plus, y * 8), word[4 + y] = __shfl_sync(0xFFFFFFFFu, minus, y * 8);
+                    const uint32_t i = first + j0 + e, kp = row_position(a, w, s_depth, i), kd = a.row_doc ? a.row_doc[w.entry + i] : 0u;
+                    for (uint32_t r = lane; r < used; r += 32)
+                        if (row_sees(a, w, s_qp, s_qd, s_tok, s_anc, r, i, kp, kd))
+#pragma unroll
+                            for (int y = 0; y < 8; ++y)
+                                if (word[y] & ~s_sign[r * 8 + y]) atomicOr(s_sign + r * 8 + y, word[y]);
+                }
+            }
+        }
+    }
+    __syncthreads();
+    for (uint32_t r = warp; r < used; r += WARPS) {
+        const uint32_t plus = s_sign[r * 8 + lane / 8] >> (lane & 7) * 4 & 15u, minus = s_sign[r * 8 + 4 + lane / 8] >> (lane & 7) * 4 & 15u;
+        if (!(plus | minus) || c >= a.d) continue;
+        const RowOut to = row_out(a, w, r);
+        for (uint32_t y = 0; y < 4; ++y) {
+            const float add = (plus >> y & 1u ? INFINITY : 0.0f) + (minus >> y & 1u ? -INFINITY : 0.0f);  // (both: NaN)
+            if (add == 0.0f) continue;
+            if (to.out) {
+                __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(to.out) + c + y;
+                *o = __float2bfloat16(__bfloat162float(*o) + add);
+            } else {
+                to.part[c + y] += add;
+            }
+        }
+    }
+}
+
+// The item again on the CUDA cores, a warp a query row and a row of the cache at a time, where a wait ran out.
 __device__ __noinline__ void by_rows(uint32_t bars, bool q_boxes, const CacheArgs& a, const Item& w, const uint32_t* s_qp, const uint32_t* s_qd, const float* s_slope, const uint32_t* s_tok,
                                      const uint32_t* s_depth, const uint32_t* s_anc, const uint32_t* s_list, uint32_t cnt) {
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -114,10 +196,8 @@ __device__ __noinline__ void by_rows(uint32_t bars, bool q_boxes, const CacheArg
         for (uint32_t j = 0; j < cnt * KT; ++j) {
             const uint32_t i = (s_list[j / KT] >> 2) * KT + j % KT;
             if (i >= w.n) continue;
-            const bool drafted = a.tree && i >= w.ctx;
-            const uint32_t kp = a.row_pos ? a.row_pos[w.entry + i] : drafted ? w.sg.base + w.ctx + s_depth[i - w.ctx] : w.sg.base + i;
-            if (!w.sight.sees(s_qp[r], kp) || (a.row_doc && a.row_doc[w.entry + i] != s_qd[r])) continue;
-            if (drafted && !(s_anc[s_tok[r] * (TREE_MOST / 32) + ((i - w.ctx) >> 5)] >> ((i - w.ctx) & 31) & 1u)) continue;
+            const uint32_t kp = row_position(a, w, s_depth, i);
+            if (!row_sees(a, w, s_qp, s_qd, s_tok, s_anc, r, i, kp, a.row_doc ? a.row_doc[w.entry + i] : 0u)) continue;
             float s = 0.0f;
             if (mine)
                 for (int e = 0; e < 4; ++e) s = fmaf(x[e], __bfloat162float(k[(uint64_t)i * a.krs + c + e]), s);
@@ -318,7 +398,8 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
     uint32_t* s_anc = s_depth + TREE_MOST;
     const uint32_t bars = sb + S::BAR_AT;
     volatile uint32_t* s_tmem = reinterpret_cast<volatile uint32_t*>(sm + S::BAR_AT + TMEM_WORD * 8);
-    volatile uint32_t* s_odd = reinterpret_cast<volatile uint32_t*>(sm + S::BAR_AT + ODD_WORD * 8);
+    volatile uint32_t* s_fail = reinterpret_cast<volatile uint32_t*>(sm + S::BAR_AT + FAIL_WORD * 8);  // a wait ran out; a tile holds values that are not finite
+    uint32_t* s_odd = reinterpret_cast<uint32_t*>(sm + S::ODD_AT);                                      // of each tile 16 bits, one for each eight rows in which there are such
     const auto bar = [&](int which) { return bars + which * 8; };
     const uint32_t tok0 = w.row0 / a.group;
 
@@ -331,12 +412,14 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
     if (tid == 0) *reinterpret_cast<Item*>(sm + S::ITEM_AT) = w;
     uint32_t cnt = 0;
     if (warp == FETCH_WARP) {
+        for (uint32_t i = lane; i < RUN_MOST / 2; i += 32) s_odd[i] = 0;
         if (lane == 0) {
             for (int i = 0; i < 2; ++i) {
                 bar_init(bar(K_FULL + i), 1);
                 bar_init(bar(V_FULL + i), 1);
                 bar_init(bar(K_FREE + i), 1);
                 bar_init(bar(V_FREE + i), 3);
+                bar_init(bar(V_CLEAN + i), 2);
                 bar_init(bar(S_FULL + i), 1);
                 bar_init(bar(P_HALF + i), 128);
                 bar_init(bar(P_FULL + i), 128);
@@ -344,7 +427,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
             bar_init(bar(O_FULL), 1);
             bar_init(bar(Q_FULL), 1);
             for (int i = 0; i < 4; ++i) bar_init(bar(META_FULL + i), 1);
-            *s_odd = 0;
+            s_fail[0] = s_fail[1] = 0;
             asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             if (maps.q_boxes) {  // 32 query rows a box
@@ -807,7 +890,8 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
             }
             for (uint32_t li = 0; li < cnt && !fail; ++li) {
                 const bool more = li + 1 < cnt;
-                if (!bar_wait(bar(V_FULL + (li & 1)), li >> 1 & 1) || !values(li, 0)) {
+                // (also for tiles that all see, which nobody looks over: to tell them apart here took longer, 228 us for 221 of a chunk under window and cap)
+                if (!bar_wait(bar(V_FULL + (li & 1)), li >> 1 & 1) || !bar_wait(bar(V_CLEAN + (li & 1)), li >> 1 & 1) || !values(li, 0)) {
                     fail = true;
                     break;
                 }
@@ -861,36 +945,57 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
             fetch(sb + S::V_AT + slot * S::TILE, &maps.v, maps.v_head_first, vb, a.vrs, first, bar(V_FULL + slot));
         }
         } else {
-        // ---- values of tiles that not all see: where one is not finite, a weight of zero does not keep it out of the sums, and the item is done again by rows
+        // ---- values of tiles that not all see: zeros take the place of those that are not finite, before the products (see odd_values)
         for (uint32_t li = 0; li < cnt; ++li) {
             if (!__all_sync(0xFFFFFFFFu, bar_wait(bar(V_FULL + (li & 1)), li >> 1 & 1))) {
                 fail = true;
                 break;
             }
             if ((s_list[li] & (two ? 3u : 1u)) != (two ? 3u : 1u)) {
-                uint32_t odd = 0;
+                uint4* const tile = reinterpret_cast<uint4*>(sm + S::V_AT + (li & 1) * S::TILE);
+                uint32_t odd = 0, parts = 0;
 #pragma unroll 8
                 for (uint32_t i = tid - 320; i < S::TILE / 16; i += 64) {
-                    const uint4 x = *reinterpret_cast<const uint4*>(sm + S::V_AT + (li & 1) * S::TILE + i * 16);
+                    const uint4 x = tile[i];
                     odd |= odd_pair(x.x) | odd_pair(x.y) | odd_pair(x.z) | odd_pair(x.w);
                 }
-                if (odd & 0x80008000u) *s_odd = 1u;
+                if (__any_sync(0xFFFFFFFFu, odd & 0x80008000u)) {
+                    const auto finite = [](uint32_t x) {
+                        const uint32_t bad = odd_pair(x);
+                        return x & ~((bad & 0x80000000u ? 0xFFFF0000u : 0u) | (bad & 0x00008000u ? 0xFFFFu : 0u));
+                    };
+                    for (uint32_t i = tid - 320; i < S::TILE / 16; i += 64) {  // (64 pieces are eight rows)
+                        const uint4 x = tile[i];
+                        if ((odd_pair(x.x) | odd_pair(x.y) | odd_pair(x.z) | odd_pair(x.w)) & 0x80008000u) parts |= 1u << (i / 64 & 15);
+                        tile[i] = make_uint4(finite(x.x), finite(x.y), finite(x.z), finite(x.w));
+                    }
+                    parts = __reduce_or_sync(0xFFFFFFFFu, parts);
+                    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                    if (lane == 0) {
+                        atomicOr(s_odd + (li >> 1), parts << (li & 1) * 16);
+                        s_fail[1] = 1u;
+                    }
+                }
             }
             __syncwarp();
-            if (lane == 0) bar_arrive(bar(V_FREE + (li & 1)));
+            if (lane == 0) {
+                bar_arrive(bar(V_CLEAN + (li & 1)));
+                bar_arrive(bar(V_FREE + (li & 1)));
+            }
         }
         }
     }
-    if (fail) *s_odd = 1u;
+    if (fail) s_fail[0] = 1u;
     tc_before();
     __syncthreads();  // (the rows' warps have given their registers back: none of the others takes them while one still has to get them)
     tc_after();
     if (warp >= 8) regs_more<REGS_ALL>();
     if (warp == MMA_WARP) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512u) : "memory");
-    if (*s_odd) {
+    if (s_fail[0] | s_fail[1]) {
         asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");  // (rows that left as boxes lie there before they are written again)
         __syncthreads();
-        by_rows(bars, maps.q_boxes != 0, a, *reinterpret_cast<const Item*>(sm + S::ITEM_AT), s_qp, s_qd, s_slope, s_tok, s_depth, s_anc, s_list, cnt);
+        if (!s_fail[0]) odd_values<D>(a, sm, cnt);
+        else by_rows(bars, maps.q_boxes != 0, a, *reinterpret_cast<const Item*>(sm + S::ITEM_AT), s_qp, s_qd, s_slope, s_tok, s_depth, s_anc, s_list, cnt);
     }
 }
 

@@ -195,3 +195,105 @@ def test_equal_inputs_give_equal_bits_whatever_lies_behind_the_queries(tokens, g
         now = o[:tokens].tobytes(), z[:tokens].tobytes(), w.download(F, 1420).tobytes()
         assert before in (None, now), other
         before = now
+
+
+
+# ---- values that are not finite
+def odd_call(rng, lens, tokens, kv, group, d, at, **kind):
+    """A call whose values hold infinities and NaN at (row, dimension, value), and its result by the definition: what a token sees counts, nothing else."""
+    call, raw = T.make(rng, lens, tokens, kv, group, d, True, **kind)
+    for row, dim, x in at:
+        raw[1][row, :, dim] = K.as_type(np.full(kv, x), True)[1]
+        call.values[row, :, dim] = x
+    return call, raw
+
+
+def held_odd(got, want, tol):
+    want = np.where(np.isnan(want), np.nan, want)
+    with np.errstate(invalid="ignore"):
+        same = (got == want) | (np.abs(got - want) <= tol) | (np.isnan(got) & np.isnan(want))
+    assert same.all(), (int((~same).sum()), np.argwhere(~same)[:4], got[~same][:4], want[~same][:4])
+
+
+@pytest.mark.parametrize("kind", ["causal", "window", "docs", "moved", "tree", "prefix", "split", "strided"])
+@pytest.mark.parametrize("tokens,group,d", [(300, 1, 128), (70, 4, 64), (40, 4, 80), (33, 8, 128), (256, 1, 128)])
+@pytest.mark.parametrize("softcap", [0.0, 9.0])
+def test_values_that_are_not_finite_reach_those_who_see_them_and_nobody_else(kind, tokens, group, d, softcap):
+    rng = np.random.default_rng(tokens + len(kind))
+    n, kv = 6000 if kind == "split" else 900, 2
+    more = dict(softcap=softcap)
+    first = n - tokens
+    # before all tokens, beside each other in one tile, among the tokens' own rows; one column with both infinities, one with NaN
+    at = [(5, 1, np.inf), (first - 3, 2, -np.inf), (first - 2, 2, np.inf), (first + 2, 3, np.inf), (first + tokens // 2, 3, -np.inf), (first + 9, d - 1, np.nan), (n - 1, 4, -np.inf),
+          (n - 2, 0, np.inf)]
+    if kind == "window":
+        more["window"] = 150
+    if kind == "prefix":
+        more["prefix"], more["window"] = np.array([40], np.uint32), 30
+    if kind == "docs":
+        doc = rng.integers(0, 3, n).astype(np.uint32)
+        doc[first:] = rng.integers(0, 2, tokens)
+        more["row_doc"], more["q_doc"] = np.stack([doc] * kv), doc[first:]
+        at += [(int(r), 6, np.inf) for r in np.flatnonzero(doc == 2)[::7]]
+    if kind == "moved":
+        pos = np.stack([rng.permutation(2 * n)[:n] for _ in range(kv)]).astype(np.uint32)
+        more["row_pos"], more["q_pos"] = pos, rng.integers(0, 2 * n, tokens).astype(np.uint32)
+    if kind == "tree":
+        if tokens > 256:
+            tokens, first = 256, n - 256
+        more["parents"] = T.tree(rng, "random", tokens)
+    call, raw = odd_call(rng, (n,), tokens, kv, group, d, at, **more)
+    if kind == "strided":  # queries and outputs [head][token]: not in boxes
+        heads = kv * group
+        q = np.ascontiguousarray(raw[2].transpose(1, 0, 2))
+        cache = S.KvCache(S.to_device(raw[0]), S.to_device(raw[1]), kv, d)
+        queries = S.CacheQueries(S.to_device(q), tokens, heads, d, softcap=softcap, token_stride=d, head_stride=tokens * d)
+        out, dl = S.DeviceBuffer(call.q.size * 2), S.DeviceBuffer(tokens * heads * 4)
+        S.attend_cache(cache, S.make_segments(call.segs), queries, out, dl, out_token_stride=d, out_head_stride=tokens * d)
+        o = K.from_bf16(out.download(np.uint16, call.q.size)).reshape(heads, tokens, d).transpose(1, 0, 2)
+        lse = dl.download(F, tokens * heads).reshape(tokens, heads)
+    else:
+        o, lse = T.results(call, True, *T.on_device(call, raw, True))
+    with np.errstate(invalid="ignore"):
+        want = call.attend(True)
+    T.held(lse, want[1], want[3])
+    held_odd(o, want[0], want[2])
+    assert not np.isfinite(want[0]).all() and np.isfinite(want[0]).any()
+
+
+def test_hidden_rows_of_any_content_cost_little():
+    # a hole in every tile of 32768 rows, whose keys and values are NaN: as quick as finite ones but for looking them over
+    torch = pytest.importorskip("torch")
+    n, kv, group, d, tokens = 32768, 2, 4, 128, 64
+    g = torch.Generator(device="cuda").manual_seed(5)
+    k, v = (torch.randn(n, kv, d, device="cuda", generator=g).bfloat16() for _ in range(2))
+    q = torch.randn(tokens, kv * group, d, device="cuda", generator=g).bfloat16()
+    doc = torch.ones(n, dtype=torch.int32, device="cuda")
+    doc[17:n - tokens:64] = 7
+    q_doc = torch.ones(tokens, dtype=torch.int32, device="cuda")
+    segs = S.make_segments([(0, n, 0, tokens, 0)])
+    took, outs = [], []
+    for fill in (0.0, float("nan")):
+        k[doc == 7] = fill
+        v[doc == 7] = fill
+        out = torch.empty_like(q)
+        cache = S.KvCache(k, v, kv, d, documents=doc)
+        queries = S.CacheQueries(q, tokens, kv * group, d, documents=q_doc)
+        torch.cuda.synchronize()
+        st = torch.cuda.Stream()
+        try:
+            S.set_stream(st.cuda_stream)
+            for _ in range(3):
+                S.attend_cache(cache, segs, queries, out)
+            begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            begin.record(st)
+            for _ in range(5):
+                S.attend_cache(cache, segs, queries, out)
+            end.record(st)
+            torch.cuda.synchronize()
+        finally:
+            S.set_stream(None)
+        took.append(begin.elapsed_time(end) / 5)
+        outs.append(out.float().cpu())
+    assert took[1] < 8 * took[0] + 0.1, took
+    assert torch.equal(outs[0], outs[1])
