@@ -12,6 +12,9 @@ namespace slha {
 constexpr uint32_t CACHE_TABLE = 64;         // segments whose table travels in a kernel's parameters
 constexpr uint32_t TREE_MOST = 256;          // drafted tokens of a segment
 constexpr uint32_t CACHE_DIM_MOST = 256;
+// Bytes of the parts of split segments that a launch may leave to be joined (the sums of a block of query rows of all KV heads may be more): a segment that can be left whole is, beyond
+// it, and one that cannot is worked off in several launches.
+constexpr uint64_t CACHE_PARTS_MOST = 512ull << 20;
 
 // A segment and its share of a launch's work.
 struct CacheSeg {
@@ -22,6 +25,7 @@ struct CacheSeg {
     uint32_t chunk_tiles;  // key tiles of an item
     uint32_t n_chunks;     // items of a block of query rows
     uint32_t seg;          // its number in the caller's table
+    uint32_t block_first, n_blocks;  // of a launch that takes some of the segment's blocks of query rows: the first, and how many
     uint32_t pad;
     uint64_t to_begin;     // its first row's place where rows go to
 };
@@ -176,7 +180,8 @@ Status cache_smem(Ctx* c, size_t bytes) {
     return Status();
 }
 
-Status cache_part_memory(CacheArgs* a, const CacheWork& w, uint32_t mb, CacheMemory* mem);  // where the parts of split segments go
+inline uint64_t cache_part_bytes(uint64_t items, uint32_t n_kv, uint32_t mb, uint32_t d) { return items * n_kv * mb * (d * 4ull + 8); }
+Status cache_part_memory(CacheArgs* a, uint64_t items, uint32_t mb, CacheMemory* mem);  // where the parts of split segments go
 Status launch_cache_join(Ctx* c, CacheArgs a, int dtype, const CacheWork& w, uint32_t mb);
 Status launch_attend_wide(Ctx* c, CacheArgs a, CacheWork w, bool* taken);
 Status launch_attend_cache(Ctx* c, CacheArgs a, int dtype, const std::vector<SlhaB200Segment>& segs);

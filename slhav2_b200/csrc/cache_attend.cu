@@ -443,7 +443,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) cache_join_kernel(const __grid_c
     const CacheSeg* table = a.table ? a.table : tab.s;
     const uint32_t seg = cache_find(a.n_segs, qb, [&](uint32_t i) { return table[i].block_begin; });
     const CacheSeg sg = table[seg];
-    const uint32_t block = qb - sg.block_begin, r = part * ROWS + warp / WARPS, row = block * mb + r;
+    const uint32_t block = qb - sg.block_begin, r = part * ROWS + warp / WARPS, row = (sg.block_first + block) * mb + r;
     if (r >= mb || row >= sg.n_queries * a.group) return;  // (with more than one warp a row: all of them)
     const uint64_t first = ((uint64_t)(sg.item_begin + block * sg.n_chunks) * a.n_kv + head) * mb + r, step = (uint64_t)a.n_kv * mb;
     float top = -INFINITY;
@@ -536,7 +536,7 @@ static void cut(CacheWork* w, uint32_t group, uint32_t mb, uint32_t kt, uint32_t
 // and half an item at the end; an item costs about four tiles to begin, joining about three and a little for every part.
 // *cluster: how many CTAs share a block of query rows and join their sums through each other's shared memory, where that takes less time than a second kernel (0: none do).
 // One token over 512 rows: 6.5 us by a cluster, 8.0 by a second kernel; 8 x 4096 rows 26.2 and 28.7; 1 x 2048, where more than eight parts are worth it, 9.1 and 8.5.
-static uint32_t longest_run(const CacheWork& w, uint32_t group, uint32_t mb, uint32_t kt, uint32_t n_kv, uint32_t slots, uint32_t* cluster) {
+static uint32_t longest_run(const CacheWork& w, uint32_t group, uint32_t mb, uint32_t kt, uint32_t n_kv, uint32_t d, uint32_t slots, uint32_t* cluster) {
     uint32_t most = 1;
     double total = 0.0;
     for (const CacheSeg& c : w.segs) {
@@ -552,6 +552,7 @@ static uint32_t longest_run(const CacheWork& w, uint32_t group, uint32_t mb, uin
             const uint32_t tiles = std::max(1u, (uint32_t)(((uint64_t)c.n_rows + kt - 1) / kt));
             items += (double)blocks_of(c, group, mb) * ((tiles + run - 1) / run) * n_kv;
         }
+        if (run < most && cache_part_bytes((uint64_t)items, 1, mb, d) > CACHE_PARTS_MOST) break;  // (items: of all KV heads)
         const double time = (items <= slots ? run : total / slots + 0.5 * run) + 4.0 * std::ceil(items / slots) +
                             (run < most ? 3.0 + 0.05 * ((most + run - 1) / run) : 0.0);
         if (time < best_time) best_time = time, best = run;
@@ -590,9 +591,9 @@ Status launch_cache_join(Ctx* c, CacheArgs a, int dtype, const CacheWork& w, uin
     count_launch();
     return Status();
 }
-Status cache_part_memory(CacheArgs* a, const CacheWork& w, uint32_t mb, CacheMemory* mem) {
-    if (!w.blocks) return Status();
-    const size_t rows = (size_t)w.items * a->n_kv * mb;
+Status cache_part_memory(CacheArgs* a, uint64_t items, uint32_t mb, CacheMemory* mem) {
+    if (!items) return Status();
+    const size_t rows = (size_t)items * a->n_kv * mb;
     void* p;
     SLHA_TRY(mem->get(pad256(rows * a->d * 4) + rows * 8, &p));
     a->part_o = (float*)p;
@@ -605,14 +606,14 @@ template <typename T, int D, int WM>
 Status launch_class(Ctx* c, CacheArgs a, CacheWork w) {
     using S = Shape<T, D, WM>;
     const uint32_t slots = (uint32_t)sm_count(c->device) * S::CTAS;
-    const uint32_t run = longest_run(w, a.group, S::MB, S::KT, a.n_kv, slots, &a.cluster);
+    const uint32_t run = longest_run(w, a.group, S::MB, S::KT, a.n_kv, a.d, slots, &a.cluster);
     cut(&w, a.group, S::MB, S::KT, run, a.cluster);
     if (w.items * a.n_kv > 0x7FFFFFFFull) return Status(SLHA_ERR_CAPACITY, "attention over a cache: too many blocks of query rows");
     CacheTable tab;
     SLHA_TRY(cache_table(c, w.segs, &tab, &a.table));
     a.n_segs = (uint32_t)w.segs.size();
     CacheMemory mem{c};
-    SLHA_TRY(cache_part_memory(&a, w, S::MB, &mem));
+    SLHA_TRY(cache_part_memory(&a, w.blocks ? w.items : 0, S::MB, &mem));
     const size_t smem = a.tree ? S::SMEM_TREE : S::SMEM;
     SLHA_TRY((cache_smem<cache_attend_kernel<T, D, WM>>(c, S::SMEM_TREE)));
     SLHA_CUDA(launch_cluster(cache_attend_kernel<T, D, WM>, dim3((uint32_t)(w.items * a.n_kv)), dim3(ATT_THREADS), smem, c->stream, std::max(a.cluster, 1u), a, tab));

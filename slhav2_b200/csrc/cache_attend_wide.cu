@@ -371,8 +371,8 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
     w.q_rows = w.sg.n_queries * a.group;
     const uint32_t block = (w.item - w.sg.item_begin) / w.sg.n_chunks, chunk = (w.item - w.sg.item_begin) - block * w.sg.n_chunks, tiles = (w.n + KT - 1) / KT;
     {   // (the last blocks first: under a causal mask they see most)
-        const uint32_t turned = (w.q_rows + MB - 1) / MB - 1 - block;
-        w.row0 = turned * MB;
+        const uint32_t turned = w.sg.n_blocks - 1 - block;
+        w.row0 = (w.sg.block_first + turned) * MB;
         w.item = w.sg.item_begin + turned * w.sg.n_chunks + chunk;  // (where the parts of its rows go)
     }
     w.sight = CacheSight{a.window_last, a.prefix ? a.prefix[w.sg.seg] : 0u, a.causal};
@@ -1034,32 +1034,50 @@ void wide_share(const CacheArgs& a, CacheWork* w, uint32_t slots) {
             if (run <= 2) break;
         }
     }
-    w->items = w->blocks = 0;
-    w->chunks = 1;
     for (size_t i = 0; i < w->segs.size(); ++i) {
         CacheSeg& s = w->segs[i];
         const uint32_t tiles = std::max(1u, (uint32_t)(((uint64_t)s.n_rows + KT - 1) / KT));
-        const uint64_t count = ((uint64_t)s.n_queries * a.group + MB - 1) / MB;
         s.n_chunks = (most[i] + best - 1) / best;
         s.chunk_tiles = (tiles + s.n_chunks - 1) / s.n_chunks;
-        s.item_begin = (uint32_t)w->items;
-        s.block_begin = (uint32_t)w->blocks;
-        w->items += count * s.n_chunks;
-        if (s.n_chunks > 1) w->blocks += count;
-        w->chunks = std::max(w->chunks, s.n_chunks);
     }
+}
+// The launches of a call: one, or where its parts would take more than CACHE_PARTS_MOST several, each of some blocks of query rows (262144 causal tokens of 32 heads on as many rows,
+// 8.6 GB at once: TIME).
+std::vector<CacheWork> wide_launches(const CacheArgs& a, const std::vector<CacheSeg>& segs) {
+    bool split = false;
+    for (const CacheSeg& s : segs) split |= s.n_chunks > 1;
+    const uint64_t most = split ? std::max<uint64_t>(1, CACHE_PARTS_MOST / cache_part_bytes(1, a.n_kv, MB, a.d)) : ~0ull;
+    std::vector<CacheWork> works(1);
+    for (CacheSeg s : segs) {
+        const uint64_t count = ((uint64_t)s.n_queries * a.group + MB - 1) / MB;
+        for (uint64_t first = 0; first < count; first += s.n_blocks) {
+            if (works.back().items && works.back().items + s.n_chunks > most) works.emplace_back();
+            CacheWork& w = works.back();
+            s.block_first = (uint32_t)first;
+            s.n_blocks = (uint32_t)std::min(count - first, std::max<uint64_t>(1, (most - std::min(most, w.items)) / s.n_chunks));
+            s.item_begin = (uint32_t)w.items;
+            s.block_begin = (uint32_t)w.blocks;
+            w.items += (uint64_t)s.n_blocks * s.n_chunks;
+            if (s.n_chunks > 1) w.blocks += s.n_blocks;
+            w.chunks = std::max(w.chunks, s.n_chunks);
+            w.segs.push_back(s);
+        }
+    }
+    return works;
 }
 
 template <int D, bool CAP, int KIND>
 Status launch_wide(Ctx* c, CacheArgs a, CacheWork w, const WideMaps& maps) {
     using S = Wide<D>;
     wide_share(a, &w, (uint32_t)sm_count(c->device));
-    if (w.items * a.n_kv > 0x7FFFFFFFull) return Status(SLHA_ERR_CAPACITY, "attention over a cache: too many blocks of query rows");
-    CacheTable tab;
-    SLHA_TRY(cache_table(c, w.segs, &tab, &a.table));
-    a.n_segs = (uint32_t)w.segs.size();
+    const std::vector<CacheWork> works = wide_launches(a, w.segs);
+    uint64_t parts = 0;
+    for (const CacheWork& x : works) {
+        if (x.items * a.n_kv > 0x7FFFFFFFull) return Status(SLHA_ERR_CAPACITY, "attention over a cache: too many blocks of query rows");
+        if (x.blocks) parts = std::max(parts, x.items);
+    }
     CacheMemory mem{c};
-    SLHA_TRY(cache_part_memory(&a, w, MB, &mem));
+    SLHA_TRY(cache_part_memory(&a, parts, MB, &mem));
     constexpr auto kernel = cache_attend_wide_kernel<D, CAP, KIND>;
     SLHA_TRY((cache_smem<kernel>(c, S::SMEM_TREE)));
     static const int regs = []() {
@@ -1067,9 +1085,14 @@ Status launch_wide(Ctx* c, CacheArgs a, CacheWork w, const WideMaps& maps) {
         return cudaFuncGetAttributes(&at, cache_attend_wide_kernel<D, CAP, KIND>) == cudaSuccess ? at.numRegs : 0;
     }();
     if (regs != REGS_ALL) return Status(SLHA_ERR_DEVICE, "attention over a cache: the kernel was built with other registers than its warps share out");
-    SLHA_CUDA(launch_behind(kernel, dim3((uint32_t)(w.items * a.n_kv)), dim3(THREADS), a.tree ? S::SMEM_TREE : S::SMEM, c->stream, a, maps, tab));
-    count_launch();
-    if (w.blocks) SLHA_TRY(launch_cache_join(c, a, SLHA_B200_BF16, w, MB));
+    for (const CacheWork& x : works) {
+        CacheTable tab;
+        SLHA_TRY(cache_table(c, x.segs, &tab, &a.table));
+        a.n_segs = (uint32_t)x.segs.size();
+        SLHA_CUDA(launch_behind(kernel, dim3((uint32_t)(x.items * a.n_kv)), dim3(THREADS), a.tree ? S::SMEM_TREE : S::SMEM, c->stream, a, maps, tab));
+        count_launch();
+        if (x.blocks) SLHA_TRY(launch_cache_join(c, a, SLHA_B200_BF16, x, MB));
+    }
     return mem.done();
 }
 

@@ -297,3 +297,34 @@ def test_hidden_rows_of_any_content_cost_little():
         outs.append(out.float().cpu())
     assert took[1] < 8 * took[0] + 0.1, took
     assert torch.equal(outs[0], outs[1])
+
+
+
+# ---- long caches
+def test_rows_of_more_than_one_run_keep_to_their_working_memory():
+    # 140000 rows take two runs a block; 32768 tokens' parts at once would be 1.1 GB
+    torch = pytest.importorskip("torch")
+    n, kv, group, d, tokens = 140000, 8, 4, 128, 32768
+    g = torch.Generator(device="cuda").manual_seed(6)
+    k, v = (torch.randn(n, kv, d, device="cuda", generator=g).bfloat16() for _ in range(2))
+    q = torch.randn(tokens, kv * group, d, device="cuda", generator=g).bfloat16()
+    segs = S.make_segments([(0, n, 0, tokens, 0)])
+    cache = S.KvCache(k, v, kv, d)
+    outs, lses = [], []
+    grown = []
+
+    def work():
+        for prefix in (None, torch.zeros(1, dtype=torch.int32, device="cuda")):  # (a prefix of nothing: the same rows are seen, but the runs are made for all)
+            out, lse = torch.full_like(q, 7.0), torch.zeros(tokens, kv * group, device="cuda")
+            queries = S.CacheQueries(q, tokens, kv * group, d, window=200, prefix=prefix)
+            torch.cuda.synchronize()
+            before = torch.cuda.mem_get_info()[0]
+            S.attend_cache(cache, segs, queries, out, lse)
+            grown.append(before - torch.cuda.mem_get_info()[0])
+            outs.append(out)
+            lses.append(lse)
+
+    in_a_thread(work)
+    assert grown[0] <= 16 << 20 and grown[1] <= 600 << 20, grown
+    assert float((lses[0] - lses[1]).abs().max()) <= 2e-5
+    assert float((outs[0].float() - outs[1].float()).abs().max()) <= 2.0 ** -6 * float(v.float().abs().max())
