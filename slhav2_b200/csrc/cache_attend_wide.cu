@@ -225,7 +225,7 @@ __device__ __noinline__ void by_rows(uint32_t bars, bool q_boxes, const CacheArg
 // A tile's scores that are more than products: capped, biased, masked.  Read from TMEM and written back, 32 columns at a time, in units of log 2 where a cap or a distance bends them; where
 // all that a warp's rows see of 32 columns is all, they stay as they are.  (A function, in loops that are hardly
 // unrolled, so that the loop over the tiles stays short: where the same stood in it, every tile's weights took 15 % longer.)  False where a wait ran out.
-template <int D, bool SLOPED>
+template <int D, bool CAP, bool SLOPED, bool APART = false>
 __device__ __noinline__ bool bend_tile(const CacheArgs& a, unsigned char* sm, uint32_t ts, uint32_t r, uint32_t t, uint32_t li) {
     using S = Wide<D>;
     const Item& w = *reinterpret_cast<const Item*>(sm + S::ITEM_AT);
@@ -239,11 +239,12 @@ __device__ __noinline__ bool bend_tile(const CacheArgs& a, unsigned char* sm, ui
     if ((has_slope || listed) && !__all_sync(0xFFFFFFFFu, bar_wait(bar(META_FULL + (li & 3)), li >> 2 & 1))) return false;
     const uint4* kp4 = reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(sm + S::META_AT) + (li & 3) * 3 * KT);
     const uint32_t qp = s_qp[r], qd = s_qp[MB + r];
+    if constexpr (SLOPED && !APART)  // (in the same function: 250 us for 231 of 4096 tokens whose tiles are all bent)
+        if (__any_sync(0xFFFFFFFFu, cache_distance(qp, w.near_pos) > (float)DISTANCE_NEAR)) return bend_tile<D, CAP, true, true>(a, sm, ts, r, t, li);
     const float slope = __uint_as_float(s_qp[2 * MB + r]), q_at = (float)((long long)qp - (long long)w.near_pos);
     const uint32_t* anc = reinterpret_cast<const uint32_t*>(sm + S::TREE_AT) + 2 * TREE_MOST + (a.tree ? s_qp[3 * MB + r] * (TREE_MOST / 32) : 0u);
-    const bool apart = has_slope && __any_sync(0xFFFFFFFFu, cache_distance(qp, w.near_pos) > (float)DISTANCE_NEAR);
     const CacheSight sight = w.sight;
-    const bool has_cap = a.cap > 0.0f, bends = has_cap || has_slope;
+    constexpr bool has_cap = CAP, bends = has_cap || has_slope;
     const float to_log2 = has_cap ? a.scale / a.cap : a.scale * LOG2E, cap2 = a.cap * LOG2E;
     // positions one after another: what is seen are one or two runs
     const long long at = (long long)w.sg.base + first;
@@ -316,15 +317,9 @@ __device__ __noinline__ bool bend_tile(const CacheArgs& a, unsigned char* sm, ui
 #pragma unroll
             for (int c = 0; c < 32; ++c) s[c] *= to_log2;
         }
-        if (apart) {
+        if constexpr (APART) {
 #pragma unroll
-            for (int c = 0; c < 32; c += 4) {
-                const uint4 k = kp4[j * 8 + c / 4];
-                s[c] = fmaf(-slope, cache_distance(qp, k.x), s[c]);
-                s[c + 1] = fmaf(-slope, cache_distance(qp, k.y), s[c + 1]);
-                s[c + 2] = fmaf(-slope, cache_distance(qp, k.z), s[c + 2]);
-                s[c + 3] = fmaf(-slope, cache_distance(qp, k.w), s[c + 3]);
-            }
+            for (int c = 0; c < 32; ++c) s[c] = fmaf(-slope, cache_distance(qp, lds(smem_addr(kp4) + (j * 32 + c) * 4)), s[c]);
         } else if (has_slope) {
 #pragma unroll
             for (int c = 0; c < 32; c += 4) {
@@ -654,7 +649,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
                     straight = __all_sync(0xFFFFFFFFu, all && !has_pos && !is_tree && (after || (long long)s_qp[r] <= at) && fabsf(slope) * (KT - 1) <= 64.0f);
                 }
                 const bool bent = !straight && (!all || has_slope);
-                if (bent && !bend_tile<D, has_slope>(a, sm, ts, r, t, li)) {
+                if (bent && !bend_tile<D, CAP, has_slope>(a, sm, ts, r, t, li)) {
                     fail = true;
                     break;
                 }
@@ -687,7 +682,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
                     if (fused) {  // (tanh grows: the largest score is that of the largest product)
                         top = cap2 * tanh_small(x);
                     } else {
-                        if (!bend_tile<D, has_slope>(a, sm, ts, r, t, li)) {
+                        if (!bend_tile<D, CAP, has_slope>(a, sm, ts, r, t, li)) {
                             fail = true;
                             break;
                         }
@@ -890,8 +885,9 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
             }
             for (uint32_t li = 0; li < cnt && !fail; ++li) {
                 const bool more = li + 1 < cnt;
-                // (also for tiles that all see, which nobody looks over: to tell them apart here took longer, 228 us for 221 of a chunk under window and cap)
-                if (!bar_wait(bar(V_FULL + (li & 1)), li >> 1 & 1) || !bar_wait(bar(V_CLEAN + (li & 1)), li >> 1 & 1) || !values(li, 0)) {
+                // (the two warps have waited for the values; so for tiles that all see, too, which nobody looks over.  With a bias the loops come out quicker where the values are waited for
+                // here too: 8192 causal tokens 609 us for 644, but a chunk under window and cap 225 for 217)
+                if ((has_slope && !bar_wait(bar(V_FULL + (li & 1)), li >> 1 & 1)) || !bar_wait(bar(V_CLEAN + (li & 1)), li >> 1 & 1) || !values(li, 0)) {
                     fail = true;
                     break;
                 }
@@ -1042,7 +1038,7 @@ void wide_share(const CacheArgs& a, CacheWork* w, uint32_t slots) {
     }
 }
 // The launches of a call: one, or where its parts would take more than CACHE_PARTS_MOST several, each of some blocks of query rows (262144 causal tokens of 32 heads on as many rows,
-// 8.6 GB at once: TIME).
+// 8.3 GB at once: 512 MB, and 596 ms for 630).
 std::vector<CacheWork> wide_launches(const CacheArgs& a, const std::vector<CacheSeg>& segs) {
     bool split = false;
     for (const CacheSeg& s : segs) split |= s.n_chunks > 1;
