@@ -461,8 +461,9 @@ typedef struct {
 
 /* Attention: out (element (token, head, i) at token * out_token_stride + head *
  * out_head_stride + i) and, where lse_out is not NULL, the logarithm of the summed
- * exponentials [n_tokens][n_heads].  Tokens of no segment are left as they are.  One
- * token a segment is a decode step, many are a prompt or a chunk of one; work is split
+ * exponentials [n_tokens][n_heads].  Tokens of no segment are left as they are, tokens
+ * of two are refused; out and lse_out overlap no input.  Rows may belong to several
+ * segments.  One token a segment is a decode step, many are a prompt or a chunk of one; work is split
  * over the rows where there are few tokens, and joined in a fixed order. */
 int32_t slha_b200_attend_cache(const SlhaB200KvCache* cache, const SlhaB200Segment* segments, size_t n_segments,
                                const SlhaB200CacheQueries* queries, void* out, uint64_t out_token_stride,
@@ -482,7 +483,9 @@ int32_t slha_b200_attend_tree(const SlhaB200KvCache* cache, const SlhaB200Segmen
  * weights_in[the same] + the sum of exp(s - lse) over the segment's tokens and the query
  * heads of KV head h that see row r; lse as slha_b200_attend_cache wrote it for the same
  * queries.  weights_in may be weights_out, or NULL (nothing received so far); entries of
- * rows of no segment are left as they are.  The cache's values are not read (may be NULL). */
+ * rows of no segment are left as they are, rows of two segments are refused (with row
+ * counts in device memory they are the caller's to avoid).  The cache's values are not
+ * read (may be NULL). */
 int32_t slha_b200_observe_cache(const SlhaB200KvCache* cache, const SlhaB200Segment* segments, size_t n_segments,
                                 const SlhaB200CacheQueries* queries, const float* lse, const float* weights_in,
                                 float decay, float* weights_out, uint64_t weight_head_stride);
@@ -494,7 +497,9 @@ int32_t slha_b200_observe_cache(const SlhaB200KvCache* cache, const SlhaB200Segm
  * below all, go by the lower row.  A row that stays and lies below the budget keeps its
  * place; the places of the others there are taken, in order, by the rows that stay from
  * beyond it, so that in place only those move.  (Attention does not depend on the order
- * of rows that carry their positions.) */
+ * of rows that carry their positions.)  Rows of two segments are refused where they are
+ * removed in place, and so are two segments' places in another cache (with row counts in
+ * device memory they are the caller's to avoid). */
 typedef struct {
     const float* weights;                /* [h * weight_head_stride + r] */
     uint64_t weight_head_stride;

@@ -73,6 +73,23 @@ Status cache_positions_fit(const std::vector<SlhaB200Segment>& segs, const char*
     return Status();
 }
 
+// Whether two of the ranges (first, behind the last) share something.
+bool cache_overlap(std::vector<std::pair<uint64_t, uint64_t>> r) {
+    r.erase(std::remove_if(r.begin(), r.end(), [](const auto& x) { return x.first >= x.second; }), r.end());
+    if (!std::is_sorted(r.begin(), r.end())) std::sort(r.begin(), r.end());
+    for (size_t i = 1; i < r.size(); ++i)
+        if (r[i].first < r[i - 1].second) return true;
+    return false;
+}
+// Rows that a call writes, or whose weights it does, belong to one segment each.  (Row counts in device memory are not known here: the caller's to see to.)
+Status cache_own_rows(const std::vector<SlhaB200Segment>& segs, const std::vector<SlhaB200Segment>& at, const uint32_t* rows, uint32_t most, const char* fn) {
+    if (rows && is_device_ptr(rows)) return Status();
+    std::vector<std::pair<uint64_t, uint64_t>> r;
+    for (size_t i = 0; i < segs.size(); ++i)
+        r.emplace_back(at[i].tile_begin, at[i].tile_begin + std::min({segs[i].n_tiles, rows ? rows[i] : segs[i].n_tiles, most}));
+    return cache_overlap(std::move(r)) ? Status(SLHA_ERR_DIMENSION, std::string(fn) + ": two segments have the same rows") : Status();
+}
+
 Status cache_check_queries(const SlhaB200KvCache* k, const SlhaB200CacheQueries* q, const char* fn) {
     const auto name = [&](const char* what) { return std::string(fn) + ": " + what; };
     const size_t each = 16 / key_elem_bytes(k->dtype);
@@ -146,12 +163,18 @@ int32_t attend_cache_any(const char* fn, const SlhaB200KvCache* cache, const Slh
         std::vector<SlhaB200Segment> segs;
         bool device_segs;
         cache_host_segments(segments, n_segments, &segs, &device_segs);
-        if (!device_segs) SLHA_TRY(cache_check_segments(cache, segs, queries, tree, fn));
+        const auto check_segments = [&]() -> Status {
+            SLHA_TRY(cache_check_segments(cache, segs, queries, tree, fn));
+            std::vector<std::pair<uint64_t, uint64_t>> tokens;
+            for (const SlhaB200Segment& s : segs) tokens.emplace_back(s.query_begin, (uint64_t)s.query_begin + s.n_queries);
+            return cache_overlap(std::move(tokens)) ? Status(SLHA_ERR_DIMENSION, name("two segments have the same query tokens")) : Status();
+        };
+        if (!device_segs) SLHA_TRY(check_segments());
         CallScope cs;
         if (!cs.ok()) return cs.st;
         Ctx* c = cs.c;
         SLHA_TRY(cache_device_segments(c, segments, &segs, device_segs, fn));
-        if (device_segs) SLHA_TRY(cache_check_segments(cache, segs, queries, tree, fn));
+        if (device_segs) SLHA_TRY(check_segments());
         SLHA_TRY(cache_memory(c, cache, fn, true));
         SLHA_TRY(cache_device_memory(c, out, fn, "out"));
         if (lse_out) SLHA_TRY(cache_device_memory(c, lse_out, fn, "lse_out"));
@@ -197,12 +220,16 @@ int32_t slha_b200_observe_cache(const SlhaB200KvCache* cache, const SlhaB200Segm
         std::vector<SlhaB200Segment> segs;
         bool device_segs;
         cache_host_segments(segments, n_segments, &segs, &device_segs);
-        if (!device_segs) SLHA_TRY(cache_check_segments(cache, segs, queries, false, fn));
+        const auto check_segments = [&]() -> Status {
+            SLHA_TRY(cache_check_segments(cache, segs, queries, false, fn));
+            return cache_own_rows(segs, segs, cache->rows, 0xFFFFFFFFu, fn);
+        };
+        if (!device_segs) SLHA_TRY(check_segments());
         CallScope cs;
         if (!cs.ok()) return cs.st;
         Ctx* c = cs.c;
         SLHA_TRY(cache_device_segments(c, segments, &segs, device_segs, fn));
-        if (device_segs) SLHA_TRY(cache_check_segments(cache, segs, queries, false, fn));
+        if (device_segs) SLHA_TRY(check_segments());
         SLHA_TRY(cache_memory(c, cache, fn, false));
         SLHA_TRY(cache_device_memory(c, lse, fn, "lse"));
         SLHA_TRY(cache_device_memory(c, weights_out, fn, "weights_out"));
@@ -254,7 +281,7 @@ int32_t slha_b200_evict_cache(const SlhaB200KvCache* cache, const SlhaB200Segmen
             for (size_t i = 0; i < to_segs.size(); ++i)
                 if (to_segs[i].n_tiles < std::min(segs[i].n_tiles, ev->budget))
                     return Status(SLHA_ERR_CAPACITY, name("segment ") + std::to_string(i) + " of the other cache has no room for the rows that stay");
-            return Status();
+            return cache_own_rows(segs, in_place ? segs : to_segs, cache->rows, in_place ? 0xFFFFFFFFu : ev->budget, fn);
         };
         if (!device_segs && !device_to) SLHA_TRY(check_segments());
         CallScope cs;

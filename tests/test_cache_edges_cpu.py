@@ -1,0 +1,42 @@
+"""What the calls on a cache of rows refuse because there is no right answer: the same tokens or rows in two segments, scales that float32 cannot hold in units of log 2,
+positions that wrap, rows that go to one place from several KV heads.  Addresses here are never read."""
+import numpy as np
+import pytest
+
+import slhav2_b200 as S
+from tests.test_cache_refusals_cpu import A, SEG, cache, queries, refused
+
+
+def passes(call, *args, **more):
+    """Past its checks of arguments: without a GPU the device is what is missing (with one the addresses would be)."""
+    with pytest.raises(S.SlhaError) as e:
+        call(*args, **more)
+    assert e.value.code == S.ERR_DEVICE, e.value.message
+
+
+# ---- the same tokens or rows twice
+TWICE = [(0, 100, 0, 2, 0), (100, 100, 2, 2, 0), (300, 100, 1, 1, 0)]
+
+
+def test_query_tokens_of_two_segments():
+    segs = S.make_segments(TWICE)
+    refused(S.ERR_DIMENSION, "tokens", S.attend_cache, cache(), segs, queries(), A)
+    refused(S.ERR_DIMENSION, "tokens", S.attend_cache, cache(), segs[::-1], queries(), A)
+    refused(S.ERR_DIMENSION, "tokens", S.attend_tree, cache(), segs, queries(), np.zeros(4, np.uint32), A)
+    passes(S.observe_cache, cache(), segs, queries(), A, A, 400)  # (which only reads them)
+    passes(S.attend_cache, cache(), S.make_segments([(0, 100, 2, 2, 0), (0, 100, 0, 2, 0), (0, 100, 1, 0, 0)]), queries(), A)  # any order, one prompt's rows for several, no tokens
+
+
+def test_rows_of_two_segments():
+    over, beside = S.make_segments([(50, 51, 0, 2, 0), (0, 50, 2, 1, 0), (100, 50, 3, 1, 0)]), S.make_segments([(50, 50, 0, 2, 0), (0, 50, 2, 1, 0), (100, 50, 3, 1, 0), (60, 0, 0, 0, 0)])
+    refused(S.ERR_DIMENSION, "rows", S.observe_cache, cache(), over, queries(), A, A, 400)
+    refused(S.ERR_DIMENSION, "rows", S.evict_cache, cache(), over, A, 400, 10)
+    passes(S.attend_cache, cache(), over, queries(), A)
+    for call, more in ((lambda k, s: S.observe_cache(k, s, queries(), A, A, 400), {}), (lambda k, s: S.evict_cache(k, s, A, 400, 10), {})):
+        passes(call, cache(), beside)
+        passes(call, cache(rows=np.array([50, 50, 50], np.uint32)), over)  # the table's room overlaps, the rows do not
+        refused(S.ERR_DIMENSION, "rows", call, cache(rows=np.array([51, 50, 50], np.uint32)), over)
+    # to another cache: where the rows go
+    to = dict(to=cache(), to_segments=S.make_segments([(0, 10, 0, 0, 0), (9, 10, 0, 0, 0), (30, 10, 0, 0, 0)]))
+    refused(S.ERR_DIMENSION, "rows", S.evict_cache, cache(), over, A, 400, 10, **to)
+    passes(S.evict_cache, cache(), over, A, 400, 9, **to)
