@@ -449,7 +449,7 @@ typedef struct {
     uint64_t token_stride;
     uint64_t head_stride;
     float scale;
-    float softcap;               /* 0: none */
+    float softcap;               /* 0: none; at most 2^100, scale / softcap a normal number */
     uint32_t window;             /* 0: none */
     int32_t causal;
     const float* slopes;         /* n_heads; NULL: none */

@@ -100,6 +100,10 @@ Status cache_check_queries(const SlhaB200KvCache* k, const SlhaB200CacheQueries*
     if (!std::isfinite(q->scale) || !std::isfinite(q->softcap) || q->softcap < 0.0f)
         return Status(SLHA_ERR_NONFINITE, name("scale must be finite, softcap finite and not negative"));
     if (q->softcap > 0.0f && !std::isfinite(q->scale / q->softcap)) return Status(SLHA_ERR_NONFINITE, name("scale / softcap must be finite"));
+    // (in units of log 2; tanh(scale / softcap * product) of a larger cap would lose the small scores, and a factor below the smallest normal number its bits)
+    if (!std::isfinite(q->scale * 1.4426950408889634f)) return Status(SLHA_ERR_NONFINITE, name("scale / log 2 must be finite"));
+    if (q->softcap > 0x1p100f || (q->softcap > 0.0f && q->scale != 0.0f && !std::isnormal(q->scale / q->softcap)))
+        return Status(SLHA_ERR_NONFINITE, name("softcap must be at most 2^100, and scale / softcap a normal float32"));
     if (k->positions && !q->positions) return Status(SLHA_ERR_NULL, name("the cache's rows have positions, the queries have none"));
     if ((k->documents != nullptr) != (q->documents != nullptr)) return Status(SLHA_ERR_NULL, name("documents must be given for rows and queries, or for neither"));
     return Status();
@@ -109,6 +113,7 @@ Status cache_check_segments(const SlhaB200KvCache* k, const std::vector<SlhaB200
     for (const SlhaB200Segment& s : segs) {
         if ((uint64_t)s.query_begin + s.n_queries > q->n_tokens) return Status(SLHA_ERR_DIMENSION, name("a segment's query tokens reach beyond n_tokens"));
         if ((uint64_t)s.n_queries * (q->n_heads / k->n_kv_heads) > 0x7FFFFFFFull) return Status(SLHA_ERR_CAPACITY, name("too many query rows in a segment"));
+        if (!q->positions && (uint64_t)s.index_base + s.n_queries > 0x100000000ull) return Status(SLHA_ERR_DIMENSION, name("index_base + n_queries exceeds 2^32"));
         if (tree && (s.n_queries > TREE_MOST || s.n_queries > s.n_tiles))
             return Status(SLHA_ERR_DIMENSION, name("a segment's drafted tokens are at most 256, and its last rows are theirs"));
     }

@@ -40,3 +40,24 @@ def test_rows_of_two_segments():
     to = dict(to=cache(), to_segments=S.make_segments([(0, 10, 0, 0, 0), (9, 10, 0, 0, 0), (30, 10, 0, 0, 0)]))
     refused(S.ERR_DIMENSION, "rows", S.evict_cache, cache(), over, A, 400, 10, **to)
     passes(S.evict_cache, cache(), over, A, 400, 9, **to)
+
+
+# ---- numbers that float32 does not hold
+@pytest.mark.parametrize("call", [lambda k, s, q: S.attend_cache(k, s, q, A), lambda k, s, q: S.attend_tree(k, s, q, np.zeros(4, np.uint32), A),
+                                  lambda k, s, q: S.observe_cache(k, s, q, A, A, 100)])
+def test_scales_and_caps_at_the_ends_of_their_range(call):
+    # scores are held in units of log 2, and a capped one as tanh(scale / softcap * product): neither factor may overflow or lose bits
+    for bad in (dict(scale=3e38), dict(scale=-3e38), dict(softcap=3e38), dict(softcap=2.0 ** 101), dict(scale=1e-20, softcap=1e19), dict(scale=-1e-20, softcap=2e18)):
+        refused(S.ERR_NONFINITE, "finite" if "softcap" not in bad else "softcap", call, cache(), SEG, queries(**bad))
+    for good in (dict(scale=2e38), dict(softcap=2.0 ** 100), dict(scale=0.0, softcap=1e19), dict(scale=1e-20), dict(scale=1e-20, softcap=1e17)):
+        passes(call, cache(), SEG, queries(**good))
+
+
+# ---- positions that wrap
+def test_tokens_whose_positions_would_wrap():
+    # more tokens than rows, and no positions of their own: token i has position index_base + i
+    top = 2 ** 32
+    refused(S.ERR_DIMENSION, "2^32", S.attend_cache, cache(), S.make_segments([(0, 2, 0, 4, top - 3)]), queries(), A)
+    refused(S.ERR_DIMENSION, "2^32", S.observe_cache, cache(), S.make_segments([(0, 0, 0, 4, top - 3)]), queries(), A, A, 100)
+    passes(S.attend_cache, cache(), S.make_segments([(0, 2, 0, 4, top - 4)]), queries(), A)
+    passes(S.attend_cache, cache(), S.make_segments([(0, 2, 0, 4, top - 3)]), queries(positions=np.zeros(4, np.uint32)), A)
