@@ -519,7 +519,9 @@ typedef struct {
 } SlhaB200CacheEviction;
 
 /* Positions and documents are moved with their rows where both caches have them; they are
- * then the KV heads' own there (entry_head_stride > 0, unless there is one KV head).  All
+ * then the KV heads' own there (entry_head_stride > 0, unless there is one KV head).  So are
+ * rows, weights and tiles (strides > 0), unless all heads keep the same rows.  Where `to` is
+ * given, no array that is written overlaps one that is read.  All
  * arrays of SlhaB200CacheEviction but to_segments are device memory. */
 int32_t slha_b200_evict_cache(const SlhaB200KvCache* cache, const SlhaB200Segment* segments, size_t n_segments,
                               const SlhaB200CacheEviction* eviction);

@@ -275,6 +275,14 @@ int32_t slha_b200_evict_cache(const SlhaB200KvCache* cache, const SlhaB200Segmen
             return Status(SLHA_ERR_DIMENSION, name("in place, tiles_to is the array of tiles or NULL"));
         SciRustSlhaTile* tiles_to = in_place ? const_cast<SciRustSlhaTile*>(ev->tiles) : ev->tiles_to;
         if (ev->tiles && (!cache_aligned(ev->tiles) || !cache_aligned(tiles_to))) return Status(SLHA_ERR_DIMENSION, name("tiles must begin on a multiple of 16 bytes"));
+        // (the heads keep the same rows where they share the weights, and the positions too or no row is kept for its position)
+        const bool alike = cache->n_kv_heads == 1 || (ev->weight_head_stride == 0 && (!cache->positions || cache->entry_head_stride == 0 || (!ev->sink_window && !ev->recent_window)));
+        if (!alike && ev->weights_to && (in_place ? ev->weight_head_stride : ev->weights_to_head_stride) == 0)
+            return Status(SLHA_ERR_DIMENSION, name("each KV head keeps other rows: weights_to must be its own (weights_to_head_stride > 0)"));
+        if (!alike && ev->tiles && (in_place ? ev->tile_head_stride : ev->tiles_to_head_stride) == 0)
+            return Status(SLHA_ERR_DIMENSION, name("each KV head keeps other rows: tiles must be its own where they go (tiles_to_head_stride > 0)"));
+        if (!alike && (to->key_head_stride == 0 || to->value_head_stride == 0))
+            return Status(SLHA_ERR_DIMENSION, name("each KV head keeps other rows: rows must be its own where they go (head strides > 0)"));
         SLHA_TRY(cache_check(cache, fn, true));
         if (!in_place) SLHA_TRY(cache_check(to, fn, true));
         std::vector<SlhaB200Segment> segs, to_segs;

@@ -61,3 +61,21 @@ def test_tokens_whose_positions_would_wrap():
     refused(S.ERR_DIMENSION, "2^32", S.observe_cache, cache(), S.make_segments([(0, 0, 0, 4, top - 3)]), queries(), A, A, 100)
     passes(S.attend_cache, cache(), S.make_segments([(0, 2, 0, 4, top - 4)]), queries(), A)
     passes(S.attend_cache, cache(), S.make_segments([(0, 2, 0, 4, top - 3)]), queries(positions=np.zeros(4, np.uint32)), A)
+
+
+# ---- places that several KV heads would write
+def test_weights_and_tiles_of_heads_that_keep_different_rows():
+    seg, to_seg = S.make_segments([(0, 100, 0, 0, 0)]), S.make_segments([(0, 50, 0, 0, 0)])
+    to = dict(to=cache(), to_segments=to_seg)
+    refused(S.ERR_DIMENSION, "weights_to", S.evict_cache, cache(), seg, A, 100, 50, weights_to=A, weights_to_head_stride=0, **to)
+    refused(S.ERR_DIMENSION, "tiles", S.evict_cache, cache(), seg, A, 100, 50, tiles=A, tile_head_stride=100, tiles_to=A, tiles_to_head_stride=0, **to)
+    refused(S.ERR_DIMENSION, "tiles", S.evict_cache, cache(), seg, A, 100, 50, tiles=A, tile_head_stride=0)  # in place
+    # weights of the heads' own, or of all heads with positions of the heads' own that count
+    own = dict(positions=A, entry_head_stride=100)
+    refused(S.ERR_DIMENSION, "weights_to", S.evict_cache, cache(**own), seg, A, 0, 50, weights_to=A, weights_to_head_stride=0, sink_window=4)
+    for bad in (dict(key_head_stride=0), dict(value_head_stride=0)):
+        refused(S.ERR_DIMENSION, "rows", S.evict_cache, cache(), seg, A, 100, 50, to=cache(**bad), to_segments=to_seg)
+    # every head keeps the same rows; a single head
+    passes(S.evict_cache, cache(), seg, A, 0, 50, weights_to=A, weights_to_head_stride=0, tiles=A, tile_head_stride=0, sink_window=4)
+    passes(S.evict_cache, cache(**own), seg, A, 0, 50, weights_to=A, weights_to_head_stride=0)
+    passes(S.evict_cache, cache(n_kv_heads=1), seg, A, 0, 50, weights_to=A, tiles=A, to=cache(n_kv_heads=1), to_segments=to_seg, tiles_to=A)
