@@ -526,6 +526,17 @@ typedef struct {
 int32_t slha_b200_evict_cache(const SlhaB200KvCache* cache, const SlhaB200Segment* segments, size_t n_segments,
                               const SlhaB200CacheEviction* eviction);
 
+/* Checking aid: which kernels the calling thread's latest call on a cache of rows
+ * launched, a bit each; 0 when there was no such call or it launched none. */
+#define SLHA_B200_CACHE_ATTEND 1        /* up to 64 query rows a block */
+#define SLHA_B200_CACHE_ATTEND_WIDE 2   /* 256 query rows a block */
+#define SLHA_B200_CACHE_OBSERVE 4       /* float32, more than 128 dimensions or 512 query rows */
+#define SLHA_B200_CACHE_OBSERVE_FEW 8   /* the others: up to 32 query rows, */
+#define SLHA_B200_CACHE_OBSERVE_MID 16  /* up to 256 */
+#define SLHA_B200_CACHE_OBSERVE_MANY 32 /* and up to 512 */
+#define SLHA_B200_CACHE_SELECT(ctas) (64 * (ctas)) /* removal by clusters of 1, 2, 4 or 8 CTAs */
+int32_t slha_b200_debug_last_cache_kernels(uint32_t* out);
+
 /*
  * Token-range sharding over the GPUs of one node, one handle per rank (one
  * process or host thread per GPU).  The reference has no multi-device path;

@@ -228,6 +228,7 @@ extern "C" {
         weights_out: *mut f32, weight_head_stride: u64) -> i32;
     pub fn slha_b200_evict_cache(cache: *const SlhaB200KvCache, segments: *const SlhaB200Segment, n_segments: usize,
         eviction: *const SlhaB200CacheEviction) -> i32;
+    pub fn slha_b200_debug_last_cache_kernels(out: *mut u32) -> i32;
     pub fn slha_b200_shard_unique_id(id_out: *mut c_void) -> i32;
     pub fn slha_b200_shard_init(nccl_unique_id: *const c_void, rank: i32, world: i32, out: *mut *mut SlhaB200Shard) -> i32;
     pub fn slha_b200_shard_destroy(shard: *mut SlhaB200Shard) -> i32;

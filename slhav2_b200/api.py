@@ -99,6 +99,7 @@ SIGNATURES = {
     "slha_b200_attend_tree": (_i32, [_vp, _vp, _sz, _vp, _vp, _vp, _u64, _u64, _vp]),
     "slha_b200_observe_cache": (_i32, [_vp, _vp, _sz, _vp, _vp, _vp, C.c_float, _vp, _u64]),
     "slha_b200_evict_cache": (_i32, [_vp, _vp, _sz, _vp]),
+    "slha_b200_debug_last_cache_kernels": (_i32, [_vp]),
     "slha_b200_shard_unique_id": (_i32, [_vp]),
     "slha_b200_shard_init": (_i32, [_vp, _i32, _i32, C.POINTER(_vp)]),
     "slha_b200_shard_destroy": (_i32, [_vp]),
@@ -601,6 +602,17 @@ def evict_cache(cache, segments, weights, weight_head_stride, budget, sink_windo
                        None if to_seg is None else to_seg.ctypes.data, ptr(weights_to), weights_to_head_stride, ptr(tiles), tile_head_stride, ptr(tiles_to),
                        tiles_to_head_stride, ptr(source_out), ptr(rows_out))
     _check(load_library().slha_b200_evict_cache(cache.address, seg.ctypes.data, len(seg), C.addressof(e)))
+
+
+CACHE_ATTEND, CACHE_ATTEND_WIDE, CACHE_OBSERVE, CACHE_OBSERVE_FEW, CACHE_OBSERVE_MID, CACHE_OBSERVE_MANY = 1, 2, 4, 8, 16, 32
+CACHE_SELECT = 64  # times the CTAs of a cluster
+
+
+def debug_last_cache_kernels():
+    """Checking aid: the kernels that this thread's latest call on a cache of rows launched (CACHE_*, a bit each)."""
+    out = np.zeros(1, np.uint32)
+    _check(load_library().slha_b200_debug_last_cache_kernels(ptr(out)))
+    return int(out[0])
 
 
 def shard_unique_id():

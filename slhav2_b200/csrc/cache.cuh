@@ -167,6 +167,8 @@ inline cudaError_t launch_cluster(void (*kernel)(P...), dim3 grid, dim3 block, s
     cfg.numAttrs = size > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...);
 }
+// Which kernels the calling thread's latest call on a cache of rows launched (SLHA_B200_CACHE_*).
+extern thread_local uint32_t g_cache_kernels;
 // The table of a launch: in the kernel's parameters, or uploaded where it is longer.
 Status cache_table(Ctx* c, const std::vector<CacheSeg>& segs, CacheTable* inl, const CacheSeg** dev);
 // Raises a kernel's limit of dynamic shared memory, once per kernel and device.

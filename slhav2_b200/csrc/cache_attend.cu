@@ -21,6 +21,7 @@
 #include "cache_mma.cuh"
 
 namespace slha {
+thread_local uint32_t g_cache_kernels = 0;
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
@@ -616,6 +617,7 @@ Status launch_class(Ctx* c, CacheArgs a, CacheWork w) {
     SLHA_TRY(cache_part_memory(&a, w.blocks ? w.items : 0, S::MB, &mem));
     const size_t smem = a.tree ? S::SMEM_TREE : S::SMEM;
     SLHA_TRY((cache_smem<cache_attend_kernel<T, D, WM>>(c, S::SMEM_TREE)));
+    g_cache_kernels |= SLHA_B200_CACHE_ATTEND;
     SLHA_CUDA(launch_cluster(cache_attend_kernel<T, D, WM>, dim3((uint32_t)(w.items * a.n_kv)), dim3(ATT_THREADS), smem, c->stream, std::max(a.cluster, 1u), a, tab));
     count_launch();
     if (w.blocks) SLHA_TRY(launch_cache_join(c, a, sizeof(T) == 2 ? SLHA_B200_BF16 : SLHA_B200_F32, w, S::MB));

@@ -1081,6 +1081,7 @@ Status launch_wide(Ctx* c, CacheArgs a, CacheWork w, const WideMaps& maps) {
         return cudaFuncGetAttributes(&at, cache_attend_wide_kernel<D, CAP, KIND>) == cudaSuccess ? at.numRegs : 0;
     }();
     if (regs != REGS_ALL) return Status(SLHA_ERR_DEVICE, "attention over a cache: the kernel was built with other registers than its warps share out");
+    g_cache_kernels |= SLHA_B200_CACHE_ATTEND_WIDE;
     for (const CacheWork& x : works) {
         CacheTable tab;
         SLHA_TRY(cache_table(c, x.segs, &tab, &a.table));

@@ -377,6 +377,7 @@ Status launch_evict_cache(Ctx* c, EvictArgs a, const std::vector<SlhaB200Segment
     uint32_t c_size = most >= 65536 ? 8 : most >= 16384 ? 4 : 1;
     while (c_size > 1 && heads * c_size > (uint64_t)sm_count(c->device) * (c_size == 8 ? 2 : 3) / 3) c_size /= 2;
     const size_t share = ((size_t)most + c_size * SEL_WARPS * 128 - 1) / (c_size * SEL_WARPS * 128) * SEL_WARPS * 128, smem = std::min<size_t>(share, SEL_HELD) * 4;
+    g_cache_kernels |= SLHA_B200_CACHE_SELECT(c_size);
     const auto select = [&](auto kernel_of) -> Status {
         constexpr auto kernel = cache_select_kernel<decltype(kernel_of)::value>;
         SLHA_TRY((cache_smem<kernel>(c, SEL_HELD * 4)));

@@ -217,6 +217,7 @@ Status launch_observe_t(Ctx* c, CacheArgs a, std::vector<CacheSeg>& segs) {
     SLHA_TRY(cache_table(c, segs, &tab, &a.table));
     a.n_segs = (uint32_t)segs.size();
     SLHA_TRY((cache_smem<cache_observe_kernel<T, D, QB>>(c, S::SMEM)));
+    g_cache_kernels |= SLHA_B200_CACHE_OBSERVE;
     SLHA_CUDA(launch_behind(cache_observe_kernel<T, D, QB>, dim3((uint32_t)(items * a.n_kv)), dim3(OBS_THREADS), S::SMEM, c->stream, a, tab));
     count_launch();
     return Status();

@@ -390,6 +390,7 @@ Status launch_observe_wide_t(Ctx* c, CacheArgs a, std::vector<CacheSeg>& segs, c
     a.n_segs = (uint32_t)segs.size();
     constexpr auto kernel = cache_observe_wide_kernel<D, MODE>;
     SLHA_TRY((cache_smem<kernel>(c, S::SMEM)));
+    g_cache_kernels |= MODE == FEW ? SLHA_B200_CACHE_OBSERVE_FEW : MODE == MID ? SLHA_B200_CACHE_OBSERVE_MID : SLHA_B200_CACHE_OBSERVE_MANY;
     SLHA_CUDA(launch_behind(kernel, dim3((uint32_t)(items * a.n_kv)), dim3(S::THREADS), S::SMEM, c->stream, a, maps, tab));
     count_launch();
     return Status();

@@ -156,6 +156,7 @@ Status cache_arguments(Ctx* c, const SlhaB200KvCache* k, size_t n_segs, const Sl
 int32_t attend_cache_any(const char* fn, const SlhaB200KvCache* cache, const SlhaB200Segment* segments, size_t n_segments, const SlhaB200CacheQueries* queries,
                          const uint32_t* parents, bool tree, void* out, uint64_t out_token_stride, uint64_t out_head_stride, float* lse_out) {
     return ffi([&]() -> Status {
+        g_cache_kernels = 0;
         const auto name = [&](const char* what) { return std::string(fn) + ": " + what; };
         if (!cache || !queries || (n_segments && !segments)) return Status(SLHA_ERR_NULL, std::string(fn) + " received a NULL pointer");
         if (n_segments == 0 || queries->n_tokens == 0) return Status();
@@ -203,6 +204,14 @@ int32_t attend_cache_any(const char* fn, const SlhaB200KvCache* cache, const Slh
 
 extern "C" {
 
+int32_t slha_b200_debug_last_cache_kernels(uint32_t* out) {
+    return ffi([&]() -> Status {
+        if (!out) return Status(SLHA_ERR_NULL, "slha_b200_debug_last_cache_kernels received a NULL pointer");
+        *out = g_cache_kernels;
+        return Status();
+    });
+}
+
 int32_t slha_b200_attend_cache(const SlhaB200KvCache* cache, const SlhaB200Segment* segments, size_t n_segments, const SlhaB200CacheQueries* queries, void* out,
                                uint64_t out_token_stride, uint64_t out_head_stride, float* lse_out) {
     return attend_cache_any("slha_b200_attend_cache", cache, segments, n_segments, queries, nullptr, false, out, out_token_stride, out_head_stride, lse_out);
@@ -215,6 +224,7 @@ int32_t slha_b200_attend_tree(const SlhaB200KvCache* cache, const SlhaB200Segmen
 int32_t slha_b200_observe_cache(const SlhaB200KvCache* cache, const SlhaB200Segment* segments, size_t n_segments, const SlhaB200CacheQueries* queries,
                                 const float* lse, const float* weights_in, float decay, float* weights_out, uint64_t weight_head_stride) {
     return ffi([&]() -> Status {
+        g_cache_kernels = 0;
         const char* fn = "slha_b200_observe_cache";
         const auto name = [&](const char* what) { return std::string(fn) + ": " + what; };
         if (!cache || !queries || !lse || !weights_out || (n_segments && !segments)) return Status(SLHA_ERR_NULL, std::string(fn) + " received a NULL pointer");
@@ -254,6 +264,7 @@ int32_t slha_b200_observe_cache(const SlhaB200KvCache* cache, const SlhaB200Segm
 
 int32_t slha_b200_evict_cache(const SlhaB200KvCache* cache, const SlhaB200Segment* segments, size_t n_segments, const SlhaB200CacheEviction* ev) {
     return ffi([&]() -> Status {
+        g_cache_kernels = 0;
         const char* fn = "slha_b200_evict_cache";
         const auto name = [&](const char* what) { return std::string(fn) + ": " + what; };
         if (!cache || !ev || (n_segments && !segments) || (ev && (!ev->weights || (ev->to && !ev->to_segments))))

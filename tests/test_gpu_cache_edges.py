@@ -328,3 +328,62 @@ def test_rows_of_more_than_one_run_keep_to_their_working_memory():
     assert grown[0] <= 16 << 20 and grown[1] <= 600 << 20, grown
     assert float((lses[0] - lses[1]).abs().max()) <= 2e-5
     assert float((outs[0].float() - outs[1].float()).abs().max()) <= 2.0 ** -6 * float(v.float().abs().max())
+
+
+
+# ---- kernels that only long caches reach
+@pytest.mark.parametrize("tokens,group,d,lens,name", [(16, 4, 128, (10000,), "MID"), (40, 4, 128, (10000,), "MID"), (64, 4, 128, (9990,), "MID"), (100, 4, 128, (10000,), "MANY"),
+                                                      (64, 8, 80, (9000, 700), "MANY"), (1, 4, 128, (20000, 77), "MID"), (8, 4, 128, (19990, 130), "MID"), (16, 4, 80, (10000,), "MID"),
+                                                      (1, 4, 128, (9000, 4100, 7000, 2900, 5200, 3300), "FEW"), (4, 4, 80, (9000, 4100, 7000, 2900, 5200, 3300), "FEW"),
+                                                      (12, 4, 64, (10000,), "MID"), (128, 4, 64, (10000,), "MANY"), (1, 4, 64, (9000, 4100, 7000, 2900, 5200, 3300), "FEW")])
+@pytest.mark.parametrize("more", [dict(), dict(softcap=5.0, alibi=True), dict(docs=True), dict(window=3000)])
+def test_weights_of_rows_by_every_kernel_in_runs_longer_than_its_ring(tokens, group, d, lens, name, more):
+    rng = np.random.default_rng(tokens * 7 + group + d)
+    kv, total = 8, sum(lens)
+    kind = {k: v for k, v in more.items() if k in ("softcap", "window")}
+    if more.get("alibi"):
+        kind["slopes"] = (2.0 ** -np.arange(1, kv * group + 1) / 64).astype(F)
+    if more.get("docs"):
+        doc = np.sort(rng.integers(1, 4, total)).astype(np.uint32)
+        kind["row_doc"] = np.stack([doc] * kv)
+        kind["q_doc"] = rng.integers(1, 5, tokens * len(lens)).astype(np.uint32)
+    call, raw = T.make(rng, lens, tokens, kv, group, d, True, **kind)
+    cache, segs, queries = T.on_device(call, raw, True)
+    _, lse = T.results(call, True, cache, segs, queries)
+    before = rng.random((kv, total)).astype(F)
+    w = S.to_device(before)
+    S.observe_cache(cache, segs, queries, S.to_device(lse), w, total, weights_in=w, decay=0.5)
+    assert S.debug_last_cache_kernels() == getattr(S, "CACHE_OBSERVE_" + name)
+    want, tol = call.received(lse, before, 0.5)
+    T.held(w.download(F, kv * total).reshape(kv, total), want, tol)
+
+
+@pytest.mark.parametrize("n_kv,n,budget,ctas", [(3, 20001, 20000, 4), (2, 16384, 90, 4), (13, 70000, 600, 4), (25, 16500, 500, 2), (1, 65536, 65535, 8), (3, 131072, 70000, 8), (1, 500000, 3000, 8), (40, 9000, 100, 1)])
+@pytest.mark.parametrize("recent", [0, 700])
+def test_removal_by_clusters_from_rows_that_have_moved(n_kv, n, budget, ctas, recent):
+    # each head's newest row lies in another CTA's share; the second segment's rows begin elsewhere
+    rng = np.random.default_rng(n)
+    lens, total = (n, n // 3), n + n // 3
+    pos = np.zeros((n_kv, total), np.uint32)
+    w = rng.integers(0, 50, (n_kv, total)).astype(F)
+    for h in range(n_kv):
+        b = 0
+        for m in lens:
+            p = rng.permutation(2 * m)[:m]
+            top = int(p.argmax())
+            to = (h * 2 + 1) * m // (2 * n_kv)
+            p[top], p[to] = p[to], p[top]
+            pos[h, b:b + m] = p
+            b += m
+    k = rng.integers(0, 65536, (total, n_kv, 8)).astype(np.uint16)
+    cache = S.KvCache(S.to_device(k), S.to_device(k), n_kv, 8, positions=S.to_device(pos), entry_head_stride=total)
+    src = S.DeviceBuffer(2 * 4 * n_kv * budget)
+    keep = S.KvCache(S.DeviceBuffer(2 * budget * n_kv * 16), S.DeviceBuffer(2 * budget * n_kv * 16), n_kv, 8)
+    S.evict_cache(cache, S.make_segments([(0, n, 0, 0, 0), (n, n // 3, 0, 0, 0)]), S.to_device(w), total, budget, sink_window=9, recent_window=recent, source_out=src, to=keep,
+                  to_segments=S.make_segments([(0, budget, 0, 0, 0), (budget, budget, 0, 0, 0)]))
+    assert S.debug_last_cache_kernels() == S.CACHE_SELECT * ctas
+    got = src.download(np.uint32, 2 * n_kv * budget).reshape(2, n_kv, budget)
+    for h in range(0, n_kv, max(1, n_kv // 4)):
+        for i, (b, m) in enumerate(((0, n), (n, n // 3))):
+            want = K.evict(w[h, b:b + m], pos[h, b:b + m], budget, 9, recent)
+            assert np.array_equal(got[i, h, :len(want)], want)
