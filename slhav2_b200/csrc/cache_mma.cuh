@@ -119,19 +119,19 @@ __device__ __forceinline__ void scores_step(float (&s)[N][4], const AFrag<T>& a,
         }
     }
 }
-// All k steps of s[n][.] = Q K^T; load(kk) brings the A operand of one.  The tensor cores cut each product's sum off towards zero: float32 sums are taken four steps at a time and added
-// here, to the nearest (7 x 18 drafted tokens over 390 rows, 128 dimensions: outputs 2.2e-6 off without, 6.5e-7 with; 5 % of the time).
-template <typename T, int D, int N, typename Load>
+// All k steps of s[n][.] = Q K^T; load(kk) brings the A operand of one.  The tensor cores cut each product's sum off towards zero: sums of which more than bfloat16 counts are taken four
+// steps at a time (AT_ONCE; 0: all) and added here, to the nearest (float32, 7 x 18 drafted tokens over 390 rows, 128 dimensions: outputs 2.2e-6 off without, 6.5e-7 with; 5 % of the time).
+template <typename T, int D, int N, int AT_ONCE = sizeof(T) == 2 ? 0 : 4, typename Load>
 __device__ __forceinline__ void scores_of(float (&s)[N][4], Load load, uint32_t kbase, int key0, int lane) {
-    if constexpr (sizeof(T) == 2) {
+    if constexpr (!AT_ONCE) {
 #pragma unroll 4
         for (int kk = 0; kk < D / 16; ++kk) scores_step<T, D, N>(s, load(kk), kbase, key0, kk, lane);
     } else {
 #pragma unroll 1
-        for (int k4 = 0; k4 < D / 8; k4 += 4) {
+        for (int k4 = 0; k4 < D / (sizeof(T) == 2 ? 16 : 8); k4 += AT_ONCE) {
             float part[N][4] = {};
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) scores_step<T, D, N>(part, load(k4 + kk), kbase, key0, k4 + kk, lane);
+            for (int kk = 0; kk < AT_ONCE; ++kk) scores_step<T, D, N>(part, load(k4 + kk), kbase, key0, k4 + kk, lane);
 #pragma unroll
             for (int n = 0; n < N; ++n)
 #pragma unroll

@@ -82,7 +82,9 @@ __global__ void __launch_bounds__(Obs<D, MODE>::THREADS, Obs<D, MODE>::CTAS)
     const auto bar = [&](int which) { return bars + which * 8; };
     // rows of a block of query rows, as columns: a multiple of 16
     // The tensor cores cut their sums off after each step of 16 elements, towards zero: eight steps of a score of 90 (8 once scaled) lose 1.3e-6 of its weight.  Where the columns
-    // suffice a score is two sums, of 64 elements each, which halves that (8 x 8192 rows after a decode step: 1.1e-6 -> 4.1e-7).
+    // suffice a score is two sums, of 64 elements each, which halves that (8 x 8192 rows after a decode step: 1.1e-6 -> 4.1e-7).  With more query rows they are left as they are: the
+    // losses of many scores partly make up for one another in a row's weight, and half the query rows a product cost more than that (256 query rows on 32768 rows: 3.3e-7 off and
+    // 41.2 us, in halves 2.3e-7 and 45.9 us; the same in float32 products of the whole 1.7e-7 to 2.7e-7).
     constexpr uint32_t SECOND = S::PLACE / 2;
     const bool halved = D > 64 && MODE != MANY && q_rows <= SECOND;
     const auto columns = [&](uint32_t b) { return min((uint32_t)S::BLOCK, (q_rows - b * S::BLOCK + 31) / 32 * 32); };

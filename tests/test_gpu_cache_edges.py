@@ -387,3 +387,25 @@ def test_removal_by_clusters_from_rows_that_have_moved(n_kv, n, budget, ctas, re
         for i, (b, m) in enumerate(((0, n), (n, n // 3))):
             want = K.evict(w[h, b:b + m], pos[h, b:b + m], budget, 9, recent)
             assert np.array_equal(got[i, h, :len(want)], want)
+
+
+# ---- sums that the tensor cores cut off
+@pytest.mark.parametrize("tokens,d", [(1, 256), (24, 200), (600, 128)])
+def test_scores_of_observed_rows_are_not_cut_off_step_by_step(tokens, d):
+    # All products are positive, so that a sum taken on the tensor cores loses half a step of 2^-23 of itself with every 16 elements: (1 + .. + 16) / 16 halves of a score of 20 for 256
+    # dimensions, 2.5 where four steps are taken at a time and added to the nearest: 20 * 2.5 * 2^-24 = 3.0e-6 of a weight, here with half as much again.
+    rng = np.random.default_rng(d)
+    n = 1000
+    keys, dk = K.as_type(2.0 ** rng.uniform(-5.0, 0.0, (n, 1, d)), True)  # (of several sizes: sums of equally large ones would be exact)
+    q, dq = K.as_type(2.0 ** rng.uniform(-5.0, 0.0, (tokens, 1, d)), True)
+    scale = float(F(20.0 / np.einsum("tgd,rgd->tr", q, keys).mean()))
+    call = K.Call(keys, keys, q, [(0, n, 0, tokens, 0)], scale, causal=False)
+    want_lse = call.attend(True)[1].astype(F)
+    cache, queries = S.KvCache(S.to_device(dk), None, 1, d), S.CacheQueries(S.to_device(dq), tokens, 1, d, scale=scale, causal=False)
+    w = S.to_device(np.zeros(n, F))
+    S.observe_cache(cache, S.make_segments(call.segs), queries, S.to_device(want_lse), w, n)
+    assert S.debug_last_cache_kernels() == S.CACHE_OBSERVE
+    want, _ = call.received(want_lse, np.zeros((1, n), F), 1.0)
+    off = w.download(F, n) / want[0] - 1.0
+    print(off.mean(), off.std())
+    assert abs(off.mean()) <= 20 * 1.5 * 2.5 * 2.0 ** -24
