@@ -498,6 +498,29 @@ def attend_topk(top_index, top_score, k, scale, values, d_v, value_dtype=F32, to
     return out
 
 
+_ROWS = {F32: ("float32",), BF16: ("bfloat16", "uint16", "int16")}
+_U32, _F32 = ("uint32", "int32"), ("float32",)
+_dtype_names = {}
+
+
+def _typed(a, names, what):
+    """ptr(a) of an array or tensor whose elements are what a call reads them as; addresses and raw buffers bring no type."""
+    dtype = getattr(a, "dtype", None)
+    if dtype is not None:
+        name = _dtype_names.get(dtype)
+        if name is None:
+            name = _dtype_names[dtype] = str(dtype).rsplit(".", 1)[-1]
+        if name not in names:
+            raise TypeError("%s: %s where %s is read" % (what, name, names[0]))
+    return ptr(a)
+
+
+def _in_order(a, given, what):
+    """A tensor that is read by default strides lies as they say."""
+    if given is None and hasattr(a, "is_contiguous") and not a.is_contiguous():
+        raise ValueError("%s: not contiguous, its strides must be given" % what)
+
+
 class _KvCache(C.Structure):
     _fields_ = [
         ("keys", _vp), ("values", _vp), ("dtype", _i32), ("head_dim", _u32), ("n_kv_heads", _u32),
@@ -531,11 +554,16 @@ class KvCache:
             return default if given is None else given
 
         rows = None if rows is None else _np(rows, np.uint32)
+        kind = _ROWS.get(dtype, ())  # (another dtype is the library's to refuse)
+        for a, row, head, what in ((keys, key_row_stride, key_head_stride, "keys"), (values, value_row_stride, value_head_stride, "values")):
+            if kind:
+                _typed(a, kind, what)
+            _in_order(a, row if row is not None else head, what)
         self.kept = (keys, values, positions, documents, rows)
         self.head_dim, self.n_kv_heads, self.dtype = head_dim, n_kv_heads, dtype
         self.c = _KvCache(ptr(keys), ptr(values), dtype, head_dim, n_kv_heads, stride(key_row_stride, n_kv_heads * head_dim), stride(key_head_stride, head_dim),
-                          stride(value_row_stride, n_kv_heads * head_dim), stride(value_head_stride, head_dim), ptr(positions), ptr(documents),
-                          entry_head_stride, ptr(rows))
+                          stride(value_row_stride, n_kv_heads * head_dim), stride(value_head_stride, head_dim), _typed(positions, _U32, "positions"),
+                          _typed(documents, _U32, "documents"), entry_head_stride, _typed(rows, _U32, "rows"))
         self.address = C.addressof(self.c)
 
 
@@ -547,11 +575,14 @@ class CacheQueries:
                  token_stride=None, head_stride=None):
         slopes = None if slopes is None else _np(slopes, np.float32)
         prefix, positions, documents = (None if x is None else _np(x, np.uint32) for x in (prefix, positions, documents))
+        _typed(q, _ROWS[F32] + _ROWS[BF16], "q")
+        _in_order(q, token_stride if token_stride is not None else head_stride, "q")
         self.kept = (q, slopes, prefix, positions, documents)
         self.n_heads, self.head_dim = n_heads, head_dim
         self.c = _CacheQueries(ptr(q), n_tokens, n_heads, n_heads * head_dim if token_stride is None else token_stride,
                                head_dim if head_stride is None else head_stride, head_dim ** -0.5 if scale is None else scale, softcap, window,
-                               1 if causal else 0, ptr(slopes), ptr(prefix), ptr(positions), ptr(documents))
+                               1 if causal else 0, _typed(slopes, _F32, "slopes"), _typed(prefix, _U32, "prefix"), _typed(positions, _U32, "positions"),
+                               _typed(documents, _U32, "documents"))
         self.address = C.addressof(self.c)
 
 
@@ -561,14 +592,23 @@ def _segments(segments):
     return np.ascontiguousarray(segments, SEGMENT_DTYPE)
 
 
+def _same_type(cache, queries, out, what="out"):
+    """The address of `out`; rows, queries and outputs of a call have one type."""
+    kind = _ROWS.get(cache.dtype)
+    if kind:
+        _typed(queries.kept[0], kind, "q")
+        return ptr(out) if out is None else _typed(out, kind, what)
+    return ptr(out)
+
+
 def attend_cache(cache, segments, queries, out, lse_out=None, out_token_stride=None, out_head_stride=None):
     """Exact attention of `queries` (CacheQueries) over `cache` (KvCache): out [token][head][head_dim] of the cache's type and, where given, lse_out
     [token][head] float32, both device memory; see slha_b200_attend_cache."""
     seg = _segments(segments)
     d = cache.head_dim
-    _check(load_library().slha_b200_attend_cache(cache.address, seg.ctypes.data, len(seg), queries.address, ptr(out),
+    _check(load_library().slha_b200_attend_cache(cache.address, seg.ctypes.data, len(seg), queries.address, _same_type(cache, queries, out),
                                                  queries.n_heads * d if out_token_stride is None else out_token_stride,
-                                                 d if out_head_stride is None else out_head_stride, ptr(lse_out)))
+                                                 d if out_head_stride is None else out_head_stride, _typed(lse_out, _F32, "lse_out")))
     return out
 
 
@@ -578,9 +618,9 @@ def attend_tree(cache, segments, queries, parents, out, lse_out=None, out_token_
     seg = _segments(segments)
     par = _np(parents, np.uint32)
     d = cache.head_dim
-    _check(load_library().slha_b200_attend_tree(cache.address, seg.ctypes.data, len(seg), queries.address, ptr(par), ptr(out),
+    _check(load_library().slha_b200_attend_tree(cache.address, seg.ctypes.data, len(seg), queries.address, _typed(par, _U32, "parents"), _same_type(cache, queries, out),
                                                 queries.n_heads * d if out_token_stride is None else out_token_stride,
-                                                d if out_head_stride is None else out_head_stride, ptr(lse_out)))
+                                                d if out_head_stride is None else out_head_stride, _typed(lse_out, _F32, "lse_out")))
     return out
 
 
@@ -588,8 +628,9 @@ def observe_cache(cache, segments, queries, lse, weights_out, weight_head_stride
     """The weight each row received: weights_out [kv_head][row] = decay * weights_in + the softmax weights of the tokens that see it (lse as attend_cache wrote
     it); see slha_b200_observe_cache."""
     seg = _segments(segments)
-    _check(load_library().slha_b200_observe_cache(cache.address, seg.ctypes.data, len(seg), queries.address, ptr(lse), ptr(weights_in), decay,
-                                                  ptr(weights_out), weight_head_stride))
+    _same_type(cache, queries, None)
+    _check(load_library().slha_b200_observe_cache(cache.address, seg.ctypes.data, len(seg), queries.address, _typed(lse, _F32, "lse"), _typed(weights_in, _F32, "weights_in"), decay,
+                                                  _typed(weights_out, _F32, "weights_out"), weight_head_stride))
     return weights_out
 
 
@@ -598,9 +639,9 @@ def evict_cache(cache, segments, weights, weight_head_stride, budget, sink_windo
     """Removal of the rows of least weight, `budget` stay a KV head; in place, or into the cache `to`; see slha_b200_evict_cache."""
     seg = _segments(segments)
     to_seg = None if to_segments is None else _segments(to_segments)
-    e = _CacheEviction(ptr(weights), weight_head_stride, budget, sink_window, recent_window, None if to is None else to.address,
-                       None if to_seg is None else to_seg.ctypes.data, ptr(weights_to), weights_to_head_stride, ptr(tiles), tile_head_stride, ptr(tiles_to),
-                       tiles_to_head_stride, ptr(source_out), ptr(rows_out))
+    e = _CacheEviction(_typed(weights, _F32, "weights"), weight_head_stride, budget, sink_window, recent_window, None if to is None else to.address,
+                       None if to_seg is None else to_seg.ctypes.data, _typed(weights_to, _F32, "weights_to"), weights_to_head_stride, ptr(tiles), tile_head_stride,
+                       ptr(tiles_to), tiles_to_head_stride, _typed(source_out, _U32, "source_out"), _typed(rows_out, _U32, "rows_out"))
     _check(load_library().slha_b200_evict_cache(cache.address, seg.ctypes.data, len(seg), C.addressof(e)))
 
 

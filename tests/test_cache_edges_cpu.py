@@ -79,3 +79,34 @@ def test_weights_and_tiles_of_heads_that_keep_different_rows():
     passes(S.evict_cache, cache(), seg, A, 0, 50, weights_to=A, weights_to_head_stride=0, tiles=A, tile_head_stride=0, sink_window=4)
     passes(S.evict_cache, cache(**own), seg, A, 0, 50, weights_to=A, weights_to_head_stride=0)
     passes(S.evict_cache, cache(n_kv_heads=1), seg, A, 0, 50, weights_to=A, tiles=A, to=cache(n_kv_heads=1), to_segments=to_seg, tiles_to=A)
+
+
+# ---- tensors of other types and orders
+def test_tensors_are_what_a_call_reads_them_as():
+    torch = pytest.importorskip("torch")
+    rows, heads, d = 8, 2, 64
+    kv = torch.zeros(rows, heads, d, dtype=torch.bfloat16)
+    u32, f32 = torch.zeros(heads * rows, dtype=torch.int32), torch.zeros(heads * rows)
+    seg = S.make_segments([(0, rows, 0, 4, 0)])
+    for what, more in (("keys", dict(keys=kv.float())), ("keys", dict(keys=kv.half())), ("values", dict(values=kv.float())), ("keys", dict(dtype=S.F32)), ("positions", dict(positions=u32.long())),
+                       ("documents", dict(documents=f32)), ("rows", dict(rows=u32.long())), ("keys", dict(keys=np.zeros((rows, heads, d))))):
+        with pytest.raises(TypeError, match=what):
+            cache(**{**dict(keys=kv, values=kv), **more})
+    for what, more in (("q", dict(q=torch.zeros(4, 4, d, dtype=torch.float64))), ("slopes", dict(slopes=f32.double())), ("prefix", dict(prefix=u32.short())), ("positions", dict(positions=u32.long())),
+                       ("documents", dict(documents=f32))):
+        with pytest.raises(TypeError, match=what):
+            queries(**more)
+    with pytest.raises(ValueError, match="keys"):
+        cache(keys=kv.transpose(0, 1), values=kv)
+    with pytest.raises(ValueError, match="q"):
+        queries(q=kv.transpose(0, 1))
+    cache(keys=kv.transpose(0, 1), values=kv, key_row_stride=heads * d)  # strides that are given are the caller's
+    k, q = cache(keys=kv, values=kv.view(torch.int16)), queries(q=torch.zeros(4, 4, d, dtype=torch.bfloat16))
+    for what, call in (("q", lambda: S.attend_cache(k, seg, queries(q=torch.zeros(4, 4, d)), A)), ("out", lambda: S.attend_cache(k, seg, q, torch.zeros(4, 4, d))),
+                       ("lse_out", lambda: S.attend_cache(k, seg, q, A, torch.zeros(4, 4, dtype=torch.bfloat16))), ("parents", lambda: S.attend_tree(k, seg, q, u32.long(), A)),
+                       ("q", lambda: S.observe_cache(k, seg, queries(q=torch.zeros(4, 4, d)), A, A, 8)), ("lse", lambda: S.observe_cache(k, seg, q, f32.double(), A, 8)),
+                       ("weights_out", lambda: S.observe_cache(k, seg, q, A, f32.double(), 8)), ("weights", lambda: S.evict_cache(k, seg, u32, 8, 4)),
+                       ("rows_out", lambda: S.evict_cache(k, seg, A, 8, 4, rows_out=u32.long())), ("source_out", lambda: S.evict_cache(k, seg, A, 8, 4, source_out=f32))):
+        with pytest.raises(TypeError, match=what):
+            call()
+    passes(S.attend_cache, k, seg, q, torch.zeros(4, 4, d, dtype=torch.bfloat16), torch.zeros(4, 4))
