@@ -498,20 +498,31 @@ def attend_topk(top_index, top_score, k, scale, values, d_v, value_dtype=F32, to
     return out
 
 
-_ROWS = {F32: ("float32",), BF16: ("bfloat16", "uint16", "int16")}
-_U32, _F32 = ("uint32", "int32"), ("float32",)
-_dtype_names = {}
+# Element types that a call reads: their names, and the types that have been found to bear them (None: addresses and raw buffers bring no type).
+_ROWS = {F32: {None, "float32"}, BF16: {None, "bfloat16", "uint16", "int16"}}
+_U32, _F32 = {None, "uint32", "int32"}, {None, "float32"}
 
 
-def _typed(a, names, what):
-    """ptr(a) of an array or tensor whose elements are what a call reads them as; addresses and raw buffers bring no type."""
+class _Any:
+    def __contains__(self, dtype):
+        return True
+
+
+def _fits(dtype, kind, what):
+    name = str(dtype).rsplit(".", 1)[-1]
+    if name not in kind:
+        raise TypeError("%s: %s where %s is read" % (what, name, " or ".join(sorted(x for x in kind if isinstance(x, str)))))
+    kind.add(dtype)
+
+
+def _typed(a, kind, what):
+    """ptr(a), whose elements are what a call reads them as."""
     dtype = getattr(a, "dtype", None)
     if dtype is not None:
-        name = _dtype_names.get(dtype)
-        if name is None:
-            name = _dtype_names[dtype] = str(dtype).rsplit(".", 1)[-1]
-        if name not in names:
-            raise TypeError("%s: %s where %s is read" % (what, name, names[0]))
+        if dtype not in kind:
+            _fits(dtype, kind, what)
+        if not isinstance(a, np.ndarray):
+            return a.data_ptr()
     return ptr(a)
 
 
@@ -554,10 +565,9 @@ class KvCache:
             return default if given is None else given
 
         rows = None if rows is None else _np(rows, np.uint32)
-        kind = _ROWS.get(dtype, ())  # (another dtype is the library's to refuse)
+        self.kind = kind = _ROWS.get(dtype) or _Any()  # (another dtype is the library's to refuse)
         for a, row, head, what in ((keys, key_row_stride, key_head_stride, "keys"), (values, value_row_stride, value_head_stride, "values")):
-            if kind:
-                _typed(a, kind, what)
+            _typed(a, kind, what)
             _in_order(a, row if row is not None else head, what)
         self.kept = (keys, values, positions, documents, rows)
         self.head_dim, self.n_kv_heads, self.dtype = head_dim, n_kv_heads, dtype
@@ -575,7 +585,8 @@ class CacheQueries:
                  token_stride=None, head_stride=None):
         slopes = None if slopes is None else _np(slopes, np.float32)
         prefix, positions, documents = (None if x is None else _np(x, np.uint32) for x in (prefix, positions, documents))
-        _typed(q, _ROWS[F32] + _ROWS[BF16], "q")
+        _typed(q, _ROWS[BF16] | _ROWS[F32], "q")
+        self.type = getattr(q, "dtype", None)
         _in_order(q, token_stride if token_stride is not None else head_stride, "q")
         self.kept = (q, slopes, prefix, positions, documents)
         self.n_heads, self.head_dim = n_heads, head_dim
@@ -592,21 +603,14 @@ def _segments(segments):
     return np.ascontiguousarray(segments, SEGMENT_DTYPE)
 
 
-def _same_type(cache, queries, out, what="out"):
-    """The address of `out`; rows, queries and outputs of a call have one type."""
-    kind = _ROWS.get(cache.dtype)
-    if kind:
-        _typed(queries.kept[0], kind, "q")
-        return ptr(out) if out is None else _typed(out, kind, what)
-    return ptr(out)
-
-
 def attend_cache(cache, segments, queries, out, lse_out=None, out_token_stride=None, out_head_stride=None):
     """Exact attention of `queries` (CacheQueries) over `cache` (KvCache): out [token][head][head_dim] of the cache's type and, where given, lse_out
     [token][head] float32, both device memory; see slha_b200_attend_cache."""
     seg = _segments(segments)
     d = cache.head_dim
-    _check(load_library().slha_b200_attend_cache(cache.address, seg.ctypes.data, len(seg), queries.address, _same_type(cache, queries, out),
+    if queries.type not in cache.kind:
+        _fits(queries.type, cache.kind, "q")
+    _check(load_library().slha_b200_attend_cache(cache.address, seg.ctypes.data, len(seg), queries.address, _typed(out, cache.kind, "out"),
                                                  queries.n_heads * d if out_token_stride is None else out_token_stride,
                                                  d if out_head_stride is None else out_head_stride, _typed(lse_out, _F32, "lse_out")))
     return out
@@ -618,7 +622,9 @@ def attend_tree(cache, segments, queries, parents, out, lse_out=None, out_token_
     seg = _segments(segments)
     par = _np(parents, np.uint32)
     d = cache.head_dim
-    _check(load_library().slha_b200_attend_tree(cache.address, seg.ctypes.data, len(seg), queries.address, _typed(par, _U32, "parents"), _same_type(cache, queries, out),
+    if queries.type not in cache.kind:
+        _fits(queries.type, cache.kind, "q")
+    _check(load_library().slha_b200_attend_tree(cache.address, seg.ctypes.data, len(seg), queries.address, _typed(par, _U32, "parents"), _typed(out, cache.kind, "out"),
                                                 queries.n_heads * d if out_token_stride is None else out_token_stride,
                                                 d if out_head_stride is None else out_head_stride, _typed(lse_out, _F32, "lse_out")))
     return out
@@ -628,7 +634,8 @@ def observe_cache(cache, segments, queries, lse, weights_out, weight_head_stride
     """The weight each row received: weights_out [kv_head][row] = decay * weights_in + the softmax weights of the tokens that see it (lse as attend_cache wrote
     it); see slha_b200_observe_cache."""
     seg = _segments(segments)
-    _same_type(cache, queries, None)
+    if queries.type not in cache.kind:
+        _fits(queries.type, cache.kind, "q")
     _check(load_library().slha_b200_observe_cache(cache.address, seg.ctypes.data, len(seg), queries.address, _typed(lse, _F32, "lse"), _typed(weights_in, _F32, "weights_in"), decay,
                                                   _typed(weights_out, _F32, "weights_out"), weight_head_stride))
     return weights_out

@@ -25,9 +25,13 @@ struct CacheSeg {
     uint32_t chunk_tiles;  // key tiles of an item
     uint32_t n_chunks;     // items of a block of query rows
     uint32_t seg;          // its number in the caller's table
-    uint32_t block_first, n_blocks;  // of a launch that takes some of the segment's blocks of query rows: the first, and how many
     uint32_t pad;
-    uint64_t to_begin;     // its first row's place where rows go to
+    union {
+        uint64_t to_begin;  // removal: its first row's place where rows go to
+        struct {
+            uint32_t block_first, n_blocks;  // attention: the first of the segment's blocks of query rows that a launch takes, and how many it does
+        };
+    };
 };
 struct CacheTable {
     CacheSeg s[CACHE_TABLE];

@@ -73,21 +73,33 @@ Status cache_positions_fit(const std::vector<SlhaB200Segment>& segs, const char*
     return Status();
 }
 
-// Whether two of the ranges (first, behind the last) share something.
-bool cache_overlap(std::vector<std::pair<uint64_t, uint64_t>> r) {
-    r.erase(std::remove_if(r.begin(), r.end(), [](const auto& x) { return x.first >= x.second; }), r.end());
-    if (!std::is_sorted(r.begin(), r.end())) std::sort(r.begin(), r.end());
-    for (size_t i = 1; i < r.size(); ++i)
+// Whether two of n ranges (first, behind the last) share something.
+template <typename F>
+bool cache_overlap(size_t n, F range) {
+    uint64_t end = 0;
+    size_t i = 0;
+    for (; i < n; ++i) {  // (most tables are in order)
+        const auto [from, to] = range(i);
+        if (from >= to) continue;
+        if (from < end) break;
+        end = to;
+    }
+    if (i == n) return false;
+    std::vector<std::pair<uint64_t, uint64_t>> r;
+    for (i = 0; i < n; ++i)
+        if (range(i).first < range(i).second) r.push_back(range(i));
+    std::sort(r.begin(), r.end());
+    for (i = 1; i < r.size(); ++i)
         if (r[i].first < r[i - 1].second) return true;
     return false;
 }
 // Rows that a call writes, or whose weights it does, belong to one segment each.  (Row counts in device memory are not known here: the caller's to see to.)
 Status cache_own_rows(const std::vector<SlhaB200Segment>& segs, const std::vector<SlhaB200Segment>& at, const uint32_t* rows, uint32_t most, const char* fn) {
-    if (rows && is_device_ptr(rows)) return Status();
-    std::vector<std::pair<uint64_t, uint64_t>> r;
-    for (size_t i = 0; i < segs.size(); ++i)
-        r.emplace_back(at[i].tile_begin, at[i].tile_begin + std::min({segs[i].n_tiles, rows ? rows[i] : segs[i].n_tiles, most}));
-    return cache_overlap(std::move(r)) ? Status(SLHA_ERR_DIMENSION, std::string(fn) + ": two segments have the same rows") : Status();
+    if (segs.size() < 2 || (rows && is_device_ptr(rows))) return Status();
+    const auto range = [&](size_t i) {
+        return std::pair<uint64_t, uint64_t>(at[i].tile_begin, at[i].tile_begin + std::min({segs[i].n_tiles, rows ? rows[i] : segs[i].n_tiles, most}));
+    };
+    return cache_overlap(segs.size(), range) ? Status(SLHA_ERR_DIMENSION, std::string(fn) + ": two segments have the same rows") : Status();
 }
 
 Status cache_check_queries(const SlhaB200KvCache* k, const SlhaB200CacheQueries* q, const char* fn) {
@@ -171,9 +183,8 @@ int32_t attend_cache_any(const char* fn, const SlhaB200KvCache* cache, const Slh
         cache_host_segments(segments, n_segments, &segs, &device_segs);
         const auto check_segments = [&]() -> Status {
             SLHA_TRY(cache_check_segments(cache, segs, queries, tree, fn));
-            std::vector<std::pair<uint64_t, uint64_t>> tokens;
-            for (const SlhaB200Segment& s : segs) tokens.emplace_back(s.query_begin, (uint64_t)s.query_begin + s.n_queries);
-            return cache_overlap(std::move(tokens)) ? Status(SLHA_ERR_DIMENSION, name("two segments have the same query tokens")) : Status();
+            const auto tokens = [&](size_t i) { return std::pair<uint64_t, uint64_t>(segs[i].query_begin, (uint64_t)segs[i].query_begin + segs[i].n_queries); };
+            return cache_overlap(segs.size(), tokens) ? Status(SLHA_ERR_DIMENSION, name("two segments have the same query tokens")) : Status();
         };
         if (!device_segs) SLHA_TRY(check_segments());
         CallScope cs;
