@@ -409,3 +409,55 @@ def test_scores_of_observed_rows_are_not_cut_off_step_by_step(tokens, d):
     off = w.download(F, n) / want[0] - 1.0
     print(off.mean(), off.std())
     assert abs(off.mean()) <= 20 * 1.5 * 2.5 * 2.0 ** -24
+
+
+# ---- shapes that fill no box
+@pytest.mark.parametrize("tokens,group,kv", [(3, 48, 1), (1, 128, 2), (5, 128, 1), (40, 12, 2), (70, 7, 1)])
+@pytest.mark.parametrize("d", [8, 40, 72, 120, 128])
+@pytest.mark.parametrize("more", [dict(), dict(softcap=7.0, window=333)])
+def test_wide_blocks_of_any_group_and_width(tokens, group, kv, d, more):
+    rng = np.random.default_rng(tokens * group + d)
+    call, raw = T.make(rng, (900, 77), tokens, kv, group, d, True, **more)
+    _, lse = T.check(call, raw, True)
+    assert S.debug_last_cache_kernels() == S.CACHE_ATTEND_WIDE
+    cache, segs, queries = T.on_device(call, raw, True)
+    w = S.to_device(np.zeros((kv, 977), F))
+    S.observe_cache(cache, segs, queries, S.to_device(lse), w, 977)
+    want, tol = call.received(lse, np.zeros((kv, 977), F), 1.0)
+    T.held(w.download(F, kv * 977).reshape(kv, 977), want, tol)
+
+
+def test_several_sequences_read_the_same_rows():
+    # a shared prompt: attention reads it for each; each sequence's tokens see what their own positions allow
+    rng = np.random.default_rng(9)
+    call, raw = T.make(rng, (600,), 3 * 50, 2, 4, 64, True)
+    call.segs = [(0, 600, 0, 50, 0), (0, 600, 50, 50, 0), (100, 400, 100, 50, 100)]
+    T.check(call, raw, True)
+
+
+def test_a_graph_of_a_step_with_large_parts_beside_eager_ones():
+    # the graph's working memory is its own: replays on one stream while the thread's next calls run on another
+    torch = pytest.importorskip("torch")
+    rng = np.random.default_rng(10)
+    call, raw = T.make(rng, (9000,), 64, 2, 4, 128, True)
+    handles = T.on_device(call, raw, True)
+    want = call.attend(True)
+    a, b = (torch.cuda.Stream() for _ in range(2))
+    outs = [torch.empty(call.q.shape, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    S.synchronize()
+    torch.cuda.synchronize()
+    try:
+        S.set_stream(a.cuda_stream)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=a):
+            S.attend_cache(*handles, outs[0])
+        S.set_stream(b.cuda_stream)
+        for _ in range(10):
+            with torch.cuda.stream(a):
+                g.replay()
+            S.attend_cache(*handles, outs[1])
+        torch.cuda.synchronize()
+    finally:
+        S.set_stream(None)
+    for o in outs:
+        T.held(o.float().cpu().numpy(), want[0], want[2])
