@@ -411,7 +411,9 @@ int32_t slha_b200_attend_topk(const uint32_t* top_index, const float* top_score,
  * (SLHA_ERR_DIMENSION otherwise).  Rows, positions, documents, queries, outputs,
  * lse and weights are device memory of the calling thread's device; the other
  * arrays, and the segments, host or device.  Host ones are copied before a call
- * returns, and may then be written again.
+ * returns, and may then be written again.  Arrays of words begin on a multiple of 4
+ * bytes.  (float32 rows are taken as two numbers of 11 bits: sizes from 3.4e38 on, and
+ * infinities, that a token sees may come out as NaN.)
  * A call can be captured into a CUDA graph where its segments (at most 64) are host
  * memory and its other arrays device memory; working memory then belongs to the
  * graph.

@@ -43,6 +43,12 @@ Status cache_device_segments(Ctx* c, const SlhaB200Segment* segments, std::vecto
     return Status();
 }
 bool cache_aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+// Arrays of single words begin on a word: the GPU faults on others.
+Status cache_words(const char* fn, std::initializer_list<const void*> arrays) {
+    for (const void* p : arrays)
+        if (reinterpret_cast<uintptr_t>(p) % 4) return Status(SLHA_ERR_DIMENSION, std::string(fn) + ": positions, documents, counts, slopes, lse and weights must begin on a multiple of 4 bytes");
+    return Status();
+}
 
 Status cache_check(const SlhaB200KvCache* k, const char* fn, bool with_values) {
     const auto name = [&](const char* what) { return std::string(fn) + ": " + what; };
@@ -55,7 +61,7 @@ Status cache_check(const SlhaB200KvCache* k, const char* fn, bool with_values) {
     if (k->key_row_stride % each || k->key_head_stride % each || (with_values && (k->value_row_stride % each || k->value_head_stride % each)))
         return Status(SLHA_ERR_DIMENSION, name("row and head strides must be multiples of 16 bytes"));
     if (!cache_aligned(k->keys) || (with_values && !cache_aligned(k->values))) return Status(SLHA_ERR_DIMENSION, name("keys and values must begin on a multiple of 16 bytes"));
-    return Status();
+    return cache_words(fn, {k->positions, k->documents, k->rows});
 }
 Status cache_memory(Ctx* c, const SlhaB200KvCache* k, const char* fn, bool with_values) {
     const auto name = [&](const char* what) { return std::string(fn) + ": " + what; };
@@ -118,7 +124,7 @@ Status cache_check_queries(const SlhaB200KvCache* k, const SlhaB200CacheQueries*
         return Status(SLHA_ERR_NONFINITE, name("softcap must be at most 2^100, and scale / softcap a normal float32"));
     if (k->positions && !q->positions) return Status(SLHA_ERR_NULL, name("the cache's rows have positions, the queries have none"));
     if ((k->documents != nullptr) != (q->documents != nullptr)) return Status(SLHA_ERR_NULL, name("documents must be given for rows and queries, or for neither"));
-    return Status();
+    return cache_words(fn, {q->slopes, q->prefix, q->positions, q->documents});
 }
 Status cache_check_segments(const SlhaB200KvCache* k, const std::vector<SlhaB200Segment>& segs, const SlhaB200CacheQueries* q, bool tree, const char* fn) {
     const auto name = [&](const char* what) { return std::string(fn) + ": " + what; };
@@ -175,6 +181,7 @@ int32_t attend_cache_any(const char* fn, const SlhaB200KvCache* cache, const Slh
         if (!out || (tree && !parents)) return Status(SLHA_ERR_NULL, std::string(fn) + " received a NULL pointer");
         SLHA_TRY(cache_check(cache, fn, true));
         SLHA_TRY(cache_check_queries(cache, queries, fn));
+        SLHA_TRY(cache_words(fn, {parents, lse_out}));
         const size_t each = 16 / key_elem_bytes(cache->dtype);
         if (out_token_stride % each || out_head_stride % each || !cache_aligned(out))
             return Status(SLHA_ERR_DIMENSION, name("out must begin on a multiple of 16 bytes and its strides be multiples of 16 bytes"));
@@ -243,6 +250,7 @@ int32_t slha_b200_observe_cache(const SlhaB200KvCache* cache, const SlhaB200Segm
         if (!std::isfinite(decay)) return Status(SLHA_ERR_NONFINITE, name("decay is not finite"));
         SLHA_TRY(cache_check(cache, fn, false));
         SLHA_TRY(cache_check_queries(cache, queries, fn));
+        SLHA_TRY(cache_words(fn, {lse, weights_in, weights_out}));
         std::vector<SlhaB200Segment> segs;
         bool device_segs;
         cache_host_segments(segments, n_segments, &segs, &device_segs);
@@ -307,6 +315,7 @@ int32_t slha_b200_evict_cache(const SlhaB200KvCache* cache, const SlhaB200Segmen
             return Status(SLHA_ERR_DIMENSION, name("each KV head keeps other rows: rows must be its own where they go (head strides > 0)"));
         SLHA_TRY(cache_check(cache, fn, true));
         if (!in_place) SLHA_TRY(cache_check(to, fn, true));
+        SLHA_TRY(cache_words(fn, {ev->weights, ev->weights_to, ev->source_out, ev->rows_out}));
         std::vector<SlhaB200Segment> segs, to_segs;
         bool device_segs, device_to = false;
         cache_host_segments(segments, n_segments, &segs, &device_segs);

@@ -110,3 +110,26 @@ def test_tensors_are_what_a_call_reads_them_as():
         with pytest.raises(TypeError, match=what):
             call()
     passes(S.attend_cache, k, seg, q, torch.zeros(4, 4, d, dtype=torch.bfloat16), torch.zeros(4, 4))
+
+
+# ---- arrays that begin within a word
+def test_arrays_of_words_begin_on_one():
+    bad, word = A + 2, "multiple of 4"
+    seg, one = SEG, S.make_segments([(0, 100, 0, 0, 0)])
+    for more in (dict(positions=bad), dict(documents=bad), dict(rows=type("Raw", (), {"data_ptr": lambda self: bad})())):
+        k = cache(**more)
+        q = queries(positions=type("Raw", (), {"data_ptr": lambda self: A})(), documents=type("Raw", (), {"data_ptr": lambda self: A})() if "documents" in more else None)
+        refused(S.ERR_DIMENSION, word, S.attend_cache, k, seg, q, A)
+        refused(S.ERR_DIMENSION, word, S.observe_cache, k, seg, q, A, A, 100)
+        refused(S.ERR_DIMENSION, word, S.evict_cache, cache(entry_head_stride=100, **more), one, A, 100, 50)
+    raw = type("Raw", (), {"data_ptr": lambda self: bad})()
+    for more in (dict(slopes=raw), dict(prefix=raw), dict(positions=raw)):
+        refused(S.ERR_DIMENSION, word, S.attend_cache, cache(), seg, queries(**more), A)
+    refused(S.ERR_DIMENSION, word, S.attend_cache, cache(), seg, queries(), A, bad)
+    refused(S.ERR_DIMENSION, word, S.attend_tree, cache(), seg, queries(), raw, A)
+    for args in ((bad, A), (A, bad)):
+        refused(S.ERR_DIMENSION, word, S.observe_cache, cache(), seg, queries(), *args, 100)
+    refused(S.ERR_DIMENSION, word, S.observe_cache, cache(), seg, queries(), A, A, 100, weights_in=bad)
+    refused(S.ERR_DIMENSION, word, S.evict_cache, cache(), one, bad, 100, 50)
+    for more in (dict(source_out=bad), dict(rows_out=bad)):
+        refused(S.ERR_DIMENSION, word, S.evict_cache, cache(), one, A, 100, 50, **more)
