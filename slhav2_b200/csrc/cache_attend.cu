@@ -5,12 +5,12 @@
 // in one pass over the rows: a running maximum m and sum l a query row, out's sums scaled by exp(m_old - m_new) when the maximum grows.  Scores are held in
 // units of log 2 (exp is one instruction there).
 //
-// One token's work is bound by the bytes of its rows: 131072 rows of 8 KV heads of 128 dimensions (537 MB), scores capped, 92 to 100 us = 5.4 to 5.8 TB/s; 48 sequences of 6000
-// on the average with positions and a distance bias 220 to 229 us (1.2 GB, 5.3 to 5.5 TB/s); 512 rows 6.5 us: a launch and the chain of one tile's loads, products, softmax and the join.  float32 rows are bound by the products (three of tf32 for one): 5 x 37 tokens of 12 heads of 96 dimensions over 1500 rows each 54 us.
+// One token's work is bound by the bytes of its rows: 131072 rows of 8 KV heads of 128 dimensions (537 MB), 91 to 101 us = 5.3 to 5.9 TB/s with scores capped, 84 without; 48 sequences of 6000
+// on the average with positions and a distance bias 227 to 232 us (1.2 GB, 5.2 to 5.3 TB/s); 512 rows 6.5 us: a launch and the chain of one tile's loads, products, softmax and the join.  float32 rows are bound by the products (three of tf32 for one): 5 x 37 tokens of 12 heads of 96 dimensions over 1500 rows each 54 us.
 //
 // A CTA takes a block of 16, 32 or 64 query rows of one KV head (row = token x the head's group of query heads, so that the keys are read once for the group) and
 // a run of the segment's rows in tiles of 64 (float32: 32).  Four warps: with 16 query rows each takes a quarter of a tile's keys, with 64 each takes
-// its own 16 rows.  Tiles arrive by cp.async, two or three ahead.
+// its own 16 rows.  Tiles arrive by cp.async, one to three ahead (STAGES - 1, by what fits).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
@@ -582,7 +582,7 @@ Status launch_cache_join(Ctx* c, CacheArgs a, int dtype, const CacheWork& w, uin
     CacheTable tab;
     SLHA_TRY(cache_table(c, split, &tab, &a.table));
     a.n_segs = (uint32_t)split.size();
-    // four warps a row where it has many parts (131072 rows in 35 parts: 90 us in all with one warp, 84 with four; 64 x 4096 rows in 2 parts 177 with one, 180 with four)
+    // four warps a row where it has many parts (131072 rows in 35 parts, scores not capped: 90 us in all with one warp, 84 with four; 64 x 4096 rows in 2 parts 177 with one, 180 with four)
     const uint32_t warps = w.chunks > 8 ? 4 : 1, at_once = JOIN_THREADS / 32 / warps, per = (rows + at_once - 1) / at_once;
     if (w.blocks * a.n_kv * per > 0x7FFFFFFFull) return Status(SLHA_ERR_CAPACITY, "attention over a cache: too many blocks of query rows");
     const dim3 grid((uint32_t)(w.blocks * a.n_kv * per));

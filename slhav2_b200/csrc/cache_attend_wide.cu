@@ -7,7 +7,7 @@
 // ends by cp.async, which reads nothing beyond the end and leaves zeros there.
 //
 // Bound by the softmax beside the products (a row a thread, 128 columns: one exponential, two multiply-adds and half a conversion a score, TMEM loads and stores): 8192 tokens x 32
-// heads x 8192 rows, nothing masked, 860 us = 1280 TFLOP/s, 78 % of what a library's matrix product reaches; causal 470 us (1170, of the half that is seen; tiles on the diagonal are
+// heads x 8192 rows, nothing masked, 846 us = 1300 TFLOP/s, 79 % of what a library's matrix product reaches; causal 456 us (1206, of the half that is seen; up to 510 where the power limit lowers the clock; tiles on the diagonal are
 // worked in full); 4096 x 4096 under a cap 370 us, where the hyperbolic tangent's polynomial is eight more multiply-adds a score; with the rows' own kernel of 64 (cache_attend.cu) the
 // prompts below took 3.6 to 3.9 times as long.  Two tiles of query rows a CTA, because one tile's softmax then hides behind the other's products, and because 256 rows of sums
 // fill half of TMEM and the two tiles' scores the other.
@@ -637,7 +637,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
                 const bool all = s_list[li] >> t & 1;
                 // Where a tile is seen as a whole and the warp's rows all have it on one side, the bias is near + step column, added on the way to the weights; its largest score is then only
                 // bounded, by the largest product and the largest bias, which may be 2^64 too high and still leaves weights from 2^-62 of the row's largest on.
-                // (8192 causal tokens, 32 heads: 961 us with all tiles bent, 534 so.)
+                // (8192 causal tokens, 32 heads: 900 us with all tiles bent, 587 so.)
                 bool straight = false;
                 float step = 0.0f, near = 0.0f;
                 if constexpr (has_slope && !CAP) {

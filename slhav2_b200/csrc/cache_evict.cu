@@ -5,7 +5,7 @@
 // second moves rows.  A kept row below the budget stays where it is, so in place only rows from beyond the budget move, into places that no row is read from.
 //
 // Bound by latency where caches are short (1100 rows, 1024 stay: 13.5 us, two launches and three passes over a few words) and by bytes where rows move: 8 prompts of up to 32768 rows
-// into caches of 4096, tiles with them, 94 us, of which the selection is 39 (its words are read once, into shared memory; the passes over them are bound by shared atomics and barriers)
+// into caches of 4096, tiles with them, 93 us, of which the selection is 39 (its words are read once, into shared memory; its warps wait most at the barriers between the passes)
 // and the moving 55 (6.2 TB/s).
 #include <cooperative_groups.h>
 

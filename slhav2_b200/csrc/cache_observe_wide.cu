@@ -4,7 +4,7 @@
 // columns: no sum crosses threads (with many query rows four threads share a key).  A CTA takes the queries of one KV head, which stay in shared memory, and a run of key tiles,
 // each of which is read once (TMA, the tile behind which a segment ends by cp.async).  While one block of scores is summed, the next is multiplied.
 // With few query rows bound by the rows' bytes (16 sequences of 5750 rows on the average after a decode step: 39 us, 5.0 TB/s), with many by one exponential a score and what surrounds it (256 query
-// rows of 8 KV heads over 32768 rows: 39 us, 1.7e12 scores a second; the special-function units alone would take 15 us).
+// rows of 8 KV heads over 32768 rows: 41 us, 1.6e12 scores a second; the special-function units alone would take 15 us).
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -24,7 +24,7 @@ constexpr int KT = 128;
 // all SMs would be uneven; MANY takes more than 32 where that share is 4 or less.  Measured, 8 KV heads of 128 dimensions, us:
 //   4 query rows, sequences: 64 x 1024 rows (runs of 8) FEW 31, MID 39, MANY 49; 1 x 8192 (4) 5.6, 6.0, 7.4; 8 x 8192 (28) 27, 25, 36; 16 of 2700 to 8192 35, 38
 //   32 query rows: 64 x 1024 41, 47, 57; 32 x 4096 62, 54, 79; 8 x 8192 38, 27, 40
-//   64 query rows: 1 x 4096 (2) MID 9.0, MANY 7.1; 1 x 16384 (7) 13.9, 14.9; 1 x 32768 (14) 16, 22; 256 query rows on 1 x 32768 40, 43
+//   64 query rows: 1 x 4096 (2) MID 9.0, MANY 7.1; 1 x 16384 (7) 13.9, 14.9; 1 x 32768 (14) 16, 22; 256 query rows on 1 x 32768 41, 43
 // and cache_observe.cu's kernel takes 40, 56 (4, 32 query rows on 8 x 8192), 39, 119 (64, 256 on 32768): it takes rows beyond 512 query rows, 128 dimensions, and float32.
 enum { FEW = 0, MID = 1, MANY = 2 };
 template <int D, int MODE>
