@@ -986,6 +986,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attend_wide_kernel(const __g
     __syncthreads();  // (the rows' warps have given their registers back: none of the others takes them while one still has to get them)
     tc_after();
     if (warp >= 8) regs_more<REGS_ALL>();
+    if (warp == MMA_WARP && s_fail[0] && cnt) bar_wait(bar(O_FULL), 0);  // (no product is under way when TMEM is given back, whoever gave up before)
     if (warp == MMA_WARP) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512u) : "memory");
     if (s_fail[0] | s_fail[1]) {
         asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");  // (rows that left as boxes lie there before they are written again)

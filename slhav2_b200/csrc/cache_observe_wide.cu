@@ -39,7 +39,7 @@ struct Obs {
     static constexpr int CTAS = MODE == FEW ? 2 : 1;
     static_assert(CTAS * (SMEM + 1024) <= 228 * 1024, "shared memory of an SM");
 };
-enum { K_FULL = 0, K_FREE = 5, S_FULL = 10, S_FREE = 14, Q_FULL = 18, TMEM_WORD = 19 };
+enum { K_FULL = 0, K_FREE = 5, S_FULL = 10, S_FREE = 14, Q_FULL = 18, TMEM_WORD = 19, DONE = 20 };
 
 // At the end of a block: no copy is under way, whoever gave up before.
 __device__ __noinline__ void settle(uint32_t keys, uint32_t fills, uint32_t stages, uint32_t queries, uint32_t boxes) {
@@ -94,6 +94,7 @@ __global__ void __launch_bounds__(Obs<D, MODE>::THREADS, Obs<D, MODE>::CTAS)
             for (int i = 0; i < S::STAGES; ++i) bar_init(bar(K_FULL + i), 1), bar_init(bar(K_FREE + i), 1);
             for (int i = 0; i < S::PLACES; ++i) bar_init(bar(S_FULL + i), 1), bar_init(bar(S_FREE + i), S::SUMMERS / S::GROUPS);
             bar_init(bar(Q_FULL), 1);
+            bar_init(bar(DONE), 1);
             asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             if (maps.q_boxes && q_rows) {
@@ -304,6 +305,8 @@ __global__ void __launch_bounds__(Obs<D, MODE>::THREADS, Obs<D, MODE>::CTAS)
                     ++step;
                 }
             }
+            tc_commit_to(bar(DONE));
+            bar_wait(bar(DONE), 0);  // (no product is under way when TMEM is given back, whoever gave up before)
         }
         __syncwarp();
     } else {
