@@ -312,6 +312,8 @@ def test_rows_of_more_than_one_run_keep_to_their_working_memory():
     cache = S.KvCache(k, v, kv, d)
     outs, lses = [], []
     grown = []
+    torch.cuda.synchronize()
+    S.attend_cache(cache, S.make_segments([(0, n, 0, 64, 0)]), S.CacheQueries(q, tokens, kv * group, d), torch.empty_like(q), torch.empty(tokens, kv * group, device="cuda"))  # (loads the kernels)
 
     def work():
         for prefix in (None, torch.zeros(1, dtype=torch.int32, device="cuda")):  # (a prefix of nothing: the same rows are seen, but the runs are made for all)
