@@ -122,6 +122,17 @@ struct ThreadState {
     Answer answer[16];
     OutPage outs[16];
     bool plans_used[16] = {false};            // by the call under way
+    // At the thread's end its working memory is given back, behind the work that still uses it; what a graph names stays.  (Relaxed: another thread may be capturing.)
+    ~ThreadState() {
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        for (int dev = 0; dev < 16; ++dev) {
+            if (blocks[dev].empty() || cudaSetDevice(dev) != cudaSuccess || cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) continue;
+            if (arena[dev].queued) cudaEventSynchronize(arena[dev].done);
+            for (Block& b : blocks[dev])
+                if (!b.named) cudaFree(b.p);
+            cudaThreadExchangeStreamCaptureMode(&mode);
+        }
+    }
 };
 thread_local ThreadState tls;
 }  // namespace

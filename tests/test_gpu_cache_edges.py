@@ -333,6 +333,26 @@ def test_rows_of_more_than_one_run_keep_to_their_working_memory():
 
 
 
+def test_working_memory_is_given_back_when_its_thread_ends():
+    torch = pytest.importorskip("torch")
+    rng = np.random.default_rng(7)
+    large = chunk_with_large_parts(rng)  # (some 14 MB beside the first 8)
+    stream = torch.cuda.Stream()
+
+    def work():
+        S.set_stream(stream.cuda_stream)
+        for _ in range(3):
+            large()
+
+    in_a_thread(work)
+    torch.cuda.synchronize()
+    before = torch.cuda.mem_get_info()[0]
+    for _ in range(8):
+        in_a_thread(work)
+    torch.cuda.synchronize()
+    assert before - torch.cuda.mem_get_info()[0] <= 32 << 20
+
+
 # ---- kernels that only long caches reach
 @pytest.mark.parametrize("tokens,group,d,lens,name", [(16, 4, 128, (10000,), "MID"), (40, 4, 128, (10000,), "MID"), (64, 4, 128, (9990,), "MID"), (100, 4, 128, (10000,), "MANY"),
                                                       (64, 8, 80, (9000, 700), "MANY"), (1, 4, 128, (20000, 77), "MID"), (8, 4, 128, (19990, 130), "MID"), (16, 4, 80, (10000,), "MID"),
