@@ -528,6 +528,129 @@ typedef struct {
 int32_t slha_b200_evict_cache(const SlhaB200KvCache* cache, const SlhaB200Segment* segments, size_t n_segments,
                               const SlhaB200CacheEviction* eviction);
 
+/*
+ * What a layer's heads go through on their way into a cache: each query and key head's
+ * norm, y = x * (mean(x^2) + eps)^(-1/2) * weight, and the rotation by its token's
+ * position, in one pass.  Pair p of the first rotary_dim elements of a head, (i, i +
+ * rotary_dim / 2) for i = p or, interleaved, (2 p, 2 p + 1), turns by the angle
+ *   positions[axes[p]][token] * frequencies[p]:
+ *   (a, b) -> magnitude * (a cos - b sin, a sin + b cos);
+ * the other elements stay.  Angles are reduced in 64 bits (to 1e-6 at positions of 2^32),
+ * the rest is float32, rounded once.  With several axes (time, height, width) each pair
+ * goes by the axis that `axes` names.  Values are copied as they are.
+ */
+typedef struct {
+    const void* q;               /* element (token, head, i) at token * q_token_stride + head * q_head_stride + i; NULL: none */
+    const void* k;               /* likewise, n_kv_heads; NULL: none */
+    const void* v;
+    int32_t dtype;               /* SLHA_B200_F32 or SLHA_B200_BF16, of what is read and written */
+    uint32_t head_dim;           /* a multiple of 8, at most 256 */
+    uint32_t n_heads;
+    uint32_t n_kv_heads;
+    uint32_t n_tokens;
+    uint64_t q_token_stride;     /* strides in elements, multiples of 16 bytes */
+    uint64_t q_head_stride;
+    uint64_t k_token_stride;
+    uint64_t k_head_stride;
+    uint64_t v_token_stride;
+    uint64_t v_head_stride;
+    int32_t norm;                /* 0: no norms */
+    float eps;
+    const float* q_weight;       /* head_dim; NULL: 1 */
+    const float* k_weight;
+} SlhaB200HeadRows;
+
+typedef struct {
+    const float* frequencies;    /* rotary_dim / 2 */
+    const uint8_t* axes;         /* rotary_dim / 2, each below n_axes (host arrays are checked, in device memory larger ones count as the last); NULL: the first */
+    const uint32_t* positions;   /* [n_axes][n_tokens] */
+    uint32_t n_axes;
+    uint32_t rotary_dim;         /* a multiple of 8, at most head_dim */
+    int32_t interleaved;
+    float magnitude;
+} SlhaB200Rotation;
+
+/* Queries to q_out (element (token, head, i) at token * q_out_token_stride + head *
+ * q_out_head_stride + i), keys and values into the rows of `to`: a segment's tokens are its
+ * last n_queries rows, as for slha_b200_attend_cache, and its query_begin .. query_begin +
+ * n_queries of the heads' tokens.  Without segments token t goes to row t.  rotation NULL:
+ * norms only.  `to` is needed where there are keys or values; tokens of no segment are left
+ * as they are, rows of two segments are refused (with row counts in device memory they are
+ * the caller's to avoid), and where a segment has fewer rows than tokens the tokens behind
+ * its last row write no keys and values.  to->positions and documents are not written.
+ * q_out may be q, with the same strides, and without segments to->keys may be k and
+ * to->values v; other arrays that are written overlap none that is read.  Weights,
+ * frequencies, axes and positions are host or device memory, heads, q_out and rows device
+ * memory; captured into a graph as slha_b200_attend_cache. */
+int32_t slha_b200_rotate_heads(const SlhaB200HeadRows* heads, const SlhaB200Rotation* rotation,
+                               const SlhaB200Segment* segments, size_t n_segments, void* q_out,
+                               uint64_t q_out_token_stride, uint64_t q_out_head_stride,
+                               const SlhaB200KvCache* to);
+
+/*
+ * A cache of rows held in 4 bits: 9/16 of a byte an element instead of 2 or 4.  Each block of
+ * 16 elements of a row of a KV head has a scale of 8 bits (float8 e4m3, without a sign), each
+ * element 4 bits (e2m1: a sign and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6); its value is element *
+ * scale * 2^exponent, exact in bfloat16.  The exponents place the scales' range (2^-9 to
+ * 448; full precision from 2^-6) where the cache's values lie: sizes up to 2688 * 2^exponent
+ * are held, blocks whose largest is below 2^(exponent - 8) or so come out coarse or as zero.
+ * Code arrays and their strides are multiples of 16 bytes, scale arrays and theirs of 4 bytes
+ * for head_dim up to 64, 8 up to 128, 16 beyond (SLHA_ERR_DIMENSION otherwise).  All device
+ * memory, and what else is said of SlhaB200KvCache.
+ */
+typedef struct {
+    const void* key_codes;       /* elements i and i + 1 (i even) of (row, KV head) in the low and high half of byte row * code_row_stride + head * code_head_stride + i / 2 */
+    const void* value_codes;
+    const void* key_scales;      /* of elements i .. i + 15: byte row * scale_row_stride + head * scale_head_stride + i / 16 */
+    const void* value_scales;
+    int32_t dtype;               /* SLHA_B200_F32 or SLHA_B200_BF16: of queries and outputs */
+    uint32_t head_dim;           /* a multiple of 16, at most 256 */
+    uint32_t n_kv_heads;
+    uint64_t code_row_stride;    /* strides in bytes */
+    uint64_t code_head_stride;
+    uint64_t scale_row_stride;
+    uint64_t scale_head_stride;
+    int32_t key_exponent;        /* -64 .. 64 */
+    int32_t value_exponent;
+    const uint32_t* positions;   /* this and the rest as in SlhaB200KvCache */
+    const uint32_t* documents;
+    uint64_t entry_head_stride;
+    const uint32_t* rows;
+} SlhaB200KvCache4;
+
+/* Rows of a segment's tokens (its last n_queries rows) from row query_begin .. query_begin +
+ * n_queries of `from`, whose keys and values are float32 or bfloat16 and whose other arrays
+ * are not read.  A block's scale is its largest size / (6 * 2^exponent), rounded to the
+ * nearest of its 8 bits (ties to even, at most 448); an element is x / (scale *
+ * 2^exponent), rounded to the nearest of its 4 bits (ties to even, at most 6), both as if
+ * computed without an error before.  A block that holds a NaN comes out as NaN, infinities
+ * as the largest size.  Where a segment has fewer rows than tokens the tokens behind its
+ * last row are not written.  Rows of two segments are refused (with row counts in device
+ * memory they are the caller's to avoid). */
+int32_t slha_b200_write_cache4(const SlhaB200KvCache4* cache, const SlhaB200Segment* segments, size_t n_segments,
+                               const SlhaB200KvCache* from, uint32_t n_tokens);
+
+/* Every row of the segments back: segment i's go to rows to_segments[i].tile_begin .. of `to`
+ * (its n_tiles at least the segment's), or, with to_segments NULL, to the rows of the same
+ * number.  `to` says where keys and values go, in float32 or bfloat16 (either may be NULL);
+ * its other arrays are not used.  Two segments' rows may not go to one place. */
+int32_t slha_b200_read_cache4(const SlhaB200KvCache4* cache, const SlhaB200Segment* segments, size_t n_segments,
+                              const SlhaB200KvCache* to, const SlhaB200Segment* to_segments);
+
+/* slha_b200_attend_cache and slha_b200_attend_tree over rows held in 4 bits: the same
+ * segments, queries, masks and outputs.  Products are exact, sums and softmax float32.  Up to
+ * 64 query rows (tokens times query heads of a KV head) are multiplied with what the codes stand for
+ * as they are read, queries and weights as float16 numbers (float32: two) scaled by powers of two; for more,
+ * a segment's rows are first laid out as rows of the queries' type in working memory of the
+ * thread (512 MB at most, or what one segment takes).  scale * 2^key_exponent keeps to what
+ * is said of scale.  (Queries that hold an infinity may come out as NaN.) */
+int32_t slha_b200_attend_cache4(const SlhaB200KvCache4* cache, const SlhaB200Segment* segments, size_t n_segments,
+                                const SlhaB200CacheQueries* queries, void* out, uint64_t out_token_stride,
+                                uint64_t out_head_stride, float* lse_out);
+int32_t slha_b200_attend_tree4(const SlhaB200KvCache4* cache, const SlhaB200Segment* segments, size_t n_segments,
+                               const SlhaB200CacheQueries* queries, const uint32_t* parents, void* out,
+                               uint64_t out_token_stride, uint64_t out_head_stride, float* lse_out);
+
 /* Checking aid: which kernels the calling thread's latest call on a cache of rows
  * launched, a bit each; 0 when there was no such call or it launched none. */
 #define SLHA_B200_CACHE_ATTEND 1        /* up to 64 query rows a block */
@@ -537,6 +660,8 @@ int32_t slha_b200_evict_cache(const SlhaB200KvCache* cache, const SlhaB200Segmen
 #define SLHA_B200_CACHE_OBSERVE_MID 16  /* up to 256 */
 #define SLHA_B200_CACHE_OBSERVE_MANY 32 /* and up to 512 */
 #define SLHA_B200_CACHE_SELECT(ctas) (64 * (ctas)) /* removal by clusters of 1, 2, 4 or 8 CTAs */
+#define SLHA_B200_CACHE_ATTEND4 1024    /* rows of 4 bits, multiplied as they are read */
+#define SLHA_B200_CACHE_LAID_OUT 2048   /* rows of 4 bits, laid out before */
 int32_t slha_b200_debug_last_cache_kernels(uint32_t* out);
 
 /*

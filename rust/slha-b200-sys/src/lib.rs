@@ -149,6 +149,66 @@ pub struct SlhaB200CacheQueries {
     pub documents: *const u32,
 }
 
+/// A layer's query, key and value heads on their way into a cache.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct SlhaB200HeadRows {
+    pub q: *const c_void,
+    pub k: *const c_void,
+    pub v: *const c_void,
+    pub dtype: i32,
+    pub head_dim: u32,
+    pub n_heads: u32,
+    pub n_kv_heads: u32,
+    pub n_tokens: u32,
+    pub q_token_stride: u64,
+    pub q_head_stride: u64,
+    pub k_token_stride: u64,
+    pub k_head_stride: u64,
+    pub v_token_stride: u64,
+    pub v_head_stride: u64,
+    pub norm: i32,
+    pub eps: f32,
+    pub q_weight: *const f32,
+    pub k_weight: *const f32,
+}
+
+/// The rotation of heads by their tokens' positions.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct SlhaB200Rotation {
+    pub frequencies: *const f32,
+    pub axes: *const u8,
+    pub positions: *const u32,
+    pub n_axes: u32,
+    pub rotary_dim: u32,
+    pub interleaved: i32,
+    pub magnitude: f32,
+}
+
+/// A cache of key and value rows held in 4 bits; strides in bytes.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct SlhaB200KvCache4 {
+    pub key_codes: *const c_void,
+    pub value_codes: *const c_void,
+    pub key_scales: *const c_void,
+    pub value_scales: *const c_void,
+    pub dtype: i32,
+    pub head_dim: u32,
+    pub n_kv_heads: u32,
+    pub code_row_stride: u64,
+    pub code_head_stride: u64,
+    pub scale_row_stride: u64,
+    pub scale_head_stride: u64,
+    pub key_exponent: i32,
+    pub value_exponent: i32,
+    pub positions: *const u32,
+    pub documents: *const u32,
+    pub entry_head_stride: u64,
+    pub rows: *const u32,
+}
+
 /// Removal of the rows that received the least weight.
 #[repr(C)]
 #[derive(Clone, Copy, Debug)]
@@ -228,6 +288,19 @@ extern "C" {
         weights_out: *mut f32, weight_head_stride: u64) -> i32;
     pub fn slha_b200_evict_cache(cache: *const SlhaB200KvCache, segments: *const SlhaB200Segment, n_segments: usize,
         eviction: *const SlhaB200CacheEviction) -> i32;
+    pub fn slha_b200_rotate_heads(heads: *const SlhaB200HeadRows, rotation: *const SlhaB200Rotation,
+        segments: *const SlhaB200Segment, n_segments: usize, q_out: *mut c_void, q_out_token_stride: u64,
+        q_out_head_stride: u64, to: *const SlhaB200KvCache) -> i32;
+    pub fn slha_b200_write_cache4(cache: *const SlhaB200KvCache4, segments: *const SlhaB200Segment, n_segments: usize,
+        from: *const SlhaB200KvCache, n_tokens: u32) -> i32;
+    pub fn slha_b200_read_cache4(cache: *const SlhaB200KvCache4, segments: *const SlhaB200Segment, n_segments: usize,
+        to: *const SlhaB200KvCache, to_segments: *const SlhaB200Segment) -> i32;
+    pub fn slha_b200_attend_cache4(cache: *const SlhaB200KvCache4, segments: *const SlhaB200Segment, n_segments: usize,
+        queries: *const SlhaB200CacheQueries, out: *mut c_void, out_token_stride: u64, out_head_stride: u64,
+        lse_out: *mut f32) -> i32;
+    pub fn slha_b200_attend_tree4(cache: *const SlhaB200KvCache4, segments: *const SlhaB200Segment, n_segments: usize,
+        queries: *const SlhaB200CacheQueries, parents: *const u32, out: *mut c_void, out_token_stride: u64,
+        out_head_stride: u64, lse_out: *mut f32) -> i32;
     pub fn slha_b200_debug_last_cache_kernels(out: *mut u32) -> i32;
     pub fn slha_b200_shard_unique_id(id_out: *mut c_void) -> i32;
     pub fn slha_b200_shard_init(nccl_unique_id: *const c_void, rank: i32, world: i32, out: *mut *mut SlhaB200Shard) -> i32;

@@ -99,6 +99,11 @@ SIGNATURES = {
     "slha_b200_attend_tree": (_i32, [_vp, _vp, _sz, _vp, _vp, _vp, _u64, _u64, _vp]),
     "slha_b200_observe_cache": (_i32, [_vp, _vp, _sz, _vp, _vp, _vp, C.c_float, _vp, _u64]),
     "slha_b200_evict_cache": (_i32, [_vp, _vp, _sz, _vp]),
+    "slha_b200_rotate_heads": (_i32, [_vp, _vp, _vp, _sz, _vp, _u64, _u64, _vp]),
+    "slha_b200_write_cache4": (_i32, [_vp, _vp, _sz, _vp, _u32]),
+    "slha_b200_read_cache4": (_i32, [_vp, _vp, _sz, _vp, _vp]),
+    "slha_b200_attend_cache4": (_i32, [_vp, _vp, _sz, _vp, _vp, _u64, _u64, _vp]),
+    "slha_b200_attend_tree4": (_i32, [_vp, _vp, _sz, _vp, _vp, _vp, _u64, _u64, _vp]),
     "slha_b200_debug_last_cache_kernels": (_i32, [_vp]),
     "slha_b200_shard_unique_id": (_i32, [_vp]),
     "slha_b200_shard_init": (_i32, [_vp, _i32, _i32, C.POINTER(_vp)]),
@@ -501,6 +506,7 @@ def attend_topk(top_index, top_score, k, scale, values, d_v, value_dtype=F32, to
 # Element types that a call reads: their names, and the types that have been found to bear them (None: addresses and raw buffers bring no type).
 _ROWS = {F32: {None, "float32"}, BF16: {None, "bfloat16", "uint16", "int16"}}
 _U32, _F32 = {None, "uint32", "int32"}, {None, "float32"}
+_U8, _CODES, _SCALES = {None, "uint8"}, {None, "uint8", "float4_e2m1fn_x2"}, {None, "uint8", "float8_e4m3fn"}
 
 
 class _Any:
@@ -652,8 +658,150 @@ def evict_cache(cache, segments, weights, weight_head_stride, budget, sink_windo
     _check(load_library().slha_b200_evict_cache(cache.address, seg.ctypes.data, len(seg), C.addressof(e)))
 
 
+def _given(a, dtype):
+    """An array of a call: None and addresses as they are."""
+    return a if a is None or isinstance(a, int) else _np(a, dtype)
+
+
+class _HeadRows(C.Structure):
+    _fields_ = [
+        ("q", _vp), ("k", _vp), ("v", _vp), ("dtype", _i32), ("head_dim", _u32), ("n_heads", _u32), ("n_kv_heads", _u32), ("n_tokens", _u32),
+        ("q_token_stride", _u64), ("q_head_stride", _u64), ("k_token_stride", _u64), ("k_head_stride", _u64), ("v_token_stride", _u64), ("v_head_stride", _u64),
+        ("norm", _i32), ("eps", C.c_float), ("q_weight", _vp), ("k_weight", _vp),
+    ]
+
+
+class _Rotation(C.Structure):
+    _fields_ = [
+        ("frequencies", _vp), ("axes", _vp), ("positions", _vp), ("n_axes", _u32), ("rotary_dim", _u32), ("interleaved", _i32), ("magnitude", C.c_float),
+    ]
+
+
+class _KvCache4(C.Structure):
+    _fields_ = [
+        ("key_codes", _vp), ("value_codes", _vp), ("key_scales", _vp), ("value_scales", _vp), ("dtype", _i32), ("head_dim", _u32), ("n_kv_heads", _u32),
+        ("code_row_stride", _u64), ("code_head_stride", _u64), ("scale_row_stride", _u64), ("scale_head_stride", _u64), ("key_exponent", _i32),
+        ("value_exponent", _i32), ("positions", _vp), ("documents", _vp), ("entry_head_stride", _u64), ("rows", _vp),
+    ]
+
+
+class HeadRows:
+    """A layer's query, key and value heads of some tokens (SlhaB200HeadRows), device memory, by default [token][head][head_dim] each (`token_stride` and
+    `head_stride`, in elements, for all three; a projection's output holds them side by side).  norm: each query and key head is divided by its root mean
+    square and multiplied with its weight (float32).  Keeps the arrays that it names alive."""
+
+    def __init__(self, q, k, v, n_tokens, n_heads, n_kv_heads, head_dim, dtype=BF16, token_stride=None, head_stride=None, norm=False, eps=1e-6, q_weight=None, k_weight=None):
+        self.kind = kind = _ROWS.get(dtype) or _Any()
+        for a, what in ((q, "q"), (k, "k"), (v, "v")):
+            _typed(a, kind, what)
+            _in_order(a, token_stride if token_stride is not None else head_stride, what)
+        q_weight, k_weight = _given(q_weight, np.float32), _given(k_weight, np.float32)
+        self.kept = (q, k, v, q_weight, k_weight)
+        self.head_dim, self.n_heads, self.n_kv_heads, self.n_tokens = head_dim, n_heads, n_kv_heads, n_tokens
+        at = head_dim if head_stride is None else head_stride
+        of = lambda heads: heads * head_dim if token_stride is None else token_stride  # noqa: E731
+        self.c = _HeadRows(ptr(q), ptr(k), ptr(v), dtype, head_dim, n_heads, n_kv_heads, n_tokens, of(n_heads), at, of(n_kv_heads), at, of(n_kv_heads), at,
+                           1 if norm else 0, eps, _typed(q_weight, _F32, "q_weight"), _typed(k_weight, _F32, "k_weight"))
+        self.address = C.addressof(self.c)
+
+
+class Rotation:
+    """The rotation of heads by their tokens' positions (SlhaB200Rotation): `frequencies` (float32) one for each pair, `positions` (uint32) [n_axes][n_tokens],
+    `axes` (uint8) the axis that each pair goes by.  Keeps the arrays that it names alive."""
+
+    def __init__(self, frequencies, positions, rotary_dim, n_axes=1, axes=None, interleaved=False, magnitude=1.0):
+        frequencies, positions, axes = _given(frequencies, np.float32), _given(positions, np.uint32), _given(axes, np.uint8)
+        self.kept = (frequencies, positions, axes)
+        self.c = _Rotation(_typed(frequencies, _F32, "frequencies"), _typed(axes, _U8, "axes"), _typed(positions, _U32, "positions"), n_axes, rotary_dim,
+                           1 if interleaved else 0, magnitude)
+        self.address = C.addressof(self.c)
+
+
+def rotate_heads(heads, rotation=None, q_out=None, to=None, segments=None, q_out_token_stride=None, q_out_head_stride=None):
+    """Norms and rotation of `heads` (HeadRows) in one pass: queries to q_out [token][head][head_dim], keys and values into the rows of `to` (KvCache) that the
+    segments' tokens have (without segments: row t for token t); see slha_b200_rotate_heads."""
+    seg = None if segments is None else _segments(segments)
+    d = heads.head_dim
+    _check(load_library().slha_b200_rotate_heads(heads.address, None if rotation is None else rotation.address, None if seg is None else seg.ctypes.data,
+                                                 0 if seg is None else len(seg), _typed(q_out, heads.kind, "q_out"),
+                                                 heads.n_heads * d if q_out_token_stride is None else q_out_token_stride,
+                                                 d if q_out_head_stride is None else q_out_head_stride, None if to is None else to.address))
+    return q_out
+
+
+def cache4_scale_bytes(head_dim):
+    """Bytes that the scales of a row of a KV head take in a cache of 4 bits: those of head_dim / 16 blocks, up to a power of two."""
+    return 4 if head_dim <= 64 else 8 if head_dim <= 128 else 16
+
+
+class KvCache4:
+    """Where a cache of key and value rows in 4 bits lies (SlhaB200KvCache4): uint8 device memory, by default codes [row][kv_head][head_dim / 2 bytes, up to a
+    multiple of 16] and scales [row][kv_head][cache4_scale_bytes(head_dim)]; strides in bytes.  dtype: of queries and outputs.  The rest as KvCache.  Keeps
+    the arrays that it names alive."""
+
+    def __init__(self, key_codes, value_codes, key_scales, value_scales, n_kv_heads, head_dim, dtype=BF16, code_row_stride=None, code_head_stride=None,
+                 scale_row_stride=None, scale_head_stride=None, key_exponent=0, value_exponent=0, positions=None, documents=None, entry_head_stride=0, rows=None):
+        rows = _given(rows, np.uint32)
+        self.kind = _ROWS.get(dtype) or _Any()
+        for a, kind, given, what in ((key_codes, _CODES, code_row_stride, "key_codes"), (value_codes, _CODES, code_row_stride, "value_codes"),
+                                     (key_scales, _SCALES, scale_row_stride, "key_scales"), (value_scales, _SCALES, scale_row_stride, "value_scales")):
+            _typed(a, kind, what)
+            _in_order(a, given, what)
+        self.kept = (key_codes, value_codes, key_scales, value_scales, positions, documents, rows)
+        self.head_dim, self.n_kv_heads, self.dtype = head_dim, n_kv_heads, dtype
+        code, scale = -(-head_dim // 32) * 16, cache4_scale_bytes(head_dim)
+        self.c = _KvCache4(ptr(key_codes), ptr(value_codes), ptr(key_scales), ptr(value_scales), dtype, head_dim, n_kv_heads,
+                           n_kv_heads * code if code_row_stride is None else code_row_stride, code if code_head_stride is None else code_head_stride,
+                           n_kv_heads * scale if scale_row_stride is None else scale_row_stride, scale if scale_head_stride is None else scale_head_stride,
+                           key_exponent, value_exponent, _typed(positions, _U32, "positions"), _typed(documents, _U32, "documents"), entry_head_stride,
+                           _typed(rows, _U32, "rows"))
+        self.address = C.addressof(self.c)
+
+
+def write_cache4(cache, segments, rows, n_tokens):
+    """The tokens of `rows` (KvCache: keys and values [token][kv_head][head_dim]) in 4 bits into the rows of `cache` (KvCache4) that the segments' tokens have;
+    see slha_b200_write_cache4."""
+    seg = _segments(segments)
+    _check(load_library().slha_b200_write_cache4(cache.address, seg.ctypes.data, len(seg), rows.address, n_tokens))
+
+
+def read_cache4(cache, segments, to, to_segments=None):
+    """The segments' rows of `cache` (KvCache4) into `to` (KvCache), at to_segments or at the same rows; see slha_b200_read_cache4."""
+    seg = _segments(segments)
+    to_seg = None if to_segments is None else _segments(to_segments)
+    if to_seg is not None and len(to_seg) != len(seg):
+        raise ValueError("to_segments: one for each segment")
+    _check(load_library().slha_b200_read_cache4(cache.address, seg.ctypes.data, len(seg), to.address, None if to_seg is None else to_seg.ctypes.data))
+
+
+def attend_cache4(cache, segments, queries, out, lse_out=None, out_token_stride=None, out_head_stride=None):
+    """attend_cache over rows in 4 bits (KvCache4); see slha_b200_attend_cache4."""
+    seg = _segments(segments)
+    d = cache.head_dim
+    if queries.type not in cache.kind:
+        _fits(queries.type, cache.kind, "q")
+    _check(load_library().slha_b200_attend_cache4(cache.address, seg.ctypes.data, len(seg), queries.address, _typed(out, cache.kind, "out"),
+                                                  queries.n_heads * d if out_token_stride is None else out_token_stride,
+                                                  d if out_head_stride is None else out_head_stride, _typed(lse_out, _F32, "lse_out")))
+    return out
+
+
+def attend_tree4(cache, segments, queries, parents, out, lse_out=None, out_token_stride=None, out_head_stride=None):
+    """attend_tree over rows in 4 bits (KvCache4); see slha_b200_attend_tree4."""
+    seg = _segments(segments)
+    par = _np(parents, np.uint32)
+    d = cache.head_dim
+    if queries.type not in cache.kind:
+        _fits(queries.type, cache.kind, "q")
+    _check(load_library().slha_b200_attend_tree4(cache.address, seg.ctypes.data, len(seg), queries.address, _typed(par, _U32, "parents"), _typed(out, cache.kind, "out"),
+                                                 queries.n_heads * d if out_token_stride is None else out_token_stride,
+                                                 d if out_head_stride is None else out_head_stride, _typed(lse_out, _F32, "lse_out")))
+    return out
+
+
 CACHE_ATTEND, CACHE_ATTEND_WIDE, CACHE_OBSERVE, CACHE_OBSERVE_FEW, CACHE_OBSERVE_MID, CACHE_OBSERVE_MANY = 1, 2, 4, 8, 16, 32
 CACHE_SELECT = 64  # times the CTAs of a cluster
+CACHE_ATTEND4, CACHE_LAID_OUT = 1024, 2048
 
 
 def debug_last_cache_kernels():

@@ -11,6 +11,7 @@
 #include <functional>
 
 #include "cache.cuh"
+#include "cache4.cuh"
 #include "pool.cuh"
 #include "runtime.cuh"
 
@@ -380,3 +381,4 @@ void slha_weights_free(SlhaModel* model) { (void)slha_weights_release(model); }
 
 #include "capi_b200.cuh"
 #include "capi_cache.cuh"
+#include "capi_cache4.cuh"
