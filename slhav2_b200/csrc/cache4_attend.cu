@@ -1,10 +1,667 @@
 // Exact attention over a cache of rows in 4 bits (slha_b200_attend_cache4, slha_b200_attend_tree4).
+//
+// As cache_attend.cu, the scores transposed: S^T = K Q^T and O^T = V^T P^T, so that what the codes stand for is the tensor cores' A operand, made in registers, and 8 query rows are its
+// narrow side.  An A operand holds pairs along the contraction.  Keys: pairs along a row, as the codes lie; a byte becomes two float16 numbers by one conversion, one product with the block's scale makes
+// their values (exact).  Values: pairs of neighbouring rows; two rows' nibbles are put together into bytes before the conversion, their two scales into a pair.  Queries are
+// float16 numbers, scaled by a power of two a row so that the largest has an exponent of 14 (bfloat16 ones exact down to 2^-31 of the largest; float32 ones as two numbers, 22 bits).
+// Weights are float16 too: against a reference that is the running maximum less 8 in units of log 2 they are at most 2^8 and lose bits below 2^-22 of the largest, 2^-33 of it at most.
+//
+// A warp takes 32 rows of a tile of 128 and all of a block's 8, 16 or 32 query rows, with a maximum and sums of its own; tiles arrive by cp.async one to three ahead.
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
 #include <algorithm>
+#include <cmath>
 
 #include "cache4.cuh"
+#include "cache_mma.cuh"
 
 namespace slha {
 namespace {
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr int ATT_THREADS = 128, WARPS = ATT_THREADS / 32;
+constexpr int ROUND = 256;  // tiles that are looked over at a time
+constexpr int KT = 128, KW = KT / WARPS, MT = KW / 16;  // rows of a tile, a warp's, and its groups of 16
+
+template <typename T, int D, int NT>
+struct Shape4 {
+    static constexpr int MB = 8 * NT, PARTS = sizeof(T) == 2 ? 1 : 2;  // query rows; float16 numbers of a query's element
+    static constexpr int CB = D / 2, SB = D / 16;                      // bytes of a row: codes, scales
+    static constexpr uint32_t CODES = KT * CB, SCALES = KT * SB, STAGE = 2 * (CODES + SCALES) + 2 * KT * 4;
+    static constexpr int STAGES = D == 64 ? 4 : D == 128 ? 3 : 2;
+    static constexpr int PITCH = D + 8;  // floats of a query row on the way out
+    static constexpr uint32_t LEAVE = (WARPS * MB * PITCH + MB * (D + 2)) * 4;
+    // behind the stages (the sums leave through them) the queries in the order of B operands; per query row position, document, slope, token within the block, factor; per tile of a round its class
+    static constexpr uint32_t Q_AT = STAGES * STAGE > LEAVE ? STAGES * STAGE : (LEAVE + 127) / 128 * 128, Q_PART = D / 16 * NT * 256;
+    static constexpr uint32_t ROWS_AT = Q_AT + PARTS * Q_PART, LIST_AT = ROWS_AT + 5 * MB * 4, CLS_AT = LIST_AT + ROUND * 2, RANGE_AT = CLS_AT + ROUND, ML_AT = RANGE_AT + 32,
+                              TREE_AT = ML_AT + 2 * WARPS * MB * 4;
+    static constexpr uint32_t SMEM = TREE_AT, SMEM_TREE = TREE_AT + TREE_MOST * 8 + MB * (TREE_MOST / 8);
+    static constexpr int CTAS = D == 256 || NT == 4 ? 2 : 3;
+    static_assert(CTAS * (SMEM_TREE + 1024) <= 228 * 1024, "shared memory of an SM");
+};
+
+// 16-byte pieces of a row in shared memory change places so that eight lanes' reads of keys (two rows) and of values (four rows) lie in different banks.
+template <int D>
+__device__ __forceinline__ uint32_t piece_at(uint32_t row, uint32_t piece) {
+    if constexpr (D == 64) return row * 32 + piece * 16;
+    else if constexpr (D == 128) return row * 64 + ((piece ^ ((row >> 1) & 2)) << 4);
+    else return row * 128 + ((piece ^ (((row & 1) ? 3 : 0) | (row & 4))) << 4);
+}
+// Row of a group of 8 that stands in place x of a tensor core tile.
+__device__ __forceinline__ uint32_t row_of(uint32_t x) { return (x & 4) | (x & 1) << 1 | ((x >> 1 ^ x) & 1); }
+
+// cp.async of N bytes, of which the first `there` are read and the others zeros
+template <int N>
+__device__ __forceinline__ void copy_some(uint32_t dst, const void* src, uint32_t there) {
+    if constexpr (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(there) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;\n" ::"r"(dst), "l"(src), "r"(there), "n"(N) : "memory");
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ float2 unpack_f16(uint32_t x) { return make_float2(__half2float(__ushort_as_half((uint16_t)x)), __half2float(__ushort_as_half((uint16_t)(x >> 16)))); }
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(x));
+    return r;
+}
+__device__ __forceinline__ uint32_t byte_pair(uint32_t w, int b) { return b == 0 ? e2m1_pair<0>(w) : b == 1 ? e2m1_pair<1>(w) : b == 2 ? e2m1_pair<2>(w) : e2m1_pair<3>(w); }
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(ATT_THREADS, Shape4<T, D, NT>::CTAS) cache4_attend_kernel(const __grid_constant__ CacheArgs a, const __grid_constant__ Rows4 in4, const __grid_constant__ CacheTable tab) {
+    using S = Shape4<T, D, NT>;
+    dep_wait();
+    extern __shared__ __align__(1024) unsigned char sm[];
+    const uint32_t sb = smem_addr(sm);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
+    namespace cg = cooperative_groups;
+    const uint32_t cl = a.cluster ? a.cluster : 1, of_cluster = blockIdx.x % cl;
+    const uint32_t head = blockIdx.x / cl % a.n_kv, item = blockIdx.x / cl / a.n_kv * cl + of_cluster;
+    const CacheSeg* table = a.table ? a.table : tab.s;
+    const uint32_t seg = cache_find(a.n_segs, item, [&](uint32_t i) { return table[i].item_begin; });
+    const CacheSeg sg = table[seg];
+    const uint32_t local = item - sg.item_begin, chunk = local % sg.n_chunks, block = local / sg.n_chunks;
+    const uint32_t n = a.rows ? min(a.rows[sg.seg], sg.n_rows) : sg.n_rows;
+    const uint32_t q_rows = sg.n_queries * a.group, row0 = block * S::MB;
+    const uint32_t ctx = n - min(n, sg.n_queries);  // rows before the tokens' own
+    const CacheSight sight{a.window_last, a.prefix ? a.prefix[sg.seg] : 0u, a.causal};
+    const bool has_pos = a.row_pos, has_doc = a.row_doc, arrays = has_pos || has_doc;
+    const uint64_t entry = head * a.entry_hs + sg.row_begin;
+
+    uint32_t* s_qp = reinterpret_cast<uint32_t*>(sm + S::ROWS_AT);
+    uint32_t* s_qd = s_qp + S::MB;
+    float* s_slope = reinterpret_cast<float*>(s_qd + S::MB);
+    uint32_t* s_tok = reinterpret_cast<uint32_t*>(s_slope + S::MB);
+    float* s_factor = reinterpret_cast<float*>(s_tok + S::MB);
+    uint16_t* s_list = reinterpret_cast<uint16_t*>(sm + S::LIST_AT);
+    unsigned char* s_cls = sm + S::CLS_AT;
+    uint32_t* s_range = reinterpret_cast<uint32_t*>(sm + S::RANGE_AT);
+    uint32_t* s_par = reinterpret_cast<uint32_t*>(sm + S::TREE_AT);
+    uint32_t* s_depth = s_par + TREE_MOST;
+    uint32_t* s_anc = s_depth + TREE_MOST;
+    const uint32_t tok0 = row0 / a.group;
+
+    if (a.tree) {
+        for (uint32_t j = tid; j < sg.n_queries; j += ATT_THREADS) {
+            const uint32_t p = a.parents[sg.query_begin + j];
+            s_par[j] = p < j ? p : 0xFFFFFFFFu;
+        }
+        for (uint32_t i = tid; i < S::MB * (TREE_MOST / 32); i += ATT_THREADS) s_anc[i] = 0;
+        __syncthreads();
+        for (uint32_t j = tid; j < sg.n_queries; j += ATT_THREADS) {  // (parents are smaller than their children: every walk ends)
+            const uint32_t mine = j - tok0;
+            uint32_t depth = 0, at = j;
+            while (true) {
+                if (mine < S::MB) s_anc[mine * (TREE_MOST / 32) + (at >> 5)] |= 1u << (at & 31);
+                if (s_par[at] == 0xFFFFFFFFu) break;
+                at = s_par[at];
+                ++depth;
+            }
+            s_depth[j] = depth;
+        }
+        __syncthreads();
+    }
+    // the block's query rows, a warp each (rows behind the last: zeros, with its position; they are not written)
+    const unsigned char* qbase = static_cast<const unsigned char*>(a.q);
+    for (int r = warp; r < S::MB; r += WARPS) {
+        constexpr int CHUNKS = D / 128 > 0 ? D / 128 : 1;  // of 4 elements a lane
+        const uint32_t row = row0 + r;
+        const uint64_t at = row < q_rows ? (sg.query_begin + row / a.group) * a.qts + (head * a.group + row % a.group) * a.qhs : 0;
+        float x[CHUNKS][4];
+        uint32_t most = 0;
+#pragma unroll
+        for (int i = 0; i < CHUNKS; ++i) {
+            const uint32_t d = (lane + i * 32) * 4;
+            x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.0f;
+            if (row < q_rows && d < a.d) {
+                if constexpr (sizeof(T) == 2) {
+                    const uint2 w = *reinterpret_cast<const uint2*>(qbase + (at + d) * 2);
+                    x[i][0] = __uint_as_float(w.x << 16), x[i][1] = __uint_as_float(w.x & 0xFFFF0000u), x[i][2] = __uint_as_float(w.y << 16), x[i][3] = __uint_as_float(w.y & 0xFFFF0000u);
+                } else {
+                    const float4 w = *reinterpret_cast<const float4*>(qbase + (at + d) * 4);
+                    x[i][0] = w.x, x[i][1] = w.y, x[i][2] = w.z, x[i][3] = w.w;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) most = max(most, __float_as_uint(x[i][e]) & 0x7FFFFFFFu);
+        }
+        most = __reduce_max_sync(0xFFFFFFFFu, most);
+        // 2^k with k = 14 less the exponent of the largest; 1 where one is not finite
+        const int k = most >= 0x7F800000u ? 0 : min(14 - (int)(max(most >> 23, 1u) - 127u), 126);
+        const float up = __uint_as_float((uint32_t)(127 + k) << 23);
+        if (lane == 0) s_factor[r] = __uint_as_float((uint32_t)(127 - k) << 23);
+#pragma unroll
+        for (int i = 0; i < CHUNKS; ++i) {
+            const uint32_t d = (lane + i * 32) * 4;
+            if (d >= D) continue;
+            const uint32_t to = S::Q_AT + ((d % (D / 4) / 4 * NT + r / 8) * 32 + r % 8 * 4 + d / (D / 4)) * 8;
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = x[i][e] * up;
+            const uint32_t h0 = pack_f16(v[0], v[1]), h1 = pack_f16(v[2], v[3]);
+            *reinterpret_cast<uint2*>(sm + to) = make_uint2(h0, h1);
+            if constexpr (S::PARTS == 2) {
+                const float2 f0 = unpack_f16(h0), f1 = unpack_f16(h1);
+                *reinterpret_cast<uint2*>(sm + to + S::Q_PART) = make_uint2(pack_f16(v[0] - f0.x, v[1] - f0.y), pack_f16(v[2] - f1.x, v[3] - f1.y));
+            }
+        }
+    }
+    for (int r = tid; r < S::MB; r += ATT_THREADS) {
+        const uint32_t row = min(row0 + r, q_rows - 1), tok = row / a.group;
+        s_qp[r] = a.q_pos ? a.q_pos[sg.query_begin + tok] : sg.base + ctx + (a.tree ? s_depth[tok] : tok);
+        s_qd[r] = has_doc ? a.q_doc[sg.query_begin + tok] : 0u;
+        s_slope[r] = a.slopes ? a.slopes[head * a.group + row % a.group] * LOG2E : 0.0f;
+        s_tok[r] = tok - tok0;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        CacheRanges q{0xFFFFFFFFu, 0u, 0xFFFFFFFFu, 0u};
+        for (int r = lane; r < S::MB; r += 32) {
+            q.pmin = min(q.pmin, s_qp[r]);
+            q.pmax = max(q.pmax, s_qp[r]);
+            q.dmin = min(q.dmin, s_qd[r]);
+            q.dmax = max(q.dmax, s_qd[r]);
+        }
+        q.pmin = __reduce_min_sync(0xFFFFFFFFu, q.pmin);
+        q.pmax = __reduce_max_sync(0xFFFFFFFFu, q.pmax);
+        q.dmin = __reduce_min_sync(0xFFFFFFFFu, q.dmin);
+        q.dmax = __reduce_max_sync(0xFFFFFFFFu, q.dmax);
+        if (lane == 0) s_range[0] = q.pmin, s_range[1] = q.pmax, s_range[2] = q.dmin, s_range[3] = q.dmax;
+    }
+    __syncthreads();
+    const CacheRanges qr{s_range[0], s_range[1], s_range[2], s_range[3]};
+    const auto tile_class = [&](const CacheRanges& k, uint32_t last) { return cache_tile_class(k, qr, sight, a.tree && last >= ctx, last < n); };
+
+    // o[m]: elements 2 m and 2 m + 1 of the lane's D / 8 from g D / 8 on, of query rows 8 nt + 2 t4 and the next
+    float o[D / 16][NT][4], m[NT][2], l[NT][2], factor[NT][2];
+    const float to_log2 = a.cap > 0.0f ? a.scale / a.cap : a.scale * LOG2E, cap2 = a.cap * LOG2E;
+    const bool has_cap = a.cap > 0.0f, has_slope = a.slopes;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) m[nt][c] = -INFINITY, l[nt][c] = 0.0f, factor[nt][c] = to_log2 * s_factor[nt * 8 + t4 * 2 + c];
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.0f;
+
+    const uint32_t tiles = (n + KT - 1) / KT, tile_end = min(tiles, (chunk + 1) * sg.chunk_tiles);
+    const unsigned char* codes[2] = {in4.codes[0] + sg.row_begin * in4.crs + head * in4.chs, in4.codes[1] + sg.row_begin * in4.crs + head * in4.chs};
+    const unsigned char* scales[2] = {in4.scales[0] + sg.row_begin * in4.srs + head * in4.shs, in4.scales[1] + sg.row_begin * in4.srs + head * in4.shs};
+    for (uint32_t r0 = chunk * sg.chunk_tiles; r0 < tile_end; r0 += ROUND) {
+        const uint32_t in_round = min((uint32_t)ROUND, tile_end - r0);
+        // which of the round's tiles are visited
+        if (arrays) {
+            for (uint32_t j = warp; j < in_round; j += WARPS) {
+                const uint32_t first = (r0 + j) * KT, last = first + KT - 1;
+                CacheRanges k{0xFFFFFFFFu, 0u, has_doc ? 0xFFFFFFFFu : 0u, 0u};
+#pragma unroll
+                for (int e = 0; e < KT / 32; ++e) {
+                    const uint32_t i = min(first + lane + e * 32, n - 1);
+                    const uint32_t p = has_pos ? a.row_pos[entry + i] : sg.base + i;
+                    k.pmin = min(k.pmin, p);
+                    k.pmax = max(k.pmax, p);
+                    if (has_doc) {
+                        const uint32_t d = a.row_doc[entry + i];
+                        k.dmin = min(k.dmin, d);
+                        k.dmax = max(k.dmax, d);
+                    }
+                }
+                k.pmin = __reduce_min_sync(0xFFFFFFFFu, k.pmin);
+                k.pmax = __reduce_max_sync(0xFFFFFFFFu, k.pmax);
+                if (has_doc) {
+                    k.dmin = __reduce_min_sync(0xFFFFFFFFu, k.dmin);
+                    k.dmax = __reduce_max_sync(0xFFFFFFFFu, k.dmax);
+                }
+                if (lane == 0) s_cls[j] = (unsigned char)tile_class(k, last);
+            }
+        } else {
+            for (uint32_t j = tid; j < in_round; j += ATT_THREADS) {
+                const uint32_t first = (r0 + j) * KT, last = first + KT - 1;
+                s_cls[j] = (unsigned char)tile_class(CacheRanges{sg.base + first, sg.base + min(last, n - 1), 0u, 0u}, last);
+            }
+        }
+        __syncthreads();
+        uint32_t cnt = 0;
+        for (uint32_t j0 = 0; j0 < in_round; j0 += 32) {  // (every warp counts, the first one writes)
+            const int cls = j0 + lane < in_round ? s_cls[j0 + lane] : 0;
+            const uint32_t mask = __ballot_sync(0xFFFFFFFFu, cls != 0);
+            if (warp == 0 && cls) s_list[cnt + __popc(mask & ((1u << lane) - 1u))] = (uint16_t)((j0 + lane) << 1 | (cls == 2));
+            cnt += __popc(mask);
+        }
+        __syncthreads();
+
+        const auto fetch = [&](uint32_t at) {
+            if (at < cnt) {
+                const uint32_t st = sb + (at % S::STAGES) * S::STAGE, first = (r0 + (s_list[at] >> 1)) * KT;
+                constexpr int PIECES = S::CB / 16;
+#pragma unroll
+                for (int v = 0; v < 2; ++v) {
+#pragma unroll
+                    for (int i = 0; i < KT * PIECES / ATT_THREADS; ++i) {
+                        const uint32_t x = i * ATT_THREADS + tid, r = x / PIECES, c = x % PIECES, row = first + r;
+                        const uint32_t there = row < n && c * 32 < a.d ? min(16u, a.d / 2 - c * 16) : 0u;
+                        copy_some<16>(st + v * S::CODES + piece_at<D>(r, c), there ? codes[v] + row * in4.crs + c * 16 : codes[v], there);
+                    }
+                    const uint32_t row = first + tid;  // (as many rows as threads)
+                    copy_some<S::SB>(st + 2 * S::CODES + v * S::SCALES + tid * S::SB, row < n ? scales[v] + row * in4.srs : scales[v], row < n ? a.d / 16 : 0u);
+                }
+                if (arrays) {
+                    const uint64_t at_entry = entry + min(first + tid, n - 1);
+                    const uint32_t to = st + 2 * (S::CODES + S::SCALES) + tid * 4;
+                    if (has_pos) copy4(to, a.row_pos + at_entry, true);
+                    if (has_doc) copy4(to + KT * 4, a.row_doc + at_entry, true);
+                }
+            }
+            copy_commit();
+        };
+#pragma unroll
+        for (int i = 0; i < S::STAGES - 1; ++i) fetch(i);
+        for (uint32_t li = 0; li < cnt; ++li) {
+            copy_wait<S::STAGES - 2>();
+            __syncthreads();
+            fetch(li + S::STAGES - 1);
+            const unsigned char* st = sm + (li % S::STAGES) * S::STAGE;
+            const uint32_t what = s_list[li], first = (r0 + (what >> 1)) * KT;
+            const bool all = what & 1;
+            const uint32_t key0 = warp * KW;
+
+            // scores: c of s[mt][nt] is row key0 + 16 mt + row_of(g) (c & 2: + 8) and query row 8 nt + 2 t4 + (c & 1)
+            float s[MT][NT][4];
+            {
+                uint32_t w[MT][2][D / 32], sc[MT][2][D / 64 > 1 ? D / 128 : 1];
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t r = key0 + mt * 16 + h * 8 + row_of(g);
+                        if constexpr (D == 64) {
+                            const uint2 x = *reinterpret_cast<const uint2*>(st + piece_at<D>(r, t4 >> 1) + (t4 & 1) * 8);
+                            w[mt][h][0] = x.x, w[mt][h][1] = x.y;
+                            const uint32_t b = st[2 * S::CODES + r * S::SB + t4] & 0x7F;
+                            sc[mt][h][0] = e4m3_pair(b | b << 8);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < D / 128; ++i) {
+                                const uint4 x = *reinterpret_cast<const uint4*>(st + piece_at<D>(r, t4 * (D / 128) + i));
+                                w[mt][h][4 * i] = x.x, w[mt][h][4 * i + 1] = x.y, w[mt][h][4 * i + 2] = x.z, w[mt][h][4 * i + 3] = x.w;
+                                sc[mt][h][i] = e4m3_pair(*reinterpret_cast<const uint16_t*>(st + 2 * S::CODES + r * S::SB + (t4 * (D / 128) + i) * 2) & 0x7F7F);
+                            }
+                        }
+                    }
+                // (float32: the products of four steps at a time are added here, to the nearest: the tensor cores cut their sums off towards zero)
+                constexpr int AT_ONCE = S::PARTS == 2 ? 4 : D / 16;
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) s[mt][nt][0] = s[mt][nt][1] = s[mt][nt][2] = s[mt][nt][3] = 0.0f;
+#pragma unroll
+                for (int k0 = 0; k0 < D / 16; k0 += AT_ONCE) {
+                    float part[MT][NT][4] = {};
+#pragma unroll
+                    for (int kk = k0; kk < k0 + AT_ONCE; ++kk) {
+                        uint32_t x[MT][4];
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                // a lane's elements 4 kk .. 4 kk + 3, of block kk / 4 of its D / 64
+                                const uint32_t two = sc[mt][h][kk / 8], scale = D == 64 ? two : __byte_perm(two, two, kk / 4 % 2 ? 0x3232 : 0x1010);
+                                x[mt][h] = mul_f16x2(byte_pair(w[mt][h][kk / 2], kk % 2 * 2), scale);
+                                x[mt][h + 2] = mul_f16x2(byte_pair(w[mt][h][kk / 2], kk % 2 * 2 + 1), scale);
+                            }
+#pragma unroll
+                        for (int p = S::PARTS - 1; p >= 0; --p)
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) {
+                                const uint2 b = *reinterpret_cast<const uint2*>(sm + S::Q_AT + p * S::Q_PART + ((kk * NT + nt) * 32 + lane) * 8);
+#pragma unroll
+                                for (int mt = 0; mt < MT; ++mt) mma_f16(S::PARTS == 2 ? part[mt][nt] : s[mt][nt], x[mt], b.x, b.y);
+                            }
+                    }
+                    if constexpr (S::PARTS == 2) {
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) s[mt][nt][e] += part[mt][nt][e];
+                    }
+                }
+            }
+            // in units of log 2
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float& x = s[mt][nt][e];
+                        x *= factor[nt][e & 1];
+                        if (has_cap) x = cap2 * cache_tanh(x);
+                    }
+            if (!all || has_slope) {
+                const uint32_t* kp_s = reinterpret_cast<const uint32_t*>(st + 2 * (S::CODES + S::SCALES));
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t col = key0 + mt * 16 + h * 8 + row_of(g), row = first + col;
+                        const bool drafted = a.tree && row >= ctx && row < n;
+                        const uint32_t kp = has_pos ? kp_s[col] : drafted ? sg.base + ctx + s_depth[row - ctx] : sg.base + row;
+                        const uint32_t kd = has_doc ? kp_s[KT + col] : 0u;
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int c = 0; c < 2; ++c) {
+                                float& x = s[mt][nt][h * 2 + c];
+                                const int r = nt * 8 + t4 * 2 + c;
+                                const uint32_t qp = s_qp[r], away = kp <= qp ? qp - kp : kp - qp;
+                                if (has_slope) x = fmaf(-s_slope[r], (float)away, x);
+                                if (!all) {
+                                    bool seen = row < n && sight.sees(qp, kp) && kd == s_qd[r];
+                                    if (drafted) seen = seen && (s_anc[s_tok[r] * (TREE_MOST / 32) + ((row - ctx) >> 5)] >> ((row - ctx) & 31) & 1u);
+                                    if (!seen) x = -INFINITY;
+                                }
+                            }
+                    }
+            }
+            // running maximum (less 8) and sum
+            float grow[NT][2];
+            bool grown = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    float mx = -INFINITY;
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) mx = fmaxf(mx, fmaxf(s[mt][nt][c], s[mt][nt][2 + c]));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 4));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 8));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 16));
+                    float ref = mx - 8.0f;
+                    if (mx - ref > 12.0f) ref = mx;  // (sizes of 2^27 and more, where steps are 16)
+                    ref = fmaxf(m[nt][c], ref);
+                    const float use = ref == -INFINITY ? 0.0f : ref;
+                    grow[nt][c] = exp2_fast(m[nt][c] - use);
+                    grown |= grow[nt][c] != 1.0f;
+                    m[nt][c] = ref;
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            s[mt][nt][h * 2 + c] = exp2_fast(s[mt][nt][h * 2 + c] - use);
+                            sum += s[mt][nt][h * 2 + c];
+                        }
+                    l[nt][c] = fmaf(l[nt][c], grow[nt][c], sum);
+                }
+            if (__any_sync(0xFFFFFFFFu, grown)) {
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[i][nt][e] *= grow[nt][e & 1];
+            }
+            // values
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                uint32_t p[S::PARTS][NT][2];  // B operands: rows 2 t4, 2 t4 + 1 (and + 8) of the 16, query row g
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t x = pack_f16(s[mt][nt][h * 2], s[mt][nt][h * 2 + 1]);
+                        p[0][nt][h] = transpose8(x);
+                        if constexpr (S::PARTS == 2) {
+                            const float2 f = unpack_f16(x);
+                            p[1][nt][h] = transpose8(pack_f16(s[mt][nt][h * 2] - f.x, s[mt][nt][h * 2 + 1] - f.y));
+                        }
+                    }
+                uint32_t w[2][2][D / 64], sc[2][D / 64 > 2 ? 2 : 1], nan[2][D / 64 > 2 ? 2 : 1];  // [+ 8][even or odd elements], pairs of rows; nan: where a scale is
+                bool odd = false;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t raw[2][D / 64], b[2];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const uint32_t r = key0 + mt * 16 + h * 8 + row_of(2 * t4 + j);
+                        const unsigned char* v = st + S::CODES;
+                        const unsigned char* vs = st + 2 * S::CODES + S::SCALES + r * S::SB;
+                        if constexpr (D == 64) {
+                            raw[j][0] = *reinterpret_cast<const uint32_t*>(v + piece_at<D>(r, g >> 2) + (g & 3) * 4);
+                            b[j] = vs[g >> 1];
+                        } else if constexpr (D == 128) {
+                            const uint2 x = *reinterpret_cast<const uint2*>(v + piece_at<D>(r, g >> 1) + (g & 1) * 8);
+                            raw[j][0] = x.x, raw[j][1] = x.y;
+                            b[j] = vs[g];
+                        } else {
+                            const uint4 x = *reinterpret_cast<const uint4*>(v + piece_at<D>(r, g));
+                            raw[j][0] = x.x, raw[j][1] = x.y, raw[j][2] = x.z, raw[j][3] = x.w;
+                            b[j] = *reinterpret_cast<const uint16_t*>(vs + 2 * g);
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < (D / 64 > 2 ? 2 : 1); ++i) {
+                        const uint32_t two = ((i ? b[0] >> 8 : b[0] & 0xFF) | (i ? b[1] & 0xFF00 : b[1] << 8 & 0xFF00)) & 0x7F7F;
+                        sc[h][i] = e4m3_pair(two);
+                        nan[h][i] = ((two & 0xFF) == 0x7F ? 0x3C00u : 0u) | (two >> 8 == 0x7F ? 0x3C000000u : 0u);
+                        odd |= nan[h][i] != 0;
+                    }
+#pragma unroll
+                    for (int i = 0; i < D / 64; ++i) {
+                        w[h][0][i] = (raw[0][i] & 0x0F0F0F0Fu) | (raw[1][i] << 4 & 0xF0F0F0F0u);
+                        w[h][1][i] = (raw[0][i] >> 4 & 0x0F0F0F0Fu) | (raw[1][i] & 0xF0F0F0F0u);
+                    }
+                }
+                // Where some rows are not seen, they may hold anything: a weight of zero does not keep a NaN out of the sum.  Its block's scale becomes zero, and the sums of the query rows
+                // that have a weight for it become NaN.
+                if (!all && __any_sync(0xFFFFFFFFu, odd)) {
+                    uint32_t one[NT][2];
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+                            one[nt][h] = transpose8((s[mt][nt][h * 2] != 0.0f ? 0x3C00u : 0u) | (s[mt][nt][h * 2 + 1] != 0.0f ? 0x3C000000u : 0u));
+#pragma unroll
+                    for (int i = 0; i < (D / 64 > 2 ? 2 : 1); ++i) {
+                        const uint32_t x[4] = {nan[0][i], nan[0][i], nan[1][i], nan[1][i]};
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            float count[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                            mma_f16(count, x, one[nt][0], one[nt][1]);
+#pragma unroll
+                            for (int md = i * 8; md < (D / 64 > 2 ? i * 8 + 8 : D / 16); ++md)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    if (count[e] != 0.0f) o[md][nt][e] = NAN;
+                        }
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            if (nan[h][i] & 0xFFFF) sc[h][i] &= 0xFFFF0000u;
+                            if (nan[h][i] >> 16) sc[h][i] &= 0xFFFFu;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int md = 0; md < D / 16; ++md) {
+                    uint32_t x[4];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) x[h * 2 + j] = mul_f16x2(byte_pair(w[h][j][md / 4], md % 4), sc[h][md / 8]);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        if constexpr (S::PARTS == 2) {  // (as for the scores)
+                            float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                            mma_f16(part, x, p[1][nt][0], p[1][nt][1]);
+                            mma_f16(part, x, p[0][nt][0], p[0][nt][1]);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) o[md][nt][e] += part[e];
+                        } else {
+                            mma_f16(o[md][nt], x, p[0][nt][0], p[0][nt][1]);
+                        }
+                    }
+                }
+            }
+        }
+        copy_wait<0>();
+        __syncthreads();  // (the next round's list and stages)
+    }
+
+    // the warps' maxima and sums meet, then their rows of sums
+    float* s_m = reinterpret_cast<float*>(sm + S::ML_AT);  // [warp][query row]
+    float* s_l = s_m + WARPS * S::MB;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            float& x = l[nt][c];
+            x += __shfl_xor_sync(0xFFFFFFFFu, x, 4);
+            x += __shfl_xor_sync(0xFFFFFFFFu, x, 8);
+            x += __shfl_xor_sync(0xFFFFFFFFu, x, 16);
+            if (g == 0) s_m[warp * S::MB + nt * 8 + t4 * 2 + c] = m[nt][c], s_l[warp * S::MB + nt * 8 + t4 * 2 + c] = x;
+        }
+    __syncthreads();
+    float* s_o = reinterpret_cast<float*>(sm);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const int r = nt * 8 + t4 * 2 + c;
+            float top = s_m[r];
+#pragma unroll
+            for (int w = 1; w < WARPS; ++w) top = fmaxf(top, s_m[w * S::MB + r]);
+            const bool none = m[nt][c] == -INFINITY;
+            const float f = none ? 0.0f : exp2_fast(m[nt][c] - top);
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i)
+                *reinterpret_cast<float2*>(s_o + (warp * S::MB + r) * S::PITCH + g * (D / 8) + 2 * i) =
+                    none ? make_float2(0.0f, 0.0f) : make_float2(o[i][nt][c] * f, o[i][nt][2 + c] * f);
+        }
+    __syncthreads();
+    const bool whole = sg.n_chunks == 1, shared = cl > 1;
+    const uint32_t used = min((uint32_t)S::MB, q_rows - row0);
+    const float up = exp2f((float)in4.exponent[1]);
+    const auto write = [&](uint32_t r, uint32_t c, const float4& x, float top, float sum) {
+        const uint32_t row = row0 + r;
+        const uint64_t tok = sg.query_begin + row / a.group;
+        const uint32_t qh = head * a.group + row % a.group;
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        unsigned char* dst = static_cast<unsigned char*>(a.out) + (tok * a.ots + qh * a.ohs + c) * sizeof(T);
+        if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
+        else *reinterpret_cast<float4*>(dst) = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+        if (a.lse && c == 0) a.lse[tok * a.n_heads + qh] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * LN2;
+    };
+    // of a cluster: the CTA's own sums, maxima and sums of weights for the others to read
+    float* const s_own = s_o + WARPS * S::MB * S::PITCH;
+    float* const s_own_m = s_own + S::MB * D;
+    float* const s_own_l = s_own_m + S::MB;
+    for (uint32_t i = tid; i < used * (D / 4); i += ATT_THREADS) {
+        const uint32_t r = i / (D / 4), c = i % (D / 4) * 4;
+        if (c >= a.d) continue;
+        float top = s_m[r];
+#pragma unroll
+        for (int w = 1; w < WARPS; ++w) top = fmaxf(top, s_m[w * S::MB + r]);
+        float sum = 0.0f;
+        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            const float mw = s_m[w * S::MB + r];
+            sum += mw == -INFINITY ? 0.0f : s_l[w * S::MB + r] * exp2_fast(mw - top);
+            const float4 y = *reinterpret_cast<const float4*>(s_o + (w * S::MB + r) * S::PITCH + c);
+            x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+        }
+        x.x *= up, x.y *= up, x.z *= up, x.w *= up;
+        if (shared) {
+            *reinterpret_cast<float4*>(s_own + r * D + c) = x;
+            if (c == 0) s_own_m[r] = top, s_own_l[r] = sum;
+        } else if (whole) {
+            write(r, c, x, top, sum);
+        } else {
+            const uint64_t at = ((uint64_t)item * a.n_kv + head) * S::MB + r;
+            *reinterpret_cast<float4*>(a.part_o + at * a.d + c) = x;
+            if (c == 0) a.part_ml[at * 2] = top, a.part_ml[at * 2 + 1] = sum;
+        }
+    }
+    if (!shared) return;
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    for (uint32_t i = of_cluster * ATT_THREADS + tid; i < used * (D / 4); i += cl * ATT_THREADS) {
+        const uint32_t r = i / (D / 4), c = i % (D / 4) * 4;
+        if (c >= a.d) continue;
+        float top = -INFINITY, sum = 0.0f;
+        for (uint32_t p = 0; p < cl; ++p) top = fmaxf(top, cluster.map_shared_rank(s_own_m, p)[r]);
+        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (uint32_t p = 0; p < cl; ++p) {
+            const float mp = cluster.map_shared_rank(s_own_m, p)[r], f = mp == -INFINITY ? 0.0f : exp2_fast(mp - top);
+            const float4 y = *reinterpret_cast<const float4*>(cluster.map_shared_rank(s_own, p) + r * D + c);
+            sum = fmaf(f, cluster.map_shared_rank(s_own_l, p)[r], sum);
+            x.x = fmaf(f, y.x, x.x);
+            x.y = fmaf(f, y.y, x.y);
+            x.z = fmaf(f, y.z, x.z);
+            x.w = fmaf(f, y.w, x.w);
+        }
+        write(r, c, x, top, sum);
+    }
+    cluster.sync();  // (the others have read this CTA's sums)
+}
+
+template <typename T, int D, int NT>
+Status launch_class4(Ctx* c, CacheArgs a, const Rows4& r, CacheWork w) {
+    using S = Shape4<T, D, NT>;
+    const uint32_t slots = (uint32_t)sm_count(c->device) * S::CTAS;
+    const uint32_t run = cache_longest_run(w, a.group, S::MB, KT, a.n_kv, a.d, slots, &a.cluster);
+    cache_cut(&w, a.group, S::MB, KT, run, a.cluster);
+    if (w.items * a.n_kv > 0x7FFFFFFFull) return Status(SLHA_ERR_CAPACITY, "attention over a cache: too many blocks of query rows");
+    CacheTable tab;
+    SLHA_TRY(cache_table(c, w.segs, &tab, &a.table));
+    a.n_segs = (uint32_t)w.segs.size();
+    CacheMemory mem{c};
+    SLHA_TRY(cache_part_memory(&a, w.blocks ? w.items : 0, S::MB, &mem));
+    const size_t smem = a.tree ? S::SMEM_TREE : S::SMEM;
+    SLHA_TRY((cache_smem<cache4_attend_kernel<T, D, NT>>(c, S::SMEM_TREE)));
+    g_cache_kernels |= SLHA_B200_CACHE_ATTEND4;
+    SLHA_CUDA(launch_cluster(cache4_attend_kernel<T, D, NT>, dim3((uint32_t)(w.items * a.n_kv)), dim3(ATT_THREADS), smem, c->stream, std::max(a.cluster, 1u), a, r, tab));
+    count_launch();
+    if (w.blocks) SLHA_TRY(launch_cache_join(c, a, sizeof(T) == 2 ? SLHA_B200_BF16 : SLHA_B200_F32, w, S::MB));
+    return mem.done();
+}
+template <typename T>
+Status launch_type4(Ctx* c, const CacheArgs& a, const Rows4& r, int nt, CacheWork w) {
+    if (a.d <= 64) return nt == 1 ? launch_class4<T, 64, 1>(c, a, r, std::move(w)) : nt == 2 ? launch_class4<T, 64, 2>(c, a, r, std::move(w)) : launch_class4<T, 64, 4>(c, a, r, std::move(w));
+    if (a.d <= 128) return nt == 1 ? launch_class4<T, 128, 1>(c, a, r, std::move(w)) : nt == 2 ? launch_class4<T, 128, 2>(c, a, r, std::move(w)) : launch_class4<T, 128, 4>(c, a, r, std::move(w));
+    return nt == 1 ? launch_class4<T, 256, 1>(c, a, r, std::move(w)) : launch_class4<T, 256, 2>(c, a, r, std::move(w));
+}
 
 // Segments whose rows are laid out as rows of the queries' type first, in order, as many at a time as CACHE4_ROWS_MOST holds (at least one).
 Status attend_laid_out(Ctx* c, const CacheArgs& args, const Rows4& r, int dtype, const std::vector<SlhaB200Segment>& segs) {
@@ -78,6 +735,33 @@ Status attend_laid_out(Ctx* c, const CacheArgs& args, const Rows4& r, int dtype,
 
 }  // namespace
 
-Status launch_attend_cache4(Ctx* c, CacheArgs a, const Rows4& r, int dtype, const std::vector<SlhaB200Segment>& segs) { return attend_laid_out(c, a, r, dtype, segs); }
+Status launch_attend_cache4(Ctx* c, CacheArgs a, const Rows4& r, int dtype, const std::vector<SlhaB200Segment>& segs) {
+    CacheWork of[3];  // blocks of 8, 16 and 32 query rows
+    std::vector<SlhaB200Segment> rest = segs;
+    bool any = false;
+    for (size_t i = 0; i < segs.size(); ++i) {
+        const SlhaB200Segment& s = segs[i];
+        if (s.n_queries == 0) continue;
+        const uint64_t rows = (uint64_t)s.n_queries * a.group;
+        if (rows > CACHE4_QUERY_ROWS) {
+            any = true;
+            continue;
+        }
+        rest[i].n_queries = 0;
+        CacheSeg g{};
+        g.row_begin = s.tile_begin;
+        g.n_rows = s.n_tiles;
+        g.query_begin = s.query_begin;
+        g.n_queries = s.n_queries;
+        g.base = s.index_base;
+        g.seg = (uint32_t)i;
+        of[rows <= 8 ? 0 : rows <= 16 ? 1 : 2].segs.push_back(g);
+    }
+    for (int k = 0; k < 3; ++k) {
+        if (of[k].segs.empty()) continue;
+        SLHA_TRY(dtype == SLHA_B200_BF16 ? launch_type4<__nv_bfloat16>(c, a, r, 1 << k, std::move(of[k])) : launch_type4<float>(c, a, r, 1 << k, std::move(of[k])));
+    }
+    return any ? attend_laid_out(c, a, r, dtype, rest) : Status();
+}
 
 }  // namespace slha

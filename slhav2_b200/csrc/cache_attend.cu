@@ -516,13 +516,13 @@ __global__ void __launch_bounds__(JOIN_THREADS) cache_join_kernel(const __grid_c
 }
 
 }  // namespace
-static uint64_t blocks_of(const CacheSeg& s, uint32_t group, uint32_t mb) { return ((uint64_t)s.n_queries * group + mb - 1) / mb; }
-static void cut(CacheWork* w, uint32_t group, uint32_t mb, uint32_t kt, uint32_t most, uint32_t cluster) {
+uint64_t cache_blocks_of(const CacheSeg& s, uint32_t group, uint32_t mb) { return ((uint64_t)s.n_queries * group + mb - 1) / mb; }
+void cache_cut(CacheWork* w, uint32_t group, uint32_t mb, uint32_t kt, uint32_t most, uint32_t cluster) {
     w->items = w->blocks = 0;
     w->chunks = 1;
     for (CacheSeg& c : w->segs) {
         const uint32_t tiles = std::max(1u, (uint32_t)(((uint64_t)c.n_rows + kt - 1) / kt));
-        const uint64_t blocks = blocks_of(c, group, mb);
+        const uint64_t blocks = cache_blocks_of(c, group, mb);
         c.n_chunks = cluster ? cluster : (tiles + most - 1) / most;
         c.chunk_tiles = (tiles + c.n_chunks - 1) / c.n_chunks;
         if (!cluster) c.n_chunks = (tiles + c.chunk_tiles - 1) / c.chunk_tiles;
@@ -537,13 +537,13 @@ static void cut(CacheWork* w, uint32_t group, uint32_t mb, uint32_t kt, uint32_t
 // and half an item at the end; an item costs about four tiles to begin, joining about three and a little for every part.
 // *cluster: how many CTAs share a block of query rows and join their sums through each other's shared memory, where that takes less time than a second kernel (0: none do).
 // One token over 512 rows: 6.5 us by a cluster, 8.0 by a second kernel; 8 x 4096 rows 26.2 and 28.7; 1 x 2048, where more than eight parts are worth it, 9.1 and 8.5.
-static uint32_t longest_run(const CacheWork& w, uint32_t group, uint32_t mb, uint32_t kt, uint32_t n_kv, uint32_t d, uint32_t slots, uint32_t* cluster) {
+uint32_t cache_longest_run(const CacheWork& w, uint32_t group, uint32_t mb, uint32_t kt, uint32_t n_kv, uint32_t d, uint32_t slots, uint32_t* cluster) {
     uint32_t most = 1;
     double total = 0.0;
     for (const CacheSeg& c : w.segs) {
         const uint32_t tiles = std::max(1u, (uint32_t)(((uint64_t)c.n_rows + kt - 1) / kt));
         most = std::max(most, tiles);
-        total += (double)blocks_of(c, group, mb) * tiles * n_kv;
+        total += (double)cache_blocks_of(c, group, mb) * tiles * n_kv;
     }
     uint32_t best = most;
     double best_time = 1e300;
@@ -551,7 +551,7 @@ static uint32_t longest_run(const CacheWork& w, uint32_t group, uint32_t mb, uin
         double items = 0.0;
         for (const CacheSeg& c : w.segs) {
             const uint32_t tiles = std::max(1u, (uint32_t)(((uint64_t)c.n_rows + kt - 1) / kt));
-            items += (double)blocks_of(c, group, mb) * ((tiles + run - 1) / run) * n_kv;
+            items += (double)cache_blocks_of(c, group, mb) * ((tiles + run - 1) / run) * n_kv;
         }
         if (run < most && cache_part_bytes((uint64_t)items, 1, mb, d) > CACHE_PARTS_MOST) break;  // (items: of all KV heads)
         const double time = (items <= slots ? run : total / slots + 0.5 * run) + 4.0 * std::ceil(items / slots) +
@@ -562,7 +562,7 @@ static uint32_t longest_run(const CacheWork& w, uint32_t group, uint32_t mb, uin
     *cluster = 0;
     for (uint32_t cl = 2; cl <= 8; cl *= 2) {
         double items = 0.0;
-        for (const CacheSeg& c : w.segs) items += (double)blocks_of(c, group, mb) * cl * n_kv;
+        for (const CacheSeg& c : w.segs) items += (double)cache_blocks_of(c, group, mb) * cl * n_kv;
         const uint32_t run = (most + cl - 1) / cl;
         const double time = (items <= slots ? run : total / slots + 0.5 * run) + 4.0 * std::ceil(items / slots) + 0.5;
         if (time < best_time) best_time = time, *cluster = cl;
@@ -607,8 +607,8 @@ template <typename T, int D, int WM>
 Status launch_class(Ctx* c, CacheArgs a, CacheWork w) {
     using S = Shape<T, D, WM>;
     const uint32_t slots = (uint32_t)sm_count(c->device) * S::CTAS;
-    const uint32_t run = longest_run(w, a.group, S::MB, S::KT, a.n_kv, a.d, slots, &a.cluster);
-    cut(&w, a.group, S::MB, S::KT, run, a.cluster);
+    const uint32_t run = cache_longest_run(w, a.group, S::MB, S::KT, a.n_kv, a.d, slots, &a.cluster);
+    cache_cut(&w, a.group, S::MB, S::KT, run, a.cluster);
     if (w.items * a.n_kv > 0x7FFFFFFFull) return Status(SLHA_ERR_CAPACITY, "attention over a cache: too many blocks of query rows");
     CacheTable tab;
     SLHA_TRY(cache_table(c, w.segs, &tab, &a.table));
