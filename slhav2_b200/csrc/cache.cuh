@@ -186,10 +186,9 @@ Status cache_smem(Ctx* c, size_t bytes) {
     return Status();
 }
 
-// Blocks of mb query rows of a segment; every segment's tiles of kt rows cut into runs of at most `most` (cluster: into so many); and the run that is quickest, see cache_attend.cu.
+// Blocks of mb query rows of a segment; and every segment's tiles of kt rows cut into runs of at most `most` (cluster: into so many).
 uint64_t cache_blocks_of(const CacheSeg& s, uint32_t group, uint32_t mb);
 void cache_cut(CacheWork* w, uint32_t group, uint32_t mb, uint32_t kt, uint32_t most, uint32_t cluster);
-uint32_t cache_longest_run(const CacheWork& w, uint32_t group, uint32_t mb, uint32_t kt, uint32_t n_kv, uint32_t d, uint32_t slots, uint32_t* cluster);
 inline uint64_t cache_part_bytes(uint64_t items, uint32_t n_kv, uint32_t mb, uint32_t d) { return items * n_kv * mb * (d * 4ull + 8); }
 Status cache_part_memory(CacheArgs* a, uint64_t items, uint32_t mb, CacheMemory* mem);  // where the parts of split segments go
 Status launch_cache_join(Ctx* c, CacheArgs a, int dtype, const CacheWork& w, uint32_t mb);

@@ -30,7 +30,7 @@ struct Shape4 {
     static constexpr int MB = 8 * NT, PARTS = sizeof(T) == 2 ? 1 : 2;  // query rows; float16 numbers of a query's element
     static constexpr int CB = D / 2, SB = D / 16;                      // bytes of a row: codes, scales
     static constexpr uint32_t CODES = KT * CB, SCALES = KT * SB, STAGE = 2 * (CODES + SCALES) + 2 * KT * 4;
-    static constexpr int STAGES = D == 64 ? 4 : D == 128 ? 3 : 2;
+    static constexpr int STAGES = D == 64 ? 4 : D == 128 ? (NT == 1 ? 2 : 3) : 2;
     static constexpr int PITCH = D + 8;  // floats of a query row on the way out
     static constexpr uint32_t LEAVE = (WARPS * MB * PITCH + MB * (D + 2)) * 4;
     // behind the stages (the sums leave through them) the queries in the order of B operands; per query row position, document, slope, token within the block, factor; per tile of a round its class
@@ -38,7 +38,7 @@ struct Shape4 {
     static constexpr uint32_t ROWS_AT = Q_AT + PARTS * Q_PART, LIST_AT = ROWS_AT + 5 * MB * 4, CLS_AT = LIST_AT + ROUND * 2, RANGE_AT = CLS_AT + ROUND, ML_AT = RANGE_AT + 32,
                               TREE_AT = ML_AT + 2 * WARPS * MB * 4;
     static constexpr uint32_t SMEM = TREE_AT, SMEM_TREE = TREE_AT + TREE_MOST * 8 + MB * (TREE_MOST / 8);
-    static constexpr int CTAS = D == 256 || NT == 4 ? 2 : 3;
+    static constexpr int CTAS = D == 256 || NT == 4 ? 2 : NT == 1 ? 4 : 3;
     static_assert(CTAS * (SMEM_TREE + 1024) <= 228 * 1024, "shared memory of an SM");
 };
 
@@ -74,6 +74,9 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     return r;
 }
 __device__ __forceinline__ uint32_t byte_pair(uint32_t w, int b) { return b == 0 ? e2m1_pair<0>(w) : b == 1 ? e2m1_pair<1>(w) : b == 2 ? e2m1_pair<2>(w) : e2m1_pair<3>(w); }
+
+// (not in line: few scores come to it)
+__device__ __noinline__ float tanh_far(float x) { return tanhf(x); }
 
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(ATT_THREADS, Shape4<T, D, NT>::CTAS) cache4_attend_kernel(const __grid_constant__ CacheArgs a, const __grid_constant__ Rows4 in4, const __grid_constant__ CacheTable tab) {
@@ -129,51 +132,6 @@ __global__ void __launch_bounds__(ATT_THREADS, Shape4<T, D, NT>::CTAS) cache4_at
         }
         __syncthreads();
     }
-    // the block's query rows, a warp each (rows behind the last: zeros, with its position; they are not written)
-    const unsigned char* qbase = static_cast<const unsigned char*>(a.q);
-    for (int r = warp; r < S::MB; r += WARPS) {
-        constexpr int CHUNKS = D / 128 > 0 ? D / 128 : 1;  // of 4 elements a lane
-        const uint32_t row = row0 + r;
-        const uint64_t at = row < q_rows ? (sg.query_begin + row / a.group) * a.qts + (head * a.group + row % a.group) * a.qhs : 0;
-        float x[CHUNKS][4];
-        uint32_t most = 0;
-#pragma unroll
-        for (int i = 0; i < CHUNKS; ++i) {
-            const uint32_t d = (lane + i * 32) * 4;
-            x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.0f;
-            if (row < q_rows && d < a.d) {
-                if constexpr (sizeof(T) == 2) {
-                    const uint2 w = *reinterpret_cast<const uint2*>(qbase + (at + d) * 2);
-                    x[i][0] = __uint_as_float(w.x << 16), x[i][1] = __uint_as_float(w.x & 0xFFFF0000u), x[i][2] = __uint_as_float(w.y << 16), x[i][3] = __uint_as_float(w.y & 0xFFFF0000u);
-                } else {
-                    const float4 w = *reinterpret_cast<const float4*>(qbase + (at + d) * 4);
-                    x[i][0] = w.x, x[i][1] = w.y, x[i][2] = w.z, x[i][3] = w.w;
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) most = max(most, __float_as_uint(x[i][e]) & 0x7FFFFFFFu);
-        }
-        most = __reduce_max_sync(0xFFFFFFFFu, most);
-        // 2^k with k = 14 less the exponent of the largest; 1 where one is not finite
-        const int k = most >= 0x7F800000u ? 0 : min(14 - (int)(max(most >> 23, 1u) - 127u), 126);
-        const float up = __uint_as_float((uint32_t)(127 + k) << 23);
-        if (lane == 0) s_factor[r] = __uint_as_float((uint32_t)(127 - k) << 23);
-#pragma unroll
-        for (int i = 0; i < CHUNKS; ++i) {
-            const uint32_t d = (lane + i * 32) * 4;
-            if (d >= D) continue;
-            const uint32_t to = S::Q_AT + ((d % (D / 4) / 4 * NT + r / 8) * 32 + r % 8 * 4 + d / (D / 4)) * 8;
-            float v[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = x[i][e] * up;
-            const uint32_t h0 = pack_f16(v[0], v[1]), h1 = pack_f16(v[2], v[3]);
-            *reinterpret_cast<uint2*>(sm + to) = make_uint2(h0, h1);
-            if constexpr (S::PARTS == 2) {
-                const float2 f0 = unpack_f16(h0), f1 = unpack_f16(h1);
-                *reinterpret_cast<uint2*>(sm + to + S::Q_PART) = make_uint2(pack_f16(v[0] - f0.x, v[1] - f0.y), pack_f16(v[2] - f1.x, v[3] - f1.y));
-            }
-        }
-    }
     for (int r = tid; r < S::MB; r += ATT_THREADS) {
         const uint32_t row = min(row0 + r, q_rows - 1), tok = row / a.group;
         s_qp[r] = a.q_pos ? a.q_pos[sg.query_begin + tok] : sg.base + ctx + (a.tree ? s_depth[tok] : tok);
@@ -198,6 +156,53 @@ __global__ void __launch_bounds__(ATT_THREADS, Shape4<T, D, NT>::CTAS) cache4_at
     }
     __syncthreads();
     const CacheRanges qr{s_range[0], s_range[1], s_range[2], s_range[3]};
+    // The block's query rows into shared memory, a warp each (rows behind the last: zeros; they are not written).
+    const auto take_queries = [&]() {
+        const unsigned char* qbase = static_cast<const unsigned char*>(a.q);
+        for (int r = warp; r < S::MB; r += WARPS) {
+            constexpr int CHUNKS = D / 128 > 0 ? D / 128 : 1;  // of 4 elements a lane
+            const uint32_t row = row0 + r;
+            const uint64_t at = row < q_rows ? (sg.query_begin + row / a.group) * a.qts + (head * a.group + row % a.group) * a.qhs : 0;
+            float x[CHUNKS][4];
+            uint32_t most = 0;
+    #pragma unroll
+            for (int i = 0; i < CHUNKS; ++i) {
+                const uint32_t d = (lane + i * 32) * 4;
+                x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.0f;
+                if (row < q_rows && d < a.d) {
+                    if constexpr (sizeof(T) == 2) {
+                        const uint2 w = *reinterpret_cast<const uint2*>(qbase + (at + d) * 2);
+                        x[i][0] = __uint_as_float(w.x << 16), x[i][1] = __uint_as_float(w.x & 0xFFFF0000u), x[i][2] = __uint_as_float(w.y << 16), x[i][3] = __uint_as_float(w.y & 0xFFFF0000u);
+                    } else {
+                        const float4 w = *reinterpret_cast<const float4*>(qbase + (at + d) * 4);
+                        x[i][0] = w.x, x[i][1] = w.y, x[i][2] = w.z, x[i][3] = w.w;
+                    }
+                }
+    #pragma unroll
+                for (int e = 0; e < 4; ++e) most = max(most, __float_as_uint(x[i][e]) & 0x7FFFFFFFu);
+            }
+            most = __reduce_max_sync(0xFFFFFFFFu, most);
+            // 2^k with k = 14 less the exponent of the largest; 1 where one is not finite
+            const int k = most >= 0x7F800000u ? 0 : min(14 - (int)(max(most >> 23, 1u) - 127u), 126);
+            const float up = __uint_as_float((uint32_t)(127 + k) << 23);
+            if (lane == 0) s_factor[r] = __uint_as_float((uint32_t)(127 - k) << 23);
+    #pragma unroll
+            for (int i = 0; i < CHUNKS; ++i) {
+                const uint32_t d = (lane + i * 32) * 4;
+                if (d >= D) continue;
+                const uint32_t to = S::Q_AT + ((d % (D / 4) / 4 * NT + r / 8) * 32 + r % 8 * 4 + d / (D / 4)) * 8;
+                float v[4];
+    #pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = x[i][e] * up;
+                const uint32_t h0 = pack_f16(v[0], v[1]), h1 = pack_f16(v[2], v[3]);
+                *reinterpret_cast<uint2*>(sm + to) = make_uint2(h0, h1);
+                if constexpr (S::PARTS == 2) {
+                    const float2 f0 = unpack_f16(h0), f1 = unpack_f16(h1);
+                    *reinterpret_cast<uint2*>(sm + to + S::Q_PART) = make_uint2(pack_f16(v[0] - f0.x, v[1] - f0.y), pack_f16(v[2] - f1.x, v[3] - f1.y));
+                }
+            }
+        }
+    };
     const auto tile_class = [&](const CacheRanges& k, uint32_t last) { return cache_tile_class(k, qr, sight, a.tree && last >= ctx, last < n); };
 
     // o[m]: elements 2 m and 2 m + 1 of the lane's D / 8 from g D / 8 on, of query rows 8 nt + 2 t4 and the next
@@ -207,7 +212,7 @@ __global__ void __launch_bounds__(ATT_THREADS, Shape4<T, D, NT>::CTAS) cache4_at
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int c = 0; c < 2; ++c) m[nt][c] = -INFINITY, l[nt][c] = 0.0f, factor[nt][c] = to_log2 * s_factor[nt * 8 + t4 * 2 + c];
+        for (int c = 0; c < 2; ++c) m[nt][c] = -INFINITY, l[nt][c] = 0.0f;
 #pragma unroll
     for (int i = 0; i < D / 16; ++i)
 #pragma unroll
@@ -259,23 +264,36 @@ __global__ void __launch_bounds__(ATT_THREADS, Shape4<T, D, NT>::CTAS) cache4_at
         }
         __syncthreads();
 
-        const auto fetch = [&](uint32_t at) {
+        // A warp's rows of tile `at` of the list into stage `slot`, by the warp that will read them.  A lane copies the same piece of rows PER apart, and one row's scales.
+        const auto fetch = [&](uint32_t at, uint32_t slot) {
             if (at < cnt) {
-                const uint32_t st = sb + (at % S::STAGES) * S::STAGE, first = (r0 + (s_list[at] >> 1)) * KT;
-                constexpr int PIECES = S::CB / 16;
+                constexpr int PIECES = S::CB / 16, PER = 32 / PIECES;
+                const uint32_t st = sb + slot * S::STAGE, first = (r0 + (s_list[at] >> 1)) * KT, mine = first + tid;
+                const uint32_t r = warp * KW + lane / PIECES, c = lane % PIECES, there = c * 32 < a.d ? min(16u, a.d / 2 - c * 16) : 0u;
+                const uint32_t to = st + piece_at<D>(r, c), to_scale = st + 2 * S::CODES + tid * S::SB;
+                const auto place = [&](int i) { return to + i * PER * S::CB ^ (D == 256 && i & 1 ? 64u : 0u); };  // piece_at's, PER rows on
+                const uint64_t at_code = there ? (first + r) * in4.crs + c * 16 : 0, step = there ? PER * in4.crs : 0;
+                if (mine - lane + KW <= n) {
 #pragma unroll
-                for (int v = 0; v < 2; ++v) {
+                    for (int v = 0; v < 2; ++v) {
+                        const unsigned char* p = codes[v] + at_code;
 #pragma unroll
-                    for (int i = 0; i < KT * PIECES / ATT_THREADS; ++i) {
-                        const uint32_t x = i * ATT_THREADS + tid, r = x / PIECES, c = x % PIECES, row = first + r;
-                        const uint32_t there = row < n && c * 32 < a.d ? min(16u, a.d / 2 - c * 16) : 0u;
-                        copy_some<16>(st + v * S::CODES + piece_at<D>(r, c), there ? codes[v] + row * in4.crs + c * 16 : codes[v], there);
+                        for (int i = 0; i < KW / PER; ++i, p += step) copy_some<16>(place(i) + v * S::CODES, p, there);
+                        copy_some<S::SB>(to_scale + v * S::SCALES, scales[v] + mine * in4.srs, a.d / 16);
                     }
-                    const uint32_t row = first + tid;  // (as many rows as threads)
-                    copy_some<S::SB>(st + 2 * S::CODES + v * S::SCALES + tid * S::SB, row < n ? scales[v] + row * in4.srs : scales[v], row < n ? a.d / 16 : 0u);
+                } else {  // (rows behind the last: zeros)
+#pragma unroll
+                    for (int v = 0; v < 2; ++v) {
+#pragma unroll
+                        for (int i = 0; i < KW / PER; ++i) {
+                            const bool row = first + r + i * PER < n;
+                            copy_some<16>(place(i) + v * S::CODES, row ? codes[v] + at_code + i * step : codes[v], row ? there : 0u);
+                        }
+                        copy_some<S::SB>(to_scale + v * S::SCALES, mine < n ? scales[v] + mine * in4.srs : scales[v], mine < n ? a.d / 16 : 0u);
+                    }
                 }
                 if (arrays) {
-                    const uint64_t at_entry = entry + min(first + tid, n - 1);
+                    const uint64_t at_entry = entry + min(mine, n - 1);
                     const uint32_t to = st + 2 * (S::CODES + S::SCALES) + tid * 4;
                     if (has_pos) copy4(to, a.row_pos + at_entry, true);
                     if (has_doc) copy4(to + KT * 4, a.row_doc + at_entry, true);
@@ -284,12 +302,23 @@ __global__ void __launch_bounds__(ATT_THREADS, Shape4<T, D, NT>::CTAS) cache4_at
             copy_commit();
         };
 #pragma unroll
-        for (int i = 0; i < S::STAGES - 1; ++i) fetch(i);
+        for (int i = 0; i < S::STAGES - 1; ++i) fetch(i, i);
+        if (r0 == chunk * sg.chunk_tiles) {  // (while the first rows are on their way)
+            take_queries();
+            __syncthreads();
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) factor[nt][c] = to_log2 * s_factor[nt * 8 + t4 * 2 + c];
+        }
+        uint32_t slot = 0, slot_next = S::STAGES - 1;
         for (uint32_t li = 0; li < cnt; ++li) {
             copy_wait<S::STAGES - 2>();
-            __syncthreads();
-            fetch(li + S::STAGES - 1);
-            const unsigned char* st = sm + (li % S::STAGES) * S::STAGE;
+            __syncwarp();
+            fetch(li + S::STAGES - 1, slot_next);
+            const unsigned char* st = sm + slot * S::STAGE;
+            slot = slot + 1 == S::STAGES ? 0 : slot + 1;
+            slot_next = slot_next + 1 == S::STAGES ? 0 : slot_next + 1;
             const uint32_t what = s_list[li], first = (r0 + (what >> 1)) * KT;
             const bool all = what & 1;
             const uint32_t key0 = warp * KW;
@@ -366,72 +395,99 @@ __global__ void __launch_bounds__(ATT_THREADS, Shape4<T, D, NT>::CTAS) cache4_at
                     for (int e = 0; e < 4; ++e) {
                         float& x = s[mt][nt][e];
                         x *= factor[nt][e & 1];
-                        if (has_cap) x = cap2 * cache_tanh(x);
+                        if (has_cap) x = cap2 * (fabsf(x) <= 1.0f ? tanh_small(x) : tanh_far(x));
                     }
             if (!all || has_slope) {
                 const uint32_t* kp_s = reinterpret_cast<const uint32_t*>(st + 2 * (S::CODES + S::SCALES));
+                const auto place = [&](int x) { return key0 + (x >> 1) * 16 + (x & 1) * 8 + row_of(g); };  // of the lane's x-th row in the tile
+                const auto position = [&](uint32_t col) {
+                    const uint32_t row = first + col;
+                    return has_pos ? kp_s[col] : a.tree && row >= ctx && row < n ? sg.base + ctx + s_depth[row - ctx] : sg.base + row;
+                };
+                if (has_slope) {
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const uint32_t col = key0 + mt * 16 + h * 8 + row_of(g), row = first + col;
-                        const bool drafted = a.tree && row >= ctx && row < n;
-                        const uint32_t kp = has_pos ? kp_s[col] : drafted ? sg.base + ctx + s_depth[row - ctx] : sg.base + row;
-                        const uint32_t kd = has_doc ? kp_s[KT + col] : 0u;
+                    for (int x = 0; x < 2 * MT; ++x) {
+                        const uint32_t kp = position(place(x));
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                             for (int c = 0; c < 2; ++c) {
-                                float& x = s[mt][nt][h * 2 + c];
                                 const int r = nt * 8 + t4 * 2 + c;
-                                const uint32_t qp = s_qp[r], away = kp <= qp ? qp - kp : kp - qp;
-                                if (has_slope) x = fmaf(-s_slope[r], (float)away, x);
-                                if (!all) {
-                                    bool seen = row < n && sight.sees(qp, kp) && kd == s_qd[r];
-                                    if (drafted) seen = seen && (s_anc[s_tok[r] * (TREE_MOST / 32) + ((row - ctx) >> 5)] >> ((row - ctx) & 31) & 1u);
-                                    if (!seen) x = -INFINITY;
-                                }
+                                float& y = s[x >> 1][nt][(x & 1) * 2 + c];
+                                y = fmaf(-s_slope[r], cache_distance(kp, s_qp[r]), y);
                             }
                     }
+                }
+                if (!all) {
+                    // (which of them are seen is found out in a loop: unrolled, it pushed the rest of the loop over the tiles out of the instruction cache)
+                    uint32_t seen = 0;
+#pragma unroll 1
+                    for (int x = 0; x < 2 * MT; ++x) {
+                        const uint32_t col = place(x), row = first + col, kp = position(col), kd = has_doc ? kp_s[KT + col] : 0u;
+                        const bool drafted = a.tree && row >= ctx && row < n;
+#pragma unroll 1
+                        for (int i = 0; i < 2 * NT; ++i) {
+                            const int r = (i >> 1) * 8 + t4 * 2 + (i & 1);
+                            bool sees = row < n && sight.sees(s_qp[r], kp) && kd == s_qd[r];
+                            if (drafted) sees = sees && (s_anc[s_tok[r] * (TREE_MOST / 32) + ((row - ctx) >> 5)] >> ((row - ctx) & 31) & 1u);
+                            seen |= (uint32_t)sees << (x * 2 * NT + i);
+                        }
+                    }
+#pragma unroll
+                    for (int x = 0; x < 2 * MT; ++x)
+#pragma unroll
+                        for (int i = 0; i < 2 * NT; ++i)
+                            if (!(seen >> (x * 2 * NT + i) & 1)) s[x >> 1][i >> 1][(x & 1) * 2 + (i & 1)] = -INFINITY;
+                }
             }
-            // running maximum (less 8) and sum
-            float grow[NT][2];
-            bool grown = false;
+            // Weights against a reference: once a score is more than 15 above it, and for a row's first scores, it becomes the largest so far less 8.  (Looking for the largest over the
+            // lanes each time cost a tenth of the instructions, and their latency.)
+            bool above = false;
+            float top[NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    float mx = -INFINITY;
+                    top[nt][c] = s[0][nt][c];
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) mx = fmaxf(mx, fmaxf(s[mt][nt][c], s[mt][nt][2 + c]));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 4));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 8));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 16));
-                    float ref = mx - 8.0f;
-                    if (mx - ref > 12.0f) ref = mx;  // (sizes of 2^27 and more, where steps are 16)
-                    ref = fmaxf(m[nt][c], ref);
-                    const float use = ref == -INFINITY ? 0.0f : ref;
-                    grow[nt][c] = exp2_fast(m[nt][c] - use);
-                    grown |= grow[nt][c] != 1.0f;
-                    m[nt][c] = ref;
-                    float sum = 0.0f;
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            s[mt][nt][h * 2 + c] = exp2_fast(s[mt][nt][h * 2 + c] - use);
-                            sum += s[mt][nt][h * 2 + c];
-                        }
-                    l[nt][c] = fmaf(l[nt][c], grow[nt][c], sum);
+                    for (int x = 1; x < 2 * MT; ++x) top[nt][c] = fmaxf(top[nt][c], s[x >> 1][nt][(x & 1) * 2 + c]);
+                    above |= top[nt][c] > m[nt][c] + 15.0f;
                 }
-            if (__any_sync(0xFFFFFFFFu, grown)) {
+            if (__any_sync(0xFFFFFFFFu, above)) {
 #pragma unroll
-                for (int i = 0; i < D / 16; ++i)
+                for (int nt = 0; nt < NT; ++nt) {
+                    float grow[2];
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
+                    for (int c = 0; c < 2; ++c) {
+                        float mx = top[nt][c];
+                        mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 4));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 8));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 16));
+                        float ref = mx - 8.0f;
+                        if (mx - ref > 12.0f) ref = mx;  // (sizes of 2^27 and more, where steps are 16)
+                        if (!(mx > m[nt][c] + 15.0f)) ref = m[nt][c];
+                        grow[c] = ref == -INFINITY ? 1.0f : exp2_fast(m[nt][c] - ref);
+                        m[nt][c] = ref;
+                        l[nt][c] *= grow[c];
+                    }
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) o[i][nt][e] *= grow[nt][e & 1];
+                    for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[i][nt][e] *= grow[e & 1];
+                }
             }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const float use = m[nt][c] == -INFINITY ? 0.0f : m[nt][c];
+#pragma unroll
+                    for (int x = 0; x < 2 * MT; ++x) {
+                        float& y = s[x >> 1][nt][(x & 1) * 2 + c];
+                        y = exp2_fast(y - use);
+                        l[nt][c] += y;
+                    }
+                }
             // values
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
@@ -447,8 +503,7 @@ __global__ void __launch_bounds__(ATT_THREADS, Shape4<T, D, NT>::CTAS) cache4_at
                             p[1][nt][h] = transpose8(pack_f16(s[mt][nt][h * 2] - f.x, s[mt][nt][h * 2 + 1] - f.y));
                         }
                     }
-                uint32_t w[2][2][D / 64], sc[2][D / 64 > 2 ? 2 : 1], nan[2][D / 64 > 2 ? 2 : 1];  // [+ 8][even or odd elements], pairs of rows; nan: where a scale is
-                bool odd = false;
+                uint32_t w[2][2][D / 64], sc[2][D / 64 > 2 ? 2 : 1], twos[2][D / 64 > 2 ? 2 : 1];  // [+ 8][even or odd elements], of pairs of rows
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     uint32_t raw[2][D / 64], b[2];
@@ -472,10 +527,8 @@ __global__ void __launch_bounds__(ATT_THREADS, Shape4<T, D, NT>::CTAS) cache4_at
                     }
 #pragma unroll
                     for (int i = 0; i < (D / 64 > 2 ? 2 : 1); ++i) {
-                        const uint32_t two = ((i ? b[0] >> 8 : b[0] & 0xFF) | (i ? b[1] & 0xFF00 : b[1] << 8 & 0xFF00)) & 0x7F7F;
-                        sc[h][i] = e4m3_pair(two);
-                        nan[h][i] = ((two & 0xFF) == 0x7F ? 0x3C00u : 0u) | (two >> 8 == 0x7F ? 0x3C000000u : 0u);
-                        odd |= nan[h][i] != 0;
+                        twos[h][i] = __byte_perm(b[0], b[1], i ? 0x4451 : 0x4440) & 0x7F7F;
+                        sc[h][i] = e4m3_pair(twos[h][i]);
                     }
 #pragma unroll
                     for (int i = 0; i < D / 64; ++i) {
@@ -485,6 +538,17 @@ __global__ void __launch_bounds__(ATT_THREADS, Shape4<T, D, NT>::CTAS) cache4_at
                 }
                 // Where some rows are not seen, they may hold anything: a weight of zero does not keep a NaN out of the sum.  Its block's scale becomes zero, and the sums of the query rows
                 // that have a weight for it become NaN.
+                uint32_t nan[2][D / 64 > 2 ? 2 : 1];
+                bool odd = false;
+                if (!all) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int i = 0; i < (D / 64 > 2 ? 2 : 1); ++i) {
+                            nan[h][i] = ((twos[h][i] & 0xFF) == 0x7F ? 0x3C00u : 0u) | (twos[h][i] >> 8 == 0x7F ? 0x3C000000u : 0u);
+                            odd |= nan[h][i] != 0;
+                        }
+                }
                 if (!all && __any_sync(0xFFFFFFFFu, odd)) {
                     uint32_t one[NT][2];
 #pragma unroll
@@ -636,11 +700,56 @@ __global__ void __launch_bounds__(ATT_THREADS, Shape4<T, D, NT>::CTAS) cache4_at
     cluster.sync();  // (the others have read this CTA's sums)
 }
 
+// The longest run of tiles of an item, or into how many CTAs of a cluster each block of query rows goes (*cluster; 0: none), by a model of the time in us: a tile of 128 dimensions takes 0.5 and 0.26
+// for each CTA that shares the SM (32 query rows: 1.6 times that), an item 1.7 of an SM's time to begin and end; a second kernel that joins parts 2.2 and a little for each part, a cluster 1.05.
+// What fits on the GPU at once takes as long as its longest item, more than that the mean load and a third of an item.  Its constants were fitted to 34 calls, each with every run: of one to
+// 64 sequences, 256 to 131072 rows, 64 to 256 dimensions; what it picks takes 2 % longer than the best of each on the average.  (One token over 2048 rows: 7.9 us in 8 clusters of 8, 9.3 of 4,
+// 8.5 in 128 items and a second kernel; 8192 rows 12.8, 19.1 and 11.0; 131072 rows in 592 items 43.5, in 552 45.2, in 824 49.)
+uint32_t run_of(const CacheWork& w, uint32_t group, uint32_t mb, uint32_t n_kv, uint32_t d, double each, uint32_t sms, uint32_t ctas, uint32_t* cluster) {
+    uint32_t most = 1;
+    double total = 0.0;
+    const auto tiles = [](const CacheSeg& c) { return std::max(1u, (uint32_t)(((uint64_t)c.n_rows + KT - 1) / KT)); };
+    for (const CacheSeg& c : w.segs) {
+        most = std::max(most, tiles(c));
+        total += (double)cache_blocks_of(c, group, mb) * tiles(c) * n_kv;
+    }
+    const double slots = (double)sms * ctas;
+    const auto time_of = [&](double items, double run) {
+        const double load = std::min(std::max(std::ceil(items / sms), 1.0), (double)ctas), tile = each * (0.5 + 0.26 * load);
+        return (items <= slots ? run : total / slots + 0.3 * run) * tile + 1.7 * load * std::max(items / slots, 1.0);
+    };
+    uint32_t best = most;
+    double best_time = 1e300;
+    const auto look = [&](uint32_t run) {
+        if (run < 1 || run > most) return;
+        double items = 0.0;
+        uint32_t longest = 1;
+        for (const CacheSeg& c : w.segs) {
+            const uint32_t n = (tiles(c) + run - 1) / run;
+            items += (double)cache_blocks_of(c, group, mb) * n * n_kv;
+            longest = std::max(longest, (tiles(c) + n - 1) / n);
+        }
+        if (run < most && cache_part_bytes((uint64_t)items, 1, mb, d) > CACHE_PARTS_MOST) return;  // (items: of all KV heads)
+        const double time = time_of(items, items <= slots ? longest : run) + (run < most ? 2.2 + 0.006 * ((most + run - 1) / run) : 0.0);
+        if (time < best_time) best_time = time, best = run;
+    };
+    for (uint32_t run = most; run >= 1; run = std::min(run - 1, run * 7 / 8)) look(run);
+    for (uint32_t of = 1; of <= 4 * ctas; ++of)  // runs that give each SM 1, 2, .. items
+        for (uint32_t more = 0; more < 3; ++more) look((uint32_t)std::min(total / sms / of, 4e9) + more);
+    *cluster = 0;
+    for (uint32_t cl = 2; cl <= 8; cl *= 2) {
+        double items = 0.0;
+        for (const CacheSeg& c : w.segs) items += (double)cache_blocks_of(c, group, mb) * cl * n_kv;
+        const double time = time_of(items, (most + cl - 1) / cl) + 1.05;
+        if (time < best_time) best_time = time, *cluster = cl;
+    }
+    return best;
+}
+
 template <typename T, int D, int NT>
 Status launch_class4(Ctx* c, CacheArgs a, const Rows4& r, CacheWork w) {
     using S = Shape4<T, D, NT>;
-    const uint32_t slots = (uint32_t)sm_count(c->device) * S::CTAS;
-    const uint32_t run = cache_longest_run(w, a.group, S::MB, KT, a.n_kv, a.d, slots, &a.cluster);
+    const uint32_t run = run_of(w, a.group, S::MB, a.n_kv, a.d, (NT == 4 ? 1.6 : 1.0) * D / 128, (uint32_t)sm_count(c->device), S::CTAS, &a.cluster);
     cache_cut(&w, a.group, S::MB, KT, run, a.cluster);
     if (w.items * a.n_kv > 0x7FFFFFFFull) return Status(SLHA_ERR_CAPACITY, "attention over a cache: too many blocks of query rows");
     CacheTable tab;

@@ -537,7 +537,7 @@ void cache_cut(CacheWork* w, uint32_t group, uint32_t mb, uint32_t kt, uint32_t 
 // and half an item at the end; an item costs about four tiles to begin, joining about three and a little for every part.
 // *cluster: how many CTAs share a block of query rows and join their sums through each other's shared memory, where that takes less time than a second kernel (0: none do).
 // One token over 512 rows: 6.5 us by a cluster, 8.0 by a second kernel; 8 x 4096 rows 26.2 and 28.7; 1 x 2048, where more than eight parts are worth it, 9.1 and 8.5.
-uint32_t cache_longest_run(const CacheWork& w, uint32_t group, uint32_t mb, uint32_t kt, uint32_t n_kv, uint32_t d, uint32_t slots, uint32_t* cluster) {
+static uint32_t longest_run(const CacheWork& w, uint32_t group, uint32_t mb, uint32_t kt, uint32_t n_kv, uint32_t d, uint32_t slots, uint32_t* cluster) {
     uint32_t most = 1;
     double total = 0.0;
     for (const CacheSeg& c : w.segs) {
@@ -607,7 +607,7 @@ template <typename T, int D, int WM>
 Status launch_class(Ctx* c, CacheArgs a, CacheWork w) {
     using S = Shape<T, D, WM>;
     const uint32_t slots = (uint32_t)sm_count(c->device) * S::CTAS;
-    const uint32_t run = cache_longest_run(w, a.group, S::MB, S::KT, a.n_kv, a.d, slots, &a.cluster);
+    const uint32_t run = longest_run(w, a.group, S::MB, S::KT, a.n_kv, a.d, slots, &a.cluster);
     cache_cut(&w, a.group, S::MB, S::KT, run, a.cluster);
     if (w.items * a.n_kv > 0x7FFFFFFFull) return Status(SLHA_ERR_CAPACITY, "attention over a cache: too many blocks of query rows");
     CacheTable tab;
