@@ -429,11 +429,22 @@ def score_segments(tiles, segments, q_coarse, q_sign, nq, out, row_offsets, row_
     return out
 
 
+class _Segments(np.ndarray):
+    """A table of segments that knows its address (numpy takes 0.7 us for it); views and copies do not."""
+
+    address = None
+
+    def __array_finalize__(self, of):
+        self.address = None
+
+
 def make_segments(rows):
     """rows: iterable of (tile_begin, n_tiles, query_begin, n_queries, index_base)."""
     seg = np.zeros(len(rows), SEGMENT_DTYPE)
     for i, r in enumerate(rows):
         seg[i] = tuple(r)
+    seg = seg.view(_Segments)
+    seg.address = seg.ctypes.data
     return seg
 
 
@@ -603,6 +614,14 @@ class CacheQueries:
         self.address = C.addressof(self.c)
 
 
+def _table(segments):
+    """(address, number) of a table of segments, and what keeps it alive."""
+    if type(segments) is not _Segments or segments.address is None:
+        segments = _segments(segments)
+        return segments.ctypes.data, len(segments), segments
+    return segments.address, len(segments), segments
+
+
 def _segments(segments):
     if isinstance(segments, np.ndarray) and segments.dtype == SEGMENT_DTYPE and segments.flags["C_CONTIGUOUS"]:
         return segments
@@ -720,10 +739,9 @@ class Rotation:
 def rotate_heads(heads, rotation=None, q_out=None, to=None, segments=None, q_out_token_stride=None, q_out_head_stride=None):
     """Norms and rotation of `heads` (HeadRows) in one pass: queries to q_out [token][head][head_dim], keys and values into the rows of `to` (KvCache) that the
     segments' tokens have (without segments: row t for token t); see slha_b200_rotate_heads."""
-    seg = None if segments is None else _segments(segments)
+    seg, n, kept = (None, 0, None) if segments is None else _table(segments)
     d = heads.head_dim
-    _check(load_library().slha_b200_rotate_heads(heads.address, None if rotation is None else rotation.address, None if seg is None else seg.ctypes.data,
-                                                 0 if seg is None else len(seg), _typed(q_out, heads.kind, "q_out"),
+    _check(load_library().slha_b200_rotate_heads(heads.address, None if rotation is None else rotation.address, seg, n, _typed(q_out, heads.kind, "q_out"),
                                                  heads.n_heads * d if q_out_token_stride is None else q_out_token_stride,
                                                  d if q_out_head_stride is None else q_out_head_stride, None if to is None else to.address))
     return q_out
@@ -761,26 +779,26 @@ class KvCache4:
 def write_cache4(cache, segments, rows, n_tokens):
     """The tokens of `rows` (KvCache: keys and values [token][kv_head][head_dim]) in 4 bits into the rows of `cache` (KvCache4) that the segments' tokens have;
     see slha_b200_write_cache4."""
-    seg = _segments(segments)
-    _check(load_library().slha_b200_write_cache4(cache.address, seg.ctypes.data, len(seg), rows.address, n_tokens))
+    seg, n, kept = _table(segments)
+    _check(load_library().slha_b200_write_cache4(cache.address, seg, n, rows.address, n_tokens))
 
 
 def read_cache4(cache, segments, to, to_segments=None):
     """The segments' rows of `cache` (KvCache4) into `to` (KvCache), at to_segments or at the same rows; see slha_b200_read_cache4."""
-    seg = _segments(segments)
-    to_seg = None if to_segments is None else _segments(to_segments)
-    if to_seg is not None and len(to_seg) != len(seg):
+    seg, n, kept = _table(segments)
+    to_seg, to_n, to_kept = (None, n, None) if to_segments is None else _table(to_segments)
+    if to_n != n:
         raise ValueError("to_segments: one for each segment")
-    _check(load_library().slha_b200_read_cache4(cache.address, seg.ctypes.data, len(seg), to.address, None if to_seg is None else to_seg.ctypes.data))
+    _check(load_library().slha_b200_read_cache4(cache.address, seg, n, to.address, to_seg))
 
 
 def attend_cache4(cache, segments, queries, out, lse_out=None, out_token_stride=None, out_head_stride=None):
     """attend_cache over rows in 4 bits (KvCache4); see slha_b200_attend_cache4."""
-    seg = _segments(segments)
+    seg, n, kept = _table(segments)
     d = cache.head_dim
     if queries.type not in cache.kind:
         _fits(queries.type, cache.kind, "q")
-    _check(load_library().slha_b200_attend_cache4(cache.address, seg.ctypes.data, len(seg), queries.address, _typed(out, cache.kind, "out"),
+    _check(load_library().slha_b200_attend_cache4(cache.address, seg, n, queries.address, _typed(out, cache.kind, "out"),
                                                   queries.n_heads * d if out_token_stride is None else out_token_stride,
                                                   d if out_head_stride is None else out_head_stride, _typed(lse_out, _F32, "lse_out")))
     return out
@@ -788,12 +806,12 @@ def attend_cache4(cache, segments, queries, out, lse_out=None, out_token_stride=
 
 def attend_tree4(cache, segments, queries, parents, out, lse_out=None, out_token_stride=None, out_head_stride=None):
     """attend_tree over rows in 4 bits (KvCache4); see slha_b200_attend_tree4."""
-    seg = _segments(segments)
+    seg, n, kept = _table(segments)
     par = _np(parents, np.uint32)
     d = cache.head_dim
     if queries.type not in cache.kind:
         _fits(queries.type, cache.kind, "q")
-    _check(load_library().slha_b200_attend_tree4(cache.address, seg.ctypes.data, len(seg), queries.address, _typed(par, _U32, "parents"), _typed(out, cache.kind, "out"),
+    _check(load_library().slha_b200_attend_tree4(cache.address, seg, n, queries.address, _typed(par, _U32, "parents"), _typed(out, cache.kind, "out"),
                                                  queries.n_heads * d if out_token_stride is None else out_token_stride,
                                                  d if out_head_stride is None else out_head_stride, _typed(lse_out, _F32, "lse_out")))
     return out

@@ -32,7 +32,8 @@ struct Rows4Args {
     uint32_t *to_pos, *to_doc;
     uint64_t entry_hs, to_entry_hs;
     const CacheSeg* table;
-    uint32_t n_segs, n_kv, units, entries, each;  // units: of 8 elements a row of a head; entries: heads whose entries are laid out; each: rows of a work item
+    uint32_t n_segs, n_kv, d, entries;                                      // entries: heads whose entries are laid out
+    uint32_t each, units, columns, passes, step, per_column, per_unit;  // rows of a work item and what a thread takes of them, see cache4_rows.cu
 };
 // One call's heads: strides in bytes.
 struct RotateArgs {
@@ -43,8 +44,8 @@ struct RotateArgs {
     const uint8_t* axes;
     const uint32_t *positions, *counts;
     const CacheSeg* table;
-    float eps, magnitude;
-    uint32_t n_segs, n_heads, n_kv, d, rotary, n_axes, n_tokens;
+    float eps, magnitude, per_dim;  // per_dim: 1 / d
+    uint32_t n_segs, n_heads, n_kv, d, rotary, n_axes, n_tokens, each;  // each: tokens of a work item
     int32_t norm, interleaved;
 };
 

@@ -826,7 +826,7 @@ Status attend_laid_out(Ctx* c, const CacheArgs& args, const Rows4& r, int dtype,
         x.to_entry_hs = b.rows;
         x.entries = entries;
         x.n_kv = args.n_kv;
-        x.units = args.d / 8;
+        x.d = args.d;
         SLHA_TRY(launch_read_cache4(c, x, dtype, of, to));
         CacheArgs a = args;
         a.keys = x.rows.p[0];

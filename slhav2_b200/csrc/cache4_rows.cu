@@ -1,10 +1,12 @@
 // Rows of keys and values into 4 bits and back (slha_b200_write_cache4, slha_b200_read_cache4, and the rows that attention by many tokens has laid out).
 //
 // Of a block of 16 elements x of a row of a head, with e the cache's exponent:  s = e4m3(max |x| / (6 2^e)),  code = e2m1(x / (s 2^e)),  value = code s 2^e.
-// A quotient is rounded once more where it becomes 3 bits: where its own rounding could land it on the border of two codes that x does not lie on, the last bit says
-// that something was cut off (rounding to odd), so that every code and scale is what the formula gives in exact arithmetic.
+// A quotient is rounded once more where it becomes 3 bits, so its own rounding must not land it on the border of two codes, or beside one that x lies on.  bfloat16: x / s, of 8 bits and of 4, is a
+// border or 2^-8 of it away; times 1 / s as the sum of two float32 it comes out on the border exactly.  float32: the quotient's last bit says whether something was cut off (rounding to
+// odd).  So every code and scale is what the formula gives in exact arithmetic.
 //
-// Bound by bytes, 2 or 4 in for 9/16 out an element: a thread takes 8 elements (16 bytes of bfloat16, 4 of codes), four such units of a work item are under way at a time.
+// Bytes bound it, 2 or 4 in for 9/16 out an element, once few instructions do: a thread takes 8 elements (16 bytes of bfloat16, 4 of codes) of one column of the rows' elements, and its addresses
+// grow by a constant; four such units are under way at a time.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -15,26 +17,19 @@
 namespace slha {
 namespace {
 
-constexpr int ROW_THREADS = 256, FLIGHT = 4;
+constexpr int ROW_THREADS = 256, FLIGHT = 4, WRITE_FLIGHT = 2;  // units under way at a time: reading, of 8 elements, writing, of 16
 
-// Unit u of a work item, counted through its rows, heads and units of 8 elements, in steps of the block's threads.
-struct UnitWalk {
-    uint32_t r, h, x, dr, dh, dx, kv, units;
-    __device__ __forceinline__ UnitWalk(uint32_t first, uint32_t step, uint32_t kv_, uint32_t units_) : kv(kv_), units(units_) {
-        const uint32_t h_all = first / units, dh_all = step / units;
-        x = first - h_all * units;
-        r = h_all / kv;
-        h = h_all - r * kv;
-        dx = step - dh_all * units;
-        dr = dh_all / kv;
-        dh = dh_all - dr * kv;
-    }
-    __device__ __forceinline__ void next() {
-        x += dx;
-        h += dh;
-        r += dr;
-        if (x >= units) x -= units, ++h;
-        if (h >= kv) h -= kv, ++r;
+// A thread's part of a work item: a column of the rows' kv x units units (the `pass`-th of its columns; threads beyond them have none), and every step-th row from `row` on.  What is divided by is
+// known to the host: below 256, x / y is x * ceil(2^16 / y) / 2^16.
+struct Column {
+    uint32_t row, head, unit;
+    bool there;
+    __device__ __forceinline__ Column(const Rows4Args& a, uint32_t pass) {
+        row = a.passes == 1 ? threadIdx.x * a.per_column >> 16 : 0;
+        const uint32_t column = pass * ROW_THREADS + threadIdx.x - row * a.columns;
+        there = row < a.step && column < a.columns;
+        head = !there ? 0 : a.passes == 1 ? column * a.per_unit >> 16 : column / a.units;
+        unit = there ? column - head * a.units : 0;
     }
 };
 // x / y (y > 0) to the nearest, for r the nearest to 1 / y: Markstein's two steps, exact remainders by fused multiply-add.
@@ -50,35 +45,39 @@ __device__ __forceinline__ float to_odd(float q, float x, float y) {
     if (rest != 0.0f) b |= 1;
     return __uint_as_float(b);
 }
-// Bit patterns of 8 elements of T as float32.
+// A block of 16 elements of T as they lie.
 template <typename T>
-struct Eight {
-    uint4 w[sizeof(T) / 2];
+struct Block16 {
+    uint4 w[sizeof(T)];
     __device__ __forceinline__ void load(const unsigned char* p) {
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
+        for (int i = 0; i < (int)sizeof(T); ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
     }
-    __device__ __forceinline__ void clear() {
-#pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = make_uint4(0, 0, 0, 0);
-    }
-    __device__ __forceinline__ void values(float (&f)[8]) const {
+    // elements 4 i .. 4 i + 3
+    __device__ __forceinline__ void four(int i, float (&f)[4]) const {
         if constexpr (sizeof(T) == 2) {
-            const uint32_t x[4] = {w[0].x, w[0].y, w[0].z, w[0].w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) f[2 * i] = __uint_as_float(x[i] << 16), f[2 * i + 1] = __uint_as_float(x[i] & 0xFFFF0000u);
+            const uint32_t x = i & 1 ? w[i / 2].z : w[i / 2].x, y = i & 1 ? w[i / 2].w : w[i / 2].y;
+            f[0] = __uint_as_float(x << 16), f[1] = __uint_as_float(x & 0xFFFF0000u), f[2] = __uint_as_float(y << 16), f[3] = __uint_as_float(y & 0xFFFF0000u);
         } else {
-            const uint32_t x[8] = {w[0].x, w[0].y, w[0].z, w[0].w, w[1].x, w[1].y, w[1].z, w[1].w};
+            f[0] = __uint_as_float(w[i].x), f[1] = __uint_as_float(w[i].y), f[2] = __uint_as_float(w[i].z), f[3] = __uint_as_float(w[i].w);
+        }
+    }
+    // the largest size, as the bits of a float32
+    __device__ __forceinline__ uint32_t largest() const {
+        if constexpr (sizeof(T) == 2) {
+            uint32_t m = 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(x[i]);
+            for (int i = 0; i < 2; ++i)
+                m = __vmaxu2(m, __vmaxu2(__vmaxu2(w[i].x & 0x7FFF7FFFu, w[i].y & 0x7FFF7FFFu), __vmaxu2(w[i].z & 0x7FFF7FFFu, w[i].w & 0x7FFF7FFFu)));
+            return max(m << 16, m & 0xFFFF0000u);
+        } else {
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m = max(m, max(max(w[i].x & 0x7FFFFFFFu, w[i].y & 0x7FFFFFFFu), max(w[i].z & 0x7FFFFFFFu, w[i].w & 0x7FFFFFFFu)));
+            return m;
         }
     }
 };
-__device__ __forceinline__ uint32_t e2m1_pack(float lo, float hi) {
-    uint32_t r;
-    asm("{\n.reg .b8 b;\ncvt.rn.satfinite.e2m1x2.f32 b, %1, %2;\ncvt.u32.u8 %0, b;\n}\n" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
 __device__ __forceinline__ uint32_t e4m3_of(float x) {
     uint16_t r;
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;\n" : "=h"(r) : "f"(0.0f), "f"(x));
@@ -86,38 +85,53 @@ __device__ __forceinline__ uint32_t e4m3_of(float x) {
 }
 __device__ __forceinline__ float e4m3_value(uint32_t byte) { return __half2float(__ushort_as_half((uint16_t)(e4m3_pair(byte) & 0xFFFF))); }
 
-// 8 elements, half a block (the other half is the neighbouring lane's): their codes and the block's scale.
+// 1 / s to the nearest, for the scales' significands of 4 bits: two steps from an approximation.
+__device__ __forceinline__ float inverse(float s) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(s));
+    r = fmaf(fmaf(-s, r, 1.0f), r, r);
+    return fmaf(fmaf(-s, r, 1.0f), r, r);
+}
+// A block's codes and scale.  down = 2^-e, up = 2^e.
 template <typename T>
-__device__ __forceinline__ uint32_t quantise(const Eight<T>& in, float down, uint32_t* scale) {
-    float x[8];
-    in.values(x);
-    uint32_t most = 0;
+__device__ __forceinline__ uint2 quantise(const Block16<T>& in, float down, float up, uint32_t* scale) {
+    const uint32_t most = in.largest();
+    constexpr float SIXTH = 1.0f / 6.0f, BEYOND = 8192.0f;  // (what is larger takes the largest scale and code)
+    const float size = fminf(__uint_as_float(most) * down, BEYOND);
+    // (a bfloat16's sixth needs no more: checked for every significand of a tie, the product with 1 / 6 comes out on it)
+    *scale = e4m3_of(sizeof(T) == 2 ? size * SIXTH : to_odd(quotient(size, 6.0f, SIXTH), size, 6.0f));
+    // (the scale's exponent apart: 1 / s within what an approximation takes)
+    const float held = e4m3_value(*scale), s = held * up, r = held > 0.0f ? inverse(held) * down : 0.0f, rest = sizeof(T) == 2 ? fmaf(-s, r, 1.0f) * r : 0.0f;  // 1 / s = r + rest
+    const float limit = BEYOND * up;
+    const bool beyond = size == BEYOND;
+    uint32_t codes[2];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(x[i]) & 0x7FFFFFFFu);
-    most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
-    if (most > 0x7F800000u) {  // a NaN
-        *scale = 0x7F;
-        return 0;
-    }
-    constexpr float SIXTH = 1.0f / 6.0f, LARGEST = 3.0e38f;
-    const float size = fminf(__uint_as_float(most) * down, LARGEST);
-    *scale = e4m3_of(to_odd(quotient(size, 6.0f, SIXTH), size, 6.0f));
-    const float s = e4m3_value(*scale), r = s > 0.0f ? __frcp_rn(s) : 0.0f;
-    uint32_t codes = 0;
+    for (int i = 0; i < 2; ++i) {
+        float q[8];
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-        float q[2];
+        for (int h = 0; h < 2; ++h) {
+            float x[4];
+            in.four(2 * i + h, x);
+            if (beyond)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const float y = fminf(fabsf(x[i + j] * down), LARGEST);
-            q[j] = quotient(y, s, r);
-            // (a bfloat16's quotient by the 4 bits of a scale lies on a border, of at most 3 bits, or 2^-8 of it away)
-            if constexpr (sizeof(T) == 4) q[j] = to_odd(q[j], y, s);
-            q[j] = copysignf(q[j], x[i + j]);
+                for (int e = 0; e < 4; ++e) x[e] = fminf(fmaxf(x[e], -limit), limit);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if constexpr (sizeof(T) == 2) {
+                    q[4 * h + e] = fmaf(x[e], r, x[e] * rest);
+                } else {
+                    const float y = fabsf(x[e]);
+                    q[4 * h + e] = copysignf(to_odd(quotient(y, s, r), y, s), x[e]);
+                }
+            }
         }
-        codes |= e2m1_pack(q[0], q[1]) << (4 * i);
+        asm("{\n.reg .b8 a, b, c, d;\ncvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\ncvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\ncvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n"
+            "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\nmov.b32 %0, {a, b, c, d};\n}\n"
+            : "=r"(codes[i]) : "f"(q[0]), "f"(q[1]), "f"(q[2]), "f"(q[3]), "f"(q[4]), "f"(q[5]), "f"(q[6]), "f"(q[7]));
     }
-    return codes;
+    if (most <= 0x7F800000u) return make_uint2(codes[0], codes[1]);
+    *scale = 0x7F;  // a NaN
+    return make_uint2(0, 0);
 }
 
 template <typename T>
@@ -130,27 +144,27 @@ __global__ void __launch_bounds__(ROW_THREADS) write_cache4_kernel(const __grid_
     const uint32_t t0 = (blockIdx.x - sg.item_begin) * a.each;  // (below n_queries)
     const uint32_t tokens = min(min(a.each, sg.n_queries - t0), n - ctx - min(n - ctx, t0));
     const int v = blockIdx.y;
-    const unsigned char* from = a.rows.p[v] + (uint64_t)(sg.query_begin + t0) * a.rows.rs[v];
-    unsigned char* codes = const_cast<unsigned char*>(a.in4.codes[v]) + (sg.row_begin + ctx + t0) * a.in4.crs;
-    unsigned char* scales = const_cast<unsigned char*>(a.in4.scales[v]) + (sg.row_begin + ctx + t0) * a.in4.srs;
-    const float down = exp2f((float)-a.in4.exponent[v]);
-    UnitWalk u(threadIdx.x, ROW_THREADS, a.n_kv, a.units);
-    // (the two halves of a block are neighbours: the number of units is even, and so are a warp's first and the step)
-    while (__any_sync(0xFFFFFFFFu, u.r < tokens)) {
-        UnitWalk w = u;
-        Eight<T> in[FLIGHT];
+    const float down = exp2f((float)-a.in4.exponent[v]), up = exp2f((float)a.in4.exponent[v]);
+    const uint32_t step = a.step;  // (in a register: read from the parameters each time the loop was unrolled another way, a fifth slower)
+    for (uint32_t pass = 0; pass < a.passes; ++pass) {
+        const Column u(a, pass);
+        if (!u.there) continue;
+        const unsigned char* from = a.rows.p[v] + (sg.query_begin + t0 + u.row) * a.rows.rs[v] + u.head * a.rows.hs[v] + u.unit * (16 * sizeof(T));
+        const uint64_t at = sg.row_begin + ctx + t0 + u.row, from_step = step * a.rows.rs[v], code_step = step * a.in4.crs, scale_step = step * a.in4.srs;
+        unsigned char* codes = const_cast<unsigned char*>(a.in4.codes[v]) + at * a.in4.crs + u.head * a.in4.chs + u.unit * 8;
+        unsigned char* scales = const_cast<unsigned char*>(a.in4.scales[v]) + at * a.in4.srs + u.head * a.in4.shs + u.unit;
+        for (uint32_t r = u.row; r < tokens; r += WRITE_FLIGHT * step) {
+            Block16<T> in[WRITE_FLIGHT];
 #pragma unroll
-        for (int i = 0; i < FLIGHT; ++i, w.next()) {
-            if (w.r < tokens) in[i].load(from + w.r * a.rows.rs[v] + w.h * a.rows.hs[v] + w.x * (8 * sizeof(T)));
-            else in[i].clear();
-        }
+            for (int i = 0; i < WRITE_FLIGHT; ++i, from += from_step)
+                if (r + i * step < tokens) in[i].load(from);
 #pragma unroll
-        for (int i = 0; i < FLIGHT; ++i, u.next()) {
-            uint32_t scale;
-            const uint32_t code = quantise<T>(in[i], down, &scale);
-            if (u.r >= tokens) continue;
-            *reinterpret_cast<uint32_t*>(codes + u.r * a.in4.crs + u.h * a.in4.chs + u.x * 4) = code;
-            if (!(u.x & 1)) scales[u.r * a.in4.srs + u.h * a.in4.shs + u.x / 2] = (unsigned char)scale;
+            for (int i = 0; i < WRITE_FLIGHT; ++i, codes += code_step, scales += scale_step) {
+                if (r + i * step >= tokens) break;
+                uint32_t scale;
+                *reinterpret_cast<uint2*>(codes) = quantise<T>(in[i], down, up, &scale);
+                *scales = (unsigned char)scale;
+            }
         }
     }
 }
@@ -177,46 +191,59 @@ __global__ void __launch_bounds__(ROW_THREADS) read_cache4_kernel(const __grid_c
                 if (a.doc) a.to_doc[to] = a.doc[at];
             }
     if (!a.rows.p[v]) return;
-    const unsigned char* codes = a.in4.codes[v] + (sg.row_begin + r0) * a.in4.crs;
-    const unsigned char* scales = a.in4.scales[v] + (sg.row_begin + r0) * a.in4.srs;
-    unsigned char* to = const_cast<unsigned char*>(a.rows.p[v]) + (sg.to_begin + r0) * a.rows.rs[v];
     const float up = exp2f((float)a.in4.exponent[v]);
-    UnitWalk u(threadIdx.x, ROW_THREADS, a.n_kv, a.units);
-    while (u.r < rows) {
-        UnitWalk w = u;
-        uint32_t code[FLIGHT], scale[FLIGHT];
+    const uint32_t step = a.step;
+    for (uint32_t pass = 0; pass < a.passes; ++pass) {
+        const Column u(a, pass);
+        if (!u.there) continue;
+        const uint64_t at = sg.row_begin + r0 + u.row, to_step = step * a.rows.rs[v], code_step = step * a.in4.crs, scale_step = step * a.in4.srs;
+        const unsigned char* codes = a.in4.codes[v] + at * a.in4.crs + u.head * a.in4.chs + u.unit * 4;
+        const unsigned char* scales = a.in4.scales[v] + at * a.in4.srs + u.head * a.in4.shs + u.unit / 2;
+        unsigned char* to = const_cast<unsigned char*>(a.rows.p[v]) + (sg.to_begin + r0 + u.row) * a.rows.rs[v] + u.head * a.rows.hs[v] + u.unit * (8 * sizeof(T));
+        for (uint32_t r = u.row; r < rows; r += FLIGHT * step) {
+            uint32_t code[FLIGHT], scale[FLIGHT];
 #pragma unroll
-        for (int i = 0; i < FLIGHT; ++i, w.next()) {
-            const bool there = w.r < rows;
-            code[i] = there ? *reinterpret_cast<const uint32_t*>(codes + w.r * a.in4.crs + w.h * a.in4.chs + w.x * 4) : 0;
-            scale[i] = there ? scales[w.r * a.in4.srs + w.h * a.in4.shs + w.x / 2] : 0;
-        }
-#pragma unroll
-        for (int i = 0; i < FLIGHT; ++i, u.next()) {
-            if (u.r >= rows) break;
-            const uint32_t s = e4m3_pair((scale[i] & 0x7F) * 0x0101u);
-            const uint32_t h[4] = {mul_f16x2(e2m1_pair<0>(code[i]), s), mul_f16x2(e2m1_pair<1>(code[i]), s), mul_f16x2(e2m1_pair<2>(code[i]), s), mul_f16x2(e2m1_pair<3>(code[i]), s)};
-            float f[8];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                f[2 * j] = __half2float(__ushort_as_half((uint16_t)h[j])) * up;
-                f[2 * j + 1] = __half2float(__ushort_as_half((uint16_t)(h[j] >> 16))) * up;
+            for (int i = 0; i < FLIGHT; ++i, codes += code_step, scales += scale_step) {
+                const bool there = r + i * step < rows;
+                code[i] = there ? *reinterpret_cast<const uint32_t*>(codes) : 0;
+                scale[i] = there ? *scales : 0;
             }
-            uint4* dst = reinterpret_cast<uint4*>(to + u.r * a.rows.rs[v] + u.h * a.rows.hs[v] + u.x * (8 * sizeof(T)));
-            if constexpr (sizeof(T) == 2) {
-                *dst = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
-            } else {
-                dst[0] = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
-                dst[1] = make_uint4(__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7]));
+#pragma unroll
+            for (int i = 0; i < FLIGHT; ++i, to += to_step) {
+                if (r + i * step >= rows) break;
+                const float s = e4m3_value(scale[i] & 0x7F) * up;
+                const uint32_t h[4] = {e2m1_pair<0>(code[i]), e2m1_pair<1>(code[i]), e2m1_pair<2>(code[i]), e2m1_pair<3>(code[i])};
+                float f[8];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
+                    f[2 * j] = x.x * s;
+                    f[2 * j + 1] = x.y * s;
+                }
+                uint4* dst = reinterpret_cast<uint4*>(to);
+                if constexpr (sizeof(T) == 2) {
+                    *dst = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+                } else {
+                    dst[0] = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+                    dst[1] = make_uint4(__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7]));
+                }
             }
         }
     }
 }
 
-// Rows of a work item: about FLIGHT units a thread, more where that would be more work items than a grid takes.
+// Rows of a work item: what is under way at a time, up to eight times as many where that leaves 8 work items an SM (16 of writing), more where there would be more than a grid takes.
 Status cut_rows(Ctx* c, Rows4Args* a, std::vector<CacheSeg>* segs, bool write, CacheTable* tab, uint32_t* items) {
-    const uint32_t per_row = a->n_kv * a->units;
-    uint64_t each = std::max(1u, ROW_THREADS * FLIGHT / per_row), count;
+    uint64_t rows = 0, count;
+    for (const CacheSeg& s : *segs) rows += write ? s.n_queries : s.n_rows;
+    a->units = a->d / (write ? 16 : 8);
+    a->columns = a->n_kv * a->units;
+    a->passes = (a->columns + ROW_THREADS - 1) / ROW_THREADS;
+    a->step = std::max(1u, ROW_THREADS / a->columns);
+    a->per_column = (65536 + a->columns - 1) / a->columns;
+    a->per_unit = (65536 + a->units - 1) / a->units;
+    const uint64_t least = (uint64_t)a->step * (write ? WRITE_FLIGHT : FLIGHT);
+    uint64_t each = least * std::min<uint64_t>(std::max<uint64_t>(rows / (least * (write ? 16 : 8) * sm_count(c->device)), 1), 8);
     for (;; each *= 2) {
         count = 0;
         for (CacheSeg& s : *segs) {

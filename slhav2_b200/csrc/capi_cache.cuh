@@ -5,10 +5,14 @@
 namespace {
 
 // Memory that kernels of the calling thread's device read or write in place.
-Status cache_device_memory(Ctx* c, const void* p, const char* fn, const char* what) {
+Status cache_device_memory(Ctx* c, const void* p, const char* fn, const char* what, bool* host = nullptr) {
     cudaPointerAttributes at;
     const bool known = cudaPointerGetAttributes(&at, p) == cudaSuccess;
     if (!known) cudaGetLastError();
+    if (host) {  // (asked for: memory of the host is no fault)
+        *host = !known || (at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged);
+        if (*host) return Status();
+    }
     if (!known || (at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged))
         return Status(SLHA_ERR_DEVICE, std::string(fn) + ": " + what + " must be device memory");
     if (at.type == cudaMemoryTypeDevice && at.device != c->device)
@@ -20,7 +24,9 @@ template <typename T>
 Status cache_stage(Ctx* c, const T* p, size_t n, const T** dev, const char* fn, const char* what) {
     *dev = p;
     if (!p || !n) return Status();
-    if (is_device_ptr(p)) return cache_device_memory(c, p, fn, what);
+    bool host;
+    SLHA_TRY(cache_device_memory(c, p, fn, what, &host));
+    if (!host) return Status();
     void* d;
     SLHA_TRY(ctx_upload(c, p, n * sizeof(T), &d));
     *dev = static_cast<const T*>(d);

@@ -182,7 +182,7 @@ int32_t slha_b200_write_cache4(const SlhaB200KvCache4* cache, const SlhaB200Segm
         a.rows = rows_of(from);
         SLHA_TRY(cache_stage(c, cache->rows, n_segments, &a.counts, fn, "rows"));
         a.n_kv = cache->n_kv_heads;
-        a.units = cache->head_dim / 8;
+        a.d = cache->head_dim;
         SLHA_TRY(launch_write_cache4(c, a, from->dtype, segs));
         if (sync_by_default(c)) SLHA_CUDA(cudaStreamSynchronize(c->stream));
         return Status();
@@ -226,7 +226,7 @@ int32_t slha_b200_read_cache4(const SlhaB200KvCache4* cache, const SlhaB200Segme
         a.rows = rows_of(to);
         SLHA_TRY(cache_stage(c, cache->rows, n_segments, &a.counts, fn, "rows"));
         a.n_kv = cache->n_kv_heads;
-        a.units = cache->head_dim / 8;
+        a.d = cache->head_dim;
         SLHA_TRY(launch_read_cache4(c, a, to->dtype, segs, to_segs));
         if (sync_by_default(c)) SLHA_CUDA(cudaStreamSynchronize(c->stream));
         return Status();

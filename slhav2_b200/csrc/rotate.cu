@@ -4,8 +4,9 @@
 // The angle is taken in turns and in float64, t / 2 pi less the nearest integer: positions of 2^32 keep 2^-23 of a turn.  Its cosine and sine are float32, one pair of them a token for all
 // heads.
 //
-// Bound by bytes, every head read and written once.  A block takes a token; 8, 16 or 32 lanes take a head, 8 elements each: four pairs (two 8- or 16-byte loads, half a rotation apart) or,
-// of interleaved pairs and what is not turned, 8 elements side by side.  No element is read by another lane than the one that writes it, so that heads may be turned in place.
+// Bytes bound it, every head read and written once, once few instructions do: 8, 16 or 32 lanes take a head, 8 elements each: four pairs (two 8- or 16-byte loads, half a rotation apart) or, of
+// interleaved pairs and what is not turned, 8 elements side by side.  A group of lanes takes a head of a block's tokens, four of them at a time, so that its addresses grow by a constant and its
+// weights stay in registers; then its next head.  No element is read by another lane than the one that writes it, so that heads may be turned in place.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -15,7 +16,7 @@
 namespace slha {
 namespace {
 
-constexpr int ROT_THREADS = 256, ROT_FLIGHT = 3;  // heads under way at a time for each group of lanes
+constexpr int ROT_THREADS = 256, ROT_FLIGHT = 4, ROT_TOKENS = 8;  // tokens under way at a time, and most of a block
 constexpr double PER_TURN = 0.15915494309189533577;  // 1 / (2 pi)
 
 template <typename T>
@@ -69,111 +70,96 @@ struct HeadUnit {  // 8 elements as they lie: two times 4
 template <typename T, int LANES>
 __global__ void __launch_bounds__(ROT_THREADS) rotate_heads_kernel(const __grid_constant__ RotateArgs a, const __grid_constant__ CacheTable tab) {
     dep_wait();
-    __shared__ float s_cos[CACHE_DIM_MOST / 2], s_sin[CACHE_DIM_MOST / 2];
+    __shared__ __align__(16) float2 s_turn[ROT_TOKENS][CACHE_DIM_MOST / 2];  // cosine and sine
     const CacheSeg* table = a.table ? a.table : tab.s;
     const uint32_t seg = cache_find(a.n_segs, blockIdx.x, [&](uint32_t i) { return table[i].item_begin; });
     const CacheSeg& sg = table[seg];
-    const uint32_t t = blockIdx.x - sg.item_begin, tok = sg.query_begin + t;
+    const uint32_t t0 = (blockIdx.x - sg.item_begin) * a.each, tokens = min(a.each, sg.n_queries - t0), tok0 = sg.query_begin + t0;
     const uint32_t n = a.counts ? min(a.counts[sg.seg], sg.n_rows) : sg.n_rows, ctx = n - min(n, sg.n_queries);
-    const bool placed = ctx + t < n;  // the token has a row
-    const uint64_t row = sg.row_begin + ctx + t;
-    const uint32_t nq = a.q ? a.n_heads : 0, nk = a.k && placed ? a.n_kv : 0, nv = a.v && placed ? a.n_kv : 0, all = nq + nk + nv;
+    const uint32_t placed = min(tokens, n - ctx - min(n - ctx, t0));  // the tokens that have a row
+    const uint64_t row0 = sg.row_begin + ctx + t0;
+    const uint32_t nq = a.q ? a.n_heads : 0, nk = a.k ? a.n_kv : 0, nv = a.v ? a.n_kv : 0, all = nq + nk + nv;
 
     const uint32_t x = threadIdx.x % LANES, group = threadIdx.x / LANES, groups = blockDim.x / LANES;
-    const bool mine = x < a.d / 8;
-    const bool turned = x < a.rotary / 8, apart = turned && !a.interleaved;
+    const bool mine = x < a.d / 8, turned = x < a.rotary / 8, apart = turned && !a.interleaved;
     const uint32_t first = apart ? 4 * x : 8 * x, second = apart ? a.rotary / 2 + 4 * x : 8 * x + 4;
-    const auto from = [&](uint32_t i) {
-        return i < nq ? a.q + tok * a.qts + i * a.qhs : i < nq + nk ? a.k + tok * a.kts + (i - nq) * a.khs : a.v + tok * a.vts + (i - nq - nk) * a.vhs;
-    };
-    const auto to = [&](uint32_t i) {
-        return i < nq ? a.q_out + tok * a.qots + i * a.qohs : i < nq + nk ? a.k_out + row * a.kors + (i - nq) * a.kohs : a.v_out + row * a.vors + (i - nq - nk) * a.vohs;
-    };
-    HeadUnit<T> in[ROT_FLIGHT];
-    const auto fetch = [&](uint32_t i0) {
-#pragma unroll
-        for (int j = 0; j < ROT_FLIGHT; ++j) {
-            const uint32_t i = i0 + j * groups;
-            if (i < all && mine) {
-                const unsigned char* p = from(i);
-                in[j].load(p + first * sizeof(T), p + second * sizeof(T), apart);
-            }
-        }
-    };
-    fetch(group);
-    for (uint32_t p = threadIdx.x; p < a.rotary / 2; p += blockDim.x) {
-        const uint32_t axis = a.axes ? min((uint32_t)a.axes[p], a.n_axes - 1) : 0;
-        const double turns = (double)a.positions[(uint64_t)axis * a.n_tokens + tok] * (double)a.freq[p] * PER_TURN;
+
+    for (uint32_t i = threadIdx.x; i < tokens * (a.rotary / 2); i += blockDim.x) {
+        const uint32_t t = i / (a.rotary / 2), p = i % (a.rotary / 2), axis = a.axes ? min((uint32_t)a.axes[p], a.n_axes - 1) : 0;
+        const double turns = (double)a.positions[(uint64_t)axis * a.n_tokens + tok0 + t] * (double)a.freq[p] * PER_TURN;
         float s, c;
         sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
-        s_cos[p] = c * a.magnitude;
-        s_sin[p] = s * a.magnitude;
+        s_turn[t][p] = make_float2(c * a.magnitude, s * a.magnitude);
     }
     __syncthreads();
-    float cs[4], sn[4];
-    if (turned) {
+    // (a warp's groups go through the loops together: sums are taken over a group's lanes)
+    for (uint32_t i = blockIdx.y * groups + group; __any_sync(0xFFFFFFFFu, i < all); i += gridDim.y * groups) {
+        const bool q = i < nq, k = !q && i < nq + nk, value = !q && !k;
+        const uint32_t h = q ? i : k ? i - nq : i - nq - nk, last = i >= all || !mine ? 0 : q ? tokens : placed;  // last: tokens whose head is written
+        const uint64_t step = q ? a.qts : k ? a.kts : a.vts, to_step = q ? a.qots : k ? a.kors : a.vors;
+        const unsigned char* from = (q ? a.q + h * a.qhs : k ? a.k + h * a.khs : a.v + h * a.vhs) + tok0 * step;
+        unsigned char* to = (q ? a.q_out + h * a.qohs : k ? a.k_out + h * a.kohs : a.v_out + h * a.vohs) + (q ? tok0 : row0) * to_step;
+        const float* weight = q ? a.q_weight : k ? a.k_weight : nullptr;
+        float w[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) cs[i] = s_cos[4 * x + i], sn[i] = s_sin[4 * x + i];
-    }
-    // (a warp's groups go through the loop together: sums are taken over a group's lanes)
-    for (uint32_t i0 = group; __any_sync(0xFFFFFFFFu, i0 < all); i0 += ROT_FLIGHT * groups) {
-        if (i0 != group) fetch(i0);
+        for (int e = 0; e < 8; ++e) w[e] = weight && last ? weight[e < 4 ? first + e : second + e - 4] : 1.0f;
+        for (uint32_t t = 0; t < tokens; t += ROT_FLIGHT) {
+            HeadUnit<T> in[ROT_FLIGHT];
 #pragma unroll
-        for (int j = 0; j < ROT_FLIGHT; ++j) {
-            const uint32_t i = i0 + j * groups;
-            const bool there = i < all && mine;
-            float f[8];
-            if (a.norm) {
-                float sum = 0.0f;
-                if (there) {
-                    in[j].get(f);
+            for (int j = 0; j < ROT_FLIGHT; ++j, from += step)
+                if (t + j < last) in[j].load(from + first * sizeof(T), from + second * sizeof(T), apart);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) sum = fmaf(f[e], f[e], sum);
-                }
+            for (int j = 0; j < ROT_FLIGHT; ++j, to += to_step) {
+                if (t + j >= tokens) break;
+                const bool there = t + j < last;
+                if (!value || a.norm) {  // (values go through the sums over the lanes: their neighbours' heads may be keys)
+                    float f[8], factor = 1.0f;
+                    if (there) in[j].get(f);
+                    if (a.norm) {
+                        float sum = 0.0f;
+                        if (there) {
 #pragma unroll
-                for (int m = LANES / 2; m; m >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, m);
-                if (!there) continue;
-                if (i < nq + nk) {
-                    const float factor = rsqrtf(sum / (float)a.d + a.eps);
-                    const float* weight = i < nq ? a.q_weight : a.k_weight;
+                            for (int e = 0; e < 8; ++e) sum = fmaf(f[e], f[e], sum);
+                        }
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) f[e] *= factor;
-                    if (weight) {
-                        const float4 u = *reinterpret_cast<const float4*>(weight + first), v = *reinterpret_cast<const float4*>(weight + second);
-                        f[0] *= u.x, f[1] *= u.y, f[2] *= u.z, f[3] *= u.w, f[4] *= v.x, f[5] *= v.y, f[6] *= v.z, f[7] *= v.w;
+                        for (int m = LANES / 2; m; m >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, m);
+                        factor = rsqrtf(sum * a.per_dim + a.eps);
+                    }
+                    if (there && !value) {
+                        if (a.norm) {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) f[e] = f[e] * factor * w[e];
+                        }
+                        if (turned) {
+                            const float4 c01 = *reinterpret_cast<const float4*>(&s_turn[t + j][4 * x]), c23 = *reinterpret_cast<const float4*>(&s_turn[t + j][4 * x + 2]);
+                            const auto turn = [&](float& u, float& v, float c, float s) {
+                                const float one = fmaf(u, c, -v * s);
+                                v = fmaf(u, s, v * c);
+                                u = one;
+                            };
+                            if (apart) {
+                                turn(f[0], f[4], c01.x, c01.y), turn(f[1], f[5], c01.z, c01.w), turn(f[2], f[6], c23.x, c23.y), turn(f[3], f[7], c23.z, c23.w);
+                            } else {
+                                turn(f[0], f[1], c01.x, c01.y), turn(f[2], f[3], c01.z, c01.w), turn(f[4], f[5], c23.x, c23.y), turn(f[6], f[7], c23.z, c23.w);
+                            }
+                        }
+                        in[j].set(f);
                     }
                 }
-            } else {
-                if (!there) continue;
-                in[j].get(f);
+                if (there) in[j].store(to + first * sizeof(T), to + second * sizeof(T), apart);  // (values as they are, NaN too)
             }
-            const auto turn = [&](float& u, float& v, int e) {
-                const float one = fmaf(u, cs[e], -v * sn[e]);
-                v = fmaf(u, sn[e], v * cs[e]);
-                u = one;
-            };
-            if (turned && i < nq + nk) {
-                if (apart) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) turn(f[e], f[4 + e], e);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) turn(f[2 * e], f[2 * e + 1], e);
-                }
-            }
-            if (i < nq + nk) in[j].set(f);  // (values as they are, NaN too)
-            unsigned char* p = to(i);
-            in[j].store(p + first * sizeof(T), p + second * sizeof(T), apart);
         }
     }
 }
 
 template <typename T>
-Status launch_lanes(Ctx* c, const RotateArgs& a, const CacheTable& tab, uint32_t tokens) {
+Status launch_lanes(Ctx* c, const RotateArgs& a, const CacheTable& tab, uint32_t items) {
     const uint32_t lanes = a.d <= 64 ? 8 : a.d <= 128 ? 16 : 32, heads = (a.q ? a.n_heads : 0) + ((a.k != nullptr) + (a.v != nullptr)) * a.n_kv;
     const uint32_t threads = std::min<uint64_t>(ROT_THREADS, ((uint64_t)heads * lanes + 31) / 32 * 32);
     const auto kernel = lanes == 8 ? rotate_heads_kernel<T, 8> : lanes == 16 ? rotate_heads_kernel<T, 16> : rotate_heads_kernel<T, 32>;
-    SLHA_CUDA(launch_behind(kernel, dim3(tokens), dim3(threads), 0, c->stream, a, tab));
+    // few tokens: their heads go to as many blocks as they fill (one token of 48 heads: 3.4 us in three blocks, 4.4 in one)
+    const uint32_t at_once = threads / lanes, blocks = items < 2u * sm_count(c->device) ? std::min((heads + at_once - 1) / at_once, 64u) : 1;
+    SLHA_CUDA(launch_behind(kernel, dim3(items, blocks), dim3(threads), 0, c->stream, a, tab));
     count_launch();
     return Status();
 }
@@ -181,8 +167,13 @@ Status launch_lanes(Ctx* c, const RotateArgs& a, const CacheTable& tab, uint32_t
 }  // namespace
 
 Status launch_rotate_heads(Ctx* c, RotateArgs a, int dtype, const std::vector<SlhaB200Segment>& segs) {
+    uint64_t tokens = 0, items = 0;
+    for (const SlhaB200Segment& s : segs) tokens += s.n_queries;
+    if (!tokens) return Status();
+    // tokens of a block: up to eight, where that leaves six blocks an SM
+    a.each = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(tokens / (6 * sm_count(c->device)), 1), ROT_TOKENS);
+    a.per_dim = 1.0f / (float)a.d;
     std::vector<CacheSeg> of;
-    uint64_t tokens = 0;
     for (size_t i = 0; i < segs.size(); ++i) {
         if (!segs[i].n_queries) continue;
         CacheSeg g{};
@@ -190,17 +181,16 @@ Status launch_rotate_heads(Ctx* c, RotateArgs a, int dtype, const std::vector<Sl
         g.n_rows = segs[i].n_tiles;
         g.query_begin = segs[i].query_begin;
         g.n_queries = segs[i].n_queries;
-        g.item_begin = (uint32_t)tokens;
+        g.item_begin = (uint32_t)items;
         g.seg = (uint32_t)i;
-        tokens += g.n_queries;
+        items += ((uint64_t)g.n_queries + a.each - 1) / a.each;
         of.push_back(g);
     }
-    if (of.empty()) return Status();
-    if (tokens > 0x7FFFFFFFull) return Status(SLHA_ERR_CAPACITY, "slha_b200_rotate_heads: too many tokens");
+    if (items > 0x7FFFFFFFull) return Status(SLHA_ERR_CAPACITY, "slha_b200_rotate_heads: too many tokens");
     CacheTable tab;
     SLHA_TRY(cache_table(c, of, &tab, &a.table));
     a.n_segs = (uint32_t)of.size();
-    return dtype == SLHA_B200_BF16 ? launch_lanes<__nv_bfloat16>(c, a, tab, (uint32_t)tokens) : launch_lanes<float>(c, a, tab, (uint32_t)tokens);
+    return dtype == SLHA_B200_BF16 ? launch_lanes<__nv_bfloat16>(c, a, tab, (uint32_t)items) : launch_lanes<float>(c, a, tab, (uint32_t)items);
 }
 
 }  // namespace slha
