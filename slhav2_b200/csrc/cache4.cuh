@@ -10,7 +10,6 @@
 namespace slha {
 
 constexpr uint32_t BLOCK4 = 16;  // elements of a scale
-constexpr uint32_t CACHE4_QUERY_ROWS = 64;  // of a KV head, that are multiplied with rows as these are read
 // Bytes of the rows that a launch lays out for attention by many tokens (a segment's own may be more).
 constexpr uint64_t CACHE4_ROWS_MOST = 512ull << 20;
 

@@ -38,7 +38,7 @@ struct Shape4 {
     static constexpr uint32_t ROWS_AT = Q_AT + PARTS * Q_PART, LIST_AT = ROWS_AT + 5 * MB * 4, CLS_AT = LIST_AT + ROUND * 2, RANGE_AT = CLS_AT + ROUND, ML_AT = RANGE_AT + 32,
                               TREE_AT = ML_AT + 2 * WARPS * MB * 4;
     static constexpr uint32_t SMEM = TREE_AT, SMEM_TREE = TREE_AT + TREE_MOST * 8 + MB * (TREE_MOST / 8);
-    static constexpr int CTAS = D == 256 || NT == 4 ? 2 : NT == 1 ? 4 : 3;
+    static constexpr int CTAS = D == 256 || NT == 4 ? 2 : NT == 1 ? 4 : 3;  // of an SM
     static_assert(CTAS * (SMEM_TREE + 1024) <= 228 * 1024, "shared memory of an SM");
 };
 
@@ -158,47 +158,58 @@ __global__ void __launch_bounds__(ATT_THREADS, Shape4<T, D, NT>::CTAS) cache4_at
     const CacheRanges qr{s_range[0], s_range[1], s_range[2], s_range[3]};
     // The block's query rows into shared memory, a warp each (rows behind the last: zeros; they are not written).
     const auto take_queries = [&]() {
+        constexpr int CHUNKS = D / 128 > 0 ? D / 128 : 1, AT_ONCE = S::MB / WARPS < 4 ? S::MB / WARPS : 4;  // chunks of 4 elements a lane; rows whose loads are under way together
         const unsigned char* qbase = static_cast<const unsigned char*>(a.q);
-        for (int r = warp; r < S::MB; r += WARPS) {
-            constexpr int CHUNKS = D / 128 > 0 ? D / 128 : 1;  // of 4 elements a lane
-            const uint32_t row = row0 + r;
-            const uint64_t at = row < q_rows ? (sg.query_begin + row / a.group) * a.qts + (head * a.group + row % a.group) * a.qhs : 0;
-            float x[CHUNKS][4];
-            uint32_t most = 0;
-    #pragma unroll
-            for (int i = 0; i < CHUNKS; ++i) {
-                const uint32_t d = (lane + i * 32) * 4;
-                x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.0f;
-                if (row < q_rows && d < a.d) {
-                    if constexpr (sizeof(T) == 2) {
-                        const uint2 w = *reinterpret_cast<const uint2*>(qbase + (at + d) * 2);
-                        x[i][0] = __uint_as_float(w.x << 16), x[i][1] = __uint_as_float(w.x & 0xFFFF0000u), x[i][2] = __uint_as_float(w.y << 16), x[i][3] = __uint_as_float(w.y & 0xFFFF0000u);
-                    } else {
-                        const float4 w = *reinterpret_cast<const float4*>(qbase + (at + d) * 4);
-                        x[i][0] = w.x, x[i][1] = w.y, x[i][2] = w.z, x[i][3] = w.w;
+#pragma unroll 1
+        for (int r0 = warp * AT_ONCE; r0 < S::MB; r0 += WARPS * AT_ONCE) {
+            float x[AT_ONCE][CHUNKS][4];
+#pragma unroll
+            for (int j = 0; j < AT_ONCE; ++j) {
+                const uint32_t row = row0 + r0 + j;
+                const uint64_t at = row < q_rows ? (sg.query_begin + row / a.group) * a.qts + (head * a.group + row % a.group) * a.qhs : 0;
+#pragma unroll
+                for (int i = 0; i < CHUNKS; ++i) {
+                    const uint32_t d = (lane + i * 32) * 4;
+                    float(&y)[4] = x[j][i];
+                    y[0] = y[1] = y[2] = y[3] = 0.0f;
+                    if (row < q_rows && d < a.d) {
+                        if constexpr (sizeof(T) == 2) {
+                            const uint2 w = *reinterpret_cast<const uint2*>(qbase + (at + d) * 2);
+                            y[0] = __uint_as_float(w.x << 16), y[1] = __uint_as_float(w.x & 0xFFFF0000u), y[2] = __uint_as_float(w.y << 16), y[3] = __uint_as_float(w.y & 0xFFFF0000u);
+                        } else {
+                            const float4 w = *reinterpret_cast<const float4*>(qbase + (at + d) * 4);
+                            y[0] = w.x, y[1] = w.y, y[2] = w.z, y[3] = w.w;
+                        }
                     }
                 }
-    #pragma unroll
-                for (int e = 0; e < 4; ++e) most = max(most, __float_as_uint(x[i][e]) & 0x7FFFFFFFu);
             }
-            most = __reduce_max_sync(0xFFFFFFFFu, most);
-            // 2^k with k = 14 less the exponent of the largest; 1 where one is not finite
-            const int k = most >= 0x7F800000u ? 0 : min(14 - (int)(max(most >> 23, 1u) - 127u), 126);
-            const float up = __uint_as_float((uint32_t)(127 + k) << 23);
-            if (lane == 0) s_factor[r] = __uint_as_float((uint32_t)(127 - k) << 23);
-    #pragma unroll
-            for (int i = 0; i < CHUNKS; ++i) {
-                const uint32_t d = (lane + i * 32) * 4;
-                if (d >= D) continue;
-                const uint32_t to = S::Q_AT + ((d % (D / 4) / 4 * NT + r / 8) * 32 + r % 8 * 4 + d / (D / 4)) * 8;
-                float v[4];
-    #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = x[i][e] * up;
-                const uint32_t h0 = pack_f16(v[0], v[1]), h1 = pack_f16(v[2], v[3]);
-                *reinterpret_cast<uint2*>(sm + to) = make_uint2(h0, h1);
-                if constexpr (S::PARTS == 2) {
-                    const float2 f0 = unpack_f16(h0), f1 = unpack_f16(h1);
-                    *reinterpret_cast<uint2*>(sm + to + S::Q_PART) = make_uint2(pack_f16(v[0] - f0.x, v[1] - f0.y), pack_f16(v[2] - f1.x, v[3] - f1.y));
+#pragma unroll
+            for (int j = 0; j < AT_ONCE; ++j) {
+                const int r = r0 + j;
+                uint32_t most = 0;
+#pragma unroll
+                for (int i = 0; i < CHUNKS; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) most = max(most, __float_as_uint(x[j][i][e]) & 0x7FFFFFFFu);
+                most = __reduce_max_sync(0xFFFFFFFFu, most);
+                // 2^k with k = 14 less the exponent of the largest; 1 where one is not finite
+                const int k = most >= 0x7F800000u ? 0 : min(14 - (int)(max(most >> 23, 1u) - 127u), 126);
+                const float up = __uint_as_float((uint32_t)(127 + k) << 23);
+                if (lane == 0) s_factor[r] = __uint_as_float((uint32_t)(127 - k) << 23);
+#pragma unroll
+                for (int i = 0; i < CHUNKS; ++i) {
+                    const uint32_t d = (lane + i * 32) * 4;
+                    if (d >= D) continue;
+                    const uint32_t to = S::Q_AT + ((d % (D / 4) / 4 * NT + r / 8) * 32 + r % 8 * 4 + d / (D / 4)) * 8;
+                    float v[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = x[j][i][e] * up;
+                    const uint32_t h0 = pack_f16(v[0], v[1]), h1 = pack_f16(v[2], v[3]);
+                    *reinterpret_cast<uint2*>(sm + to) = make_uint2(h0, h1);
+                    if constexpr (S::PARTS == 2) {
+                        const float2 f0 = unpack_f16(h0), f1 = unpack_f16(h1);
+                        *reinterpret_cast<uint2*>(sm + to + S::Q_PART) = make_uint2(pack_f16(v[0] - f0.x, v[1] - f0.y), pack_f16(v[2] - f1.x, v[3] - f1.y));
+                    }
                 }
             }
         }
@@ -628,8 +639,8 @@ __global__ void __launch_bounds__(ATT_THREADS, Shape4<T, D, NT>::CTAS) cache4_at
             const bool none = m[nt][c] == -INFINITY;
             const float f = none ? 0.0f : exp2_fast(m[nt][c] - top);
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i)
-                *reinterpret_cast<float2*>(s_o + (warp * S::MB + r) * S::PITCH + g * (D / 8) + 2 * i) =
+            for (int i = 0; i < D / 16; ++i)  // (pairs of elements of the lanes' parts in turn: side by side eight lanes' would lie in the same banks)
+                *reinterpret_cast<float2*>(s_o + (warp * S::MB + r) * S::PITCH + (i * 8 + g) * 2) =
                     none ? make_float2(0.0f, 0.0f) : make_float2(o[i][nt][c] * f, o[i][nt][2 + c] * f);
         }
     __syncthreads();
@@ -662,8 +673,9 @@ __global__ void __launch_bounds__(ATT_THREADS, Shape4<T, D, NT>::CTAS) cache4_at
         for (int w = 0; w < WARPS; ++w) {
             const float mw = s_m[w * S::MB + r];
             sum += mw == -INFINITY ? 0.0f : s_l[w * S::MB + r] * exp2_fast(mw - top);
-            const float4 y = *reinterpret_cast<const float4*>(s_o + (w * S::MB + r) * S::PITCH + c);
-            x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+            const float* from = s_o + (w * S::MB + r) * S::PITCH + (c % (D / 8) / 2 * 8 + c / (D / 8)) * 2;
+            const float2 y = *reinterpret_cast<const float2*>(from), z = *reinterpret_cast<const float2*>(from + 16);
+            x.x += y.x, x.y += y.y, x.z += z.x, x.w += z.y;
         }
         x.x *= up, x.y *= up, x.z *= up, x.w *= up;
         if (shared) {
@@ -700,57 +712,67 @@ __global__ void __launch_bounds__(ATT_THREADS, Shape4<T, D, NT>::CTAS) cache4_at
     cluster.sync();  // (the others have read this CTA's sums)
 }
 
-// The longest run of tiles of an item, or into how many CTAs of a cluster each block of query rows goes (*cluster; 0: none), by a model of the time in us: a tile of 128 dimensions takes 0.5 and 0.26
-// for each CTA that shares the SM (32 query rows: 1.6 times that), an item 1.7 of an SM's time to begin and end; a second kernel that joins parts 2.2 and a little for each part, a cluster 1.05.
-// What fits on the GPU at once takes as long as its longest item, more than that the mean load and a third of an item.  Its constants were fitted to 34 calls, each with every run: of one to
-// 64 sequences, 256 to 131072 rows, 64 to 256 dimensions; what it picks takes 2 % longer than the best of each on the average.  (One token over 2048 rows: 7.9 us in 8 clusters of 8, 9.3 of 4,
-// 8.5 in 128 items and a second kernel; 8192 rows 12.8, 19.1 and 11.0; 131072 rows in 592 items 43.5, in 552 45.2, in 824 49.)
-uint32_t run_of(const CacheWork& w, uint32_t group, uint32_t mb, uint32_t n_kv, uint32_t d, double each, uint32_t sms, uint32_t ctas, uint32_t* cluster) {
+// How a call's segments are worked off: with blocks of 8 nt query rows, runs of at most `run` tiles an item, or each block by a cluster of `cluster` CTAs (0: none); and how long that takes, in us.
+struct Plan4 {
+    uint32_t run = 1, cluster = 0;
+    double time = 1e300;
+};
+// By a model: a launch takes `fixed` (most of it the first pass through the kernel's instructions), a tile of 128 dimensions `tile` and `shared` more for each CTA that shares the SM, an item `item` of
+// an SM's time to begin and end; a second kernel that joins parts 1.6 and a little for each part, a cluster 1.6.  What fits on the GPU at once takes as long as its longest item, more
+// than that the mean load and 0.4 of an item.  The constants were fitted to 69 calls, each with every run and cluster and with all the blocks it can have: one to 64 sequences of 300 to
+// 131072 rows, 4 to 512 query rows a KV head, 64 to 256 dimensions, both types.  What it picks takes 0.8 % longer than the best of each on the average, 8 % at most.  (One token over
+// 4096 rows: 9.2 us in 128 items and a second kernel, 9.5 by 8 clusters of 8; 131072 rows 41.5 in 432 items, 43 in 592, 49 in 824.  28 query rows over 1000 rows: 9.3 in blocks of 8, 10.8 of 16,
+// 15.4 of 32; over 16 sequences of up to 8192 rows: 104, 77, 69.)
+struct Cost4 {
+    double tile, shared, item, fixed;
+};
+constexpr Cost4 COST_BF16[3] = {{0.51, 0.34, 0.95, 5.8}, {0.57, 0.49, 1.9, 6.8}, {0.84, 0.65, 4.5, 7.2}}, COST_F32[2] = {{0.62, 0.42, 1.24, 5.1}, {0.87, 0.6, 2.7, 5.6}};
+
+Plan4 plan_of(const CacheWork& w, const CacheArgs& a, uint32_t mb, const Cost4& cost, uint32_t sms, uint32_t ctas) {
     uint32_t most = 1;
     double total = 0.0;
     const auto tiles = [](const CacheSeg& c) { return std::max(1u, (uint32_t)(((uint64_t)c.n_rows + KT - 1) / KT)); };
     for (const CacheSeg& c : w.segs) {
         most = std::max(most, tiles(c));
-        total += (double)cache_blocks_of(c, group, mb) * tiles(c) * n_kv;
+        total += (double)cache_blocks_of(c, a.group, mb) * tiles(c) * a.n_kv;
     }
-    const double slots = (double)sms * ctas;
-    const auto time_of = [&](double items, double run) {
-        const double load = std::min(std::max(std::ceil(items / sms), 1.0), (double)ctas), tile = each * (0.5 + 0.26 * load);
-        return (items <= slots ? run : total / slots + 0.3 * run) * tile + 1.7 * load * std::max(items / slots, 1.0);
+    const double slots = (double)sms * ctas, dims = a.d <= 64 ? 0.56 : a.d <= 128 ? 1.0 : 1.8;
+    const auto time_of = [&](double items, double longest, double run) {
+        const double load = std::min(std::max(std::ceil(items / sms), 1.0), (double)ctas), tile = (cost.tile + cost.shared * load) * dims;
+        return (items <= slots ? longest : total / slots + 0.4 * run) * tile + cost.item * load * std::max(items / slots, 1.0) + cost.fixed;
     };
-    uint32_t best = most;
-    double best_time = 1e300;
+    Plan4 best;
     const auto look = [&](uint32_t run) {
         if (run < 1 || run > most) return;
         double items = 0.0;
         uint32_t longest = 1;
         for (const CacheSeg& c : w.segs) {
             const uint32_t n = (tiles(c) + run - 1) / run;
-            items += (double)cache_blocks_of(c, group, mb) * n * n_kv;
+            items += (double)cache_blocks_of(c, a.group, mb) * n * a.n_kv;
             longest = std::max(longest, (tiles(c) + n - 1) / n);
         }
-        if (run < most && cache_part_bytes((uint64_t)items, 1, mb, d) > CACHE_PARTS_MOST) return;  // (items: of all KV heads)
-        const double time = time_of(items, items <= slots ? longest : run) + (run < most ? 2.2 + 0.006 * ((most + run - 1) / run) : 0.0);
-        if (time < best_time) best_time = time, best = run;
+        if (run < most && cache_part_bytes((uint64_t)items, 1, mb, a.d) > CACHE_PARTS_MOST) return;  // (items: of all KV heads)
+        const double time = time_of(items, longest, run) + (run < most ? 1.6 + 0.007 * ((most + run - 1) / run) : 0.0);
+        if (time < best.time) best.time = time, best.run = run;
     };
     for (uint32_t run = most; run >= 1; run = std::min(run - 1, run * 7 / 8)) look(run);
     for (uint32_t of = 1; of <= 4 * ctas; ++of)  // runs that give each SM 1, 2, .. items
         for (uint32_t more = 0; more < 3; ++more) look((uint32_t)std::min(total / sms / of, 4e9) + more);
-    *cluster = 0;
     for (uint32_t cl = 2; cl <= 8; cl *= 2) {
         double items = 0.0;
-        for (const CacheSeg& c : w.segs) items += (double)cache_blocks_of(c, group, mb) * cl * n_kv;
-        const double time = time_of(items, (most + cl - 1) / cl) + 1.05;
-        if (time < best_time) best_time = time, *cluster = cl;
+        for (const CacheSeg& c : w.segs) items += (double)cache_blocks_of(c, a.group, mb) * cl * a.n_kv;
+        const uint32_t run = (most + cl - 1) / cl;
+        const double time = time_of(items, run, run) + 1.6;
+        if (time < best.time) best.time = time, best.cluster = cl;
     }
     return best;
 }
 
 template <typename T, int D, int NT>
-Status launch_class4(Ctx* c, CacheArgs a, const Rows4& r, CacheWork w) {
+Status launch_class4(Ctx* c, CacheArgs a, const Rows4& r, CacheWork w, const Plan4& plan) {
     using S = Shape4<T, D, NT>;
-    const uint32_t run = run_of(w, a.group, S::MB, a.n_kv, a.d, (NT == 4 ? 1.6 : 1.0) * D / 128, (uint32_t)sm_count(c->device), S::CTAS, &a.cluster);
-    cache_cut(&w, a.group, S::MB, KT, run, a.cluster);
+    a.cluster = plan.cluster;
+    cache_cut(&w, a.group, S::MB, KT, plan.run, plan.cluster);
     if (w.items * a.n_kv > 0x7FFFFFFFull) return Status(SLHA_ERR_CAPACITY, "attention over a cache: too many blocks of query rows");
     CacheTable tab;
     SLHA_TRY(cache_table(c, w.segs, &tab, &a.table));
@@ -765,16 +787,17 @@ Status launch_class4(Ctx* c, CacheArgs a, const Rows4& r, CacheWork w) {
     if (w.blocks) SLHA_TRY(launch_cache_join(c, a, sizeof(T) == 2 ? SLHA_B200_BF16 : SLHA_B200_F32, w, S::MB));
     return mem.done();
 }
-template <typename T>
-Status launch_type4(Ctx* c, const CacheArgs& a, const Rows4& r, int nt, CacheWork w) {
-    if (a.d <= 64) return nt == 1 ? launch_class4<T, 64, 1>(c, a, r, std::move(w)) : nt == 2 ? launch_class4<T, 64, 2>(c, a, r, std::move(w)) : launch_class4<T, 64, 4>(c, a, r, std::move(w));
-    if (a.d <= 128) return nt == 1 ? launch_class4<T, 128, 1>(c, a, r, std::move(w)) : nt == 2 ? launch_class4<T, 128, 2>(c, a, r, std::move(w)) : launch_class4<T, 128, 4>(c, a, r, std::move(w));
-    return nt == 1 ? launch_class4<T, 256, 1>(c, a, r, std::move(w)) : launch_class4<T, 256, 2>(c, a, r, std::move(w));
+template <typename T, int D>
+Status launch_dim4(Ctx* c, const CacheArgs& a, const Rows4& r, int nt, CacheWork w, const Plan4& plan) {
+    if constexpr (sizeof(T) == 2 && D <= 128)  // (32 query rows' sums fill the registers; for float32 blocks of 16 are never slower)
+        if (nt == 4) return launch_class4<T, D, 4>(c, a, r, std::move(w), plan);
+    return nt == 1 ? launch_class4<T, D, 1>(c, a, r, std::move(w), plan) : launch_class4<T, D, 2>(c, a, r, std::move(w), plan);
 }
 
-// Segments whose rows are laid out as rows of the queries' type first, in order, as many at a time as CACHE4_ROWS_MOST holds (at least one).
-Status attend_laid_out(Ctx* c, const CacheArgs& args, const Rows4& r, int dtype, const std::vector<SlhaB200Segment>& segs) {
-    const uint64_t e = dtype == SLHA_B200_BF16 ? 2 : 4, row = 2 * args.n_kv * args.d * e;
+// Segments whose rows are laid out as rows of bfloat16 first, in order, as many at a time as CACHE4_ROWS_MOST holds (at least one).
+Status attend_laid_out(Ctx* c, const CacheArgs& args, const Rows4& r, const std::vector<SlhaB200Segment>& segs) {
+    constexpr uint64_t e = 2;
+    const uint64_t row = 2 * args.n_kv * args.d * e;
     const uint32_t entries = (args.row_pos || args.row_doc) ? (args.entry_hs ? args.n_kv : 1) : 0;
     const uint64_t row_bytes = row + 4ull * entries * ((args.row_pos != nullptr) + (args.row_doc != nullptr));
     // a batch: segments first .. last, their rows one behind another
@@ -827,7 +850,7 @@ Status attend_laid_out(Ctx* c, const CacheArgs& args, const Rows4& r, int dtype,
         x.entries = entries;
         x.n_kv = args.n_kv;
         x.d = args.d;
-        SLHA_TRY(launch_read_cache4(c, x, dtype, of, to));
+        SLHA_TRY(launch_read_cache4(c, x, SLHA_B200_BF16, of, to));
         CacheArgs a = args;
         a.keys = x.rows.p[0];
         a.values = x.rows.p[1];
@@ -836,7 +859,7 @@ Status attend_laid_out(Ctx* c, const CacheArgs& args, const Rows4& r, int dtype,
         if (a.row_pos) a.row_pos = x.to_pos;
         if (a.row_doc) a.row_doc = x.to_doc;
         a.entry_hs = args.entry_hs ? b.rows : 0;
-        SLHA_TRY(launch_attend_cache(c, a, dtype, to));
+        SLHA_TRY(launch_attend_cache(c, a, SLHA_B200_BF16, to));
     }
     g_cache_kernels |= SLHA_B200_CACHE_LAID_OUT;
     return mem.done();
@@ -845,18 +868,11 @@ Status attend_laid_out(Ctx* c, const CacheArgs& args, const Rows4& r, int dtype,
 }  // namespace
 
 Status launch_attend_cache4(Ctx* c, CacheArgs a, const Rows4& r, int dtype, const std::vector<SlhaB200Segment>& segs) {
-    CacheWork of[3];  // blocks of 8, 16 and 32 query rows
-    std::vector<SlhaB200Segment> rest = segs;
-    bool any = false;
+    // Segments of at most 8, 16, 64 and of more query rows a KV head: a launch each, so that decoded tokens beside a prompt keep the blocks that suit them.
+    CacheWork of[4];
     for (size_t i = 0; i < segs.size(); ++i) {
         const SlhaB200Segment& s = segs[i];
         if (s.n_queries == 0) continue;
-        const uint64_t rows = (uint64_t)s.n_queries * a.group;
-        if (rows > CACHE4_QUERY_ROWS) {
-            any = true;
-            continue;
-        }
-        rest[i].n_queries = 0;
         CacheSeg g{};
         g.row_begin = s.tile_begin;
         g.n_rows = s.n_tiles;
@@ -864,13 +880,49 @@ Status launch_attend_cache4(Ctx* c, CacheArgs a, const Rows4& r, int dtype, cons
         g.n_queries = s.n_queries;
         g.base = s.index_base;
         g.seg = (uint32_t)i;
-        of[rows <= 8 ? 0 : rows <= 16 ? 1 : 2].segs.push_back(g);
+        const uint64_t rows = (uint64_t)s.n_queries * a.group;
+        of[rows <= 8 ? 0 : rows <= 16 ? 1 : rows <= 64 ? 2 : 3].segs.push_back(g);
     }
-    for (int k = 0; k < 3; ++k) {
+    const bool bf = dtype == SLHA_B200_BF16;
+    const uint32_t sms = (uint32_t)sm_count(c->device);
+    std::vector<SlhaB200Segment> rest;
+    for (int k = 0; k < 4; ++k) {
         if (of[k].segs.empty()) continue;
-        SLHA_TRY(dtype == SLHA_B200_BF16 ? launch_type4<__nv_bfloat16>(c, a, r, 1 << k, std::move(of[k])) : launch_type4<float>(c, a, r, 1 << k, std::move(of[k])));
+        Plan4 plan;
+        int nt = 1;
+        for (int x = 0; x <= std::min(k, bf && a.d <= 128 ? 2 : 1); ++x) {
+            const uint32_t ctas = a.d > 128 ? 2 : x == 0 ? 4 : x == 1 ? 3 : 2;  // (Shape4's)
+            const Plan4 p = plan_of(of[k], a, 8u << x, bf ? COST_BF16[x] : COST_F32[x], sms, ctas);
+            if (p.time < plan.time) plan = p, nt = 1 << x;
+        }
+        // What the kernel for many query rows takes: the rows laid out, and read again by it while it multiplies.  (16 sequences of 4096 rows, bfloat16, 128 dimensions, us: 64 query rows 120 against
+        // 88 here, 96: 121 against 161; one of 8192 rows, 96: 29.3 and 29.2, 256: 36 and 53.)
+        if (k >= 2 && bf && a.d <= 128 && a.scale > 0.0f) {
+            double elements = 0.0, products = 0.0;
+            for (const CacheSeg& g : of[k].segs) {
+                const double rows = 2.0 * g.n_rows * a.n_kv * a.d;
+                elements += rows;
+                products += rows * g.n_queries * a.group;
+            }
+            if (16.0 + elements * 4.7e-7 + std::max(elements * 3.6e-7, products * 2e-9) < plan.time) {
+                if (rest.empty()) {
+                    rest = segs;
+                    for (SlhaB200Segment& s : rest) s.n_queries = 0;
+                }
+                for (const CacheSeg& g : of[k].segs) rest[g.seg].n_queries = g.n_queries;
+                continue;
+            }
+        }
+        if (bf)
+            SLHA_TRY(a.d <= 64 ? (launch_dim4<__nv_bfloat16, 64>(c, a, r, nt, std::move(of[k]), plan))
+                     : a.d <= 128 ? (launch_dim4<__nv_bfloat16, 128>(c, a, r, nt, std::move(of[k]), plan))
+                                  : (launch_dim4<__nv_bfloat16, 256>(c, a, r, nt, std::move(of[k]), plan)));
+        else
+            SLHA_TRY(a.d <= 64 ? (launch_dim4<float, 64>(c, a, r, nt, std::move(of[k]), plan))
+                     : a.d <= 128 ? (launch_dim4<float, 128>(c, a, r, nt, std::move(of[k]), plan))
+                                  : (launch_dim4<float, 256>(c, a, r, nt, std::move(of[k]), plan)));
     }
-    return any ? attend_laid_out(c, a, r, dtype, rest) : Status();
+    return rest.empty() ? Status() : attend_laid_out(c, a, r, rest);
 }
 
 }  // namespace slha
