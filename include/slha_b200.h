@@ -638,12 +638,14 @@ int32_t slha_b200_read_cache4(const SlhaB200KvCache4* cache, const SlhaB200Segme
                               const SlhaB200KvCache* to, const SlhaB200Segment* to_segments);
 
 /* slha_b200_attend_cache and slha_b200_attend_tree over rows held in 4 bits: the same
- * segments, queries, masks and outputs.  Products are exact, sums and softmax float32.  Up to
- * 64 query rows (tokens times query heads of a KV head) are multiplied with what the codes stand for
- * as they are read, queries and weights as float16 numbers (float32: two) scaled by powers of two; for more,
- * a segment's rows are first laid out as rows of the queries' type in working memory of the
- * thread (512 MB at most, or what one segment takes).  scale * 2^key_exponent keeps to what
- * is said of scale.  (Queries that hold an infinity may come out as NaN.) */
+ * segments, queries, masks and outputs.  Products are exact, sums and softmax float32.  Few
+ * tokens, float32 queries and more than 128 dimensions are multiplied with what the codes
+ * stand for as they are read, queries and weights as float16 numbers (of float32: two)
+ * scaled by powers of two; for many bfloat16 tokens a segment's rows are first laid out as
+ * bfloat16 (exact) in working memory of the thread (512 MB at most, or what one segment
+ * takes), and weights are rounded to bfloat16.  scale * 2^key_exponent keeps to what is
+ * said of scale.  A NaN that a token sees is in its results; queries that hold an infinity
+ * may come out as NaN. */
 int32_t slha_b200_attend_cache4(const SlhaB200KvCache4* cache, const SlhaB200Segment* segments, size_t n_segments,
                                 const SlhaB200CacheQueries* queries, void* out, uint64_t out_token_stride,
                                 uint64_t out_head_stride, float* lse_out);

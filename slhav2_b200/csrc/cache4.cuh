@@ -31,6 +31,7 @@ struct Rows4Args {
     uint32_t *to_pos, *to_doc;
     uint64_t entry_hs, to_entry_hs;
     const CacheSeg* table;
+    uint32_t seen_last;  // reading: rows further than this before a segment's first token are left out; 0xFFFFFFFF: none are
     uint32_t n_segs, n_kv, d, entries;                                      // entries: heads whose entries are laid out
     uint32_t each, units, columns, passes, step, per_column, per_unit;  // rows of a work item and what a thread takes of them, see cache4_rows.cu
 };

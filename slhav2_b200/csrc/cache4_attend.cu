@@ -672,7 +672,7 @@ __global__ void __launch_bounds__(ATT_THREADS, Shape4<T, D, NT>::CTAS) cache4_at
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
             const float mw = s_m[w * S::MB + r];
-            sum += mw == -INFINITY ? 0.0f : s_l[w * S::MB + r] * exp2_fast(mw - top);
+            sum += mw == -INFINITY ? s_l[w * S::MB + r] : s_l[w * S::MB + r] * exp2_fast(mw - top);  // (of scores that are all NaN: NaN, else zero)
             const float* from = s_o + (w * S::MB + r) * S::PITCH + (c % (D / 8) / 2 * 8 + c / (D / 8)) * 2;
             const float2 y = *reinterpret_cast<const float2*>(from), z = *reinterpret_cast<const float2*>(from + 16);
             x.x += y.x, x.y += y.y, x.z += z.x, x.w += z.y;
@@ -825,7 +825,7 @@ Status attend_laid_out(Ctx* c, const CacheArgs& args, const Rows4& r, const std:
         uint64_t at = 0;
         for (size_t i = 0; i < segs.size(); ++i) {
             if (i < b.first || i > b.last || !segs[i].n_queries) {
-                of[i].n_tiles = of[i].n_queries = to[i].n_queries = 0;
+                of[i].n_tiles = to[i].n_queries = 0;
                 continue;
             }
             to[i].tile_begin = at;
@@ -850,6 +850,8 @@ Status attend_laid_out(Ctx* c, const CacheArgs& args, const Rows4& r, const std:
         x.entries = entries;
         x.n_kv = args.n_kv;
         x.d = args.d;
+        // (where the order of rows is that of positions, and no prefix is seen from everywhere)
+        x.seen_last = args.causal && !args.row_pos && !args.q_pos && !args.prefix && !args.tree ? args.window_last : 0xFFFFFFFFu;
         SLHA_TRY(launch_read_cache4(c, x, SLHA_B200_BF16, of, to));
         CacheArgs a = args;
         a.keys = x.rows.p[0];

@@ -182,6 +182,9 @@ __global__ void __launch_bounds__(ROW_THREADS) read_cache4_kernel(const __grid_c
     const CacheSeg& sg = table[seg];
     const uint32_t n = a.counts ? min(a.counts[sg.seg], sg.n_rows) : sg.n_rows;
     const uint32_t r0 = (blockIdx.x - sg.item_begin) * a.each, rows = min(a.each, n - min(n, r0));
+    // (rows to be attended to: those before what the window of the segment's first token leaves are seen by none)
+    const uint32_t ctx = n - min(n, sg.n_queries);
+    if (a.seen_last != 0xFFFFFFFFu && ctx > a.seen_last && r0 + rows <= ctx - a.seen_last) return;
     const int v = blockIdx.y;
     if (v == 0)
         for (uint32_t e = 0; e < a.entries; ++e)
@@ -288,6 +291,7 @@ Status launch_read_cache4(Ctx* c, Rows4Args a, int dtype, const std::vector<Slha
         CacheSeg g{};
         g.row_begin = segs[i].tile_begin;
         g.n_rows = segs[i].n_tiles;
+        g.n_queries = segs[i].n_queries;
         g.seg = (uint32_t)i;
         g.to_begin = to_segs[i].tile_begin;
         of.push_back(g);

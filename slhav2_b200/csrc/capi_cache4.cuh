@@ -227,6 +227,7 @@ int32_t slha_b200_read_cache4(const SlhaB200KvCache4* cache, const SlhaB200Segme
         SLHA_TRY(cache_stage(c, cache->rows, n_segments, &a.counts, fn, "rows"));
         a.n_kv = cache->n_kv_heads;
         a.d = cache->head_dim;
+        a.seen_last = 0xFFFFFFFFu;
         SLHA_TRY(launch_read_cache4(c, a, to->dtype, segs, to_segs));
         if (sync_by_default(c)) SLHA_CUDA(cudaStreamSynchronize(c->stream));
         return Status();

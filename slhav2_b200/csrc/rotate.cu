@@ -5,7 +5,7 @@
 // heads.
 //
 // Bytes bound it, every head read and written once, once few instructions do: 8, 16 or 32 lanes take a head, 8 elements each: four pairs (two 8- or 16-byte loads, half a rotation apart) or, of
-// interleaved pairs and what is not turned, 8 elements side by side.  A group of lanes takes a head of a block's tokens, four of them at a time, so that its addresses grow by a constant and its
+// interleaved pairs and what is not turned, 8 elements side by side.  A group of lanes takes a head of a block's tokens, two of them at a time, so that its addresses grow by a constant and its
 // weights stay in registers; then its next head.  No element is read by another lane than the one that writes it, so that heads may be turned in place.
 #include <cuda_bf16.h>
 
@@ -16,7 +16,24 @@
 namespace slha {
 namespace {
 
-constexpr int ROT_THREADS = 256, ROT_FLIGHT = 4, ROT_TOKENS = 8;  // tokens under way at a time, and most of a block
+constexpr int ROT_THREADS = 256, ROT_FLIGHT = 2, ROT_TOKENS = 8;  // tokens under way at a time, and most of a block
+// two float32 at a time
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t r, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;\n" : "=f"(x), "=f"(y) : "l"(r)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
 constexpr double PER_TURN = 0.15915494309189533577;  // 1 / (2 pi)
 
 template <typename T>
@@ -70,7 +87,7 @@ struct HeadUnit {  // 8 elements as they lie: two times 4
 template <typename T, int LANES>
 __global__ void __launch_bounds__(ROT_THREADS) rotate_heads_kernel(const __grid_constant__ RotateArgs a, const __grid_constant__ CacheTable tab) {
     dep_wait();
-    __shared__ __align__(16) float2 s_turn[ROT_TOKENS][CACHE_DIM_MOST / 2];  // cosine and sine
+    __shared__ __align__(16) float s_turn[ROT_TOKENS][2][CACHE_DIM_MOST / 2];  // cosines, sines
     const CacheSeg* table = a.table ? a.table : tab.s;
     const uint32_t seg = cache_find(a.n_segs, blockIdx.x, [&](uint32_t i) { return table[i].item_begin; });
     const CacheSeg& sg = table[seg];
@@ -89,7 +106,8 @@ __global__ void __launch_bounds__(ROT_THREADS) rotate_heads_kernel(const __grid_
         const double turns = (double)a.positions[(uint64_t)axis * a.n_tokens + tok0 + t] * (double)a.freq[p] * PER_TURN;
         float s, c;
         sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
-        s_turn[t][p] = make_float2(c * a.magnitude, s * a.magnitude);
+        s_turn[t][0][p] = c * a.magnitude;
+        s_turn[t][1][p] = s * a.magnitude;
     }
     __syncthreads();
     // (a warp's groups go through the loops together: sums are taken over a group's lanes)
@@ -100,9 +118,12 @@ __global__ void __launch_bounds__(ROT_THREADS) rotate_heads_kernel(const __grid_
         const unsigned char* from = (q ? a.q + h * a.qhs : k ? a.k + h * a.khs : a.v + h * a.vhs) + tok0 * step;
         unsigned char* to = (q ? a.q_out + h * a.qohs : k ? a.k_out + h * a.kohs : a.v_out + h * a.vohs) + (q ? tok0 : row0) * to_step;
         const float* weight = q ? a.q_weight : k ? a.k_weight : nullptr;
-        float w[8];
+        uint64_t w[4];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = weight && last ? weight[e < 4 ? first + e : second + e - 4] : 1.0f;
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t at = e < 2 ? first + 2 * e : second + 2 * e - 4;
+            w[e] = weight && last ? pair(weight[at], weight[at + 1]) : pair(1.0f, 1.0f);
+        }
         for (uint32_t t = 0; t < tokens; t += ROT_FLIGHT) {
             HeadUnit<T> in[ROT_FLIGHT];
 #pragma unroll
@@ -118,31 +139,46 @@ __global__ void __launch_bounds__(ROT_THREADS) rotate_heads_kernel(const __grid_
                     if (a.norm) {
                         float sum = 0.0f;
                         if (there) {
+                            uint64_t two = 0;
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) sum = fmaf(f[e], f[e], sum);
+                            for (int e = 0; e < 8; e += 2) two = fma2(pair(f[e], f[e + 1]), pair(f[e], f[e + 1]), two);
+                            float odd;
+                            unpair(two, sum, odd);
+                            sum += odd;
                         }
 #pragma unroll
                         for (int m = LANES / 2; m; m >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, m);
                         factor = rsqrtf(sum * a.per_dim + a.eps);
                     }
                     if (there && !value) {
-                        if (a.norm) {
+                        uint64_t y[4];  // two elements at a time: apart, of two pairs; side by side, a pair's
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) f[e] = f[e] * factor * w[e];
+                        for (int e = 0; e < 4; ++e) {
+                            y[e] = pair(f[2 * e], f[2 * e + 1]);
+                            if (a.norm) y[e] = mul2(mul2(y[e], pair(factor, factor)), w[e]);
                         }
                         if (turned) {
-                            const float4 c01 = *reinterpret_cast<const float4*>(&s_turn[t + j][4 * x]), c23 = *reinterpret_cast<const float4*>(&s_turn[t + j][4 * x + 2]);
-                            const auto turn = [&](float& u, float& v, float c, float s) {
-                                const float one = fmaf(u, c, -v * s);
-                                v = fmaf(u, s, v * c);
-                                u = one;
-                            };
+                            const float4 c = *reinterpret_cast<const float4*>(&s_turn[t + j][0][4 * x]), s = *reinterpret_cast<const float4*>(&s_turn[t + j][1][4 * x]);
                             if (apart) {
-                                turn(f[0], f[4], c01.x, c01.y), turn(f[1], f[5], c01.z, c01.w), turn(f[2], f[6], c23.x, c23.y), turn(f[3], f[7], c23.z, c23.w);
+                                const uint64_t cs[2] = {pair(c.x, c.y), pair(c.z, c.w)}, sn[2] = {pair(s.x, s.y), pair(s.z, s.w)}, back[2] = {pair(-s.x, -s.y), pair(-s.z, -s.w)};
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    const uint64_t u = y[e], v = y[2 + e];
+                                    y[e] = fma2(u, cs[e], mul2(v, back[e]));
+                                    y[2 + e] = fma2(u, sn[e], mul2(v, cs[e]));
+                                }
                             } else {
-                                turn(f[0], f[1], c01.x, c01.y), turn(f[2], f[3], c01.z, c01.w), turn(f[4], f[5], c23.x, c23.y), turn(f[6], f[7], c23.z, c23.w);
+                                const float cs[4] = {c.x, c.y, c.z, c.w}, sn[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    float u, v;
+                                    unpair(y[e], u, v);
+                                    y[e] = fma2(pair(u, u), pair(cs[e], sn[e]), mul2(pair(v, v), pair(-sn[e], cs[e])));
+                                }
                             }
                         }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) unpair(y[e], f[2 * e], f[2 * e + 1]);
                         in[j].set(f);
                     }
                 }
@@ -170,8 +206,9 @@ Status launch_rotate_heads(Ctx* c, RotateArgs a, int dtype, const std::vector<Sl
     uint64_t tokens = 0, items = 0;
     for (const SlhaB200Segment& s : segs) tokens += s.n_queries;
     if (!tokens) return Status();
-    // tokens of a block: up to eight, where that leaves six blocks an SM
-    a.each = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(tokens / (6 * sm_count(c->device)), 1), ROT_TOKENS);
+    // tokens of a block: up to eight, so that the blocks come in whole rounds of four an SM (8192 tokens: in two rounds of 7 tokens each 47.5 us, of 8 each 49.5)
+    const uint64_t round = 4ull * sm_count(c->device), rounds = (tokens + round * ROT_TOKENS - 1) / (round * ROT_TOKENS);
+    a.each = (uint32_t)((tokens + round * rounds - 1) / (round * rounds));
     a.per_dim = 1.0f / (float)a.d;
     std::vector<CacheSeg> of;
     for (size_t i = 0; i < segs.size(); ++i) {
