@@ -712,6 +712,95 @@ __global__ void __launch_bounds__(ATT_THREADS, Shape4<T, D, NT>::CTAS) cache4_at
     cluster.sync();  // (the others have read this CTA's sums)
 }
 
+// Joins the parts of query rows whose segment's rows were split: WARPS warps a query row, each every WARPS-th part, eight at a time with their maxima and sums, so that nothing waits for what another
+// load says; the warps' sums meet in shared memory, in the warps' order.  (131072 rows in 74 parts, one token: 44.0 us in all, 47.0 by two passes over the parts with four warps; 48 sequences in 2 to 6 parts 101.2 and 102.9.)
+constexpr int JOIN_FLIGHT = 8;
+template <typename T, int WARPS>
+__global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) cache4_join_kernel(const __grid_constant__ CacheArgs a, const __grid_constant__ CacheTable tab, uint32_t mb, uint32_t rows_of) {
+    dep_wait();
+    constexpr int ROWS = WARPS == 1 ? 4 : 1;  // of a block
+    __shared__ float4 s_acc[WARPS > 1 ? WARPS : 1][64];
+    __shared__ float2 s_ml[WARPS];
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, mine = WARPS == 1 ? 0 : warp;
+    const uint32_t part = blockIdx.x % rows_of, at = blockIdx.x / rows_of, head = at % a.n_kv, qb = at / a.n_kv;
+    const CacheSeg* table = a.table ? a.table : tab.s;
+    const uint32_t seg = cache_find(a.n_segs, qb, [&](uint32_t i) { return table[i].block_begin; });
+    const CacheSeg& sg = table[seg];
+    const uint32_t block = qb - sg.block_begin, r = part * ROWS + (WARPS == 1 ? warp : 0), row = block * mb + r;
+    if (r >= mb || row >= sg.n_queries * a.group) return;  // (with more than one warp a row: all of them)
+    const uint64_t first = ((uint64_t)(sg.item_begin + block * sg.n_chunks) * a.n_kv + head) * mb + r, step = (uint64_t)a.n_kv * mb;
+    float m = -INFINITY, sum = 0.0f;
+    float4 acc[2] = {make_float4(0.0f, 0.0f, 0.0f, 0.0f), make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
+    const auto add = [](float4& x, float f, const float4& y) { x.x = fmaf(f, y.x, x.x), x.y = fmaf(f, y.y, x.y), x.z = fmaf(f, y.z, x.z), x.w = fmaf(f, y.w, x.w); };
+    const auto times = [](float4& x, float f) { x.x *= f, x.y *= f, x.z *= f, x.w *= f; };
+    for (uint32_t c0 = mine; c0 < sg.n_chunks; c0 += WARPS * JOIN_FLIGHT) {
+        float2 ml[JOIN_FLIGHT];
+        float4 x[JOIN_FLIGHT];
+#pragma unroll
+        for (int i = 0; i < JOIN_FLIGHT; ++i) {
+            const uint32_t c = c0 + i * WARPS;
+            const bool there = c < sg.n_chunks;
+            ml[i] = there ? *reinterpret_cast<const float2*>(a.part_ml + (first + c * step) * 2) : make_float2(-INFINITY, 0.0f);
+            x[i] = there && lane * 4 < a.d ? *reinterpret_cast<const float4*>(a.part_o + (first + c * step) * a.d + lane * 4) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+        float top = m;
+#pragma unroll
+        for (int i = 0; i < JOIN_FLIGHT; ++i) top = fmaxf(top, ml[i].x);
+        const float keep = m == -INFINITY ? 0.0f : exp2_fast(m - top);
+        if (m != -INFINITY) sum *= keep;  // (of scores that are all NaN: NaN, without a maximum)
+        times(acc[0], keep);
+        times(acc[1], keep);
+        m = top;
+#pragma unroll
+        for (int i = 0; i < JOIN_FLIGHT; ++i) {
+            const float f = ml[i].x == -INFINITY ? 0.0f : exp2_fast(ml[i].x - top);
+            sum = fmaf(f, ml[i].y, sum);
+            add(acc[0], f, x[i]);
+        }
+        if (a.d > 128)
+#pragma unroll
+            for (int i = 0; i < JOIN_FLIGHT; ++i) {
+                const uint32_t c = c0 + i * WARPS;
+                if (c >= sg.n_chunks || lane * 4 + 128 >= a.d) continue;
+                add(acc[1], ml[i].x == -INFINITY ? 0.0f : exp2_fast(ml[i].x - top), *reinterpret_cast<const float4*>(a.part_o + (first + c * step) * a.d + lane * 4 + 128));
+            }
+    }
+    if constexpr (WARPS > 1) {
+        s_acc[mine][lane] = acc[0];
+        s_acc[mine][32 + lane] = acc[1];
+        if (lane == 0) s_ml[mine] = make_float2(m, sum);
+        __syncthreads();
+        if (mine) return;
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) top = fmaxf(top, s_ml[w].x);
+        sum = 0.0f;
+        acc[0] = acc[1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            const float2 ml = s_ml[w];
+            const float f = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - top);
+            sum = fmaf(ml.x == -INFINITY ? 1.0f : f, ml.y, sum);
+            add(acc[0], f, s_acc[w][lane]);
+            if (a.d > 128) add(acc[1], f, s_acc[w][32 + lane]);
+        }
+        m = top;
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const uint64_t tok = sg.query_begin + row / a.group;
+    const uint32_t qh = head * a.group + row % a.group;
+    unsigned char* dst = static_cast<unsigned char*>(a.out) + (tok * a.ots + qh * a.ohs) * sizeof(T);
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+        const uint32_t c = lane * 4 + v * 128;
+        if (c >= a.d) continue;
+        const float4 x = acc[v];
+        if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(dst + c * 2) = make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
+        else *reinterpret_cast<float4*>(dst + c * 4) = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+    }
+    if (a.lse && lane == 0) a.lse[tok * a.n_heads + qh] = sum == 0.0f ? -INFINITY : (m + log2f(sum)) * LN2;
+}
+
 // How a call's segments are worked off: with blocks of 8 nt query rows, runs of at most `run` tiles an item, or each block by a cluster of `cluster` CTAs (0: none); and how long that takes, in us.
 struct Plan4 {
     uint32_t run = 1, cluster = 0;
@@ -768,6 +857,28 @@ Plan4 plan_of(const CacheWork& w, const CacheArgs& a, uint32_t mb, const Cost4& 
     return best;
 }
 
+// The segments that were split, their blocks of query rows numbered through.
+template <typename T>
+Status launch_join4(Ctx* c, CacheArgs a, const CacheWork& w, uint32_t mb) {
+    std::vector<CacheSeg> split;
+    uint32_t rows = 0;
+    for (const CacheSeg& s : w.segs)
+        if (s.n_chunks > 1) {
+            split.push_back(s);
+            rows = std::max(rows, std::min(mb, s.n_queries * a.group));
+        }
+    CacheTable tab;
+    SLHA_TRY(cache_table(c, split, &tab, &a.table));
+    a.n_segs = (uint32_t)split.size();
+    const int warps = w.chunks <= 8 ? 1 : w.chunks <= 32 ? 4 : 16;
+    const uint32_t per = warps == 1 ? (rows + 3) / 4 : rows;
+    if (w.blocks * a.n_kv * per > 0x7FFFFFFFull) return Status(SLHA_ERR_CAPACITY, "attention over a cache: too many blocks of query rows");
+    const auto kernel = warps == 1 ? cache4_join_kernel<T, 1> : warps == 4 ? cache4_join_kernel<T, 4> : cache4_join_kernel<T, 16>;
+    SLHA_CUDA(launch_behind(kernel, dim3((uint32_t)(w.blocks * a.n_kv * per)), dim3(warps == 16 ? 512 : 128), 0, c->stream, a, tab, mb, per));
+    count_launch();
+    return Status();
+}
+
 template <typename T, int D, int NT>
 Status launch_class4(Ctx* c, CacheArgs a, const Rows4& r, CacheWork w, const Plan4& plan) {
     using S = Shape4<T, D, NT>;
@@ -784,7 +895,7 @@ Status launch_class4(Ctx* c, CacheArgs a, const Rows4& r, CacheWork w, const Pla
     g_cache_kernels |= SLHA_B200_CACHE_ATTEND4;
     SLHA_CUDA(launch_cluster(cache4_attend_kernel<T, D, NT>, dim3((uint32_t)(w.items * a.n_kv)), dim3(ATT_THREADS), smem, c->stream, std::max(a.cluster, 1u), a, r, tab));
     count_launch();
-    if (w.blocks) SLHA_TRY(launch_cache_join(c, a, sizeof(T) == 2 ? SLHA_B200_BF16 : SLHA_B200_F32, w, S::MB));
+    if (w.blocks) SLHA_TRY(launch_join4<T>(c, a, w, S::MB));
     return mem.done();
 }
 template <typename T, int D>
