@@ -17,7 +17,9 @@
 namespace slha {
 namespace {
 
-constexpr int ROW_THREADS = 256, FLIGHT = 4, WRITE_FLIGHT = 2;  // units under way at a time: reading, of 8 elements, writing, of 16
+// Units under way at a time: reading, of 8 elements, and writing, of 16 (32768 tokens of 8 heads of 128 dimensions written and read back, us, with 1, 2 and 3 blocks under way: bfloat16 62.0, 68.3, 63.8;
+// float32 136, 158, 152: what the registers take in warps costs more than the loads gain).
+constexpr int ROW_THREADS = 256, FLIGHT = 4, WRITE_FLIGHT = 1;
 
 // A thread's part of a work item: a column of the rows' kv x units units (the `pass`-th of its columns; threads beyond them have none), and every step-th row from `row` on.  What is divided by is
 // known to the host: below 256, x / y is x * ceil(2^16 / y) / 2^16.
@@ -62,13 +64,16 @@ struct Block16 {
             f[0] = __uint_as_float(w[i].x), f[1] = __uint_as_float(w[i].y), f[2] = __uint_as_float(w[i].z), f[3] = __uint_as_float(w[i].w);
         }
     }
-    // the largest size, as the bits of a float32
+    // the largest size, as the bits of a float32; a NaN where there is one
     __device__ __forceinline__ uint32_t largest() const {
         if constexpr (sizeof(T) == 2) {
-            uint32_t m = 0;
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-                m = __vmaxu2(m, __vmaxu2(__vmaxu2(w[i].x & 0x7FFF7FFFu, w[i].y & 0x7FFF7FFFu), __vmaxu2(w[i].z & 0x7FFF7FFFu, w[i].w & 0x7FFF7FFFu)));
+            const auto both = [](uint32_t x, uint32_t y) {
+                uint32_t m;
+                asm("max.NaN.bf16x2 %0, %1, %2;\n" : "=r"(m) : "r"(x), "r"(y));
+                return m;
+            };
+            constexpr uint32_t M = 0x7FFF7FFFu;
+            const uint32_t m = both(both(both(w[0].x & M, w[0].y & M), both(w[0].z & M, w[0].w & M)), both(both(w[1].x & M, w[1].y & M), both(w[1].z & M, w[1].w & M)));
             return max(m << 16, m & 0xFFFF0000u);
         } else {
             uint32_t m = 0;
@@ -97,13 +102,22 @@ template <typename T>
 __device__ __forceinline__ uint2 quantise(const Block16<T>& in, float down, float up, uint32_t* scale) {
     const uint32_t most = in.largest();
     constexpr float SIXTH = 1.0f / 6.0f, BEYOND = 8192.0f;  // (what is larger takes the largest scale and code)
-    const float size = fminf(__uint_as_float(most) * down, BEYOND);
+    const float size = sizeof(T) == 2 ? __uint_as_float(most) * down : fminf(__uint_as_float(most) * down, BEYOND), limit = BEYOND * up;
     // (a bfloat16's sixth needs no more: checked for every significand of a tie, the product with 1 / 6 comes out on it)
     *scale = e4m3_of(sizeof(T) == 2 ? size * SIXTH : to_odd(quotient(size, 6.0f, SIXTH), size, 6.0f));
     // (the scale's exponent apart: 1 / s within what an approximation takes)
-    const float held = e4m3_value(*scale), s = held * up, r = held > 0.0f ? inverse(held) * down : 0.0f, rest = sizeof(T) == 2 ? fmaf(-s, r, 1.0f) * r : 0.0f;  // 1 / s = r + rest
-    const float limit = BEYOND * up;
-    const bool beyond = size == BEYOND;
+    const float held = e4m3_value(*scale), s = held * up;
+    float r = held > 0.0f ? inverse(held) : 0.0f, rest = 0.0f;
+    if constexpr (sizeof(T) == 2) {
+        // 1 / s = r + rest, r the float32 below it: both parts of x / s have x's sign, so that what overflows comes out as the infinity that it should
+        rest = fmaf(-held, r, 1.0f);
+        if (rest < 0.0f) {
+            r = __uint_as_float(__float_as_uint(r) - 1);
+            rest = fmaf(-held, r, 1.0f);
+        }
+        rest *= r * down;
+    }
+    r *= down;
     uint32_t codes[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -112,15 +126,12 @@ __device__ __forceinline__ uint2 quantise(const Block16<T>& in, float down, floa
         for (int h = 0; h < 2; ++h) {
             float x[4];
             in.four(2 * i + h, x);
-            if (beyond)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = fminf(fmaxf(x[e], -limit), limit);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 if constexpr (sizeof(T) == 2) {
                     q[4 * h + e] = fmaf(x[e], r, x[e] * rest);
                 } else {
-                    const float y = fabsf(x[e]);
+                    const float y = fminf(fabsf(x[e]), limit);
                     q[4 * h + e] = copysignf(to_odd(quotient(y, s, r), y, s), x[e]);
                 }
             }
