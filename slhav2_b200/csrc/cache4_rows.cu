@@ -5,8 +5,9 @@
 // border or 2^-8 of it away; times 1 / s as the sum of two float32 it comes out on the border exactly.  float32: the quotient's last bit says whether something was cut off (rounding to
 // odd).  So every code and scale is what the formula gives in exact arithmetic.
 //
-// Bytes bound it, 2 or 4 in for 9/16 out an element, once few instructions do: a thread takes 8 elements (16 bytes of bfloat16, 4 of codes) of one column of the rows' elements, and its addresses
-// grow by a constant; four such units are under way at a time.
+// Bytes bound it, 2 or 4 in for 9/16 out an element, once few instructions do: a thread takes one column of the rows' elements, 8 of them reading (4 bytes of codes, 16 of bfloat16) and a whole block
+// of 16 writing, so that its addresses grow by a constant.  32768 tokens of 8 heads of 128 dimensions: written 31.7 us = 5.4 TB/s (bfloat16; float32 59, 5.2 TB/s), read back 30.3 = 5.7 TB/s
+// (float32 77; 9001 rows of 7 prompts, 80 dimensions, float32 36 = 3.6 TB/s: a column's rows lie apart).  48 tokens are one launch each way, 3 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

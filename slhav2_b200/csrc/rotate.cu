@@ -7,6 +7,9 @@
 // Bytes bound it, every head read and written once, once few instructions do: 8, 16 or 32 lanes take a head, 8 elements each: four pairs (two 8- or 16-byte loads, half a rotation apart) or, of
 // interleaved pairs and what is not turned, 8 elements side by side.  A group of lanes takes a head of a block's tokens, two of them at a time, so that its addresses grow by a constant and its
 // weights stay in registers; then its next head.  No element is read by another lane than the one that writes it, so that heads may be turned in place.
+//
+// 8192 tokens of 32 + 8 + 8 heads of 128 dimensions, three axes: bfloat16 46.3 us = 4.3 TB/s (without norms 41.8; 150 instructions for 8 elements, 63 % of the issue slots), float32 72 us =
+// 5.6 TB/s.  One token 2.2 us, its call 6.5 with the host's time.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -206,7 +209,7 @@ Status launch_rotate_heads(Ctx* c, RotateArgs a, int dtype, const std::vector<Sl
     uint64_t tokens = 0, items = 0;
     for (const SlhaB200Segment& s : segs) tokens += s.n_queries;
     if (!tokens) return Status();
-    // tokens of a block: up to eight, so that the blocks come in whole rounds of four an SM (8192 tokens: in two rounds of 7 tokens each 47.5 us, of 8 each 49.5)
+    // tokens of a block: up to eight, so that the blocks come in whole rounds of four an SM (8192 tokens come in two rounds of 7 tokens a block)
     const uint64_t round = 4ull * sm_count(c->device), rounds = (tokens + round * ROT_TOKENS - 1) / (round * ROT_TOKENS);
     a.each = (uint32_t)((tokens + round * rounds - 1) / (round * rounds));
     a.per_dim = 1.0f / (float)a.d;
