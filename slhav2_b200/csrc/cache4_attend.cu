@@ -19,6 +19,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <functional>
 
 #include "cache4.cuh"
 #include "cache_mma.cuh"
@@ -824,40 +825,52 @@ struct Cost4 {
 constexpr Cost4 COST_BF16[3] = {{0.51, 0.34, 0.95, 5.8}, {0.57, 0.49, 1.9, 6.8}, {0.84, 0.65, 4.5, 7.2}}, COST_F32[2] = {{0.62, 0.42, 1.24, 5.1}, {0.87, 0.6, 2.7, 5.6}};
 
 Plan4 plan_of(const CacheWork& w, const CacheArgs& a, uint32_t mb, const Cost4& cost, uint32_t sms, uint32_t ctas) {
+    // (64 segments and 60 runs to look at: 2 us of the host's time, 16 with divisions of whole numbers)
+    std::vector<float> tiles, blocks;
     uint32_t most = 1;
-    double total = 0.0;
-    const auto tiles = [](const CacheSeg& c) { return std::max(1u, (uint32_t)(((uint64_t)c.n_rows + KT - 1) / KT)); };
+    float total = 0.0f, all_blocks = 0.0f;
     for (const CacheSeg& c : w.segs) {
-        most = std::max(most, tiles(c));
-        total += (double)cache_blocks_of(c, a.group, mb) * tiles(c) * a.n_kv;
+        const uint32_t n = std::max(1u, (uint32_t)(((uint64_t)c.n_rows + KT - 1) / KT));
+        most = std::max(most, n);
+        tiles.push_back((float)n);
+        blocks.push_back((float)(cache_blocks_of(c, a.group, mb) * a.n_kv));
+        total += tiles.back() * blocks.back();
+        all_blocks += blocks.back();
     }
     const double slots = (double)sms * ctas, dims = a.d <= 64 ? 0.56 : a.d <= 128 ? 1.0 : 1.8;
-    const auto time_of = [&](double items, double longest, double run) {
+    const auto time_of = [&](double items, uint32_t longest, uint32_t run) {
         const double load = std::min(std::max(std::ceil(items / sms), 1.0), (double)ctas), tile = (cost.tile + cost.shared * load) * dims;
         return (items <= slots ? longest : total / slots + 0.4 * run) * tile + cost.item * load * std::max(items / slots, 1.0) + cost.fixed;
     };
     Plan4 best;
-    const auto look = [&](uint32_t run) {
-        if (run < 1 || run > most) return;
-        double items = 0.0;
-        uint32_t longest = 1;
-        for (const CacheSeg& c : w.segs) {
-            const uint32_t n = (tiles(c) + run - 1) / run;
-            items += (double)cache_blocks_of(c, a.group, mb) * n * a.n_kv;
-            longest = std::max(longest, (tiles(c) + n - 1) / n);
-        }
-        if (run < most && cache_part_bytes((uint64_t)items, 1, mb, a.d) > CACHE_PARTS_MOST) return;  // (items: of all KV heads)
-        const double time = time_of(items, longest, run) + (run < most ? 1.6 + 0.007 * ((most + run - 1) / run) : 0.0);
-        if (time < best.time) best.time = time, best.run = run;
-    };
-    for (uint32_t run = most; run >= 1; run = std::min(run - 1, run * 7 / 8)) look(run);
+    std::vector<uint32_t> runs;
+    for (uint32_t run = most; run >= 1; run = std::min(run - 1, run / 8 * 7 + run % 8 * 7 / 8)) runs.push_back(run);
     for (uint32_t of = 1; of <= 4 * ctas; ++of)  // runs that give each SM 1, 2, .. items
-        for (uint32_t more = 0; more < 3; ++more) look((uint32_t)std::min(total / sms / of, 4e9) + more);
+        for (uint32_t more = 0; more < 2; ++more) runs.push_back(std::min((uint32_t)std::min(total / sms / of, 4e9f) + more, most));
+    std::sort(runs.begin(), runs.end(), std::greater<uint32_t>());
+    runs.erase(std::unique(runs.begin(), runs.end()), runs.end());
+    for (const uint32_t run : runs) {
+        if (run < 1) continue;
+        float items = 0.0f;
+        const float up = (float)run - 0.5f, of_run = 1.0f / (float)run;  // (the half keeps a rounding from a whole number less)
+        for (size_t i = 0; i < tiles.size(); ++i) items += blocks[i] * (float)(int)((tiles[i] + up) * of_run);
+        if (run < most && cache_part_bytes((uint64_t)items, 1, mb, a.d) > CACHE_PARTS_MOST) continue;  // (items: of all KV heads)
+        uint32_t longest = run;
+        if (items <= slots) {  // (a segment's runs are evened out)
+            float l = 1.0f;
+            for (size_t i = 0; i < tiles.size(); ++i) {
+                const float n = (float)(int)((tiles[i] + up) * of_run);
+                l = std::max(l, (tiles[i] + n - 0.5f) / n);
+            }
+            longest = (uint32_t)l;
+        }
+        const uint32_t parts = (most - 1) / run + 1;
+        const double time = time_of(items, longest, run) + (run < most ? 1.6 + 0.007 * parts : 0.0);
+        if (time < best.time) best.time = time, best.run = run;
+    }
     for (uint32_t cl = 2; cl <= 8; cl *= 2) {
-        double items = 0.0;
-        for (const CacheSeg& c : w.segs) items += (double)cache_blocks_of(c, a.group, mb) * cl * a.n_kv;
-        const uint32_t run = (most + cl - 1) / cl;
-        const double time = time_of(items, run, run) + 1.6;
+        const uint32_t run = (most - 1) / cl + 1;
+        const double time = time_of((double)all_blocks * cl, run, run) + 1.6;
         if (time < best.time) best.time = time, best.cluster = cl;
     }
     return best;

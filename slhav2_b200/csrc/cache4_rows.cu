@@ -6,8 +6,8 @@
 // odd).  So every code and scale is what the formula gives in exact arithmetic.
 //
 // Bytes bound it, 2 or 4 in for 9/16 out an element, once few instructions do: a thread takes one column of the rows' elements, 8 of them reading (4 bytes of codes, 16 of bfloat16) and a whole block
-// of 16 writing, so that its addresses grow by a constant.  32768 tokens of 8 heads of 128 dimensions: written 31.7 us = 5.4 TB/s (bfloat16; float32 59, 5.2 TB/s), read back 30.3 = 5.7 TB/s
-// (float32 77; 9001 rows of 7 prompts, 80 dimensions, float32 36 = 3.6 TB/s: a column's rows lie apart).  48 tokens are one launch each way, 3 us.
+// of 16 writing, so that its addresses grow by a constant.  32768 tokens of 8 heads of 128 dimensions: written 31.7 us = 5.4 TB/s (bfloat16; float32 58, 5.3 TB/s), read back 30.3 = 5.7 TB/s
+// (float32 63, 4.9 TB/s; 9001 rows of 7 prompts, 80 dimensions, float32 35 = 3.8 TB/s: rows of 80 dimensions leave 16 of 256 threads idle).  48 tokens are one launch each way, 3 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -18,8 +18,8 @@
 namespace slha {
 namespace {
 
-// Units under way at a time: reading, of 8 elements, and writing, of 16 (32768 tokens of 8 heads of 128 dimensions written and read back, us, with 1, 2 and 3 blocks under way: bfloat16 62.0, 68.3, 63.8;
-// float32 136, 158, 152: what the registers take in warps costs more than the loads gain).
+// Units under way at a time: reading, of 8 elements, and writing, of 16 (32768 tokens of 8 heads of 128 dimensions written, us, with 1, 2 and 3 blocks under way: bfloat16 31.7, 38.0, 33.5; float32
+// 58.8, 80.5, 74.4: what the registers take in warps costs more than the loads gain).
 constexpr int ROW_THREADS = 256, FLIGHT = 4, WRITE_FLIGHT = 1;
 
 // A thread's part of a work item: a column of the rows' kv x units units (the `pass`-th of its columns; threads beyond them have none), and every step-th row from `row` on.  What is divided by is
@@ -235,12 +235,20 @@ __global__ void __launch_bounds__(ROW_THREADS) read_cache4_kernel(const __grid_c
                     f[2 * j] = x.x * s;
                     f[2 * j + 1] = x.y * s;
                 }
-                uint4* dst = reinterpret_cast<uint4*>(to);
                 if constexpr (sizeof(T) == 2) {
-                    *dst = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+                    *reinterpret_cast<uint4*>(to) = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
                 } else {
-                    dst[0] = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
-                    dst[1] = make_uint4(__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7]));
+                    // Neighbours exchange halves, so that each of the two stores fills whole sectors of 32 bytes (32768 tokens read, us: 62.7, 78.6 without).  (Units come in pairs, the even one to an even lane, of one row and head.)
+                    const bool odd = u.unit & 1;
+                    const uint32_t both = 3u << (threadIdx.x & 30);
+                    float4 own = odd ? make_float4(f[4], f[5], f[6], f[7]) : make_float4(f[0], f[1], f[2], f[3]), other = odd ? make_float4(f[0], f[1], f[2], f[3]) : make_float4(f[4], f[5], f[6], f[7]);
+                    other.x = __shfl_xor_sync(both, other.x, 1);
+                    other.y = __shfl_xor_sync(both, other.y, 1);
+                    other.z = __shfl_xor_sync(both, other.z, 1);
+                    other.w = __shfl_xor_sync(both, other.w, 1);
+                    float4* pair = reinterpret_cast<float4*>(to) - (odd ? 1 : 0);  // (of the four halves the even lane writes the first and third, the odd one the others)
+                    pair[0] = odd ? other : own;
+                    pair[2] = odd ? own : other;
                 }
             }
         }

@@ -167,6 +167,18 @@ def test_graphs_with_parts_and_rows_laid_out_beside_eager_calls_and_on_other_str
         S.set_stream(None)
 
 
+def test_many_tokens_of_segments_without_rows():
+    rng = np.random.default_rng(11)
+    for lens in ((0,), (0, 0, 300)):
+        call, raw = T.make(rng, lens, 1200 if len(lens) == 1 else (900, 0, 250), 2, 8, 64, True)
+        out, lse = T.results(call, True, *T.on_device(call, raw, True))
+        n = 1200 if len(lens) == 1 else 900
+        assert np.all(out[:n] == 0) and np.all(lse[:n] == -np.inf)
+        if len(lens) > 1:
+            want = call.attend(True)
+            T.held(out[n:], want[0][n:], want[2][n:])
+
+
 def test_two_threads_at_once():
     rng = np.random.default_rng(9)
     calls = [T.make(rng, (3000 + 500 * i, 700), (1, 9), 4, 4, 128, True) for i in range(2)]
