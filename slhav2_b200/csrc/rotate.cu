@@ -8,8 +8,8 @@
 // interleaved pairs and what is not turned, 8 elements side by side.  A group of lanes takes a head of a block's tokens, two of them at a time, so that its addresses grow by a constant and its
 // weights stay in registers; then its next head.  No element is read by another lane than the one that writes it, so that heads may be turned in place.
 //
-// 8192 tokens of 32 + 8 + 8 heads of 128 dimensions, three axes: bfloat16 46.3 us = 4.3 TB/s (without norms 41.8; 150 instructions for 8 elements, 63 % of the issue slots), float32 72 us =
-// 5.6 TB/s.  One token 2.2 us, its call 6.5 with the host's time.
+// 8192 tokens of 32 + 8 + 8 heads of 128 dimensions, three axes: bfloat16 43.9 us = 4.6 TB/s (without norms 39.6; 150 instructions for 8 elements, 63 % of the issue slots), float32 68.7 us =
+// 5.9 TB/s.  One token 2.2 us, its call 6.5 with the host's time.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -19,7 +19,7 @@
 namespace slha {
 namespace {
 
-constexpr int ROT_THREADS = 256, ROT_FLIGHT = 2, ROT_TOKENS = 8;  // tokens under way at a time, and most of a block
+constexpr int ROT_THREADS = 256, ROT_FLIGHT = 2, ROT_TOKENS = 16;  // tokens under way at a time, and most of a block
 // two float32 at a time
 __device__ __forceinline__ uint64_t pair(float x, float y) {
     uint64_t r;
@@ -209,8 +209,8 @@ Status launch_rotate_heads(Ctx* c, RotateArgs a, int dtype, const std::vector<Sl
     uint64_t tokens = 0, items = 0;
     for (const SlhaB200Segment& s : segs) tokens += s.n_queries;
     if (!tokens) return Status();
-    // tokens of a block: up to eight, so that the blocks come in whole rounds of four an SM (8192 tokens come in two rounds of 7 tokens a block)
-    const uint64_t round = 4ull * sm_count(c->device), rounds = (tokens + round * ROT_TOKENS - 1) / (round * ROT_TOKENS);
+    // tokens of a block: up to 16, so that the blocks come in whole rounds of what an SM holds of them (8192 tokens: bfloat16 43.9 us in one round of 14 each, 46.3 in two of 7)
+    const uint64_t round = (dtype == SLHA_B200_BF16 ? 4ull : 3ull) * sm_count(c->device), rounds = (tokens + round * ROT_TOKENS - 1) / (round * ROT_TOKENS);
     a.each = (uint32_t)((tokens + round * rounds - 1) / (round * rounds));
     a.per_dim = 1.0f / (float)a.d;
     std::vector<CacheSeg> of;
