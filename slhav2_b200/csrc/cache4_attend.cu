@@ -999,7 +999,17 @@ Status attend_laid_out(Ctx* c, const CacheArgs& args, const Rows4& r, const std:
 
 }  // namespace
 
-Status launch_attend_cache4(Ctx* c, CacheArgs a, const Rows4& r, int dtype, const std::vector<SlhaB200Segment>& segs) {
+Status launch_attend_cache4(Ctx* c, CacheArgs a, const Rows4& r, int dtype, const std::vector<SlhaB200Segment>& whole) {
+    // Rows that the window of a segment's first token leaves behind are seen by none: where their number is known here, the segment begins behind them, so that the work is shared out by what is seen
+    // (one token over 131072 rows, window 4096: 8.9 us, 20.0 where the table of all rows is shared out; 48 sequences of up to 9001, window 1000: 21.4 and 43.0).
+    std::vector<SlhaB200Segment> segs = whole;
+    if (a.causal && a.window_last != 0xFFFFFFFFu && !a.row_pos && !a.q_pos && !a.prefix && !a.tree && !a.rows)
+        for (SlhaB200Segment& s : segs) {
+            const uint32_t ctx = s.n_tiles - std::min(s.n_tiles, s.n_queries), behind = ctx - std::min(ctx, a.window_last);
+            s.tile_begin += behind;
+            s.n_tiles -= behind;
+            s.index_base += behind;
+        }
     // Segments of at most 8, 16, 64 and of more query rows a KV head: a launch each, so that decoded tokens beside a prompt keep the blocks that suit them.
     CacheWork of[4];
     for (size_t i = 0; i < segs.size(); ++i) {

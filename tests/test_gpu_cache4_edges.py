@@ -167,6 +167,30 @@ def test_graphs_with_parts_and_rows_laid_out_beside_eager_calls_and_on_other_str
         S.set_stream(None)
 
 
+@pytest.mark.parametrize("bf16", [True, False])
+@pytest.mark.parametrize("tokens,window,docs", [(1, 1, False), (1, 300, False), (3, 300, True), (40, 1000, False), (40, 5000, True)])
+def test_windows_that_leave_most_rows_behind(bf16, tokens, window, docs):
+    rng = np.random.default_rng(window)
+    lens, kv, group = (4000, 1200, 50), 2, 4
+    kind = {}
+    if docs:
+        doc = np.concatenate([np.sort(rng.integers(1, 4, n)) for n in lens]).astype(np.uint32)
+        kind = dict(row_doc=np.stack([doc] * kv), q_doc=np.concatenate([doc[e - tokens:e] for e in np.cumsum(lens)]))
+    call, raw = T.make(rng, lens, tokens, kv, group, 64, bf16, window=window, bases=(7, 0, 1 << 31), **kind)
+    want = call.attend(bf16)
+    for b, n in ((0, 4000), (4000, 1200)):
+        behind = max(0, n - tokens - window + 1)
+        for x in (2, 3):
+            raw[x][b:b + behind] = 0x7F
+    got = T.results(call, bf16, *T.on_device(call, raw, bf16))
+    T.held(got[1], want[1], want[3])
+    T.held(got[0], want[0], want[2])
+    call.rows = np.array(lens, np.uint32)  # the same with counts that the host does not look at
+    got = T.results(call, bf16, *T.on_device(call, raw, bf16))
+    T.held(got[1], want[1], want[3])
+    T.held(got[0], want[0], want[2])
+
+
 def test_many_tokens_of_segments_without_rows():
     rng = np.random.default_rng(11)
     for lens in ((0,), (0, 0, 300)):
