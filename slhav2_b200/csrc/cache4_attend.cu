@@ -813,8 +813,8 @@ struct Plan4 {
     uint32_t run = 1, cluster = 0;
     double time = 1e300;
 };
-// By a model: a launch takes `fixed` (most of it the first pass through the kernel's instructions), a tile of 128 dimensions `tile` and `shared` more for each CTA that shares the SM, an item `item` of
-// an SM's time to begin and end; a second kernel that joins parts 1.6 and a little for each part, a cluster 1.6.  What fits on the GPU at once takes as long as its longest item, more
+// By a model: a launch takes `fixed` (most of it the first pass through the kernel's instructions), a tile of 128 dimensions `tile` and `shared` more for each CTA that shares the SM, an item `item`
+// of an SM's time to begin and end; a second kernel that joins parts 1.6 and a little for each part, a cluster 1.6.  What fits on the GPU at once takes as long as its longest item, more
 // than that the mean load and 0.4 of an item.  The constants were fitted to 69 calls, each with every run and cluster and with all the blocks it can have: one to 64 sequences of 300 to
 // 131072 rows, 4 to 512 query rows a KV head, 64 to 256 dimensions, both types.  What it picks takes 0.8 % longer than the best of each on the average, 8 % at most.  (One token over
 // 4096 rows: 9.2 us in 128 items and a second kernel, 9.5 by 8 clusters of 8; 131072 rows 41.5 in 432 items, 43 in 592, 49 in 824.  28 query rows over 1000 rows: 9.3 in blocks of 8, 10.8 of 16,
@@ -840,7 +840,7 @@ Plan4 plan_of(const CacheWork& w, const CacheArgs& a, uint32_t mb, const Cost4& 
     const double slots = (double)sms * ctas, dims = a.d <= 64 ? 0.56 : a.d <= 128 ? 1.0 : 1.8;
     const auto time_of = [&](double items, uint32_t longest, uint32_t run) {
         const double load = std::min(std::max(std::ceil(items / sms), 1.0), (double)ctas), tile = (cost.tile + cost.shared * load) * dims;
-        return (items <= slots ? longest : total / slots + 0.4 * run) * tile + cost.item * load * std::max(items / slots, 1.0) + cost.fixed;
+        return (items <= slots ? longest : total / slots + 0.4 * run) * tile + cost.item * dims * load * std::max(items / slots, 1.0) + cost.fixed;
     };
     Plan4 best;
     std::vector<uint32_t> runs;
@@ -870,7 +870,7 @@ Plan4 plan_of(const CacheWork& w, const CacheArgs& a, uint32_t mb, const Cost4& 
     }
     for (uint32_t cl = 2; cl <= 8; cl *= 2) {
         const uint32_t run = (most - 1) / cl + 1;
-        const double time = time_of((double)all_blocks * cl, run, run) + 1.6;
+        const double time = time_of((double)all_blocks * cl, run, run) + 1.6 * std::max(all_blocks * cl / slots, 1.0);
         if (time < best.time) best.time = time, best.cluster = cl;
     }
     return best;
