@@ -4,7 +4,8 @@
 // narrow side.  An A operand holds pairs along the contraction.  Keys: pairs along a row, as the codes lie; a byte becomes two float16 numbers by one conversion, one product with the block's scale makes
 // their values (exact).  Values: pairs of neighbouring rows; two rows' nibbles are put together into bytes before the conversion, their two scales into a pair.  Queries are
 // float16 numbers, scaled by a power of two a row so that the largest has an exponent of 14 (bfloat16 ones exact down to 2^-31 of the largest; float32 ones as two numbers, 22 bits).
-// Weights are float16 too: against a reference that is the running maximum less 8 in units of log 2 they are at most 2^8 and lose bits below 2^-22 of the largest, 2^-33 of it at most.
+// Weights are float16 too: against a reference that is the largest score less 8 in units of log 2, and stays until a score is more than 15 above it, the largest is 2^8 to 2^15, and weights lose bits
+// below 2^-22 of it, 2^-33 of it at most.
 //
 // A warp takes 32 rows of a tile of 128 and all of a block's 8, 16 or 32 query rows, with a maximum and sums of its own; it copies its own rows (cp.async, one to three tiles ahead), so that a block's
 // warps meet only where its list of tiles ends.
@@ -469,7 +470,7 @@ __global__ void __launch_bounds__(ATT_THREADS, Shape4<T, D, NT>::CTAS) cache4_at
                     top[nt][c] = s[0][nt][c];
 #pragma unroll
                     for (int x = 1; x < 2 * MT; ++x) top[nt][c] = fmaxf(top[nt][c], s[x >> 1][nt][(x & 1) * 2 + c]);
-                    above |= top[nt][c] > m[nt][c] + 15.0f;
+                    above |= top[nt][c] - m[nt][c] > 15.0f;  // (the difference: exact where it counts, infinite for a row's first scores; m + 15 is rounded from sizes of 2^24 on)
                 }
             if (__any_sync(0xFFFFFFFFu, above)) {
 #pragma unroll
@@ -483,7 +484,7 @@ __global__ void __launch_bounds__(ATT_THREADS, Shape4<T, D, NT>::CTAS) cache4_at
                         mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 16));
                         float ref = mx - 8.0f;
                         if (mx - ref > 12.0f) ref = mx;  // (sizes of 2^27 and more, where steps are 16)
-                        if (!(mx > m[nt][c] + 15.0f)) ref = m[nt][c];
+                        if (!(mx - m[nt][c] > 15.0f)) ref = m[nt][c];
                         grow[c] = ref == -INFINITY ? 1.0f : exp2_fast(m[nt][c] - ref);
                         m[nt][c] = ref;
                         l[nt][c] *= grow[c];
