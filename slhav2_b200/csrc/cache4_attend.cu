@@ -416,6 +416,7 @@ __global__ void __launch_bounds__(ATT_THREADS, Shape4<T, D, NT>::CTAS) cache4_at
                         x *= factor[nt][e & 1];
                         if (has_cap) x = cap2 * (fabsf(x) <= 1.0f ? tanh_small(x) : tanh_far(x));
                     }
+            uint32_t seen = 0;  // where not all are: a bit for each of the lane's rows and query rows
             if (!all || has_slope) {
                 const uint32_t* kp_s = reinterpret_cast<const uint32_t*>(st + 2 * (S::CODES + S::SCALES));
                 const auto place = [&](int x) { return key0 + (x >> 1) * 16 + (x & 1) * 8 + row_of(g); };  // of the lane's x-th row in the tile
@@ -439,7 +440,6 @@ __global__ void __launch_bounds__(ATT_THREADS, Shape4<T, D, NT>::CTAS) cache4_at
                 }
                 if (!all) {
                     // (which of them are seen is found out in a loop: unrolled, it pushed the rest of the loop over the tiles out of the instruction cache)
-                    uint32_t seen = 0;
 #pragma unroll 1
                     for (int x = 0; x < 2 * MT; ++x) {
                         const uint32_t col = place(x), row = first + col, kp = position(col), kd = has_doc ? kp_s[KT + col] : 0u;
@@ -556,7 +556,7 @@ __global__ void __launch_bounds__(ATT_THREADS, Shape4<T, D, NT>::CTAS) cache4_at
                     }
                 }
                 // Where some rows are not seen, they may hold anything: a weight of zero does not keep a NaN out of the sum.  Its block's scale becomes zero, and the sums of the query rows
-                // that have a weight for it become NaN.
+                // that see it become NaN, whatever is left of its weight.
                 uint32_t nan[2][D / 64 > 2 ? 2 : 1];
                 bool odd = false;
                 if (!all) {
@@ -573,8 +573,10 @@ __global__ void __launch_bounds__(ATT_THREADS, Shape4<T, D, NT>::CTAS) cache4_at
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int h = 0; h < 2; ++h)
-                            one[nt][h] = transpose8((s[mt][nt][h * 2] != 0.0f ? 0x3C00u : 0u) | (s[mt][nt][h * 2 + 1] != 0.0f ? 0x3C000000u : 0u));
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t two = seen >> ((2 * mt + h) * 2 * NT + 2 * nt);
+                            one[nt][h] = transpose8((two & 1 ? 0x3C00u : 0u) | (two & 2 ? 0x3C000000u : 0u));
+                        }
 #pragma unroll
                     for (int i = 0; i < (D / 64 > 2 ? 2 : 1); ++i) {
                         const uint32_t x[4] = {nan[0][i], nan[0][i], nan[1][i], nan[1][i]};
