@@ -8,7 +8,9 @@
 // interleaved pairs and what is not turned, 8 elements side by side.  A group of lanes takes a head of a block's tokens, two of them at a time, so that its addresses grow by a constant and its
 // weights stay in registers; then its next head.  No element is read by another lane than the one that writes it, so that heads may be turned in place.
 //
-// 8192 tokens of 32 + 8 + 8 heads of 128 dimensions, three axes: bfloat16 43.9 us = 4.6 TB/s (without norms 39.6; 150 instructions for 8 elements, 63 % of the issue slots), float32 68.7 us =
+// Squares are summed in float32; a head for which that is too narrow is scaled by a power of two first (44.8 us instead of 43.4 for the look at each sum, in the case below).
+//
+// 8192 tokens of 32 + 8 + 8 heads of 128 dimensions, three axes: bfloat16 44.8 us = 4.5 TB/s (without norms 39.6; 150 instructions for 8 elements, 63 % of the issue slots), float32 68.7 us =
 // 5.9 TB/s.  One token 2.2 us, its call 6.5 with the host's time.
 #include <cuda_bf16.h>
 
@@ -87,6 +89,35 @@ struct HeadUnit {  // 8 elements as they lie: two times 4
     }
 };
 
+template <int LANES>
+__device__ __forceinline__ float mean_square(const float (&f)[8], bool there, float per_dim, float eps, uint32_t lanes) {
+    float sum = 0.0f;
+    if (there) {
+        uint64_t two = 0;
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) two = fma2(pair(f[e], f[e + 1]), pair(f[e], f[e + 1]), two);
+        float odd;
+        unpair(two, sum, odd);
+        sum += odd;
+    }
+#pragma unroll
+    for (int m = LANES / 2; m; m >>= 1) sum += __shfl_xor_sync(lanes, sum, m);
+    return sum * per_dim + eps;
+}
+// Whether a sum of squares has overflown, or squares that count have lost bits: their mean is below 2^-96, or no number.
+__device__ __forceinline__ bool beyond(float mean) { return __float_as_uint(mean) - (31u << 23) >= (224u << 23); }
+// What such a head is multiplied with, a power of two, so that its largest element (eps' root where that is larger) is 1 to 4: y stays the same, and elements that lose bits are below 2^-120 of
+// the largest.  1 where there is an infinity, a NaN or nothing but zeros.
+template <int LANES>
+__device__ __noinline__ float head_down(float most, float eps, uint32_t lanes) {
+#pragma unroll
+    for (int m = LANES / 2; m; m >>= 1) most = fmaxf(most, __shfl_xor_sync(lanes, most, m));
+    most = fmaxf(most, sqrtf(eps));
+    if (__float_as_uint(most) >= 0x7F800000u || most == 0.0f) return 1.0f;
+    const int k = min((int)(max(__float_as_uint(most) >> 23, 1u) - 127u), 126);
+    return __uint_as_float((uint32_t)(127 - k) << 23);
+}
+
 template <typename T, int LANES>
 __global__ void __launch_bounds__(ROT_THREADS) rotate_heads_kernel(const __grid_constant__ RotateArgs a, const __grid_constant__ CacheTable tab) {
     dep_wait();
@@ -140,18 +171,18 @@ __global__ void __launch_bounds__(ROT_THREADS) rotate_heads_kernel(const __grid_
                     float f[8], factor = 1.0f;
                     if (there) in[j].get(f);
                     if (a.norm) {
-                        float sum = 0.0f;
-                        if (there) {
-                            uint64_t two = 0;
+                        float mean = mean_square<LANES>(f, there, a.per_dim, a.eps, 0xFFFFFFFFu);
+                        if (beyond(mean)) {  // (elements of 2^60 and more; an eps of zero and elements below 2^-48.  All lanes of a head or none)
+                            const uint32_t lanes = LANES == 32 ? 0xFFFFFFFFu : ((1u << LANES % 32) - 1) << (threadIdx.x & 31 & ~(LANES - 1));
+                            float most = 0.0f;
 #pragma unroll
-                            for (int e = 0; e < 8; e += 2) two = fma2(pair(f[e], f[e + 1]), pair(f[e], f[e + 1]), two);
-                            float odd;
-                            unpair(two, sum, odd);
-                            sum += odd;
+                            for (int e = 0; e < 8; ++e) most = there ? fmaxf(most, fabsf(f[e])) : 0.0f;
+                            const float down = head_down<LANES>(most, a.eps, lanes);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) f[e] *= down;
+                            mean = mean_square<LANES>(f, there, a.per_dim, a.eps * down * down, lanes);
                         }
-#pragma unroll
-                        for (int m = LANES / 2; m; m >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, m);
-                        factor = rsqrtf(sum * a.per_dim + a.eps);
+                        factor = rsqrtf(mean);
                     }
                     if (there && !value) {
                         uint64_t y[4];  // two elements at a time: apart, of two pairs; side by side, a pair's
