@@ -642,8 +642,9 @@ int32_t slha_b200_read_cache4(const SlhaB200KvCache4* cache, const SlhaB200Segme
  * tokens, float32 queries and more than 128 dimensions are multiplied with what the codes
  * stand for as they are read, queries and weights as float16 numbers (of float32: two)
  * scaled by powers of two; for many bfloat16 tokens a segment's rows are first laid out as
- * bfloat16 (exact) in working memory of the thread (512 MB at most, or what one segment
- * takes), and weights are rounded to bfloat16.  scale * 2^key_exponent keeps to what is
+ * bfloat16 (exact) in working memory of the thread (as many segments at a time as fit
+ * 512 MB, at least one, which may take more; beside them the parts of long segments, 512 MB
+ * at most), and weights are rounded to bfloat16.  scale * 2^key_exponent keeps to what is
  * said of scale.  A NaN that a token sees is in its results; queries that hold an infinity
  * may come out as NaN. */
 int32_t slha_b200_attend_cache4(const SlhaB200KvCache4* cache, const SlhaB200Segment* segments, size_t n_segments,

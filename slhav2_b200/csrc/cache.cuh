@@ -139,18 +139,26 @@ struct CacheWork {
     uint32_t chunks = 1;             // the most runs of one segment
 };
 
-// Working memory of one call: the thread's, or under capture memory that the graph allocates and frees with every run, so that graphs share none.
+// Working memory of one launch and what joins its parts, the call's next launches may have it again: the thread's, or under capture memory that the graph allocates and frees with every run, so
+// that graphs share none.
 struct CacheMemory {
     Ctx* c;
     void* graph = nullptr;
+    size_t mark = 0;
+    bool taken = false;
     Status get(size_t bytes, void** out) {
-        if (!ctx_capturing(c)) return ctx_device_scratch(c, bytes, out);
+        if (!ctx_capturing(c)) {
+            mark = ctx_scratch_mark(c);
+            taken = true;
+            return ctx_device_scratch(c, bytes, out);
+        }
         SLHA_CUDA(cudaMallocAsync(&graph, bytes, c->stream));
         *out = graph;
         return Status();
     }
     Status done() {
         if (graph) SLHA_CUDA(cudaFreeAsync(graph, c->stream));
+        if (taken) ctx_scratch_back(c, mark);
         return Status();
     }
 };

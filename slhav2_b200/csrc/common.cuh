@@ -51,6 +51,9 @@ struct Ctx {
 };
 Status get_ctx(Ctx** out);  // fails with SLHA_ERR_DEVICE when there is no GPU
 Status ctx_device_scratch(Ctx* c, size_t bytes, void** out);
+// What the call has taken of its scratch since the mark is given back to it: what it takes next, for work behind this on the same stream, may lie there.
+size_t ctx_scratch_mark(Ctx* c);
+void ctx_scratch_back(Ctx* c, size_t mark);
 Status ctx_host_scratch(Ctx* c, size_t bytes, void** out);
 // Host tables to the device, on the call's stream: `src` may go away when this returns.  ctx_upload: into the call's scratch.  Only on a stream
 // that is not being captured: ctx_no_capture fails on one that is, and ends the capture as invalid.

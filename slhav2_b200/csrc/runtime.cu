@@ -49,6 +49,7 @@ struct Block {
     size_t cap = 0, off = 0;
     bool named = false;  // by a graph, which a captured call took memory for: never given back before the thread ends
 };
+constexpr size_t ARENA_FIRST = (size_t)8 << 20, ARENA_STEP = (size_t)64 << 20;
 // The small tables that calls upload (ctx_upload): a copy may read its slot until the slot's event, so a slot is written again
 // only after that.  One wait per stream, for its newest event in half the ring, covers the half; a wait for an event that is long
 // over still costs 1.4 us.  Short tables lie
@@ -114,6 +115,8 @@ struct ThreadState {
     Ctx ctx[16];
     bool ctx_init[16] = {false};
     std::vector<Block> blocks[16];
+    std::vector<std::pair<uint32_t, size_t>> taken[16];  // what the call under way has taken, in order: of which block, from where
+    bool arena_used[16] = {false};                       // by the call under way
     std::vector<std::pair<void*, size_t>> hblocks[16];
     UploadSlot upload[16][UPLOAD_SLOTS];
     uint32_t upload_next[16] = {0};
@@ -183,22 +186,31 @@ Status ctx_device_scratch(Ctx* c, size_t bytes, void** out) {
     bytes = pad256(std::max<size_t>(bytes, 256));
     auto& blocks = tls.blocks[c->device];
     const bool named = capturing(c->stream);
+    tls.arena_used[c->device] = true;
     for (Block& b : blocks) {
         if (b.cap - b.off >= bytes) {
+            tls.taken[c->device].push_back({(uint32_t)(&b - blocks.data()), b.off});
             *out = b.p + b.off;
             b.off += bytes;
             b.named |= named;
             return Status();
         }
     }
+    // (twice the last one, so that a call of many small pieces chains few blocks; not of large ones, which would leave as much again unused)
     Block nb;
-    nb.cap = std::max<size_t>(bytes, blocks.empty() ? (size_t)8 << 20 : blocks.back().cap * 2);
+    nb.cap = std::max<size_t>(bytes, blocks.empty() ? ARENA_FIRST : std::min(blocks.back().cap * 2, ARENA_STEP));
     SLHA_CUDA(cudaMalloc((void**)&nb.p, nb.cap));
     nb.off = bytes;
     nb.named = named;
     *out = nb.p;
+    tls.taken[c->device].push_back({(uint32_t)blocks.size(), 0});
     blocks.push_back(nb);
     return Status();
+}
+size_t ctx_scratch_mark(Ctx* c) { return tls.taken[c->device].size(); }
+void ctx_scratch_back(Ctx* c, size_t mark) {
+    auto& taken = tls.taken[c->device];
+    for (; taken.size() > mark; taken.pop_back()) tls.blocks[c->device][taken.back().first].off = taken.back().second;
 }
 Status ctx_host_scratch(Ctx* c, size_t bytes, void** out) {
     void* p = nullptr;
@@ -319,6 +331,8 @@ CallScope::CallScope() {
         cudaGetLastError();
     }
     for (Block& b : blocks) b.off = 0;
+    tls.taken[c->device].clear();
+    tls.arena_used[c->device] = false;
     for (auto& hb : tls.hblocks[c->device]) cudaFreeHost(hb.first);
     tls.hblocks[c->device].clear();
 }
@@ -333,8 +347,7 @@ CallScope::~CallScope() {
     }
     UploadSlot* up = tls.upload_used[c->device];
     if (c->own_stream && !up) return;  // library stream: the call drained it before returning
-    bool arena = false;
-    for (const Block& b : tls.blocks[c->device]) arena |= b.off != 0;
+    const bool arena = tls.arena_used[c->device];
     const bool plans = tls.plans_used[c->device];
     if ((!up && !arena && !plans) || capturing(c->stream)) return;
     const unsigned long long id = stream_id(c->stream);

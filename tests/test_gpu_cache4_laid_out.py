@@ -1,5 +1,7 @@
 """Attention by many tokens over rows in 4 bits, whose rows are laid out as bfloat16 first: counts of rows, windows, trees, documents and positions of heads, several batches of segments, other
 layouts, and rows that hold anything.  Every test asserts that this path ran; before each call the thread's working memory holds rows of NaN.  The bounds are those of tests/cache4_cases.py."""
+import threading
+
 import numpy as np
 import pytest
 
@@ -204,3 +206,37 @@ def test_rows_that_hold_anything_and_nan_that_is_seen():
     bad[sees, 6 * group:7 * group] = True
     assert np.isnan(got[0][bad]).all() and np.array_equal(got[0][~bad], clean[0][~bad])
     assert np.isnan(got[1][sees][:, 6 * group:7 * group]).all()
+
+
+@pytest.mark.parametrize("sequences", [1, 4])
+def test_working_memory_of_rows_and_parts(sequences):
+    # 131072 rows laid out are 512 MB, a batch of one segment; 256 tokens are few blocks, so that the rows are split.  A thread keeps what its calls took
+    torch = pytest.importorskip("torch")
+    rng = np.random.default_rng(7)
+    kv, group, d, n, tokens = 8, 4, 128, 131072, 256
+    codes, scales = S.to_device(rng.integers(0, 256, (n, kv, d // 2), np.uint8)), S.to_device(rng.integers(40, 72, (n, kv, 8), np.uint8))
+    cache = S.KvCache4(codes, codes, scales, scales, kv, d, key_exponent=-3, value_exponent=-3)
+    q = 0.3 * rng.standard_normal((tokens, kv * group, d))
+    queries = S.CacheQueries(S.to_device(np.concatenate([K.as_type(q, True)[1]] * sequences)), sequences * tokens, kv * group, d)
+    out = S.DeviceBuffer(sequences * tokens * kv * group * d * 2)
+    S.attend_cache4(cache, S.make_segments([(0, 8000, 0, tokens, 0)]), queries, out)  # (the kernels are loaded)
+    S.synchronize()
+    segs = S.make_segments([(0, n, i * tokens, tokens, 0) for i in range(sequences)])  # (sequences that share their rows)
+    taken, got = [], []
+
+    def work():
+        before = torch.cuda.mem_get_info()[0]
+        for _ in range(3):
+            S.attend_cache4(cache, segs, queries, out)
+            assert S.debug_last_cache_kernels() & S.CACHE_LAID_OUT
+            S.synchronize()
+            taken.append(before - torch.cuda.mem_get_info()[0])
+            got.append(out.download(np.uint16, sequences * q.size).reshape(sequences, -1))
+
+    t = threading.Thread(target=work)
+    t.start()
+    t.join()
+    # rows, parts (at most 512 MB; here 256 rows of 520 bytes of 8 KV heads for each of 4 blocks and at most 10 runs: 43 MB), a step of the arena of 64 MB
+    assert len(taken) == 3 and max(taken) <= 640 << 20, [x >> 20 for x in taken]
+    for x in got:  # the same inputs, the same bits, whichever batch
+        assert np.array_equal(x, got[0][:1].repeat(sequences, 0)) and np.isfinite(K.from_bf16(x)).all()
