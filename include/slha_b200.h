@@ -578,6 +578,9 @@ typedef struct {
  * as they are, rows of two segments are refused (with row counts in device memory they are
  * the caller's to avoid), and where a segment has fewer rows than tokens the tokens behind
  * its last row write no keys and values.  to->positions and documents are not written.
+ * Each token or row and head has a place of its own where it is written, here and in the two
+ * calls below: strides that lead two to the same bytes are refused (with row counts in device
+ * memory those that do so for neighbours).
  * q_out may be q, with the same strides, and without segments to->keys may be k and
  * to->values v; other arrays that are written overlap none that is read.  Weights,
  * frequencies, axes and positions are host or device memory, heads, q_out and rows device

@@ -56,9 +56,36 @@ Status rows_check(const SlhaB200KvCache* k, uint32_t head_dim, uint32_t n_kv, bo
         return Status(SLHA_ERR_DIMENSION, name("keys and values must begin on a multiple of 16 bytes and their strides be multiples of 16 bytes"));
     return Status();
 }
-// Where rows go, every row and KV head has a place of its own.
-Status rows_apart(uint64_t row_stride, uint64_t head_stride, uint32_t n_kv, const char* fn, const char* what) {
-    return row_stride == 0 || (n_kv > 1 && head_stride == 0) ? Status(SLHA_ERR_DIMENSION, std::string(fn) + ": " + what + " must have a place for each row and KV head (strides > 0)") : Status();
+// The rows that a call writes: from the first to the last, and whether the host knows which those are (row counts in device memory: as many as there are at most).
+struct Written {
+    uint64_t first = ~0ull, end = 0;
+    bool known = true;
+    void add(uint64_t from, uint64_t to) {
+        if (from >= to) return;
+        first = std::min(first, from);
+        end = std::max(end, to);
+    }
+    uint64_t rows() const { return end > first ? end - first : 0; }
+};
+// Where rows go, every row and head has a place of its own of `bytes`; strides in bytes.
+Status rows_apart(unsigned __int128 row, unsigned __int128 head, uint32_t n_heads, uint64_t bytes, const Written& w, const char* fn, const char* what) {
+    const uint64_t rows = w.rows();
+    bool apart = row != 0 && (n_heads == 1 || head != 0);
+    if (rows) apart &= (rows == 1 || row >= bytes) && (n_heads == 1 || head >= bytes);
+    // neither rows of heads nor heads of rows: r rows and h heads on may be the same place
+    if (apart && rows > 1 && n_heads > 1 && w.known && row < head * (n_heads - 1) + bytes && head < row * (rows - 1) + bytes)
+        for (uint32_t h = 1; apart && h < n_heads && head * h < row * (rows - 1) + bytes; ++h) {
+            const unsigned __int128 r = head * h / row, rest = head * h - r * row;
+            apart = !(r < rows && rest < bytes) && !(r + 1 < rows && row - rest < bytes);
+        }
+    return apart ? Status() : Status(SLHA_ERR_DIMENSION, std::string(fn) + ": " + what + " must have a place for each row and head (strides)");
+}
+Status rows_to_apart(const SlhaB200KvCache* to, const Written& w, const char* fn) {
+    const unsigned __int128 e = key_elem_bytes(to->dtype);
+    const uint64_t bytes = to->head_dim * (uint64_t)e;
+    if (to->keys) SLHA_TRY(rows_apart(to->key_row_stride * e, to->key_head_stride * e, to->n_kv_heads, bytes, w, fn, "keys"));
+    if (to->values) SLHA_TRY(rows_apart(to->value_row_stride * e, to->value_head_stride * e, to->n_kv_heads, bytes, w, fn, "values"));
+    return Status();
 }
 RowsOf rows_of(const SlhaB200KvCache* k) {
     const uint64_t e = key_elem_bytes(k->dtype);
@@ -71,16 +98,22 @@ RowsOf rows_of(const SlhaB200KvCache* k) {
     r.hs[1] = k->value_head_stride * e;
     return r;
 }
-// Segments whose tokens are written to their last rows: tokens that there are, rows that no other segment's tokens are written to.
-Status token_segments(const std::vector<SlhaB200Segment>& segs, uint32_t n_tokens, const uint32_t* rows, bool written, const char* fn) {
+// Segments whose tokens are written to their last rows: tokens that there are, rows that no other segment's tokens are written to.  w: those rows.
+Status token_segments(const std::vector<SlhaB200Segment>& segs, uint32_t n_tokens, const uint32_t* rows, Written* w, const char* fn) {
     for (const SlhaB200Segment& s : segs)
         if ((uint64_t)s.query_begin + s.n_queries > n_tokens) return Status(SLHA_ERR_DIMENSION, std::string(fn) + ": a segment's tokens reach beyond n_tokens");
-    if (!written || segs.size() < 2 || (rows && is_device_ptr(rows))) return Status();
+    if (!w) return Status();
+    if (rows && is_device_ptr(rows)) {
+        w->known = false;
+        for (const SlhaB200Segment& s : segs) w->add(s.tile_begin, s.tile_begin + (s.n_queries ? s.n_tiles : 0));
+        return Status();
+    }
     const auto range = [&](size_t i) {
         const uint64_t n = rows ? std::min(rows[i], segs[i].n_tiles) : segs[i].n_tiles;
         return std::pair<uint64_t, uint64_t>(segs[i].tile_begin + n - std::min<uint64_t>(n, segs[i].n_queries), segs[i].tile_begin + n);
     };
-    return cache_overlap(segs.size(), range) ? Status(SLHA_ERR_DIMENSION, std::string(fn) + ": two segments' tokens have the same rows") : Status();
+    for (size_t i = 0; i < segs.size(); ++i) w->add(range(i).first, range(i).second);
+    return segs.size() > 1 && cache_overlap(segs.size(), range) ? Status(SLHA_ERR_DIMENSION, std::string(fn) + ": two segments' tokens have the same rows") : Status();
 }
 
 int32_t attend_cache4_any(const char* fn, const SlhaB200KvCache4* cache, const SlhaB200Segment* segments, size_t n_segments, const SlhaB200CacheQueries* queries,
@@ -163,17 +196,21 @@ int32_t slha_b200_write_cache4(const SlhaB200KvCache4* cache, const SlhaB200Segm
         if (n_segments == 0 || n_tokens == 0) return Status();
         SLHA_TRY(cache4_check(cache, fn));
         SLHA_TRY(rows_check(from, cache->head_dim, cache->n_kv_heads, true, fn, "from"));
-        SLHA_TRY(rows_apart(cache->code_row_stride, cache->code_head_stride, cache->n_kv_heads, fn, "codes"));
-        SLHA_TRY(rows_apart(cache->scale_row_stride, cache->scale_head_stride, cache->n_kv_heads, fn, "scales"));
         std::vector<SlhaB200Segment> segs;
         bool device_segs;
         cache_host_segments(segments, n_segments, &segs, &device_segs);
-        if (!device_segs) SLHA_TRY(token_segments(segs, n_tokens, cache->rows, true, fn));
+        const auto check_segments = [&]() -> Status {
+            Written w;
+            SLHA_TRY(token_segments(segs, n_tokens, cache->rows, &w, fn));
+            SLHA_TRY(rows_apart(cache->code_row_stride, cache->code_head_stride, cache->n_kv_heads, cache->head_dim / 2, w, fn, "codes"));
+            return rows_apart(cache->scale_row_stride, cache->scale_head_stride, cache->n_kv_heads, cache->head_dim / BLOCK4, w, fn, "scales");
+        };
+        if (!device_segs) SLHA_TRY(check_segments());
         CallScope cs;
         if (!cs.ok()) return cs.st;
         Ctx* c = cs.c;
         SLHA_TRY(cache_device_segments(c, segments, &segs, device_segs, fn));
-        if (device_segs) SLHA_TRY(token_segments(segs, n_tokens, cache->rows, true, fn));
+        if (device_segs) SLHA_TRY(check_segments());
         SLHA_TRY(cache4_memory(c, cache, fn));
         SLHA_TRY(cache_device_memory(c, from->keys, fn, "keys"));
         SLHA_TRY(cache_device_memory(c, from->values, fn, "values"));
@@ -199,8 +236,6 @@ int32_t slha_b200_read_cache4(const SlhaB200KvCache4* cache, const SlhaB200Segme
         if (n_segments == 0) return Status();
         SLHA_TRY(cache4_check(cache, fn));
         SLHA_TRY(rows_check(to, cache->head_dim, cache->n_kv_heads, false, fn, "to"));
-        if (to->keys) SLHA_TRY(rows_apart(to->key_row_stride, to->key_head_stride, to->n_kv_heads, fn, "keys"));
-        if (to->values) SLHA_TRY(rows_apart(to->value_row_stride, to->value_head_stride, to->n_kv_heads, fn, "values"));
         std::vector<SlhaB200Segment> segs, to_segs;
         bool device_segs, device_to = false;
         cache_host_segments(segments, n_segments, &segs, &device_segs);
@@ -209,7 +244,12 @@ int32_t slha_b200_read_cache4(const SlhaB200KvCache4* cache, const SlhaB200Segme
             if (!to_segments) to_segs = segs;
             for (size_t i = 0; i < segs.size(); ++i)
                 if (to_segs[i].n_tiles < segs[i].n_tiles) return Status(SLHA_ERR_CAPACITY, name("segment " + std::to_string(i) + " has no room for its rows where they go"));
-            return cache_own_rows(segs, to_segs, cache->rows, 0xFFFFFFFFu, fn);
+            SLHA_TRY(cache_own_rows(segs, to_segs, cache->rows, 0xFFFFFFFFu, fn));
+            Written w;
+            w.known = !cache->rows || !is_device_ptr(cache->rows);
+            for (size_t i = 0; i < segs.size(); ++i)
+                w.add(to_segs[i].tile_begin, to_segs[i].tile_begin + (cache->rows && w.known ? std::min(cache->rows[i], segs[i].n_tiles) : segs[i].n_tiles));
+            return rows_to_apart(to, w, fn);
         };
         if (!device_segs && !device_to) SLHA_TRY(check_segments());
         CallScope cs;
@@ -256,15 +296,13 @@ int32_t slha_b200_rotate_heads(const SlhaB200HeadRows* heads, const SlhaB200Rota
         if (!lies(heads->q, heads->q_token_stride, heads->q_head_stride) || !lies(heads->k, heads->k_token_stride, heads->k_head_stride) ||
             !lies(heads->v, heads->v_token_stride, heads->v_head_stride) || (heads->q && !lies(q_out, q_out_token_stride, q_out_head_stride)))
             return Status(SLHA_ERR_DIMENSION, name("heads and q_out must begin on a multiple of 16 bytes and their strides be multiples of 16 bytes"));
-        if (heads->q) SLHA_TRY(rows_apart(q_out_token_stride, q_out_head_stride, heads->n_heads, fn, "q_out"));
+        SlhaB200KvCache there{};  // what is written of `to`
         if (n_kv) {
-            SlhaB200KvCache there = *to;  // what is written of it
+            there = *to;
             if (!heads->k) there.keys = nullptr;
             if (!heads->v) there.values = nullptr;
             if (to->dtype != heads->dtype) return Status(SLHA_ERR_DIMENSION, name("heads and rows must have the same dtype"));
             SLHA_TRY(rows_check(&there, d, n_kv, false, fn, "to"));
-            if (there.keys) SLHA_TRY(rows_apart(to->key_row_stride, to->key_head_stride, n_kv, fn, "keys"));
-            if (there.values) SLHA_TRY(rows_apart(to->value_row_stride, to->value_head_stride, n_kv, fn, "values"));
             SLHA_TRY(cache_words(fn, {to->rows}));
         }
         if (heads->norm) {
@@ -291,7 +329,11 @@ int32_t slha_b200_rotate_heads(const SlhaB200HeadRows* heads, const SlhaB200Rota
         if (segments) cache_host_segments(segments, n_segments, &segs, &device_segs);
         else segs.push_back(SlhaB200Segment{0, heads->n_tokens, 0, heads->n_tokens, 0});
         const auto check_segments = [&]() -> Status {
-            SLHA_TRY(token_segments(segs, heads->n_tokens, rows, n_kv > 0, fn));
+            Written w, turned;
+            SLHA_TRY(token_segments(segs, heads->n_tokens, rows, n_kv ? &w : nullptr, fn));
+            if (n_kv) SLHA_TRY(rows_to_apart(&there, w, fn));
+            for (const SlhaB200Segment& s : segs) turned.add(s.query_begin, (uint64_t)s.query_begin + s.n_queries);
+            if (heads->q) SLHA_TRY(rows_apart((unsigned __int128)q_out_token_stride * e, (unsigned __int128)q_out_head_stride * e, heads->n_heads, d * e, turned, fn, "q_out"));
             const auto tokens = [&](size_t i) { return std::pair<uint64_t, uint64_t>(segs[i].query_begin, (uint64_t)segs[i].query_begin + segs[i].n_queries); };
             return heads->q && cache_overlap(segs.size(), tokens) ? Status(SLHA_ERR_DIMENSION, name("two segments have the same tokens")) : Status();
         };
