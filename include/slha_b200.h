@@ -556,7 +556,7 @@ typedef struct {
     uint64_t v_head_stride;
     int32_t norm;                /* 0: no norms */
     float eps;
-    const float* q_weight;       /* head_dim; NULL: 1 */
+    const float* q_weight;       /* head_dim; NULL: 1.  On a multiple of 16 bytes in host memory, of 4 in device memory */
     const float* k_weight;
 } SlhaB200HeadRows;
 

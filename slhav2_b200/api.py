@@ -714,7 +714,7 @@ class HeadRows:
         for a, what in ((q, "q"), (k, "k"), (v, "v")):
             _typed(a, kind, what)
             _in_order(a, token_stride if token_stride is not None else head_stride, what)
-        q_weight, k_weight = _given(q_weight, np.float32), _given(k_weight, np.float32)
+        q_weight, k_weight = (w.copy() if isinstance(w, np.ndarray) and w.ctypes.data % 16 else w for w in (_given(q_weight, np.float32), _given(k_weight, np.float32)))
         self.kept = (q, k, v, q_weight, k_weight)
         self.head_dim, self.n_heads, self.n_kv_heads, self.n_tokens = head_dim, n_heads, n_kv_heads, n_tokens
         at = head_dim if head_stride is None else head_stride

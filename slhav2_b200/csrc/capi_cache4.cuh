@@ -307,7 +307,9 @@ int32_t slha_b200_rotate_heads(const SlhaB200HeadRows* heads, const SlhaB200Rota
         }
         if (heads->norm) {
             if (!std::isfinite(heads->eps) || heads->eps < 0.0f) return Status(SLHA_ERR_NONFINITE, name("eps must be finite and not negative"));
-            if (!cache_aligned(heads->q_weight) || !cache_aligned(heads->k_weight)) return Status(SLHA_ERR_DIMENSION, name("weights must begin on a multiple of 16 bytes"));
+            for (const float* w : {heads->q_weight, heads->k_weight})  // (read word by word)
+                if (!cache_aligned(w) && (reinterpret_cast<uintptr_t>(w) % 4 || !is_device_ptr(w)))
+                    return Status(SLHA_ERR_DIMENSION, name("weights must begin on a multiple of 4 bytes in device memory, of 16 in host memory"));
         } else if (heads->q_weight || heads->k_weight) {
             return Status(SLHA_ERR_DIMENSION, name("weights are given, but no norm"));
         }
