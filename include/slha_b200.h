@@ -536,7 +536,8 @@ int32_t slha_b200_evict_cache(const SlhaB200KvCache* cache, const SlhaB200Segmen
  *   positions[axes[p]][token] * frequencies[p]:
  *   (a, b) -> magnitude * (a cos - b sin, a sin + b cos);
  * the other elements stay.  Angles are reduced in 64 bits (to 1e-6 at positions of 2^32),
- * the rest is float32, rounded once.  With several axes (time, height, width) each pair
+ * the rest is float32, rounded once (heads whose squares leave its range, on either side, are
+ * scaled by a power of two first).  With several axes (time, height, width) each pair
  * goes by the axis that `axes` names.  Values are copied as they are.
  */
 typedef struct {
@@ -581,8 +582,8 @@ typedef struct {
  * Each token or row and head has a place of its own where it is written, here and in the two
  * calls below: strides that lead two to the same bytes are refused (with row counts in device
  * memory those that do so for neighbours).
- * q_out may be q, with the same strides, and without segments to->keys may be k and
- * to->values v; other arrays that are written overlap none that is read.  Weights,
+ * q_out may be q, and without segments to->keys may be k and to->values v, with the same
+ * strides each; other arrays that are written overlap none that is read.  Weights,
  * frequencies, axes and positions are host or device memory, heads, q_out and rows device
  * memory; captured into a graph as slha_b200_attend_cache. */
 int32_t slha_b200_rotate_heads(const SlhaB200HeadRows* heads, const SlhaB200Rotation* rotation,
@@ -596,7 +597,8 @@ int32_t slha_b200_rotate_heads(const SlhaB200HeadRows* heads, const SlhaB200Rota
  * element 4 bits (e2m1: a sign and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6); its value is element *
  * scale * 2^exponent, exact in bfloat16.  The exponents place the scales' range (2^-9 to
  * 448; full precision from 2^-6) where the cache's values lie: sizes up to 2688 * 2^exponent
- * are held, blocks whose largest is below 2^(exponent - 8) or so come out coarse or as zero.
+ * are held; blocks whose largest is below 6 * 2^(exponent - 6) have scales of 3 bits down to
+ * 1, those up to 6 * 2^(exponent - 10) come out as zero.
  * Code arrays and their strides are multiples of 16 bytes, scale arrays and theirs of 4 bytes
  * for head_dim up to 64, 8 up to 128, 16 beyond (SLHA_ERR_DIMENSION otherwise).  All device
  * memory, and what else is said of SlhaB200KvCache.

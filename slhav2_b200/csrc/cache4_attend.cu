@@ -819,8 +819,8 @@ struct Plan4 {
 // By a model: a launch takes `fixed` (most of it the first pass through the kernel's instructions), a tile of 128 dimensions `tile` and `shared` more for each CTA that shares the SM, an item `item`
 // of an SM's time to begin and end; a second kernel that joins parts 1.6 and a little for each part, a cluster 1.6.  What fits on the GPU at once takes as long as its longest item, more
 // than that the mean load and 0.4 of an item.  The constants were fitted to 69 calls, each with every run and cluster and with all the blocks it can have: one to 64 sequences of 300 to
-// 131072 rows, 4 to 512 query rows a KV head, 64 to 256 dimensions, both types.  What it picks takes 0.8 % longer than the best of each on the average, 8 % at most.  (One token over
-// 4096 rows: 9.2 us in 128 items and a second kernel, 9.5 by 8 clusters of 8; 131072 rows 41.5 in 432 items, 43 in 592, 49 in 824.  28 query rows over 1000 rows: 9.3 in blocks of 8, 10.8 of 16,
+// 131072 rows, 4 to 512 query rows a KV head, 64 to 256 dimensions, both types.  What it picks takes 0.8 % longer than the best of each of those on the average, 8 % at most.  (One token over
+// 4096 rows: 9.2 us in 128 items and a second kernel, 9.5 by 8 clusters of 8; 131072 rows 41.5 in 432 items, 43 in the 592 that it picks, for which it says 38, 49 in 824.  28 query rows over 1000 rows: 9.3 in blocks of 8, 10.8 of 16,
 // 15.4 of 32; over 16 sequences of up to 8192 rows: 104, 77, 69.)
 struct Cost4 {
     double tile, shared, item, fixed;

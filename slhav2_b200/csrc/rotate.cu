@@ -10,8 +10,8 @@
 //
 // Squares are summed in float32; a head for which that is too narrow is scaled by a power of two first (44.8 us instead of 43.4 for the look at each sum, in the case below).
 //
-// 8192 tokens of 32 + 8 + 8 heads of 128 dimensions, three axes: bfloat16 44.8 us = 4.5 TB/s (without norms 39.6; 150 instructions for 8 elements, 63 % of the issue slots), float32 68.7 us =
-// 5.9 TB/s.  One token 2.2 us, its call 6.5 with the host's time.
+// 8192 tokens of 32 + 8 + 8 heads of 128 dimensions, three axes: bfloat16 44.8 us = 4.5 TB/s (without norms 40.2), float32 69.4 us = 5.8 TB/s.  146 instructions for 8 elements take
+// 63 % of the issue slots; the largest wait is for loads (4.5 of 11 warps an issue), of which a group of lanes has two tokens' under way.  One token 2.2 us, its call 6.5 with the host's time.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -240,7 +240,7 @@ Status launch_rotate_heads(Ctx* c, RotateArgs a, int dtype, const std::vector<Sl
     uint64_t tokens = 0, items = 0;
     for (const SlhaB200Segment& s : segs) tokens += s.n_queries;
     if (!tokens) return Status();
-    // tokens of a block: up to 16, so that the blocks come in whole rounds of what an SM holds of them (8192 tokens: bfloat16 43.9 us in one round of 14 each, 46.3 in two of 7)
+    // tokens of a block: up to 16, so that the blocks come in whole rounds of what an SM holds of them (8192 tokens, bfloat16: two rounds of 7 each took 2.4 us more than one of 14)
     const uint64_t round = (dtype == SLHA_B200_BF16 ? 4ull : 3ull) * sm_count(c->device), rounds = (tokens + round * ROT_TOKENS - 1) / (round * ROT_TOKENS);
     a.each = (uint32_t)((tokens + round * rounds - 1) / (round * rounds));
     a.per_dim = 1.0f / (float)a.d;
