@@ -56,29 +56,67 @@ Status rows_check(const SlhaB200KvCache* k, uint32_t head_dim, uint32_t n_kv, bo
         return Status(SLHA_ERR_DIMENSION, name("keys and values must begin on a multiple of 16 bytes and their strides be multiples of 16 bytes"));
     return Status();
 }
-// The rows that a call writes: from the first to the last, and whether the host knows which those are (row counts in device memory: as many as there are at most).
+// What a call writes of a table's segments, a range of rows each: their tokens' rows, all of them (where `at` says), or their tokens as rows of queries.
 struct Written {
+    enum Of { TOKENS, ROWS, QUERIES } of;
+    const std::vector<SlhaB200Segment>&segs, &at;
+    const uint32_t* rows;       // counts on the host, or null
+    bool known = true;          // false: counts in device memory, rows are among these
     uint64_t first = ~0ull, end = 0;
-    bool known = true;
-    void add(uint64_t from, uint64_t to) {
-        if (from >= to) return;
-        first = std::min(first, from);
-        end = std::max(end, to);
-    }
-    uint64_t rows() const { return end > first ? end - first : 0; }
-};
-// Where rows go, every row and head has a place of its own of `bytes`; strides in bytes.
-Status rows_apart(unsigned __int128 row, unsigned __int128 head, uint32_t n_heads, uint64_t bytes, const Written& w, const char* fn, const char* what) {
-    const uint64_t rows = w.rows();
-    bool apart = row != 0 && (n_heads == 1 || head != 0);
-    if (rows) apart &= (rows == 1 || row >= bytes) && (n_heads == 1 || head >= bytes);
-    // neither rows of heads nor heads of rows: r rows and h heads on may be the same place
-    if (apart && rows > 1 && n_heads > 1 && w.known && row < head * (n_heads - 1) + bytes && head < row * (rows - 1) + bytes)
-        for (uint32_t h = 1; apart && h < n_heads && head * h < row * (rows - 1) + bytes; ++h) {
-            const unsigned __int128 r = head * h / row, rest = head * h - r * row;
-            apart = !(r < rows && rest < bytes) && !(r + 1 < rows && row - rest < bytes);
+    bool single = true;         // one row each
+    Written(Of of, const std::vector<SlhaB200Segment>& segs, const std::vector<SlhaB200Segment>& at, const uint32_t* counts) : of(of), segs(segs), at(at), rows(counts) {
+        if (rows && is_device_ptr(rows)) {
+            known = false;
+            rows = nullptr;
         }
-    return apart ? Status() : Status(SLHA_ERR_DIMENSION, std::string(fn) + ": " + what + " must have a place for each row and head (strides)");
+        for (size_t i = 0; i < segs.size(); ++i) {
+            const auto [from, to] = range(i);
+            if (from >= to) continue;
+            first = std::min(first, from);
+            end = std::max(end, to);
+            single &= to - from == 1;
+        }
+    }
+    std::pair<uint64_t, uint64_t> range(size_t i) const {  // first, behind the last
+        const SlhaB200Segment& s = segs[i];
+        if (of == QUERIES) return {s.query_begin, (uint64_t)s.query_begin + s.n_queries};
+        const uint64_t n = rows ? std::min(rows[i], s.n_tiles) : s.n_tiles, begin = at[i].tile_begin;
+        if (of == ROWS) return {begin, begin + n};
+        return {begin + (known ? n - std::min<uint64_t>(n, s.n_queries) : s.n_queries ? 0 : n), begin + n};
+    }
+};
+// Where rows go, every row that is written has a place of its own of `bytes` for each head; strides in bytes.  Where neither a row's heads lie before the next row nor a head's rows before the
+// next head, places are compared: of rows `by` apart, the one h heads on.
+Status rows_apart(unsigned __int128 row, unsigned __int128 head, uint32_t n_heads, uint64_t bytes, const Written& w, const char* fn, const char* what) {
+    const auto apart = [&]() {
+        if (row == 0 || (n_heads > 1 && head == 0)) return false;
+        if (w.first >= w.end) return true;
+        if (n_heads > 1 && head < bytes) return false;
+        if (!w.known) return row >= bytes || w.single;
+        if (row >= (n_heads > 1 ? head * (n_heads - 1) : 0) + bytes) return true;
+        const uint64_t most = w.end - 1 - w.first;  // between two rows
+        if (row >= bytes && head >= row * most + bytes) return true;
+        std::vector<std::pair<uint64_t, uint64_t>> r;  // (they share no row)
+        for (size_t i = 0; i < w.segs.size(); ++i)
+            if (w.range(i).first < w.range(i).second) r.push_back(w.range(i));
+        std::sort(r.begin(), r.end());
+        const auto twice = [&](uint64_t by) {  // whether two rows lie `by` apart
+            for (size_t i = 0, j = 0; i < r.size() && j < r.size();) {
+                if (r[i].second <= r[j].first + by) ++i;
+                else if (r[j].second + by <= r[i].first) ++j;
+                else return true;
+            }
+            return false;
+        };
+        for (uint32_t h = 0; h < n_heads; ++h) {
+            const unsigned __int128 on = head * h, least = h ? (on - bytes) / row + 1 : 1;  // (the first multiple of row beyond on - bytes; head >= bytes)
+            if (least > most) break;
+            for (unsigned __int128 by = least; by <= most && by * row < on + bytes; ++by)
+                if (twice((uint64_t)by)) return false;
+        }
+        return true;
+    };
+    return apart() ? Status() : Status(SLHA_ERR_DIMENSION, std::string(fn) + ": " + what + " must have a place for each row and head (strides)");
 }
 Status rows_to_apart(const SlhaB200KvCache* to, const Written& w, const char* fn) {
     const unsigned __int128 e = key_elem_bytes(to->dtype);
@@ -98,22 +136,12 @@ RowsOf rows_of(const SlhaB200KvCache* k) {
     r.hs[1] = k->value_head_stride * e;
     return r;
 }
-// Segments whose tokens are written to their last rows: tokens that there are, rows that no other segment's tokens are written to.  w: those rows.
-Status token_segments(const std::vector<SlhaB200Segment>& segs, uint32_t n_tokens, const uint32_t* rows, Written* w, const char* fn) {
+// Segments whose tokens there are, and (w: where they are written to their last rows) whose rows no other segment's tokens are written to.
+Status token_segments(const std::vector<SlhaB200Segment>& segs, uint32_t n_tokens, const Written* w, const char* fn) {
     for (const SlhaB200Segment& s : segs)
         if ((uint64_t)s.query_begin + s.n_queries > n_tokens) return Status(SLHA_ERR_DIMENSION, std::string(fn) + ": a segment's tokens reach beyond n_tokens");
-    if (!w) return Status();
-    if (rows && is_device_ptr(rows)) {
-        w->known = false;
-        for (const SlhaB200Segment& s : segs) w->add(s.tile_begin, s.tile_begin + (s.n_queries ? s.n_tiles : 0));
-        return Status();
-    }
-    const auto range = [&](size_t i) {
-        const uint64_t n = rows ? std::min(rows[i], segs[i].n_tiles) : segs[i].n_tiles;
-        return std::pair<uint64_t, uint64_t>(segs[i].tile_begin + n - std::min<uint64_t>(n, segs[i].n_queries), segs[i].tile_begin + n);
-    };
-    for (size_t i = 0; i < segs.size(); ++i) w->add(range(i).first, range(i).second);
-    return segs.size() > 1 && cache_overlap(segs.size(), range) ? Status(SLHA_ERR_DIMENSION, std::string(fn) + ": two segments' tokens have the same rows") : Status();
+    if (!w || !w->known || segs.size() < 2) return Status();
+    return cache_overlap(segs.size(), [&](size_t i) { return w->range(i); }) ? Status(SLHA_ERR_DIMENSION, std::string(fn) + ": two segments' tokens have the same rows") : Status();
 }
 
 int32_t attend_cache4_any(const char* fn, const SlhaB200KvCache4* cache, const SlhaB200Segment* segments, size_t n_segments, const SlhaB200CacheQueries* queries,
@@ -200,8 +228,8 @@ int32_t slha_b200_write_cache4(const SlhaB200KvCache4* cache, const SlhaB200Segm
         bool device_segs;
         cache_host_segments(segments, n_segments, &segs, &device_segs);
         const auto check_segments = [&]() -> Status {
-            Written w;
-            SLHA_TRY(token_segments(segs, n_tokens, cache->rows, &w, fn));
+            const Written w(Written::TOKENS, segs, segs, cache->rows);
+            SLHA_TRY(token_segments(segs, n_tokens, &w, fn));
             SLHA_TRY(rows_apart(cache->code_row_stride, cache->code_head_stride, cache->n_kv_heads, cache->head_dim / 2, w, fn, "codes"));
             return rows_apart(cache->scale_row_stride, cache->scale_head_stride, cache->n_kv_heads, cache->head_dim / BLOCK4, w, fn, "scales");
         };
@@ -245,10 +273,7 @@ int32_t slha_b200_read_cache4(const SlhaB200KvCache4* cache, const SlhaB200Segme
             for (size_t i = 0; i < segs.size(); ++i)
                 if (to_segs[i].n_tiles < segs[i].n_tiles) return Status(SLHA_ERR_CAPACITY, name("segment " + std::to_string(i) + " has no room for its rows where they go"));
             SLHA_TRY(cache_own_rows(segs, to_segs, cache->rows, 0xFFFFFFFFu, fn));
-            Written w;
-            w.known = !cache->rows || !is_device_ptr(cache->rows);
-            for (size_t i = 0; i < segs.size(); ++i)
-                w.add(to_segs[i].tile_begin, to_segs[i].tile_begin + (cache->rows && w.known ? std::min(cache->rows[i], segs[i].n_tiles) : segs[i].n_tiles));
+            const Written w(Written::ROWS, segs, to_segs, cache->rows);
             return rows_to_apart(to, w, fn);
         };
         if (!device_segs && !device_to) SLHA_TRY(check_segments());
@@ -331,10 +356,9 @@ int32_t slha_b200_rotate_heads(const SlhaB200HeadRows* heads, const SlhaB200Rota
         if (segments) cache_host_segments(segments, n_segments, &segs, &device_segs);
         else segs.push_back(SlhaB200Segment{0, heads->n_tokens, 0, heads->n_tokens, 0});
         const auto check_segments = [&]() -> Status {
-            Written w, turned;
-            SLHA_TRY(token_segments(segs, heads->n_tokens, rows, n_kv ? &w : nullptr, fn));
+            const Written w(Written::TOKENS, segs, segs, rows), turned(Written::QUERIES, segs, segs, nullptr);
+            SLHA_TRY(token_segments(segs, heads->n_tokens, n_kv ? &w : nullptr, fn));
             if (n_kv) SLHA_TRY(rows_to_apart(&there, w, fn));
-            for (const SlhaB200Segment& s : segs) turned.add(s.query_begin, (uint64_t)s.query_begin + s.n_queries);
             if (heads->q) SLHA_TRY(rows_apart((unsigned __int128)q_out_token_stride * e, (unsigned __int128)q_out_head_stride * e, heads->n_heads, d * e, turned, fn, "q_out"));
             const auto tokens = [&](size_t i) { return std::pair<uint64_t, uint64_t>(segs[i].query_begin, (uint64_t)segs[i].query_begin + segs[i].n_queries); };
             return heads->q && cache_overlap(segs.size(), tokens) ? Status(SLHA_ERR_DIMENSION, name("two segments have the same tokens")) : Status();
